@@ -244,6 +244,41 @@ TOKENIZER_SIGNATURES = {
     "plamo_translation_prefix": (c_uint64, [c_char_p, c_char_p, c_uint64]),
 }
 
+class PagedPlanArgs(ctypes.Structure):
+    """struct plamo_paged_plan_args (include/plamo_paged.h)."""
+    _fields_ = [(n, c_void_p) for n in ("held", "added", "tables", "free_pages", "head", "lengths", "starts", "slots",
+                                        "positions", "summary")] + \
+               [(n, c_uint64) for n in ("requests", "table_stride", "free_count", "rows")] + \
+               [("base", c_int64), ("stream", c_void_p)]
+
+
+class PagedStoreArgs(ctypes.Structure):
+    """struct plamo_paged_store_args (include/plamo_paged.h)."""
+    _fields_ = [(n, c_void_p) for n in ("qkv", "pool", "q", "slots", "positions", "q_norm", "k_norm", "table", "status")] + \
+               [(n, c_uint64) for n in ("rows", "qkv_stride", "q_stride", "pages", "positions_count")] + \
+               [(n, c_uint32) for n in ("query_heads", "kv_heads", "qkv_type", "pool_type")] + [("stream", c_void_p)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """struct plamo_paged_attention_args (include/plamo_paged.h)."""
+    _fields_ = [(n, c_void_p) for n in ("q", "pool", "out", "starts", "lengths", "tables", "prefix_pages", "workspace")] + \
+               [("workspace_bytes", c_uint64), ("status", c_void_p)] + \
+               [(n, c_uint64) for n in ("rows", "q_stride", "out_stride", "requests", "table_stride", "prefix_rows",
+                                        "pages", "window")] + \
+               [("query_heads", c_uint32), ("kv_heads", c_uint32), ("type", c_uint32), ("scale", ctypes.c_float),
+                ("stream", c_void_p)]
+
+
+PAGED_ROWS, PAGED_DIM = 64, 128  # PLAMO_PAGED_ROWS, PLAMO_PAGED_DIM
+PAGED_BF16, PAGED_FP32 = 0, 1  # PLAMO_PAGED_BF16, PLAMO_PAGED_FP32
+# include/plamo_paged.h: operators of a paged batch step
+PAGED_SIGNATURES = {
+    "plamo_paged_plan": (c_int, [P, POINTER(PagedPlanArgs)]),
+    "plamo_paged_store": (c_int, [P, POINTER(PagedStoreArgs)]),
+    "plamo_paged_attention": (c_int, [P, POINTER(PagedAttentionArgs)]),
+    "plamo_paged_attention_workspace": (c_uint64, [P, POINTER(PagedAttentionArgs)]),
+}
+
 _libs = {}
 
 
@@ -257,7 +292,8 @@ def load(path=LIB_PATH):
                       "__graft_entry__.build()); there is no non-CUDA implementation")
     lib = ctypes.CDLL(path)
     for name, (restype, argtypes) in (list(SIGNATURES.items()) + list(LOADER_SIGNATURES.items()) +
-                                      list(LAYOUT_SIGNATURES.items()) + list(TOKENIZER_SIGNATURES.items())):
+                                      list(LAYOUT_SIGNATURES.items()) + list(TOKENIZER_SIGNATURES.items()) +
+                                      list(PAGED_SIGNATURES.items())):
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes

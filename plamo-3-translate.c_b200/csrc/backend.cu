@@ -6,6 +6,7 @@
 #include "../../include/plamo_cuda.h"
 #include "../../include/plamo_synthetic.h"
 #include "common.cuh"
+#include "context.h"
 #include "gemv.cuh"
 #include "attention.cuh"
 #include "rows.cuh"
@@ -1774,7 +1775,8 @@ struct plamo_cuda *plamo_cuda_open(const struct plamo_cuda_config *config, char 
     prefer_carveout(tp_epoch_kernel, carveout);
     cudaFuncSetAttribute(decode_attention128_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     cudaFuncSetAttribute(decode_attention128_batch_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if ((e = cudaGetLastError()) != cudaSuccess) {
+    e = paged_configure();
+    if (e != cudaSuccess || (e = cudaGetLastError()) != cudaSuccess) {
         if (error && cap) snprintf(error, cap, "cannot configure kernels: %s", cudaGetErrorString(e));
         plamo_cuda_close(c);
         return nullptr;
@@ -3393,3 +3395,37 @@ bool sync_kv(plamo_cuda *c, DModel *m) {
     return true;
 }
 }  // namespace
+
+// ---- context.h: what the other translation units use ------------------------
+namespace plamo {
+ContextDevice::ContextDevice(const plamo_cuda *c) : before_(c->device), device_(c->device) {
+    cudaGetDevice(&before_);
+    if (before_ != device_) cudaSetDevice(device_);
+}
+ContextDevice::~ContextDevice() {
+    if (before_ != device_) cudaSetDevice(before_);
+}
+cudaStream_t context_stream(const plamo_cuda *c) { return c->stream; }
+int context_sms(const plamo_cuda *c) { return c->sm_count; }
+bool context_pdl(const plamo_cuda *c) { return c->pdl; }
+int context_decline(plamo_cuda *c, const char *why) {
+    c->info.declines++;
+    snprintf(c->info.note, sizeof c->info.note, "%s", why);
+    return 0;
+}
+bool context_launched(plamo_cuda *c, const char *what, cudaError_t e) {
+    c->info.launches++;
+    return note(c, what, e);
+}
+bool tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t element_bytes, const void *ptr, uint64_t rows,
+                   uint64_t cols, uint32_t box_cols, uint32_t box_rows) {
+    if (!tensor_maps_available()) return false;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {cols * element_bytes};
+    cuuint32_t box[2] = {box_cols, box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    return g_encode_tiled(map, type, 2, const_cast<void *>(ptr), dims, strides, box, elem,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+}  // namespace plamo

@@ -1,0 +1,233 @@
+// Host side of the paged batch operators (include/plamo_paged.h).
+#include "../../include/plamo_cuda.h"
+#include "../../include/plamo_paged.h"
+#include "context.h"
+#include "paged.cuh"
+#include "paged_attention.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+using namespace plamo;
+
+namespace {
+
+cudaStream_t stream_of(const plamo_cuda *c, void *stream) {
+    return stream ? static_cast<cudaStream_t>(stream) : context_stream(c);
+}
+bool aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+uint64_t element_bytes(uint32_t type) { return type == PLAMO_PAGED_FP32 ? 4 : 2; }
+bool type_ok(uint32_t type) { return type == PLAMO_PAGED_BF16 || type == PLAMO_PAGED_FP32; }
+uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+template <typename... KArgs, typename... Args>
+bool launch(plamo_cuda *c, const char *what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+            cudaStream_t stream, bool dependent, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    if (dependent && context_pdl(c)) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    return context_launched(c, what, cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+}
+
+// Shapes of an attention call; NULL when they are fine, else what is wrong.
+const char *attention_shapes(const plamo_paged_attention_args *d) {
+    if (!type_ok(d->type)) return "paged_attention: type must be PLAMO_PAGED_BF16 or PLAMO_PAGED_FP32";
+    if (!d->kv_heads || !d->query_heads || d->query_heads % d->kv_heads || d->query_heads > 4096)
+        return "paged_attention: query_heads must be a multiple of kv_heads, at most 4096";
+    if (d->rows > INT32_MAX || d->requests > INT32_MAX - 1 || d->rows * d->query_heads > INT32_MAX)
+        return "paged_attention: too many rows or requests";
+    if (!d->pages || d->pages > static_cast<uint64_t>(kPgMaxPages) / 4)
+        return "paged_attention: pages must be 1 to 2^23";
+    if (d->prefix_rows > d->pages * kPgRows) return "paged_attention: the prefix does not fit the pool";
+    if (d->table_stride > static_cast<uint64_t>(kPgMaxPages)) return "paged_attention: table_stride above 2^25";
+    return nullptr;
+}
+
+// How an attention call is laid out: the workspace's parts and the grid.
+struct AttentionLayout {
+    uint32_t prefix_tiles, prefix_splits, own_groups, target;
+    uint64_t record, own_sum, own_ml, prefix_sum, prefix_ml, bytes;
+};
+
+AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attention_args *d) {
+    AttentionLayout a{};
+    const uint64_t group = d->query_heads / d->kv_heads, sms = static_cast<uint64_t>(context_sms(c));
+    const uint64_t pairs = d->rows * group, prefix_pages = ceil_div(d->prefix_rows, kPgRows);
+    a.prefix_tiles = static_cast<uint32_t>(ceil_div(pairs, kRtM));
+    if (prefix_pages && a.prefix_tiles) {
+        const uint64_t want = ceil_div(4 * sms, static_cast<uint64_t>(a.prefix_tiles) * d->kv_heads);
+        a.prefix_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(want, prefix_pages / kRtMinPages)));
+    }
+    a.target = static_cast<uint32_t>(4 * sms);
+    // Every request's last tile and last run of pages may be partial.
+    a.own_groups = static_cast<uint32_t>(std::min<uint64_t>(
+        pairs / kRtM + std::min<uint64_t>(d->requests, d->rows) + ceil_div(a.target, d->kv_heads), INT32_MAX / d->kv_heads));
+    uint64_t at = 0;
+    auto part = [&](uint64_t bytes) {
+        const uint64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const uint64_t own = static_cast<uint64_t>(a.own_groups) * d->kv_heads;
+    const uint64_t prefix = static_cast<uint64_t>(a.prefix_splits) * a.prefix_tiles * d->kv_heads;
+    a.record = part(d->requests * sizeof(int2));
+    a.own_sum = part(own * kRtM * kPgDim * 4);
+    a.own_ml = part(own * kRtM * sizeof(float2));
+    a.prefix_sum = part(prefix * kRtM * kPgDim * 4);
+    a.prefix_ml = part(prefix * kRtM * sizeof(float2));
+    a.bytes = std::max<uint64_t>(at, 256);
+    return a;
+}
+
+template <bool F32>
+bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const AttentionLayout &a, cudaStream_t stream) {
+    CUtensorMap map;
+    if (!tensor_map_2d(&map, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, F32 ? 4 : 2,
+                       d->pool, d->pages * 2 * kPgRows, static_cast<uint64_t>(d->kv_heads) * kPgDim, F32 ? 32 : 64,
+                       rt_stage_rows<F32>()))
+        return context_launched(c, "paged_attention: tensor map", cudaErrorInvalidValue);
+    char *ws = static_cast<char *>(d->workspace);
+    PagedAttnParams p{};
+    p.q = d->q;
+    p.out = d->out;
+    p.starts = d->starts;
+    p.lengths = d->lengths;
+    p.tables = d->tables;
+    p.prefix_pages = d->prefix_pages;
+    p.q_stride = d->q_stride;
+    p.out_stride = d->out_stride;
+    p.table_stride = d->table_stride;
+    p.status = d->status;
+    p.rows = static_cast<uint32_t>(d->rows);
+    p.requests = static_cast<uint32_t>(d->requests);
+    p.pages = static_cast<uint32_t>(d->pages);
+    p.qh = d->query_heads;
+    p.kh = d->kv_heads;
+    p.group = d->query_heads / d->kv_heads;
+    p.prefix = static_cast<int64_t>(d->prefix_rows);
+    p.window = static_cast<int64_t>(std::min<uint64_t>(d->window, 1ull << 40));
+    p.scale2 = d->scale * 1.4426950408889634f;
+    p.own_record = reinterpret_cast<int2 *>(ws + a.record);
+    p.own_sum = reinterpret_cast<float *>(ws + a.own_sum);
+    p.own_ml = reinterpret_cast<float2 *>(ws + a.own_ml);
+    p.prefix_sum = reinterpret_cast<float *>(ws + a.prefix_sum);
+    p.prefix_ml = reinterpret_cast<float2 *>(ws + a.prefix_ml);
+    p.own_groups = a.own_groups;
+    p.prefix_splits = a.prefix_splits;
+    p.prefix_tiles = a.prefix_tiles;
+    p.target = a.target;
+    return launch(c, "paged_attention", paged_rows_kernel<F32>, dim3(2 * context_sms(c)), dim3(kRtThreads), kRtSmem, stream,
+                  false, map, p) &&
+           launch(c, "paged_attention join", paged_join_kernel<F32>, dim3(p.rows, (p.qh + 7) / 8), dim3(256), 0, stream,
+                  true, p);
+}
+
+template <typename In, typename Out>
+bool run_store(plamo_cuda *c, const plamo_paged_store_args *d, cudaStream_t stream) {
+    const uint64_t heads = d->query_heads + 2ull * d->kv_heads;
+    // Four heads to a warp once that still gives every SM eight warps and more;
+    // one to a warp for the few rows of a decode step.
+    const bool wide = d->rows * heads >= 4ull * 8 * static_cast<uint64_t>(context_sms(c));
+    const uint64_t units = d->rows * ceil_div(heads, wide ? 4 : 1);
+    const dim3 grid(static_cast<uint32_t>(ceil_div(units, 8)));
+    if (wide)
+        return launch(c, "paged_store", paged_store_kernel<In, Out, 4>, grid, dim3(256), 0, stream, false, *d);
+    return launch(c, "paged_store", paged_store_kernel<In, Out, 1>, grid, dim3(256), 0, stream, false, *d);
+}
+
+}  // namespace
+
+namespace plamo {
+cudaError_t paged_configure() {
+    cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRtSmem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(paged_rows_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRtSmem);
+    return e;
+}
+}  // namespace plamo
+
+extern "C" {
+
+int plamo_paged_plan(struct plamo_cuda *c, const struct plamo_paged_plan_args *d) {
+    if (!c || !d) return 0;
+    if (!d->lengths || !d->starts || !d->summary || (d->requests && (!d->held || !d->added || !d->tables)) ||
+        (d->rows && (!d->slots || !d->positions)) || (d->free_count && !d->free_pages))
+        return context_decline(c, "paged_plan: a buffer is missing");
+    if (d->rows > INT32_MAX - kPlanThreads || d->requests >= INT32_MAX || d->free_count > INT32_MAX ||
+        d->table_stride > static_cast<uint64_t>(kPgMaxPages) || d->base < 0 || d->base > INT32_MAX)
+        return context_decline(c, "paged_plan: a count is out of range");
+    if (d->head && d->head >= d->summary && d->head < d->summary + 4)
+        return context_decline(c, "paged_plan: head must not lie in this plan's own summary");
+    ContextDevice device(c);
+    const uint32_t grid = static_cast<uint32_t>(std::max<uint64_t>(1, ceil_div(d->rows, kPlanThreads)));
+    return launch(c, "paged_plan", paged_plan_kernel, dim3(grid), dim3(kPlanThreads), 0, stream_of(c, d->stream), false,
+                  PlanParams{*d})
+               ? 1
+               : -1;
+}
+
+int plamo_paged_store(struct plamo_cuda *c, const struct plamo_paged_store_args *d) {
+    if (!c || !d) return 0;
+    if (!type_ok(d->qkv_type) || !type_ok(d->pool_type))
+        return context_decline(c, "paged_store: types must be PLAMO_PAGED_BF16 or PLAMO_PAGED_FP32");
+    if (!d->kv_heads || !d->query_heads || d->query_heads % d->kv_heads || d->query_heads > 4096)
+        return context_decline(c, "paged_store: query_heads must be a multiple of kv_heads, at most 4096");
+    if (!d->pages || d->pages > static_cast<uint64_t>(kPgMaxPages) || d->rows > INT32_MAX / 4096)
+        return context_decline(c, "paged_store: pages must be 1 to 2^25 and rows below 2^19");
+    const uint64_t heads = d->query_heads + 2ull * d->kv_heads;
+    if (d->qkv_stride < heads * kPgDim || d->q_stride < static_cast<uint64_t>(d->query_heads) * kPgDim)
+        return context_decline(c, "paged_store: a row stride is shorter than its row");
+    if (!d->rows) return 1;
+    if (!d->qkv || !d->pool || !d->q || !d->slots || !d->positions || !d->q_norm || !d->k_norm || !d->table)
+        return context_decline(c, "paged_store: a buffer is missing");
+    // Four elements at a time.
+    if (!aligned(d->qkv, 4 * element_bytes(d->qkv_type)) || !aligned(d->q, 4 * element_bytes(d->pool_type)) ||
+        d->qkv_stride % 4 || d->q_stride % 4 || !aligned(d->pool, 16) || !aligned(d->q_norm, 8) ||
+        !aligned(d->k_norm, 8) || !aligned(d->table, 16))
+        return context_decline(c, "paged_store: rows must start on four-element boundaries, pool and table on 16 bytes, norms on 8");
+    ContextDevice device(c);
+    const cudaStream_t stream = stream_of(c, d->stream);
+    const bool in32 = d->qkv_type == PLAMO_PAGED_FP32, out32 = d->pool_type == PLAMO_PAGED_FP32;
+    const bool ok = in32 ? (out32 ? run_store<float, float>(c, d, stream) : run_store<float, uint16_t>(c, d, stream))
+                         : (out32 ? run_store<uint16_t, float>(c, d, stream) : run_store<uint16_t, uint16_t>(c, d, stream));
+    return ok ? 1 : -1;
+}
+
+uint64_t plamo_paged_attention_workspace(struct plamo_cuda *c, const struct plamo_paged_attention_args *d) {
+    if (!c || !d) return 0;
+    if (const char *why = attention_shapes(d)) return static_cast<uint64_t>(context_decline(c, why));
+    return attention_layout(c, d).bytes;
+}
+
+int plamo_paged_attention(struct plamo_cuda *c, const struct plamo_paged_attention_args *d) {
+    if (!c || !d) return 0;
+    if (const char *why = attention_shapes(d)) return context_decline(c, why);
+    const uint64_t width = static_cast<uint64_t>(d->query_heads) * kPgDim, per16 = 16 / element_bytes(d->type);
+    if (d->q_stride < width || d->out_stride < width)
+        return context_decline(c, "paged_attention: a row stride is shorter than its row");
+    if (!std::isfinite(d->scale)) return context_decline(c, "paged_attention: scale must be finite");
+    if (!d->rows) return 1;
+    if (!d->q || !d->pool || !d->out || !d->starts || (d->requests && (!d->lengths || !d->tables)) ||
+        (d->prefix_rows && !d->prefix_pages))
+        return context_decline(c, "paged_attention: a buffer is missing");
+    if (!aligned(d->q, 16) || !aligned(d->out, 16) || !aligned(d->pool, 16) || d->q_stride % per16 || d->out_stride % per16)
+        return context_decline(c, "paged_attention: pool, queries and results must start on 16-byte boundaries, row by row");
+    const AttentionLayout a = attention_layout(c, d);
+    if (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < a.bytes)
+        return context_decline(c, "paged_attention: the workspace is missing, too small or not 256-byte aligned");
+    ContextDevice device(c);
+    const cudaStream_t stream = stream_of(c, d->stream);
+    const bool ok = d->type == PLAMO_PAGED_FP32 ? run_attention<true>(c, d, a, stream) : run_attention<false>(c, d, a, stream);
+    return ok ? 1 : -1;
+}
+
+}  // extern "C"

@@ -17,7 +17,7 @@ from dataclasses import dataclass, field, replace
 
 import numpy as np
 
-from . import _abi
+from . import _abi, paged
 
 
 @dataclass(frozen=True)
@@ -590,6 +590,21 @@ class Backend:
     def prepare(self, hm):
         if self.lib.plamo_cuda_prepare_model(self.ctx, hm.ptr) != 1:
             raise RuntimeError("prepare_model failed: " + self.info().note.decode())
+
+    # ---- operators of a paged batch step (torch tensors; include/plamo_paged.h) ----
+    def paged_plan(self, held, added, tables, free_pages, rows, base=0, after=None):
+        """Page tables and slot maps of a step; see paged.plan."""
+        return paged.plan(self, held, added, tables, free_pages, rows, base, after)
+
+    def paged_store(self, qkv, pool, slots, positions, q_norm, k_norm, table, status=None):
+        """Normalised, rotated queries; keys and values into their slots; see paged.store."""
+        return paged.store(self, qkv, pool, slots, positions, q_norm, k_norm, table, status)
+
+    def paged_attention(self, q, pool, starts, lengths, tables, prefix_pages=None, prefix_rows=0, window=0, scale=None,
+                        out=None, status=None):
+        """Attention over a shared prefix and each request's own rows; see paged.attention."""
+        return paged.attention(self, q, pool, starts, lengths, tables, prefix_pages, prefix_rows, window, scale, out,
+                               status)
 
     def __enter__(self):
         return self
