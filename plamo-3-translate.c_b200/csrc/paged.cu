@@ -4,6 +4,7 @@
 #include "context.h"
 #include "paged.cuh"
 #include "paged_attention.cuh"
+#include "paged_tiles.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -54,23 +55,35 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
-    uint32_t prefix_tiles, prefix_splits, own_groups, target;
-    uint64_t record, own_sum, own_ml, prefix_sum, prefix_ml, bytes;
+    uint32_t row_tile, prefix_tiles, prefix_splits, own_groups, target, tile_rows, tile_cap;
+    uint64_t record, own_sum, own_ml, prefix_sum, prefix_ml;
+    uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
 };
 
 AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attention_args *d) {
     AttentionLayout a{};
     const uint64_t group = d->query_heads / d->kv_heads, sms = static_cast<uint64_t>(context_sms(c));
     const uint64_t pairs = d->rows * group, prefix_pages = ceil_div(d->prefix_rows, kPgRows);
-    a.prefix_tiles = static_cast<uint32_t>(ceil_div(pairs, kRtM));
-    if (prefix_pages && a.prefix_tiles) {
-        const uint64_t want = ceil_div(4 * sms, static_cast<uint64_t>(a.prefix_tiles) * d->kv_heads);
+    if (d->type == PLAMO_PAGED_BF16 && group <= kTlPairs && (prefix_pages || pairs > kTlShortPairs)) {
+        a.tile_rows = static_cast<uint32_t>(kTlPairs / group);
+        // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
+        a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
+    }
+    // Eight pairs to a tile while a request has no more on average (the heads of
+    // a group of eight, one row each); FP32 sums leave no registers for more.
+    a.row_tile = d->type == PLAMO_PAGED_FP32 || pairs <= 8 * d->requests ? 8 : 16;
+    a.prefix_tiles = static_cast<uint32_t>(ceil_div(pairs, a.row_tile));
+    if (prefix_pages && a.prefix_tiles && !a.tile_rows) {
+        const uint64_t want = ceil_div(2 * sms, static_cast<uint64_t>(a.prefix_tiles) * d->kv_heads);
         a.prefix_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(want, prefix_pages / kRtMinPages)));
     }
-    a.target = static_cast<uint32_t>(4 * sms);
-    // Every request's last tile and last run of pages may be partial.
+    a.target = static_cast<uint32_t>(2 * sms);  // one item to a CTA
+    // Every request's last tile and last run of pages may be partial. Beside the
+    // tile kernel only requests of up to kTlShortPairs pairs are here.
+    const uint64_t own_tiles = pairs / a.row_tile + std::min<uint64_t>(d->requests, d->rows);
     a.own_groups = static_cast<uint32_t>(std::min<uint64_t>(
-        pairs / kRtM + std::min<uint64_t>(d->requests, d->rows) + ceil_div(a.target, d->kv_heads), INT32_MAX / d->kv_heads));
+        (a.tile_rows ? std::min<uint64_t>(own_tiles, kTlShortPairs / a.row_tile * d->requests) : own_tiles) + ceil_div(a.target, d->kv_heads),
+        INT32_MAX / d->kv_heads));
     uint64_t at = 0;
     auto part = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -79,21 +92,34 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     };
     const uint64_t own = static_cast<uint64_t>(a.own_groups) * d->kv_heads;
     const uint64_t prefix = static_cast<uint64_t>(a.prefix_splits) * a.prefix_tiles * d->kv_heads;
-    a.record = part(d->requests * sizeof(int2));
-    a.own_sum = part(own * kRtM * kPgDim * 4);
-    a.own_ml = part(own * kRtM * sizeof(float2));
-    a.prefix_sum = part(prefix * kRtM * kPgDim * 4);
-    a.prefix_ml = part(prefix * kRtM * sizeof(float2));
+    a.header = part(kTlHeader * 4);
+    a.short_list = part(d->rows * sizeof(int4));
+    a.record = part(d->requests * sizeof(int4));
+    a.own_sum = part(own * a.row_tile * kPgDim * 4);
+    a.own_ml = part(own * a.row_tile * sizeof(float2));
+    a.prefix_sum = part(prefix * a.row_tile * kPgDim * 4);
+    a.prefix_ml = part(prefix * a.row_tile * sizeof(float2));
+    if (a.tile_rows) {
+        // Two runs of a CTA may end inside a prompt's tile; every run of a prefix tile is a part.
+        const uint64_t shared = prefix_pages ? sms + ceil_div(d->rows, a.tile_rows) * d->kv_heads : 0;
+        const uint64_t slots = 2 * sms + shared;
+        a.tile_shape = part(a.tile_cap * sizeof(TileShape));
+        a.tile_unit = part((a.tile_cap + 1ull) * 4);
+        a.tile_sum = part(slots * kTlPairs * kPgDim * 4);
+        a.tile_ml = part(slots * kTlPairs * sizeof(float2));
+    }
     a.bytes = std::max<uint64_t>(at, 256);
     return a;
 }
 
 template <bool F32>
 bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const AttentionLayout &a, cudaStream_t stream) {
-    CUtensorMap map;
-    if (!tensor_map_2d(&map, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, F32 ? 4 : 2,
-                       d->pool, d->pages * 2 * kPgRows, static_cast<uint64_t>(d->kv_heads) * kPgDim, F32 ? 32 : 64,
-                       rt_stage_rows<F32>()))
+    const auto pool_map = [&](CUtensorMap *map, uint32_t rows) {
+        return tensor_map_2d(map, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, F32 ? 4 : 2,
+                             d->pool, d->pages * 2 * kPgRows, static_cast<uint64_t>(d->kv_heads) * kPgDim, F32 ? 32 : 64, rows);
+    };
+    CUtensorMap map, page_map;
+    if (!pool_map(&map, kRtKeys) || (a.tile_rows && !pool_map(&page_map, kPgRows)))
         return context_launched(c, "paged_attention: tensor map", cudaErrorInvalidValue);
     char *ws = static_cast<char *>(d->workspace);
     PagedAttnParams p{};
@@ -116,19 +142,46 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.prefix = static_cast<int64_t>(d->prefix_rows);
     p.window = static_cast<int64_t>(std::min<uint64_t>(d->window, 1ull << 40));
     p.scale2 = d->scale * 1.4426950408889634f;
-    p.own_record = reinterpret_cast<int2 *>(ws + a.record);
+    // The tile kernel masks before it scales: -inf must stay so.
+    if (std::fabs(p.scale2) < 1e-30f) p.scale2 = std::copysign(1e-30f, p.scale2);
+    p.own_record = reinterpret_cast<int4 *>(ws + a.record);
+    p.header = reinterpret_cast<int32_t *>(ws + a.header);
+    p.short_list = reinterpret_cast<int4 *>(ws + a.short_list);
     p.own_sum = reinterpret_cast<float *>(ws + a.own_sum);
     p.own_ml = reinterpret_cast<float2 *>(ws + a.own_ml);
     p.prefix_sum = reinterpret_cast<float *>(ws + a.prefix_sum);
     p.prefix_ml = reinterpret_cast<float2 *>(ws + a.prefix_ml);
+    p.row_tile = a.row_tile;
     p.own_groups = a.own_groups;
     p.prefix_splits = a.prefix_splits;
     p.prefix_tiles = a.prefix_tiles;
     p.target = a.target;
-    return launch(c, "paged_attention", paged_rows_kernel<F32>, dim3(2 * context_sms(c)), dim3(kRtThreads), kRtSmem, stream,
-                  false, map, p) &&
-           launch(c, "paged_attention join", paged_join_kernel<F32>, dim3(p.rows, (p.qh + 7) / 8), dim3(256), 0, stream,
-                  true, p);
+    if (a.tile_rows) {
+        p.pool = d->pool;
+        p.tile_rows = a.tile_rows;
+        p.tile_grid = static_cast<uint32_t>(context_sms(c));
+        p.tile_cap = a.tile_cap;
+        p.tile_shape = reinterpret_cast<TileShape *>(ws + a.tile_shape);
+        p.tile_unit = reinterpret_cast<uint32_t *>(ws + a.tile_unit);
+        p.tile_sum = reinterpret_cast<float *>(ws + a.tile_sum);
+        p.tile_ml = reinterpret_cast<float2 *>(ws + a.tile_ml);
+    }
+    // The row kernel needs no schedule and hides its time; the tile kernel's CTAs
+    // follow as SMs come free.
+    void (*rows)(const CUtensorMap, const PagedAttnParams) = paged_rows_kernel<F32, 1>;
+    if constexpr (!F32)
+        if (a.row_tile == 16) rows = paged_rows_kernel<F32, 2>;
+    if (!launch(c, "paged_attention schedule", paged_schedule_kernel, dim3(1), dim3(kScThreads), 0, stream, false, p) ||
+        !launch(c, "paged_attention rows", rows, dim3(2 * context_sms(c)), dim3(kRtThreads), kRtSmem, stream, true, map, p) ||
+        (a.tile_rows && !launch(c, "paged_attention tiles", paged_tile_kernel, dim3(p.tile_grid), dim3(kTlThreads), kTlSmem,
+                                stream, true, page_map, p)))
+        return false;
+    // Eight warps to a result while one each would leave SMs idle.
+    const uint64_t results = d->rows * d->query_heads, wave = 8ull * context_sms(c);
+    return results <= wave
+               ? launch(c, "paged_attention join", paged_join_kernel<F32, 8>, dim3(static_cast<uint32_t>(results)), dim3(256), 0, stream, true, p)
+               : launch(c, "paged_attention join", paged_join_kernel<F32, 1>,
+                        dim3(static_cast<uint32_t>(std::min(ceil_div(results, 8), wave))), dim3(256), 0, stream, true, p);
 }
 
 template <typename In, typename Out>
@@ -148,9 +201,13 @@ bool run_store(plamo_cuda *c, const plamo_paged_store_args *d, cudaStream_t stre
 
 namespace plamo {
 cudaError_t paged_configure() {
-    cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRtSmem);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(paged_rows_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRtSmem);
+    const auto allow = [](auto kernel, int bytes) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    cudaError_t e = allow(paged_rows_kernel<false, 1>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_rows_kernel<false, 2>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_rows_kernel<true, 1>, kRtSmem);
+      if (e == cudaSuccess) e = allow(paged_tile_kernel, kTlSmem);
     return e;
 }
 }  // namespace plamo

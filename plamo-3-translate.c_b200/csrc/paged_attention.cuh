@@ -21,29 +21,48 @@ struct PagedAttnParams {
     uint32_t rows, requests, pages, qh, kh, group;
     int64_t prefix, window;  // window: rows seen, 0 for all
     float scale2;            // scale * log2(e)
-    // Partial results, unnormalised: [slot][16][128] sums and [slot][16] {m, l}.
-    int2 *own_record;  // [requests] {first own slot / kv heads, splits}
+    uint32_t row_tile;       // pairs to a tile of the row kernel
+    // Partial results, unnormalised: [slot][row_tile][128] sums and [slot][row_tile] {m, l}.
+    int4 *own_record;  // [requests] {first own slot / kv heads, splits, row tiles}
     float *own_sum, *prefix_sum;
     float2 *own_ml, *prefix_ml;
     uint32_t own_groups;  // capacity of the own partials, in slots per KV head
     uint32_t prefix_splits, prefix_tiles;
     uint32_t target;  // own items wanted in all
+    // The schedule (paged_tiles.cuh).
+    int32_t *header;   // [kTlHeader]
+    int4 *short_list;  // [rows] {batch row, own row, request, row of it} of the short requests' rows
+    // The tile kernel's share; tile_rows 0: it has none.
+    const void *pool;
+    uint32_t tile_rows;  // batch rows to a tile
+    uint32_t tile_grid, tile_cap;
+    struct TileShape *tile_shape;  // [tile_cap]
+    uint32_t *tile_unit;           // [tile_cap + 1] key steps before each tile
+    float *tile_sum;               // [slot][256][128], [slot][256] {m, l}
+    float2 *tile_ml;
 };
+enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlHeader = 8 };
+constexpr int kTlPairs = 256;     // (row, head) pairs to a tile
+constexpr int kTlShortPairs = 32; // requests of up to so many keep their own rows in the row kernel
+constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 
-// Row tile of the row kernel: 16 (row, head-in-group) pairs, the M of one MMA.
-constexpr int kRtM = 16;
-constexpr int kRtWarps = 4;                        // warps sharing a stage's keys
-constexpr int kRtThreads = 32 * (kRtWarps + 1);    // and the copying warp
-constexpr int kRtStages = 3;
-constexpr int kRtStageBytes = 32768;               // keys, then values
-constexpr int kRtMinPages = 2;                     // least pages worth an item of their own
-constexpr int kRtBatch = 8;                        // items looked up at a time
+// The row kernel works on slabs of 16 keys, the M of one mma.sync, against
+// tiles of 8 or 16 (row, head-in-group) pairs, its N.
+constexpr int kRtKeys = 16;
+constexpr int kRtWarps = 6;                      // computing warps, a slab each in turn
+constexpr int kRtThreads = 32 * (kRtWarps + 1);  // and the copying warp
+constexpr int kRtMinPages = 2;                   // least pages worth an item of their own
+constexpr int kRtBatch = 8;                      // items looked up at a time
 template <bool F32>
-__host__ __device__ constexpr int rt_stage_rows() {
-    return F32 ? 32 : 64;
+__host__ __device__ constexpr int rt_slab_bytes() {  // keys, then values
+    return 2 * kRtKeys * kPgDim * (F32 ? 4 : 2);
 }
-constexpr int kRtQBytes = kRtM * kPgDim * 4;  // FP32 queries; joined sums of the warps
-constexpr int kRtSmem = 1024 + kRtStages * kRtStageBytes + kRtQBytes;
+// A ring of slabs and, behind it, the queries or the warps' joined sums; two
+// CTAs to an SM. The ring's places are a multiple of the warps, so each place
+// serves one warp and that warp sees all of its phases in turn: a wait by
+// parity could not tell a phase from the one before the last.
+constexpr int kRtRing = 98304;
+constexpr int kRtSmem = 1024 + kRtRing + 16 * kPgDim * 4;
 
 // A request's new rows and visible own keys.
 struct OwnShape {
@@ -65,8 +84,39 @@ __device__ __forceinline__ OwnShape own_shape(const PagedAttnParams &p, int64_t 
     const int64_t first = p.window ? max(s.at0 - p.window + 1, static_cast<int64_t>(0)) : 0;
     s.page0 = static_cast<int32_t>(first / kPgRows);
     s.pages = s.rows ? max((s.length + kPgRows - 1) / kPgRows - s.page0, 0) : 0;
-    s.tiles = static_cast<int32_t>((static_cast<int64_t>(s.rows) * p.group + kRtM - 1) / kRtM);
+    s.tiles = static_cast<int32_t>((static_cast<int64_t>(s.rows) * p.group + p.row_tile - 1) / p.row_tile);
     return s;
+}
+
+// Short requests' own rows go through the row kernel, 16 pairs at a time; the
+// others are the tile kernel's, where there is one.
+__device__ __forceinline__ bool request_is_short(const PagedAttnParams &p, const OwnShape &s) {
+    return !p.tile_rows || static_cast<int64_t>(s.rows) * p.group <= kTlShortPairs;
+}
+__device__ __forceinline__ OwnShape short_shape(const PagedAttnParams &p, int64_t r) {
+    OwnShape s = own_shape(p, r);
+    if (!request_is_short(p, s)) s.tiles = s.pages = 0;
+    return s;
+}
+
+// What one tile covers, as the schedule lays it down. Key steps are of 128.
+struct __align__(16) TileShape {
+    int32_t request;     // -1: rows of the short list, prefix only
+    int32_t row0, rows;  // in the batch, or in that list
+    int32_t at0;         // own row of its first batch row
+    int32_t pre0, pre1;  // prefix key steps
+    int32_t own0, own1;  // own key steps
+    int32_t own_limit;   // own keys from here on are seen by none
+    int32_t unused[3];
+    __device__ int32_t steps() const { return pre1 - pre0 + own1 - own0; }
+};
+__device__ __forceinline__ int32_t tile_first_row(const PagedAttnParams &p, int32_t tile) { return p.tile_shape[tile].row0; }
+__device__ __forceinline__ int32_t tile_row_count(const PagedAttnParams &p, int32_t tile) { return p.tile_shape[tile].rows; }
+
+// The tile kernel's CTAs take equal runs of all units.
+__device__ __forceinline__ int64_t tile_cta_start(int64_t units, int32_t ctas, int32_t c) { return units * c / ctas; }
+__device__ __forceinline__ int32_t tile_cta_of(int64_t units, int32_t ctas, int64_t unit) {
+    return static_cast<int32_t>(((unit + 1) * ctas - 1) / units);
 }
 
 struct RowItem {
@@ -131,66 +181,476 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// FP32 as two TF32 terms (11 significant bits each): x = hi + lo to 2^-22.
-__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    const float rest = __fsub_rn(x, __uint_as_float(hi));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+// The 8x8 transpose of a matrix of 16-bit elements held two to a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ void rt_bar() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kRtWarps) : "memory"); }
+constexpr float kLazy = 8.0f;  // a maximum is renewed when passed by 2^8
 
-// Byte offset of a 16-byte chunk in a stage's [boxes][rows][128 bytes] tile
-// with the copy engine's 128-byte swizzle.
-template <int ROWS>
+// Byte offset of a 16-byte chunk in a slab's [boxes][16][128 bytes] rows with
+// the copy engine's 128-byte swizzle.
 __device__ __forceinline__ uint32_t rt_chunk(uint32_t row, uint32_t chunk) {
-    return (chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+    return (chunk >> 3) * (kRtKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// A CTA's shared state, as its computing warps use it.
+template <int PAIRS>
+struct RowCta {
+    uint64_t *full, *empty;
+    const unsigned char *slabs;
+    float *joined;              // [groups][PAIRS][128]; queries in operand order before that
+    float2 (*warp_ml)[PAIRS];   // [warps]
+};
+
+// The keys that a pair of an item sees, [lo, hi); lo -1 where there is no such pair.
+__device__ __forceinline__ int2 rt_sees(const PagedAttnParams &p, const RowItem &it, int64_t pair) {
+    if (pair >= static_cast<int64_t>(it.rows) * p.group) return make_int2(-1, 0);
+    const int32_t i = static_cast<int32_t>(pair / p.group);
+    if (it.request >= 0) {
+        const int64_t at = it.at0 + i;
+        const int64_t lo = p.window ? max(at - p.window + 1, static_cast<int64_t>(0)) : 0;
+        return make_int2(static_cast<int32_t>(lo), static_cast<int32_t>(max(at + 1, static_cast<int64_t>(0))));
+    }
+    int64_t lo = 0;
+    if (p.window && p.requests) {  // its request's length decides: the last one to start at or before row i
+        uint32_t r = 0, n = p.requests;
+        while (n > 1) {
+            const uint32_t half = n / 2;
+            const bool below = p.starts[r + half] <= i;
+            r = below ? r + half : r;
+            n = below ? n - half : half;
+        }
+        const OwnShape s = own_shape(p, r);
+        lo = min(max(p.prefix + s.at0 + i - s.row0 - p.window + 1, static_cast<int64_t>(0)), p.prefix);
+    }
+    return make_int2(static_cast<int32_t>(lo), static_cast<int32_t>(p.prefix));
+}
+// Where a pair's query starts (in elements), or -1.
+__device__ __forceinline__ int64_t rt_query(const PagedAttnParams &p, const RowItem &it, int64_t pair) {
+    if (pair >= static_cast<int64_t>(it.rows) * p.group) return -1;
+    const uint64_t row = static_cast<uint64_t>(it.row0) + pair / p.group;
+    return static_cast<int64_t>(row * p.q_stride + (static_cast<uint64_t>(it.head) * p.group + pair % p.group) * kPgDim);
+}
+
+template <int NT>
+__device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const RowItem &it, const RowCta<8 * NT> &cta, int64_t begin,
+                                             int64_t end, int32_t slabs, uint32_t ring, bool &dead) {
+    constexpr int PAIRS = 8 * NT, SLAB = rt_slab_bytes<false>(), SLABS = kRtRing / SLAB;
+    constexpr int GROUPS = 16 / PAIRS;  // of warps whose sums are joined side by side
+    constexpr bool QSM = NT > 1;        // queries read from shared memory at each use, to save registers
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int64_t pair0 = static_cast<int64_t>(it.tile) * PAIRS;
+    // This thread's pairs, 8 nt + 2 t + c: which keys they see.
+    int32_t see_lo[NT][2], see_hi[NT][2];
+#pragma unroll
+    for (int x = 0; x < 2 * NT; ++x) {
+        const int2 sees = rt_sees(p, it, pair0 + 8 * (x >> 1) + 2 * t + (x & 1));
+        see_lo[x >> 1][x & 1] = sees.x;
+        see_hi[x >> 1][x & 1] = sees.y;
+    }
+    // Queries as MMA operands, in registers or in shared memory in operand order.
+    uint32_t qf[QSM ? 1 : kPgDim / 16][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int64_t at = rt_query(p, it, pair0 + 8 * nt + g);
+        const uint16_t *src = static_cast<const uint16_t *>(p.q) + at;
+        const auto pick = [&](int ks, int x) { return at >= 0 ? *reinterpret_cast<const uint32_t *>(src + 16 * ks + 2 * t + 8 * x) : 0u; };
+        if constexpr (QSM) {
+            for (int ks = warp; ks < kPgDim / 16; ks += kRtWarps)
+                reinterpret_cast<uint2 *>(cta.joined)[(ks * NT + nt) * 32 + lane] = make_uint2(pick(ks, 0), pick(ks, 1));
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < kPgDim / 16; ++ks)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) qf[ks][nt][x] = pick(ks, x);
+        }
+    }
+    if (QSM) rt_bar();
+    float o[8][NT][4];  // dims 16 j + g (+ 8) x pairs 2 t (+ 1)
+    float mx[NT][2], sum[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[j][nt][x] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            mx[nt][c] = -INFINITY;
+            sum[nt][c] = 0.0f;
+        }
+    }
+
+    for (int32_t n = warp; n < slabs && !dead; n += kRtWarps) {
+        const uint32_t q = ring + n, st = q % SLABS;
+        if (!mbar_wait(&cta.full[st], (q / SLABS) & 1u)) dead = true;
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
+        const int32_t key0 = static_cast<int32_t>(begin) + n * kRtKeys;
+        const uint32_t kbase = smem_u32(cta.slabs + st * SLAB), vbase = kbase + SLAB / 2;
+        // ---- scores: key g (x = 0, 1) and g + 8 (2, 3) of pairs 2 t, 2 t + 1
+        float s[NT][4], c1[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[nt][x] = c1[nt][x] = 0.0f;
+        {
+            const uint32_t r = lane & 15, half = lane >> 4;
+#pragma unroll
+            for (int ks = 0; ks < kPgDim / 16; ++ks) {
+                uint32_t a[4];
+                ldsm4(kbase + rt_chunk(r, 2 * ks + half), a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    uint2 b;
+                    if constexpr (QSM) b = reinterpret_cast<const uint2 *>(cta.joined)[(ks * NT + nt) * 32 + lane];
+                    else b = make_uint2(qf[ks][nt][0], qf[ks][nt][1]);
+                    mma_bf16(ks & 1 ? c1[nt] : s[nt], a, b.x, b.y);
+                }
+            }
+        }
+        // ---- masks; a key that exists and that some pair does not see?
+        const int32_t left = static_cast<int32_t>(min(end - key0, static_cast<int64_t>(kRtKeys)));
+        bool hidden = false, move = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int c = x & 1, key = g + 8 * (x >> 1);
+                const bool seen = key0 + key >= see_lo[nt][c] && key0 + key < see_hi[nt][c] && key < left;
+                hidden |= !seen && key < left && see_lo[nt][c] >= 0;
+                s[nt][x] = seen ? (s[nt][x] + c1[nt][x]) * p.scale2 : -INFINITY;
+                move |= s[nt][x] > mx[nt][c] + kLazy;
+            }
+        // The reference point moves when a score passes it by 2^8 (the first one always does):
+        // weights stay below 2^8, and the sums are rarely scaled.
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float top = fmaxf(mx[nt][c], fmaxf(s[nt][c], s[nt][2 + c]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float corr = top == -INFINITY ? 1.0f : pg_exp2(mx[nt][c] - top);
+                    mx[nt][c] = top;
+                    sum[nt][c] *= corr;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[j][nt][c] *= corr;
+                        o[j][nt][2 + c] *= corr;
+                    }
+                }
+        }
+        // ---- weights, transposed into the product's operand; the sums are those of the rounded ones
+        uint32_t pf[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float e[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) e[c] = mx[nt][c] == -INFINITY ? 0.0f : pg_exp2(s[nt][2 * h + c] - mx[nt][c]);
+                const uint32_t w = pg_pack(e[0], e[1]);
+                pf[nt][h] = transpose8(w);
+                s[nt][2 * h] = bf16_lo(w);
+                s[nt][2 * h + 1] = bf16_hi(w);
+                sum[nt][0] += s[nt][2 * h];
+                sum[nt][1] += s[nt][2 * h + 1];
+            }
+        // ---- sums. A weight of zero times a value that is not finite would be NaN: such values
+        // leave the products and are added where they are seen. Only slabs with masked keys are
+        // looked over; keys past the end are zeroed in any case.
+        const bool careful = __any_sync(0xffffffffu, hidden) || left < kRtKeys;
+        bool odd = false;
+        const uint32_t r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t a[4];
+            ldsm4_t(vbase + rt_chunk(r, 2 * j + half), a);
+            if (careful) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int key = 2 * t + 8 * (x >> 1);
+                    const bool bad0 = (a[x] & 0x7f80u) == 0x7f80u, bad1 = (a[x] & 0x7f800000u) == 0x7f800000u;
+                    odd |= (bad0 && key < left) || (bad1 && key + 1 < left);
+                    if (bad0 || key >= left) a[x] &= 0xffff0000u;
+                    if (bad1 || key + 1 >= left) a[x] &= 0x0000ffffu;
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_bf16(o[j][nt], a, pf[nt][0], pf[nt][1]);
+        }
+        if (careful && __any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+            for (int key = 0; key < left; ++key)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[2];
+                    bool seen[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int src = (key & 7) * 4 + t;
+                        const float a = __shfl_sync(0xffffffffu, s[nt][c], src), b = __shfl_sync(0xffffffffu, s[nt][2 + c], src);
+                        w[c] = key < 8 ? a : b;
+                        seen[c] = key0 + key >= see_lo[nt][c] && key0 + key < see_hi[nt][c];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t dim = 16 * j + 8 * x + g;
+                            const float v = __uint_as_float(lds_u16(vbase + rt_chunk(key, dim / 8) + 2 * (dim & 7)) << 16);
+                            if (!isfinite(v)) {
+                                if (seen[0]) o[j][nt][2 * x] += w[0] * v;
+                                if (seen[1]) o[j][nt][2 * x + 1] += w[1] * v;
+                            }
+                        }
+                }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&cta.empty[st]);
+    }
+
+    // ---- join the warps: {m, l} of each pair, then the sums, a group's warps in turn
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float l = sum[nt][c];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            if (g == 0) cta.warp_ml[warp][8 * nt + 2 * t + c] = make_float2(mx[nt][c], l);
+        }
+    rt_bar();  // and every warp is done with the queries
+    float factor[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kRtWarps; ++w) top = fmaxf(top, cta.warp_ml[w][8 * nt + 2 * t + c].x);
+            factor[nt][c] = mx[nt][c] == -INFINITY ? 0.0f : pg_exp2(mx[nt][c] - top);
+        }
+#pragma unroll 1
+    for (int w = 0; w < kRtWarps / GROUPS; ++w) {
+        if (w == warp / GROUPS) {
+            float *dst = cta.joined + (warp % GROUPS) * PAIRS * kPgDim;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        float *to = dst + (8 * nt + 2 * t + (x & 1)) * kPgDim + 16 * j + 8 * (x >> 1) + g;
+                        const float v = o[j][nt][x] * factor[nt][x & 1];
+                        *to = w ? *to + v : v;
+                    }
+        }
+        rt_bar();
+    }
+}
+
+// FP32: lane l holds dimensions 4l..4l+3 of all eight pairs' queries and sums.
+// Four keys' scores are 32 numbers, partial over the lanes: a butterfly leaves
+// lane l the score of key l / 8 and pair l % 8. Each step of it keeps half of
+// the numbers and sends the other; with key and pair of a register chosen by
+// the lane's own number (key ^ l / 8, pair ^ l % 8) it is always the same half
+// of the registers, and nothing is selected.
+__device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowItem &it, const RowCta<8> &cta, float *weights,
+                                            int64_t begin, int64_t end, int32_t slabs, uint32_t ring, bool &dead) {
+    constexpr int SLAB = rt_slab_bytes<true>(), SLABS = kRtRing / SLAB;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t pair0 = static_cast<int64_t>(it.tile) * 8;
+    const int2 sees = rt_sees(p, it, pair0 + (lane & 7));
+    float4 q[8], o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t at = rt_query(p, it, pair0 + (i ^ (lane & 7)));
+        q[i] = at >= 0 ? ld4(static_cast<const float *>(p.q) + at + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float m = -INFINITY, l = 0.0f;  // of pair lane % 8, l over this lane's keys
+    const uint32_t box = (lane >> 3) * (kRtKeys * 128);
+    for (int32_t n = warp; n < slabs && !dead; n += kRtWarps) {
+        const uint32_t x = ring + n, st = x % SLABS;
+        if (!mbar_wait(&cta.full[st], (x / SLABS) & 1u)) dead = true;
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
+        const int32_t key0 = static_cast<int32_t>(begin) + n * kRtKeys;
+        const unsigned char *keys = cta.slabs + st * SLAB + box, *values = keys + SLAB / 2;
+        const auto piece = [&](const unsigned char *base, int row) {
+            return *reinterpret_cast<const float4 *>(base + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+        };
+        float s[4];
+#pragma unroll
+        for (int four = 0; four < 4; ++four) {
+            float v[4][8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 kv = piece(keys, 4 * four + (k ^ (lane >> 3)));
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[k][i] = fmaf(q[i].w, kv.w, fmaf(q[i].z, kv.z, fmaf(q[i].y, kv.y, __fmul_rn(q[i].x, kv.x))));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[0][i] += __shfl_xor_sync(0xffffffffu, v[2][i], 16);
+                v[1][i] += __shfl_xor_sync(0xffffffffu, v[3][i], 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[0][i] += __shfl_xor_sync(0xffffffffu, v[1][i], 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[0][i] += __shfl_xor_sync(0xffffffffu, v[0][i + 4], 4);
+            v[0][0] += __shfl_xor_sync(0xffffffffu, v[0][2], 2);
+            v[0][1] += __shfl_xor_sync(0xffffffffu, v[0][3], 2);
+            s[four] = v[0][0] + __shfl_xor_sync(0xffffffffu, v[0][1], 1);
+        }
+        const int32_t left = static_cast<int32_t>(min(end - key0, static_cast<int64_t>(kRtKeys)));
+        bool hidden = false, move = false;
+        uint32_t seen_by[4];  // bit 8 * key + pair of four keys
+#pragma unroll
+        for (int four = 0; four < 4; ++four) {
+            const int key = 4 * four + (lane >> 3);
+            const bool seen = key0 + key >= sees.x && key0 + key < sees.y && key < left;
+            hidden |= !seen && sees.x >= 0;
+            seen_by[four] = __ballot_sync(0xffffffffu, seen);
+            s[four] = seen ? s[four] * p.scale2 : -INFINITY;
+            move |= s[four] > m + kLazy;
+        }
+        if (__any_sync(0xffffffffu, move)) {
+            float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), m);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float corr = top == -INFINITY ? 1.0f : pg_exp2(m - top);
+            m = top;
+            l *= corr;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = __shfl_sync(0xffffffffu, corr, i);
+                o[i] = make_float4(o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f);
+            }
+        }
+#pragma unroll
+        for (int four = 0; four < 4; ++four) {
+            const float w = m == -INFINITY ? 0.0f : pg_exp2(s[four] - m);
+            l += w;
+            weights[32 * four + lane] = w;  // [key][pair]
+        }
+        __syncwarp();
+        if (__any_sync(0xffffffffu, hidden)) {
+            // Keys that some pair does not see, or that do not exist: their values, whatever they
+            // are, are added for the pairs that see them only.
+#pragma unroll 1
+            for (int key = 0; key < left; ++key) {
+                const float4 v = piece(values, key);
+                const uint32_t by = seen_by[0] * (key < 4) | seen_by[1] * (key >= 4 && key < 8) |
+                                    seen_by[2] * (key >= 8 && key < 12) | seen_by[3] * (key >= 12);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float w = weights[8 * key + i];
+                    if ((by >> (8 * (key & 3) + i)) & 1u)
+                        o[i] = make_float4(fmaf(w, v.x, o[i].x), fmaf(w, v.y, o[i].y), fmaf(w, v.z, o[i].z), fmaf(w, v.w, o[i].w));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int key = 0; key < kRtKeys; ++key) {
+                const float4 v = piece(values, key);
+                const float4 a = ld4(weights + 8 * key), b = ld4(weights + 8 * key + 4);
+                const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    o[i] = make_float4(fmaf(w[i], v.x, o[i].x), fmaf(w[i], v.y, o[i].y), fmaf(w[i], v.z, o[i].z), fmaf(w[i], v.w, o[i].w));
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&cta.empty[st]);
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    if (lane < 8) cta.warp_ml[warp][lane] = make_float2(m, l);
+    rt_bar();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kRtWarps; ++w) top = fmaxf(top, cta.warp_ml[w][lane & 7].x);
+    const float factor = m == -INFINITY ? 0.0f : pg_exp2(m - top);
+#pragma unroll 1
+    for (int w = 0; w < kRtWarps / 2; ++w) {
+        if (w == warp / 2) {
+            float *dst = cta.joined + (warp & 1) * 8 * kPgDim + 4 * lane;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = __shfl_sync(0xffffffffu, factor, i);
+                float4 v = make_float4(o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f);
+                if (w) {
+                    const float4 u = ld4(dst + i * kPgDim);
+                    v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
+                }
+                *reinterpret_cast<float4 *>(dst + i * kPgDim) = v;
+            }
+        }
+        rt_bar();
+    }
 }
 
 // ---- the row kernel ---------------------------------------------------------------
-// Items of 16 (row, head) pairs over a run of pages, persistent CTAs taking
-// every gridDim-th item. Own keys are read once per 16 rows and the products
-// are far below the tensor pipe's rate, so this is a streaming kernel: one
-// warp copies pages into a ring of three 32 KB stages, two CTAs to an SM, and
-// the other four each take a quarter of a stage's keys with their own running
-// maximum and sums, joined at the end of the item.
-template <bool F32>
+// Items of one tile of pairs over a run of pages; persistent CTAs take every
+// gridDim-th. Own keys are read once per tile and the products are far below
+// the tensor pipe's rate, so this is a streaming kernel: one warp copies slabs
+// of 16 keys into a ring, two CTAs to an SM, and six warps take a slab
+// each in turn, with a running maximum and sums of their own that are joined
+// at the end of the item. Scores are computed transposed, keys x pairs: a
+// group of up to eight heads then fills the N of an MMA instead of half its M,
+// and the value sums (dimensions x pairs) take 32 registers a thread instead
+// of 64, which leaves room for 14 warps on an SM.
+// FP32 pools take the CUDA cores: 32 multiply-adds a lane for each key's
+// scores and as many for its values are 350 issue cycles of an SM per slab,
+// half of what the slab's 16 KB take to arrive, and lose nothing to splitting.
+// (Measured before: TF32 mma.sync with two terms to an operand, 5 us per slab
+// and warp against 0.7 us for BF16.)
+template <bool F32, int NT>
 __global__ void __launch_bounds__(kRtThreads, 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map, const PagedAttnParams p) {
-    constexpr int SR = rt_stage_rows<F32>(), WK = SR / kRtWarps;  // rows per stage, keys per warp
-    constexpr int NK = WK / 8;                                    // 8-key score tiles per warp
-    constexpr uint32_t kValues = kRtStageBytes / 2;
-    extern __shared__ __align__(128) unsigned char rt_smem[];
-    __shared__ __align__(8) uint64_t full[kRtStages], empty[kRtStages];
-    __shared__ int32_t stage_page[kRtStages];
+    constexpr int PAIRS = 8 * NT, SLAB = rt_slab_bytes<F32>(), SLABS = kRtRing / SLAB;
+    static_assert(SLABS % kRtWarps == 0, "a place of the ring serves one warp");
+    constexpr int GROUPS = 16 / PAIRS;  // of warps whose sums are joined side by side
+    static_assert(!F32 || NT == 1, "FP32: eight pairs");
+    constexpr int PER = kPgRows / kRtKeys;  // slabs per page
+    extern __shared__ __align__(128) unsigned char rt_raw[];
+    __shared__ __align__(8) uint64_t full[SLABS], empty[SLABS];
     __shared__ int64_t scan[kRtThreads / 32];
     __shared__ RowItem items[kRtBatch];
-    __shared__ float2 warp_ml[kRtWarps][kRtM];
+    __shared__ float2 warp_ml[kRtWarps][PAIRS];
+    __shared__ __align__(16) float weights[F32 ? kRtWarps : 1][F32 ? kRtKeys * 8 : 4];
     __shared__ int64_t shared_min;
     unsigned char *base = reinterpret_cast<unsigned char *>(
-        (reinterpret_cast<uintptr_t>(rt_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-    float *qsm = reinterpret_cast<float *>(base + kRtStages * kRtStageBytes);
+        (reinterpret_cast<uintptr_t>(rt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    float *joined = reinterpret_cast<float *>(base + kRtRing);  // [GROUPS][PAIRS][128]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const RowCta<PAIRS> cta{full, empty, base, joined, warp_ml};
     if (tid == 0) {
-        for (int s = 0; s < kRtStages; ++s) {
+        for (int s = 0; s < SLABS; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], kRtWarps);
+            mbar_init(&empty[s], 1);
         }
         fence_barrier_init();
         prefetch_tensormap(&map);
     }
+    pdl_launch_dependents();
 
     // Every CTA lays the items out by itself from the requests' lengths.
     const int64_t R = p.requests, per = (R + kRtThreads - 1) / kRtThreads;
     const int64_t r0 = min(R, tid * per), r1 = min(R, r0 + per);
     int64_t units = 0, lowest = INT64_MAX;
     for (int64_t r = r0; r < r1; ++r) {
-        const OwnShape s = own_shape(p, r);
+        const OwnShape s = short_shape(p, r);
         units += static_cast<int64_t>(s.tiles) * s.pages;
         if (s.rows) lowest = min(lowest, s.at0);
     }
@@ -203,7 +663,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                               (total_units * p.kh + p.target - 1) / p.target);
     int64_t mine = 0;
     for (int64_t r = r0; r < r1; ++r) {
-        const OwnShape s = own_shape(p, r);
+        const OwnShape s = short_shape(p, r);
         mine += s.tiles * ((s.pages + chunk - 1) / chunk);
     }
     const int64_t first = pg_block_scan<kRtThreads>(mine, scan, &total);
@@ -214,9 +674,9 @@ __global__ void __launch_bounds__(kRtThreads, 2)
     if (blockIdx.x == 0) {
         int64_t at = first;
         for (int64_t r = r0; r < r1; ++r) {
-            const OwnShape s = own_shape(p, r);
+            const OwnShape s = short_shape(p, r);
             const int64_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
-            p.own_record[r] = at + n <= total ? make_int2(static_cast<int>(at), static_cast<int>(splits)) : make_int2(0, 0);
+            p.own_record[r] = at + n <= total ? make_int4(static_cast<int>(at), static_cast<int>(splits), s.tiles, 0) : make_int4(0, 0, 0, 0);
             at += n;
         }
     }
@@ -229,7 +689,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
     const int64_t own_items = total * p.kh;
     const int64_t all_items = own_items + static_cast<int64_t>(p.prefix_splits) * p.prefix_tiles * p.kh;
 
-    uint32_t stage = 0, phase = 0, issued = 0;
+    uint32_t ring = 0, issued = 0;  // slabs of the items before; copied ones
     bool dead = false;
     for (int64_t batch = blockIdx.x; batch < all_items; batch += static_cast<int64_t>(gridDim.x) * kRtBatch) {
         __syncthreads();  // the last batch's items are done with
@@ -261,7 +721,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
             if (group >= first && group < first + mine) {
                 int64_t at = first;
                 for (int64_t r = r0; r < r1; ++r) {
-                    const OwnShape s = own_shape(p, r);
+                    const OwnShape s = short_shape(p, r);
                     const int64_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
                     if (group < at + n) {
                         RowItem it;
@@ -273,13 +733,13 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                         it.page0 = s.page0 + static_cast<int32_t>(split * chunk);
                         it.pages = static_cast<int32_t>(min(chunk, s.page0 + static_cast<int64_t>(s.pages) - it.page0));
                         // Keys past the tile's last row are seen by none of its rows.
-                        const int64_t last = s.at0 + min(static_cast<int64_t>(s.rows) - 1, (static_cast<int64_t>(it.tile) * kRtM + kRtM - 1) / p.group);
+                        const int64_t last = s.at0 + min(static_cast<int64_t>(s.rows) - 1, (static_cast<int64_t>(it.tile) * PAIRS + PAIRS - 1) / p.group);
                         it.limit = static_cast<int32_t>(min(max(last + 1, static_cast<int64_t>(0)), static_cast<int64_t>(s.length)));
                         it.row0 = s.row0;
                         it.rows = s.rows;
                         it.at0 = s.at0;
                         it.slot = static_cast<uint32_t>(id);
-                        it.direct = splits == 1 && p.prefix_splits == 0;
+                        it.direct = splits == 1 && p.prefix == 0;
                         items[k] = it;
                         break;
                     }
@@ -294,460 +754,249 @@ __global__ void __launch_bounds__(kRtThreads, 2)
             const RowItem it = items[k];
             const int64_t begin = static_cast<int64_t>(it.page0) * kPgRows;
             const int64_t end = min(begin + static_cast<int64_t>(it.pages) * kPgRows, static_cast<int64_t>(it.limit));
-            const int32_t stages = end > begin ? static_cast<int32_t>((end - begin + SR - 1) / SR) : 0;
+            const int32_t slabs = end > begin ? static_cast<int32_t>((end - begin + kRtKeys - 1) / kRtKeys) : 0;
             if (warp == kRtWarps) {
                 // ---- the copying warp: page ids 32 at a time, one lane issues.
                 const int32_t *table = it.request < 0 ? p.prefix_pages
                                                       : p.tables + static_cast<uint64_t>(it.request) * p.table_stride;
-                constexpr int PER = kPgRows / SR;  // stages per page
-                int32_t ids = 0;
-                for (int32_t n = 0; n < stages && !dead; ++n) {
-                    const int32_t pg = n / PER;
-                    if (n % (32 * PER) == 0) ids = pg + lane < it.pages ? table[it.page0 + pg + lane] : -1;
-                    int32_t id = __shfl_sync(0xffffffffu, ids, pg & 31);
-                    if (lane == 0) {
-                        if (issued >= kRtStages && !mbar_wait(&empty[stage], phase ^ 1u)) dead = true;
-                        if (!dead) {
-                            if (id < 0 || id >= static_cast<int32_t>(p.pages)) {
-                                pg_flag(p.status, PLAMO_PAGED_PAGE);
-                                id = -1;
-                            }
-                            stage_page[stage] = id;
-                            if (id < 0) {
-                                mbar_arrive(&full[stage]);  // nothing to copy
+                for (int32_t n0 = 0; n0 < slabs && !dead; n0 += 32 * PER) {
+                    int32_t id = n0 / PER + lane < it.pages ? table[it.page0 + n0 / PER + lane] : 0;
+                    if (n0 / PER + lane < it.pages && (id < 0 || id >= static_cast<int32_t>(p.pages))) {
+                        pg_flag(p.status, PLAMO_PAGED_PAGE);
+                        id = static_cast<int32_t>(p.pages);  // past the pool: the copy brings zeros
+                    }
+                    for (int32_t n = n0; n < min(slabs, n0 + 32 * PER); ++n) {
+                        const int32_t page = __shfl_sync(0xffffffffu, id, (n / PER) & 31);
+                        if (lane == 0 && !dead) {
+                            const uint32_t q = ring + n, st = q % SLABS;
+                            if (q >= SLABS && !mbar_wait(&empty[st], (q / SLABS - 1) & 1u)) {
+                                dead = true;
                             } else {
-                                unsigned char *dst = base + stage * kRtStageBytes;
-                                const int y = id * 2 * kPgRows + (n % PER) * SR, x = it.head * kPgDim;
-                                mbar_expect_tx(&full[stage], kRtStageBytes);
+                                unsigned char *dst = base + st * SLAB;
+                                const int y = page * 2 * kPgRows + (n % PER) * kRtKeys, x = it.head * kPgDim;
+                                mbar_expect_tx(&full[st], SLAB);
                                 constexpr int BOX = F32 ? 32 : 64;  // elements in 128 bytes
 #pragma unroll
                                 for (int b = 0; b < kPgDim / BOX; ++b) {
-                                    tma_load_2d(dst + b * SR * 128, &map, x + b * BOX, y, &full[stage]);
-                                    tma_load_2d(dst + kValues + b * SR * 128, &map, x + b * BOX, y + kPgRows, &full[stage]);
+                                    tma_load_2d(dst + b * kRtKeys * 128, &map, x + b * BOX, y, &full[st]);
+                                    tma_load_2d(dst + SLAB / 2 + b * kRtKeys * 128, &map, x + b * BOX, y + kPgRows, &full[st]);
                                 }
+                                issued = q + 1;
                             }
                         }
                     }
                     dead = __shfl_sync(0xffffffffu, dead, 0);
-                    ++issued;
-                    if (++stage == kRtStages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
                 }
+                ring += slabs;
                 continue;
             }
             // ---- the computing warps
-            const int g = lane >> 2, t = lane & 3;
-            // This thread's two rows of the tile (g and g + 8): which keys they see.
-            int32_t see_lo[2], see_hi[2];
-            bool there[2];
-            const int64_t pairs = static_cast<int64_t>(it.rows) * p.group;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int64_t m = static_cast<int64_t>(it.tile) * kRtM + g + 8 * x;
-                see_lo[x] = see_hi[x] = 0;
-                there[x] = m < pairs;
-                if (!there[x]) continue;
-                const int32_t i = static_cast<int32_t>(m / p.group);
-                if (it.request >= 0) {
-                    const int64_t at = it.at0 + i;
-                    see_hi[x] = static_cast<int32_t>(max(at + 1, static_cast<int64_t>(0)));
-                    if (p.window) see_lo[x] = static_cast<int32_t>(max(at - p.window + 1, static_cast<int64_t>(0)));
-                } else {
-                    see_hi[x] = static_cast<int32_t>(p.prefix);
-                }
-            }
-            if (it.request < 0 && p.window) {
-                for (int m = 0; m < kRtM; ++m) {  // position of each row: its request's length decides
-                    const int64_t pair = static_cast<int64_t>(it.tile) * kRtM + m;
-                    if (pair >= pairs) break;
-                    const int32_t i = static_cast<int32_t>(pair / p.group);
-                    int32_t lo = 0;
-                    if (R) {
-                        const OwnShape s = own_shape(p, pg_owner(p.starts, p.requests, i));
-                        const int64_t at = s.at0 + i - s.row0;
-                        lo = static_cast<int32_t>(min(max(p.prefix + at - p.window + 1, static_cast<int64_t>(0)), p.prefix));
-                    }
-                    if ((m & 7) == g) see_lo[m >> 3] = lo;
-                }
-            }
-            // Queries: BF16 as MMA fragments in registers, FP32 in shared memory in fragment order.
-            uint32_t qf[F32 ? 1 : kPgDim / 16][4];
-            {
-                const uint64_t head0 = static_cast<uint64_t>(it.head) * p.group;
-                const unsigned char *row_ptr[2];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int64_t m = static_cast<int64_t>(it.tile) * kRtM + g + 8 * x;
-                    row_ptr[x] = nullptr;
-                    if (m < pairs) {
-                        const uint64_t row = static_cast<uint64_t>(it.row0) + m / p.group, h = head0 + m % p.group;
-                        row_ptr[x] = static_cast<const unsigned char *>(p.q) + (row * p.q_stride + h * kPgDim) * (F32 ? 4 : 2);
-                    }
-                }
-                if constexpr (F32) {
-                    // k-step ks: {row g dim 8ks+t, row g+8, row g dim 8ks+t+4, row g+8} at [ks][lane]
-                    rt_bar();  // the last item's joined sums have been read
-                    for (int ks = warp; ks < kPgDim / 8; ks += kRtWarps) {
-                        float4 v;
-                        const float *a = reinterpret_cast<const float *>(row_ptr[0]), *b = reinterpret_cast<const float *>(row_ptr[1]);
-                        v.x = a ? a[8 * ks + t] : 0.0f;
-                        v.y = b ? b[8 * ks + t] : 0.0f;
-                        v.z = a ? a[8 * ks + t + 4] : 0.0f;
-                        v.w = b ? b[8 * ks + t + 4] : 0.0f;
-                        reinterpret_cast<float4 *>(qsm)[ks * 32 + lane] = v;
-                    }
-                    rt_bar();
-                } else {
-#pragma unroll
-                    for (int ks = 0; ks < kPgDim / 16; ++ks)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const unsigned char *src = row_ptr[x & 1];
-                            qf[ks][x] = src ? *reinterpret_cast<const uint32_t *>(src + 2 * (16 * ks + 2 * t + 8 * (x >> 1))) : 0u;
-                        }
-                }
-            }
-            float o[16][4];
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[j][x] = 0.0f;
-            float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-
-            for (int32_t n = 0; n < stages && !dead; ++n) {
-                if (!mbar_wait(&full[stage], phase)) dead = true;
-                dead = __any_sync(0xffffffffu, dead);
-                if (dead) break;
-                const int32_t key0 = static_cast<int32_t>(begin) + n * SR + warp * WK;  // this warp's first key
-                // Only warps with keys that exist: the copy brings whole boxes.
-                if (stage_page[stage] >= 0 && key0 < end) {
-                    const uint32_t kbase = smem_u32(base + stage * kRtStageBytes), vbase = kbase + kValues;
-                    const uint32_t krow = warp * WK;
-                    float s[NK][4];
-                    if constexpr (F32) {
-                        // Products of the high terms in two chains, the cross terms in a third:
-                        // the tensor cores truncate as they add, so chains are kept short.
-                        float c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
-#pragma unroll
-                        for (int ks = 0; ks < kPgDim / 8; ++ks) {
-                            const float4 qv = reinterpret_cast<const float4 *>(qsm)[ks * 32 + lane];
-                            uint32_t ah[4], al[4], bh0, bl0, bh1, bl1;
-                            split_tf32(qv.x, ah[0], al[0]);
-                            split_tf32(qv.y, ah[1], al[1]);
-                            split_tf32(qv.z, ah[2], al[2]);
-                            split_tf32(qv.w, ah[3], al[3]);
-                            split_tf32(lds_f32(kbase + rt_chunk<SR>(krow + g, 2 * ks) + 4 * t), bh0, bl0);
-                            split_tf32(lds_f32(kbase + rt_chunk<SR>(krow + g, 2 * ks + 1) + 4 * t), bh1, bl1);
-                            if (ks & 1) mma_tf32(c1, ah, bh0, bh1);
-                            else mma_tf32(c0, ah, bh0, bh1);
-                            mma_tf32(c2, ah, bl0, bl1);
-                            mma_tf32(c2, al, bh0, bh1);
-                        }
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) s[0][x] = __fadd_rn(__fadd_rn(c0[x], c1[x]), c2[x]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < NK; ++j)
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) s[j][x] = 0.0f;
-                        const uint32_t r = krow + (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
-#pragma unroll
-                        for (int ks = 0; ks < kPgDim / 16; ++ks) {
-                            uint32_t b[4];
-                            ldsm4(kbase + rt_chunk<SR>(r, 2 * ks + half), b);
-                            mma_bf16(s[0], qf[ks], b[0], b[1]);
-                            mma_bf16(s[1], qf[ks], b[2], b[3]);
-                        }
-                    }
-                    // Masks and the running maximum.
-                    bool hidden = false;  // a key that exists is masked for one of this thread's rows
-                    float top[2] = {mx[0], mx[1]};
-#pragma unroll
-                    for (int j = 0; j < NK; ++j)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int32_t key = key0 + 8 * j + 2 * t + (x & 1);
-                            const int row = x >> 1;
-                            const bool seen = key >= see_lo[row] && key < see_hi[row] && key < end;
-                            hidden |= there[row] && !seen && key < end;
-                            s[j][x] = seen ? s[j][x] * p.scale2 : -INFINITY;
-                            top[row] = fmaxf(top[row], s[j][x]);
-                        }
-                    float corr[2];
-#pragma unroll
-                    for (int row = 0; row < 2; ++row) {
-                        top[row] = fmaxf(top[row], __shfl_xor_sync(0xffffffffu, top[row], 1));
-                        top[row] = fmaxf(top[row], __shfl_xor_sync(0xffffffffu, top[row], 2));
-                        corr[row] = top[row] == -INFINITY ? 1.0f : pg_exp2(mx[row] - top[row]);
-                        mx[row] = top[row];
-                        sum[row] *= corr[row];
-                    }
-#pragma unroll
-                    for (int j = 0; j < NK; ++j)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int row = x >> 1;
-                            s[j][x] = mx[row] == -INFINITY ? 0.0f : pg_exp2(s[j][x] - mx[row]);
-                        }
-                    const bool scaled = __any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f);
-                    if (scaled) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            o[j][0] *= corr[0];
-                            o[j][1] *= corr[0];
-                            o[j][2] *= corr[1];
-                            o[j][3] *= corr[1];
-                        }
-                    }
-                    // A weight of zero times a value that is not finite would be NaN: such values
-                    // leave the products and are added where they are seen. Only tiles with masked
-                    // keys are looked over; keys past `end` are zeroed in any case.
-                    const bool careful = __any_sync(0xffffffffu, hidden);
-                    const bool tail = key0 + WK > end;
-                    bool odd = false;
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) sum[x >> 1] += s[0][x];
-                        // Score column 2t is product index t, 2t + 1 is t + 4.
-                        uint32_t ph[4], pl[4];
-                        split_tf32(s[0][0], ph[0], pl[0]);
-                        split_tf32(s[0][2], ph[1], pl[1]);
-                        split_tf32(s[0][1], ph[2], pl[2]);
-                        split_tf32(s[0][3], ph[3], pl[3]);
-                        const bool in0 = key0 + 2 * t < end, in1 = key0 + 2 * t + 1 < end;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const uint32_t chunk = 2 * j + (g >> 2), word = 4 * (g & 3);
-                            float v0 = lds_f32(vbase + rt_chunk<SR>(krow + 2 * t, chunk) + word);
-                            float v1 = lds_f32(vbase + rt_chunk<SR>(krow + 2 * t + 1, chunk) + word);
-                            if (tail || careful) {
-                                const bool bad0 = !isfinite(v0), bad1 = !isfinite(v1);
-                                odd |= (in0 && bad0) || (in1 && bad1);
-                                if (!in0 || bad0) v0 = 0.0f;
-                                if (!in1 || bad1) v1 = 0.0f;
-                            }
-                            uint32_t vh0, vl0, vh1, vl1;
-                            split_tf32(v0, vh0, vl0);
-                            split_tf32(v1, vh1, vl1);
-                            float c[4] = {0, 0, 0, 0};
-                            mma_tf32(c, ph, vl0, vl1);
-                            mma_tf32(c, pl, vh0, vh1);
-                            mma_tf32(c, ph, vh0, vh1);
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) o[j][x] = __fadd_rn(o[j][x], c[x]);
-                        }
-                    } else {
-                        uint32_t pf[4];
-                        pf[0] = pg_pack(s[0][0], s[0][1]);
-                        pf[1] = pg_pack(s[0][2], s[0][3]);
-                        pf[2] = pg_pack(s[1][0], s[1][1]);
-                        pf[3] = pg_pack(s[1][2], s[1][3]);
-                        // The sums are those of the rounded weights.
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            s[x >> 1][2 * (x & 1)] = bf16_lo(pf[x]);
-                            s[x >> 1][2 * (x & 1) + 1] = bf16_hi(pf[x]);
-                            sum[x & 1] += bf16_lo(pf[x]) + bf16_hi(pf[x]);
-                        }
-                        const uint32_t r = krow + ((lane >> 3) & 1) * 8 + (lane & 7), half = lane >> 4;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            uint32_t b[4];
-                            ldsm4_t(vbase + rt_chunk<SR>(r, 2 * j + half), b);
-                            if (tail || careful) {
-#pragma unroll
-                                for (int x = 0; x < 4; ++x) {
-                                    const int32_t key = key0 + 2 * t + 8 * (x & 1);
-                                    const bool bad0 = (b[x] & 0x7f80u) == 0x7f80u, bad1 = (b[x] & 0x7f800000u) == 0x7f800000u;
-                                    odd |= (bad0 && key < end) || (bad1 && key + 1 < end);
-                                    if (bad0 || key >= end) b[x] &= 0xffff0000u;
-                                    if (bad1 || key + 1 >= end) b[x] &= 0x0000ffffu;
-                                }
-                            }
-                            mma_bf16(o[2 * j], pf, b[0], b[1]);
-                            mma_bf16(o[2 * j + 1], pf, b[2], b[3]);
-                        }
-                    }
-                    if ((tail || careful) && __any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-                        for (int key = 0; key < WK; ++key) {
-                            if (key0 + key >= end) break;
-                            // This row pair's weights of the key, from the lane that holds them.
-                            float w[2];
-#pragma unroll
-                            for (int row = 0; row < 2; ++row) {
-                                const int src = (lane & ~3) | ((key & 7) >> 1);
-                                float a = 0.0f;
-#pragma unroll
-                                for (int j = 0; j < NK; ++j)
-#pragma unroll
-                                    for (int c = 0; c < 2; ++c) {
-                                        const float x = __shfl_sync(0xffffffffu, s[j][2 * row + c], src);
-                                        if (key == 8 * j + (key & 6) + c) a = x;
-                                    }
-                                w[row] = a;
-                            }
-                            const bool seen0 = key0 + key >= see_lo[0] && key0 + key < see_hi[0];
-                            const bool seen1 = key0 + key >= see_lo[1] && key0 + key < see_hi[1];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-#pragma unroll
-                                for (int c = 0; c < 2; ++c) {
-                                    const uint32_t dim = 8 * j + 2 * t + c;
-                                    float v;
-                                    if constexpr (F32)
-                                        v = lds_f32(vbase + rt_chunk<SR>(krow + key, dim / 4) + 4 * (dim & 3));
-                                    else
-                                        v = __uint_as_float(lds_u16(vbase + rt_chunk<SR>(krow + key, dim / 8) + 2 * (dim & 7)) << 16);
-                                    if (!isfinite(v)) {
-                                        if (seen0) o[j][c] += w[0] * v;
-                                        if (seen1) o[j][2 + c] += w[1] * v;
-                                    }
-                                }
-                        }
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[stage]);
-                if (++stage == kRtStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            }
-
-            // ---- join the warps' sums: {m, l} of each row, then the sums one warp after another
-#pragma unroll
-            for (int row = 0; row < 2; ++row) {
-                sum[row] += __shfl_xor_sync(0xffffffffu, sum[row], 1);
-                sum[row] += __shfl_xor_sync(0xffffffffu, sum[row], 2);
-                if (t == 0) warp_ml[warp][g + 8 * row] = make_float2(mx[row], sum[row]);
-            }
-            rt_bar();  // and, FP32, every warp is done with the queries
-            float factor[2];
-            float2 joined[2];
-#pragma unroll
-            for (int row = 0; row < 2; ++row) {
+            const int64_t pair0 = static_cast<int64_t>(it.tile) * PAIRS, pairs = static_cast<int64_t>(it.rows) * p.group;
+            if constexpr (F32) rt_item_f32(p, it, cta, weights[warp], begin, end, slabs, ring, dead);
+            else rt_item_bf16<NT>(p, it, cta, begin, end, slabs, ring, dead);
+            ring += slabs;
+            // ---- result, or the tile's partial sums
+            for (int x = tid; x < PAIRS * kPgDim / 4; x += 32 * kRtWarps) {
+                const int pair = x / (kPgDim / 4), d = 4 * (x % (kPgDim / 4));
                 float top = -INFINITY, l = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kRtWarps; ++w) top = fmaxf(top, warp_ml[w][g + 8 * row].x);
+                for (int w = 0; w < kRtWarps; ++w) top = fmaxf(top, warp_ml[w][pair].x);
 #pragma unroll
                 for (int w = 0; w < kRtWarps; ++w) {
-                    const float2 ml = warp_ml[w][g + 8 * row];
+                    const float2 ml = warp_ml[w][pair];
                     if (ml.x != -INFINITY) l += pg_exp2(ml.x - top) * ml.y;
                 }
-                factor[row] = mx[row] == -INFINITY ? 0.0f : pg_exp2(mx[row] - top);
-                joined[row] = make_float2(top, l);
-            }
-#pragma unroll 1
-            for (int w = 0; w < kRtWarps; ++w) {
-                if (w == warp) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-#pragma unroll
-                        for (int row = 0; row < 2; ++row) {
-                            float2 *dst = reinterpret_cast<float2 *>(qsm + (g + 8 * row) * kPgDim + 8 * j + 2 * t);
-                            float2 v = make_float2(o[j][2 * row] * factor[row], o[j][2 * row + 1] * factor[row]);
-                            if (w) {
-                                const float2 before = *dst;
-                                v = make_float2(before.x + v.x, before.y + v.y);
-                            }
-                            *dst = v;
-                        }
-                    if (w == kRtWarps - 1 && t == 0) {
-                        warp_ml[0][g] = joined[0];
-                        warp_ml[0][g + 8] = joined[1];
-                    }
+                float4 v = ld4(joined + pair * kPgDim + d);
+                if constexpr (GROUPS == 2) {
+                    const float4 u = ld4(joined + (PAIRS + pair) * kPgDim + d);
+                    v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
                 }
-                rt_bar();
-            }
-            // ---- result, or the tile's partial sums
-            const int ctid = tid;  // 0..127
-            if (it.direct) {
-                for (int x = ctid; x < kRtM * kPgDim / 4; x += 32 * kRtWarps) {
-                    const int m16 = x / (kPgDim / 4), d = 4 * (x % (kPgDim / 4));
-                    const int64_t m = static_cast<int64_t>(it.tile) * kRtM + m16;
+                if (it.direct) {
+                    const int64_t m = pair0 + pair;
                     if (m >= pairs) continue;
-                    const float l = warp_ml[0][m16].y, inv = warp_ml[0][m16].x == -INFINITY ? 0.0f : 1.0f / l;
-                    float4 v = *reinterpret_cast<const float4 *>(qsm + m16 * kPgDim + d);
+                    const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
                     v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                     const uint64_t row = static_cast<uint64_t>(it.row0) + m / p.group;
                     const uint64_t at = row * p.out_stride + (static_cast<uint64_t>(it.head) * p.group + m % p.group) * kPgDim + d;
                     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + at, v);
                     else pg_store4(static_cast<uint16_t *>(p.out) + at, v);
+                } else {
+                    const uint64_t at = static_cast<uint64_t>(it.slot) * PAIRS + pair;
+                    *reinterpret_cast<float4 *>((it.request < 0 ? p.prefix_sum : p.own_sum) + at * kPgDim + d) = v;
+                    if (d == 0) (it.request < 0 ? p.prefix_ml : p.own_ml)[at] = make_float2(top, l);
                 }
-            } else {
-                float *dst = (it.request < 0 ? p.prefix_sum : p.own_sum) + static_cast<uint64_t>(it.slot) * kRtM * kPgDim;
-                float2 *ml = (it.request < 0 ? p.prefix_ml : p.own_ml) + static_cast<uint64_t>(it.slot) * kRtM;
-                for (int x = ctid; x < kRtM * kPgDim / 4; x += 32 * kRtWarps)
-                    reinterpret_cast<float4 *>(dst)[x] = reinterpret_cast<const float4 *>(qsm)[x];
-                if (ctid < kRtM) ml[ctid] = warp_ml[0][ctid];
             }
             rt_bar();  // before the next item writes warp_ml or the sums
         }
     }
     if (warp == kRtWarps && lane == 0) {
         // Every copy issued has landed before the CTA can exit.
-        const uint32_t from = issued > kRtStages ? issued - kRtStages : 0;
-        for (uint32_t n = from; n < issued; ++n)
-            if (!mbar_wait(&full[n % kRtStages], (n / kRtStages) & 1u)) break;
+        for (uint32_t n = issued > SLABS ? issued - SLABS : 0; n < issued; ++n)
+            if (!mbar_wait(&full[n % SLABS], (n / SLABS) & 1u)) break;
     }
     if (dead && lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
-    pdl_launch_dependents();
+    pdl_wait();  // done only when the schedule is: the kernels after it wait for this one alone
 }
 
 // ---- joining the parts ----------------------------------------------------------------
-// One warp per (row, query head): the prefix's splits and the request's own,
-// always in the same order. Rows with one part were written by the row kernel.
-template <bool F32>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
-    const uint32_t lane = threadIdx.x & 31;
-    const uint32_t row = blockIdx.x, head = blockIdx.y * 8 + (threadIdx.x >> 5);
-    pdl_wait();
-    if (head >= p.qh) return;
-    const uint32_t kv = head / p.group, in_group = head % p.group;
-    OwnShape s{};
-    int2 rec = make_int2(0, 0);
-    bool real = false;
-    if (p.requests && static_cast<int32_t>(row) < p.starts[p.requests]) {
-        const int32_t r = pg_owner(p.starts, p.requests, static_cast<int32_t>(row));
-        s = own_shape(p, r);
-        const int64_t i = static_cast<int64_t>(row) - s.row0;
-        real = i >= 0 && i < s.rows && s.at0 + i >= 0;
-        rec = p.own_record[r];
-    }
-    if (real && rec.y == 1 && p.prefix_splits == 0) return;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float top = -INFINITY, l = 0.0f;
-    if (real) {
-        const uint64_t m = static_cast<uint64_t>(row - s.row0) * p.group + in_group;
-        const uint64_t pm = static_cast<uint64_t>(row) * p.group + in_group;
-        const uint32_t parts = p.prefix_splits + rec.y;
-        auto slot = [&](uint32_t x) -> uint64_t {
-            if (x < p.prefix_splits) return (static_cast<uint64_t>(x) * p.prefix_tiles + pm / kRtM) * p.kh + kv;
-            return (static_cast<uint64_t>(rec.x) + static_cast<uint64_t>(x - p.prefix_splits) * s.tiles + m / kRtM) * p.kh + kv;
-        };
-        for (uint32_t x = lane; x < parts; x += 32)
-            top = fmaxf(top, x < p.prefix_splits ? p.prefix_ml[slot(x) * kRtM + pm % kRtM].x : p.own_ml[slot(x) * kRtM + m % kRtM].x);
-        top = warp_max(top);
-        if (top != -INFINITY)
-            for (uint32_t x = 0; x < parts; ++x) {
-                const bool shared = x < p.prefix_splits;
-                const uint64_t at = slot(x) * kRtM + (shared ? pm : m) % kRtM;
-                const float2 ml = shared ? p.prefix_ml[at] : p.own_ml[at];
-                if (ml.x == -INFINITY) continue;
-                const float w = pg_exp2(ml.x - top);
-                const float4 v = ld4((shared ? p.prefix_sum : p.own_sum) + at * kPgDim + 4 * lane);
-                o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
-                l = fmaf(w, ml.y, l);
+// One result (a row and head): parts [0, n0) at (first + x * stride) * rows +
+// place of one array, the rest in another; the sums joined in that order.
+struct PartList {
+    const float *sum;
+    const float2 *ml;
+    uint64_t first, stride;
+    uint32_t rows, place, count;
+    __device__ uint64_t at(uint32_t x) const { return (first + x * stride) * rows + place; }
+};
+// WPH warps work on it, `sub` is this one; every lane returns with the sums
+// over its share of parts, 32 at a time to a warp, and the common maximum.
+template <int WPH>
+__device__ __forceinline__ void join_parts(const PartList &a, const PartList &b, uint32_t sub, float4 &o, float &l, float &top) {
+    const uint32_t lane = threadIdx.x & 31, all = a.count + b.count;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    top = -INFINITY;
+    l = 0.0f;
+    const auto ml = [&](uint32_t x) { return x < a.count ? a.ml[a.at(x)] : b.ml[b.at(x - a.count)]; };
+    for (uint32_t x = lane; x < all; x += 32) top = fmaxf(top, ml(x).x);
+    top = warp_max(top);
+    if (top == -INFINITY) return;
+    for (uint32_t x0 = 32 * sub; x0 < all; x0 += 32 * WPH) {
+        // A lane weighs one part, then the parts' sums are loaded eight at once.
+        const uint32_t x = x0 + lane;
+        float w = 0.0f, part_l = 0.0f;
+        uint64_t here = 0;
+        if (x < all) {
+            const float2 y = ml(x);
+            w = y.x == -INFINITY ? 0.0f : pg_exp2(y.x - top);
+            part_l = w * y.y;
+            here = x < a.count ? a.at(x) : b.at(x - a.count);
+        }
+        const uint32_t some = min(32u, all - x0);
+        for (uint32_t y0 = 0; y0 < some; y0 += 8) {
+            float4 v[8];
+            float f[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const uint32_t z = (y0 + y) & 31;
+                f[y] = __shfl_sync(0xffffffffu, w, z);
+                l += __shfl_sync(0xffffffffu, part_l, z);
+                const uint64_t from = __shfl_sync(0xffffffffu, here, z);
+                v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (f[y] != 0.0f) v[y] = ld4((x0 + z < a.count ? a.sum : b.sum) + from * kPgDim + 4 * lane);
             }
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+                o = make_float4(fmaf(f[y], v[y].x, o.x), fmaf(f[y], v[y].y, o.y), fmaf(f[y], v[y].z, o.z), fmaf(f[y], v[y].w, o.w));
+        }
     }
+}
+template <bool F32>
+__device__ __forceinline__ void join_store(const PagedAttnParams &p, uint64_t row, uint32_t head, float4 o, float l, float top) {
     const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    const uint64_t at = row * p.out_stride + static_cast<uint64_t>(head) * kPgDim + 4 * lane;
-    if constexpr (F32) pg_store4(static_cast<float *>(p.out) + at, o);
-    else pg_store4(static_cast<uint16_t *>(p.out) + at, o);
+    const uint64_t to = row * p.out_stride + static_cast<uint64_t>(head) * kPgDim + 4 * (threadIdx.x & 31);
+    if constexpr (F32) pg_store4(static_cast<float *>(p.out) + to, o);
+    else pg_store4(static_cast<uint16_t *>(p.out) + to, o);
+}
+
+// Joins the short requests' rows (WPH warps each: eight where few rows were
+// split into many parts, one where there are rows enough), the prompts' tiles
+// that two or more CTAs shared, and zeroes the rows that see nothing.
+template <bool F32, int WPH>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
+    __shared__ float4 warp_sum_at[WPH][32];
+    __shared__ float warp_l[WPH];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WPH == 1 ? 0 : warp;
+    pdl_wait();
+    const int32_t tiles = p.tile_rows ? p.header[kTlTiles] : 0, pre_tiles = p.tile_rows ? p.header[kTlPreTiles] : 0;
+    const int32_t ctas = p.tile_rows ? p.header[kTlCtas] : 0;
+    const int64_t units = tiles ? static_cast<int64_t>(p.tile_unit[tiles]) * p.kh : 0;
+    const uint64_t results = static_cast<uint64_t>(p.header[kTlShortRows]) * p.qh;
+    const uint32_t lanes = WPH == 1 ? gridDim.x * 8 : gridDim.x;  // of results in flight
+    for (uint64_t n = WPH == 1 ? blockIdx.x * 8 + warp : blockIdx.x; n < results; n += lanes) {
+        const uint32_t listed = static_cast<uint32_t>(n / p.qh), head = static_cast<uint32_t>(n % p.qh);
+        const uint32_t kv = head / p.group, in_group = head % p.group;
+        const int4 e = p.short_list[listed];
+        PartList shared{}, own{};
+        if (e.y >= 0) {
+            const int4 rec = p.own_record[e.z];
+            if (rec.y == 1 && p.prefix == 0) continue;  // written where it was computed
+            const uint32_t m = e.w * p.group + in_group;
+            own = PartList{p.own_sum, p.own_ml, (static_cast<uint64_t>(rec.x) + m / p.row_tile) * p.kh + kv,
+                           static_cast<uint64_t>(rec.z) * p.kh, p.row_tile, m % p.row_tile, static_cast<uint32_t>(rec.y)};
+            if (p.prefix_splits) {
+                const uint64_t pm = static_cast<uint64_t>(e.x) * p.group + in_group;
+                shared = PartList{p.prefix_sum, p.prefix_ml, pm / p.row_tile * p.kh + kv, static_cast<uint64_t>(p.prefix_tiles) * p.kh,
+                                  p.row_tile, static_cast<uint32_t>(pm % p.row_tile), p.prefix_splits};
+            } else if (pre_tiles && ctas) {
+                const uint32_t tile = listed / p.tile_rows;
+                const int64_t steps = static_cast<int64_t>(p.tile_unit[tile + 1]) - p.tile_unit[tile];
+                const int64_t u0 = static_cast<int64_t>(p.tile_unit[tile]) * p.kh + kv * steps;
+                const int32_t c0 = tile_cta_of(units, ctas, u0);
+                const uint32_t count = steps ? tile_cta_of(units, ctas, u0 + steps - 1) - c0 + 1 : 0;
+                shared = PartList{p.tile_sum, p.tile_ml, 2ull * p.tile_grid + c0 + static_cast<uint64_t>(tile) * p.kh + kv, 1,
+                                  kTlPairs, listed % p.tile_rows * p.group + in_group, count};
+            }
+        }
+        float4 o;
+        float l, top;
+        join_parts<WPH>(shared, own, sub, o, l, top);
+        if constexpr (WPH > 1) {  // the warps' sums, in order
+            warp_sum_at[sub][lane] = o;
+            if (lane == 0) warp_l[sub] = l;
+            __syncthreads();
+            if (sub == 0) {
+#pragma unroll
+                for (int w = 1; w < WPH; ++w) {
+                    const float4 v = warp_sum_at[w][lane];
+                    o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+                    l += warp_l[w];
+                }
+                join_store<F32>(p, e.x, head, o, l, top);
+            }
+            __syncthreads();
+        } else {
+            join_store<F32>(p, e.x, head, o, l, top);
+        }
+    }
+    // Prompts' tiles that a CTA's end cuts: the first such end does the tile, 32 pairs to a block.
+    for (int64_t n = blockIdx.x; n < 8ll * (ctas - 1); n += gridDim.x) {
+        const int32_t c = static_cast<int32_t>(n / 8) + 1;
+        const int64_t cut = tile_cta_start(units, ctas, c);
+        const int32_t tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles),
+                                      static_cast<int32_t>(cut / p.kh));
+        if (tile < pre_tiles) continue;
+        const int64_t steps = static_cast<int64_t>(p.tile_unit[tile + 1]) - p.tile_unit[tile];
+        const int64_t head0 = static_cast<int64_t>(p.tile_unit[tile]) * p.kh;
+        const int64_t kv = (cut - head0) / steps, u0 = head0 + kv * steps;
+        if (cut == u0 || tile_cta_start(units, ctas, c - 1) > u0) continue;
+        const int32_t last = tile_cta_of(units, ctas, u0 + steps - 1);
+        // CTA c - 1 has this tile as its last run unless it begins with it; the others begin with it.
+        const bool begins = tile_cta_start(units, ctas, c - 1) == u0;
+        const int32_t row0 = tile_first_row(p, tile), rows = tile_row_count(p, tile);
+        for (uint32_t pair = static_cast<uint32_t>(n % 8) * 32 + warp; pair < static_cast<uint32_t>(n % 8) * 32 + 32; pair += 8) {
+            if (pair >= rows * p.group) break;
+            const PartList one{p.tile_sum, p.tile_ml, 2ull * (c - 1) + (begins ? 0 : 1), 0, kTlPairs, pair, 1};
+            const PartList more{p.tile_sum, p.tile_ml, 2ull * c, 2, kTlPairs, pair, static_cast<uint32_t>(last - c + 1)};
+            float4 o;
+            float l, top;
+            join_parts<1>(one, more, 0, o, l, top);
+            join_store<F32>(p, static_cast<uint64_t>(row0) + pair / p.group, static_cast<uint32_t>(kv) * p.group + pair % p.group, o, l, top);
+        }
+    }
+    // Rows that no request has, and tiles without a key.
+    const int32_t taken = p.requests ? max(p.starts[p.requests], 0) : 0;
+    const uint32_t width = p.qh * kPgDim / 4;
+    const auto clear = [&](uint64_t row) {
+        for (uint32_t x = threadIdx.x; x < width; x += blockDim.x) {
+            if constexpr (F32) pg_store4(static_cast<float *>(p.out) + row * p.out_stride + 4 * x, make_float4(0.f, 0.f, 0.f, 0.f));
+            else pg_store4(static_cast<uint16_t *>(p.out) + row * p.out_stride + 4 * x, make_float4(0.f, 0.f, 0.f, 0.f));
+        }
+    };
+    for (uint64_t row = static_cast<uint64_t>(taken) + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
+    for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); tile < tiles; tile += gridDim.x)
+        if (p.tile_unit[tile + 1] == p.tile_unit[tile])
+            for (int32_t i = 0; i < tile_row_count(p, tile); ++i) clear(static_cast<uint64_t>(tile_first_row(p, tile)) + i);
 }
 
 }  // namespace plamo
