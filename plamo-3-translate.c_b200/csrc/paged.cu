@@ -48,14 +48,15 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
         return "paged_attention: too many rows or requests";
     if (!d->pages || d->pages > static_cast<uint64_t>(kPgMaxPages) / 4)
         return "paged_attention: pages must be 1 to 2^23";
+    if (d->prefix_rows > INT32_MAX / 2 || d->table_stride > INT32_MAX / 2 / kPgRows)
+        return "paged_attention: the prefix and a request's page table hold at most 2^30 rows each";
     if (d->prefix_rows > d->pages * kPgRows) return "paged_attention: the prefix does not fit the pool";
-    if (d->table_stride > static_cast<uint64_t>(kPgMaxPages)) return "paged_attention: table_stride above 2^25";
     return nullptr;
 }
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
-    uint32_t row_tile, prefix_tiles, prefix_splits, own_groups, target, tile_rows, tile_cap;
+    uint32_t row_tile, prefix_tiles, prefix_splits, own_groups, workers, tile_rows, tile_cap;
     uint64_t record, own_sum, own_ml, prefix_sum, prefix_ml;
     uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
 };
@@ -77,12 +78,12 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
         const uint64_t want = ceil_div(2 * sms, static_cast<uint64_t>(a.prefix_tiles) * d->kv_heads);
         a.prefix_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(want, prefix_pages / kRtMinPages)));
     }
-    a.target = static_cast<uint32_t>(2 * sms);  // one item to a CTA
+    a.workers = static_cast<uint32_t>(2 * sms - 1);  // beside the schedule's CTA
     // Every request's last tile and last run of pages may be partial. Beside the
     // tile kernel only requests of up to kTlShortPairs pairs are here.
     const uint64_t own_tiles = pairs / a.row_tile + std::min<uint64_t>(d->requests, d->rows);
     a.own_groups = static_cast<uint32_t>(std::min<uint64_t>(
-        (a.tile_rows ? std::min<uint64_t>(own_tiles, kTlShortPairs / a.row_tile * d->requests) : own_tiles) + ceil_div(a.target, d->kv_heads),
+        (a.tile_rows ? std::min<uint64_t>(own_tiles, kTlShortPairs / a.row_tile * d->requests) : own_tiles) + ceil_div(a.workers, d->kv_heads),
         INT32_MAX / d->kv_heads));
     uint64_t at = 0;
     auto part = [&](uint64_t bytes) {
@@ -133,14 +134,19 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.out_stride = d->out_stride;
     p.table_stride = d->table_stride;
     p.status = d->status;
-    p.rows = static_cast<uint32_t>(d->rows);
-    p.requests = static_cast<uint32_t>(d->requests);
-    p.pages = static_cast<uint32_t>(d->pages);
-    p.qh = d->query_heads;
-    p.kh = d->kv_heads;
-    p.group = d->query_heads / d->kv_heads;
-    p.prefix = static_cast<int64_t>(d->prefix_rows);
-    p.window = static_cast<int64_t>(std::min<uint64_t>(d->window, 1ull << 40));
+    p.rows = static_cast<int32_t>(d->rows);
+    p.requests = static_cast<int32_t>(d->requests);
+    p.pages = static_cast<int32_t>(d->pages);
+    p.qh = static_cast<int32_t>(d->query_heads);
+    p.kh = static_cast<int32_t>(d->kv_heads);
+    p.group = p.qh / p.kh;
+    p.by_group = FastDiv::of(p.group);
+    p.by_kh = FastDiv::of(p.kh);
+    p.by_qh = FastDiv::of(p.qh);
+    p.prefix = static_cast<int32_t>(d->prefix_rows);
+    p.max_length = static_cast<int32_t>(d->table_stride * kPgRows);
+    // A window that reaches back past every row hides nothing.
+    p.window = d->window > d->prefix_rows + d->table_stride * kPgRows ? 0 : static_cast<int32_t>(d->window);
     p.scale2 = d->scale * 1.4426950408889634f;
     // The tile kernel masks before it scales: -inf must stay so.
     if (std::fabs(p.scale2) < 1e-30f) p.scale2 = std::copysign(1e-30f, p.scale2);
@@ -151,28 +157,27 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.own_ml = reinterpret_cast<float2 *>(ws + a.own_ml);
     p.prefix_sum = reinterpret_cast<float *>(ws + a.prefix_sum);
     p.prefix_ml = reinterpret_cast<float2 *>(ws + a.prefix_ml);
-    p.row_tile = a.row_tile;
-    p.own_groups = a.own_groups;
-    p.prefix_splits = a.prefix_splits;
-    p.prefix_tiles = a.prefix_tiles;
-    p.target = a.target;
+    p.row_tile = static_cast<int32_t>(a.row_tile);
+    p.row_shift = a.row_tile == 8 ? 3 : 4;
+    p.own_groups = static_cast<int32_t>(a.own_groups);
+    p.prefix_splits = static_cast<int32_t>(a.prefix_splits);
+    p.prefix_tiles = static_cast<int32_t>(a.prefix_tiles);
+    p.workers = static_cast<int32_t>(a.workers);
     if (a.tile_rows) {
         p.pool = d->pool;
-        p.tile_rows = a.tile_rows;
-        p.tile_grid = static_cast<uint32_t>(context_sms(c));
-        p.tile_cap = a.tile_cap;
+        p.tile_rows = static_cast<int32_t>(a.tile_rows);
+        p.by_tile_rows = FastDiv::of(a.tile_rows);
+        p.tile_grid = context_sms(c);
+        p.tile_cap = static_cast<int32_t>(a.tile_cap);
         p.tile_shape = reinterpret_cast<TileShape *>(ws + a.tile_shape);
         p.tile_unit = reinterpret_cast<uint32_t *>(ws + a.tile_unit);
         p.tile_sum = reinterpret_cast<float *>(ws + a.tile_sum);
         p.tile_ml = reinterpret_cast<float2 *>(ws + a.tile_ml);
     }
-    // The row kernel needs no schedule and hides its time; the tile kernel's CTAs
-    // follow as SMs come free.
     void (*rows)(const CUtensorMap, const PagedAttnParams) = paged_rows_kernel<F32, 1>;
     if constexpr (!F32)
         if (a.row_tile == 16) rows = paged_rows_kernel<F32, 2>;
-    if (!launch(c, "paged_attention schedule", paged_schedule_kernel, dim3(1), dim3(kScThreads), 0, stream, false, p) ||
-        !launch(c, "paged_attention rows", rows, dim3(2 * context_sms(c)), dim3(kRtThreads), kRtSmem, stream, true, map, p) ||
+    if (!launch(c, "paged_attention rows", rows, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
         (a.tile_rows && !launch(c, "paged_attention tiles", paged_tile_kernel, dim3(p.tile_grid), dim3(kTlThreads), kTlSmem,
                                 stream, true, page_map, p)))
         return false;

@@ -12,36 +12,59 @@
 
 namespace plamo {
 
+// x / d for x < 2^31 by a multiplication: the kernels run for microseconds, in
+// which the code of divisions would take longer to fetch than to execute.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    __host__ static FastDiv of(uint32_t d) {
+        FastDiv f{d, 0, 0};
+        if (d > 1) {
+            uint32_t bits = 0;
+            while ((1ull << bits) < d) ++bits;
+            f.shift = bits - 1;
+            f.mul = static_cast<uint32_t>(((1ull << (31 + bits)) + d - 1) / d);
+        }
+        return f;
+    }
+    __device__ __forceinline__ int32_t div(int32_t x) const {
+        return d == 1 ? x : static_cast<int32_t>(__umulhi(static_cast<uint32_t>(x), mul) >> shift);
+    }
+};
+
+// All counts, rows and positions are below 2^31 (checked by the host).
 struct PagedAttnParams {
     const void *q;
     void *out;
     const int32_t *starts, *lengths, *tables, *prefix_pages;
     uint64_t q_stride, out_stride, table_stride;
     uint32_t *status;
-    uint32_t rows, requests, pages, qh, kh, group;
-    int64_t prefix, window;  // window: rows seen, 0 for all
+    int32_t rows, requests, pages, qh, kh, group;
+    FastDiv by_group, by_kh, by_qh;
+    int32_t prefix, window;  // window: rows seen, 0 for all
+    int32_t max_length;      // own rows a page table holds
     float scale2;            // scale * log2(e)
-    uint32_t row_tile;       // pairs to a tile of the row kernel
-    // Partial results, unnormalised: [slot][row_tile][128] sums and [slot][row_tile] {m, l}.
+    int32_t row_tile, row_shift;  // pairs to a tile of the row kernel: 1 << row_shift
+    // Its partial results, unnormalised: [slot][row_tile][128] sums and [slot][row_tile] {m, l}.
     int4 *own_record;  // [requests] {first own slot / kv heads, splits, row tiles}
     float *own_sum, *prefix_sum;
     float2 *own_ml, *prefix_ml;
-    uint32_t own_groups;  // capacity of the own partials, in slots per KV head
-    uint32_t prefix_splits, prefix_tiles;
-    uint32_t target;  // own items wanted in all
+    int32_t own_groups;  // capacity of the own partials, in slots per KV head
+    int32_t prefix_splits, prefix_tiles;
+    int32_t workers;     // CTAs of the row kernel that take items
     // The schedule (paged_tiles.cuh).
     int32_t *header;   // [kTlHeader]
     int4 *short_list;  // [rows] {batch row, own row, request, row of it} of the short requests' rows
     // The tile kernel's share; tile_rows 0: it has none.
     const void *pool;
-    uint32_t tile_rows;  // batch rows to a tile
-    uint32_t tile_grid, tile_cap;
+    int32_t tile_rows;  // batch rows to a tile
+    FastDiv by_tile_rows;
+    int32_t tile_grid, tile_cap;
     struct TileShape *tile_shape;  // [tile_cap]
     uint32_t *tile_unit;           // [tile_cap + 1] key steps before each tile
     float *tile_sum;               // [slot][256][128], [slot][256] {m, l}
     float2 *tile_ml;
 };
-enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlHeader = 8 };
+enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlHeader = 8 };
 constexpr int kTlPairs = 256;     // (row, head) pairs to a tile
 constexpr int kTlShortPairs = 32; // requests of up to so many keep their own rows in the row kernel
 constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
@@ -67,33 +90,29 @@ constexpr int kRtSmem = 1024 + kRtRing + 16 * kPgDim * 4;
 // A request's new rows and visible own keys.
 struct OwnShape {
     int32_t row0, rows;  // batch rows
-    int64_t at0;         // own row of the first one (negative: not held)
+    int32_t at0;         // own row of the first one (negative: not held)
     int32_t length;      // own rows held
     int32_t page0, pages;
     int32_t tiles;
 };
-__device__ __forceinline__ OwnShape own_shape(const PagedAttnParams &p, int64_t r) {
+__device__ __forceinline__ OwnShape own_shape(const PagedAttnParams &p, int32_t r) {
     OwnShape s;
-    const int64_t lo = min(max(p.starts[r], 0), static_cast<int32_t>(p.rows));
-    const int64_t hi = min(max(p.starts[r + 1], 0), static_cast<int32_t>(p.rows));
-    s.row0 = static_cast<int32_t>(lo);
-    s.rows = static_cast<int32_t>(max(hi - lo, static_cast<int64_t>(0)));
-    const int64_t most = min(static_cast<int64_t>(p.table_stride) * kPgRows, static_cast<int64_t>(INT32_MAX));
-    s.length = static_cast<int32_t>(min(max(static_cast<int64_t>(p.lengths[r]), static_cast<int64_t>(0)), most));
-    s.at0 = static_cast<int64_t>(s.length) - s.rows;
-    const int64_t first = p.window ? max(s.at0 - p.window + 1, static_cast<int64_t>(0)) : 0;
-    s.page0 = static_cast<int32_t>(first / kPgRows);
+    s.row0 = min(max(p.starts[r], 0), p.rows);
+    s.rows = min(max(p.starts[r + 1], s.row0), p.rows) - s.row0;
+    s.length = min(max(p.lengths[r], 0), p.max_length);
+    s.at0 = s.length - s.rows;
+    const int32_t first = p.window ? max(max(s.at0, 0) - p.window + 1, 0) : 0;
+    s.page0 = first / kPgRows;
     s.pages = s.rows ? max((s.length + kPgRows - 1) / kPgRows - s.page0, 0) : 0;
-    s.tiles = static_cast<int32_t>((static_cast<int64_t>(s.rows) * p.group + p.row_tile - 1) / p.row_tile);
+    s.tiles = (s.rows * p.group + p.row_tile - 1) >> p.row_shift;
     return s;
 }
-
-// Short requests' own rows go through the row kernel, 16 pairs at a time; the
-// others are the tile kernel's, where there is one.
+// Short requests' own rows go through the row kernel, 8 or 16 pairs at a time;
+// the others are the tile kernel's, where there is one.
 __device__ __forceinline__ bool request_is_short(const PagedAttnParams &p, const OwnShape &s) {
-    return !p.tile_rows || static_cast<int64_t>(s.rows) * p.group <= kTlShortPairs;
+    return !p.tile_rows || s.rows * p.group <= kTlShortPairs;
 }
-__device__ __forceinline__ OwnShape short_shape(const PagedAttnParams &p, int64_t r) {
+__device__ __forceinline__ OwnShape short_shape(const PagedAttnParams &p, int32_t r) {
     OwnShape s = own_shape(p, r);
     if (!request_is_short(p, s)) s.tiles = s.pages = 0;
     return s;
@@ -110,14 +129,18 @@ struct __align__(16) TileShape {
     int32_t unused[3];
     __device__ int32_t steps() const { return pre1 - pre0 + own1 - own0; }
 };
-__device__ __forceinline__ int32_t tile_first_row(const PagedAttnParams &p, int32_t tile) { return p.tile_shape[tile].row0; }
-__device__ __forceinline__ int32_t tile_row_count(const PagedAttnParams &p, int32_t tile) { return p.tile_shape[tile].rows; }
 
-// The tile kernel's CTAs take equal runs of all units.
-__device__ __forceinline__ int64_t tile_cta_start(int64_t units, int32_t ctas, int32_t c) { return units * c / ctas; }
-__device__ __forceinline__ int32_t tile_cta_of(int64_t units, int32_t ctas, int64_t unit) {
-    return static_cast<int32_t>(((unit + 1) * ctas - 1) / units);
-}
+// The tile kernel's CTAs take equal runs of all units (key steps of a tile and
+// KV head): the first `longer` of them run + 1, the others run.
+struct TileRuns {
+    int32_t run, longer;
+    __device__ __forceinline__ int32_t start(int32_t cta) const { return cta * run + min(cta, longer); }
+    __device__ __forceinline__ int32_t cta_of(int32_t unit) const {
+        const int32_t cut = longer * (run + 1);
+        return unit < cut ? unit / (run + 1) : longer + (unit - cut) / run;
+    }
+};
+__device__ __forceinline__ TileRuns tile_runs(const PagedAttnParams &p) { return TileRuns{p.header[kTlRun], p.header[kTlLonger]}; }
 
 struct RowItem {
     int32_t request;  // -1: prefix
@@ -125,14 +148,14 @@ struct RowItem {
     int32_t page0, pages;  // of the request's table or the prefix's
     int32_t limit;         // keys from here on hold nothing
     int32_t row0, rows;    // batch rows of the tile's source
-    int64_t at0;
-    uint32_t slot;
+    int32_t at0;
+    int32_t slot;
     int32_t direct;  // the only part of its rows: normalise and write the result
 };
 
 // 32-way search for the last request whose first row is at or before `row`
 // (the one that holds it, since starts never decrease); whole warp.
-__device__ __forceinline__ int32_t pg_owner(const int32_t *starts, uint32_t requests, int32_t row) {
+__device__ __noinline__ int32_t pg_owner(const int32_t *starts, uint32_t requests, int32_t row) {
     const uint32_t lane = threadIdx.x & 31;
     uint32_t lo = 0, n = requests;  // the answer is in [lo, lo + n)
     while (n > 1) {
@@ -206,43 +229,42 @@ struct RowCta {
 };
 
 // The keys that a pair of an item sees, [lo, hi); lo -1 where there is no such pair.
-__device__ __forceinline__ int2 rt_sees(const PagedAttnParams &p, const RowItem &it, int64_t pair) {
-    if (pair >= static_cast<int64_t>(it.rows) * p.group) return make_int2(-1, 0);
-    const int32_t i = static_cast<int32_t>(pair / p.group);
+__device__ __noinline__ int2 rt_sees(const PagedAttnParams &p, const RowItem &it, int32_t pair) {
+    if (pair >= it.rows * p.group) return make_int2(-1, 0);
+    const int32_t i = p.by_group.div(pair);
     if (it.request >= 0) {
-        const int64_t at = it.at0 + i;
-        const int64_t lo = p.window ? max(at - p.window + 1, static_cast<int64_t>(0)) : 0;
-        return make_int2(static_cast<int32_t>(lo), static_cast<int32_t>(max(at + 1, static_cast<int64_t>(0))));
+        const int32_t at = it.at0 + i;
+        return make_int2(p.window ? max(max(at, 0) - p.window + 1, 0) : 0, max(at + 1, 0));
     }
-    int64_t lo = 0;
+    int32_t lo = 0;
     if (p.window && p.requests) {  // its request's length decides: the last one to start at or before row i
-        uint32_t r = 0, n = p.requests;
+        int32_t r = 0, n = p.requests;
         while (n > 1) {
-            const uint32_t half = n / 2;
+            const int32_t half = n / 2;
             const bool below = p.starts[r + half] <= i;
             r = below ? r + half : r;
             n = below ? n - half : half;
         }
         const OwnShape s = own_shape(p, r);
-        lo = min(max(p.prefix + s.at0 + i - s.row0 - p.window + 1, static_cast<int64_t>(0)), p.prefix);
+        lo = min(max(p.prefix + max(s.at0 + i - s.row0, 0) - p.window + 1, 0), p.prefix);
     }
-    return make_int2(static_cast<int32_t>(lo), static_cast<int32_t>(p.prefix));
+    return make_int2(lo, p.prefix);
 }
 // Where a pair's query starts (in elements), or -1.
-__device__ __forceinline__ int64_t rt_query(const PagedAttnParams &p, const RowItem &it, int64_t pair) {
-    if (pair >= static_cast<int64_t>(it.rows) * p.group) return -1;
-    const uint64_t row = static_cast<uint64_t>(it.row0) + pair / p.group;
-    return static_cast<int64_t>(row * p.q_stride + (static_cast<uint64_t>(it.head) * p.group + pair % p.group) * kPgDim);
+__device__ __forceinline__ int64_t rt_query(const PagedAttnParams &p, const RowItem &it, int32_t pair) {
+    if (pair >= it.rows * p.group) return -1;
+    const int32_t i = p.by_group.div(pair);
+    return static_cast<int64_t>(it.row0 + i) * static_cast<int64_t>(p.q_stride) + (it.head * p.group + pair - i * p.group) * kPgDim;
 }
 
 template <int NT>
-__device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const RowItem &it, const RowCta<8 * NT> &cta, int64_t begin,
-                                             int64_t end, int32_t slabs, uint32_t ring, bool &dead) {
+__device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const RowItem &it, const RowCta<8 * NT> &cta, int32_t begin,
+                                             int32_t end, int32_t slabs, uint32_t ring, bool &dead) {
     constexpr int PAIRS = 8 * NT, SLAB = rt_slab_bytes<false>(), SLABS = kRtRing / SLAB;
     constexpr int GROUPS = 16 / PAIRS;  // of warps whose sums are joined side by side
     constexpr bool QSM = NT > 1;        // queries read from shared memory at each use, to save registers
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int64_t pair0 = static_cast<int64_t>(it.tile) * PAIRS;
+    const int32_t pair0 = it.tile * PAIRS;
     // This thread's pairs, 8 nt + 2 t + c: which keys they see.
     int32_t see_lo[NT][2], see_hi[NT][2];
 #pragma unroll
@@ -289,7 +311,7 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
         if (!mbar_wait(&cta.full[st], (q / SLABS) & 1u)) dead = true;
         dead = __any_sync(0xffffffffu, dead);
         if (dead) break;
-        const int32_t key0 = static_cast<int32_t>(begin) + n * kRtKeys;
+        const int32_t key0 = begin + n * kRtKeys;
         const uint32_t kbase = smem_u32(cta.slabs + st * SLAB), vbase = kbase + SLAB / 2;
         // ---- scores: key g (x = 0, 1) and g + 8 (2, 3) of pairs 2 t, 2 t + 1
         float s[NT][4], c1[NT][4];
@@ -313,7 +335,7 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
             }
         }
         // ---- masks; a key that exists and that some pair does not see?
-        const int32_t left = static_cast<int32_t>(min(end - key0, static_cast<int64_t>(kRtKeys)));
+        const int32_t left = min(end - key0, kRtKeys);
         bool hidden = false, move = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -464,10 +486,10 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
 // the lane's own number (key ^ l / 8, pair ^ l % 8) it is always the same half
 // of the registers, and nothing is selected.
 __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowItem &it, const RowCta<8> &cta, float *weights,
-                                            int64_t begin, int64_t end, int32_t slabs, uint32_t ring, bool &dead) {
+                                            int32_t begin, int32_t end, int32_t slabs, uint32_t ring, bool &dead) {
     constexpr int SLAB = rt_slab_bytes<true>(), SLABS = kRtRing / SLAB;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t pair0 = static_cast<int64_t>(it.tile) * 8;
+    const int32_t pair0 = it.tile * 8;
     const int2 sees = rt_sees(p, it, pair0 + (lane & 7));
     float4 q[8], o[8];
 #pragma unroll
@@ -483,14 +505,14 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
         if (!mbar_wait(&cta.full[st], (x / SLABS) & 1u)) dead = true;
         dead = __any_sync(0xffffffffu, dead);
         if (dead) break;
-        const int32_t key0 = static_cast<int32_t>(begin) + n * kRtKeys;
+        const int32_t key0 = begin + n * kRtKeys;
         const unsigned char *keys = cta.slabs + st * SLAB + box, *values = keys + SLAB / 2;
         const auto piece = [&](const unsigned char *base, int row) {
             return *reinterpret_cast<const float4 *>(base + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
         };
         float s[4];
-#pragma unroll
-        for (int four = 0; four < 4; ++four) {
+#pragma unroll 1
+        for (int four = 0; four < 4; ++four) {  // (rolled: the kernel's code is mostly run once)
             float v[4][8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -510,9 +532,11 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
             for (int i = 0; i < 4; ++i) v[0][i] += __shfl_xor_sync(0xffffffffu, v[0][i + 4], 4);
             v[0][0] += __shfl_xor_sync(0xffffffffu, v[0][2], 2);
             v[0][1] += __shfl_xor_sync(0xffffffffu, v[0][3], 2);
-            s[four] = v[0][0] + __shfl_xor_sync(0xffffffffu, v[0][1], 1);
+            weights[32 * four + lane] = v[0][0] + __shfl_xor_sync(0xffffffffu, v[0][1], 1);
         }
-        const int32_t left = static_cast<int32_t>(min(end - key0, static_cast<int64_t>(kRtKeys)));
+#pragma unroll
+        for (int four = 0; four < 4; ++four) s[four] = weights[32 * four + lane];  // this lane's own
+        const int32_t left = min(end - key0, kRtKeys);
         bool hidden = false, move = false;
         uint32_t seen_by[4];  // bit 8 * key + pair of four keys
 #pragma unroll
@@ -550,8 +574,7 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
 #pragma unroll 1
             for (int key = 0; key < left; ++key) {
                 const float4 v = piece(values, key);
-                const uint32_t by = seen_by[0] * (key < 4) | seen_by[1] * (key >= 4 && key < 8) |
-                                    seen_by[2] * (key >= 8 && key < 12) | seen_by[3] * (key >= 12);
+                const uint32_t by = key < 8 ? (key < 4 ? seen_by[0] : seen_by[1]) : (key < 12 ? seen_by[2] : seen_by[3]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float w = weights[8 * key + i];
@@ -560,7 +583,7 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
                 }
             }
         } else {
-#pragma unroll
+#pragma unroll 4
             for (int key = 0; key < kRtKeys; ++key) {
                 const float4 v = piece(values, key);
                 const float4 a = ld4(weights + 8 * key), b = ld4(weights + 8 * key + 4);
@@ -615,13 +638,18 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
 // half of what the slab's 16 KB take to arrive, and lose nothing to splitting.
 // (Measured before: TF32 mma.sync with two terms to an operand, 5 us per slab
 // and warp against 0.7 us for BF16.)
+__device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums);  // paged_tiles.cuh
+
+constexpr int kRtChunks = 6;  // item sizes weighed, in pages: the least * 4/4, 5/4, 6/4, 2, 3, 4
+__device__ __forceinline__ int32_t rt_chunk_pages(int32_t least, int x) { return x < 3 ? (least * (4 + x) + 3) / 4 : least * (x - 1); }
+
 template <bool F32, int NT>
 __global__ void __launch_bounds__(kRtThreads, 2)
-    paged_rows_kernel(const __grid_constant__ CUtensorMap map, const PagedAttnParams p) {
+    paged_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
+    static_assert(!F32 || NT == 1, "FP32: eight pairs");
     constexpr int PAIRS = 8 * NT, SLAB = rt_slab_bytes<F32>(), SLABS = kRtRing / SLAB;
     static_assert(SLABS % kRtWarps == 0, "a place of the ring serves one warp");
     constexpr int GROUPS = 16 / PAIRS;  // of warps whose sums are joined side by side
-    static_assert(!F32 || NT == 1, "FP32: eight pairs");
     constexpr int PER = kPgRows / kRtKeys;  // slabs per page
     extern __shared__ __align__(128) unsigned char rt_raw[];
     __shared__ __align__(8) uint64_t full[SLABS], empty[SLABS];
@@ -629,11 +657,17 @@ __global__ void __launch_bounds__(kRtThreads, 2)
     __shared__ RowItem items[kRtBatch];
     __shared__ float2 warp_ml[kRtWarps][PAIRS];
     __shared__ __align__(16) float weights[F32 ? kRtWarps : 1][F32 ? kRtKeys * 8 : 4];
-    __shared__ int64_t shared_min;
+    __shared__ int32_t item_counts[kRtChunks], lowest_at;
     unsigned char *base = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(rt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float *joined = reinterpret_cast<float *>(base + kRtRing);  // [GROUPS][PAIRS][128]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_launch_dependents();
+    if (blockIdx.x == 0) {  // for the kernels that follow, while the others work
+        paged_schedule(p, scan);
+        return;
+    }
+    const int32_t worker = static_cast<int32_t>(blockIdx.x) - 1;
     const RowCta<PAIRS> cta{full, empty, base, joined, warp_ml};
     if (tid == 0) {
         for (int s = 0; s < SLABS; ++s) {
@@ -642,129 +676,152 @@ __global__ void __launch_bounds__(kRtThreads, 2)
         }
         fence_barrier_init();
         prefetch_tensormap(&map);
+        lowest_at = INT32_MAX;
     }
-    pdl_launch_dependents();
+    if (tid < kRtChunks) item_counts[tid] = 0;
 
     // Every CTA lays the items out by itself from the requests' lengths.
-    const int64_t R = p.requests, per = (R + kRtThreads - 1) / kRtThreads;
-    const int64_t r0 = min(R, tid * per), r1 = min(R, r0 + per);
-    int64_t units = 0, lowest = INT64_MAX;
-    for (int64_t r = r0; r < r1; ++r) {
+    const int32_t per = (p.requests + kRtThreads - 1) / kRtThreads;
+    const int32_t r0 = min(p.requests, tid * per), r1 = min(p.requests, r0 + per);
+    int64_t units = 0, total_units;
+    int32_t lowest = INT32_MAX;
+    for (int32_t r = r0; r < r1; ++r) {
         const OwnShape s = short_shape(p, r);
         units += static_cast<int64_t>(s.tiles) * s.pages;
-        if (s.rows) lowest = min(lowest, s.at0);
+        if (s.rows) lowest = min(lowest, max(s.at0, 0));
     }
-    int64_t total_units, total;
     pg_block_scan<kRtThreads>(units, scan, &total_units);
-    if (tid == 0) shared_min = INT64_MAX;
-    __syncthreads();
-    if (p.window && lowest != INT64_MAX) atomicMin(reinterpret_cast<long long *>(&shared_min), static_cast<long long>(lowest));
-    const int64_t chunk = max(static_cast<int64_t>(kRtMinPages),
-                              (total_units * p.kh + p.target - 1) / p.target);
-    int64_t mine = 0;
-    for (int64_t r = r0; r < r1; ++r) {
+    // Pages to an item: whole rounds of items over the CTAs, each costing its
+    // pages and about four more to begin and end.
+    const int32_t least = max(kRtMinPages, static_cast<int32_t>(fminf(1e8f, ceilf(1.0001f * static_cast<float>(total_units) * p.kh / p.workers))));
+    int32_t counts[kRtChunks];
+#pragma unroll
+    for (int x = 0; x < kRtChunks; ++x) counts[x] = 0;
+#pragma unroll 1
+    for (int32_t r = r0; r < r1; ++r) {
         const OwnShape s = short_shape(p, r);
-        mine += s.tiles * ((s.pages + chunk - 1) / chunk);
+#pragma unroll
+        for (int x = 0; x < kRtChunks; ++x) {
+            const int32_t c = rt_chunk_pages(least, x);
+            counts[x] += s.tiles * ((s.pages + c - 1) / c);
+        }
     }
-    const int64_t first = pg_block_scan<kRtThreads>(mine, scan, &total);
-    if (total > p.own_groups) {
-        if (tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
-        total = p.own_groups;
+#pragma unroll
+    for (int x = 0; x < kRtChunks; ++x) {
+        const int32_t sum = __reduce_add_sync(0xffffffffu, counts[x]);
+        if (lane == 0 && sum) atomicAdd(&item_counts[x], sum);
     }
-    if (blockIdx.x == 0) {
-        int64_t at = first;
-        for (int64_t r = r0; r < r1; ++r) {
+    if (p.window) {
+        lowest = __reduce_min_sync(0xffffffffu, lowest);
+        if (lane == 0) atomicMin(&lowest_at, lowest);
+    }
+    __syncthreads();
+    int32_t chunk = least, mine = counts[0];
+    float cost = INFINITY;
+#pragma unroll
+    for (int x = 0; x < kRtChunks; ++x) {
+        const int32_t c = rt_chunk_pages(least, x);
+        const float y = ceilf(static_cast<float>(item_counts[x]) * p.kh / p.workers) * (c + 4);
+        if (y < cost) {
+            cost = y;
+            chunk = c;
+            mine = counts[x];
+        }
+    }
+    int64_t all;
+    const int32_t first = static_cast<int32_t>(pg_block_scan<kRtThreads>(mine, scan, &all));
+    const int32_t total = static_cast<int32_t>(min(all, static_cast<int64_t>(p.own_groups)));
+    if (all > total && tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
+    if (worker == 0) {
+        int32_t at = first;
+#pragma unroll 1
+        for (int32_t r = r0; r < r1; ++r) {
             const OwnShape s = short_shape(p, r);
-            const int64_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
-            p.own_record[r] = at + n <= total ? make_int4(static_cast<int>(at), static_cast<int>(splits), s.tiles, 0) : make_int4(0, 0, 0, 0);
+            const int32_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
+            p.own_record[r] = at + n <= total ? make_int4(at, splits, s.tiles, 0) : make_int4(0, 0, 0, 0);
             at += n;
         }
     }
     // Prefix pages that some row still sees.
-    const int32_t prefix_pages = static_cast<int32_t>((p.prefix + kPgRows - 1) / kPgRows);
+    const int32_t prefix_pages = (p.prefix + kPgRows - 1) / kPgRows;
     int32_t pp0 = 0;
-    if (p.window && shared_min != INT64_MAX)
-        pp0 = static_cast<int32_t>(min(max(p.prefix + shared_min - p.window + 1, static_cast<int64_t>(0)), p.prefix) / kPgRows);
-    const int32_t pchunk = p.prefix_splits ? (prefix_pages - pp0 + p.prefix_splits - 1) / static_cast<int32_t>(p.prefix_splits) : 0;
-    const int64_t own_items = total * p.kh;
-    const int64_t all_items = own_items + static_cast<int64_t>(p.prefix_splits) * p.prefix_tiles * p.kh;
+    if (p.window && lowest_at != INT32_MAX) pp0 = min(max(p.prefix + lowest_at - p.window + 1, 0), p.prefix) / kPgRows;
+    const int32_t pchunk = p.prefix_splits ? (prefix_pages - pp0 + p.prefix_splits - 1) / p.prefix_splits : 0;
+    const int32_t own_items = total * p.kh, all_items = own_items + p.prefix_splits * p.prefix_tiles * p.kh;
 
     uint32_t ring = 0, issued = 0;  // slabs of the items before; copied ones
     bool dead = false;
-    for (int64_t batch = blockIdx.x; batch < all_items; batch += static_cast<int64_t>(gridDim.x) * kRtBatch) {
+    for (int32_t batch = worker; batch < all_items; batch += p.workers * kRtBatch) {
         __syncthreads();  // the last batch's items are done with
+        {
+            // The thread that lays out a request fills in those of its items that this CTA takes.
+            int32_t at = first;
 #pragma unroll 1
-        for (int k = 0; k < kRtBatch; ++k) {
-            const int64_t id = batch + static_cast<int64_t>(k) * gridDim.x;
-            if (id >= all_items) break;
-            if (id >= own_items) {
-                if (tid == 0) {
-                    const int64_t x = id - own_items, y = x / p.kh;
-                    RowItem it;
-                    it.request = -1;
-                    it.head = static_cast<int32_t>(x % p.kh);
-                    it.tile = static_cast<int32_t>(y % p.prefix_tiles);
-                    const int32_t split = static_cast<int32_t>(y / p.prefix_tiles);
-                    it.page0 = min(pp0 + split * pchunk, prefix_pages);
-                    it.pages = min(pchunk, prefix_pages - it.page0);
-                    it.limit = static_cast<int32_t>(p.prefix);
-                    it.row0 = 0;
-                    it.rows = static_cast<int32_t>(p.rows);
-                    it.at0 = 0;
-                    it.slot = static_cast<uint32_t>(x);
-                    it.direct = 0;
-                    items[k] = it;
-                }
-                continue;
-            }
-            const int64_t group = id / p.kh;
-            if (group >= first && group < first + mine) {
-                int64_t at = first;
-                for (int64_t r = r0; r < r1; ++r) {
-                    const OwnShape s = short_shape(p, r);
-                    const int64_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
-                    if (group < at + n) {
+            for (int32_t r = r0; r < r1; ++r) {
+                const OwnShape s = short_shape(p, r);
+                const int32_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
+                if (n)
+#pragma unroll 1
+                    for (int k = 0; k < kRtBatch; ++k) {
+                        const int32_t id = batch + k * p.workers, group = p.by_kh.div(id);
+                        if (id >= own_items || group < at || group >= at + n) continue;
+                        const int32_t split = (group - at) / s.tiles, even = (s.pages + splits - 1) / splits;
                         RowItem it;
-                        const int64_t y = group - at;
-                        const int32_t split = static_cast<int32_t>(y / s.tiles);
-                        it.request = static_cast<int32_t>(r);
-                        it.tile = static_cast<int32_t>(y % s.tiles);
-                        it.head = static_cast<int32_t>(id % p.kh);
-                        it.page0 = s.page0 + static_cast<int32_t>(split * chunk);
-                        it.pages = static_cast<int32_t>(min(chunk, s.page0 + static_cast<int64_t>(s.pages) - it.page0));
+                        it.request = r;
+                        it.tile = group - at - split * s.tiles;
+                        it.head = id - group * p.kh;
+                        it.page0 = s.page0 + min(split * even, s.pages);
+                        it.pages = min(even, s.page0 + s.pages - it.page0);
                         // Keys past the tile's last row are seen by none of its rows.
-                        const int64_t last = s.at0 + min(static_cast<int64_t>(s.rows) - 1, (static_cast<int64_t>(it.tile) * PAIRS + PAIRS - 1) / p.group);
-                        it.limit = static_cast<int32_t>(min(max(last + 1, static_cast<int64_t>(0)), static_cast<int64_t>(s.length)));
+                        const int32_t last = s.at0 + min(s.rows - 1, p.by_group.div(it.tile * PAIRS + PAIRS - 1));
+                        it.limit = min(max(last + 1, 0), s.length);
                         it.row0 = s.row0;
                         it.rows = s.rows;
                         it.at0 = s.at0;
-                        it.slot = static_cast<uint32_t>(id);
+                        it.slot = id;
                         it.direct = splits == 1 && p.prefix == 0;
                         items[k] = it;
-                        break;
                     }
-                    at += n;
+                at += n;
+            }
+            if (tid < kRtBatch) {
+                const int32_t id = batch + tid * p.workers;
+                if (id >= own_items && id < all_items) {
+                    const int32_t x = id - own_items, y = p.by_kh.div(x), split = y / p.prefix_tiles;
+                    RowItem it;
+                    it.request = -1;
+                    it.head = x - y * p.kh;
+                    it.tile = y - split * p.prefix_tiles;
+                    it.page0 = min(pp0 + split * pchunk, prefix_pages);
+                    it.pages = min(pchunk, prefix_pages - it.page0);
+                    it.limit = p.prefix;
+                    it.row0 = 0;
+                    it.rows = p.rows;
+                    it.at0 = 0;
+                    it.slot = x;
+                    it.direct = 0;
+                    items[tid] = it;
                 }
             }
         }
         __syncthreads();
 #pragma unroll 1
         for (int k = 0; k < kRtBatch; ++k) {
-            if (batch + static_cast<int64_t>(k) * gridDim.x >= all_items) break;
+            if (batch + k * p.workers >= all_items) break;
             const RowItem it = items[k];
-            const int64_t begin = static_cast<int64_t>(it.page0) * kPgRows;
-            const int64_t end = min(begin + static_cast<int64_t>(it.pages) * kPgRows, static_cast<int64_t>(it.limit));
-            const int32_t slabs = end > begin ? static_cast<int32_t>((end - begin + kRtKeys - 1) / kRtKeys) : 0;
+            const int32_t begin = it.page0 * kPgRows, end = min(begin + it.pages * kPgRows, it.limit);
+            const int32_t slabs = end > begin ? (end - begin + kRtKeys - 1) / kRtKeys : 0;
             if (warp == kRtWarps) {
                 // ---- the copying warp: page ids 32 at a time, one lane issues.
                 const int32_t *table = it.request < 0 ? p.prefix_pages
                                                       : p.tables + static_cast<uint64_t>(it.request) * p.table_stride;
                 for (int32_t n0 = 0; n0 < slabs && !dead; n0 += 32 * PER) {
                     int32_t id = n0 / PER + lane < it.pages ? table[it.page0 + n0 / PER + lane] : 0;
-                    if (n0 / PER + lane < it.pages && (id < 0 || id >= static_cast<int32_t>(p.pages))) {
+                    if (n0 / PER + lane < it.pages && (id < 0 || id >= p.pages)) {
                         pg_flag(p.status, PLAMO_PAGED_PAGE);
-                        id = static_cast<int32_t>(p.pages);  // past the pool: the copy brings zeros
+                        id = p.pages;  // past the pool: the copy brings zeros
                     }
+#pragma unroll 1
                     for (int32_t n = n0; n < min(slabs, n0 + 32 * PER); ++n) {
                         const int32_t page = __shfl_sync(0xffffffffu, id, (n / PER) & 31);
                         if (lane == 0 && !dead) {
@@ -791,11 +848,11 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                 continue;
             }
             // ---- the computing warps
-            const int64_t pair0 = static_cast<int64_t>(it.tile) * PAIRS, pairs = static_cast<int64_t>(it.rows) * p.group;
             if constexpr (F32) rt_item_f32(p, it, cta, weights[warp], begin, end, slabs, ring, dead);
             else rt_item_bf16<NT>(p, it, cta, begin, end, slabs, ring, dead);
             ring += slabs;
             // ---- result, or the tile's partial sums
+#pragma unroll 1
             for (int x = tid; x < PAIRS * kPgDim / 4; x += 32 * kRtWarps) {
                 const int pair = x / (kPgDim / 4), d = 4 * (x % (kPgDim / 4));
                 float top = -INFINITY, l = 0.0f;
@@ -812,12 +869,12 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                     v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
                 }
                 if (it.direct) {
-                    const int64_t m = pair0 + pair;
-                    if (m >= pairs) continue;
+                    const int32_t m = it.tile * PAIRS + pair;
+                    if (m >= it.rows * p.group) continue;
                     const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
                     v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                    const uint64_t row = static_cast<uint64_t>(it.row0) + m / p.group;
-                    const uint64_t at = row * p.out_stride + (static_cast<uint64_t>(it.head) * p.group + m % p.group) * kPgDim + d;
+                    const int32_t i = p.by_group.div(m);
+                    const uint64_t at = (it.row0 + i) * p.out_stride + (it.head * p.group + m - i * p.group) * kPgDim + d;
                     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + at, v);
                     else pg_store4(static_cast<uint16_t *>(p.out) + at, v);
                 } else {
@@ -835,66 +892,66 @@ __global__ void __launch_bounds__(kRtThreads, 2)
             if (!mbar_wait(&full[n % SLABS], (n / SLABS) & 1u)) break;
     }
     if (dead && lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
-    pdl_wait();  // done only when the schedule is: the kernels after it wait for this one alone
 }
 
 // ---- joining the parts ----------------------------------------------------------------
-// One result (a row and head): parts [0, n0) at (first + x * stride) * rows +
-// place of one array, the rest in another; the sums joined in that order.
+// One result (a row and head): its parts lie in two arrays, the sums of part x
+// at (first + x * stride) * rows + place, joined in that order.
 struct PartList {
     const float *sum;
     const float2 *ml;
-    uint64_t first, stride;
-    uint32_t rows, place, count;
-    __device__ uint64_t at(uint32_t x) const { return (first + x * stride) * rows + place; }
+    int32_t first, stride, rows, place, count;
+    __device__ __forceinline__ int64_t at(int32_t x) const { return static_cast<int64_t>(first + x * stride) * rows + place; }
 };
 // WPH warps work on it, `sub` is this one; every lane returns with the sums
-// over its share of parts, 32 at a time to a warp, and the common maximum.
+// over its warp's share of parts, 32 at a time, and the common maximum.
 template <int WPH>
-__device__ __forceinline__ void join_parts(const PartList &a, const PartList &b, uint32_t sub, float4 &o, float &l, float &top) {
-    const uint32_t lane = threadIdx.x & 31, all = a.count + b.count;
+__device__ __noinline__ void join_parts(const PartList &a, const PartList &b, int32_t sub, float4 &o, float &l, float &top) {
+    const int32_t lane = threadIdx.x & 31, all = a.count + b.count;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
     top = -INFINITY;
     l = 0.0f;
-    const auto ml = [&](uint32_t x) { return x < a.count ? a.ml[a.at(x)] : b.ml[b.at(x - a.count)]; };
-    for (uint32_t x = lane; x < all; x += 32) top = fmaxf(top, ml(x).x);
+    const auto place = [&](int32_t x) { return x < a.count ? a.at(x) : b.at(x - a.count); };
+    for (int32_t x = lane; x < all; x += 32) top = fmaxf(top, (x < a.count ? a.ml : b.ml)[place(x)].x);
     top = warp_max(top);
     if (top == -INFINITY) return;
-    for (uint32_t x0 = 32 * sub; x0 < all; x0 += 32 * WPH) {
+#pragma unroll 1
+    for (int32_t x0 = 32 * sub; x0 < all; x0 += 32 * WPH) {
         // A lane weighs one part, then the parts' sums are loaded eight at once.
-        const uint32_t x = x0 + lane;
+        const int32_t x = x0 + lane;
         float w = 0.0f, part_l = 0.0f;
-        uint64_t here = 0;
+        const float *from = nullptr;
         if (x < all) {
-            const float2 y = ml(x);
+            const int64_t here = place(x);
+            const float2 y = (x < a.count ? a.ml : b.ml)[here];
             w = y.x == -INFINITY ? 0.0f : pg_exp2(y.x - top);
             part_l = w * y.y;
-            here = x < a.count ? a.at(x) : b.at(x - a.count);
+            from = (x < a.count ? a.sum : b.sum) + here * kPgDim;
         }
-        const uint32_t some = min(32u, all - x0);
-        for (uint32_t y0 = 0; y0 < some; y0 += 8) {
+        const int32_t some = min(32, all - x0);
+#pragma unroll 1
+        for (int32_t y0 = 0; y0 < some; y0 += 8) {
             float4 v[8];
             float f[8];
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
-                const uint32_t z = (y0 + y) & 31;
-                f[y] = __shfl_sync(0xffffffffu, w, z);
-                l += __shfl_sync(0xffffffffu, part_l, z);
-                const uint64_t from = __shfl_sync(0xffffffffu, here, z);
+                f[y] = __shfl_sync(0xffffffffu, w, y0 + y);
+                const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), y0 + y));
                 v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (f[y] != 0.0f) v[y] = ld4((x0 + z < a.count ? a.sum : b.sum) + from * kPgDim + 4 * lane);
+                if (f[y] != 0.0f) v[y] = ld4(src + 4 * lane);
             }
 #pragma unroll
             for (int y = 0; y < 8; ++y)
                 o = make_float4(fmaf(f[y], v[y].x, o.x), fmaf(f[y], v[y].y, o.y), fmaf(f[y], v[y].z, o.z), fmaf(f[y], v[y].w, o.w));
         }
+        l += warp_sum(part_l);
     }
 }
 template <bool F32>
-__device__ __forceinline__ void join_store(const PagedAttnParams &p, uint64_t row, uint32_t head, float4 o, float l, float top) {
+__device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row, int32_t head, float4 o, float l, float top) {
     const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    const uint64_t to = row * p.out_stride + static_cast<uint64_t>(head) * kPgDim + 4 * (threadIdx.x & 31);
+    const uint64_t to = row * p.out_stride + head * kPgDim + 4 * (threadIdx.x & 31);
     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + to, o);
     else pg_store4(static_cast<uint16_t *>(p.out) + to, o);
 }
@@ -903,43 +960,43 @@ __device__ __forceinline__ void join_store(const PagedAttnParams &p, uint64_t ro
 // split into many parts, one where there are rows enough), the prompts' tiles
 // that two or more CTAs shared, and zeroes the rows that see nothing.
 template <bool F32, int WPH>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
     __shared__ float4 warp_sum_at[WPH][32];
     __shared__ float warp_l[WPH];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WPH == 1 ? 0 : warp;
+    const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WPH == 1 ? 0 : warp;
     pdl_wait();
     const int32_t tiles = p.tile_rows ? p.header[kTlTiles] : 0, pre_tiles = p.tile_rows ? p.header[kTlPreTiles] : 0;
     const int32_t ctas = p.tile_rows ? p.header[kTlCtas] : 0;
-    const int64_t units = tiles ? static_cast<int64_t>(p.tile_unit[tiles]) * p.kh : 0;
-    const uint64_t results = static_cast<uint64_t>(p.header[kTlShortRows]) * p.qh;
-    const uint32_t lanes = WPH == 1 ? gridDim.x * 8 : gridDim.x;  // of results in flight
-    for (uint64_t n = WPH == 1 ? blockIdx.x * 8 + warp : blockIdx.x; n < results; n += lanes) {
-        const uint32_t listed = static_cast<uint32_t>(n / p.qh), head = static_cast<uint32_t>(n % p.qh);
-        const uint32_t kv = head / p.group, in_group = head % p.group;
+    const TileRuns runs = tile_runs(p);
+    const int32_t results = p.header[kTlShortRows] * p.qh;
+    const int32_t lanes = WPH == 1 ? gridDim.x * 8 : gridDim.x;  // of results in flight
+    PartList shared, own;
+    float4 o;
+    float l, top;
+#pragma unroll 1
+    for (int32_t n = WPH == 1 ? blockIdx.x * 8 + warp : blockIdx.x; n < results; n += lanes) {
+        const int32_t listed = p.by_qh.div(n), head = n - listed * p.qh;
+        const int32_t kv = p.by_group.div(head), in_group = head - kv * p.group;
         const int4 e = p.short_list[listed];
-        PartList shared{}, own{};
+        shared.count = own.count = 0;
         if (e.y >= 0) {
             const int4 rec = p.own_record[e.z];
             if (rec.y == 1 && p.prefix == 0) continue;  // written where it was computed
-            const uint32_t m = e.w * p.group + in_group;
-            own = PartList{p.own_sum, p.own_ml, (static_cast<uint64_t>(rec.x) + m / p.row_tile) * p.kh + kv,
-                           static_cast<uint64_t>(rec.z) * p.kh, p.row_tile, m % p.row_tile, static_cast<uint32_t>(rec.y)};
+            const int32_t m = e.w * p.group + in_group;
+            own = PartList{p.own_sum, p.own_ml, (rec.x + (m >> p.row_shift)) * p.kh + kv, rec.z * p.kh, p.row_tile,
+                           m & (p.row_tile - 1), rec.y};
             if (p.prefix_splits) {
-                const uint64_t pm = static_cast<uint64_t>(e.x) * p.group + in_group;
-                shared = PartList{p.prefix_sum, p.prefix_ml, pm / p.row_tile * p.kh + kv, static_cast<uint64_t>(p.prefix_tiles) * p.kh,
-                                  p.row_tile, static_cast<uint32_t>(pm % p.row_tile), p.prefix_splits};
+                const int32_t pm = e.x * p.group + in_group;
+                shared = PartList{p.prefix_sum, p.prefix_ml, (pm >> p.row_shift) * p.kh + kv, p.prefix_tiles * p.kh, p.row_tile,
+                                  pm & (p.row_tile - 1), p.prefix_splits};
             } else if (pre_tiles && ctas) {
-                const uint32_t tile = listed / p.tile_rows;
-                const int64_t steps = static_cast<int64_t>(p.tile_unit[tile + 1]) - p.tile_unit[tile];
-                const int64_t u0 = static_cast<int64_t>(p.tile_unit[tile]) * p.kh + kv * steps;
-                const int32_t c0 = tile_cta_of(units, ctas, u0);
-                const uint32_t count = steps ? tile_cta_of(units, ctas, u0 + steps - 1) - c0 + 1 : 0;
-                shared = PartList{p.tile_sum, p.tile_ml, 2ull * p.tile_grid + c0 + static_cast<uint64_t>(tile) * p.kh + kv, 1,
-                                  kTlPairs, listed % p.tile_rows * p.group + in_group, count};
+                const int32_t tile = p.by_tile_rows.div(listed);
+                const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
+                const int32_t u0 = unit * p.kh + kv * steps, c0 = runs.cta_of(u0);
+                shared = PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, kTlPairs,
+                                  (listed - tile * p.tile_rows) * p.group + in_group, steps ? runs.cta_of(u0 + steps - 1) - c0 + 1 : 0};
             }
         }
-        float4 o;
-        float l, top;
         join_parts<WPH>(shared, own, sub, o, l, top);
         if constexpr (WPH > 1) {  // the warps' sums, in order
             warp_sum_at[sub][lane] = o;
@@ -952,51 +1009,46 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
                     o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
                     l += warp_l[w];
                 }
-                join_store<F32>(p, e.x, head, o, l, top);
             }
-            __syncthreads();
-        } else {
-            join_store<F32>(p, e.x, head, o, l, top);
         }
+        if (sub == 0) join_store<F32>(p, e.x, head, o, l, top);
+        if constexpr (WPH > 1) __syncthreads();
     }
     // Prompts' tiles that a CTA's end cuts: the first such end does the tile, 32 pairs to a block.
-    for (int64_t n = blockIdx.x; n < 8ll * (ctas - 1); n += gridDim.x) {
-        const int32_t c = static_cast<int32_t>(n / 8) + 1;
-        const int64_t cut = tile_cta_start(units, ctas, c);
-        const int32_t tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles),
-                                      static_cast<int32_t>(cut / p.kh));
+#pragma unroll 1
+    for (int32_t n = blockIdx.x; n < 8 * (ctas - 1); n += gridDim.x) {
+        const int32_t c = n / 8 + 1, cut = runs.start(c);
+        const int32_t tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles), p.by_kh.div(cut));
         if (tile < pre_tiles) continue;
-        const int64_t steps = static_cast<int64_t>(p.tile_unit[tile + 1]) - p.tile_unit[tile];
-        const int64_t head0 = static_cast<int64_t>(p.tile_unit[tile]) * p.kh;
-        const int64_t kv = (cut - head0) / steps, u0 = head0 + kv * steps;
-        if (cut == u0 || tile_cta_start(units, ctas, c - 1) > u0) continue;
-        const int32_t last = tile_cta_of(units, ctas, u0 + steps - 1);
+        const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
+        const int32_t kv = (cut - unit * p.kh) / steps, u0 = unit * p.kh + kv * steps, before = runs.start(c - 1);
+        if (cut == u0 || before > u0) continue;
         // CTA c - 1 has this tile as its last run unless it begins with it; the others begin with it.
-        const bool begins = tile_cta_start(units, ctas, c - 1) == u0;
-        const int32_t row0 = tile_first_row(p, tile), rows = tile_row_count(p, tile);
-        for (uint32_t pair = static_cast<uint32_t>(n % 8) * 32 + warp; pair < static_cast<uint32_t>(n % 8) * 32 + 32; pair += 8) {
-            if (pair >= rows * p.group) break;
-            const PartList one{p.tile_sum, p.tile_ml, 2ull * (c - 1) + (begins ? 0 : 1), 0, kTlPairs, pair, 1};
-            const PartList more{p.tile_sum, p.tile_ml, 2ull * c, 2, kTlPairs, pair, static_cast<uint32_t>(last - c + 1)};
-            float4 o;
-            float l, top;
-            join_parts<1>(one, more, 0, o, l, top);
-            join_store<F32>(p, static_cast<uint64_t>(row0) + pair / p.group, static_cast<uint32_t>(kv) * p.group + pair % p.group, o, l, top);
+        shared = PartList{p.tile_sum, p.tile_ml, 2 * (c - 1) + (before == u0 ? 0 : 1), 0, kTlPairs, 0, 1};
+        own = PartList{p.tile_sum, p.tile_ml, 2 * c, 2, kTlPairs, 0, runs.cta_of(u0 + steps - 1) - c + 1};
+        const int32_t row0 = p.tile_shape[tile].row0, pairs = p.tile_shape[tile].rows * p.group;
+#pragma unroll 1
+        for (int32_t pair = (n & 7) * 32 + warp; pair < min((n & 7) * 32 + 32, pairs); pair += 8) {
+            shared.place = own.place = pair;
+            join_parts<1>(shared, own, 0, o, l, top);
+            const int32_t i = p.by_group.div(pair);
+            join_store<F32>(p, row0 + i, kv * p.group + pair - i * p.group, o, l, top);
         }
     }
     // Rows that no request has, and tiles without a key.
     const int32_t taken = p.requests ? max(p.starts[p.requests], 0) : 0;
-    const uint32_t width = p.qh * kPgDim / 4;
-    const auto clear = [&](uint64_t row) {
-        for (uint32_t x = threadIdx.x; x < width; x += blockDim.x) {
+    const auto clear = [&](int32_t row) {
+        for (int32_t x = threadIdx.x; x < p.qh * kPgDim / 4; x += blockDim.x) {
             if constexpr (F32) pg_store4(static_cast<float *>(p.out) + row * p.out_stride + 4 * x, make_float4(0.f, 0.f, 0.f, 0.f));
             else pg_store4(static_cast<uint16_t *>(p.out) + row * p.out_stride + 4 * x, make_float4(0.f, 0.f, 0.f, 0.f));
         }
     };
-    for (uint64_t row = static_cast<uint64_t>(taken) + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
+#pragma unroll 1
+    for (int32_t row = min(taken, p.rows) + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
+#pragma unroll 1
     for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); tile < tiles; tile += gridDim.x)
         if (p.tile_unit[tile + 1] == p.tile_unit[tile])
-            for (int32_t i = 0; i < tile_row_count(p, tile); ++i) clear(static_cast<uint64_t>(tile_first_row(p, tile)) + i);
+            for (int32_t i = 0; i < p.tile_shape[tile].rows; ++i) clear(p.tile_shape[tile].row0 + i);
 }
 
 }  // namespace plamo
