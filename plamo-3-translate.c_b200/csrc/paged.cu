@@ -56,8 +56,8 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
-    uint32_t row_tile, prefix_tiles, prefix_splits, own_groups, workers, tile_rows, tile_cap;
-    uint64_t record, own_sum, own_ml, prefix_sum, prefix_ml;
+    uint32_t row_tile, prefix_tiles, row_slots, workers, tile_rows, tile_cap;
+    uint64_t record, row_sum, row_ml;
     uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
 };
 
@@ -73,33 +73,26 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     // Eight pairs to a tile while a request has no more on average (the heads of
     // a group of eight, one row each); FP32 sums leave no registers for more.
     a.row_tile = d->type == PLAMO_PAGED_FP32 || pairs <= 8 * d->requests ? 8 : 16;
-    a.prefix_tiles = static_cast<uint32_t>(ceil_div(pairs, a.row_tile));
-    if (prefix_pages && a.prefix_tiles && !a.tile_rows) {
-        const uint64_t want = ceil_div(2 * sms, static_cast<uint64_t>(a.prefix_tiles) * d->kv_heads);
-        a.prefix_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(want, prefix_pages / kRtMinPages)));
-    }
+    a.prefix_tiles = prefix_pages && !a.tile_rows ? static_cast<uint32_t>(ceil_div(pairs, a.row_tile)) : 0;
     a.workers = static_cast<uint32_t>(2 * sms - 1);  // beside the schedule's CTA
-    // Every request's last tile and last run of pages may be partial. Beside the
-    // tile kernel only requests of up to kTlShortPairs pairs are here.
-    const uint64_t own_tiles = pairs / a.row_tile + std::min<uint64_t>(d->requests, d->rows);
-    a.own_groups = static_cast<uint32_t>(std::min<uint64_t>(
-        (a.tile_rows ? std::min<uint64_t>(own_tiles, kTlShortPairs / a.row_tile * d->requests) : own_tiles) + ceil_div(a.workers, d->kv_heads),
-        INT32_MAX / d->kv_heads));
+    // A slot for each strip (a row tile and KV head; every request's last tile
+    // may be partial), one more for each CTA. Beside the tile kernel only
+    // requests of up to kTlShortPairs pairs are here.
+    const uint64_t tiles = pairs / a.row_tile + std::min<uint64_t>(d->requests, d->rows);
+    a.row_slots = static_cast<uint32_t>(std::min<uint64_t>(
+        a.workers + d->kv_heads * (a.prefix_tiles + (a.tile_rows ? std::min<uint64_t>(tiles, kTlShortPairs / a.row_tile * d->requests) : tiles)),
+        INT32_MAX));
     uint64_t at = 0;
     auto part = [&](uint64_t bytes) {
         const uint64_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    const uint64_t own = static_cast<uint64_t>(a.own_groups) * d->kv_heads;
-    const uint64_t prefix = static_cast<uint64_t>(a.prefix_splits) * a.prefix_tiles * d->kv_heads;
     a.header = part(kTlHeader * 4);
     a.short_list = part(d->rows * sizeof(int4));
-    a.record = part(d->requests * sizeof(int4));
-    a.own_sum = part(own * a.row_tile * kPgDim * 4);
-    a.own_ml = part(own * a.row_tile * sizeof(float2));
-    a.prefix_sum = part(prefix * a.row_tile * kPgDim * 4);
-    a.prefix_ml = part(prefix * a.row_tile * sizeof(float2));
+    a.record = part((d->requests + 1) * sizeof(int4));
+    a.row_sum = part(static_cast<uint64_t>(a.row_slots) * a.row_tile * kPgDim * 4);
+    a.row_ml = part(static_cast<uint64_t>(a.row_slots) * a.row_tile * sizeof(float2));
     if (a.tile_rows) {
         // Two runs of a CTA may end inside a prompt's tile; every run of a prefix tile is a part.
         const uint64_t shared = prefix_pages ? sms + ceil_div(d->rows, a.tile_rows) * d->kv_heads : 0;
@@ -150,17 +143,14 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.scale2 = d->scale * 1.4426950408889634f;
     // The tile kernel masks before it scales: -inf must stay so.
     if (std::fabs(p.scale2) < 1e-30f) p.scale2 = std::copysign(1e-30f, p.scale2);
-    p.own_record = reinterpret_cast<int4 *>(ws + a.record);
+    p.row_record = reinterpret_cast<int4 *>(ws + a.record);
     p.header = reinterpret_cast<int32_t *>(ws + a.header);
     p.short_list = reinterpret_cast<int4 *>(ws + a.short_list);
-    p.own_sum = reinterpret_cast<float *>(ws + a.own_sum);
-    p.own_ml = reinterpret_cast<float2 *>(ws + a.own_ml);
-    p.prefix_sum = reinterpret_cast<float *>(ws + a.prefix_sum);
-    p.prefix_ml = reinterpret_cast<float2 *>(ws + a.prefix_ml);
+    p.row_sum = reinterpret_cast<float *>(ws + a.row_sum);
+    p.row_ml = reinterpret_cast<float2 *>(ws + a.row_ml);
     p.row_tile = static_cast<int32_t>(a.row_tile);
     p.row_shift = a.row_tile == 8 ? 3 : 4;
-    p.own_groups = static_cast<int32_t>(a.own_groups);
-    p.prefix_splits = static_cast<int32_t>(a.prefix_splits);
+    p.row_slots = static_cast<int32_t>(a.row_slots);
     p.prefix_tiles = static_cast<int32_t>(a.prefix_tiles);
     p.workers = static_cast<int32_t>(a.workers);
     if (a.tile_rows) {

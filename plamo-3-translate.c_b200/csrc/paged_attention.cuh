@@ -45,12 +45,12 @@ struct PagedAttnParams {
     float scale2;            // scale * log2(e)
     int32_t row_tile, row_shift;  // pairs to a tile of the row kernel: 1 << row_shift
     // Its partial results, unnormalised: [slot][row_tile][128] sums and [slot][row_tile] {m, l}.
-    int4 *own_record;  // [requests] {first own slot / kv heads, splits, row tiles}
-    float *own_sum, *prefix_sum;
-    float2 *own_ml, *prefix_ml;
-    int32_t own_groups;  // capacity of the own partials, in slots per KV head
-    int32_t prefix_splits, prefix_tiles;
-    int32_t workers;     // CTAs of the row kernel that take items
+    float *row_sum;
+    float2 *row_ml;
+    int4 *row_record;      // [requests + 1] where a request's units begin, its pages, its first strip, tiles; last: the prefix
+    int32_t row_slots;     // capacity
+    int32_t workers;       // CTAs that take work
+    int32_t prefix_tiles;  // row tiles over the prefix, 0: the tile kernel's
     // The schedule (paged_tiles.cuh).
     int32_t *header;   // [kTlHeader]
     int4 *short_list;  // [rows] {batch row, own row, request, row of it} of the short requests' rows
@@ -64,7 +64,7 @@ struct PagedAttnParams {
     float *tile_sum;               // [slot][256][128], [slot][256] {m, l}
     float2 *tile_ml;
 };
-enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlHeader = 8 };
+enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kRtRun, kRtLonger, kTlHeader };
 constexpr int kTlPairs = 256;     // (row, head) pairs to a tile
 constexpr int kTlShortPairs = 32; // requests of up to so many keep their own rows in the row kernel
 constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
@@ -74,8 +74,8 @@ constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 constexpr int kRtKeys = 16;
 constexpr int kRtWarps = 6;                      // computing warps, a slab each in turn
 constexpr int kRtThreads = 32 * (kRtWarps + 1);  // and the copying warp
-constexpr int kRtMinPages = 2;                   // least pages worth an item of their own
-constexpr int kRtBatch = 8;                      // items looked up at a time
+constexpr int kRtMinPages = 2;                   // least pages worth a CTA
+constexpr int kRtBatch = 8;                      // items laid out at a time
 template <bool F32>
 __host__ __device__ constexpr int rt_slab_bytes() {  // keys, then values
     return 2 * kRtKeys * kPgDim * (F32 ? 4 : 2);
@@ -130,9 +130,12 @@ struct __align__(16) TileShape {
     __device__ int32_t steps() const { return pre1 - pre0 + own1 - own0; }
 };
 
-// The tile kernel's CTAs take equal runs of all units (key steps of a tile and
-// KV head): the first `longer` of them run + 1, the others run.
-struct TileRuns {
+// Work comes in strips, the keys of one tile and KV head, of so many units
+// (pages in the row kernel, key steps in the tile kernel). CTAs take equal runs
+// of all units, whatever strips they cut: the first `longer` of them run + 1,
+// the others run. Strip x's part in CTA c has slot c + x, its own since each
+// part begins with the next CTA or the next strip.
+struct Runs {
     int32_t run, longer;
     __device__ __forceinline__ int32_t start(int32_t cta) const { return cta * run + min(cta, longer); }
     __device__ __forceinline__ int32_t cta_of(int32_t unit) const {
@@ -140,7 +143,8 @@ struct TileRuns {
         return unit < cut ? unit / (run + 1) : longer + (unit - cut) / run;
     }
 };
-__device__ __forceinline__ TileRuns tile_runs(const PagedAttnParams &p) { return TileRuns{p.header[kTlRun], p.header[kTlLonger]}; }
+__device__ __forceinline__ Runs tile_runs(const PagedAttnParams &p) { return Runs{p.header[kTlRun], p.header[kTlLonger]}; }
+__device__ __forceinline__ Runs row_runs(const PagedAttnParams &p) { return Runs{p.header[kRtRun], p.header[kRtLonger]}; }
 
 struct RowItem {
     int32_t request;  // -1: prefix
@@ -640,8 +644,21 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
 // and warp against 0.7 us for BF16.)
 __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums);  // paged_tiles.cuh
 
-constexpr int kRtChunks = 6;  // item sizes weighed, in pages: the least * 4/4, 5/4, 6/4, 2, 3, 4
-__device__ __forceinline__ int32_t rt_chunk_pages(int32_t least, int x) { return x < 3 ? (least * (4 + x) + 3) / 4 : least * (x - 1); }
+// Request r's work, or the prefix's (r == requests) from page pp0 on.
+__device__ __forceinline__ OwnShape row_work(const PagedAttnParams &p, int32_t r, int32_t pp0) {
+    if (r < p.requests) {
+        OwnShape s = short_shape(p, r);
+        if (!s.pages) s.tiles = 0;
+        return s;
+    }
+    OwnShape s{};
+    s.rows = p.rows;
+    s.length = p.prefix;
+    s.page0 = pp0;
+    s.pages = (p.prefix + kPgRows - 1) / kPgRows - pp0;
+    s.tiles = s.pages ? p.prefix_tiles : 0;
+    return s;
+}
 
 template <bool F32, int NT>
 __global__ void __launch_bounds__(kRtThreads, 2)
@@ -657,7 +674,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
     __shared__ RowItem items[kRtBatch];
     __shared__ float2 warp_ml[kRtWarps][PAIRS];
     __shared__ __align__(16) float weights[F32 ? kRtWarps : 1][F32 ? kRtKeys * 8 : 4];
-    __shared__ int32_t item_counts[kRtChunks], lowest_at;
+    __shared__ int32_t first_strip, last_strip, lowest_at;
     unsigned char *base = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(rt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float *joined = reinterpret_cast<float *>(base + kRtRing);  // [GROUPS][PAIRS][128]
@@ -677,137 +694,106 @@ __global__ void __launch_bounds__(kRtThreads, 2)
         fence_barrier_init();
         prefetch_tensormap(&map);
         lowest_at = INT32_MAX;
+        first_strip = 0;
+        last_strip = -1;
     }
-    if (tid < kRtChunks) item_counts[tid] = 0;
 
-    // Every CTA lays the items out by itself from the requests' lengths.
+    // Every CTA lays the work out by itself from the requests' lengths: thread
+    // t's share of the requests, and the prefix after the last one's.
     const int32_t per = (p.requests + kRtThreads - 1) / kRtThreads;
-    const int32_t r0 = min(p.requests, tid * per), r1 = min(p.requests, r0 + per);
-    int64_t units = 0, total_units;
-    int32_t lowest = INT32_MAX;
-    for (int32_t r = r0; r < r1; ++r) {
-        const OwnShape s = short_shape(p, r);
-        units += static_cast<int64_t>(s.tiles) * s.pages;
-        if (s.rows) lowest = min(lowest, max(s.at0, 0));
-    }
-    pg_block_scan<kRtThreads>(units, scan, &total_units);
-    // Pages to an item: whole rounds of items over the CTAs, each costing its
-    // pages and about four more to begin and end.
-    const int32_t least = max(kRtMinPages, static_cast<int32_t>(fminf(1e8f, ceilf(1.0001f * static_cast<float>(total_units) * p.kh / p.workers))));
-    int32_t counts[kRtChunks];
-#pragma unroll
-    for (int x = 0; x < kRtChunks; ++x) counts[x] = 0;
-#pragma unroll 1
-    for (int32_t r = r0; r < r1; ++r) {
-        const OwnShape s = short_shape(p, r);
-#pragma unroll
-        for (int x = 0; x < kRtChunks; ++x) {
-            const int32_t c = rt_chunk_pages(least, x);
-            counts[x] += s.tiles * ((s.pages + c - 1) / c);
+    const int32_t r0 = min(p.requests, tid * per);
+    const int32_t r1 = min(p.requests, r0 + per) + (tid == kRtThreads - 1 && p.prefix_tiles);
+    int32_t pp0 = 0;  // first prefix page that some row sees
+    if (p.window && p.prefix_tiles) {
+        __syncthreads();
+        int32_t lowest = INT32_MAX;
+        for (int32_t r = r0; r < min(r1, p.requests); ++r) {
+            const OwnShape s = own_shape(p, r);
+            if (s.rows) lowest = min(lowest, max(s.at0, 0));
         }
-    }
-#pragma unroll
-    for (int x = 0; x < kRtChunks; ++x) {
-        const int32_t sum = __reduce_add_sync(0xffffffffu, counts[x]);
-        if (lane == 0 && sum) atomicAdd(&item_counts[x], sum);
-    }
-    if (p.window) {
         lowest = __reduce_min_sync(0xffffffffu, lowest);
         if (lane == 0) atomicMin(&lowest_at, lowest);
+        __syncthreads();
+        if (lowest_at != INT32_MAX) pp0 = min(max(p.prefix + lowest_at - p.window + 1, 0), p.prefix) / kPgRows;
     }
-    __syncthreads();
-    int32_t chunk = least, mine = counts[0];
-    float cost = INFINITY;
-#pragma unroll
-    for (int x = 0; x < kRtChunks; ++x) {
-        const int32_t c = rt_chunk_pages(least, x);
-        const float y = ceilf(static_cast<float>(item_counts[x]) * p.kh / p.workers) * (c + 4);
-        if (y < cost) {
-            cost = y;
-            chunk = c;
-            mine = counts[x];
-        }
+    int64_t units = 0, strips = 0, all_units, all_strips;
+#pragma unroll 1
+    for (int32_t r = r0; r < r1; ++r) {
+        const OwnShape s = row_work(p, r, pp0);
+        strips += s.tiles * p.kh;
+        units += static_cast<int64_t>(s.tiles) * s.pages * p.kh;
     }
-    int64_t all;
-    const int32_t first = static_cast<int32_t>(pg_block_scan<kRtThreads>(mine, scan, &all));
-    const int32_t total = static_cast<int32_t>(min(all, static_cast<int64_t>(p.own_groups)));
-    if (all > total && tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
-    if (worker == 0) {
-        int32_t at = first;
+    const int64_t unit0 = pg_block_scan<kRtThreads>(units, scan, &all_units);
+    const int32_t strip0 = static_cast<int32_t>(pg_block_scan<kRtThreads>(strips, scan, &all_strips));
+    if (all_units > INT32_MAX - 1024 || all_strips + p.workers > p.row_slots) {  // only starts that overlap ask for this
+        if (tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
+        all_units = 0;
+    }
+    const int32_t total = static_cast<int32_t>(all_units);
+    const int32_t ctas = min(p.workers, (total + kRtMinPages - 1) / kRtMinPages);
+    const Runs runs{ctas ? total / ctas : 1, ctas ? total % ctas : 0};
+    const int32_t begin_unit = runs.start(min(worker, ctas)), end_unit = runs.start(min(worker + 1, ctas));
+    // The request or prefix of this thread: its strips that this CTA has a part of, as
+    // f(shape, request, first unit, first strip).
+    const auto each = [&](auto f) {
+        int32_t unit = static_cast<int32_t>(unit0), strip = strip0;
 #pragma unroll 1
         for (int32_t r = r0; r < r1; ++r) {
-            const OwnShape s = short_shape(p, r);
-            const int32_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
-            p.own_record[r] = at + n <= total ? make_int4(at, splits, s.tiles, 0) : make_int4(0, 0, 0, 0);
-            at += n;
+            const OwnShape s = row_work(p, r, pp0);
+            f(s, r, unit, strip);
+            strip += s.tiles * p.kh;
+            unit += s.tiles * s.pages * p.kh;
+        }
+    };
+    if (worker == 0) {
+        each([&](const OwnShape &s, int32_t r, int32_t unit, int32_t strip) {
+            p.row_record[r] = total ? make_int4(unit, s.pages, strip, s.tiles) : make_int4(0, 0, 0, 0);
+        });
+        if (tid == 0) {
+            p.header[kRtRun] = runs.run;
+            p.header[kRtLonger] = runs.longer;
         }
     }
-    // Prefix pages that some row still sees.
-    const int32_t prefix_pages = (p.prefix + kPgRows - 1) / kPgRows;
-    int32_t pp0 = 0;
-    if (p.window && lowest_at != INT32_MAX) pp0 = min(max(p.prefix + lowest_at - p.window + 1, 0), p.prefix) / kPgRows;
-    const int32_t pchunk = p.prefix_splits ? (prefix_pages - pp0 + p.prefix_splits - 1) / p.prefix_splits : 0;
-    const int32_t own_items = total * p.kh, all_items = own_items + p.prefix_splits * p.prefix_tiles * p.kh;
+    if (begin_unit < end_unit)
+        each([&](const OwnShape &s, int32_t, int32_t unit, int32_t strip) {
+            const int32_t n = s.tiles * s.pages * p.kh;
+            if (begin_unit >= unit && begin_unit < unit + n) first_strip = strip + (begin_unit - unit) / s.pages;
+            if (end_unit > unit && end_unit <= unit + n) last_strip = strip + (end_unit - 1 - unit) / s.pages;
+        });
+    __syncthreads();
 
     uint32_t ring = 0, issued = 0;  // slabs of the items before; copied ones
     bool dead = false;
-    for (int32_t batch = worker; batch < all_items; batch += p.workers * kRtBatch) {
+#pragma unroll 1
+    for (int32_t batch = first_strip; batch <= last_strip; batch += kRtBatch) {
         __syncthreads();  // the last batch's items are done with
-        {
-            // The thread that lays out a request fills in those of its items that this CTA takes.
-            int32_t at = first;
+        each([&](const OwnShape &s, int32_t r, int32_t unit, int32_t strip) {
+            const int32_t x0 = max(batch, strip), x1 = min(min(batch + kRtBatch, last_strip + 1), strip + s.tiles * p.kh);
 #pragma unroll 1
-            for (int32_t r = r0; r < r1; ++r) {
-                const OwnShape s = short_shape(p, r);
-                const int32_t splits = (s.pages + chunk - 1) / chunk, n = s.tiles * splits;
-                if (n)
-#pragma unroll 1
-                    for (int k = 0; k < kRtBatch; ++k) {
-                        const int32_t id = batch + k * p.workers, group = p.by_kh.div(id);
-                        if (id >= own_items || group < at || group >= at + n) continue;
-                        const int32_t split = (group - at) / s.tiles, even = (s.pages + splits - 1) / splits;
-                        RowItem it;
-                        it.request = r;
-                        it.tile = group - at - split * s.tiles;
-                        it.head = id - group * p.kh;
-                        it.page0 = s.page0 + min(split * even, s.pages);
-                        it.pages = min(even, s.page0 + s.pages - it.page0);
-                        // Keys past the tile's last row are seen by none of its rows.
-                        const int32_t last = s.at0 + min(s.rows - 1, p.by_group.div(it.tile * PAIRS + PAIRS - 1));
-                        it.limit = min(max(last + 1, 0), s.length);
-                        it.row0 = s.row0;
-                        it.rows = s.rows;
-                        it.at0 = s.at0;
-                        it.slot = id;
-                        it.direct = splits == 1 && p.prefix == 0;
-                        items[k] = it;
-                    }
-                at += n;
+            for (int32_t x = x0; x < x1; ++x) {
+                const int32_t y = x - strip, from = unit + y * s.pages;  // the strip's units: [from, from + pages)
+                RowItem it;
+                it.request = r < p.requests ? r : -1;
+                it.tile = p.by_kh.div(y);
+                it.head = y - it.tile * p.kh;
+                const int32_t lo = max(begin_unit - from, 0), hi = min(end_unit - from, s.pages);
+                it.page0 = s.page0 + lo;
+                it.pages = hi - lo;
+                // Keys past the tile's last row are seen by none of its rows.
+                const int32_t last = s.at0 + min(s.rows - 1, p.by_group.div(it.tile * PAIRS + PAIRS - 1));
+                it.limit = r < p.requests ? min(max(last + 1, 0), s.length) : p.prefix;
+                it.row0 = s.row0;
+                it.rows = s.rows;
+                it.at0 = s.at0;
+                it.slot = worker + x;
+                it.direct = it.pages == s.pages && p.prefix == 0;
+                items[x - batch] = it;
             }
-            if (tid < kRtBatch) {
-                const int32_t id = batch + tid * p.workers;
-                if (id >= own_items && id < all_items) {
-                    const int32_t x = id - own_items, y = p.by_kh.div(x), split = y / p.prefix_tiles;
-                    RowItem it;
-                    it.request = -1;
-                    it.head = x - y * p.kh;
-                    it.tile = y - split * p.prefix_tiles;
-                    it.page0 = min(pp0 + split * pchunk, prefix_pages);
-                    it.pages = min(pchunk, prefix_pages - it.page0);
-                    it.limit = p.prefix;
-                    it.row0 = 0;
-                    it.rows = p.rows;
-                    it.at0 = 0;
-                    it.slot = x;
-                    it.direct = 0;
-                    items[tid] = it;
-                }
-            }
-        }
+        });
         __syncthreads();
 #pragma unroll 1
         for (int k = 0; k < kRtBatch; ++k) {
-            if (batch + k * p.workers >= all_items) break;
+            if (batch + k > last_strip) break;
             const RowItem it = items[k];
             const int32_t begin = it.page0 * kPgRows, end = min(begin + it.pages * kPgRows, it.limit);
             const int32_t slabs = end > begin ? (end - begin + kRtKeys - 1) / kRtKeys : 0;
@@ -879,8 +865,8 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                     else pg_store4(static_cast<uint16_t *>(p.out) + at, v);
                 } else {
                     const uint64_t at = static_cast<uint64_t>(it.slot) * PAIRS + pair;
-                    *reinterpret_cast<float4 *>((it.request < 0 ? p.prefix_sum : p.own_sum) + at * kPgDim + d) = v;
-                    if (d == 0) (it.request < 0 ? p.prefix_ml : p.own_ml)[at] = make_float2(top, l);
+                    *reinterpret_cast<float4 *>(p.row_sum + at * kPgDim + d) = v;
+                    if (d == 0) p.row_ml[at] = make_float2(top, l);
                 }
             }
             rt_bar();  // before the next item writes warp_ml or the sums
@@ -967,7 +953,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     pdl_wait();
     const int32_t tiles = p.tile_rows ? p.header[kTlTiles] : 0, pre_tiles = p.tile_rows ? p.header[kTlPreTiles] : 0;
     const int32_t ctas = p.tile_rows ? p.header[kTlCtas] : 0;
-    const TileRuns runs = tile_runs(p);
+    const Runs runs = tile_runs(p), of_rows = row_runs(p);
     const int32_t results = p.header[kTlShortRows] * p.qh;
     const int32_t lanes = WPH == 1 ? gridDim.x * 8 : gridDim.x;  // of results in flight
     PartList shared, own;
@@ -980,15 +966,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         const int4 e = p.short_list[listed];
         shared.count = own.count = 0;
         if (e.y >= 0) {
-            const int4 rec = p.own_record[e.z];
-            if (rec.y == 1 && p.prefix == 0) continue;  // written where it was computed
-            const int32_t m = e.w * p.group + in_group;
-            own = PartList{p.own_sum, p.own_ml, (rec.x + (m >> p.row_shift)) * p.kh + kv, rec.z * p.kh, p.row_tile,
-                           m & (p.row_tile - 1), rec.y};
-            if (p.prefix_splits) {
-                const int32_t pm = e.x * p.group + in_group;
-                shared = PartList{p.prefix_sum, p.prefix_ml, (pm >> p.row_shift) * p.kh + kv, p.prefix_tiles * p.kh, p.row_tile,
-                                  pm & (p.row_tile - 1), p.prefix_splits};
+            // The parts of row tile t of request r (or of the prefix) for this head.
+            const auto row_parts = [&](int32_t r, int32_t m) {
+                const int4 rec = p.row_record[r];
+                const int32_t strip = (m >> p.row_shift) * p.kh + kv, u0 = rec.x + strip * rec.y;
+                const int32_t c0 = rec.y ? of_rows.cta_of(u0) : 0;
+                return PartList{p.row_sum, p.row_ml, c0 + rec.z + strip, 1, p.row_tile, m & (p.row_tile - 1),
+                                rec.y ? of_rows.cta_of(u0 + rec.y - 1) - c0 + 1 : 0};
+            };
+            own = row_parts(e.z, e.w * p.group + in_group);
+            if (own.count == 1 && p.prefix == 0) continue;  // written where it was computed
+            if (p.prefix_tiles) {
+                shared = row_parts(p.requests, e.x * p.group + in_group);
             } else if (pre_tiles && ctas) {
                 const int32_t tile = p.by_tile_rows.div(listed);
                 const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     const int32_t tiles = p.header[kTlTiles], pre_tiles = p.header[kTlPreTiles];
     TileWalk w{};
     if (cta < ctas) {
-        const TileRuns runs = tile_runs(p);
+        const Runs runs = tile_runs(p);
         w.unit = runs.start(cta);
         w.end = runs.start(cta + 1);
         w.tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles), p.by_kh.div(w.unit));
