@@ -56,7 +56,7 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
-    uint32_t row_tile, prefix_tiles, row_slots, workers, tile_rows, tile_cap;
+    uint32_t row_tile, prefix_tiles, row_slots, workers, tile_rows, tile_grid, tile_cap;
     uint64_t record, row_sum, row_ml;
     uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
 };
@@ -65,8 +65,16 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     AttentionLayout a{};
     const uint64_t group = d->query_heads / d->kv_heads, sms = static_cast<uint64_t>(context_sms(c));
     const uint64_t pairs = d->rows * group, prefix_pages = ceil_div(d->prefix_rows, kPgRows);
-    if (d->type == PLAMO_PAGED_BF16 && group <= kTlPairs && (prefix_pages || pairs > kTlShortPairs)) {
-        a.tile_rows = static_cast<uint32_t>(kTlPairs / group);
+    // The tile kernel is for prompts (more rows than requests, some request with
+    // more pairs than the row kernel takes) and for a prefix that would keep the
+    // row kernel, eight pairs at a time, longer than another kernel takes to
+    // begin and end (about 15 us: 4,000 pages and heads in BF16, 2,000 in FP32).
+    const bool f32 = d->type == PLAMO_PAGED_FP32;
+    const uint64_t tile_pairs = f32 ? kTfPairs : kTlPairs;
+    const uint64_t prefix_work = ceil_div(pairs, 8) * prefix_pages * d->kv_heads;
+    if (group <= tile_pairs && ((d->rows > d->requests && pairs > kTlShortPairs) || prefix_work > (f32 ? 2000 : 4000))) {
+        a.tile_rows = static_cast<uint32_t>(tile_pairs / group);
+        a.tile_grid = static_cast<uint32_t>(f32 ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
         a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
     }
@@ -95,12 +103,12 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     a.row_ml = part(static_cast<uint64_t>(a.row_slots) * a.row_tile * sizeof(float2));
     if (a.tile_rows) {
         // Two runs of a CTA may end inside a prompt's tile; every run of a prefix tile is a part.
-        const uint64_t shared = prefix_pages ? sms + ceil_div(d->rows, a.tile_rows) * d->kv_heads : 0;
-        const uint64_t slots = 2 * sms + shared;
+        const uint64_t shared = prefix_pages ? a.tile_grid + ceil_div(d->rows, a.tile_rows) * d->kv_heads : 0;
+        const uint64_t slots = 2ull * a.tile_grid + shared;
         a.tile_shape = part(a.tile_cap * sizeof(TileShape));
         a.tile_unit = part((a.tile_cap + 1ull) * 4);
-        a.tile_sum = part(slots * kTlPairs * kPgDim * 4);
-        a.tile_ml = part(slots * kTlPairs * sizeof(float2));
+        a.tile_sum = part(slots * tile_pairs * kPgDim * 4);
+        a.tile_ml = part(slots * tile_pairs * sizeof(float2));
     }
     a.bytes = std::max<uint64_t>(at, 256);
     return a;
@@ -157,7 +165,9 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
         p.pool = d->pool;
         p.tile_rows = static_cast<int32_t>(a.tile_rows);
         p.by_tile_rows = FastDiv::of(a.tile_rows);
-        p.tile_grid = context_sms(c);
+        p.tile_pairs = F32 ? kTfPairs : kTlPairs;
+        p.tile_keys = F32 ? kTfKeys : kTlKeys;
+        p.tile_grid = static_cast<int32_t>(a.tile_grid);
         p.tile_cap = static_cast<int32_t>(a.tile_cap);
         p.tile_shape = reinterpret_cast<TileShape *>(ws + a.tile_shape);
         p.tile_unit = reinterpret_cast<uint32_t *>(ws + a.tile_unit);
@@ -168,8 +178,8 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     if constexpr (!F32)
         if (a.row_tile == 16) rows = paged_rows_kernel<F32, 2>;
     if (!launch(c, "paged_attention rows", rows, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
-        (a.tile_rows && !launch(c, "paged_attention tiles", paged_tile_kernel, dim3(p.tile_grid), dim3(kTlThreads), kTlSmem,
-                                stream, true, page_map, p)))
+        (a.tile_rows && !launch(c, "paged_attention tiles", F32 ? paged_tile_f32_kernel : paged_tile_kernel, dim3(a.tile_grid),
+                                dim3(F32 ? kTfThreads : kTlThreads), F32 ? kTfSmem : kTlSmem, stream, true, page_map, p)))
         return false;
     // Eight warps to a result while one each would leave SMs idle.
     const uint64_t results = d->rows * d->query_heads, wave = 8ull * context_sms(c);
@@ -203,6 +213,7 @@ cudaError_t paged_configure() {
     if (e == cudaSuccess) e = allow(paged_rows_kernel<false, 2>, kRtSmem);
     if (e == cudaSuccess) e = allow(paged_rows_kernel<true, 1>, kRtSmem);
       if (e == cudaSuccess) e = allow(paged_tile_kernel, kTlSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_f32_kernel, kTfSmem);
     return e;
 }
 }  // namespace plamo

@@ -56,16 +56,17 @@ struct PagedAttnParams {
     int4 *short_list;  // [rows] {batch row, own row, request, row of it} of the short requests' rows
     // The tile kernel's share; tile_rows 0: it has none.
     const void *pool;
-    int32_t tile_rows;  // batch rows to a tile
+    int32_t tile_rows;   // batch rows to a tile
+    int32_t tile_pairs;  // pairs to a tile: 256 in BF16, 64 in FP32
+    int32_t tile_keys;   // keys to a step: 128, 64
     FastDiv by_tile_rows;
     int32_t tile_grid, tile_cap;
     struct TileShape *tile_shape;  // [tile_cap]
     uint32_t *tile_unit;           // [tile_cap + 1] key steps before each tile
-    float *tile_sum;               // [slot][256][128], [slot][256] {m, l}
+    float *tile_sum;               // [slot][tile_pairs][128], [slot][tile_pairs] {m, l}
     float2 *tile_ml;
 };
 enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kRtRun, kRtLonger, kTlHeader };
-constexpr int kTlPairs = 256;     // (row, head) pairs to a tile
 constexpr int kTlShortPairs = 32; // requests of up to so many keep their own rows in the row kernel
 constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 
@@ -118,7 +119,7 @@ __device__ __forceinline__ OwnShape short_shape(const PagedAttnParams &p, int32_
     return s;
 }
 
-// What one tile covers, as the schedule lays it down. Key steps are of 128.
+// What one tile covers, as the schedule lays it down.
 struct __align__(16) TileShape {
     int32_t request;     // -1: rows of the short list, prefix only
     int32_t row0, rows;  // in the batch, or in that list
@@ -982,7 +983,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
                 const int32_t tile = p.by_tile_rows.div(listed);
                 const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
                 const int32_t u0 = unit * p.kh + kv * steps, c0 = runs.cta_of(u0);
-                shared = PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, kTlPairs,
+                shared = PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, p.tile_pairs,
                                   (listed - tile * p.tile_rows) * p.group + in_group, steps ? runs.cta_of(u0 + steps - 1) - c0 + 1 : 0};
             }
         }
@@ -1013,8 +1014,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         const int32_t kv = (cut - unit * p.kh) / steps, u0 = unit * p.kh + kv * steps, before = runs.start(c - 1);
         if (cut == u0 || before > u0) continue;
         // CTA c - 1 has this tile as its last run unless it begins with it; the others begin with it.
-        shared = PartList{p.tile_sum, p.tile_ml, 2 * (c - 1) + (before == u0 ? 0 : 1), 0, kTlPairs, 0, 1};
-        own = PartList{p.tile_sum, p.tile_ml, 2 * c, 2, kTlPairs, 0, runs.cta_of(u0 + steps - 1) - c + 1};
+        shared = PartList{p.tile_sum, p.tile_ml, 2 * (c - 1) + (before == u0 ? 0 : 1), 0, p.tile_pairs, 0, 1};
+        own = PartList{p.tile_sum, p.tile_ml, 2 * c, 2, p.tile_pairs, 0, runs.cta_of(u0 + steps - 1) - c + 1};
         const int32_t row0 = p.tile_shape[tile].row0, pairs = p.tile_shape[tile].rows * p.group;
 #pragma unroll 1
         for (int32_t pair = (n & 7) * 32 + warp; pair < min((n & 7) * 32 + 32, pairs); pair += 8) {

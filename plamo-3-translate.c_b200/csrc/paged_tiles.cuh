@@ -14,6 +14,7 @@ namespace plamo {
 // of the tensor pipe (128 x 128 x 128 at 4096 multiply-adds a cycle) and
 // 1024 cycles of exponentials (16 a cycle): the halves run half a step apart,
 // so that one's exponentials cover the other's products.
+constexpr int kTlPairs = 256;
 constexpr int kTlKeys = 128;
 constexpr int kTlThreads = 352;  // 8 softmax warps, copies, products, mending
 constexpr int kTlCopies = 8, kTlProducts = 9, kTlMending = 10;  // warps; 0-7 are softmax
@@ -33,11 +34,11 @@ __device__ __forceinline__ TileShape prompt_tile(const PagedAttnParams &p, int32
     const int32_t last = s.at0 + s.rows - 1;
     if (last < 0) return s;  // rows before own row 0 see nothing
     const int32_t held = max(s.at0, 0);
-    s.pre1 = (p.prefix + kTlKeys - 1) / kTlKeys;
-    s.pre0 = p.window ? min(max(p.prefix + held - p.window + 1, 0) / kTlKeys, s.pre1) : 0;
+    s.pre1 = (p.prefix + p.tile_keys - 1) / p.tile_keys;
+    s.pre0 = p.window ? min(max(p.prefix + held - p.window + 1, 0) / p.tile_keys, s.pre1) : 0;
     s.own_limit = min(last + 1, o.length);
-    s.own1 = (s.own_limit + kTlKeys - 1) / kTlKeys;
-    s.own0 = p.window ? min(max(held - p.window + 1, 0) / kTlKeys, s.own1) : 0;
+    s.own1 = (s.own_limit + p.tile_keys - 1) / p.tile_keys;
+    s.own0 = p.window ? min(max(held - p.window + 1, 0) / p.tile_keys, s.own1) : 0;
     return s;
 }
 
@@ -82,8 +83,8 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     if (p.tile_rows && p.prefix) {
         pre_tiles = p.by_tile_rows.div(all_short + p.tile_rows - 1);
         pre.request = -1;
-        pre.pre1 = (p.prefix + kTlKeys - 1) / kTlKeys;
-        if (p.window && first_at != INT32_MAX) pre.pre0 = min(max(p.prefix + first_at - p.window + 1, 0) / kTlKeys, pre.pre1);
+        pre.pre1 = (p.prefix + p.tile_keys - 1) / p.tile_keys;
+        if (p.window && first_at != INT32_MAX) pre.pre0 = min(max(p.prefix + first_at - p.window + 1, 0) / p.tile_keys, pre.pre1);
     }
     const int32_t pre_steps = pre.steps();
     const int64_t total = static_cast<int64_t>(pre_tiles) * pre_steps + all_steps;
@@ -648,6 +649,247 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     if (warp == kTlProducts) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---- FP32 tiles ------------------------------------------------------------------------------
+// FP32 has no products on the tensor cores, so these tiles run on the CUDA
+// cores, 64 pairs by steps of 64 keys (a page), 128 threads, two CTAs to an SM
+// so that one multiplies while the other waits for its copies. Both products
+// are register-tiled: thread (ty, tx) of 8 x 16 holds the scores of pairs 8 ty
+// to 8 ty + 7 with keys tx + 16 j (128 multiply-adds to 12 shared loads of 16
+// bytes) and the sums of the same pairs in dimensions 4 tx and 64 + 4 tx (64 to
+// 4). Bound: 128 multiply-adds a cycle and SM, 8192 cycles for a step's two
+// products. (Three BF16 terms to an operand on tcgen05 would be bound by six
+// products each, 3072 cycles, but a long sum there drifts by 2^-24 a product.)
+constexpr int kTfPairs = 64, kTfKeys = 64, kTfThreads = 128;
+constexpr int kTfTile = kTfKeys * kPgDim * 4;  // keys, values or queries
+constexpr int kTfSmem = 1024 + 3 * kTfTile + kTfPairs * kTfKeys * 4;
+
+// A 16-byte piece of row r: the copy engine's swizzle; the queries' rows r and
+// r + 8, read together, lie apart too; the weights' keys are rows.
+__device__ __forceinline__ const float4 *tf_piece(const unsigned char *base, int r, int c) {
+    return reinterpret_cast<const float4 *>(base + (c >> 3) * (kTfKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ float4 *tf_query(unsigned char *base, int r, int c) {
+    return reinterpret_cast<float4 *>(base + r * 512 + ((c ^ ((r + (r >> 3)) & 7)) << 4));
+}
+__device__ __forceinline__ float4 *tf_weight(unsigned char *base, int key, int c) {
+    return reinterpret_cast<float4 *>(base + key * (kTfPairs * 4) + ((c ^ (key & 15)) << 4));
+}
+
+__global__ void __launch_bounds__(kTfThreads, 2)
+    paged_tile_f32_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
+    extern __shared__ __align__(128) unsigned char tf_smem[];
+    __shared__ __align__(8) uint64_t full[2];  // keys, values
+    __shared__ int64_t pair_query[kTfPairs], pair_out[kTfPairs];
+    __shared__ int32_t pair_at[kTfPairs];
+    unsigned char *base = reinterpret_cast<unsigned char *>(
+        (reinterpret_cast<uintptr_t>(tf_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char *const tile_at[2] = {base, base + kTfTile};
+    unsigned char *const queries = base + 2 * kTfTile, *const weights = base + 3 * kTfTile;
+    const int tid = threadIdx.x, lane = tid & 31, tx = tid & 15, ty = tid >> 4;
+    if (tid == 0) {
+        mbar_init(&full[0], 1);
+        mbar_init(&full[1], 1);
+        fence_barrier_init();
+        prefetch_tensormap(&map);
+    }
+    __syncthreads();
+    pdl_launch_dependents();
+    pdl_wait();
+    const int32_t ctas = p.header[kTlCtas], cta = static_cast<int32_t>(blockIdx.x);
+    const int32_t tiles = p.header[kTlTiles], pre_tiles = p.header[kTlPreTiles];
+    if (cta >= ctas) return;
+    const Runs runs = tile_runs(p);
+    TileWalk w{};
+    w.unit = runs.start(cta);
+    w.end = runs.start(cta + 1);
+    w.tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles), p.by_kh.div(w.unit));
+    bool ok = true;
+    uint32_t phase = 0;
+#pragma unroll 1
+    for (bool begins = true; ok && walk_next(p, w); w.unit += w.steps, begins = false) {
+        const TileShape s = p.tile_shape[w.tile];
+        const int32_t pre_steps = s.pre1 - s.pre0, pairs = s.rows * p.group;
+        // Step n's page, first key and the key from which on nothing is seen.
+        const auto key0_of = [&](int32_t step) { return (step >= pre_steps ? s.own0 + step - pre_steps : s.pre0 + step) * kTfKeys; };
+        const auto copy = [&](int32_t n, int kind) {  // one thread
+            const int32_t step = w.step + n, page = key0_of(step) / kTfKeys;
+            int32_t id = step >= pre_steps ? p.tables[static_cast<uint64_t>(s.request) * p.table_stride + page] : p.prefix_pages[page];
+            if (id < 0 || id >= p.pages) {
+                pg_flag(p.status, PLAMO_PAGED_PAGE);
+                id = p.pages;  // past the pool: reads as zeros
+            }
+            mbar_expect_tx(&full[kind], kTfTile);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                tma_load_2d(tile_at[kind] + b * kTfKeys * 128, &map, w.head * kPgDim + 32 * b, (id * 2 + kind) * kPgRows, &full[kind]);
+        };
+        __syncthreads();  // the last segment's tiles and tables have been read
+        if (tid == 0) {
+            copy(0, 0);
+            copy(0, 1);
+        }
+        const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles;
+        const int32_t slot = w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
+        if (tid < kTfPairs) {
+            int64_t query = -1, out = -1;
+            int32_t at = -1;
+            if (tid < pairs) {
+                const int32_t local = p.by_group.div(tid), head = w.head * p.group + tid - local * p.group;
+                int32_t row = s.row0 + local;
+                at = s.at0 + local;
+                if (s.request < 0) {
+                    const int4 e = p.short_list[row];
+                    row = e.x;
+                    at = e.y;
+                }
+                query = row * static_cast<int64_t>(p.q_stride) + head * kPgDim;
+                out = whole ? row * static_cast<int64_t>(p.out_stride) + head * kPgDim : (static_cast<int64_t>(slot) * kTfPairs + tid) * kPgDim;
+            }
+            pair_query[tid] = query;
+            pair_out[tid] = out;
+            pair_at[tid] = at;
+        }
+        __syncthreads();
+        {
+            float4 v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {  // a warp to a row of 512 bytes
+                const int64_t src = pair_query[4 * k + (tid >> 5)];
+                v[k] = src >= 0 ? ld4(static_cast<const float *>(p.q) + src + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) *tf_query(queries, 4 * k + (tid >> 5), lane) = v[k];
+        }
+        float o[8][8], m[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o[i][d] = 0.0f;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int32_t n = 0; n < w.steps; ++n) {
+            const int32_t step = w.step + n, key0 = key0_of(step);
+            const bool own = step >= pre_steps;
+            const int32_t limit = own ? s.own_limit : p.prefix;
+            ok = mbar_wait(&full[0], phase);
+            if (__syncthreads_or(!ok)) {
+                ok = false;
+                break;
+            }
+            float x[8][4];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
+#pragma unroll 2
+            for (int c = 0; c < kPgDim / 4; ++c) {
+                float4 k[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) k[j] = *tf_piece(tile_at[0], tx + 16 * j, c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float4 q = *tf_query(queries, 8 * ty + i, c);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        x[i][j] = fmaf(q.w, k[j].w, fmaf(q.z, k[j].z, fmaf(q.y, k[j].y, fmaf(q.x, k[j].x, x[i][j]))));
+                }
+            }
+            // Keys that each pair sees, of this step's: [lo, hi).
+            int32_t lo[8], hi[8];
+            bool hidden = false, move = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int32_t at = pair_at[8 * ty + i], place = own ? at : p.prefix + at;
+                lo[i] = p.window ? max(place - p.window + 1 - key0, 0) : 0;
+                hi[i] = at < 0 ? 0 : min((own ? min(at + 1, limit) : limit) - key0, kTfKeys);
+                hidden |= lo[i] > 0 || hi[i] < kTfKeys;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int key = tx + 16 * j;
+                    x[i][j] = key >= lo[i] && key < hi[i] ? x[i][j] * p.scale2 : -INFINITY;
+                    move |= x[i][j] > m[i] + kLazy;
+                }
+            }
+            // (the pairs of a thread are those of 16 lanes; both halves of a warp take the turn together)
+            if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float top = fmaxf(fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])), m[i]);
+#pragma unroll
+                    for (int b = 1; b < 16; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+                    const float corr = top == -INFINITY ? 1.0f : pg_exp2(m[i] - top);
+                    m[i] = top;
+                    l[i] *= corr;
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) o[i][d] *= corr;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    y[i] = m[i] == -INFINITY ? 0.0f : pg_exp2(x[i][j] - m[i]);
+                    l[i] += y[i];
+                }
+                *tf_weight(weights, tx + 16 * j, 2 * ty) = make_float4(y[0], y[1], y[2], y[3]);
+                *tf_weight(weights, tx + 16 * j, 2 * ty + 1) = make_float4(y[4], y[5], y[6], y[7]);
+            }
+            ok = mbar_wait(&full[1], phase);
+            if (__syncthreads_or(!ok)) {  // the weights are there, and the keys have been read
+                ok = false;
+                break;
+            }
+            if (tid == 0 && n + 1 < w.steps) copy(n + 1, 0);
+            const auto add = [&](int key, bool all) {
+                const float4 a = *tf_weight(weights, key, 2 * ty), b = *tf_weight(weights, key, 2 * ty + 1);
+                const float4 u = *tf_piece(tile_at[1], key, tx), v = *tf_piece(tile_at[1], key, 16 + tx);
+                const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, z[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (all || (key >= lo[i] && key < hi[i])) {
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) o[i][d] = fmaf(y[i], z[d], o[i][d]);
+                    }
+            };
+            // Where some pair does not see a key, its value, whatever it is, is left out for that pair.
+            if (__any_sync(0xffffffffu, hidden)) {
+#pragma unroll 1
+                for (int key = 0; key < kTfKeys; ++key) add(key, false);
+            } else {
+#pragma unroll 4
+                for (int key = 0; key < kTfKeys; ++key) add(key, true);
+            }
+            __syncthreads();  // values and weights have been read
+            if (tid == 0 && n + 1 < w.steps) copy(n + 1, 1);
+            phase ^= 1u;
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float sum = l[i];
+#pragma unroll
+            for (int b = 1; b < 16; b <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
+            const int pair = 8 * ty + i;
+            const int64_t to = pair_out[pair];
+            if (to < 0) continue;
+            const float inv = !whole ? 1.0f : m[i] == -INFINITY ? 0.0f : 1.0f / sum;
+            float *dst = (whole ? static_cast<float *>(p.out) : p.tile_sum) + to + 4 * tx;
+            *reinterpret_cast<float4 *>(dst) = make_float4(o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
+            *reinterpret_cast<float4 *>(dst + 64) = make_float4(o[i][4] * inv, o[i][5] * inv, o[i][6] * inv, o[i][7] * inv);
+            if (!whole && tx == 0) p.tile_ml[static_cast<int64_t>(slot) * kTfPairs + pair] = make_float2(m[i], sum);
+        }
+    }
+    if (!ok && tid == 0) {  // copies in flight land before the CTA ends
+        pg_flag(p.status, PLAMO_PAGED_FAILED);
+        mbar_wait(&full[0], phase);
+        mbar_wait(&full[1], phase);
     }
 }
 

@@ -26,37 +26,60 @@ class Plan(NamedTuple):
     summary: object    # [4] status bits, new rows, free-list entries used so far, longest length
 
 
+_t = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _t
+    if _t is None:
+        import torch
+        _t = torch
+    return _t
 
 
 def _stream(torch, device):
-    return torch.cuda.current_stream(device).cuda_stream or 1  # 0 names the context's own stream there
+    """torch's current stream of device index `device`; 0 would name the context's own stream, 1 is the default one."""
+    return torch.cuda.current_stream(device).cuda_stream or 1
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+# The checks sit on the path of calls that take a few microseconds in all: plain
+# comparisons, messages only when one fails.
 
-
-def _ints(torch, t, shape, name):
-    _need(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and
-          (shape is None or tuple(t.shape) == shape), f"{name}: a contiguous int32 tensor on the GPU"
-          + (f" of shape {shape}" if shape else ""))
+def _ints(torch, t, count, device, name):
+    if t.dtype != torch.int32 or t.get_device() != device or not t.is_contiguous() or (count >= 0 and t.numel() != count):
+        raise ValueError(f"{name}: a contiguous int32 tensor on GPU {device}" + (f" with {count} entries" if count >= 0 else ""))
 
 
 def _type(torch, t, name):
     if t.dtype == torch.bfloat16:
         return _abi.PAGED_BF16
-    _need(t.dtype == torch.float32, f"{name}: BF16 or FP32")
+    if t.dtype != torch.float32:
+        raise ValueError(f"{name}: BF16 or FP32")
     return _abi.PAGED_FP32
 
 
 def _pool(torch, pool):
-    _need(pool.dim() == 5 and tuple(pool.shape[1:3]) == (2, ROWS) and pool.shape[4] == DIM and pool.is_cuda and
-          pool.is_contiguous(), f"pool: a contiguous [pages, 2, {ROWS}, kv_heads, {DIM}] tensor on the GPU")
-    return _type(torch, pool, "pool"), pool.shape[0], pool.shape[3]
+    """(type, pages, kv_heads, device index) of a pool."""
+    if pool.dim() != 5 or not pool.is_contiguous() or pool.get_device() < 0:
+        raise ValueError(f"pool: a contiguous [pages, 2, {ROWS}, kv_heads, {DIM}] tensor on the GPU")
+    pages, two, rows, kv_heads, dim = pool.shape
+    if two != 2 or rows != ROWS or dim != DIM:
+        raise ValueError(f"pool: a contiguous [pages, 2, {ROWS}, kv_heads, {DIM}] tensor on the GPU")
+    return _type(torch, pool, "pool"), pages, kv_heads, pool.get_device()
+
+
+def _tables(torch, tables, requests, device):
+    if tables.dim() != 2 or tables.shape[0] != requests:
+        raise ValueError("tables: [requests, pages per request]")
+    _ints(torch, tables, -1, device, "tables")
+    return tables.shape[1]
+
+
+def _status(torch, status, device):
+    if status is None:
+        return 0
+    _ints(torch, status, 1, device, "status")
+    return status.data_ptr()
 
 
 def _run(backend, call, args):
@@ -65,13 +88,6 @@ def _run(backend, call, args):
         raise ValueError(backend.info().note.decode())
     if rc < 0:
         raise RuntimeError(backend.info().note.decode())
-
-
-def _same_device(*tensors):
-    first = tensors[0].device
-    for t in tensors[1:]:
-        _need(t is None or t.device == first, "all tensors must be on one GPU")
-    return first
 
 
 def plan(backend, held, added, tables, free_pages, rows, base=0, after=None):
@@ -86,31 +102,29 @@ def plan(backend, held, added, tables, free_pages, rows, base=0, after=None):
     slot is then -1, every other state as before.
     """
     torch = _torch()
-    requests = held.shape[0]
-    _ints(torch, held, (requests,), "held")
-    _ints(torch, added, (requests,), "added")
-    _need(tables.dim() == 2 and tables.shape[0] == requests, "tables: [requests, pages per request]")
-    _ints(torch, tables, None, "tables")
-    _need(free_pages.dim() == 1, "free_pages: one dimension")
-    _ints(torch, free_pages, None, "free_pages")
-    _need(rows >= 0, "rows: not negative")
-    device = _same_device(held, added, tables, free_pages, None if after is None else after.summary)
-    # One allocation, a 16-byte boundary for each part.
-    sizes = [requests, requests + 1, rows, rows, 4]
-    offsets, total = [], 0
-    for n in sizes:
-        offsets.append(total)
-        total += -(-n // 4) * 4
-    buffer = torch.empty(total, dtype=torch.int32, device=device)
-    parts = [buffer[o:o + n] for o, n in zip(offsets, sizes)]
+    requests, device = held.numel(), held.get_device()
+    if device < 0 or rows < 0:
+        raise ValueError("held: on the GPU; rows: not negative")
+    _ints(torch, held, requests, device, "held")
+    _ints(torch, added, requests, device, "added")
+    _ints(torch, free_pages, -1, device, "free_pages")
+    if free_pages.dim() != 1:
+        raise ValueError("free_pages: one dimension")
+    stride = _tables(torch, tables, requests, device)
+    head = 0
+    if after is not None:
+        _ints(torch, after.summary, 4, device, "after.summary")
+        head = after.summary.data_ptr() + 8
+    buffer = torch.empty(2 * requests + 2 * rows + 5, dtype=torch.int32, device=held.device)
     at = buffer.data_ptr()
-    p = [at + 4 * o for o in offsets]
-    head = 0 if after is None else after.summary.data_ptr() + 8
-    args = _abi.PagedPlanArgs(held.data_ptr(), added.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), head, p[0], p[1],
-                              p[2], p[3], p[4], requests, tables.shape[1], free_pages.shape[0], rows, base,
+    starts = at + 4 * requests
+    slots = starts + 4 * requests + 4
+    positions = slots + 4 * rows
+    args = _abi.PagedPlanArgs(held.data_ptr(), added.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), head, at, starts,
+                              slots, positions, positions + 4 * rows, requests, stride, free_pages.numel(), rows, base,
                               _stream(torch, device))
     _run(backend, backend.lib.plamo_paged_plan, args)
-    return Plan(*parts)
+    return Plan(*buffer.unsafe_split_with_sizes((requests, requests + 1, rows, rows, 4)))  # (split takes 3 us more)
 
 
 def store(backend, qkv, pool, slots, positions, q_norm, k_norm, table, status=None):
@@ -123,29 +137,28 @@ def store(backend, qkv, pool, slots, positions, q_norm, k_norm, table, status=No
     queries, [rows, query_heads, 128] of the pool's type.
     """
     torch = _torch()
-    kind, pages, kv_heads = _pool(torch, pool)
-    _need(qkv.dim() == 2 and qkv.shape[1] % DIM == 0 and qkv.is_cuda and (qkv.stride(1) == 1 or qkv.shape[0] == 0),
-          f"qkv: [rows, heads * {DIM}] on the GPU, each row contiguous")
-    rows, heads = qkv.shape[0], qkv.shape[1] // DIM
-    query_heads = heads - 2 * kv_heads
-    _need(query_heads > 0, "qkv: no query heads beside the pool's kv_heads")
+    kind, pages, kv_heads, device = _pool(torch, pool)
+    if qkv.dim() != 2 or qkv.get_device() != device:
+        raise ValueError(f"qkv: [rows, heads * {DIM}] on the pool's GPU")
+    rows, width = qkv.shape
+    row_stride, step = qkv.stride()
+    query_heads = width // DIM - 2 * kv_heads
+    if width % DIM or query_heads <= 0 or (step != 1 and rows):
+        raise ValueError(f"qkv: contiguous rows of {DIM} * (query heads + 2 * {kv_heads}) entries")
     qkv_kind = _type(torch, qkv, "qkv")
-    _ints(torch, slots, (rows,), "slots")
-    _ints(torch, positions, (rows,), "positions")
+    _ints(torch, slots, rows, device, "slots")
+    _ints(torch, positions, rows, device, "positions")
     for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _need(t.dtype == torch.bfloat16 and tuple(t.shape) == (DIM,) and t.is_cuda and t.is_contiguous(),
-              f"{name}: a contiguous BF16 [{DIM}] tensor on the GPU")
-    _need(table.dtype == torch.float32 and table.dim() == 2 and table.shape[1] == DIM and table.is_cuda and
-          table.is_contiguous(), f"table: a contiguous FP32 [positions, {DIM}] tensor on the GPU")
-    if status is not None:
-        _ints(torch, status, (1,), "status")
-    device = _same_device(qkv, pool, slots, positions, q_norm, k_norm, table, status)
-    q = torch.empty(rows, query_heads, DIM, dtype=pool.dtype, device=device)
+        if t.dtype != torch.bfloat16 or t.numel() != DIM or t.get_device() != device or not t.is_contiguous():
+            raise ValueError(f"{name}: a contiguous BF16 [{DIM}] tensor on the pool's GPU")
+    if (table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != DIM or table.get_device() != device or
+            not table.is_contiguous()):
+        raise ValueError(f"table: a contiguous FP32 [positions, {DIM}] tensor on the pool's GPU")
+    q = torch.empty(rows, query_heads, DIM, dtype=pool.dtype, device=pool.device)
     args = _abi.PagedStoreArgs(qkv.data_ptr(), pool.data_ptr(), q.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-                               q_norm.data_ptr(), k_norm.data_ptr(), table.data_ptr(),
-                               0 if status is None else status.data_ptr(), rows, max(qkv.stride(0), heads * DIM) if rows <= 1
-                               else qkv.stride(0), query_heads * DIM, pages, table.shape[0], query_heads, kv_heads, qkv_kind,
-                               kind, _stream(torch, device))
+                               q_norm.data_ptr(), k_norm.data_ptr(), table.data_ptr(), _status(torch, status, device), rows,
+                               row_stride if rows > 1 else width, query_heads * DIM, pages, table.shape[0], query_heads,
+                               kv_heads, qkv_kind, kind, _stream(torch, device))
     _run(backend, backend.lib.plamo_paged_store, args)
     return q
 
@@ -161,43 +174,46 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
     the scores, 1 / sqrt(128) unless given. Returns `out`, allocated if None.
     """
     torch = _torch()
-    kind, pages, kv_heads = _pool(torch, pool)
-
-    def rows_of(t, name):
-        _need(t.dim() == 3 and t.shape[2] == DIM and t.is_cuda and t.dtype == pool.dtype and
-              (t.shape[0] == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == DIM))),
-              f"{name}: [rows, query_heads, {DIM}] of the pool's type on the GPU, each row contiguous")
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * DIM
-
-    q_stride = rows_of(q, "q")
-    rows, query_heads = q.shape[0], q.shape[1]
-    requests = lengths.shape[0]
-    _ints(torch, lengths, (requests,), "lengths")
-    _ints(torch, starts, (requests + 1,), "starts")
-    _need(tables.dim() == 2 and tables.shape[0] == requests, "tables: [requests, pages per request]")
-    _ints(torch, tables, None, "tables")
-    _need(prefix_rows >= 0 and window >= 0, "prefix_rows and window: not negative")
+    kind, pages, kv_heads, device = _pool(torch, pool)
+    q_stride = _rows(torch, q, pool, device, "q")
+    rows, query_heads, _ = q.shape
+    requests = lengths.numel()
+    _ints(torch, lengths, requests, device, "lengths")
+    _ints(torch, starts, requests + 1, device, "starts")
+    stride = _tables(torch, tables, requests, device)
+    if prefix_rows < 0 or window < 0:
+        raise ValueError("prefix_rows and window: not negative")
+    prefix = 0
     if prefix_rows:
-        _need(prefix_pages is not None and prefix_pages.dim() == 1 and prefix_pages.shape[0] * ROWS >= prefix_rows,
-              "prefix_pages: one dimension, pages for prefix_rows rows")
-        _ints(torch, prefix_pages, None, "prefix_pages")
-    if status is not None:
-        _ints(torch, status, (1,), "status")
+        if prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.numel() * ROWS < prefix_rows:
+            raise ValueError("prefix_pages: one dimension, pages for prefix_rows rows")
+        _ints(torch, prefix_pages, -1, device, "prefix_pages")
+        prefix = prefix_pages.data_ptr()
     if out is None:
-        out = torch.empty(rows, query_heads, DIM, dtype=pool.dtype, device=q.device)
+        out = torch.empty(rows, query_heads, DIM, dtype=pool.dtype, device=pool.device)
+        out_stride = query_heads * DIM
     else:
-        _need(out.shape == q.shape, "out: of q's shape")
-    out_stride = rows_of(out, "out")
-    device = _same_device(q, pool, out, starts, lengths, tables, prefix_pages, status)
+        if out.shape != q.shape:
+            raise ValueError("out: of q's shape")
+        out_stride = _rows(torch, out, pool, device, "out")
     args = _abi.PagedAttentionArgs(q.data_ptr(), pool.data_ptr(), out.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
-                                   tables.data_ptr(), prefix_pages.data_ptr() if prefix_rows else 0, 0, 0,
-                                   0 if status is None else status.data_ptr(), rows, q_stride, out_stride, requests,
-                                   tables.shape[1], prefix_rows, pages, window, query_heads, kv_heads, kind,
+                                   tables.data_ptr(), prefix, 0, 0, _status(torch, status, device), rows, q_stride, out_stride,
+                                   requests, stride, prefix_rows, pages, window, query_heads, kv_heads, kind,
                                    DIM ** -0.5 if scale is None else scale, _stream(torch, device))
     size = backend.lib.plamo_paged_attention_workspace(backend.ctx, ctypes.byref(args))
     if not size:
         raise ValueError(backend.info().note.decode())
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=pool.device)
     args.workspace, args.workspace_bytes = workspace.data_ptr(), size
     _run(backend, backend.lib.plamo_paged_attention, args)
     return out
+
+
+def _rows(torch, t, pool, device, name):
+    """Row stride of [rows, heads, 128] queries or results."""
+    if t.dim() == 3 and t.dtype == pool.dtype and t.get_device() == device:
+        rows, heads, dim = t.shape
+        row, head, step = t.stride()
+        if dim == DIM and (rows == 0 or (step == 1 and (heads == 1 or head == DIM))):
+            return row if rows > 1 else heads * DIM
+    raise ValueError(f"{name}: [rows, query_heads, {DIM}] of the pool's type and GPU, each row contiguous")
