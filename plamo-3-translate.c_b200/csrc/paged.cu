@@ -143,7 +143,6 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.group = p.qh / p.kh;
     p.by_group = FastDiv::of(p.group);
     p.by_kh = FastDiv::of(p.kh);
-    p.by_qh = FastDiv::of(p.qh);
     p.prefix = static_cast<int32_t>(d->prefix_rows);
     p.max_length = static_cast<int32_t>(d->table_stride * kPgRows);
     // A window that reaches back past every row hides nothing.
@@ -181,12 +180,10 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
         (a.tile_rows && !launch(c, "paged_attention tiles", F32 ? paged_tile_f32_kernel : paged_tile_kernel, dim3(a.tile_grid),
                                 dim3(F32 ? kTfThreads : kTlThreads), F32 ? kTfSmem : kTlSmem, stream, true, page_map, p)))
         return false;
-    // Eight warps to a result while one each would leave SMs idle.
-    const uint64_t results = d->rows * d->query_heads, wave = 8ull * context_sms(c);
-    return results <= wave
-               ? launch(c, "paged_attention join", paged_join_kernel<F32, 8>, dim3(static_cast<uint32_t>(results)), dim3(256), 0, stream, true, p)
-               : launch(c, "paged_attention join", paged_join_kernel<F32, 1>,
-                        dim3(static_cast<uint32_t>(std::min(ceil_div(results, 8), wave))), dim3(256), 0, stream, true, p);
+    // A block to eight results of short requests, or to a part of a cut tile.
+    const uint64_t blocks = std::max(d->rows * ceil_div(d->query_heads, 8), static_cast<uint64_t>(4 * a.tile_grid));
+    return launch(c, "paged_attention join", paged_join_kernel<F32>,
+                  dim3(static_cast<uint32_t>(std::min<uint64_t>(blocks, 6ull * context_sms(c)))), dim3(kJoinThreads), 0, stream, true, p);
 }
 
 template <typename In, typename Out>

@@ -39,7 +39,7 @@ struct PagedAttnParams {
     uint64_t q_stride, out_stride, table_stride;
     uint32_t *status;
     int32_t rows, requests, pages, qh, kh, group;
-    FastDiv by_group, by_kh, by_qh;
+    FastDiv by_group, by_kh;
     int32_t prefix, window;  // window: rows seen, 0 for all
     int32_t max_length;      // own rows a page table holds
     float scale2;            // scale * log2(e)
@@ -890,49 +890,62 @@ struct PartList {
     int32_t first, stride, rows, place, count;
     __device__ __forceinline__ int64_t at(int32_t x) const { return static_cast<int64_t>(first + x * stride) * rows + place; }
 };
-// WPH warps work on it, `sub` is this one; every lane returns with the sums
-// over its warp's share of parts, 32 at a time, and the common maximum.
-template <int WPH>
-__device__ __noinline__ void join_parts(const PartList &a, const PartList &b, int32_t sub, float4 &o, float &l, float &top) {
+// Joins eight results, lane y's lists those of result y % 8 (empty where there
+// is none). Warp `sub` of `warps` takes every warps-th part of each, four at a
+// time: a lane weighs one part of one result, then the parts' sums are loaded
+// eight at once. Every lane returns with four dimensions of the sums over its
+// warp's parts, and l and the maximum m over them of its own result.
+__device__ __forceinline__ void join_parts(const PartList &a, const PartList &b, int32_t sub, int32_t warps, float4 (&o)[8], float &l,
+                                           float &m) {
     const int32_t lane = threadIdx.x & 31, all = a.count + b.count;
-    o = make_float4(0.f, 0.f, 0.f, 0.f);
-    top = -INFINITY;
+    const int32_t most = __reduce_max_sync(0xffffffffu, all);
+    m = -INFINITY;
     l = 0.0f;
-    const auto place = [&](int32_t x) { return x < a.count ? a.at(x) : b.at(x - a.count); };
-    for (int32_t x = lane; x < all; x += 32) top = fmaxf(top, (x < a.count ? a.ml : b.ml)[place(x)].x);
-    top = warp_max(top);
-    if (top == -INFINITY) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int32_t x0 = 32 * sub; x0 < all; x0 += 32 * WPH) {
-        // A lane weighs one part, then the parts' sums are loaded eight at once.
-        const int32_t x = x0 + lane;
-        float w = 0.0f, part_l = 0.0f;
+    for (int32_t x0 = sub; x0 < most; x0 += 4 * warps) {
+        const int32_t x = x0 + (lane >> 3) * warps;
+        float2 v = make_float2(-INFINITY, 0.0f);
         const float *from = nullptr;
         if (x < all) {
-            const int64_t here = place(x);
-            const float2 y = (x < a.count ? a.ml : b.ml)[here];
-            w = y.x == -INFINITY ? 0.0f : pg_exp2(y.x - top);
-            part_l = w * y.y;
-            from = (x < a.count ? a.sum : b.sum) + here * kPgDim;
+            const bool first = x < a.count;
+            const int64_t at = first ? a.at(x) : b.at(x - a.count);
+            v = (first ? a.ml : b.ml)[at];
+            from = (first ? a.sum : b.sum) + at * kPgDim;
         }
-        const int32_t some = min(32, all - x0);
-#pragma unroll 1
-        for (int32_t y0 = 0; y0 < some; y0 += 8) {
-            float4 v[8];
+        float top = fmaxf(m, v.x);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float w = v.x == -INFINITY ? 0.0f : pg_exp2(v.x - top), corr = m == -INFINITY ? 0.0f : pg_exp2(m - top);
+        m = top;
+        l = fmaf(w, v.y, l * corr);
+        if (x0 != sub) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = __shfl_sync(0xffffffffu, corr, i);
+                o[i] = make_float4(o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f);
+            }
+        }
+#pragma unroll 2
+        for (int k = 0; k < 32; k += 8) {
+            if (x0 + (k >> 3) * warps >= most) break;
+            float4 u[8];
             float f[8];
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                f[y] = __shfl_sync(0xffffffffu, w, y0 + y);
-                const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), y0 + y));
-                v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (f[y] != 0.0f) v[y] = ld4(src + 4 * lane);
+            for (int i = 0; i < 8; ++i) {
+                f[i] = __shfl_sync(0xffffffffu, w, k + i);
+                const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), k + i));
+                u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (f[i] != 0.0f) u[i] = ld4(src + 4 * lane);
             }
 #pragma unroll
-            for (int y = 0; y < 8; ++y)
-                o = make_float4(fmaf(f[y], v[y].x, o.x), fmaf(f[y], v[y].y, o.y), fmaf(f[y], v[y].z, o.z), fmaf(f[y], v[y].w, o.w));
+            for (int i = 0; i < 8; ++i)
+                o[i] = make_float4(fmaf(f[i], u[i].x, o[i].x), fmaf(f[i], u[i].y, o[i].y), fmaf(f[i], u[i].z, o[i].z), fmaf(f[i], u[i].w, o[i].w));
         }
-        l += warp_sum(part_l);
     }
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
 }
 template <bool F32>
 __device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row, int32_t head, float4 o, float l, float top) {
@@ -943,31 +956,32 @@ __device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row
     else pg_store4(static_cast<uint16_t *>(p.out) + to, o);
 }
 
-// Joins the short requests' rows (WPH warps each: eight where few rows were
-// split into many parts, one where there are rows enough), the prompts' tiles
-// that two or more CTAs shared, and zeroes the rows that see nothing.
-template <bool F32, int WPH>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
-    __shared__ float4 warp_sum_at[WPH][32];
-    __shared__ float warp_l[WPH];
-    const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WPH == 1 ? 0 : warp;
+// Joins the short requests' rows (a block to eight heads of a row, each warp a
+// share of their parts), the prompts' tiles that two or more CTAs shared (a
+// warp to eight pairs), and zeroes the rows that see nothing.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+template <bool F32>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
+    __shared__ float4 warp_sums[kJoinWarps][8][32];
+    __shared__ float2 warp_ml[kJoinWarps][8];
+    const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
     const int32_t tiles = p.tile_rows ? p.header[kTlTiles] : 0, pre_tiles = p.tile_rows ? p.header[kTlPreTiles] : 0;
     const int32_t ctas = p.tile_rows ? p.header[kTlCtas] : 0;
     const Runs runs = tile_runs(p), of_rows = row_runs(p);
-    const int32_t results = p.header[kTlShortRows] * p.qh;
-    const int32_t lanes = WPH == 1 ? gridDim.x * 8 : gridDim.x;  // of results in flight
-    PartList shared, own;
-    float4 o;
+    PartList shared{}, own{};
+    float4 o[8];
     float l, top;
+    const int32_t eights = (p.qh + 7) / 8, items = p.header[kTlShortRows] * eights;
 #pragma unroll 1
-    for (int32_t n = WPH == 1 ? blockIdx.x * 8 + warp : blockIdx.x; n < results; n += lanes) {
-        const int32_t listed = p.by_qh.div(n), head = n - listed * p.qh;
-        const int32_t kv = p.by_group.div(head), in_group = head - kv * p.group;
+    for (int32_t n = blockIdx.x; n < items; n += gridDim.x) {
+        const int32_t listed = n / eights, head0 = 8 * (n - listed * eights), head = head0 + (lane & 7);
         const int4 e = p.short_list[listed];
         shared.count = own.count = 0;
-        if (e.y >= 0) {
-            // The parts of row tile t of request r (or of the prefix) for this head.
+        bool written = false;
+        if (e.y >= 0 && head < p.qh) {
+            const int32_t kv = p.by_group.div(head), in_group = head - kv * p.group;
+            // The parts of row tile m / row_tile of request r (or of the prefix) for this head.
             const auto row_parts = [&](int32_t r, int32_t m) {
                 const int4 rec = p.row_record[r];
                 const int32_t strip = (m >> p.row_shift) * p.kh + kv, u0 = rec.x + strip * rec.y;
@@ -976,7 +990,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
                                 rec.y ? of_rows.cta_of(u0 + rec.y - 1) - c0 + 1 : 0};
             };
             own = row_parts(e.z, e.w * p.group + in_group);
-            if (own.count == 1 && p.prefix == 0) continue;  // written where it was computed
+            written = own.count == 1 && p.prefix == 0;  // where it was computed
             if (p.prefix_tiles) {
                 shared = row_parts(p.requests, e.x * p.group + in_group);
             } else if (pre_tiles && ctas) {
@@ -987,42 +1001,52 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
                                   (listed - tile * p.tile_rows) * p.group + in_group, steps ? runs.cta_of(u0 + steps - 1) - c0 + 1 : 0};
             }
         }
-        join_parts<WPH>(shared, own, sub, o, l, top);
-        if constexpr (WPH > 1) {  // the warps' sums, in order
-            warp_sum_at[sub][lane] = o;
-            if (lane == 0) warp_l[sub] = l;
-            __syncthreads();
-            if (sub == 0) {
+        const uint32_t skip = __ballot_sync(0xffffffffu, written || head >= p.qh);
+        if ((skip & 0xffu) == 0xffu) continue;  // (the same for all warps)
+        join_parts(shared, own, warp, kJoinWarps, o, l, top);
 #pragma unroll
-                for (int w = 1; w < WPH; ++w) {
-                    const float4 v = warp_sum_at[w][lane];
-                    o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-                    l += warp_l[w];
-                }
-            }
+        for (int i = 0; i < 8; ++i) warp_sums[warp][i][lane] = o[i];
+        if (lane < 8) warp_ml[warp][lane] = make_float2(top, l);
+        __syncthreads();
+        // Warp y puts result y together, the warps' shares in order.
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        top = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, warp_ml[i][warp].x);
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i) {
+            const float2 ml = warp_ml[i][warp];
+            const float f = ml.x == -INFINITY ? 0.0f : pg_exp2(ml.x - top);
+            const float4 u = warp_sums[i][warp][lane];
+            v = make_float4(fmaf(f, u.x, v.x), fmaf(f, u.y, v.y), fmaf(f, u.z, v.z), fmaf(f, u.w, v.w));
+            l = fmaf(f, ml.y, l);
         }
-        if (sub == 0) join_store<F32>(p, e.x, head, o, l, top);
-        if constexpr (WPH > 1) __syncthreads();
+        if (!((skip >> warp) & 1u)) join_store<F32>(p, e.x, head0 + warp, v, l, top);
+        __syncthreads();
     }
-    // Prompts' tiles that a CTA's end cuts: the first such end does the tile, 32 pairs to a block.
+    // Prompts' tiles that a CTA's end cuts: the first such end does the tile.
+    const int32_t blocks = p.tile_pairs / (8 * kJoinWarps);  // to a tile
 #pragma unroll 1
-    for (int32_t n = blockIdx.x; n < 8 * (ctas - 1); n += gridDim.x) {
-        const int32_t c = n / 8 + 1, cut = runs.start(c);
+    for (int32_t n = blockIdx.x; n < blocks * (ctas - 1); n += gridDim.x) {
+        const int32_t c = n / blocks + 1, pair0 = ((n - (c - 1) * blocks) * kJoinWarps + warp) * 8, cut = runs.start(c);
         const int32_t tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles), p.by_kh.div(cut));
         if (tile < pre_tiles) continue;
         const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
         const int32_t kv = (cut - unit * p.kh) / steps, u0 = unit * p.kh + kv * steps, before = runs.start(c - 1);
-        if (cut == u0 || before > u0) continue;
-        // CTA c - 1 has this tile as its last run unless it begins with it; the others begin with it.
-        shared = PartList{p.tile_sum, p.tile_ml, 2 * (c - 1) + (before == u0 ? 0 : 1), 0, p.tile_pairs, 0, 1};
-        own = PartList{p.tile_sum, p.tile_ml, 2 * c, 2, p.tile_pairs, 0, runs.cta_of(u0 + steps - 1) - c + 1};
         const int32_t row0 = p.tile_shape[tile].row0, pairs = p.tile_shape[tile].rows * p.group;
-#pragma unroll 1
-        for (int32_t pair = (n & 7) * 32 + warp; pair < min((n & 7) * 32 + 32, pairs); pair += 8) {
-            shared.place = own.place = pair;
-            join_parts<1>(shared, own, 0, o, l, top);
-            const int32_t i = p.by_group.div(pair);
-            join_store<F32>(p, row0 + i, kv * p.group + pair - i * p.group, o, l, top);
+        if (cut == u0 || before > u0 || pair0 >= pairs) continue;
+        // CTA c - 1 has this tile as its last run unless it begins with it; the others begin with it.
+        const int32_t pair = pair0 + (lane & 7), there = pair < pairs;
+        shared = PartList{p.tile_sum, p.tile_ml, 2 * (c - 1) + (before == u0 ? 0 : 1), 0, p.tile_pairs, pair, there};
+        own = PartList{p.tile_sum, p.tile_ml, 2 * c, 2, p.tile_pairs, pair, there * (runs.cta_of(u0 + steps - 1) - c + 1)};
+        join_parts(shared, own, 0, 1, o, l, top);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float li = __shfl_sync(0xffffffffu, l, i), ti = __shfl_sync(0xffffffffu, top, i);
+            if (pair0 + i >= pairs) break;
+            const int32_t row = p.by_group.div(pair0 + i);
+            join_store<F32>(p, row0 + row, kv * p.group + pair0 + i - row * p.group, o[i], li, ti);
         }
     }
     // Rows that no request has, and tiles without a key.

@@ -664,7 +664,8 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 // products each, 3072 cycles, but a long sum there drifts by 2^-24 a product.)
 constexpr int kTfPairs = 64, kTfKeys = 64, kTfThreads = 128;
 constexpr int kTfTile = kTfKeys * kPgDim * 4;  // keys, values or queries
-constexpr int kTfSmem = 1024 + 3 * kTfTile + kTfPairs * kTfKeys * 4;
+constexpr int kTfTables = 3 * kTfTile + kTfPairs * kTfKeys * 4;  // barriers and the pairs' rows behind the tiles
+constexpr int kTfSmem = kTfTables + 16 + 2 * kTfPairs * 4;       // no static part: two CTAs just fit an SM
 
 // A 16-byte piece of row r: the copy engine's swizzle; the queries' rows r and
 // r + 8, read together, lie apart too; the weights' keys are rows.
@@ -672,20 +673,29 @@ __device__ __forceinline__ const float4 *tf_piece(const unsigned char *base, int
     return reinterpret_cast<const float4 *>(base + (c >> 3) * (kTfKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 __device__ __forceinline__ float4 *tf_query(unsigned char *base, int r, int c) {
-    return reinterpret_cast<float4 *>(base + r * 512 + ((c ^ ((r + (r >> 3)) & 7)) << 4));
+    return reinterpret_cast<float4 *>(base + r * 512 + (c >> 3) * 128 + (((c & 7) ^ ((r + (r >> 3)) & 7)) << 4));
 }
 __device__ __forceinline__ float4 *tf_weight(unsigned char *base, int key, int c) {
     return reinterpret_cast<float4 *>(base + key * (kTfPairs * 4) + ((c ^ (key & 15)) << 4));
 }
 
+__device__ __forceinline__ float4 lds_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 __global__ void __launch_bounds__(kTfThreads, 2)
     paged_tile_f32_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
-    extern __shared__ __align__(128) unsigned char tf_smem[];
-    __shared__ __align__(8) uint64_t full[2];  // keys, values
-    __shared__ int64_t pair_query[kTfPairs], pair_out[kTfPairs];
-    __shared__ int32_t pair_at[kTfPairs];
-    unsigned char *base = reinterpret_cast<unsigned char *>(
-        (reinterpret_cast<uintptr_t>(tf_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+    extern __shared__ __align__(1024) unsigned char tf_smem[];
+    unsigned char *const base = tf_smem;
+    uint64_t *const full = reinterpret_cast<uint64_t *>(base + kTfTables);           // keys, values
+    int32_t *const pair_row = reinterpret_cast<int32_t *>(base + kTfTables + 16);    // batch row, -1: no such pair
+    int32_t *const pair_at = pair_row + kTfPairs;                                    // own row
+    if (smem_u32(base) & 1023u) {  // the copies' swizzle needs it; dynamic shared memory starts so when there is no other
+        pg_flag(p.status, PLAMO_PAGED_FAILED);
+        return;
+    }
     unsigned char *const tile_at[2] = {base, base + kTfTile};
     unsigned char *const queries = base + 2 * kTfTile, *const weights = base + 3 * kTfTile;
     const int tid = threadIdx.x, lane = tid & 31, tx = tid & 15, ty = tid >> 4;
@@ -734,31 +744,29 @@ __global__ void __launch_bounds__(kTfThreads, 2)
         const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles;
         const int32_t slot = w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
         if (tid < kTfPairs) {
-            int64_t query = -1, out = -1;
-            int32_t at = -1;
+            int32_t row = -1, at = 0;
             if (tid < pairs) {
-                const int32_t local = p.by_group.div(tid), head = w.head * p.group + tid - local * p.group;
-                int32_t row = s.row0 + local;
+                const int32_t local = p.by_group.div(tid);
+                row = s.row0 + local;
                 at = s.at0 + local;
                 if (s.request < 0) {
                     const int4 e = p.short_list[row];
                     row = e.x;
                     at = e.y;
                 }
-                query = row * static_cast<int64_t>(p.q_stride) + head * kPgDim;
-                out = whole ? row * static_cast<int64_t>(p.out_stride) + head * kPgDim : (static_cast<int64_t>(slot) * kTfPairs + tid) * kPgDim;
             }
-            pair_query[tid] = query;
-            pair_out[tid] = out;
+            pair_row[tid] = row;
             pair_at[tid] = at;
         }
+        const auto head_of = [&](int32_t pair) { return w.head * p.group + pair - p.by_group.div(pair) * p.group; };
         __syncthreads();
         {
             float4 v[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {  // a warp to a row of 512 bytes
-                const int64_t src = pair_query[4 * k + (tid >> 5)];
-                v[k] = src >= 0 ? ld4(static_cast<const float *>(p.q) + src + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int32_t pair = 4 * k + (tid >> 5), row = pair_row[pair];
+                v[k] = row >= 0 ? ld4(static_cast<const float *>(p.q) + row * p.q_stride + head_of(pair) * kPgDim + 4 * lane)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int k = 0; k < 16; ++k) *tf_query(queries, 4 * k + (tid >> 5), lane) = v[k];
@@ -787,28 +795,47 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
-#pragma unroll 2
-            for (int c = 0; c < kPgDim / 4; ++c) {
-                float4 k[4];
+            {
+                // Addresses: a row's swizzle and the piece's number join by exclusive or. The next
+                // piece's loads are under way while this one is multiplied.
+                uint32_t k_at[4], q_at[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) k[j] = *tf_piece(tile_at[0], tx + 16 * j, c);
+                for (int j = 0; j < 4; ++j) k_at[j] = smem_u32(tf_piece(tile_at[0], tx + 16 * j, 0));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 q = *tf_query(queries, 8 * ty + i, c);
+                for (int i = 0; i < 8; ++i) q_at[i] = smem_u32(tf_query(queries, 8 * ty + i, 0));
+                float4 k[2][4], q[2][8];
+                const auto load = [&](int box, int c) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        x[i][j] = fmaf(q.w, k[j].w, fmaf(q.z, k[j].z, fmaf(q.y, k[j].y, fmaf(q.x, k[j].x, x[i][j]))));
-                }
+                    for (int j = 0; j < 4; ++j) k[c & 1][j] = lds_f32x4((k_at[j] ^ (c << 4)) + box * (kTfKeys * 128));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) q[c & 1][i] = lds_f32x4((q_at[i] ^ (c << 4)) + box * 128);
+                };
+                load(0, 0);
+#pragma unroll 1
+                for (int box = 0; box < 4; ++box)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        if (c < 7) load(box, c + 1);
+                        else if (box < 3) load(box + 1, 0);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float4 a = q[c & 1][i], b = k[c & 1][j];
+                                x[i][j] = fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, x[i][j]))));
+                            }
+                    }
             }
             // Keys that each pair sees, of this step's: [lo, hi).
             int32_t lo[8], hi[8];
             bool hidden = false, move = false;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int32_t at = pair_at[8 * ty + i], place = own ? at : p.prefix + at;
+                const int32_t at = pair_at[8 * ty + i], place = max(at, 0) + (own ? 0 : p.prefix);
                 lo[i] = p.window ? max(place - p.window + 1 - key0, 0) : 0;
+                const bool there = pair_row[8 * ty + i] >= 0;
                 hi[i] = at < 0 ? 0 : min((own ? min(at + 1, limit) : limit) - key0, kTfKeys);
-                hidden |= lo[i] > 0 || hi[i] < kTfKeys;
+                hidden |= there && (lo[i] > 0 || hi[i] < kTfKeys);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = tx + 16 * j;
@@ -847,9 +874,8 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                 break;
             }
             if (tid == 0 && n + 1 < w.steps) copy(n + 1, 0);
-            const auto add = [&](int key, bool all) {
-                const float4 a = *tf_weight(weights, key, 2 * ty), b = *tf_weight(weights, key, 2 * ty + 1);
-                const float4 u = *tf_piece(tile_at[1], key, tx), v = *tf_piece(tile_at[1], key, 16 + tx);
+            // Where some pair does not see a key, its value, whatever it is, is left out for that pair.
+            const auto add = [&](int key, float4 a, float4 b, float4 u, float4 v, bool all) {
                 const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, z[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -858,13 +884,31 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                         for (int d = 0; d < 8; ++d) o[i][d] = fmaf(y[i], z[d], o[i][d]);
                     }
             };
-            // Where some pair does not see a key, its value, whatever it is, is left out for that pair.
             if (__any_sync(0xffffffffu, hidden)) {
 #pragma unroll 1
-                for (int key = 0; key < kTfKeys; ++key) add(key, false);
+                for (int key = 0; key < kTfKeys; ++key)
+                    add(key, *tf_weight(weights, key, 2 * ty), *tf_weight(weights, key, 2 * ty + 1), *tf_piece(tile_at[1], key, tx),
+                        *tf_piece(tile_at[1], key, 16 + tx), false);
             } else {
-#pragma unroll 4
-                for (int key = 0; key < kTfKeys; ++key) add(key, true);
+                const uint32_t w_at = smem_u32(tf_weight(weights, 0, 2 * ty)), v_at = smem_u32(tf_piece(tile_at[1], 0, tx));
+                float4 a[2], b[2], u[2], v[2];
+                const auto load = [&](int sixteen, int key) {
+                    const uint32_t wa = (w_at ^ (key << 4)) + (16 * sixteen + key) * (kTfPairs * 4);
+                    const uint32_t va = (v_at ^ ((key & 7) << 4)) + (16 * sixteen + key) * 128;
+                    a[key & 1] = lds_f32x4(wa);
+                    b[key & 1] = lds_f32x4(wa ^ 16);
+                    u[key & 1] = lds_f32x4(va);
+                    v[key & 1] = lds_f32x4(va + 2 * kTfKeys * 128);
+                };
+                load(0, 0);
+#pragma unroll 1
+                for (int sixteen = 0; sixteen < kTfKeys / 16; ++sixteen)
+#pragma unroll
+                    for (int key = 0; key < 16; ++key) {
+                        if (key < 15) load(sixteen, key + 1);
+                        else if (sixteen < kTfKeys / 16 - 1) load(sixteen + 1, 0);
+                        add(key, a[key & 1], b[key & 1], u[key & 1], v[key & 1], true);
+                    }
             }
             __syncthreads();  // values and weights have been read
             if (tid == 0 && n + 1 < w.steps) copy(n + 1, 1);
@@ -877,8 +921,9 @@ __global__ void __launch_bounds__(kTfThreads, 2)
 #pragma unroll
             for (int b = 1; b < 16; b <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
             const int pair = 8 * ty + i;
-            const int64_t to = pair_out[pair];
-            if (to < 0) continue;
+            const int32_t row = pair_row[pair];
+            if (row < 0) continue;
+            const uint64_t to = whole ? row * p.out_stride + head_of(pair) * kPgDim : (static_cast<uint64_t>(slot) * kTfPairs + pair) * kPgDim;
             const float inv = !whole ? 1.0f : m[i] == -INFINITY ? 0.0f : 1.0f / sum;
             float *dst = (whole ? static_cast<float *>(p.out) : p.tile_sum) + to + 4 * tx;
             *reinterpret_cast<float4 *>(dst) = make_float4(o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
