@@ -180,10 +180,18 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
         (a.tile_rows && !launch(c, "paged_attention tiles", F32 ? paged_tile_f32_kernel : paged_tile_kernel, dim3(a.tile_grid),
                                 dim3(F32 ? kTfThreads : kTlThreads), F32 ? kTfSmem : kTlSmem, stream, true, page_map, p)))
         return false;
-    // A block to eight results of short requests, or to a part of a cut tile.
-    const uint64_t blocks = std::max(d->rows * ceil_div(d->query_heads, 8), static_cast<uint64_t>(4 * a.tile_grid));
-    return launch(c, "paged_attention join", paged_join_kernel<F32>,
-                  dim3(static_cast<uint32_t>(std::min<uint64_t>(blocks, 6ull * context_sms(c)))), dim3(kJoinThreads), 0, stream, true, p);
+    // Two results to a block, its warps sharing their parts, while that takes two
+    // blocks to an SM at most (one request over 131,072 rows, 74 parts each: 10 us
+    // against 26 with eight to a block); then eight to a block, up to four blocks
+    // (61 requests behind a long prefix, 19 parts: 14 us against 27 with two to a
+    // warp); then eight to a warp (256 requests, 6 parts: 21 us against 39).
+    const uint64_t sms = static_cast<uint64_t>(context_sms(c)), twos = d->rows * ceil_div(d->query_heads, 2);
+    const uint64_t eights = d->rows * ceil_div(d->query_heads, 8);
+    const auto join = twos <= 2 * sms     ? paged_join_kernel<F32, 2, true>
+                      : eights <= 4 * sms ? paged_join_kernel<F32, 8, true>
+                                          : paged_join_kernel<F32, 8, false>;
+    const uint64_t blocks = std::min(4 * sms, std::max<uint64_t>(a.tile_rows ? 4 * sms : 1, twos <= 2 * sms ? twos : eights));
+    return launch(c, "paged_attention join", join, dim3(static_cast<uint32_t>(blocks)), dim3(kJoinThreads), 0, stream, true, p);
 }
 
 template <typename In, typename Out>

@@ -890,22 +890,23 @@ struct PartList {
     int32_t first, stride, rows, place, count;
     __device__ __forceinline__ int64_t at(int32_t x) const { return static_cast<int64_t>(first + x * stride) * rows + place; }
 };
-// Joins eight results, lane y's lists those of result y % 8 (empty where there
-// is none). Warp `sub` of `warps` takes every warps-th part of each, four at a
-// time: a lane weighs one part of one result, then the parts' sums are loaded
-// eight at once. Every lane returns with four dimensions of the sums over its
-// warp's parts, and l and the maximum m over them of its own result.
-__device__ __forceinline__ void join_parts(const PartList &a, const PartList &b, int32_t sub, int32_t warps, float4 (&o)[8], float &l,
+// Joins RES (2 or 8) results, lane y's lists those of result y % RES (empty
+// where there is none). Warp `sub` of `warps` takes every warps-th part of each,
+// 32 / RES at a time: a lane weighs one part of one result, then the parts' sums
+// are loaded eight at once. Every lane returns with four dimensions of the sums
+// over its warp's parts, and l and the maximum m over them of its own result.
+template <int RES>
+__device__ __forceinline__ void join_parts(const PartList &a, const PartList &b, int32_t sub, int32_t warps, float4 (&o)[RES], float &l,
                                            float &m) {
     const int32_t lane = threadIdx.x & 31, all = a.count + b.count;
     const int32_t most = __reduce_max_sync(0xffffffffu, all);
     m = -INFINITY;
     l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < RES; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int32_t x0 = sub; x0 < most; x0 += 4 * warps) {
-        const int32_t x = x0 + (lane >> 3) * warps;
+    for (int32_t x0 = sub; x0 < most; x0 += 32 / RES * warps) {
+        const int32_t x = x0 + (lane / RES) * warps;
         float2 v = make_float2(-INFINITY, 0.0f);
         const float *from = nullptr;
         if (x < all) {
@@ -915,21 +916,21 @@ __device__ __forceinline__ void join_parts(const PartList &a, const PartList &b,
             from = (first ? a.sum : b.sum) + at * kPgDim;
         }
         float top = fmaxf(m, v.x);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+#pragma unroll
+        for (int k = RES; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
         const float w = v.x == -INFINITY ? 0.0f : pg_exp2(v.x - top), corr = m == -INFINITY ? 0.0f : pg_exp2(m - top);
         m = top;
         l = fmaf(w, v.y, l * corr);
         if (x0 != sub) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < RES; ++i) {
                 const float f = __shfl_sync(0xffffffffu, corr, i);
                 o[i] = make_float4(o[i].x * f, o[i].y * f, o[i].z * f, o[i].w * f);
             }
         }
-#pragma unroll 2
+#pragma unroll 1
         for (int k = 0; k < 32; k += 8) {
-            if (x0 + (k >> 3) * warps >= most) break;
+            if (x0 + k / RES * warps >= most) break;
             float4 u[8];
             float f[8];
 #pragma unroll
@@ -940,12 +941,14 @@ __device__ __forceinline__ void join_parts(const PartList &a, const PartList &b,
                 if (f[i] != 0.0f) u[i] = ld4(src + 4 * lane);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                o[i] = make_float4(fmaf(f[i], u[i].x, o[i].x), fmaf(f[i], u[i].y, o[i].y), fmaf(f[i], u[i].z, o[i].z), fmaf(f[i], u[i].w, o[i].w));
+            for (int i = 0; i < 8; ++i) {
+                float4 &t = o[i % RES];
+                t = make_float4(fmaf(f[i], u[i].x, t.x), fmaf(f[i], u[i].y, t.y), fmaf(f[i], u[i].z, t.z), fmaf(f[i], u[i].w, t.w));
+            }
         }
     }
-    l += __shfl_xor_sync(0xffffffffu, l, 8);
-    l += __shfl_xor_sync(0xffffffffu, l, 16);
+#pragma unroll
+    for (int k = RES; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
 }
 template <bool F32>
 __device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row, int32_t head, float4 o, float l, float top) {
@@ -956,26 +959,26 @@ __device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row
     else pg_store4(static_cast<uint16_t *>(p.out) + to, o);
 }
 
-// Joins the short requests' rows (a block to eight heads of a row, each warp a
-// share of their parts), the prompts' tiles that two or more CTAs shared (a
-// warp to eight pairs), and zeroes the rows that see nothing.
+// Joins the short requests' rows, the prompts' tiles that two or more CTAs
+// shared (a warp to RES pairs), and zeroes the rows that see nothing. FEW: a
+// block to RES results, its warps sharing their parts; else a warp to RES.
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
-template <bool F32>
+template <bool F32, int RES, bool FEW>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
-    __shared__ float4 warp_sums[kJoinWarps][8][32];
-    __shared__ float2 warp_ml[kJoinWarps][8];
+    __shared__ float4 warp_sums[FEW ? kJoinWarps : 1][RES][32];
+    __shared__ float2 warp_ml[FEW ? kJoinWarps : 1][RES];
     const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
     const int32_t tiles = p.tile_rows ? p.header[kTlTiles] : 0, pre_tiles = p.tile_rows ? p.header[kTlPreTiles] : 0;
     const int32_t ctas = p.tile_rows ? p.header[kTlCtas] : 0;
     const Runs runs = tile_runs(p), of_rows = row_runs(p);
     PartList shared{}, own{};
-    float4 o[8];
+    float4 o[RES];
     float l, top;
-    const int32_t eights = (p.qh + 7) / 8, items = p.header[kTlShortRows] * eights;
+    const int32_t groups = (p.qh + RES - 1) / RES, items = p.header[kTlShortRows] * groups;
 #pragma unroll 1
-    for (int32_t n = blockIdx.x; n < items; n += gridDim.x) {
-        const int32_t listed = n / eights, head0 = 8 * (n - listed * eights), head = head0 + (lane & 7);
+    for (int32_t n = FEW ? blockIdx.x : blockIdx.x * kJoinWarps + warp; n < items; n += FEW ? gridDim.x : gridDim.x * kJoinWarps) {
+        const int32_t listed = n / groups, head0 = RES * (n - listed * groups), head = head0 + (lane & (RES - 1));
         const int4 e = p.short_list[listed];
         shared.count = own.count = 0;
         bool written = false;
@@ -1001,35 +1004,44 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                                   (listed - tile * p.tile_rows) * p.group + in_group, steps ? runs.cta_of(u0 + steps - 1) - c0 + 1 : 0};
             }
         }
-        const uint32_t skip = __ballot_sync(0xffffffffu, written || head >= p.qh);
-        if ((skip & 0xffu) == 0xffu) continue;  // (the same for all warps)
-        join_parts(shared, own, warp, kJoinWarps, o, l, top);
+        const uint32_t skip = __ballot_sync(0xffffffffu, written || head >= p.qh);  // (the same in all warps of an item)
+        if (skip == 0xffffffffu) continue;
+        join_parts<RES>(shared, own, FEW ? warp : 0, FEW ? kJoinWarps : 1, o, l, top);
+        if constexpr (FEW) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) warp_sums[warp][i][lane] = o[i];
-        if (lane < 8) warp_ml[warp][lane] = make_float2(top, l);
-        __syncthreads();
-        // Warp y puts result y together, the warps' shares in order.
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        top = -INFINITY;
-        l = 0.0f;
+            for (int i = 0; i < RES; ++i) warp_sums[warp][i][lane] = o[i];
+            if (lane < RES) warp_ml[warp][lane] = make_float2(top, l);
+            __syncthreads();
+            if (warp < RES && !((skip >> warp) & 1u)) {  // warp y puts result y together, the warps' shares in order
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                top = -INFINITY;
+                l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, warp_ml[i][warp].x);
+                for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, warp_ml[i][warp].x);
 #pragma unroll
-        for (int i = 0; i < kJoinWarps; ++i) {
-            const float2 ml = warp_ml[i][warp];
-            const float f = ml.x == -INFINITY ? 0.0f : pg_exp2(ml.x - top);
-            const float4 u = warp_sums[i][warp][lane];
-            v = make_float4(fmaf(f, u.x, v.x), fmaf(f, u.y, v.y), fmaf(f, u.z, v.z), fmaf(f, u.w, v.w));
-            l = fmaf(f, ml.y, l);
+                for (int i = 0; i < kJoinWarps; ++i) {
+                    const float2 ml = warp_ml[i][warp];
+                    const float f = ml.x == -INFINITY ? 0.0f : pg_exp2(ml.x - top);
+                    const float4 u = warp_sums[i][warp][lane];
+                    if (f != 0.0f) v = make_float4(fmaf(f, u.x, v.x), fmaf(f, u.y, v.y), fmaf(f, u.z, v.z), fmaf(f, u.w, v.w));
+                    l = fmaf(f, ml.y, l);
+                }
+                join_store<F32>(p, e.x, head0 + warp, v, l, top);
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int i = 0; i < RES; ++i) {
+                const float li = __shfl_sync(0xffffffffu, l, i), ti = __shfl_sync(0xffffffffu, top, i);
+                if (!((skip >> i) & 1u)) join_store<F32>(p, e.x, head0 + i, o[i], li, ti);
+            }
         }
-        if (!((skip >> warp) & 1u)) join_store<F32>(p, e.x, head0 + warp, v, l, top);
-        __syncthreads();
     }
     // Prompts' tiles that a CTA's end cuts: the first such end does the tile.
-    const int32_t blocks = p.tile_pairs / (8 * kJoinWarps);  // to a tile
+    const int32_t blocks = p.tile_pairs / (RES * kJoinWarps);  // to a tile
 #pragma unroll 1
     for (int32_t n = blockIdx.x; n < blocks * (ctas - 1); n += gridDim.x) {
-        const int32_t c = n / blocks + 1, pair0 = ((n - (c - 1) * blocks) * kJoinWarps + warp) * 8, cut = runs.start(c);
+        const int32_t c = n / blocks + 1, pair0 = ((n - (c - 1) * blocks) * kJoinWarps + warp) * RES, cut = runs.start(c);
         const int32_t tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles), p.by_kh.div(cut));
         if (tile < pre_tiles) continue;
         const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
@@ -1037,12 +1049,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         const int32_t row0 = p.tile_shape[tile].row0, pairs = p.tile_shape[tile].rows * p.group;
         if (cut == u0 || before > u0 || pair0 >= pairs) continue;
         // CTA c - 1 has this tile as its last run unless it begins with it; the others begin with it.
-        const int32_t pair = pair0 + (lane & 7), there = pair < pairs;
+        const int32_t pair = pair0 + (lane & (RES - 1)), there = pair < pairs;
         shared = PartList{p.tile_sum, p.tile_ml, 2 * (c - 1) + (before == u0 ? 0 : 1), 0, p.tile_pairs, pair, there};
         own = PartList{p.tile_sum, p.tile_ml, 2 * c, 2, p.tile_pairs, pair, there * (runs.cta_of(u0 + steps - 1) - c + 1)};
-        join_parts(shared, own, 0, 1, o, l, top);
+        join_parts<RES>(shared, own, 0, 1, o, l, top);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < RES; ++i) {
             const float li = __shfl_sync(0xffffffffu, l, i), ti = __shfl_sync(0xffffffffu, top, i);
             if (pair0 + i >= pairs) break;
             const int32_t row = p.by_group.div(pair0 + i);
