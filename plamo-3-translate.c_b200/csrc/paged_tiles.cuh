@@ -55,7 +55,7 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     const int32_t r0 = min(p.requests, tid * per), r1 = min(p.requests, r0 + per);
     if (tid == 0) first_at = INT32_MAX;
     __syncthreads();
-    int64_t counts = 0, steps = 0;  // short rows | prompts' tiles << 32; the tiles' key steps
+    int64_t counts = 0, all_counts;  // short rows | prompts' tiles << 32
     int32_t lowest = INT32_MAX;
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
@@ -64,17 +64,12 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
             counts += s.rows;
             if (s.rows) lowest = min(lowest, max(s.at0, 0));
         } else {
-            const int32_t n = p.by_tile_rows.div(s.rows + p.tile_rows - 1);
-            counts += static_cast<int64_t>(n) << 32;
-#pragma unroll 1
-            for (int32_t t = 0; t < n; ++t) steps += prompt_tile(p, r, s, t).steps();
+            counts += static_cast<int64_t>(p.by_tile_rows.div(s.rows + p.tile_rows - 1)) << 32;
         }
     }
     lowest = __reduce_min_sync(0xffffffffu, lowest);
     if ((tid & 31) == 0) atomicMin(&first_at, lowest);
-    int64_t all_counts, all_steps;
     const int64_t before = pg_block_scan<kRtThreads>(counts, sums, &all_counts);
-    int64_t step_at = pg_block_scan<kRtThreads>(steps, sums, &all_steps);
     int32_t short_at = static_cast<int32_t>(before), tile_at = static_cast<int32_t>(before >> 32);
     // Ranges that overlap (starts that decrease) could ask for more than there is.
     const int32_t all_short = min(static_cast<int32_t>(all_counts & 0x7fffffff), p.rows);
@@ -86,13 +81,8 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         pre.pre1 = (p.prefix + p.tile_keys - 1) / p.tile_keys;
         if (p.window && first_at != INT32_MAX) pre.pre0 = min(max(p.prefix + first_at - p.window + 1, 0) / p.tile_keys, pre.pre1);
     }
-    const int32_t pre_steps = pre.steps();
-    const int64_t total = static_cast<int64_t>(pre_tiles) * pre_steps + all_steps;
-    const bool fits = !p.tile_rows || (pre_tiles + all_tiles <= p.tile_cap && total * p.kh <= INT32_MAX - 256);
-    if (!fits) {  // only starts or lengths that no pool holds ask for this
-        if (tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
-        pre_tiles = all_tiles = 0;
-    }
+    bool fits = !p.tile_rows || pre_tiles + all_tiles <= p.tile_cap;
+    if (!fits) pre_tiles = all_tiles = 0;
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
         const OwnShape s = own_shape(p, r);
@@ -103,20 +93,38 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         } else if (fits) {
             const int32_t n = p.by_tile_rows.div(s.rows + p.tile_rows - 1);
 #pragma unroll 1
-            for (int32_t t = 0; t < n; ++t, ++tile_at) {
-                const TileShape shape = prompt_tile(p, r, s, t);
-                p.tile_shape[pre_tiles + tile_at] = shape;
-                p.tile_unit[pre_tiles + tile_at] = static_cast<uint32_t>(pre_tiles * pre_steps + step_at);
-                step_at += shape.steps();
+            for (int32_t t = 0; t < n; ++t, ++tile_at) {  // whose it is; the rest below, by all threads
+                p.tile_shape[pre_tiles + tile_at].request = r;
+                p.tile_shape[pre_tiles + tile_at].row0 = t;
             }
         }
     }
+    __syncthreads();
+    int64_t total = 0;
 #pragma unroll 1
-    for (int32_t t = tid; t < pre_tiles; t += kRtThreads) {
-        pre.row0 = t * p.tile_rows;
-        pre.rows = min(p.tile_rows, all_short - pre.row0);
-        p.tile_shape[t] = pre;
-        p.tile_unit[t] = static_cast<uint32_t>(t * pre_steps);
+    for (int32_t t0 = 0; t0 < pre_tiles + all_tiles; t0 += kRtThreads) {
+        const int32_t t = t0 + tid;
+        TileShape shape{};
+        if (t < pre_tiles) {
+            shape = pre;
+            shape.row0 = t * p.tile_rows;
+            shape.rows = min(p.tile_rows, all_short - shape.row0);
+        } else if (t < pre_tiles + all_tiles) {
+            const int32_t r = p.tile_shape[t].request;
+            shape = prompt_tile(p, r, own_shape(p, r), p.tile_shape[t].row0);
+        }
+        int64_t sum;
+        const int64_t at = total + pg_block_scan<kRtThreads>(shape.steps(), sums, &sum);
+        if (t < pre_tiles + all_tiles) {
+            p.tile_shape[t] = shape;
+            p.tile_unit[t] = static_cast<uint32_t>(at);
+        }
+        total += sum;
+    }
+    fits = fits && total * p.kh <= INT32_MAX - 256;
+    if (!fits) {  // only starts or lengths that no pool holds ask for this
+        if (tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
+        pre_tiles = all_tiles = 0;
     }
     if (tid == 0) {
         p.header[kTlShortRows] = all_short;
@@ -804,19 +812,20 @@ __global__ void __launch_bounds__(kTfThreads, 2)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) q_at[i] = smem_u32(tf_query(queries, 8 * ty + i, 0));
                 float4 k[2][4], q[2][8];
-                const auto load = [&](int box, int c) {
+                const auto load = [&](int four, int c) {  // piece 4 four + c
+                    const uint32_t turn = (four & 1) << 6, k_box = (four >> 1) * (kTfKeys * 128), q_box = (four >> 1) * 128;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) k[c & 1][j] = lds_f32x4((k_at[j] ^ (c << 4)) + box * (kTfKeys * 128));
+                    for (int j = 0; j < 4; ++j) k[c & 1][j] = lds_f32x4(((k_at[j] ^ turn) ^ (c << 4)) + k_box);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) q[c & 1][i] = lds_f32x4((q_at[i] ^ (c << 4)) + box * 128);
+                    for (int i = 0; i < 8; ++i) q[c & 1][i] = lds_f32x4(((q_at[i] ^ turn) ^ (c << 4)) + q_box);
                 };
                 load(0, 0);
 #pragma unroll 1
-                for (int box = 0; box < 4; ++box)
+                for (int four = 0; four < kPgDim / 16; ++four)
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        if (c < 7) load(box, c + 1);
-                        else if (box < 3) load(box + 1, 0);
+                    for (int c = 0; c < 4; ++c) {
+                        if (c < 3) load(four, c + 1);
+                        else if (four < kPgDim / 16 - 1) load(four + 1, 0);
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -892,9 +901,9 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             } else {
                 const uint32_t w_at = smem_u32(tf_weight(weights, 0, 2 * ty)), v_at = smem_u32(tf_piece(tile_at[1], 0, tx));
                 float4 a[2], b[2], u[2], v[2];
-                const auto load = [&](int sixteen, int key) {
-                    const uint32_t wa = (w_at ^ (key << 4)) + (16 * sixteen + key) * (kTfPairs * 4);
-                    const uint32_t va = (v_at ^ ((key & 7) << 4)) + (16 * sixteen + key) * 128;
+                const auto load = [&](int eight, int key) {  // key 8 eight + key
+                    const uint32_t wa = ((w_at ^ ((eight & 1) << 7)) ^ (key << 4)) + (8 * eight + key) * (kTfPairs * 4);
+                    const uint32_t va = (v_at ^ (key << 4)) + (8 * eight + key) * 128;
                     a[key & 1] = lds_f32x4(wa);
                     b[key & 1] = lds_f32x4(wa ^ 16);
                     u[key & 1] = lds_f32x4(va);
@@ -902,11 +911,11 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                 };
                 load(0, 0);
 #pragma unroll 1
-                for (int sixteen = 0; sixteen < kTfKeys / 16; ++sixteen)
+                for (int eight = 0; eight < kTfKeys / 8; ++eight)
 #pragma unroll
-                    for (int key = 0; key < 16; ++key) {
-                        if (key < 15) load(sixteen, key + 1);
-                        else if (sixteen < kTfKeys / 16 - 1) load(sixteen + 1, 0);
+                    for (int key = 0; key < 8; ++key) {
+                        if (key < 7) load(eight, key + 1);
+                        else if (eight < kTfKeys / 8 - 1) load(eight + 1, 0);
                         add(key, a[key & 1], b[key & 1], u[key & 1], v[key & 1], true);
                     }
             }

@@ -39,7 +39,7 @@ def _torch():
 
 def _stream(torch, device):
     """torch's current stream of device index `device`; 0 would name the context's own stream, 1 is the default one."""
-    return torch.cuda.current_stream(device).cuda_stream or 1
+    return torch._C._cuda_getCurrentRawStream(device) or 1
 
 
 # The checks sit on the path of calls that take a few microseconds in all: plain
