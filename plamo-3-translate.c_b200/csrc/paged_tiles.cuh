@@ -162,13 +162,13 @@ __device__ __forceinline__ bool tl_wait(uint64_t *bar, uint32_t parity, volatile
 // or keys that exist and some row of the tile does not see.
 __device__ __forceinline__ bool step_is_mended(const PagedAttnParams &p, const TileShape &s, int32_t step, bool *masked) {
     const bool own = step >= s.pre1 - s.pre0;
-    const int32_t key0 = (own ? s.own0 + step - (s.pre1 - s.pre0) : s.pre0 + step) * kTlKeys;
+    const int32_t key0 = (own ? s.own0 + step - (s.pre1 - s.pre0) : s.pre0 + step) * p.tile_keys;
     const int32_t limit = own ? s.own_limit : p.prefix;
     bool m = s.request >= 0 && s.at0 < 0;
-    if (own) m |= s.at0 + 1 < min(key0 + kTlKeys, limit) || (p.window && max(s.at0 + s.rows, 0) - p.window > key0);
+    if (own) m |= s.at0 + 1 < min(key0 + p.tile_keys, limit) || (p.window && max(s.at0 + s.rows, 0) - p.window > key0);
     else if (p.window) m |= s.request < 0 || p.prefix + max(s.at0 + s.rows, 0) - p.window > key0;
     *masked = m;
-    return m || key0 + kTlKeys > limit;
+    return m || key0 + p.tile_keys > limit;
 }
 
 // Bits k of the 32 in [lo, hi).
@@ -837,14 +837,12 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             }
             // Keys that each pair sees, of this step's: [lo, hi).
             int32_t lo[8], hi[8];
-            bool hidden = false, move = false;
+            bool move = false;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int32_t at = pair_at[8 * ty + i], place = max(at, 0) + (own ? 0 : p.prefix);
                 lo[i] = p.window ? max(place - p.window + 1 - key0, 0) : 0;
-                const bool there = pair_row[8 * ty + i] >= 0;
                 hi[i] = at < 0 ? 0 : min((own ? min(at + 1, limit) : limit) - key0, kTfKeys);
-                hidden |= there && (lo[i] > 0 || hi[i] < kTfKeys);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = tx + 16 * j;
@@ -878,12 +876,24 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                 *tf_weight(weights, tx + 16 * j, 2 * ty + 1) = make_float4(y[4], y[5], y[6], y[7]);
             }
             ok = mbar_wait(&full[1], phase);
+            // A weight of zero leaves a value out only if that is finite: where keys are hidden from
+            // some pair, the values are looked over.
+            bool masked, odd = false;
+            const int32_t valid = min(limit - key0, kTfKeys);  // keys that exist
+            step_is_mended(p, s, step, &masked);
+            if (masked) {
+#pragma unroll 4
+                for (int k = tid; k < valid * (kPgDim / 4); k += kTfThreads) {
+                    const float4 v = *tf_piece(tile_at[1], k >> 5, k & 31);
+                    odd |= !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
+                }
+                odd = __syncthreads_or(odd);
+            }
             if (__syncthreads_or(!ok)) {  // the weights are there, and the keys have been read
                 ok = false;
                 break;
             }
             if (tid == 0 && n + 1 < w.steps) copy(n + 1, 0);
-            // Where some pair does not see a key, its value, whatever it is, is left out for that pair.
             const auto add = [&](int key, float4 a, float4 b, float4 u, float4 v, bool all) {
                 const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, z[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -893,12 +903,10 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                         for (int d = 0; d < 8; ++d) o[i][d] = fmaf(y[i], z[d], o[i][d]);
                     }
             };
-            if (__any_sync(0xffffffffu, hidden)) {
-#pragma unroll 1
-                for (int key = 0; key < kTfKeys; ++key)
-                    add(key, *tf_weight(weights, key, 2 * ty), *tf_weight(weights, key, 2 * ty + 1), *tf_piece(tile_at[1], key, tx),
-                        *tf_piece(tile_at[1], key, 16 + tx), false);
-            } else {
+            // Eights of keys at full speed; the rest, and all where a value is odd, for the pairs that
+            // see them only.
+            const int eights = odd ? 0 : valid / 8;
+            if (eights) {
                 const uint32_t w_at = smem_u32(tf_weight(weights, 0, 2 * ty)), v_at = smem_u32(tf_piece(tile_at[1], 0, tx));
                 float4 a[2], b[2], u[2], v[2];
                 const auto load = [&](int eight, int key) {  // key 8 eight + key
@@ -911,14 +919,18 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                 };
                 load(0, 0);
 #pragma unroll 1
-                for (int eight = 0; eight < kTfKeys / 8; ++eight)
+                for (int eight = 0; eight < eights; ++eight)
 #pragma unroll
                     for (int key = 0; key < 8; ++key) {
                         if (key < 7) load(eight, key + 1);
-                        else if (eight < kTfKeys / 8 - 1) load(eight + 1, 0);
+                        else if (eight < eights - 1) load(eight + 1, 0);
                         add(key, a[key & 1], b[key & 1], u[key & 1], v[key & 1], true);
                     }
             }
+#pragma unroll 1
+            for (int key = 8 * eights; key < valid; ++key)
+                add(key, *tf_weight(weights, key, 2 * ty), *tf_weight(weights, key, 2 * ty + 1), *tf_piece(tile_at[1], key, tx),
+                    *tf_piece(tile_at[1], key, 16 + tx), false);
             __syncthreads();  // values and weights have been read
             if (tid == 0 && n + 1 < w.steps) copy(n + 1, 1);
             phase ^= 1u;
