@@ -31,11 +31,13 @@
  *
  * Return convention, as plamo_cuda.h: 1 enqueued; 0 declined, nothing
  * enqueued (the reason is in plamo_cuda_info.note); -1 a launch failed.
- * What only the device can see is reported there: entries whose page, slot,
- * position or row lies outside its array are left out (never read or
- * written), and `status` (a device word, may be NULL) gets a PLAMO_PAGED_*
- * bit. Buffers must stay valid until the stream has run the call; calls with
- * a workspace of their own may overlap on different streams.
+ * What only the device can see is reported there: rows whose slot or position
+ * lies outside its array are left out, a page outside the pool reads as rows
+ * of zeros, nothing out of range is read or written, and `status` (a device
+ * word, may be NULL) gets a PLAMO_PAGED_* bit. Buffers must stay valid until
+ * the stream has run the call; calls with a workspace of their own may overlap
+ * on different streams. Every call can be captured in a CUDA graph: none
+ * allocates, waits or reads a length on the host.
  */
 #ifndef PLAMO_PAGED_H
 #define PLAMO_PAGED_H
@@ -124,7 +126,8 @@ struct plamo_paged_attention_args {
     void *stream;
 };
 /* Device bytes a call with these shapes needs (its pointers are not read);
-   0 when the shapes would be declined. */
+   0 when the shapes would be declined. The prefix and a request's page table
+   hold at most 2^30 rows each. */
 uint64_t plamo_paged_attention_workspace(struct plamo_cuda *, const struct plamo_paged_attention_args *);
 /* out = sum over the rows j it sees of softmax_j(scale * q . k_j) v_j, for
    every new row and query head (head h reads KV head h / (query_heads /

@@ -65,14 +65,18 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     AttentionLayout a{};
     const uint64_t group = d->query_heads / d->kv_heads, sms = static_cast<uint64_t>(context_sms(c));
     const uint64_t pairs = d->rows * group, prefix_pages = ceil_div(d->prefix_rows, kPgRows);
-    // The tile kernel is for prompts (more rows than requests, some request with
-    // more pairs than the row kernel takes) and for a prefix that would keep the
-    // row kernel, eight pairs at a time, longer than another kernel takes to
-    // begin and end (about 15 us: 4,000 pages and heads in BF16, 2,000 in FP32).
+    // The tile kernel is for prompts (more rows than requests, and more pairs than
+    // a short request has), and in BF16 for a prefix that would keep the row
+    // kernel, eight pairs at a time, longer than another kernel takes to begin and
+    // end: 61 requests of eight heads to a KV head, own rows as they are, took 41,
+    // 50 us there behind 512, 1,000 rows (1,952, 3,904 tiles of eight pairs times
+    // pages) and 58, 51 us with tiles behind 1,100, 2,000. In FP32 the tiles' rate is
+    // no better than the row kernel's (76 us in it behind 512 rows; 103, 136 with
+    // tiles behind 1,000, 2,000: the same slope, 12 us more).
     const bool f32 = d->type == PLAMO_PAGED_FP32;
     const uint64_t tile_pairs = f32 ? kTfPairs : kTlPairs;
-    const uint64_t prefix_work = ceil_div(pairs, 8) * prefix_pages * d->kv_heads;
-    if (group <= tile_pairs && ((d->rows > d->requests && pairs > kTlShortPairs) || prefix_work > (f32 ? 2000 : 4000))) {
+    const bool prompts = d->rows > d->requests && pairs > kTlShortPairs;
+    if (group <= tile_pairs && (prompts || (!f32 && ceil_div(pairs, 8) * prefix_pages * d->kv_heads > 4000))) {
         a.tile_rows = static_cast<uint32_t>(tile_pairs / group);
         a.tile_grid = static_cast<uint32_t>(f32 ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.

@@ -181,6 +181,9 @@ __device__ __forceinline__ float pg_exp2(float x) {  // 2^x to about 2 ulp, 2^-i
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// A part's {m, l}: m of -inf says that it saw nothing, so a part that saw scores
+// of which none is a number (no maximum, l not a number) gets another.
+__device__ __forceinline__ float2 pg_ml(float m, float l) { return make_float2(l != l && m == -INFINITY ? 0.0f : m, l); }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -381,7 +384,7 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
             for (int h = 0; h < 2; ++h) {
                 float e[2];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) e[c] = mx[nt][c] == -INFINITY ? 0.0f : pg_exp2(s[nt][2 * h + c] - mx[nt][c]);
+                for (int c = 0; c < 2; ++c) e[c] = pg_exp2(s[nt][2 * h + c] - (mx[nt][c] == -INFINITY ? 0.0f : mx[nt][c]));
                 const uint32_t w = pg_pack(e[0], e[1]);
                 pf[nt][h] = transpose8(w);
                 s[nt][2 * h] = bf16_lo(w);
@@ -452,7 +455,7 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (g == 0) cta.warp_ml[warp][8 * nt + 2 * t + c] = make_float2(mx[nt][c], l);
+            if (g == 0) cta.warp_ml[warp][8 * nt + 2 * t + c] = pg_ml(mx[nt][c], l);
         }
     rt_bar();  // and every warp is done with the queries
     float factor[NT][2];
@@ -568,7 +571,7 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
         }
 #pragma unroll
         for (int four = 0; four < 4; ++four) {
-            const float w = m == -INFINITY ? 0.0f : pg_exp2(s[four] - m);
+            const float w = pg_exp2(s[four] - (m == -INFINITY ? 0.0f : m));
             l += w;
             weights[32 * four + lane] = w;  // [key][pair]
         }
@@ -603,7 +606,7 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
     }
     l += __shfl_xor_sync(0xffffffffu, l, 8);
     l += __shfl_xor_sync(0xffffffffu, l, 16);
-    if (lane < 8) cta.warp_ml[warp][lane] = make_float2(m, l);
+    if (lane < 8) cta.warp_ml[warp][lane] = pg_ml(m, l);
     rt_bar();
     float top = -INFINITY;
 #pragma unroll

@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     __syncwarp();
                 }
             }
-            if (there && !whole) p.tile_ml[static_cast<int64_t>(slot) * kTlPairs + pair] = make_float2(m, l);
+            if (there && !whole) p.tile_ml[static_cast<int64_t>(slot) * kTlPairs + pair] = pg_ml(m, l);
             tc_fence_before();
         }
     }
@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                 float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    y[i] = m[i] == -INFINITY ? 0.0f : pg_exp2(x[i][j] - m[i]);
+                    y[i] = pg_exp2(x[i][j] - (m[i] == -INFINITY ? 0.0f : m[i]));
                     l[i] += y[i];
                 }
                 *tf_weight(weights, tx + 16 * j, 2 * ty) = make_float4(y[0], y[1], y[2], y[3]);
@@ -945,11 +945,12 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             const int32_t row = pair_row[pair];
             if (row < 0) continue;
             const uint64_t to = whole ? row * p.out_stride + head_of(pair) * kPgDim : (static_cast<uint64_t>(slot) * kTfPairs + pair) * kPgDim;
-            const float inv = !whole ? 1.0f : m[i] == -INFINITY ? 0.0f : 1.0f / sum;
+            const float2 ml = pg_ml(m[i], sum);
+            const float inv = !whole ? 1.0f : ml.x == -INFINITY ? 0.0f : 1.0f / sum;
             float *dst = (whole ? static_cast<float *>(p.out) : p.tile_sum) + to + 4 * tx;
             *reinterpret_cast<float4 *>(dst) = make_float4(o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
             *reinterpret_cast<float4 *>(dst + 64) = make_float4(o[i][4] * inv, o[i][5] * inv, o[i][6] * inv, o[i][7] * inv);
-            if (!whole && tx == 0) p.tile_ml[static_cast<int64_t>(slot) * kTfPairs + pair] = make_float2(m[i], sum);
+            if (!whole && tx == 0) p.tile_ml[static_cast<int64_t>(slot) * kTfPairs + pair] = ml;
         }
     }
     if (!ok && tid == 0) {  // copies in flight land before the CTA ends

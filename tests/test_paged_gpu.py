@@ -275,6 +275,19 @@ def test_attention_rows_not_seen_never_matter(be, bad, window, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("requests", [[(0, 1), (5, 1)], [(0, 40), (70, 1)], [(0, 300)]])
+def test_attention_of_keys_that_are_no_numbers(be, requests, dtype):
+    """A row all of whose keys are NaN has no result; its neighbours have theirs."""
+    s = Scene(requests, 0, 8, 2, dtype, seed=3)
+    want, tol = s.expected()
+    s.pool[s.tables[0, 0], 0, 0] = float("nan")  # the first request's first key: all its rows see it
+    got = attend(be, s)
+    n = requests[0][1]
+    assert torch.isnan(got[:n]).all()
+    check(got[n:], want[n:], tol[n:], "the others")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_attention_values_fallen_out_of_the_window(be, dtype):
     s = Scene([(80, 40), (70, 1)], 100, 8, 2, dtype, seed=3)
     want, tol = s.expected(60)
@@ -382,6 +395,21 @@ def test_a_step_on_another_stream_and_in_a_graph(be):
             assert torch.equal(out, want)
     torch.cuda.synchronize()
     assert kept.tolist() == [5, 67, 125] and torch.equal(tables2, tables)
+
+
+@pytest.mark.parametrize("args,bound", [([], 2e-2), (["--fp32"], 2e-4)])
+def test_example_serves_a_batch_as_each_request_alone(args, bound):
+    """BF16: each layer's keys, values, queries and results are rounded to 2^-8,
+    differently placed pages only regroup the sums, so a few roundings' worth
+    (2 layers, 20 fed-back steps) may differ; FP32: the same of 2^-24, with the
+    projections' 1e-6 and the feedback's growth on top."""
+    import importlib.util
+    import os
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("paged_batch", os.path.join(ROOT, "examples", "paged_batch.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    assert module.main(args) <= bound
 
 
 # ---- refusals ----------------------------------------------------------------------
