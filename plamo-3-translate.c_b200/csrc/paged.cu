@@ -201,13 +201,14 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
 template <typename In, typename Out>
 bool run_store(plamo_cuda *c, const plamo_paged_store_args *d, cudaStream_t stream) {
     const uint64_t heads = d->query_heads + 2ull * d->kv_heads;
-    // Four heads to a warp once that still gives every SM eight warps and more;
-    // one to a warp for the few rows of a decode step.
+    // Eight heads to a warp once one head each would be four rounds of eight warps
+    // to an SM; one to a warp for the few rows of a decode step, where latency
+    // counts (8 rows: 3.7 us).
     const bool wide = d->rows * heads >= 4ull * 8 * static_cast<uint64_t>(context_sms(c));
-    const uint64_t units = d->rows * ceil_div(heads, wide ? 4 : 1);
+    const uint64_t units = d->rows * ceil_div(heads, wide ? 8 : 1);
     const dim3 grid(static_cast<uint32_t>(ceil_div(units, 8)));
     if (wide)
-        return launch(c, "paged_store", paged_store_kernel<In, Out, 4>, grid, dim3(256), 0, stream, false, *d);
+        return launch(c, "paged_store", paged_store_kernel<In, Out, 8>, grid, dim3(256), 0, stream, false, *d);
     return launch(c, "paged_store", paged_store_kernel<In, Out, 1>, grid, dim3(256), 0, stream, false, *d);
 }
 

@@ -183,17 +183,22 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanParams p) 
 }
 
 // ---- store ----------------------------------------------------------------------
-// A warp takes HPW heads of one row: lane l holds dimensions 4l..4l+3, its
-// rotation partner (d +- 64) is lane l ^ 16, and the row's cos/sin stay in
-// registers for all of its heads. All loads of a warp are issued before the
-// first is used.
+// A warp takes HPW heads of one row: lane l holds dimensions 2l, 2l + 1 and
+// their rotation partners 64 + 2l, 64 + 2l + 1, so that a head's only exchange
+// is the sum of its squares, and the row's cos/sin stay in registers for all of
+// its heads. All loads of a warp are issued before the first is used. Streaming:
+// 8,191 rows of 40 heads are 168 MB in and 84 MB out, 39 us at the copy rate;
+// 40 us with eight heads to a warp, 43 with four (fewer bytes in flight); lanes
+// of four neighbouring dimensions, their partners exchanged, took 48.
+// {x[2l], x[2l + 1], x[64 + 2l], x[64 + 2l + 1]}
 template <typename T>
-__device__ __forceinline__ float4 pg_load4(const T *p) {
+__device__ __forceinline__ float4 pg_load_pairs(const T *x, uint32_t lane) {
     if constexpr (sizeof(T) == 4) {
-        return *reinterpret_cast<const float4 *>(p);
+        const float2 a = *reinterpret_cast<const float2 *>(x + 2 * lane), b = *reinterpret_cast<const float2 *>(x + kPgDim / 2 + 2 * lane);
+        return make_float4(a.x, a.y, b.x, b.y);
     } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
+        const uint32_t a = *reinterpret_cast<const uint32_t *>(x + 2 * lane), b = *reinterpret_cast<const uint32_t *>(x + kPgDim / 2 + 2 * lane);
+        return make_float4(bf16_lo(a), bf16_hi(a), bf16_lo(b), bf16_hi(b));
     }
 }
 __device__ __forceinline__ uint32_t pg_pack(float lo, float hi) {  // round to nearest even
@@ -209,6 +214,17 @@ __device__ __forceinline__ void pg_store4(T *p, float4 v) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(pg_pack(v.x, v.y), pg_pack(v.z, v.w));
 }
 
+template <typename T>
+__device__ __forceinline__ void pg_store_pairs(T *x, uint32_t lane, float4 v) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2 *>(x + 2 * lane) = make_float2(v.x, v.y);
+        *reinterpret_cast<float2 *>(x + kPgDim / 2 + 2 * lane) = make_float2(v.z, v.w);
+    } else {
+        *reinterpret_cast<uint32_t *>(x + 2 * lane) = pg_pack(v.x, v.y);
+        *reinterpret_cast<uint32_t *>(x + kPgDim / 2 + 2 * lane) = pg_pack(v.z, v.w);
+    }
+}
+
 template <typename In, typename Out, int HPW>
 __global__ void __launch_bounds__(256) paged_store_kernel(plamo_paged_store_args d) {
     const uint32_t lane = threadIdx.x & 31;
@@ -221,7 +237,7 @@ __global__ void __launch_bounds__(256) paged_store_kernel(plamo_paged_store_args
     float4 v[HPW];
 #pragma unroll
     for (int i = 0; i < HPW; ++i)
-        if (h0 + i < heads) v[i] = pg_load4(x + static_cast<uint64_t>(h0 + i) * kPgDim + 4 * lane);
+        if (h0 + i < heads) v[i] = pg_load_pairs(x + static_cast<uint64_t>(h0 + i) * kPgDim, lane);
     const int64_t slot = d.slots[row], position = d.positions[row];
     bool keep = slot >= 0;
     if (slot < -1 || slot >= static_cast<int64_t>(d.pages) * kPgRows) {
@@ -237,13 +253,11 @@ __global__ void __launch_bounds__(256) paged_store_kernel(plamo_paged_store_args
 #pragma unroll
         for (int i = 0; i < HPW; ++i)
             if (h0 + i < d.query_heads)
-                pg_store4(q + static_cast<uint64_t>(h0 + i) * kPgDim + 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
+                pg_store_pairs(q + static_cast<uint64_t>(h0 + i) * kPgDim, lane, make_float4(0.f, 0.f, 0.f, 0.f));
         return;
     }
-    const float *turn = d.table + position * kPgDim + 4 * (lane & 15);
-    const float4 c = ld4(turn), s = ld4(turn + kPgDim / 2);
-    const float4 wq = norm4(*reinterpret_cast<const uint2 *>(d.q_norm + 4 * lane), 1.0f);
-    const float4 wk = norm4(*reinterpret_cast<const uint2 *>(d.k_norm + 4 * lane), 1.0f);
+    const float4 turn = pg_load_pairs(d.table + position * kPgDim, lane);  // cos, cos, sin, sin
+    const float4 q_norm = pg_load_pairs(d.q_norm, lane), k_norm = pg_load_pairs(d.k_norm, lane);
     const uint64_t page = static_cast<uint64_t>(slot) / kPgRows, off = static_cast<uint64_t>(slot) % kPgRows;
     const uint64_t width = static_cast<uint64_t>(d.kv_heads) * kPgDim;
     Out *key = static_cast<Out *>(d.pool) + (page * 2 * kPgRows + off) * width;
@@ -253,26 +267,21 @@ __global__ void __launch_bounds__(256) paged_store_kernel(plamo_paged_store_args
         const uint32_t h = h0 + i;
         if (h >= heads) break;
         if (h >= d.query_heads + d.kv_heads) {
-            pg_store4(value + static_cast<uint64_t>(h - d.query_heads - d.kv_heads) * kPgDim + 4 * lane, v[i]);
+            pg_store_pairs(value + static_cast<uint64_t>(h - d.query_heads - d.kv_heads) * kPgDim, lane, v[i]);
             continue;
         }
         const bool query = h < d.query_heads;
-        const float inv = rms_inverse(warp_sum(sq4(v[i])), kPgDim);
-        const float4 a = apply4(v[i], inv, query ? wq : wk);
-        float4 b;
-        b.x = __shfl_xor_sync(0xffffffffu, a.x, 16);
-        b.y = __shfl_xor_sync(0xffffffffu, a.y, 16);
-        b.z = __shfl_xor_sync(0xffffffffu, a.z, 16);
-        b.w = __shfl_xor_sync(0xffffffffu, a.w, 16);
-        if (lane < 16) b = make_float4(-b.x, -b.y, -b.z, -b.w);
-        const float4 o = make_float4(__fadd_rn(__fmul_rn(a.x, c.x), __fmul_rn(b.x, s.x)),
-                                     __fadd_rn(__fmul_rn(a.y, c.y), __fmul_rn(b.y, s.y)),
-                                     __fadd_rn(__fmul_rn(a.z, c.z), __fmul_rn(b.z, s.z)),
-                                     __fadd_rn(__fmul_rn(a.w, c.w), __fmul_rn(b.w, s.w)));
+        // (to 2 ulp; a rounded root and quotient cost 7 us of 55 in 8,191 rows)
+        const float inv = rsqrtf(fmaf(warp_sum(sq4(v[i])), 1.0f / kPgDim, 1e-6f));
+        const float4 w = query ? q_norm : k_norm;
+        const float4 a = make_float4(v[i].x * inv * (w.x + 1.0f), v[i].y * inv * (w.y + 1.0f), v[i].z * inv * (w.z + 1.0f),
+                                     v[i].w * inv * (w.w + 1.0f));
+        const float4 o = make_float4(fmaf(a.x, turn.x, -a.z * turn.z), fmaf(a.y, turn.y, -a.w * turn.w),
+                                     fmaf(a.z, turn.x, a.x * turn.z), fmaf(a.w, turn.y, a.y * turn.w));
         if (query)
-            pg_store4(q + static_cast<uint64_t>(h) * kPgDim + 4 * lane, o);
+            pg_store_pairs(q + static_cast<uint64_t>(h) * kPgDim, lane, o);
         else
-            pg_store4(key + static_cast<uint64_t>(h - d.query_heads) * kPgDim + 4 * lane, o);
+            pg_store_pairs(key + static_cast<uint64_t>(h - d.query_heads) * kPgDim, lane, o);
     }
 }
 
