@@ -82,9 +82,10 @@ __host__ __device__ constexpr int rt_slab_bytes() {  // keys, then values
     return 2 * kRtKeys * kPgDim * (F32 ? 4 : 2);
 }
 // A ring of slabs and, behind it, the queries or the warps' joined sums; two
-// CTAs to an SM. The ring's places are a multiple of the warps, so each place
-// serves one warp and that warp sees all of its phases in turn: a wait by
-// parity could not tell a phase from the one before the last.
+// CTAs to an SM. The ring's places are a multiple of the warps, so that within
+// an item a place serves one warp, which has seen each of its phases before the
+// next (and between items all warps meet): a wait by parity could not tell a
+// phase from the one before the last.
 constexpr int kRtRing = 98304;
 constexpr int kRtSmem = 1024 + kRtRing + 16 * kPgDim * 4;
 

@@ -118,7 +118,7 @@ class Scene:
                     p = torch.softmax(s, -1)
                     out[row, heads] = p @ vv[:, h]
                     a = p @ vv[:, h].abs()
-                    e = (q[row, heads].abs() @ kk[:, h].abs().T).amax(-1, keepdim=True) * scale * 2.0 ** -17
+                    e = (q[row, heads].abs() @ kk[:, h].abs().T).amax(-1, keepdim=True) * abs(scale) * 2.0 ** -17
                     t = a * (2 * torch.expm1(e) + 2.0 ** -17)
                     if self.dtype == torch.bfloat16:
                         t = t + 2.0 ** -8 * out[row, heads].abs() + 2 * 2.0 ** -8 * a

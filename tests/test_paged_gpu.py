@@ -191,7 +191,7 @@ def test_attention_matches_its_formula(be, name, prefix, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-@pytest.mark.parametrize("heads", [(1, 1), (3, 3), (16, 1), (32, 4), (64, 8), (40, 1), (14, 2)])
+@pytest.mark.parametrize("heads", [(1, 1), (3, 3), (16, 1), (32, 4), (64, 8), (40, 1), (14, 2), (70, 1), (300, 1)])
 def test_attention_head_layouts(be, heads, dtype):
     s = Scene([(70, 1), (0, 3), (20, 21)], 77, *heads, dtype, seed=heads[0])
     check(attend(be, s), *s.expected(), str(heads))
@@ -209,6 +209,24 @@ def test_attention_windows(be, window, dtype):
 def test_attention_split_along_the_keys(be, prefix, held, dtype):
     s = Scene([(held, 1)], prefix, 12, 2, dtype, seed=held)
     check(attend(be, s), *s.expected(), "split")
+
+
+@pytest.mark.parametrize("window", [0, 700])
+@pytest.mark.parametrize("heads", [(16, 2), (14, 2)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_attention_of_a_batch_behind_a_long_prefix(be, dtype, heads, window):
+    """Prefix work that takes tiles in BF16 though every request is short."""
+    s = Scene([(i * 7 % 130, 1 if i % 10 else 2) for i in range(150)], 1500, *heads, dtype, seed=11)
+    check(attend(be, s, window=window), *s.expected(window), "long prefix")
+    s = Scene([(i * 7 % 130, 1) for i in range(150)], 1500, *heads, dtype, seed=12)
+    check(attend(be, s, window=window), *s.expected(window), "long prefix, one row each")
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-20, 0.3])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_attention_scales(be, dtype, scale):
+    s = Scene([(0, 70), (90, 1)], 40, 8, 2, dtype, seed=13)
+    check(attend(be, s, scale=scale), *s.expected(scale=scale), f"scale {scale}")
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
