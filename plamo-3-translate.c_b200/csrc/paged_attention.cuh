@@ -75,7 +75,7 @@ constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 constexpr int kRtKeys = 16;
 constexpr int kRtWarps = 6;                      // computing warps, a slab each in turn
 constexpr int kRtThreads = 32 * (kRtWarps + 1);  // and the copying warp
-constexpr int kRtMinPages = 2;                   // least pages worth a CTA
+constexpr int kRtMinPages = 1;                   // least pages worth a CTA (8 requests of 450 FP32 rows: 18.5 us; 22.6 with 2)
 constexpr int kRtBatch = 8;                      // items laid out at a time
 template <bool F32>
 __host__ __device__ constexpr int rt_slab_bytes() {  // keys, then values
