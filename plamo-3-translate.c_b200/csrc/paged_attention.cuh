@@ -633,20 +633,25 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
 }
 
 // ---- the row kernel ---------------------------------------------------------------
-// Items of one tile of pairs over a run of pages; persistent CTAs take every
-// gridDim-th. Own keys are read once per tile and the products are far below
+// Items are parts of strips: one tile of pairs over a run of pages. CTAs take
+// equal runs of all pages, whatever requests they cut, so ragged lengths cost
+// no waiting (whole chunks of a request to a CTA left the last ones alone with
+// their work). Own keys are read once per tile and the products are far below
 // the tensor pipe's rate, so this is a streaming kernel: one warp copies slabs
-// of 16 keys into a ring, two CTAs to an SM, and six warps take a slab
-// each in turn, with a running maximum and sums of their own that are joined
-// at the end of the item. Scores are computed transposed, keys x pairs: a
-// group of up to eight heads then fills the N of an MMA instead of half its M,
-// and the value sums (dimensions x pairs) take 32 registers a thread instead
-// of 64, which leaves room for 14 warps on an SM.
+// of 16 keys into a ring, two CTAs to an SM, and six warps take a slab each in
+// turn, with a running maximum and sums of their own that are joined at the end
+// of the item. Scores are computed transposed, keys x pairs: a group of up to
+// eight heads then fills the N of an MMA instead of half its M, and the value
+// sums (dimensions x pairs) take 32 registers a thread instead of 64, which
+// leaves room for 14 warps on an SM.
 // FP32 pools take the CUDA cores: 32 multiply-adds a lane for each key's
 // scores and as many for its values are 350 issue cycles of an SM per slab,
 // half of what the slab's 16 KB take to arrive, and lose nothing to splitting.
-// (Measured before: TF32 mma.sync with two terms to an operand, 5 us per slab
-// and warp against 0.7 us for BF16.)
+// (TF32 mma.sync with two terms to an operand took 5 us per slab and warp; this
+// takes 2 to 3, BF16 0.7.)
+// Bound: HBM on long runs (one request over 131,072 rows of 1 KB: 50 us, 5.4
+// TB/s); on short items their ends, about 4 us each (256 requests of 500 rows
+// and eight KV heads: 130 us, 4.1 TB/s).
 __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums);  // paged_tiles.cuh
 
 // Request r's work, or the prefix's (r == requests) from page pp0 on.

@@ -331,6 +331,22 @@ def test_attention_reports_pages_outside_the_pool(be, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("new", [1, 50])
+def test_attention_reports_counts_outside_their_arrays(be, dtype, new):
+    """Lengths past the table, negative ones, and rows past the batch: a bit each, the other request as ever."""
+    s = Scene([(100, new), (70, 1)], 30, 8, 2, dtype, seed=9)
+    want, tol = s.expected()
+    good = s.lengths.clone(), s.starts.clone()
+    for lengths, starts, bit in (([2 ** 31 - 1, 71], None, 2), ([-5, 71], None, 8), (None, [-3, new, new + 1], 4)):
+        s.lengths = good[0] if lengths is None else ints(lengths)
+        s.starts = good[1] if starts is None else ints(starts)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = attend(be, s, status=status)
+        assert status.item() & bit and not status.item() & 64
+        check(got[new:], want[new:], tol[new:], "the other request")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_attention_is_the_same_every_time(be, dtype):
     s = Scene([(i * 29 % 400, 1 + i % 3) for i in range(60)], 700, 16, 2, dtype, seed=4)
     first = attend(be, s)
