@@ -115,7 +115,7 @@ def plan(backend, held, added, tables, free_pages, rows, base=0, after=None):
     if after is not None:
         _ints(torch, after.summary, 4, device, "after.summary")
         head = after.summary.data_ptr() + 8
-    buffer = torch.empty(2 * requests + 2 * rows + 5, dtype=torch.int32, device=held.device)
+    buffer = held.new_empty(2 * requests + 2 * rows + 5)
     at = buffer.data_ptr()
     starts = at + 4 * requests
     slots = starts + 4 * requests + 4
@@ -154,7 +154,7 @@ def store(backend, qkv, pool, slots, positions, q_norm, k_norm, table, status=No
     if (table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != DIM or table.get_device() != device or
             not table.is_contiguous()):
         raise ValueError(f"table: a contiguous FP32 [positions, {DIM}] tensor on the pool's GPU")
-    q = torch.empty(rows, query_heads, DIM, dtype=pool.dtype, device=pool.device)
+    q = pool.new_empty((rows, query_heads, DIM))
     args = _abi.PagedStoreArgs(qkv.data_ptr(), pool.data_ptr(), q.data_ptr(), slots.data_ptr(), positions.data_ptr(),
                                q_norm.data_ptr(), k_norm.data_ptr(), table.data_ptr(), _status(torch, status, device), rows,
                                row_stride if rows > 1 else width, query_heads * DIM, pages, table.shape[0], query_heads,
@@ -190,7 +190,7 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
         _ints(torch, prefix_pages, -1, device, "prefix_pages")
         prefix = prefix_pages.data_ptr()
     if out is None:
-        out = torch.empty(rows, query_heads, DIM, dtype=pool.dtype, device=pool.device)
+        out = pool.new_empty((rows, query_heads, DIM))
         out_stride = query_heads * DIM
     else:
         if out.shape != q.shape:
@@ -203,7 +203,7 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
     size = backend.lib.plamo_paged_attention_workspace(backend.ctx, ctypes.byref(args))
     if not size:
         raise ValueError(backend.info().note.decode())
-    workspace = torch.empty(size, dtype=torch.uint8, device=pool.device)
+    workspace = pool.new_empty(size, dtype=torch.uint8)
     args.workspace, args.workspace_bytes = workspace.data_ptr(), size
     _run(backend, backend.lib.plamo_paged_attention, args)
     return out
