@@ -136,8 +136,9 @@ uint64_t plamo_paged_attention_workspace(struct plamo_cuda *, const struct plamo
    that sees nothing gets zeros: padding, and rows whose request holds fewer
    rows (lengths) than it adds, before the first held one. Rows past a request's length, of other
    requests and after a query's own never reach its result, whatever they
-   hold. Scores, softmax sums and products are FP32 for both types (a BF16
-   pool rounds the softmax weights of a tile to BF16 for the value product). */
+   hold. Scores, softmax sums and products are FP32 for both types; against a
+   BF16 pool's values the softmax weights of prompts and long prefixes go in as
+   two BF16 terms, those of other rows as one. */
 int plamo_paged_attention(struct plamo_cuda *, const struct plamo_paged_attention_args *);
 
 #ifdef __cplusplus

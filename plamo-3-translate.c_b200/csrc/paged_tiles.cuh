@@ -9,19 +9,22 @@ namespace plamo {
 // A tile is two halves of 128 pairs (the M of one MMA), each with its own
 // scores, weights and sums in tensor memory and four warps of softmax; both
 // read the same keys and values, 128 at a time. Tensor memory (512 columns):
-// scores of half i at 128 i (FP32; the weights replace them as BF16, 64
-// columns), sums at 256 + 128 i. Per 128 keys each half needs 2 x 512 cycles
-// of the tensor pipe (128 x 128 x 128 at 4096 multiply-adds a cycle) and
+// scores of half i at 128 i (FP32; the weights replace them, 64 keys in 64
+// columns: 32 of a first BF16 term, 32 of the second), sums at 256 + 128 i. Per
+// 128 keys each half needs 512 cycles of the tensor pipe for the scores and two
+// times 512 for the values (128 x 128 x 128 at 4096 multiply-adds a cycle) and
 // 1024 cycles of exponentials (16 a cycle): the halves run half a step apart,
 // so that one's exponentials cover the other's products. Measured: 329 GFLOP of
-// ragged prompts behind 2,048 rows in 500 us, 0.66 PFLOP/s, the tensor pipe busy
-// for 36 % of it. A half's chain bounds it, 2.5 us a step: scores, softmax (1.1
-// us), the value product, and the next scores only when that is done, since they
-// replace the weights; then 8 us at each segment's ends.
-// The weights are rounded to BF16 because the value product takes both operands
-// in one type and the values are BF16: results are then 2.3e-3 from 64 bits
-// (relative L2) where their own rounding to BF16 makes 1.7e-3; a second term
-// would double the value product in the chain that bounds the kernel.
+// ragged prompts behind 2,048 rows in 604 us, 0.54 PFLOP/s. A half's chain bounds
+// it, 3 us a step: scores, softmax, the value product, and the next scores only
+// when that is done, since they replace the weights; then 8 us at each segment's
+// ends.
+// The value product takes both operands in one type and the values are BF16, so
+// the FP32 weights go in as two BF16 terms, 16 bits together: the results are
+// then the exact ones rounded to BF16 (those prompts: 1.66e-3 from 64 bits,
+// relative L2). One term was 2.32e-3 off in 502 us beside the unrounded weights'
+// sums, 2.30e-3 in 508 us beside the rounded ones'; on rows whose weight lies on
+// few keys those two differ more.
 constexpr int kTlPairs = 256;
 constexpr int kTlKeys = 128;
 constexpr int kTlThreads = 352;  // 8 softmax warps, copies, products, mending
@@ -400,8 +403,11 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                         tc_fence_after();
                         const uint64_t b = v_desc + vs * (kTlUnitBytes / 16);
 #pragma unroll
-                        for (int k = 0; k < kTlKeys / 16; ++k)
-                            tc_mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, b + k * 128, idesc_o, n || k ? 1u : 0u);
+                        for (int k = 0; k < kTlKeys / 16; ++k) {  // both terms of 16 keys' weights
+                            const uint32_t a = tmem + 128 * i + 64 * (k / 4) + 8 * (k % 4);
+                            tc_mma_ts(tmem + 256 + 128 * i, a, b + k * 128, idesc_o, n || k ? 1u : 0u);
+                            tc_mma_ts(tmem + 256 + 128 * i, a + 32, b + k * 128, idesc_o, 1u);
+                        }
                         tc_commit(&pv_done[i]);
                         if (more) {  // the next scores replace the weights just read
                             ok = tl_wait(&pv_done[i], (products >> i) & 1u, quit);
@@ -531,7 +537,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 const int32_t lo = min(max((own ? own_lo : pre_lo) - key0, 0), kTlKeys);
                 const bool partial = __any_sync(0xffffffffu, there && (lo > 0 || hi < kTlKeys));
                 // 64 scores at a time, twice: for the maximum, then for the weights, which replace them
-                // (BF16, half their place). Loops, not straight code: a segment is a few steps long, and
+                // (two BF16 terms). Loops, not straight code: a segment is a few steps long, and
                 // code that runs a few times costs its fetching.
                 uint32_t x[64];
                 const auto load = [&](int half) {
@@ -583,16 +589,21 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     if (half) load(1);  // (the first half is there from before)
-                    uint32_t r[32];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const float a = pg_exp2(fmaf(__uint_as_float(x[2 * k]), scale2, shift));
-                        const float b = pg_exp2(fmaf(__uint_as_float(x[2 * k + 1]), scale2, shift));
-                        l0 += a;
-                        l1 += b;
-                        r[k] = pg_pack(a, b);
+                    for (int part = 0; part < 2; ++part) {
+                        uint32_t r[16], rest[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float a = pg_exp2(fmaf(__uint_as_float(x[32 * part + 2 * k]), scale2, shift));
+                            const float b = pg_exp2(fmaf(__uint_as_float(x[32 * part + 2 * k + 1]), scale2, shift));
+                            l0 += a;
+                            l1 += b;
+                            r[k] = pg_pack(a, b);
+                            rest[k] = pg_pack(a - bf16_lo(r[k]), b - bf16_hi(r[k]));
+                        }
+                        tmem_st16(scol + 64 * half + 16 * part, r);
+                        tmem_st16(scol + 64 * half + 32 + 16 * part, rest);
                     }
-                    tmem_st32(scol + 32 * half, r);
                 }
                 l += l0 + l1;
                 tmem_wait_st();
