@@ -136,9 +136,8 @@ uint64_t plamo_paged_attention_workspace(struct plamo_cuda *, const struct plamo
    that sees nothing gets zeros: padding, and rows whose request holds fewer
    rows (lengths) than it adds, before the first held one. Rows past a request's length, of other
    requests and after a query's own never reach its result, whatever they
-   hold. Scores, softmax sums and products are FP32 for both types; against a
-   BF16 pool's values the softmax weights of prompts and long prefixes go in as
-   two BF16 terms, those of other rows as one. */
+   hold. Scores, softmax sums and products are FP32 for both types (against
+   a BF16 pool's values the softmax weights go in as two BF16 terms, 16 bits). */
 int plamo_paged_attention(struct plamo_cuda *, const struct plamo_paged_attention_args *);
 
 #ifdef __cplusplus

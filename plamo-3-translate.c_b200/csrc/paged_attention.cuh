@@ -372,21 +372,24 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
                     }
                 }
         }
-        // ---- weights, transposed into the product's operand; the sums are those of the rounded ones
-        uint32_t pf[NT][2];
+        // ---- weights, transposed into the product's operand as two BF16 terms (16 bits together:
+        // the values are BF16 and both operands have one type). Keys bound the kernel: one request
+        // over 131,072 rows takes 59.3 us, 58.9 with one term, 256 requests of 500 rows 142 and 139;
+        // one term's results are 2.28e-3 from 64 bits where their own rounding makes 1.69e-3.
+        uint32_t pf[NT][2], pr[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float e[2];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) e[c] = pg_exp2(s[nt][2 * h + c] - (mx[nt][c] == -INFINITY ? 0.0f : mx[nt][c]));
-                const uint32_t w = pg_pack(e[0], e[1]);
+                for (int c = 0; c < 2; ++c) {
+                    float &e = s[nt][2 * h + c];
+                    e = pg_exp2(e - (mx[nt][c] == -INFINITY ? 0.0f : mx[nt][c]));
+                    sum[nt][c] += e;
+                }
+                const uint32_t w = pg_pack(s[nt][2 * h], s[nt][2 * h + 1]);
                 pf[nt][h] = transpose8(w);
-                s[nt][2 * h] = bf16_lo(w);
-                s[nt][2 * h + 1] = bf16_hi(w);
-                sum[nt][0] += s[nt][2 * h];
-                sum[nt][1] += s[nt][2 * h + 1];
+                pr[nt][h] = transpose8(pg_pack(s[nt][2 * h] - bf16_lo(w), s[nt][2 * h + 1] - bf16_hi(w)));
             }
         // ---- sums. A weight of zero times a value that is not finite would be NaN: such values
         // leave the products and are added where they are seen. Only slabs with masked keys are
@@ -409,7 +412,10 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
                 }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_bf16(o[j][nt], a, pf[nt][0], pf[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+                mma_bf16(o[j][nt], a, pf[nt][0], pf[nt][1]);
+                mma_bf16(o[j][nt], a, pr[nt][0], pr[nt][1]);
+            }
         }
         if (careful && __any_sync(0xffffffffu, odd)) {
 #pragma unroll 1

@@ -54,3 +54,11 @@ def test_a_shared_prefix_in_tiles_loses_only_the_results_rounding(be):
     s = Scene([(0, 1)] * 1200, 130, 16, 2, BF16, seed=22, spread=1.0)
     off, bound = beyond_rounding(be, s)
     assert off <= bound, f"{off:.3e}, bound {bound:.3e}"
+
+
+@pytest.mark.parametrize("heads", [(8, 1), (16, 1)])
+@pytest.mark.parametrize("prefix", [0, 7])
+def test_decode_rows_lose_only_their_results_rounding(be, prefix, heads):
+    s = Scene([(i * 7 % 30, 1) for i in range(150)], prefix, *heads, BF16, seed=23, spread=1.0)
+    off, bound = beyond_rounding(be, s)
+    assert off <= bound, f"{off:.3e}, bound {bound:.3e}"
