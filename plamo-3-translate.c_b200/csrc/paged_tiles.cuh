@@ -66,7 +66,8 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     const int32_t r0 = min(p.requests, tid * per), r1 = min(p.requests, r0 + per);
     if (tid == 0) first_at = INT32_MAX;
     __syncthreads();
-    int64_t counts = 0, all_counts;  // short rows | prompts' tiles << 32
+    // 64 bits: starts that decrease make ranges that overlap, and their sums more than there is of either.
+    int64_t short_rows = 0, prompt_tiles = 0, all_short_rows, all_tiles = 0;
     int32_t lowest = INT32_MAX;
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
@@ -75,19 +76,18 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         if (p.lengths[r] < 0) pg_flag(p.status, PLAMO_PAGED_COUNT);
         if (p.starts[r] < 0 || p.starts[r + 1] < p.starts[r] || p.starts[r + 1] > p.rows) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
         if (request_is_short(p, s)) {
-            counts += s.rows;
+            short_rows += s.rows;
             if (s.rows) lowest = min(lowest, max(s.at0, 0));
         } else {
-            counts += static_cast<int64_t>(p.by_tile_rows.div(s.rows + p.tile_rows - 1)) << 32;
+            prompt_tiles += p.by_tile_rows.div(s.rows + p.tile_rows - 1);
         }
     }
     lowest = __reduce_min_sync(0xffffffffu, lowest);
     if ((tid & 31) == 0) atomicMin(&first_at, lowest);
-    const int64_t before = pg_block_scan<kRtThreads>(counts, sums, &all_counts);
-    int32_t short_at = static_cast<int32_t>(before), tile_at = static_cast<int32_t>(before >> 32);
-    // Ranges that overlap (starts that decrease) could ask for more than there is.
-    const int32_t all_short = min(static_cast<int32_t>(all_counts & 0x7fffffff), p.rows);
-    int32_t all_tiles = static_cast<int32_t>(all_counts >> 32), pre_tiles = 0;
+    int64_t short_at = pg_block_scan<kRtThreads>(short_rows, sums, &all_short_rows);
+    int64_t tile_at = p.tile_rows ? pg_block_scan<kRtThreads>(prompt_tiles, sums, &all_tiles) : 0;
+    const int32_t all_short = static_cast<int32_t>(min(all_short_rows, static_cast<int64_t>(p.rows)));
+    int32_t pre_tiles = 0;
     TileShape pre{};
     if (p.tile_rows && p.prefix) {
         pre_tiles = p.by_tile_rows.div(all_short + p.tile_rows - 1);
@@ -95,15 +95,17 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         pre.pre1 = (p.prefix + p.tile_keys - 1) / p.tile_keys;
         if (p.window && first_at != INT32_MAX) pre.pre0 = min(max(p.prefix + first_at - p.window + 1, 0) / p.tile_keys, pre.pre1);
     }
-    bool fits = !p.tile_rows || pre_tiles + all_tiles <= p.tile_cap;
+    bool fits = pre_tiles + all_tiles <= p.tile_cap;  // (no tile kernel: 0 <= 0)
     if (!fits) pre_tiles = all_tiles = 0;
+    const int32_t all = pre_tiles + static_cast<int32_t>(all_tiles);
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
         const OwnShape s = own_shape(p, r);
         if (request_is_short(p, s)) {
 #pragma unroll 1
-            for (int32_t i = 0; i < s.rows; ++i, ++short_at)
-                if (short_at < all_short) p.short_list[short_at] = make_int4(s.row0 + i, max(s.at0 + i, -1), r, i);
+            for (int32_t i = 0; i < s.rows && short_at + i < all_short; ++i)
+                p.short_list[short_at + i] = make_int4(s.row0 + i, max(s.at0 + i, -1), r, i);
+            short_at += s.rows;
         } else if (fits) {
             const int32_t n = p.by_tile_rows.div(s.rows + p.tile_rows - 1);
 #pragma unroll 1
@@ -116,20 +118,20 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     __syncthreads();
     int64_t total = 0;
 #pragma unroll 1
-    for (int32_t t0 = 0; t0 < pre_tiles + all_tiles; t0 += kRtThreads) {
+    for (int32_t t0 = 0; t0 < all; t0 += kRtThreads) {
         const int32_t t = t0 + tid;
         TileShape shape{};
         if (t < pre_tiles) {
             shape = pre;
             shape.row0 = t * p.tile_rows;
             shape.rows = min(p.tile_rows, all_short - shape.row0);
-        } else if (t < pre_tiles + all_tiles) {
+        } else if (t < all) {
             const int32_t r = p.tile_shape[t].request;
             shape = prompt_tile(p, r, own_shape(p, r), p.tile_shape[t].row0);
         }
         int64_t sum;
         const int64_t at = total + pg_block_scan<kRtThreads>(shape.steps(), sums, &sum);
-        if (t < pre_tiles + all_tiles) {
+        if (t < all) {
             p.tile_shape[t] = shape;
             p.tile_unit[t] = static_cast<uint32_t>(at);
         }
@@ -138,7 +140,6 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     fits = fits && total * p.kh <= INT32_MAX - 256;
     if (!fits) {  // only starts or lengths that no pool holds ask for this
         if (tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
-        pre_tiles = all_tiles = 0;
     }
     if (tid == 0) {
         p.header[kTlShortRows] = all_short;
@@ -148,9 +149,9 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         p.header[kTlRun] = ctas ? units / ctas : 1;
         p.header[kTlLonger] = ctas ? units % ctas : 0;
         if (p.tile_rows) {
-            p.tile_unit[pre_tiles + all_tiles] = fits ? static_cast<uint32_t>(total) : 0;
-            p.header[kTlTiles] = pre_tiles + all_tiles;
-            p.header[kTlPreTiles] = pre_tiles;
+            p.tile_unit[fits ? all : 0] = fits ? static_cast<uint32_t>(total) : 0;
+            p.header[kTlTiles] = fits ? all : 0;
+            p.header[kTlPreTiles] = fits ? pre_tiles : 0;
         }
     }
 }
