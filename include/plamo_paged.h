@@ -127,7 +127,8 @@ struct plamo_paged_attention_args {
 };
 /* Device bytes a call with these shapes needs (its pointers are not read);
    0 when the shapes would be declined. The prefix and a request's page table
-   hold at most 2^30 rows each. */
+   hold at most 2^30 rows each; requests, and rows times query heads, are at
+   most 2^30. */
 uint64_t plamo_paged_attention_workspace(struct plamo_cuda *, const struct plamo_paged_attention_args *);
 /* out = sum over the rows j it sees of softmax_j(scale * q . k_j) v_j, for
    every new row and query head (head h reads KV head h / (query_heads /

@@ -44,8 +44,9 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
     if (!type_ok(d->type)) return "paged_attention: type must be PLAMO_PAGED_BF16 or PLAMO_PAGED_FP32";
     if (!d->kv_heads || !d->query_heads || d->query_heads % d->kv_heads || d->query_heads > 4096)
         return "paged_attention: query_heads must be a multiple of kv_heads, at most 4096";
-    if (d->rows > INT32_MAX || d->requests > INT32_MAX - 1 || d->rows * d->query_heads > INT32_MAX)
-        return "paged_attention: too many rows or requests";
+    // (threads step through both in 32 bits, a grid past the end)
+    if (d->rows > kPgMaxCount || d->requests > kPgMaxCount || d->rows * d->query_heads > kPgMaxCount)
+        return "paged_attention: at most 2^30 requests, and rows times query heads";
     if (!d->pages || d->pages > static_cast<uint64_t>(kPgMaxPages) / 4)
         return "paged_attention: pages must be 1 to 2^23";
     if (d->prefix_rows > INT32_MAX / 2 || d->table_stride > INT32_MAX / 2 / kPgRows)

@@ -12,6 +12,7 @@ constexpr int kPgRows = PLAMO_PAGED_ROWS;
 constexpr int kPgDim = PLAMO_PAGED_DIM;
 // Largest page id + 1: slots (page * 64 + row) stay below 2^31.
 constexpr int32_t kPgMaxPages = 1 << 25;
+constexpr uint64_t kPgMaxCount = 1u << 30;
 
 __device__ __forceinline__ void pg_flag(uint32_t *status, uint32_t bit) {
     if (status) atomicOr(status, bit);

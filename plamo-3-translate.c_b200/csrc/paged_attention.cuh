@@ -31,7 +31,8 @@ struct FastDiv {
     }
 };
 
-// All counts, rows and positions are below 2^31 (checked by the host).
+// All lengths and positions are below 2^31, requests and (row, head) pairs at
+// most 2^30 (checked by the host).
 struct PagedAttnParams {
     const void *q;
     void *out;

@@ -56,3 +56,18 @@ def test_overlapping_rows_past_2_31_stay_in_the_workspace(be, rows, requests):
     assert (out[0] == 7).all() and (out[-1] == 7).all()
     s = Scene([(5, 1), (70, 40)], 0, 1, 1, BF16)  # the next call is as ever
     check(attend(be, s), *s.expected())
+
+
+def test_counts_near_2_31_are_declined(be):
+    """Shapes alone: nothing is enqueued."""
+    abi = load_package()._abi
+
+    def size(**change):
+        shape = dict(rows=8, requests=4, table_stride=2, pages=8, query_heads=8, kv_heads=2, type=0)
+        return be.lib.plamo_paged_attention_workspace(be.ctx, ctypes.byref(abi.PagedAttentionArgs(**{**shape, **change})))
+
+    assert size() and size(requests=1 << 30) and size(rows=1 << 27)
+    for change in (dict(requests=(1 << 30) + 1), dict(requests=2 ** 31 - 100), dict(rows=(1 << 27) + 1),
+                   dict(rows=(1 << 30) + 1, query_heads=1, kv_heads=1), dict(requests=1 << 62), dict(rows=1 << 62)):
+        assert size(**change) == 0, change
+        assert "2^30" in be.info().note.decode()
