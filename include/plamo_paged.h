@@ -4,7 +4,7 @@
  * server that batches translation requests behind a common prompt (the
  * template, an instruction, a document) keeps every layer's keys and values
  * in one pool of pages and runs three operators per step, all on device
- * buffers and all asynchronous on one stream:
+ * buffers of the context's GPU and all asynchronous on one stream of it:
  *
  *   plamo_paged_plan       page tables and slot maps from the requests' row
  *                          counts (once per step);

@@ -510,7 +510,7 @@ class Backend:
     """Thin owner of one plamo_cuda context."""
 
     def __init__(self, device=0, max_context=0, max_prefill=0, copy_kv_to_host=False):
-        self.lib = _abi.load()
+        self.lib, self.device = _abi.load(), device
         cfg = _abi.CudaConfig(device=device, max_context=max_context, max_prefill=max_prefill,
                               reserve=0, copy_kv_to_host=int(copy_kv_to_host))
         err = ctypes.create_string_buffer(512)

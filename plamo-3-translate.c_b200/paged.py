@@ -5,9 +5,9 @@ of 64-row pages, [pages, 2, 64, kv_heads, 128] in BF16 or FP32. A step plans
 its rows once (`plan`), then per layer stores the projection's rows (`store`)
 and attends (`attention`). Calls are enqueued on torch's current stream and
 return without waiting; tensors they allocate come from torch's allocator.
-Wrong arguments raise ValueError. What only the GPU can see is reported as
-PLAMO_PAGED_* bits, in the plan's summary or in a `status` tensor (one int32,
-zeroed by the caller).
+Wrong arguments raise ValueError, tensors of another GPU than the backend's
+among them. What only the GPU can see is reported as PLAMO_PAGED_* bits, in the
+plan's summary or in a `status` tensor (one int32, zeroed by the caller).
 """
 import ctypes
 from typing import NamedTuple
@@ -58,10 +58,10 @@ def _type(torch, t, name):
     return _abi.PAGED_FP32
 
 
-def _pool(torch, pool):
+def _pool(torch, pool, backend):
     """(type, pages, kv_heads, device index) of a pool."""
-    if pool.dim() != 5 or not pool.is_contiguous() or pool.get_device() < 0:
-        raise ValueError(f"pool: a contiguous [pages, 2, {ROWS}, kv_heads, {DIM}] tensor on the GPU")
+    if pool.dim() != 5 or not pool.is_contiguous() or pool.get_device() != backend.device:
+        raise ValueError(f"pool: a contiguous [pages, 2, {ROWS}, kv_heads, {DIM}] tensor on the backend's GPU, {backend.device}")
     pages, two, rows, kv_heads, dim = pool.shape
     if two != 2 or rows != ROWS or dim != DIM:
         raise ValueError(f"pool: a contiguous [pages, 2, {ROWS}, kv_heads, {DIM}] tensor on the GPU")
@@ -103,8 +103,8 @@ def plan(backend, held, added, tables, free_pages, rows, base=0, after=None):
     """
     torch = _torch()
     requests, device = held.numel(), held.get_device()
-    if device < 0 or rows < 0:
-        raise ValueError("held: on the GPU; rows: not negative")
+    if device != backend.device or rows < 0:
+        raise ValueError(f"held: on the backend's GPU, {backend.device}; rows: not negative")
     _ints(torch, held, requests, device, "held")
     _ints(torch, added, requests, device, "added")
     _ints(torch, free_pages, -1, device, "free_pages")
@@ -137,7 +137,7 @@ def store(backend, qkv, pool, slots, positions, q_norm, k_norm, table, status=No
     queries, [rows, query_heads, 128] of the pool's type.
     """
     torch = _torch()
-    kind, pages, kv_heads, device = _pool(torch, pool)
+    kind, pages, kv_heads, device = _pool(torch, pool, backend)
     if qkv.dim() != 2 or qkv.get_device() != device:
         raise ValueError(f"qkv: [rows, heads * {DIM}] on the pool's GPU")
     rows, width = qkv.shape
@@ -174,7 +174,7 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
     the scores, 1 / sqrt(128) unless given. Returns `out`, allocated if None.
     """
     torch = _torch()
-    kind, pages, kv_heads, device = _pool(torch, pool)
+    kind, pages, kv_heads, device = _pool(torch, pool, backend)
     q_stride = _rows(torch, q, pool, device, "q")
     rows, query_heads, _ = q.shape
     requests = lengths.numel()
