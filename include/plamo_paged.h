@@ -86,7 +86,9 @@ struct plamo_paged_plan_args {
    depends on the inputs alone. A request takes a page when a row reaches it.
    A step that cannot be taken as a whole (status bits 1, 2, 4, 8) changes
    nothing: lengths = held, starts = 0, every slot -1, no table entry or page
-   taken, so that a captured step's following operators do nothing. */
+   taken, so that a captured step's following operators do nothing. `lengths`
+   may be `held` itself, to advance a step in place; buffers that overlap in
+   any other way are declined. */
 int plamo_paged_plan(struct plamo_cuda *, const struct plamo_paged_plan_args *);
 
 struct plamo_paged_store_args {

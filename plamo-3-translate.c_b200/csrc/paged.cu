@@ -19,6 +19,7 @@ cudaStream_t stream_of(const plamo_cuda *c, void *stream) {
 bool aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 uint64_t element_bytes(uint32_t type) { return type == PLAMO_PAGED_FP32 ? 4 : 2; }
 bool type_ok(uint32_t type) { return type == PLAMO_PAGED_BF16 || type == PLAMO_PAGED_FP32; }
+bool overlap(const int32_t *a, uint64_t na, const int32_t *b, uint64_t nb) { return a && b && na && nb && a < b + nb && b < a + na; }
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 template <typename... KArgs, typename... Args>
@@ -239,12 +240,32 @@ int plamo_paged_plan(struct plamo_cuda *c, const struct plamo_paged_plan_args *d
     if (d->rows > INT32_MAX - kPlanThreads || d->requests >= INT32_MAX || d->free_count > INT32_MAX ||
         d->table_stride > static_cast<uint64_t>(kPgMaxPages) || d->base < 0 || d->base > INT32_MAX)
         return context_decline(c, "paged_plan: a count is out of range");
-    if (d->head && d->head >= d->summary && d->head < d->summary + 4)
-        return context_decline(c, "paged_plan: head must not lie in this plan's own summary");
+    if (overlap(d->head, 1, d->summary, 4)) return context_decline(c, "paged_plan: head must not lie in this plan's own summary");
+    // Every CTA reads the counts by itself, so none may write what another reads. Lengths that
+    // replace `held` are written by a launch of their own, or by the only CTA, whose threads
+    // read the entries that they write.
+    const uint64_t R = d->requests;
+    const bool in_place = R && d->lengths == d->held;
+    const struct {
+        const int32_t *at;
+        uint64_t count;
+    } buffers[] = {{d->lengths, R}, {d->starts, R + 1}, {d->slots, d->rows}, {d->positions, d->rows}, {d->summary, 4},
+                   {d->tables, R * d->table_stride},  // (read and written)
+                   {d->held, R}, {d->added, R}, {d->free_pages, d->free_count}, {d->head, 1}};
+    for (int i = 0; i < 6; ++i)
+        for (int j = i + 1; j < 10; ++j)
+            if (!(i == 0 && j == 6 && in_place) && overlap(buffers[i].at, buffers[i].count, buffers[j].at, buffers[j].count))
+                return context_decline(c, "paged_plan: buffers overlap (only lengths may be held itself)");
     ContextDevice device(c);
     const uint32_t grid = static_cast<uint32_t>(std::max<uint64_t>(1, ceil_div(d->rows, kPlanThreads)));
-    return launch(c, "paged_plan", paged_plan_kernel, dim3(grid), dim3(kPlanThreads), 0, stream_of(c, d->stream), false,
-                  PlanParams{*d})
+    const cudaStream_t stream = stream_of(c, d->stream);
+    PlanParams p{*d};
+    const bool apart = in_place && grid > 1;
+    if (apart) p.d.lengths = nullptr;
+    if (!launch(c, "paged_plan", paged_plan_kernel, dim3(grid), dim3(kPlanThreads), 0, stream, false, p)) return -1;
+    if (!apart) return 1;
+    return launch(c, "paged_plan lengths", paged_plan_lengths_kernel, dim3(static_cast<uint32_t>(ceil_div(R, kPlanThreads))),
+                  dim3(kPlanThreads), 0, stream, false, d->lengths, d->added, d->summary, R)
                ? 1
                : -1;
 }

@@ -55,7 +55,7 @@ __device__ __forceinline__ int64_t pg_block_scan(int64_t v, int64_t *sm, int64_t
 constexpr int kPlanThreads = 1024;
 
 struct PlanParams {
-    plamo_paged_plan_args d;
+    plamo_paged_plan_args d;  // lengths NULL: written by paged_plan_lengths_kernel
 };
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanParams p) {
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanParams p) 
         }
         if (blockIdx.x == 0) {
             for (int64_t r = r0; r < r1; ++r) {
-                d.lengths[r] = d.held[r];
+                if (d.lengths) d.lengths[r] = d.held[r];
                 d.starts[r + 1] = 0;
             }
             if (tid == 0) {
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanParams p) 
     for (int64_t r = r0; r < r1; ++r) {
         const int32_t held = d.held[r], added = d.added[r];
         if (blockIdx.x == 0) {
-            d.lengths[r] = held + added;
+            if (d.lengths) d.lengths[r] = held + added;
             d.starts[r + 1] = static_cast<int32_t>(row + added);
         }
         if (added && row < tile + kPlanThreads && row + added > tile) {
@@ -183,6 +183,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanParams p) 
     }
     d.slots[my_row] = slot;
     d.positions[my_row] = position;
+}
+
+// Advances the lengths in place, after every CTA of the plan has read them.
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_lengths_kernel(int32_t *lengths, const int32_t *added, const int32_t *summary,
+                                                                          uint64_t requests) {
+    const uint64_t r = static_cast<uint64_t>(blockIdx.x) * kPlanThreads + threadIdx.x;
+    if (r < requests && !summary[0]) lengths[r] += added[r];
 }
 
 // ---- store ----------------------------------------------------------------------

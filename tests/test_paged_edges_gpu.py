@@ -71,3 +71,57 @@ def test_counts_near_2_31_are_declined(be):
                    dict(rows=(1 << 30) + 1, query_heads=1, kv_heads=1), dict(requests=1 << 62), dict(rows=1 << 62)):
         assert size(**change) == 0, change
         assert "2^30" in be.info().note.decode()
+
+
+def plan_args(abi, held, added, tables, free, rows, out):
+    """A plan's record over int32 tensors; `out`: lengths, starts, slots, positions, summary."""
+    return abi.PagedPlanArgs(
+        held=held.data_ptr(), added=added.data_ptr(), tables=tables.data_ptr(), free_pages=free.data_ptr(), head=0,
+        lengths=out[0].data_ptr(), starts=out[1].data_ptr(), slots=out[2].data_ptr(), positions=out[3].data_ptr(),
+        summary=out[4].data_ptr(), requests=held.numel(), table_stride=tables.shape[1], free_count=free.numel(), rows=rows,
+        base=7, stream=1)
+
+
+@pytest.mark.parametrize("requests,new", [(5, 3), (64, 16), (64, 17), (2000, 1), (300, 2000)])
+@pytest.mark.parametrize("short", [0, 1])
+def test_plan_advances_its_lengths_in_place(be, requests, new, short):
+    """lengths == held, below and above the 1,024 rows of one CTA, and where the step is declined."""
+    abi = load_package()._abi
+    held, added = ints([i * 37 % 200 for i in range(requests)]), ints([new] * requests)
+    rows = requests * new - short  # one row too few: declined as a whole
+    tables = torch.arange(requests * 40, dtype=torch.int32, device="cuda").view(requests, 40)
+    free = torch.arange(100000, 200000, dtype=torch.int32, device="cuda")
+    want_tables = tables.clone()
+    want = be.paged_plan(held, added, want_tables, free, rows, base=7)
+    out = [torch.full((n,), -9, dtype=torch.int32, device="cuda") for n in (requests, requests + 1, rows, rows, 4)]
+    out[0] = held  # in place
+    torch.cuda.synchronize()
+    assert be.lib.plamo_paged_plan(be.ctx, ctypes.byref(plan_args(abi, held, added, tables, free, rows, out))) == 1
+    for got, w in zip(out, want):
+        assert torch.equal(got, w)
+    assert torch.equal(tables, want_tables) and bool(want.summary[0]) == bool(short)
+
+
+def test_plan_declines_buffers_that_overlap(be):
+    abi = load_package()._abi
+    requests, rows = 8, 3000
+    buf = torch.zeros(20000, dtype=torch.int32, device="cuda")
+    held, added, tables, free = buf[:8], buf[100:108], buf[200:600].view(8, 50), buf[1000:1100]
+    out = [buf[2000:2008], buf[3000:3009], buf[4000:7000], buf[8000:11000], buf[12000:12004]]
+
+    def call(**change):
+        args = plan_args(abi, held, added, tables, free, rows, out)
+        for name, value in change.items():
+            setattr(args, name, value)
+        return be.lib.plamo_paged_plan(be.ctx, ctypes.byref(args))
+
+    launches = be.lib.plamo_cuda_kernel_launches(be.ctx)
+    at = buf.data_ptr()
+    for change in (dict(lengths=at + 4), dict(lengths=at + 4 * 100), dict(starts=at), dict(slots=at + 4 * 300),
+                   dict(positions=at + 4 * 1099), dict(summary=at + 4 * 107), dict(held=at + 4 * 201), dict(head=at + 4 * 3004),
+                   dict(slots=at + 4 * 7500), dict(tables=at + 4 * 990), dict(starts=at + 4 * 12003)):
+        assert call(**change) == 0, change
+        assert "overlap" in be.info().note.decode()
+    assert be.lib.plamo_cuda_kernel_launches(be.ctx) == launches
+    assert call() == 1
+    torch.cuda.synchronize()
