@@ -74,7 +74,8 @@ struct plamo_paged_plan_args {
     const int32_t *head;       /* NULL, or where to begin in free_pages: &summary[2] of an earlier plan */
     int32_t *lengths;          /* [requests] out: held + added */
     int32_t *starts;           /* [requests + 1] out: first batch row of each request */
-    int32_t *slots;            /* [rows] out: slot of each new row, -1 for padding */
+    int32_t *slots;            /* [rows] out: slot of each new row, -1 for padding, -2 where the table or the free
+                                  list has a negative page id or one from 2^25 up (the store reports the row) */
     int32_t *positions;        /* [rows] out: base + own row, 0 for padding */
     int32_t *summary;          /* [4] out: status bits, new rows, free-list entries used so far
                                   (head + pages taken), longest length */

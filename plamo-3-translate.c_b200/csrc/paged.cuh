@@ -178,7 +178,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanParams p) 
         int32_t *entry = d.tables + static_cast<uint64_t>(row_owner[at]) * d.table_stride + k;
         const int32_t id = k >= have ? d.free_pages[row_page[at] + k - have] : *entry;
         if (own % kPgRows == 0) *entry = id;  // a new page, reached by this row
-        if (id >= 0 && id < kPgMaxPages) slot = id * kPgRows + static_cast<int32_t>(own % kPgRows);
+        // (-2: no page has this id; the store reports it, where -1 is padding)
+        slot = id >= 0 && id < kPgMaxPages ? id * kPgRows + static_cast<int32_t>(own % kPgRows) : -2;
         position = static_cast<int32_t>(d.base + own);
     }
     d.slots[my_row] = slot;

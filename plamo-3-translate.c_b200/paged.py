@@ -21,7 +21,7 @@ class Plan(NamedTuple):
     """What a step's operators need of its rows (int32 tensors)."""
     lengths: object    # [requests] own rows after the step
     starts: object     # [requests + 1] first batch row of each request
-    slots: object      # [rows] page * 64 + row in the page, -1 for padding
+    slots: object      # [rows] page * 64 + row in the page, -1 for padding, -2 where the page id is none
     positions: object  # [rows]
     summary: object    # [4] status bits, new rows, free-list entries used so far, longest length
 

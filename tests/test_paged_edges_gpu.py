@@ -125,3 +125,25 @@ def test_plan_declines_buffers_that_overlap(be):
     assert be.lib.plamo_cuda_kernel_launches(be.ctx) == launches
     assert call() == 1
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bad", [-1, -64, 1 << 25, 2 ** 31 - 1])
+@pytest.mark.parametrize("where", ["table", "free list"])
+def test_rows_on_page_ids_that_are_none_are_reported(be, where, bad):
+    """Not taken for padding: the store leaves them out and says so."""
+    tables, free = ints([[0, -1, -1], [1, -1, -1]]), ints([2, 3, 4])
+    if where == "table":
+        tables[1, 0] = bad  # rows 70, 71 of the batch: held page of the second request
+    else:
+        free[1] = bad       # the second request's first new page: its rows from own row 64 on
+    plan = be.paged_plan(ints([10, 62]), ints([70, 4]), tables, free, 80)
+    lost = [70, 71] if where == "table" else [72, 73]
+    slots = plan.slots.tolist()
+    assert [i for i, s in enumerate(slots) if s == -2] == lost and slots[74:] == [-1] * 6
+    assert all(s >= 0 for i, s in enumerate(slots[:74]) if i not in lost) and plan.summary.tolist()[:2] == [0, 74]
+    pool = torch.zeros(5, 2, ROWS, 2, DIM, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    norm, table = torch.zeros(DIM, dtype=BF16, device="cuda"), torch.ones(100, DIM, device="cuda")
+    q = be.paged_store(torch.randn(80, 6 * DIM, device="cuda"), pool, plan.slots, plan.positions, norm, norm, table, status=status)
+    assert status.item() == 16 and (q[lost] == 0).all() and (q[74:] == 0).all()
+    assert int((pool.abs().amax((1, 3, 4)) > 0).sum()) == 72
