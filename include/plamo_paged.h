@@ -54,7 +54,7 @@ enum { PLAMO_PAGED_BF16 = 0, PLAMO_PAGED_FP32 = 1 };
 enum {
     PLAMO_PAGED_NO_PAGES = 1,   /* plan: the free list does not hold the pages the step needs */
     PLAMO_PAGED_TABLE = 2,      /* a request's rows do not fit its page table */
-    PLAMO_PAGED_BATCH_ROWS = 4, /* the new rows exceed the batch's row count */
+    PLAMO_PAGED_BATCH_ROWS = 4, /* the new rows exceed the batch's row count, or starts are out of order */
     PLAMO_PAGED_COUNT = 8,      /* a negative row count, or one past 2^31 - 1 */
     PLAMO_PAGED_PAGE = 16,      /* a page id or slot outside the pool */
     PLAMO_PAGED_POSITION = 32,  /* a position outside the rotation table */
@@ -137,8 +137,10 @@ uint64_t plamo_paged_attention_workspace(struct plamo_cuda *, const struct plamo
    every new row and query head (head h reads KV head h / (query_heads /
    kv_heads)). The row at position p sees the prefix's rows and its request's
    own rows up to itself, of these the last `window` when there is one. A row
-   that sees nothing gets zeros: padding, and rows whose request holds fewer
-   rows (lengths) than it adds, before the first held one. Rows past a request's length, of other
+   that sees nothing gets zeros: padding, rows before starts[0], and rows whose
+   request holds fewer rows (lengths) than it adds, before the first held one.
+   Where the starts do not rise from 0 to at most `rows`, `status` gets
+   PLAMO_PAGED_BATCH_ROWS; where they decrease, every row gets zeros. Rows past a request's length, of other
    requests and after a query's own never reach its result, whatever they
    hold. Scores, softmax sums and products are FP32 for both types (against
    a BF16 pool's values the softmax weights go in as two BF16 terms, 16 bits). */

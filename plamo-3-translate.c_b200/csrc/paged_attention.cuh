@@ -67,7 +67,7 @@ struct PagedAttnParams {
     float *tile_sum;               // [slot][tile_pairs][128], [slot][tile_pairs] {m, l}
     float2 *tile_ml;
 };
-enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kRtRun, kRtLonger, kTlHeader };
+enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlFirst, kTlTaken, kRtRun, kRtLonger, kTlHeader };
 constexpr int kTlShortPairs = 32; // requests of up to so many keep their own rows in the row kernel
 constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 
@@ -1073,7 +1073,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         }
     }
     // Rows that no request has, and tiles without a key.
-    const int32_t taken = p.requests ? max(p.starts[p.requests], 0) : 0;
     const auto clear = [&](int32_t row) {
         for (int32_t x = threadIdx.x; x < p.qh * kPgDim / 4; x += blockDim.x) {
             if constexpr (F32) pg_store4(static_cast<float *>(p.out) + row * p.out_stride + 4 * x, make_float4(0.f, 0.f, 0.f, 0.f));
@@ -1081,7 +1080,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         }
     };
 #pragma unroll 1
-    for (int32_t row = min(taken, p.rows) + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
+    for (int32_t row = blockIdx.x; row < p.header[kTlFirst]; row += gridDim.x) clear(row);
+#pragma unroll 1
+    for (int32_t row = p.header[kTlTaken] + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
 #pragma unroll 1
     for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); tile < tiles; tile += gridDim.x)
         if (p.tile_unit[tile + 1] == p.tile_unit[tile])

@@ -66,7 +66,9 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     const int32_t r0 = min(p.requests, tid * per), r1 = min(p.requests, r0 + per);
     if (tid == 0) first_at = INT32_MAX;
     __syncthreads();
-    // 64 bits: starts that decrease make ranges that overlap, and their sums more than there is of either.
+    // 64 bits: starts that decrease make ranges that overlap, and their sums more than there is of
+    // either. Nothing is laid out then.
+    int decreases = 0;
     int64_t short_rows = 0, prompt_tiles = 0, all_short_rows, all_tiles = 0;
     int32_t lowest = INT32_MAX;
 #pragma unroll 1
@@ -74,7 +76,8 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         const OwnShape s = own_shape(p, r);
         if (p.lengths[r] > p.max_length) pg_flag(p.status, PLAMO_PAGED_TABLE);
         if (p.lengths[r] < 0) pg_flag(p.status, PLAMO_PAGED_COUNT);
-        if (p.starts[r] < 0 || p.starts[r + 1] < p.starts[r] || p.starts[r + 1] > p.rows) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
+        if (p.starts[r] < 0 || p.starts[r + 1] > p.rows) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
+        decreases |= p.starts[r + 1] < p.starts[r];
         if (request_is_short(p, s)) {
             short_rows += s.rows;
             if (s.rows) lowest = min(lowest, max(s.at0, 0));
@@ -86,7 +89,8 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     if ((tid & 31) == 0) atomicMin(&first_at, lowest);
     int64_t short_at = pg_block_scan<kRtThreads>(short_rows, sums, &all_short_rows);
     int64_t tile_at = p.tile_rows ? pg_block_scan<kRtThreads>(prompt_tiles, sums, &all_tiles) : 0;
-    const int32_t all_short = static_cast<int32_t>(min(all_short_rows, static_cast<int64_t>(p.rows)));
+    const bool ordered = !__syncthreads_or(decreases);
+    const int32_t all_short = ordered ? static_cast<int32_t>(all_short_rows) : 0;
     int32_t pre_tiles = 0;
     TileShape pre{};
     if (p.tile_rows && p.prefix) {
@@ -95,7 +99,7 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         pre.pre1 = (p.prefix + p.tile_keys - 1) / p.tile_keys;
         if (p.window && first_at != INT32_MAX) pre.pre0 = min(max(p.prefix + first_at - p.window + 1, 0) / p.tile_keys, pre.pre1);
     }
-    bool fits = pre_tiles + all_tiles <= p.tile_cap;  // (no tile kernel: 0 <= 0)
+    bool fits = ordered && pre_tiles + all_tiles <= p.tile_cap;  // (no tile kernel: 0 <= 0)
     if (!fits) pre_tiles = all_tiles = 0;
     const int32_t all = pre_tiles + static_cast<int32_t>(all_tiles);
 #pragma unroll 1
@@ -138,11 +142,14 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         total += sum;
     }
     fits = fits && total * p.kh <= INT32_MAX - 256;
-    if (!fits) {  // only starts or lengths that no pool holds ask for this
-        if (tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
-    }
     if (tid == 0) {
-        p.header[kTlShortRows] = all_short;
+        const int32_t first = p.requests ? p.starts[0] : 0, taken = p.requests ? p.starts[p.requests] : 0;
+        if (!fits || first) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
+        // Rows of no request, [0, first) and [taken, rows), become zeros; so do all of a batch that
+        // is not laid out.
+        p.header[kTlFirst] = fits ? min(max(first, 0), p.rows) : 0;
+        p.header[kTlTaken] = fits ? min(max(taken, 0), p.rows) : 0;
+        p.header[kTlShortRows] = fits ? all_short : 0;
         const int32_t units = fits ? static_cast<int32_t>(total * p.kh) : 0;
         const int32_t ctas = p.tile_rows ? min(p.tile_grid, (units + kTlMinUnits - 1) / kTlMinUnits) : 0;
         p.header[kTlCtas] = ctas;

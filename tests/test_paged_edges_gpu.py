@@ -147,3 +147,34 @@ def test_rows_on_page_ids_that_are_none_are_reported(be, where, bad):
     q = be.paged_store(torch.randn(80, 6 * DIM, device="cuda"), pool, plan.slots, plan.positions, norm, norm, table, status=status)
     assert status.item() == 16 and (q[lost] == 0).all() and (q[74:] == 0).all()
     assert int((pool.abs().amax((1, 3, 4)) > 0).sum()) == 72
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("prefix", [0, 40])
+@pytest.mark.parametrize("new", [1, 60])
+def test_rows_before_the_first_start_are_zero_and_reported(be, new, prefix, dtype):
+    s = Scene([(100, new), (70, 1)], prefix, 8, 2, dtype, seed=9)
+    want, tol = s.expected()
+    first = 3
+    s.q = torch.cat([s.q.new_full((first, 8, DIM), 2.0), s.q])
+    s.starts = s.starts + first
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full_like(s.q, float("nan"))
+    assert attend(be, s, out=out, status=status) is out
+    assert status.item() == 4 and (out[:first] == 0).all()
+    check(out[first:], want, tol, "the requests' rows")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("prefix", [0, 40])
+@pytest.mark.parametrize("rows,starts", [(20, [0, 12, 5, 20]), (20, [0, 6, 0, 20]), (300, [0, 200, 100, 250]), (20, [9, 4, 2, 0])])
+def test_starts_that_decrease_leave_zeros(be, rows, starts, prefix, dtype):
+    s = Scene([(100, 1)] * 3, prefix, 8, 2, dtype, seed=9)
+    s.q = torch.randn(rows, 8, DIM, device="cuda").to(dtype)
+    s.starts = ints(starts)
+    for _ in range(2):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = torch.full_like(s.q, float("nan"))
+        attend(be, s, out=out, status=status)
+        assert status.item() & 4 and not status.item() & 64
+        assert (out == 0).all()
