@@ -183,9 +183,14 @@ __device__ __forceinline__ float pg_exp2(float x) {  // 2^x to about 2 ulp, 2^-i
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// A part's {m, l}: m of -inf says that it saw nothing, so a part that saw scores
-// of which none is a number (no maximum, l not a number) gets another.
+// A part's {m, l}: m of -inf says that it saw no score above that and has no say,
+// so a part that saw scores of which none is a number (no maximum, l not a
+// number) gets another.
 __device__ __forceinline__ float2 pg_ml(float m, float l) { return make_float2(l != l && m == -INFINITY ? 0.0f : m, l); }
+// What the sums of a row at own row `at` are multiplied with. A row that is held
+// sees itself at least: where l is zero all the same, every score is -inf, and
+// the result is none (0 / 0). One that is not held sees nothing: zero.
+__device__ __forceinline__ float pg_inverse(int32_t at, float l) { return at < 0 ? 0.0f : 1.0f / l; }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -869,9 +874,9 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                 if (it.direct) {
                     const int32_t m = it.tile * PAIRS + pair;
                     if (m >= it.rows * p.group) continue;
-                    const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
-                    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                     const int32_t i = p.by_group.div(m);
+                    const float inv = pg_inverse(it.at0 + i, l);
+                    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                     const uint64_t at = (it.row0 + i) * p.out_stride + (it.head * p.group + m - i * p.group) * kPgDim + d;
                     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + at, v);
                     else pg_store4(static_cast<uint16_t *>(p.out) + at, v);
@@ -962,8 +967,8 @@ __device__ __forceinline__ void join_parts(const PartList &a, const PartList &b,
     for (int k = RES; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
 }
 template <bool F32>
-__device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row, int32_t head, float4 o, float l, float top) {
-    const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
+__device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row, int32_t at, int32_t head, float4 o, float l) {
+    const float inv = pg_inverse(at, l);
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     const uint64_t to = row * p.out_stride + head * kPgDim + 4 * (threadIdx.x & 31);
     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + to, o);
@@ -1037,14 +1042,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                     if (f != 0.0f) v = make_float4(fmaf(f, u.x, v.x), fmaf(f, u.y, v.y), fmaf(f, u.z, v.z), fmaf(f, u.w, v.w));
                     l = fmaf(f, ml.y, l);
                 }
-                join_store<F32>(p, e.x, head0 + warp, v, l, top);
+                join_store<F32>(p, e.x, e.y, head0 + warp, v, l);
             }
             __syncthreads();
         } else {
 #pragma unroll
             for (int i = 0; i < RES; ++i) {
-                const float li = __shfl_sync(0xffffffffu, l, i), ti = __shfl_sync(0xffffffffu, top, i);
-                if (!((skip >> i) & 1u)) join_store<F32>(p, e.x, head0 + i, o[i], li, ti);
+                const float li = __shfl_sync(0xffffffffu, l, i);
+                if (!((skip >> i) & 1u)) join_store<F32>(p, e.x, e.y, head0 + i, o[i], li);
             }
         }
     }
@@ -1066,10 +1071,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         join_parts<RES>(shared, own, 0, 1, o, l, top);
 #pragma unroll
         for (int i = 0; i < RES; ++i) {
-            const float li = __shfl_sync(0xffffffffu, l, i), ti = __shfl_sync(0xffffffffu, top, i);
+            const float li = __shfl_sync(0xffffffffu, l, i);
             if (pair0 + i >= pairs) break;
             const int32_t row = p.by_group.div(pair0 + i);
-            join_store<F32>(p, row0 + row, kv * p.group + pair0 + i - row * p.group, o[i], li, ti);
+            join_store<F32>(p, row0 + row, p.tile_shape[tile].at0 + row, kv * p.group + pair0 + i - row * p.group, o[i], li);
         }
     }
     // Rows that no request has, and tiles without a key.

@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles;
             const int32_t slot = w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
             const bool odd = *reinterpret_cast<volatile int *>(&odd_values);
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const float inv = pg_inverse(at, l);
             // Through shared memory (the queries' place: the scores are done with them), so that rows
             // leave 256 bytes at a time: the whole result, or half of the partial sums.
             const int64_t to = !there ? -1 : whole ? row * static_cast<int64_t>(p.out_stride) + head * kPgDim
@@ -976,7 +976,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             if (row < 0) continue;
             const uint64_t to = whole ? row * p.out_stride + head_of(pair) * kPgDim : (static_cast<uint64_t>(slot) * kTfPairs + pair) * kPgDim;
             const float2 ml = pg_ml(m[i], sum);
-            const float inv = !whole ? 1.0f : ml.x == -INFINITY ? 0.0f : 1.0f / sum;
+            const float inv = whole ? pg_inverse(pair_at[pair], sum) : 1.0f;
             float *dst = (whole ? static_cast<float *>(p.out) : p.tile_sum) + to + 4 * tx;
             *reinterpret_cast<float4 *>(dst) = make_float4(o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
             *reinterpret_cast<float4 *>(dst + 64) = make_float4(o[i][4] * inv, o[i][5] * inv, o[i][6] * inv, o[i][7] * inv);

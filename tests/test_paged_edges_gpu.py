@@ -178,3 +178,30 @@ def test_starts_that_decrease_leave_zeros(be, rows, starts, prefix, dtype):
         attend(be, s, out=out, status=status)
         assert status.item() & 4 and not status.item() & 64
         assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("prefix", [0, 100])
+@pytest.mark.parametrize("requests", [[(0, 1), (70, 1), (200, 1)], [(0, 3), (70, 2), (5, 4)], [(0, 90), (70, 40), (300, 1)]])
+def test_rows_all_of_whose_scores_are_minus_infinity(be, requests, prefix, dtype):
+    """They see keys, so theirs is 0 / 0, no result; one finite score is the whole result;
+    rows that are not held stay zero."""
+    s = Scene(requests, prefix, 8, 2, dtype, seed=5, spread=0.2)
+    s.q[..., 0] = 1.0
+    s.pool[s.prefix_pages.long(), 0, :, :, 0] = -float("inf")
+    for r, (held, new) in enumerate(requests):
+        for row in range(held + new):
+            s.pool[s.tables[r, row // ROWS], 0, row % ROWS, :, 0] = -float("inf")
+    # The last request's own row 2 (its new row, or one held) has an ordinary key.
+    r, (held, new) = len(requests) - 1, requests[-1]
+    s.pool[s.tables[r, 0], 0, 2, :, 0] = 0.5
+    got = attend(be, s)
+    first = int(s.starts[r])
+    assert torch.isnan(got[:first]).all()
+    value = s.own[r][1][2].repeat_interleave(4, 0)
+    want = value.expand(new, 8, DIM).clone()
+    check(got[first:], want, 2.0 ** -8 * want.abs() + 1e-30 if dtype == BF16 else 2.0 ** -20 * want.abs() + 1e-30, "one score")
+    s.lengths = s.lengths.clone()
+    s.lengths[0] = 0
+    got = attend(be, s)
+    assert (got[:requests[0][1]] == 0).all() and torch.isnan(got[requests[0][1]:first]).all()
