@@ -110,6 +110,8 @@ def serve(model, prefix, prompts, steps, shared):
         held, added = plan.lengths, torch.ones(requests, **ints)
         if plan.summary[0].item():
             raise RuntimeError(f"plan declined: status {plan.summary[0].item()}")
+    if status := model.backend.paged_status():
+        raise RuntimeError(f"the layers' calls report status {status}")
     return torch.stack(outputs)
 
 

@@ -34,7 +34,8 @@
  * What only the device can see is reported there: rows whose slot or position
  * lies outside its array are left out, a page outside the pool reads as rows
  * of zeros, nothing out of range is read or written, and `status` (a device
- * word, may be NULL) gets a PLAMO_PAGED_* bit. Buffers must stay valid until
+ * word) gets a PLAMO_PAGED_* bit; where it is NULL a word of the context does,
+ * which plamo_paged_status reads. Buffers must stay valid until
  * the stream has run the call; calls with a workspace of their own may overlap
  * on different streams. Every call can be captured in a CUDA graph: none
  * allocates, waits or reads a length on the host.
@@ -110,6 +111,13 @@ struct plamo_paged_store_args {
    it as they are. rotate pairs dimension d with d + 64: the lower becomes
    a*cos - b*sin, the upper b*cos + a*sin. */
 int plamo_paged_store(struct plamo_cuda *, const struct plamo_paged_store_args *);
+
+/* The PLAMO_PAGED_* bits that store and attention calls without a word of their
+   own have set since it was last asked; they are then clear. Waits for the
+   context's own stream: a call on another one counts once that has run it
+   (synchronise it first). PLAMO_PAGED_FAILED also where the word cannot be
+   read. Not while a stream is being captured. */
+uint32_t plamo_paged_status(struct plamo_cuda *);
 
 struct plamo_paged_attention_args {
     const void *q;           /* [rows][query_heads][128] of the pool's type, rows q_stride elements apart */

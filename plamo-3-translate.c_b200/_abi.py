@@ -275,6 +275,7 @@ PAGED_BF16, PAGED_FP32 = 0, 1  # PLAMO_PAGED_BF16, PLAMO_PAGED_FP32
 PAGED_SIGNATURES = {
     "plamo_paged_plan": (c_int, [P, POINTER(PagedPlanArgs)]),
     "plamo_paged_store": (c_int, [P, POINTER(PagedStoreArgs)]),
+    "plamo_paged_status": (c_uint32, [P]),
     "plamo_paged_attention": (c_int, [P, POINTER(PagedAttentionArgs)]),
     "plamo_paged_attention_workspace": (c_uint64, [P, POINTER(PagedAttentionArgs)]),
 }

@@ -194,6 +194,7 @@ struct plamo_cuda {
     int pt_stages;      // ring stages of the persistent step (PLAMO_CUDA_PT_STAGES; 0: as many as fit)
     int gemv_ctas;
     uint32_t *sink;
+    uint32_t *paged_status;  // status bits of paged calls that were given no word, and a copy being read
     float *static_scratch;  // device address of g_linear_static_scratch (set on first use)
     std::map<uint64_t, KvPool> kv_pools;  // by floats per K row (kv heads x head dim)
     char *staging = nullptr;   // grow-only device staging of linear / mlp (host buffers in and out)
@@ -1724,8 +1725,12 @@ struct plamo_cuda *plamo_cuda_open(const struct plamo_cuda_config *config, char 
     if ((e = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking)) != cudaSuccess ||
         (e = cudaEventCreate(&c->ev0)) != cudaSuccess || (e = cudaEventCreate(&c->ev1)) != cudaSuccess ||
         (e = cudaMallocHost(&c->pinned_u32, 64 * 1024 * 4)) != cudaSuccess ||
-        (e = cudaMalloc(&c->sink, 4)) != cudaSuccess) {
+        (e = cudaMalloc(&c->sink, 4)) != cudaSuccess || (e = cudaMalloc(&c->paged_status, 8)) != cudaSuccess ||
+        (e = cudaMemsetAsync(c->paged_status, 0, 8, c->stream)) != cudaSuccess ||
+        (e = cudaStreamSynchronize(c->stream)) != cudaSuccess) {
         if (error && cap) snprintf(error, cap, "cannot create CUDA stream: %s", cudaGetErrorString(e));
+        cudaFree(c->paged_status);
+        cudaFree(c->sink);
         if (c->pinned_u32) cudaFreeHost(c->pinned_u32);
         if (c->ev1) cudaEventDestroy(c->ev1);
         if (c->ev0) cudaEventDestroy(c->ev0);
@@ -1797,6 +1802,7 @@ void plamo_cuda_close(struct plamo_cuda *c) {
     for (Range &r : c->ranges) cudaFree(r.dev);
     cudaFreeHost(c->pinned_u32);
     cudaFree(c->sink);
+    cudaFree(c->paged_status);
     cudaFree(c->staging);
     cudaEventDestroy(c->ev0);
     cudaEventDestroy(c->ev1);
@@ -3408,6 +3414,8 @@ ContextDevice::~ContextDevice() {
 cudaStream_t context_stream(const plamo_cuda *c) { return c->stream; }
 int context_sms(const plamo_cuda *c) { return c->sm_count; }
 bool context_pdl(const plamo_cuda *c) { return c->pdl; }
+uint32_t *context_paged_status(const plamo_cuda *c) { return c->paged_status; }
+bool context_note(plamo_cuda *c, const char *what, cudaError_t e) { return note(c, what, e); }
 int context_decline(plamo_cuda *c, const char *why) {
     c->info.declines++;
     snprintf(c->info.note, sizeof c->info.note, "%s", why);

@@ -24,8 +24,12 @@ private:
 cudaStream_t context_stream(const plamo_cuda *c);
 int context_sms(const plamo_cuda *c);
 bool context_pdl(const plamo_cuda *c);
+// Two device words: status bits of paged calls that were given no word of their own, and a copy being read.
+uint32_t *context_paged_status(const plamo_cuda *c);
 // Returns 0 (declined) with `why` in the context's note.
 int context_decline(plamo_cuda *c, const char *why);
+// Records an error, if any. True when there is none.
+bool context_note(plamo_cuda *c, const char *what, cudaError_t e);
 // Counts a launch; records its error, if any. True when it was enqueued.
 bool context_launched(plamo_cuda *c, const char *what, cudaError_t e);
 

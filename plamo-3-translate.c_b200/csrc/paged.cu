@@ -140,7 +140,7 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.q_stride = d->q_stride;
     p.out_stride = d->out_stride;
     p.table_stride = d->table_stride;
-    p.status = d->status;
+    p.status = d->status ? d->status : context_paged_status(c);
     p.rows = static_cast<int32_t>(d->rows);
     p.requests = static_cast<int32_t>(d->requests);
     p.pages = static_cast<int32_t>(d->pages);
@@ -209,9 +209,11 @@ bool run_store(plamo_cuda *c, const plamo_paged_store_args *d, cudaStream_t stre
     const bool wide = d->rows * heads >= 4ull * 8 * static_cast<uint64_t>(context_sms(c));
     const uint64_t units = d->rows * ceil_div(heads, wide ? 8 : 1);
     const dim3 grid(static_cast<uint32_t>(ceil_div(units, 8)));
+    plamo_paged_store_args args = *d;
+    if (!args.status) args.status = context_paged_status(c);
     if (wide)
-        return launch(c, "paged_store", paged_store_kernel<In, Out, 8>, grid, dim3(256), 0, stream, false, *d);
-    return launch(c, "paged_store", paged_store_kernel<In, Out, 1>, grid, dim3(256), 0, stream, false, *d);
+        return launch(c, "paged_store", paged_store_kernel<In, Out, 8>, grid, dim3(256), 0, stream, false, args);
+    return launch(c, "paged_store", paged_store_kernel<In, Out, 1>, grid, dim3(256), 0, stream, false, args);
 }
 
 }  // namespace
@@ -295,6 +297,17 @@ int plamo_paged_store(struct plamo_cuda *c, const struct plamo_paged_store_args 
     const bool ok = in32 ? (out32 ? run_store<float, float>(c, d, stream) : run_store<float, uint16_t>(c, d, stream))
                          : (out32 ? run_store<uint16_t, float>(c, d, stream) : run_store<uint16_t, uint16_t>(c, d, stream));
     return ok ? 1 : -1;
+}
+
+uint32_t plamo_paged_status(struct plamo_cuda *c) {
+    if (!c) return 0;
+    ContextDevice device(c);
+    uint32_t bits = 0, *words = context_paged_status(c);
+    const cudaStream_t stream = context_stream(c);
+    const bool ok = launch(c, "paged_status", paged_status_kernel, dim3(1), dim3(1), 0, stream, false, words) &&
+                    context_note(c, "paged_status", cudaMemcpyAsync(&bits, words + 1, 4, cudaMemcpyDeviceToHost, stream)) &&
+                    context_note(c, "paged_status", cudaStreamSynchronize(stream));
+    return ok ? bits : PLAMO_PAGED_FAILED;
 }
 
 uint64_t plamo_paged_attention_workspace(struct plamo_cuda *c, const struct plamo_paged_attention_args *d) {

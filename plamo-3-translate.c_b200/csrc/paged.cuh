@@ -14,9 +14,9 @@ constexpr int kPgDim = PLAMO_PAGED_DIM;
 constexpr int32_t kPgMaxPages = 1 << 25;
 constexpr uint64_t kPgMaxCount = 1u << 30;
 
-__device__ __forceinline__ void pg_flag(uint32_t *status, uint32_t bit) {
-    if (status) atomicOr(status, bit);
-}
+__device__ __forceinline__ void pg_flag(uint32_t *status, uint32_t bit) { atomicOr(status, bit); }
+// Takes the bits of words[0] to words[1].
+__global__ void paged_status_kernel(uint32_t *words) { words[1] = atomicExch(words, 0u); }
 
 // Exclusive scan of one 64-bit value per thread over a block of NT threads;
 // *total gets the sum. `sm` holds NT / 32 values. Ends with a barrier.

@@ -606,6 +606,10 @@ class Backend:
         return paged.attention(self, q, pool, starts, lengths, tables, prefix_pages, prefix_rows, window, scale, out,
                                status)
 
+    def paged_status(self):
+        """PLAMO_PAGED_* bits of stores and attention calls without a status tensor; see paged.status."""
+        return paged.status(self)
+
     def __enter__(self):
         return self
 

@@ -7,7 +7,8 @@ and attends (`attention`). Calls are enqueued on torch's current stream and
 return without waiting; tensors they allocate come from torch's allocator.
 Wrong arguments raise ValueError, tensors of another GPU than the backend's
 among them. What only the GPU can see is reported as PLAMO_PAGED_* bits, in the
-plan's summary or in a `status` tensor (one int32, zeroed by the caller).
+plan's summary and in a `status` tensor (one int32, zeroed by the caller), or
+where a call is given none in a word of the backend's that `status()` reads.
 """
 import ctypes
 from typing import NamedTuple
@@ -207,6 +208,14 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
     args.workspace, args.workspace_bytes = workspace.data_ptr(), size
     _run(backend, backend.lib.plamo_paged_attention, args)
     return out
+
+
+def status(backend):
+    """PLAMO_PAGED_* bits set by stores and attention calls without a `status`
+    tensor since last asked (they are then clear). Waits for torch's current
+    stream; calls on others count once those have run them."""
+    _torch().cuda.current_stream(backend.device).synchronize()
+    return backend.lib.plamo_paged_status(backend.ctx)
 
 
 def _rows(torch, t, pool, device, name):

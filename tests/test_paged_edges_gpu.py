@@ -205,3 +205,26 @@ def test_rows_all_of_whose_scores_are_minus_infinity(be, requests, prefix, dtype
     s.lengths[0] = 0
     got = attend(be, s)
     assert (got[:requests[0][1]] == 0).all() and torch.isnan(got[requests[0][1]:first]).all()
+
+
+def test_calls_without_a_status_word_report_to_the_backend(be):
+    be.paged_status()
+    s = Scene([(100, 1), (200, 1)], 0, 8, 2, BF16, seed=9)
+    attend(be, s)
+    assert be.paged_status() == 0
+    s.tables[0, 1] = -1
+    attend(be, s)
+    s.lengths = ints([2 ** 31 - 1, 201])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(be, s)
+        assert be.paged_status() == 16 | 2
+        assert be.paged_status() == 0
+    pool, norm = torch.zeros(1, 2, ROWS, 2, DIM, device="cuda"), torch.zeros(DIM, dtype=BF16, device="cuda")
+    store = (torch.ones(2, 6 * DIM, device="cuda"), pool, ints([0, 1]), ints([0, 9]), norm, norm, torch.ones(5, DIM, device="cuda"))
+    be.paged_store(*store)
+    own = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert be.paged_status() == 32
+    be.paged_store(*store, status=own)  # a word of its own: there only
+    assert be.paged_status() == 0 and own.item() == 32
