@@ -126,10 +126,12 @@ def main(argv=None):
     backend = load_package().Backend(device=0)
     try:
         hidden = 512
-        model = Model(backend, a.layers, hidden, 8, 2, 100, torch.float32 if a.fp32 else torch.bfloat16, a.prefix + 400)
+        lengths = [5 + 31 * i % 90 for i in range(a.requests)]
+        model = Model(backend, a.layers, hidden, 8, 2, 100, torch.float32 if a.fp32 else torch.bfloat16,
+                      a.prefix + max(lengths) + a.steps)
         g = torch.Generator().manual_seed(2)
         prefix = torch.randn(a.prefix, hidden, generator=g).cuda()
-        prompts = [torch.randn(5 + 31 * i % 90, hidden, generator=g).cuda() for i in range(a.requests)]
+        prompts = [torch.randn(n, hidden, generator=g).cuda() for n in lengths]
         together = serve(model, prefix, prompts, a.steps, shared=True)
         alone = torch.cat([serve(model, prefix, [p], a.steps, shared=False) for p in prompts], 1)
         off = ((together - alone).norm() / alone.norm()).item()

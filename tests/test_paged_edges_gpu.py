@@ -228,3 +228,14 @@ def test_calls_without_a_status_word_report_to_the_backend(be):
     assert be.paged_status() == 32
     be.paged_store(*store, status=own)  # a word of its own: there only
     assert be.paged_status() == 0 and own.item() == 32
+
+
+def test_example_of_many_steps_has_a_rotation_for_each():
+    """FP32 and one layer: the bound of a step's roundings in the shorter run holds, whatever the steps."""
+    import importlib.util
+    import os
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("paged_batch", os.path.join(ROOT, "examples", "paged_batch.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    assert module.main(["--fp32", "--steps", "420", "--requests", "1", "--layers", "1", "--prefix", "3"]) <= 2e-4
