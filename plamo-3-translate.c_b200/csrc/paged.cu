@@ -58,7 +58,7 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
-    uint32_t row_tile, prefix_tiles, row_slots, workers, tile_rows, tile_grid, tile_cap;
+    uint32_t prefix_tiles, row_slots, workers, tile_rows, tile_grid, tile_cap;
     uint64_t record, row_sum, row_ml;
     uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
 };
@@ -84,17 +84,14 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
         a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
     }
-    // Eight pairs to a tile while a request has no more on average (the heads of
-    // a group of eight, one row each); FP32 sums leave no registers for more.
-    a.row_tile = d->type == PLAMO_PAGED_FP32 || pairs <= 8 * d->requests ? 8 : 16;
-    a.prefix_tiles = prefix_pages && !a.tile_rows ? static_cast<uint32_t>(ceil_div(pairs, a.row_tile)) : 0;
+    a.prefix_tiles = prefix_pages && !a.tile_rows ? static_cast<uint32_t>(ceil_div(pairs, kRtPairs)) : 0;
     a.workers = static_cast<uint32_t>(2 * sms - 1);  // beside the schedule's CTA
     // A slot for each strip (a row tile and KV head; every request's last tile
     // may be partial), one more for each CTA. Beside the tile kernel only
     // requests of up to kTlShortPairs pairs are here.
-    const uint64_t tiles = pairs / a.row_tile + std::min<uint64_t>(d->requests, d->rows);
+    const uint64_t tiles = pairs / kRtPairs + std::min<uint64_t>(d->requests, d->rows);
     a.row_slots = static_cast<uint32_t>(std::min<uint64_t>(
-        a.workers + d->kv_heads * (a.prefix_tiles + (a.tile_rows ? std::min<uint64_t>(tiles, kTlShortPairs / a.row_tile * d->requests) : tiles)),
+        a.workers + d->kv_heads * (a.prefix_tiles + (a.tile_rows ? std::min<uint64_t>(tiles, kTlShortPairs / kRtPairs * d->requests) : tiles)),
         INT32_MAX));
     uint64_t at = 0;
     auto part = [&](uint64_t bytes) {
@@ -105,8 +102,8 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     a.header = part(kTlHeader * 4);
     a.short_list = part(d->rows * sizeof(int4));
     a.record = part((d->requests + 1) * sizeof(int4));
-    a.row_sum = part(static_cast<uint64_t>(a.row_slots) * a.row_tile * kPgDim * 4);
-    a.row_ml = part(static_cast<uint64_t>(a.row_slots) * a.row_tile * sizeof(float2));
+    a.row_sum = part(static_cast<uint64_t>(a.row_slots) * kRtPairs * kPgDim * 4);
+    a.row_ml = part(static_cast<uint64_t>(a.row_slots) * kRtPairs * sizeof(float2));
     if (a.tile_rows) {
         // Two runs of a CTA may end inside a prompt's tile; every run of a prefix tile is a part.
         const uint64_t shared = prefix_pages ? a.tile_grid + ceil_div(d->rows, a.tile_rows) * d->kv_heads : 0;
@@ -161,8 +158,6 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.short_list = reinterpret_cast<int4 *>(ws + a.short_list);
     p.row_sum = reinterpret_cast<float *>(ws + a.row_sum);
     p.row_ml = reinterpret_cast<float2 *>(ws + a.row_ml);
-    p.row_tile = static_cast<int32_t>(a.row_tile);
-    p.row_shift = a.row_tile == 8 ? 3 : 4;
     p.row_slots = static_cast<int32_t>(a.row_slots);
     p.prefix_tiles = static_cast<int32_t>(a.prefix_tiles);
     p.workers = static_cast<int32_t>(a.workers);
@@ -179,10 +174,7 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
         p.tile_sum = reinterpret_cast<float *>(ws + a.tile_sum);
         p.tile_ml = reinterpret_cast<float2 *>(ws + a.tile_ml);
     }
-    void (*rows)(const CUtensorMap, const PagedAttnParams) = paged_rows_kernel<F32, 1>;
-    if constexpr (!F32)
-        if (a.row_tile == 16) rows = paged_rows_kernel<F32, 2>;
-    if (!launch(c, "paged_attention rows", rows, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
+    if (!launch(c, "paged_attention rows", paged_rows_kernel<F32>, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
         (a.tile_rows && !launch(c, "paged_attention tiles", F32 ? paged_tile_f32_kernel : paged_tile_kernel, dim3(a.tile_grid),
                                 dim3(F32 ? kTfThreads : kTlThreads), F32 ? kTfSmem : kTlSmem, stream, true, page_map, p)))
         return false;
@@ -223,10 +215,9 @@ cudaError_t paged_configure() {
     const auto allow = [](auto kernel, int bytes) {
         return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-    cudaError_t e = allow(paged_rows_kernel<false, 1>, kRtSmem);
-    if (e == cudaSuccess) e = allow(paged_rows_kernel<false, 2>, kRtSmem);
-    if (e == cudaSuccess) e = allow(paged_rows_kernel<true, 1>, kRtSmem);
-      if (e == cudaSuccess) e = allow(paged_tile_kernel, kTlSmem);
+    cudaError_t e = allow(paged_rows_kernel<false>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_rows_kernel<true>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_kernel, kTlSmem);
     if (e == cudaSuccess) e = allow(paged_tile_f32_kernel, kTfSmem);
     return e;
 }

@@ -44,8 +44,7 @@ struct PagedAttnParams {
     int32_t prefix, window;  // window: rows seen, 0 for all
     int32_t max_length;      // own rows a page table holds
     float scale2;            // scale * log2(e)
-    int32_t row_tile, row_shift;  // pairs to a tile of the row kernel: 1 << row_shift
-    // Its partial results, unnormalised: [slot][row_tile][128] sums and [slot][row_tile] {m, l}.
+    // The row kernel's partial results, unnormalised: [slot][kRtPairs][128] sums and [slot][kRtPairs] {m, l}.
     float *row_sum;
     float2 *row_ml;
     int4 *row_record;      // [requests + 1] where a request's units begin, its pages, its first strip, tiles; last: the prefix
@@ -72,8 +71,14 @@ constexpr int kTlShortPairs = 32; // requests of up to so many keep their own ro
 constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 
 // The row kernel works on slabs of 16 keys, the M of one mma.sync, against
-// tiles of 8 or 16 (row, head-in-group) pairs, its N.
+// tiles of 8 (row, head-in-group) pairs, its N. Tiles of 16 for more pairs than
+// that to a request read its keys half as often, in twice the code, which a CTA's
+// few slabs do not pay for: 61 requests of 1,000 rows and 16 heads 47 us against
+// 23, 8 of 450 rows and two rows of eight heads 28 against 14; only one request
+// of four rows over 131,072, 32 pairs whose keys outlast the L2 cache, gained
+// (135 against 177).
 constexpr int kRtKeys = 16;
+constexpr int kRtPairs = 8;
 constexpr int kRtWarps = 6;                      // computing warps, a slab each in turn
 constexpr int kRtThreads = 32 * (kRtWarps + 1);  // and the copying warp
 constexpr int kRtMinPages = 1;                   // least pages worth a CTA (8 requests of 450 FP32 rows: 18.5 us; 22.6 with 2)
@@ -107,10 +112,10 @@ __device__ __forceinline__ OwnShape own_shape(const PagedAttnParams &p, int32_t 
     const int32_t first = p.window ? max(max(s.at0, 0) - p.window + 1, 0) : 0;
     s.page0 = first / kPgRows;
     s.pages = s.rows ? max((s.length + kPgRows - 1) / kPgRows - s.page0, 0) : 0;
-    s.tiles = (s.rows * p.group + p.row_tile - 1) >> p.row_shift;
+    s.tiles = (s.rows * p.group + kRtPairs - 1) / kRtPairs;
     return s;
 }
-// Short requests' own rows go through the row kernel, 8 or 16 pairs at a time;
+// Short requests' own rows go through the row kernel, eight pairs at a time;
 // the others are the tile kernel's, where there is one.
 __device__ __forceinline__ bool request_is_short(const PagedAttnParams &p, const OwnShape &s) {
     return !p.tile_rows || s.rows * p.group <= kTlShortPairs;
@@ -230,12 +235,11 @@ __device__ __forceinline__ uint32_t rt_chunk(uint32_t row, uint32_t chunk) {
 }
 
 // A CTA's shared state, as its computing warps use it.
-template <int PAIRS>
 struct RowCta {
     uint64_t *full, *empty;
     const unsigned char *slabs;
-    float *joined;              // [groups][PAIRS][128]; queries in operand order before that
-    float2 (*warp_ml)[PAIRS];   // [warps]
+    float *joined;              // [2][kRtPairs][128]: the sums of half of the warps each
+    float2 (*warp_ml)[kRtPairs];  // [warps]
 };
 
 // The keys that a pair of an item sees, [lo, hi); lo -1 where there is no such pair.
@@ -267,54 +271,35 @@ __device__ __forceinline__ int64_t rt_query(const PagedAttnParams &p, const RowI
     return static_cast<int64_t>(it.row0 + i) * static_cast<int64_t>(p.q_stride) + (it.head * p.group + pair - i * p.group) * kPgDim;
 }
 
-template <int NT>
-__device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const RowItem &it, const RowCta<8 * NT> &cta, int32_t begin,
-                                             int32_t end, int32_t slabs, uint32_t ring, bool &dead) {
-    constexpr int PAIRS = 8 * NT, SLAB = rt_slab_bytes<false>(), SLABS = kRtRing / SLAB;
-    constexpr int GROUPS = 16 / PAIRS;  // of warps whose sums are joined side by side
-    constexpr bool QSM = NT > 1;        // queries read from shared memory at each use, to save registers
+__device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const RowItem &it, const RowCta &cta, int32_t begin, int32_t end,
+                                             int32_t slabs, uint32_t ring, bool &dead) {
+    constexpr int SLAB = rt_slab_bytes<false>(), SLABS = kRtRing / SLAB;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int32_t pair0 = it.tile * PAIRS;
-    // This thread's pairs, 8 nt + 2 t + c: which keys they see.
-    int32_t see_lo[NT][2], see_hi[NT][2];
+    const int32_t pair0 = it.tile * kRtPairs;
+    // This thread's pairs, 2 t + c: which keys they see.
+    int32_t see_lo[2], see_hi[2];
 #pragma unroll
-    for (int x = 0; x < 2 * NT; ++x) {
-        const int2 sees = rt_sees(p, it, pair0 + 8 * (x >> 1) + 2 * t + (x & 1));
-        see_lo[x >> 1][x & 1] = sees.x;
-        see_hi[x >> 1][x & 1] = sees.y;
+    for (int c = 0; c < 2; ++c) {
+        const int2 sees = rt_sees(p, it, pair0 + 2 * t + c);
+        see_lo[c] = sees.x;
+        see_hi[c] = sees.y;
     }
-    // Queries as MMA operands, in registers or in shared memory in operand order.
-    uint32_t qf[QSM ? 1 : kPgDim / 16][NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int64_t at = rt_query(p, it, pair0 + 8 * nt + g);
+    // Queries as MMA operands.
+    uint32_t qf[kPgDim / 16][2];
+    {
+        const int64_t at = rt_query(p, it, pair0 + g);
         const uint16_t *src = static_cast<const uint16_t *>(p.q) + at;
-        const auto pick = [&](int ks, int x) { return at >= 0 ? *reinterpret_cast<const uint32_t *>(src + 16 * ks + 2 * t + 8 * x) : 0u; };
-        if constexpr (QSM) {
-            for (int ks = warp; ks < kPgDim / 16; ks += kRtWarps)
-                reinterpret_cast<uint2 *>(cta.joined)[(ks * NT + nt) * 32 + lane] = make_uint2(pick(ks, 0), pick(ks, 1));
-        } else {
 #pragma unroll
-            for (int ks = 0; ks < kPgDim / 16; ++ks)
+        for (int ks = 0; ks < kPgDim / 16; ++ks)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) qf[ks][nt][x] = pick(ks, x);
-        }
+            for (int x = 0; x < 2; ++x) qf[ks][x] = at >= 0 ? *reinterpret_cast<const uint32_t *>(src + 16 * ks + 2 * t + 8 * x) : 0u;
     }
-    if (QSM) rt_bar();
-    float o[8][NT][4];  // dims 16 j + g (+ 8) x pairs 2 t (+ 1)
-    float mx[NT][2], sum[NT][2];
+    float o[8][4];  // dims 16 j + g (+ 8) x pairs 2 t (+ 1)
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[j][nt][x] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            mx[nt][c] = -INFINITY;
-            sum[nt][c] = 0.0f;
-        }
-    }
+        for (int x = 0; x < 4; ++x) o[j][x] = 0.0f;
 
     for (int32_t n = warp; n < slabs && !dead; n += kRtWarps) {
         const uint32_t q = ring + n, st = q % SLABS;
@@ -324,79 +309,65 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
         const int32_t key0 = begin + n * kRtKeys;
         const uint32_t kbase = smem_u32(cta.slabs + st * SLAB), vbase = kbase + SLAB / 2;
         // ---- scores: key g (x = 0, 1) and g + 8 (2, 3) of pairs 2 t, 2 t + 1
-        float s[NT][4], c1[NT][4];
+        float s[4], c1[4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) s[nt][x] = c1[nt][x] = 0.0f;
+        for (int x = 0; x < 4; ++x) s[x] = c1[x] = 0.0f;
         {
             const uint32_t r = lane & 15, half = lane >> 4;
 #pragma unroll
             for (int ks = 0; ks < kPgDim / 16; ++ks) {
                 uint32_t a[4];
                 ldsm4(kbase + rt_chunk(r, 2 * ks + half), a);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    uint2 b;
-                    if constexpr (QSM) b = reinterpret_cast<const uint2 *>(cta.joined)[(ks * NT + nt) * 32 + lane];
-                    else b = make_uint2(qf[ks][nt][0], qf[ks][nt][1]);
-                    mma_bf16(ks & 1 ? c1[nt] : s[nt], a, b.x, b.y);
-                }
+                mma_bf16(ks & 1 ? c1 : s, a, qf[ks][0], qf[ks][1]);
             }
         }
         // ---- masks; a key that exists and that some pair does not see?
         const int32_t left = min(end - key0, kRtKeys);
         bool hidden = false, move = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int c = x & 1, key = g + 8 * (x >> 1);
-                const bool seen = key0 + key >= see_lo[nt][c] && key0 + key < see_hi[nt][c] && key < left;
-                hidden |= !seen && key < left && see_lo[nt][c] >= 0;
-                s[nt][x] = seen ? (s[nt][x] + c1[nt][x]) * p.scale2 : -INFINITY;
-                move |= s[nt][x] > mx[nt][c] + kLazy;
-            }
+        for (int x = 0; x < 4; ++x) {
+            const int c = x & 1, key = g + 8 * (x >> 1);
+            const bool seen = key0 + key >= see_lo[c] && key0 + key < see_hi[c] && key < left;
+            hidden |= !seen && key < left && see_lo[c] >= 0;
+            s[x] = seen ? (s[x] + c1[x]) * p.scale2 : -INFINITY;
+            move |= s[x] > mx[c] + kLazy;
+        }
         // The reference point moves when a score passes it by 2^8 (the first one always does):
         // weights stay below 2^8, and the sums are rarely scaled.
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int c = 0; c < 2; ++c) {
+                float top = fmaxf(mx[c], fmaxf(s[c], s[2 + c]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                const float corr = top == -INFINITY ? 1.0f : pg_exp2(mx[c] - top);
+                mx[c] = top;
+                sum[c] *= corr;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float top = fmaxf(mx[nt][c], fmaxf(s[nt][c], s[nt][2 + c]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float corr = top == -INFINITY ? 1.0f : pg_exp2(mx[nt][c] - top);
-                    mx[nt][c] = top;
-                    sum[nt][c] *= corr;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        o[j][nt][c] *= corr;
-                        o[j][nt][2 + c] *= corr;
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    o[j][c] *= corr;
+                    o[j][2 + c] *= corr;
                 }
+            }
         }
         // ---- weights, transposed into the product's operand as two BF16 terms (16 bits together:
         // the values are BF16 and both operands have one type). Keys bound the kernel: one request
         // over 131,072 rows takes 59.3 us, 58.9 with one term, 256 requests of 500 rows 142 and 139;
         // one term's results are 2.28e-3 from 64 bits where their own rounding makes 1.69e-3.
-        uint32_t pf[NT][2], pr[NT][2];
+        uint32_t pf[2], pr[2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float &e = s[nt][2 * h + c];
-                    e = pg_exp2(e - (mx[nt][c] == -INFINITY ? 0.0f : mx[nt][c]));
-                    sum[nt][c] += e;
-                }
-                const uint32_t w = pg_pack(s[nt][2 * h], s[nt][2 * h + 1]);
-                pf[nt][h] = transpose8(w);
-                pr[nt][h] = transpose8(pg_pack(s[nt][2 * h] - bf16_lo(w), s[nt][2 * h + 1] - bf16_hi(w)));
+            for (int c = 0; c < 2; ++c) {
+                float &e = s[2 * h + c];
+                e = pg_exp2(e - (mx[c] == -INFINITY ? 0.0f : mx[c]));
+                sum[c] += e;
             }
+            const uint32_t w = pg_pack(s[2 * h], s[2 * h + 1]);
+            pf[h] = transpose8(w);
+            pr[h] = transpose8(pg_pack(s[2 * h] - bf16_lo(w), s[2 * h + 1] - bf16_hi(w)));
+        }
         // ---- sums. A weight of zero times a value that is not finite would be NaN: such values
         // leave the products and are added where they are seen. Only slabs with masked keys are
         // looked over; keys past the end are zeroed in any case.
@@ -417,79 +388,68 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
                     if (bad1 || key + 1 >= left) a[x] &= 0x0000ffffu;
                 }
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                mma_bf16(o[j][nt], a, pf[nt][0], pf[nt][1]);
-                mma_bf16(o[j][nt], a, pr[nt][0], pr[nt][1]);
-            }
+            mma_bf16(o[j], a, pf[0], pf[1]);
+            mma_bf16(o[j], a, pr[0], pr[1]);
         }
         if (careful && __any_sync(0xffffffffu, odd)) {
 #pragma unroll 1
-            for (int key = 0; key < left; ++key)
+            for (int key = 0; key < left; ++key) {
+                float w[2];
+                bool seen[2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float w[2];
-                    bool seen[2];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int src = (key & 7) * 4 + t;
-                        const float a = __shfl_sync(0xffffffffu, s[nt][c], src), b = __shfl_sync(0xffffffffu, s[nt][2 + c], src);
-                        w[c] = key < 8 ? a : b;
-                        seen[c] = key0 + key >= see_lo[nt][c] && key0 + key < see_hi[nt][c];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t dim = 16 * j + 8 * x + g;
-                            const float v = __uint_as_float(lds_u16(vbase + rt_chunk(key, dim / 8) + 2 * (dim & 7)) << 16);
-                            if (!isfinite(v)) {
-                                if (seen[0]) o[j][nt][2 * x] += w[0] * v;
-                                if (seen[1]) o[j][nt][2 * x + 1] += w[1] * v;
-                            }
-                        }
+                for (int c = 0; c < 2; ++c) {
+                    const int src = (key & 7) * 4 + t;
+                    const float a = __shfl_sync(0xffffffffu, s[c], src), b = __shfl_sync(0xffffffffu, s[2 + c], src);
+                    w[c] = key < 8 ? a : b;
+                    seen[c] = key0 + key >= see_lo[c] && key0 + key < see_hi[c];
                 }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t dim = 16 * j + 8 * x + g;
+                        const float v = __uint_as_float(lds_u16(vbase + rt_chunk(key, dim / 8) + 2 * (dim & 7)) << 16);
+                        if (!isfinite(v)) {
+                            if (seen[0]) o[j][2 * x] += w[0] * v;
+                            if (seen[1]) o[j][2 * x + 1] += w[1] * v;
+                        }
+                    }
+            }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&cta.empty[st]);
     }
 
-    // ---- join the warps: {m, l} of each pair, then the sums, a group's warps in turn
+    // ---- join the warps: {m, l} of each pair, then the sums, half of the warps' beside the others'
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int c = 0; c < 2; ++c) {
+        float l = sum[c];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        if (g == 0) cta.warp_ml[warp][2 * t + c] = pg_ml(mx[c], l);
+    }
+    rt_bar();
+    float factor[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float l = sum[nt][c];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (g == 0) cta.warp_ml[warp][8 * nt + 2 * t + c] = pg_ml(mx[nt][c], l);
-        }
-    rt_bar();  // and every warp is done with the queries
-    float factor[NT][2];
+    for (int c = 0; c < 2; ++c) {
+        float top = -INFINITY;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kRtWarps; ++w) top = fmaxf(top, cta.warp_ml[w][8 * nt + 2 * t + c].x);
-            factor[nt][c] = mx[nt][c] == -INFINITY ? 0.0f : pg_exp2(mx[nt][c] - top);
-        }
+        for (int w = 0; w < kRtWarps; ++w) top = fmaxf(top, cta.warp_ml[w][2 * t + c].x);
+        factor[c] = mx[c] == -INFINITY ? 0.0f : pg_exp2(mx[c] - top);
+    }
 #pragma unroll 1
-    for (int w = 0; w < kRtWarps / GROUPS; ++w) {
-        if (w == warp / GROUPS) {
-            float *dst = cta.joined + (warp % GROUPS) * PAIRS * kPgDim;
+    for (int w = 0; w < kRtWarps / 2; ++w) {
+        if (w == warp / 2) {
+            float *dst = cta.joined + (warp & 1) * kRtPairs * kPgDim;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        float *to = dst + (8 * nt + 2 * t + (x & 1)) * kPgDim + 16 * j + 8 * (x >> 1) + g;
-                        const float v = o[j][nt][x] * factor[nt][x & 1];
-                        *to = w ? *to + v : v;
-                    }
+                for (int x = 0; x < 4; ++x) {
+                    float *to = dst + (2 * t + (x & 1)) * kPgDim + 16 * j + 8 * (x >> 1) + g;
+                    const float v = o[j][x] * factor[x & 1];
+                    *to = w ? *to + v : v;
+                }
         }
         rt_bar();
     }
@@ -501,7 +461,7 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
 // the numbers and sends the other; with key and pair of a register chosen by
 // the lane's own number (key ^ l / 8, pair ^ l % 8) it is always the same half
 // of the registers, and nothing is selected.
-__device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowItem &it, const RowCta<8> &cta, float *weights,
+__device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowItem &it, const RowCta &cta, float *weights,
                                             int32_t begin, int32_t end, int32_t slabs, uint32_t ring, bool &dead) {
     constexpr int SLAB = rt_slab_bytes<true>(), SLABS = kRtRing / SLAB;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -677,24 +637,22 @@ __device__ __forceinline__ OwnShape row_work(const PagedAttnParams &p, int32_t r
     return s;
 }
 
-template <bool F32, int NT>
+template <bool F32>
 __global__ void __launch_bounds__(kRtThreads, 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
-    static_assert(!F32 || NT == 1, "FP32: eight pairs");
-    constexpr int PAIRS = 8 * NT, SLAB = rt_slab_bytes<F32>(), SLABS = kRtRing / SLAB;
+    constexpr int SLAB = rt_slab_bytes<F32>(), SLABS = kRtRing / SLAB;
     static_assert(SLABS % kRtWarps == 0, "a place of the ring serves one warp");
-    constexpr int GROUPS = 16 / PAIRS;  // of warps whose sums are joined side by side
     constexpr int PER = kPgRows / kRtKeys;  // slabs per page
     extern __shared__ __align__(128) unsigned char rt_raw[];
     __shared__ __align__(8) uint64_t full[SLABS], empty[SLABS];
     __shared__ int64_t scan[kRtThreads / 32];
     __shared__ RowItem items[kRtBatch];
-    __shared__ float2 warp_ml[kRtWarps][PAIRS];
+    __shared__ float2 warp_ml[kRtWarps][kRtPairs];
     __shared__ __align__(16) float weights[F32 ? kRtWarps : 1][F32 ? kRtKeys * 8 : 4];
     __shared__ int32_t first_strip, last_strip, lowest_at;
     unsigned char *base = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(rt_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    float *joined = reinterpret_cast<float *>(base + kRtRing);  // [GROUPS][PAIRS][128]
+    float *joined = reinterpret_cast<float *>(base + kRtRing);  // [2][kRtPairs][128]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_launch_dependents();
     if (blockIdx.x == 0) {  // for the kernels that follow, while the others work
@@ -702,7 +660,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
         return;
     }
     const int32_t worker = static_cast<int32_t>(blockIdx.x) - 1;
-    const RowCta<PAIRS> cta{full, empty, base, joined, warp_ml};
+    const RowCta cta{full, empty, base, joined, warp_ml};
     if (tid == 0) {
         for (int s = 0; s < SLABS; ++s) {
             mbar_init(&full[s], 1);
@@ -797,7 +755,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                 it.page0 = s.page0 + lo;
                 it.pages = hi - lo;
                 // Keys past the tile's last row are seen by none of its rows.
-                const int32_t last = s.at0 + min(s.rows - 1, p.by_group.div(it.tile * PAIRS + PAIRS - 1));
+                const int32_t last = s.at0 + min(s.rows - 1, p.by_group.div(it.tile * kRtPairs + kRtPairs - 1));
                 it.limit = r < p.requests ? min(max(last + 1, 0), s.length) : p.prefix;
                 it.row0 = s.row0;
                 it.rows = s.rows;
@@ -852,11 +810,11 @@ __global__ void __launch_bounds__(kRtThreads, 2)
             }
             // ---- the computing warps
             if constexpr (F32) rt_item_f32(p, it, cta, weights[warp], begin, end, slabs, ring, dead);
-            else rt_item_bf16<NT>(p, it, cta, begin, end, slabs, ring, dead);
+            else rt_item_bf16(p, it, cta, begin, end, slabs, ring, dead);
             ring += slabs;
             // ---- result, or the tile's partial sums
 #pragma unroll 1
-            for (int x = tid; x < PAIRS * kPgDim / 4; x += 32 * kRtWarps) {
+            for (int x = tid; x < kRtPairs * kPgDim / 4; x += 32 * kRtWarps) {
                 const int pair = x / (kPgDim / 4), d = 4 * (x % (kPgDim / 4));
                 float top = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -867,12 +825,10 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                     if (ml.x != -INFINITY) l += pg_exp2(ml.x - top) * ml.y;
                 }
                 float4 v = ld4(joined + pair * kPgDim + d);
-                if constexpr (GROUPS == 2) {
-                    const float4 u = ld4(joined + (PAIRS + pair) * kPgDim + d);
-                    v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
-                }
+                const float4 u = ld4(joined + (kRtPairs + pair) * kPgDim + d);
+                v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
                 if (it.direct) {
-                    const int32_t m = it.tile * PAIRS + pair;
+                    const int32_t m = it.tile * kRtPairs + pair;
                     if (m >= it.rows * p.group) continue;
                     const int32_t i = p.by_group.div(m);
                     const float inv = pg_inverse(it.at0 + i, l);
@@ -881,7 +837,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + at, v);
                     else pg_store4(static_cast<uint16_t *>(p.out) + at, v);
                 } else {
-                    const uint64_t at = static_cast<uint64_t>(it.slot) * PAIRS + pair;
+                    const uint64_t at = static_cast<uint64_t>(it.slot) * kRtPairs + pair;
                     *reinterpret_cast<float4 *>(p.row_sum + at * kPgDim + d) = v;
                     if (d == 0) p.row_ml[at] = make_float2(top, l);
                 }
@@ -1000,12 +956,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         bool written = false;
         if (e.y >= 0 && head < p.qh) {
             const int32_t kv = p.by_group.div(head), in_group = head - kv * p.group;
-            // The parts of row tile m / row_tile of request r (or of the prefix) for this head.
+            // The parts of row tile m / kRtPairs of request r (or of the prefix) for this head.
             const auto row_parts = [&](int32_t r, int32_t m) {
                 const int4 rec = p.row_record[r];
-                const int32_t strip = (m >> p.row_shift) * p.kh + kv, u0 = rec.x + strip * rec.y;
+                const int32_t strip = m / kRtPairs * p.kh + kv, u0 = rec.x + strip * rec.y;
                 const int32_t c0 = rec.y ? of_rows.cta_of(u0) : 0;
-                return PartList{p.row_sum, p.row_ml, c0 + rec.z + strip, 1, p.row_tile, m & (p.row_tile - 1),
+                return PartList{p.row_sum, p.row_ml, c0 + rec.z + strip, 1, kRtPairs, m % kRtPairs,
                                 rec.y ? of_rows.cta_of(u0 + rec.y - 1) - c0 + 1 : 0};
             };
             own = row_parts(e.z, e.w * p.group + in_group);
