@@ -68,13 +68,13 @@ class Model:
             raise RuntimeError(self.backend.info().note.decode())
         return y
 
-    def step(self, x, pools, plan, tables, prefix_pages, prefix_rows):
-        """The batch's rows [rows, hidden] through every layer."""
+    def step(self, x, pools, plan, tables, prefix_pages, prefix_rows, most_new):
+        """The batch's rows [rows, hidden] through every layer, at most `most_new` of them one request's."""
         for layer, pool in zip(self.layers, pools):
             qkv = self.project(x, layer["qkv"])
             q = self.backend.paged_store(qkv, pool, plan.slots, plan.positions, *layer["norms"], self.table)
             a = self.backend.paged_attention(q, pool, plan.starts, plan.lengths, tables, prefix_pages=prefix_pages,
-                                             prefix_rows=prefix_rows, window=layer["window"])
+                                             prefix_rows=prefix_rows, window=layer["window"], most_new=most_new)
             x = x + self.project(a.float().reshape(x.shape[0], -1), layer["out"])
         return x
 
@@ -94,7 +94,7 @@ def serve(model, prefix, prompts, steps, shared):
         table = torch.full((1, prefix_count), -1, **ints)
         plan = model.backend.paged_plan(torch.zeros(1, **ints), torch.full((1,), prefix.shape[0], **ints), table,
                                         torch.arange(prefix_count, **ints), prefix.shape[0])
-        model.step(prefix, pools, plan, table, None, 0)
+        model.step(prefix, pools, plan, table, None, 0, prefix.shape[0])
         prefix_pages, prefix_rows = table[0].contiguous(), prefix.shape[0]
     free = prefix_count + torch.randperm(requests * per_request, generator=torch.Generator().manual_seed(1)).int().cuda()
     tables = torch.full((requests, per_request), -1, **ints)
@@ -103,7 +103,7 @@ def serve(model, prefix, prompts, steps, shared):
     x, plan, outputs = torch.cat(prompts), None, []
     for step in range(steps + 1):
         plan = model.backend.paged_plan(held, added, tables, free, x.shape[0], base=prefix_rows, after=plan)
-        y = model.step(x, pools, plan, tables, prefix_pages, prefix_rows)
+        y = model.step(x, pools, plan, tables, prefix_pages, prefix_rows, 1 if step else max(p.shape[0] for p in prompts))
         last = (plan.starts[1:] - 1).long()
         outputs.append(y[last])
         x = torch.nn.functional.normalize(y[last], dim=1) * model.hidden ** 0.5  # the next row of each request

@@ -135,6 +135,9 @@ struct plamo_paged_attention_args {
     uint32_t query_heads, kv_heads, type;
     float scale;             /* of the scores, 1 / sqrt(128) as a rule */
     void *stream;
+    uint64_t most_new;       /* rows of the request that adds most (1 in a decode step), 0: not known. It chooses the
+                                kernels, where `rows` counts padding or `requests` idle slots that hide it; every row
+                                gets its result whatever it says. The workspace's size depends on it. */
 };
 /* Device bytes a call with these shapes needs (its pointers are not read);
    0 when the shapes would be declined. The prefix and a request's page table

@@ -266,7 +266,7 @@ class PagedAttentionArgs(ctypes.Structure):
                [(n, c_uint64) for n in ("rows", "q_stride", "out_stride", "requests", "table_stride", "prefix_rows",
                                         "pages", "window")] + \
                [("query_heads", c_uint32), ("kv_heads", c_uint32), ("type", c_uint32), ("scale", ctypes.c_float),
-                ("stream", c_void_p)]
+                ("stream", c_void_p), ("most_new", c_uint64)]
 
 
 PAGED_ROWS, PAGED_DIM = 64, 128  # PLAMO_PAGED_ROWS, PLAMO_PAGED_DIM

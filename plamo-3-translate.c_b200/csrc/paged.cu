@@ -67,8 +67,17 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     AttentionLayout a{};
     const uint64_t group = d->query_heads / d->kv_heads, sms = static_cast<uint64_t>(context_sms(c));
     const uint64_t pairs = d->rows * group, prefix_pages = ceil_div(d->prefix_rows, kPgRows);
-    // The tile kernel is for prompts (more rows than requests, and more pairs than
-    // a short request has), and in BF16 for a prefix that would keep the row
+    // The tile kernel is for prompts, requests of more pairs than a short one has:
+    // where the caller says so, or says nothing and there are more rows than
+    // requests; a step whose padding or idle slots hide what it is says it. And
+    // only where the row kernel's work, a unit per eight pairs, KV head and page,
+    // is more than another kernel takes to begin and end, with page tables as full
+    // as they can be, since lengths are on the device: one request of eight heads to a KV head
+    // behind 12 rows, 320 units 14 us there and 33 with tiles, 1,536 31 and 38,
+    // 3,584 64 and 40; 16 requests of nine rows behind 12, 2,880 units 53 and 36; in
+    // FP32 four KV heads, six requests of 32 rows, 3,072 units 57 and 49, of 16
+    // rows, 1,536, 35 and 48.
+    // And in BF16 it is for a prefix that would keep the row
     // kernel, eight pairs at a time, longer than another kernel takes to begin and
     // end: 61 requests of eight heads to a KV head, own rows as they are, took 41,
     // 50 us there behind 512, 1,000 rows (1,952, 3,904 tiles of eight pairs times
@@ -77,8 +86,10 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     // tiles behind 1,000, 2,000: the same slope, 12 us more).
     const bool f32 = d->type == PLAMO_PAGED_FP32;
     const uint64_t tile_pairs = f32 ? kTfPairs : kTlPairs;
-    const bool prompts = d->rows > d->requests && pairs > kTlShortPairs;
-    if (group <= tile_pairs && (prompts || (!f32 && ceil_div(pairs, 8) * prefix_pages * d->kv_heads > 4000))) {
+    const uint64_t strips = ceil_div(pairs, kRtPairs) * d->kv_heads;
+    const bool prompts = (d->most_new ? std::min(d->most_new, d->rows) * group : d->rows > d->requests ? pairs : 0) > kTlShortPairs;
+    if (group <= tile_pairs && ((prompts && strips * (prefix_pages + d->table_stride) > kTlPromptUnits) ||
+                                (!f32 && strips * prefix_pages > kTlPrefixUnits))) {
         a.tile_rows = static_cast<uint32_t>(tile_pairs / group);
         a.tile_grid = static_cast<uint32_t>(f32 ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.

@@ -601,10 +601,10 @@ class Backend:
         return paged.store(self, qkv, pool, slots, positions, q_norm, k_norm, table, status)
 
     def paged_attention(self, q, pool, starts, lengths, tables, prefix_pages=None, prefix_rows=0, window=0, scale=None,
-                        out=None, status=None):
+                        out=None, status=None, most_new=0):
         """Attention over a shared prefix and each request's own rows; see paged.attention."""
         return paged.attention(self, q, pool, starts, lengths, tables, prefix_pages, prefix_rows, window, scale, out,
-                               status)
+                               status, most_new)
 
     def paged_status(self):
         """PLAMO_PAGED_* bits of stores and attention calls without a status tensor; see paged.status."""

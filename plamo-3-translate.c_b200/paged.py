@@ -165,14 +165,16 @@ def store(backend, qkv, pool, slots, positions, q_norm, k_norm, table, status=No
 
 
 def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, prefix_rows=0, window=0, scale=None, out=None,
-              status=None):
+              status=None, most_new=0):
     """Every query over the shared prefix and its own request's rows, causal.
 
     q: [rows, query_heads, 128] of the pool's type (rows may be strided);
     starts, lengths: of the plan; tables: [requests, pages per request];
     prefix_pages: the shared prefix's pages, prefix_rows rows of them used;
     window: rows a query sees, itself included (0: all before it); scale: of
-    the scores, 1 / sqrt(128) unless given. Returns `out`, allocated if None.
+    the scores, 1 / sqrt(128) unless given; most_new: rows of the request that
+    adds most (1 in a decode step; 0: not known), which chooses the kernels where
+    q has rows of padding or lengths idle slots. Returns `out`, allocated if None.
     """
     torch = _torch()
     kind, pages, kv_heads, device = _pool(torch, pool, backend)
@@ -182,8 +184,8 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
     _ints(torch, lengths, requests, device, "lengths")
     _ints(torch, starts, requests + 1, device, "starts")
     stride = _tables(torch, tables, requests, device)
-    if prefix_rows < 0 or window < 0:
-        raise ValueError("prefix_rows and window: not negative")
+    if prefix_rows < 0 or window < 0 or most_new < 0:
+        raise ValueError("prefix_rows, window and most_new: not negative")
     prefix = 0
     if prefix_rows:
         if prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.numel() * ROWS < prefix_rows:
@@ -200,7 +202,7 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
     args = _abi.PagedAttentionArgs(q.data_ptr(), pool.data_ptr(), out.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
                                    tables.data_ptr(), prefix, 0, 0, _status(torch, status, device), rows, q_stride, out_stride,
                                    requests, stride, prefix_rows, pages, window, query_heads, kv_heads, kind,
-                                   DIM ** -0.5 if scale is None else scale, _stream(torch, device))
+                                   DIM ** -0.5 if scale is None else scale, _stream(torch, device), most_new)
     size = backend.lib.plamo_paged_attention_workspace(backend.ctx, ctypes.byref(args))
     if not size:
         raise ValueError(backend.info().note.decode())

@@ -239,3 +239,45 @@ def test_example_of_many_steps_has_a_rotation_for_each():
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     assert module.main(["--fp32", "--steps", "420", "--requests", "1", "--layers", "1", "--prefix", "3"]) <= 2e-4
+
+
+def launches_of(be, call):
+    before = be.lib.plamo_cuda_kernel_launches(be.ctx)
+    result = call()
+    return result, be.lib.plamo_cuda_kernel_launches(be.ctx) - before
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("prefix", [0, 12, 300])
+@pytest.mark.parametrize("spare", [1, 7])
+def test_spare_rows_of_a_decode_step_ask_for_no_other_kernels(be, spare, prefix, dtype):
+    """(The prefix's units are numbered over spare rows too, so sums may be cut elsewhere.)"""
+    s = Scene([(i * 53 % 400, 1) for i in range(61)], prefix, 32, 4, dtype, seed=31)
+    s.tables = torch.nn.functional.pad(s.tables, (0, 64), value=-7)  # room for 4,096 rows more
+    want, tol = s.expected()
+    _, few = launches_of(be, lambda: attend(be, s))
+    s.q = torch.cat([s.q, s.q[:1].expand(spare, -1, -1)])
+    got, some = launches_of(be, lambda: attend(be, s, most_new=1))
+    check(got[:61], want, tol, "requests' rows")
+    assert (got[61:] == 0).all() and some == few
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_a_prompt_among_idle_slots_gets_tiles(be, dtype):
+    s = Scene([(0, 0)] * 200 + [(30, 190)] + [(0, 0)] * 200, 300, 16, 2, dtype, seed=32)
+    s.tables = torch.nn.functional.pad(s.tables, (0, 20), value=-7)
+    alone = Scene([(30, 190)], 300, 16, 2, dtype, seed=32)
+    alone.tables = torch.nn.functional.pad(alone.tables, (0, 20), value=-7)
+    _, tiles = launches_of(be, lambda: attend(be, alone))
+    got, count = launches_of(be, lambda: attend(be, s, most_new=190))
+    assert count == tiles
+    check(got, *s.expected(), "prompt among idle slots")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("most_new", [1, 2, 40, 150, 10 ** 9])
+def test_results_do_not_depend_on_what_most_new_says(be, most_new, dtype):
+    s = Scene([(200, 1), (0, 150), (5, 1), (0, 0), (333, 7), (90, 40)], 70, 24, 4, dtype, seed=33)
+    check(attend(be, s, most_new=most_new), *s.expected(), f"most_new {most_new}")
+    with pytest.raises(ValueError):
+        attend(be, s, most_new=-1)
