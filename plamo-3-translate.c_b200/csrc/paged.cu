@@ -77,19 +77,21 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     // 3,584 64 and 40; 16 requests of nine rows behind 12, 2,880 units 53 and 36; in
     // FP32 four KV heads, six requests of 32 rows, 3,072 units 57 and 49, of 16
     // rows, 1,536, 35 and 48.
-    // And in BF16 it is for a prefix that would keep the row
-    // kernel, eight pairs at a time, longer than another kernel takes to begin and
-    // end: 61 requests of eight heads to a KV head, own rows as they are, took 41,
-    // 50 us there behind 512, 1,000 rows (1,952, 3,904 tiles of eight pairs times
-    // pages) and 58, 51 us with tiles behind 1,100, 2,000. In FP32 the tiles' rate is
-    // no better than the row kernel's (76 us in it behind 512 rows; 103, 136 with
-    // tiles behind 1,000, 2,000: the same slope, 12 us more).
+    // And in BF16 it is for a prefix that would keep the row kernel longer. A step of
+    // 128 keys costs here what four units do there, however few of its tile's 256
+    // pairs there are, so few pairs stay there: one request of eight heads to each
+    // of four KV heads behind 65,536 rows 38 us there and 71 with tiles, two 55 and
+    // 73, four 98 and 74; 16 behind 2,048 24 and 29, behind 4,096 36 and 31; 61
+    // behind 512 29 and 37, behind 1,024 39 and 38, behind 2,048 58 and 39. In FP32 the tiles' rate is
+    // no better than the row kernel's (61 behind 512 rows 76 us in it; behind 1,000, 2,000
+    // with tiles 103, 136: the same slope, 12 us more).
     const bool f32 = d->type == PLAMO_PAGED_FP32;
     const uint64_t tile_pairs = f32 ? kTfPairs : kTlPairs;
     const uint64_t strips = ceil_div(pairs, kRtPairs) * d->kv_heads;
+    const uint64_t prefix_steps = ceil_div(pairs, kTlPairs) * d->kv_heads * ceil_div(d->prefix_rows, kTlKeys);
     const bool prompts = (d->most_new ? std::min(d->most_new, d->rows) * group : d->rows > d->requests ? pairs : 0) > kTlShortPairs;
     if (group <= tile_pairs && ((prompts && strips * (prefix_pages + d->table_stride) > kTlPromptUnits) ||
-                                (!f32 && strips * prefix_pages > kTlPrefixUnits))) {
+                                (!f32 && strips * prefix_pages > kTlPrefixUnits + 4 * prefix_steps))) {
         a.tile_rows = static_cast<uint32_t>(tile_pairs / group);
         a.tile_grid = static_cast<uint32_t>(f32 ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.

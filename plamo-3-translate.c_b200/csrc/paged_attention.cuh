@@ -70,7 +70,7 @@ enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlFirst
 constexpr int kTlShortPairs = 32; // requests of up to so many keep their own rows in the row kernel
 constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 // Units of the row kernel, strips times pages, that the tile kernel is worth: prompts', a prefix's.
-constexpr uint64_t kTlPromptUnits = 2000, kTlPrefixUnits = 4000;
+constexpr uint64_t kTlPromptUnits = 2000, kTlPrefixUnits = 3000;
 
 // The row kernel works on slabs of 16 keys, the M of one mma.sync, against
 // tiles of 8 (row, head-in-group) pairs, its N. Tiles of 16 for more pairs than

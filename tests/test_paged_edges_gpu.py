@@ -281,3 +281,21 @@ def test_results_do_not_depend_on_what_most_new_says(be, most_new, dtype):
     check(attend(be, s, most_new=most_new), *s.expected(), f"most_new {most_new}")
     with pytest.raises(ValueError):
         attend(be, s, most_new=-1)
+
+
+def test_few_pairs_read_a_long_prefix_in_the_row_kernel(be):
+    """One request's prefix is read once there; many requests' in the tile kernel."""
+    pool = torch.zeros(1200, 2, ROWS, 4, DIM, dtype=BF16, device="cuda")
+    pages = torch.arange(1, 1025, dtype=torch.int32, device="cuda")
+
+    def count(requests, rows):
+        q = torch.ones(requests, 32, DIM, dtype=BF16, device="cuda")
+        one = torch.ones(requests, dtype=torch.int32, device="cuda")
+        starts = torch.arange(requests + 1, dtype=torch.int32, device="cuda")
+        out, launches = launches_of(be, lambda: be.paged_attention(q, pool, starts, one, torch.zeros(requests, 1, dtype=torch.int32, device="cuda"),
+                                                                   prefix_pages=pages, prefix_rows=rows))
+        assert (out == 0).all()
+        return launches
+
+    assert count(1, 65536) == count(2, 65536) == count(16, 1000) == 2
+    assert count(8, 65536) == count(61, 4096) == 3
