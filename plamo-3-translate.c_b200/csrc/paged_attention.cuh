@@ -228,6 +228,16 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 __device__ __forceinline__ void rt_bar() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kRtWarps) : "memory"); }
+// Two weights as two BF16 terms each: the upper half of each's bits, and what is
+// left of the weight and 2^-22 of it more, which is never zero or negative beside a first
+// term that is not (a zero times an infinite value, or infinities of two signs,
+// would be no number; weights below 2^-104 aside). Of a weight of zero both are zero.
+__device__ __forceinline__ void pg_split(float a, float b, uint32_t &first, uint32_t &rest) {
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    constexpr float kMore = 1.0f + 0x1p-22f;
+    first = __byte_perm(x, y, 0x7632);
+    rest = pg_pack(fmaf(a, kMore, -__uint_as_float(x & 0xffff0000u)), fmaf(b, kMore, -__uint_as_float(y & 0xffff0000u)));
+}
 constexpr float kLazy = 8.0f;  // a maximum is renewed when passed by 2^8
 
 // Byte offset of a 16-byte chunk in a slab's [boxes][16][128 bytes] rows with
@@ -366,9 +376,10 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
                 e = pg_exp2(e - (mx[c] == -INFINITY ? 0.0f : mx[c]));
                 sum[c] += e;
             }
-            const uint32_t w = pg_pack(s[2 * h], s[2 * h + 1]);
-            pf[h] = transpose8(w);
-            pr[h] = transpose8(pg_pack(s[2 * h] - bf16_lo(w), s[2 * h + 1] - bf16_hi(w)));
+            uint32_t first, rest;
+            pg_split(s[2 * h], s[2 * h + 1], first, rest);
+            pf[h] = transpose8(first);
+            pr[h] = transpose8(rest);
         }
         // ---- sums. A weight of zero times a value that is not finite would be NaN: such values
         // leave the products and are added where they are seen. Only slabs with masked keys are

@@ -606,8 +606,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                             const float b = pg_exp2(fmaf(__uint_as_float(x[32 * part + 2 * k + 1]), scale2, shift));
                             l0 += a;
                             l1 += b;
-                            r[k] = pg_pack(a, b);
-                            rest[k] = pg_pack(a - bf16_lo(r[k]), b - bf16_hi(r[k]));
+                            pg_split(a, b, r[k], rest[k]);
                         }
                         tmem_st16(scol + 64 * half + 16 * part, r);
                         tmem_st16(scol + 64 * half + 32 + 16 * part, rest);

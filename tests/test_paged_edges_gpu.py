@@ -299,3 +299,23 @@ def test_few_pairs_read_a_long_prefix_in_the_row_kernel(be):
 
     assert count(1, 65536) == count(2, 65536) == count(16, 1000) == 2
     assert count(8, 65536) == count(61, 4096) == 3
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("requests,prefix", [([(300, 1), (40, 1)], 0), ([(300, 1), (40, 1)], 200), ([(0, 300), (60, 90)], 200),
+                                             ([(20, 5), (200, 8)], 30)])
+def test_infinite_values_that_are_seen_make_infinite_results(be, requests, prefix, sign, dtype):
+    """No number would be a zero part of a weight times an infinity."""
+    s = Scene(requests, prefix, 8, 2, dtype, seed=41)
+    want, tol = s.expected()
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    if prefix:
+        s.pool[s.prefix_pages[0], 1, 3, :, 7] = sign * float("inf")
+        hit[:, :, 7] = True
+    first, (held, new) = 0, requests[0]
+    s.pool[s.tables[0, 0], 1, 9, :, 100] = sign * float("inf")
+    hit[first + max(0, 9 - held):first + new, :, 100] = True
+    got = attend(be, s).double().cpu()
+    assert (got[hit] == sign * float("inf")).all()
+    check(torch.where(hit, 0.0, got), torch.where(hit, 0.0, want), tol, "the other dimensions")

@@ -25,8 +25,8 @@ def beyond_rounding(be, s):
     """(relative L2 of the result, its bound).
 
     A result is y = o + d rounded to BF16, with |d| <= (2 (e^E - 1) + 2^-17) A
-    from scores, exponentials and FP32 sums (Scene.expected), and 2^-16 A from
-    the softmax weights, carried in two BF16 terms: the second is at most 2^-8 of
+    from scores, exponentials and FP32 sums (Scene.expected), and 2^-15 A from
+    the softmax weights, carried in two BF16 terms: the second is at most 2^-7 of
     the weight, its own rounding 2^-8 of that. The last rounding is not
     correlated with d, so the squares add; 2 % covers the chance correlation
     over the thousands of elements here.
@@ -39,7 +39,7 @@ def beyond_rounding(be, s):
     a, _ = sizes.expected()
     rounding = o.to(BF16).double() - o
     got = be.paged_attention(s.q, s.pool, s.starts, s.lengths, s.tables, prefix_pages=s.prefix_pages, prefix_rows=s.prefix)
-    bound = 1.02 * torch.sqrt(rounding.norm() ** 2 + (d + 2.0 ** -16 * a).norm() ** 2) / o.norm()
+    bound = 1.02 * torch.sqrt(rounding.norm() ** 2 + (d + 2.0 ** -15 * a).norm() ** 2) / o.norm()
     return ((got.double().cpu() - o).norm() / o.norm()).item(), bound.item()
 
 

@@ -7,7 +7,8 @@ import torch
 import test_paged_edges_gpu as edges
 import test_paged_gpu as base
 from paged_reference import Scene
-from test_paged_edges_gpu import (test_rows_all_of_whose_scores_are_minus_infinity,  # noqa: F401
+from test_paged_edges_gpu import (test_infinite_values_that_are_seen_make_infinite_results,  # noqa: F401
+                                  test_rows_all_of_whose_scores_are_minus_infinity,
                                   test_rows_before_the_first_start_are_zero_and_reported, test_starts_that_decrease_leave_zeros)
 from test_paged_gpu import (be, test_attention_head_layouts, test_attention_is_the_same_every_time,  # noqa: F401
                             test_attention_many_requests, test_attention_matches_its_formula,
