@@ -11,9 +11,12 @@
  *   plamo_paged_store      per layer, between the QKV projection and
  *                          attention: normalises and rotates the query and
  *                          key heads, puts keys and values into their slots;
- *   plamo_paged_attention  per layer: every query over the shared prefix,
- *                          read once for the whole batch, and over its own
- *                          request's rows.
+ *   plamo_paged_attention  per layer: every query over the shared prefix and
+ *                          over its own request's rows. The prefix is read
+ *                          once for up to 256 (row, head) pairs of the
+ *                          requests that add few rows (BF16; FP32, and short
+ *                          prefixes: for eight), and once for each of the
+ *                          tiles of those that add many.
  *
  * Pool: [pages][2][64][kv_heads][128] elements of BF16 or FP32, 16-byte
  * aligned: a page holds 64 key rows, then 64 value rows, as the token loop's

@@ -199,8 +199,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_lengths_kernel(int32_
 // is the sum of its squares, and the row's cos/sin stay in registers for all of
 // its heads. All loads of a warp are issued before the first is used. Streaming:
 // 8,191 rows of 40 heads are 168 MB in and 84 MB out, 39 us at the copy rate;
-// 40 us with eight heads to a warp, 43 with four (fewer bytes in flight); lanes
-// of four neighbouring dimensions, their partners exchanged, took 48.
+// 42 us back to back (93 %) with eight heads to a warp; four took 3 us more
+// (fewer bytes in flight), lanes of four neighbouring dimensions, their partners
+// exchanged, 8.
 // {x[2l], x[2l + 1], x[64 + 2l], x[64 + 2l + 1]}
 template <typename T>
 __device__ __forceinline__ float4 pg_load_pairs(const T *x, uint32_t lane) {

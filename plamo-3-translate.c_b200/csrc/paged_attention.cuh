@@ -67,7 +67,12 @@ struct PagedAttnParams {
     float2 *tile_ml;
 };
 enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlFirst, kTlTaken, kRtRun, kRtLonger, kTlHeader };
-constexpr int kTlShortPairs = 32; // requests of up to so many keep their own rows in the row kernel
+// Requests of up to so many pairs keep their own rows in the row kernel and share
+// the prefix's tiles. Over 4 to 64 requests of 300 and 2,000 rows: with a bound of 16,
+// requests of 17 to 32 pairs take 1.41 times as long behind 4,096 rows (BF16; FP32
+// 1.60), 0.96 (1.11) behind 455; with one of 64, those of 33 to 64 pairs 0.97
+// (0.97) behind 4,096, 1.28 (1.15) behind 455, 1.19 (1.05) behind none.
+constexpr int kTlShortPairs = 32;
 constexpr int kTlMinUnits = 2;     // least key steps worth a CTA
 // Units of the row kernel, strips times pages, that the tile kernel is worth: prompts', a prefix's.
 constexpr uint64_t kTlPromptUnits = 2000, kTlPrefixUnits = 3000;
@@ -629,9 +634,10 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
 // half of what the slab's 16 KB take to arrive, and lose nothing to splitting.
 // (TF32 mma.sync with two terms to an operand took 5 us per slab and warp; this
 // takes 2 to 3, BF16 0.7.)
-// Bound: HBM on long runs (one request over 131,072 rows of 1 KB: 50 us, 5.4
+// Bound: HBM on long runs (one request over 131,072 rows of 1 KB: 53 us cold, 5.1
 // TB/s); on short items their ends, about 4 us each (256 requests of 500 rows
-// and eight KV heads: 130 us, 4.1 TB/s).
+// and eight KV heads: 133 us, 4.0 TB/s). The FP32 kernel spills (48 bytes
+// stored, 112 loaded) at the 128 registers that two CTAs to an SM leave a thread.
 __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums);  // paged_tiles.cuh
 
 // Request r's work, or the prefix's (r == requests) from page pp0 on.

@@ -15,8 +15,8 @@ namespace plamo {
 // times 512 for the values (128 x 128 x 128 at 4096 multiply-adds a cycle) and
 // 1024 cycles of exponentials (16 a cycle): the halves run half a step apart,
 // so that one's exponentials cover the other's products. Measured: 329 GFLOP of
-// ragged prompts behind 2,048 rows in 604 us, 0.54 PFLOP/s. A half's chain bounds
-// it, 3 us a step: scores, softmax, the value product, and the next scores only
+// ragged prompts behind 2,048 rows in 614 us, 0.54 PFLOP/s, the tensor pipe busy
+// for 43 % of it (the weights' second term among that). A half's chain bounds it, 3 us a step: scores, softmax, the value product, and the next scores only
 // when that is done, since they replace the weights; then 8 us at each segment's
 // ends.
 // The value product takes both operands in one type and the values are BF16, so
@@ -698,7 +698,8 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 // bytes) and the sums of the same pairs in dimensions 4 tx and 64 + 4 tx (64 to
 // 4). Bound: 128 multiply-adds a cycle and SM, 8192 cycles for a step's two
 // products. (Three BF16 terms to an operand on tcgen05 would be bound by six
-// products each, 3072 cycles, but a long sum there drifts by 2^-24 a product.)
+// products each, 3072 cycles, with a fold to FP32 registers every step as the
+// projections' tiles have it: a kernel of its own, not written.)
 constexpr int kTfPairs = 64, kTfKeys = 64, kTfThreads = 128;
 constexpr int kTfTile = kTfKeys * kPgDim * 4;  // keys, values or queries
 constexpr int kTfTables = 3 * kTfTile + kTfPairs * kTfKeys * 4;  // barriers and the pairs' rows behind the tiles
