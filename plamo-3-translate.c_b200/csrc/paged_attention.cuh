@@ -962,6 +962,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     pdl_wait();
     const int32_t tiles = p.tile_rows ? p.header[kTlTiles] : 0, pre_tiles = p.tile_rows ? p.header[kTlPreTiles] : 0;
     const int32_t ctas = p.tile_rows ? p.header[kTlCtas] : 0;
+    const int32_t first_row = p.header[kTlFirst], end_row = p.header[kTlTaken];  // of the requests'
     const Runs runs = tile_runs(p), of_rows = row_runs(p);
     PartList shared{}, own{};
     float4 o[RES];
@@ -1060,9 +1061,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         }
     };
 #pragma unroll 1
-    for (int32_t row = blockIdx.x; row < p.header[kTlFirst]; row += gridDim.x) clear(row);
+    for (int32_t row = blockIdx.x; row < first_row; row += gridDim.x) clear(row);
 #pragma unroll 1
-    for (int32_t row = p.header[kTlTaken] + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
+    for (int32_t row = end_row + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
 #pragma unroll 1
     for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); tile < tiles; tile += gridDim.x)
         if (p.tile_unit[tile + 1] == p.tile_unit[tile])
