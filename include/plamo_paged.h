@@ -154,7 +154,9 @@ uint64_t plamo_paged_attention_workspace(struct plamo_cuda *, const struct plamo
    that sees nothing gets zeros: padding, rows before starts[0], and rows whose
    request holds fewer rows (lengths) than it adds, before the first held one.
    Where the starts do not rise from 0 to at most `rows`, `status` gets
-   PLAMO_PAGED_BATCH_ROWS; where they decrease, every row gets zeros. A row
+   PLAMO_PAGED_BATCH_ROWS; where they decrease, every row gets zeros. So
+   reported, and without results, is a batch whose (row, head) pairs times the
+   pages that they see pass 2^34. A row
    that sees a score of NaN, or scores of -infinity only, gets NaN. Rows past a request's length, of other
    requests and after a query's own never reach its result, whatever they
    hold. Scores, softmax sums and products are FP32 for both types (against

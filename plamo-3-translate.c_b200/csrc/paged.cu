@@ -69,22 +69,21 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     const uint64_t pairs = d->rows * group, prefix_pages = ceil_div(d->prefix_rows, kPgRows);
     // The tile kernel is for prompts, requests of more pairs than a short one has:
     // where the caller says so, or says nothing and there are more rows than
-    // requests; a step whose padding or idle slots hide what it is says it. And
-    // only where the row kernel's work, a unit per eight pairs, KV head and page,
-    // is more than another kernel takes to begin and end, with page tables as full
-    // as they can be, since lengths are on the device: one request of eight heads to a KV head
-    // behind 12 rows, 320 units 14 us there and 33 with tiles, 1,536 31 and 38,
-    // 3,584 64 and 40; 16 requests of nine rows behind 12, 2,880 units 53 and 36; in
-    // FP32 four KV heads, six requests of 32 rows, 3,072 units 57 and 49, of 16
-    // rows, 1,536, 35 and 48.
-    // And in BF16 it is for a prefix that would keep the row kernel longer. A step of
-    // 128 keys costs here what four units do there, however few of its tile's 256
-    // pairs there are, so few pairs stay there: one request of eight heads to each
-    // of four KV heads behind 65,536 rows 38 us there and 71 with tiles, two 55 and
-    // 73, four 98 and 74; 16 behind 2,048 24 and 29, behind 4,096 36 and 31; 61
-    // behind 512 29 and 37, behind 1,024 39 and 38, behind 2,048 58 and 39. In FP32 the tiles' rate is
-    // no better than the row kernel's (61 behind 512 rows 76 us in it; behind 1,000, 2,000
-    // with tiles 103, 136: the same slope, 12 us more).
+    // requests (a step whose padding or idle slots hide what it is has to say). And
+    // only where the row kernel's work, a unit for eight pairs, a KV head and a page,
+    // takes longer than another kernel to begin and end, with the page tables as
+    // full as they can be, since lengths are on the device. Eight heads to each of
+    // four KV heads: one request behind 12 rows, 320 units 14 us there and 33 with
+    // tiles, 1,536 31 and 38, 3,584 64 and 40; 16 of nine rows behind 12, 2,880 units
+    // 53 and 36; in FP32 six of 16 rows, 1,536 units 35 and 48, of 32, 3,072 57 and 49.
+    // In BF16 it is also for a prefix that would keep the row kernel longer. A step
+    // of 128 keys costs what four units do, however few of its tile's 256 pairs there
+    // are, so few pairs stay there: one request behind 65,536 rows 38 us there and 71
+    // with tiles, two 55 and 73, four 98 and 74; 16 behind 2,048 24 and 29, behind
+    // 4,096 36 and 31; 61 behind 512 29 and 37, behind 1,024 39 and 38, behind 2,048
+    // 58 and 39. In FP32 the tiles' rate is no better than the row kernel's (61 behind
+    // 512 rows 76 us in it; behind 1,000, 2,000 with tiles 103, 136: the same slope,
+    // 12 us more).
     const bool f32 = d->type == PLAMO_PAGED_FP32;
     const uint64_t tile_pairs = f32 ? kTfPairs : kTlPairs;
     const uint64_t strips = ceil_div(pairs, kRtPairs) * d->kv_heads;

@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
     }
     const int64_t unit0 = pg_block_scan<kRtThreads>(units, scan, &all_units);
     const int32_t strip0 = static_cast<int32_t>(pg_block_scan<kRtThreads>(strips, scan, &all_strips));
-    if (all_units > INT32_MAX - 1024 || all_strips + p.workers > p.row_slots) {  // only starts that overlap ask for this
+    if (all_units > INT32_MAX - 1024 || all_strips + p.workers > p.row_slots) {  // starts that overlap, or 2^31 units
         if (tid == 0) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
         all_units = 0;
     }

@@ -16,9 +16,9 @@ namespace plamo {
 // 1024 cycles of exponentials (16 a cycle): the halves run half a step apart,
 // so that one's exponentials cover the other's products. Measured: 329 GFLOP of
 // ragged prompts behind 2,048 rows in 614 us, 0.54 PFLOP/s, the tensor pipe busy
-// for 43 % of it (the weights' second term among that). A half's chain bounds it, 3 us a step: scores, softmax, the value product, and the next scores only
-// when that is done, since they replace the weights; then 8 us at each segment's
-// ends.
+// for 43 % of it (the weights' second term among that). A half's chain bounds it,
+// 3 us a step: scores, softmax, the value product, and the next scores only when
+// that is done, since they replace the weights; then 8 us at each segment's ends.
 // The value product takes both operands in one type and the values are BF16, so
 // the FP32 weights go in as two BF16 terms, 16 bits together: the results are
 // then the exact ones rounded to BF16 (those prompts: 1.66e-3 from 64 bits,
