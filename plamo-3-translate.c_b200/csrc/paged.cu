@@ -239,7 +239,7 @@ extern "C" {
 
 int plamo_paged_plan(struct plamo_cuda *c, const struct plamo_paged_plan_args *d) {
     if (!c || !d) return 0;
-    if (!d->lengths || !d->starts || !d->summary || (d->requests && (!d->held || !d->added || !d->tables)) ||
+    if (!d->lengths || !d->starts || !d->summary || (d->requests && (!d->held || !d->added || (d->table_stride && !d->tables))) ||
         (d->rows && (!d->slots || !d->positions)) || (d->free_count && !d->free_pages))
         return context_decline(c, "paged_plan: a buffer is missing");
     if (d->rows > INT32_MAX - kPlanThreads || d->requests >= INT32_MAX || d->free_count > INT32_MAX ||
@@ -287,7 +287,8 @@ int plamo_paged_store(struct plamo_cuda *c, const struct plamo_paged_store_args 
     if (d->qkv_stride < heads * kPgDim || d->q_stride < static_cast<uint64_t>(d->query_heads) * kPgDim)
         return context_decline(c, "paged_store: a row stride is shorter than its row");
     if (!d->rows) return 1;
-    if (!d->qkv || !d->pool || !d->q || !d->slots || !d->positions || !d->q_norm || !d->k_norm || !d->table)
+    if (!d->qkv || !d->pool || !d->q || !d->slots || !d->positions || !d->q_norm || !d->k_norm ||
+        (d->positions_count && !d->table))
         return context_decline(c, "paged_store: a buffer is missing");
     // Four elements at a time.
     if (!aligned(d->qkv, 4 * element_bytes(d->qkv_type)) || !aligned(d->q, 4 * element_bytes(d->pool_type)) ||
@@ -327,7 +328,7 @@ int plamo_paged_attention(struct plamo_cuda *c, const struct plamo_paged_attenti
         return context_decline(c, "paged_attention: a row stride is shorter than its row");
     if (!std::isfinite(d->scale)) return context_decline(c, "paged_attention: scale must be finite");
     if (!d->rows) return 1;
-    if (!d->q || !d->pool || !d->out || !d->starts || (d->requests && (!d->lengths || !d->tables)) ||
+    if (!d->q || !d->pool || !d->out || !d->starts || (d->requests && (!d->lengths || (d->table_stride && !d->tables))) ||
         (d->prefix_rows && !d->prefix_pages))
         return context_decline(c, "paged_attention: a buffer is missing");
     if (!aligned(d->q, 16) || !aligned(d->out, 16) || !aligned(d->pool, 16) || d->q_stride % per16 || d->out_stride % per16)

@@ -319,3 +319,25 @@ def test_infinite_values_that_are_seen_make_infinite_results(be, requests, prefi
     got = attend(be, s).double().cpu()
     assert (got[hit] == sign * float("inf")).all()
     check(torch.where(hit, 0.0, got), torch.where(hit, 0.0, want), tol, "the other dimensions")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_requests_that_hold_nothing_need_no_page_table(be, dtype):
+    """Tables of no columns, and a rotation table of no positions, beside rows that are all padding."""
+    tables, none = torch.empty(2, 0, dtype=torch.int32, device="cuda"), ints([0, 0])
+    plan = be.paged_plan(none, none, tables, ints([]), 3)
+    assert plan.summary.tolist() == [0, 0, 0, 0] and plan.slots.tolist() == [-1] * 3
+    assert be.paged_plan(none, ints([0, 1]), tables, ints([4]), 3).summary[0].item() == 2
+    pool, norm = torch.ones(2, 2, ROWS, 2, DIM, dtype=dtype, device="cuda"), torch.zeros(DIM, dtype=BF16, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    empty = torch.empty(0, DIM, device="cuda")
+    q = be.paged_store(torch.ones(3, 6 * DIM, device="cuda"), pool, plan.slots, plan.positions, norm, norm, empty, status=status)
+    assert (q == 0).all() and (pool == 1).all()
+    for prefix in (0, 70):
+        out = be.paged_attention(q, pool, plan.starts, plan.lengths, tables, prefix_pages=ints([0, 1]), prefix_rows=prefix, status=status)
+        assert (out == 0).all()
+    assert status.item() == 0
+    be.paged_store(torch.ones(3, 6 * DIM, device="cuda"), pool, ints([5, -1, -1]), plan.positions, norm, norm, empty, status=status)
+    assert status.item() == 32 and (pool == 1).all()
+    be.paged_attention(q, pool, ints([0, 1, 3]), ints([1, 2]), tables, status=status)
+    assert status.item() & 2
