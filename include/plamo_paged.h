@@ -18,6 +18,22 @@
  *                          prefixes: for eight), and once for each of the
  *                          tiles of those that add many.
  *
+ * A step that verifies drafted tokens adds, per request, a tree of them: the
+ * last token, continuations of it, continuations of those. Four more operators
+ * serve it, and one serves steps of any kind:
+ *
+ *   plamo_paged_tree            positions and visibility masks from the rows'
+ *                               parents (once per step, before the store);
+ *   plamo_paged_tree_attention  plamo_paged_attention whose new rows see, of
+ *                               their step's rows, those of their mask only;
+ *   plamo_paged_accept          the path of drafts that the model's choices
+ *                               confirm, and the pages that it gives back
+ *                               (once per step, after the last layer);
+ *   plamo_paged_keep            the confirmed rows moved together, in the pools
+ *                               of up to any number of layers;
+ *   plamo_paged_adapters        beside a projection of the batch's rows, each
+ *                               request's own low-rank adapter.
+ *
  * Pool: [pages][2][64][kv_heads][128] elements of BF16 or FP32, 16-byte
  * aligned: a page holds 64 key rows, then 64 value rows, as the token loop's
  * own KV pages do (there FP32 and unrotated; here keys are stored rotated).
@@ -62,8 +78,11 @@ enum {
     PLAMO_PAGED_COUNT = 8,      /* a negative row count, or one past 2^31 - 1 */
     PLAMO_PAGED_PAGE = 16,      /* a page id or slot outside the pool */
     PLAMO_PAGED_POSITION = 32,  /* a position outside the rotation table */
-    PLAMO_PAGED_FAILED = 64     /* a bounded wait of a kernel ran out: its results are not valid */
+    PLAMO_PAGED_FAILED = 64,    /* a bounded wait of a kernel ran out: its results are not valid */
+    PLAMO_PAGED_TREE = 128,     /* a parent that is no earlier row of its request, or more rows than a mask has bits */
+    PLAMO_PAGED_ADAPTER = 256   /* an adapter id that is none */
 };
+enum { PLAMO_PAGED_TREE_ROWS = 256 }; /* rows of a request's tree, at most */
 
 struct plamo_cuda;
 
@@ -162,6 +181,117 @@ uint64_t plamo_paged_attention_workspace(struct plamo_cuda *, const struct plamo
    hold. Scores, softmax sums and products are FP32 for both types (against
    a BF16 pool's values the softmax weights go in as two BF16 terms, 16 bits). */
 int plamo_paged_attention(struct plamo_cuda *, const struct plamo_paged_attention_args *);
+
+struct plamo_paged_tree_args {
+    const int32_t *parents; /* [rows] place of a row's parent among its request's new rows, before its own;
+                               -1: it follows the held rows */
+    const int32_t *starts;  /* [requests + 1] */
+    const int32_t *lengths; /* [requests] own rows, those of this step included */
+    int32_t *positions;     /* [rows] out: base + held rows + generations above; 0 for padding */
+    uint32_t *masks;        /* [rows][words] out: bit j: the row sees its request's j-th new row (itself and the
+                               rows above it); 0 for padding */
+    uint32_t *status;
+    uint64_t rows, requests;
+    uint32_t words;         /* 1 to 8: trees have at most 32 * words rows */
+    int64_t base;           /* position of own row 0: the prefix's rows */
+    void *stream;
+};
+/* Slots are the plan's: a tree's rows lie one after another in their pages,
+   whatever their positions. A row whose parent is out of range is reported
+   (PLAMO_PAGED_TREE) and taken as one that follows the held rows; so reported
+   are requests of more than 32 * words rows, whose rows from there on get no
+   bits. Neither output may overlap an input. */
+int plamo_paged_tree(struct plamo_cuda *, const struct plamo_paged_tree_args *);
+
+struct plamo_paged_tree_attention_args {
+    struct plamo_paged_attention_args step;
+    const uint32_t *masks; /* [rows][words], of plamo_paged_tree or any others */
+    uint32_t words;        /* 1 to 8 */
+};
+uint64_t plamo_paged_tree_attention_workspace(struct plamo_cuda *, const struct plamo_paged_tree_attention_args *);
+/* plamo_paged_attention, but for the rows seen: a new row sees the prefix's
+   rows, the rows that its request held before the step (lengths less its new
+   rows) and those of its new rows whose bits are set, in this order; of all
+   these the last `window` when there is one. (With masks of trees that is the
+   rows at the last `window` positions.) Bits past the request's rows mean
+   nothing. A row that sees nothing gets zeros, and so do all rows of a request
+   that holds fewer rows than it adds. Requests of more than 32 * words rows are
+   reported (PLAMO_PAGED_TREE); no row sees those from there on. */
+int plamo_paged_tree_attention(struct plamo_cuda *, const struct plamo_paged_tree_attention_args *);
+
+struct plamo_paged_accept_args {
+    const int32_t *parents; /* [rows] as plamo_paged_tree's */
+    const int32_t *tokens;  /* [rows] each row's token */
+    const int32_t *chosen;  /* [rows] the token that the model chooses after each row */
+    const int32_t *starts, *lengths; /* of the step's plan */
+    const int32_t *tables;  /* [requests][table_stride] */
+    int32_t *free_pages;    /* [free_count] the plan's list; pages given back are written before its head */
+    const int32_t *plan;    /* [4] the plan's summary */
+    int32_t *counts;        /* [requests] out: confirmed rows, 0 where a request has none */
+    int32_t *kept;          /* [requests] out: own rows after the step, held + confirmed */
+    int32_t *last;          /* [requests] out: the last token, chosen after the last confirmed row; -1 where none is */
+    int32_t *path;          /* [rows] out: at starts[r] + k the k-th confirmed row's place among request r's; else -1 */
+    int32_t *next;          /* [rows] out: at starts[r] + k the token chosen after it; else -1 */
+    int32_t *summary;       /* [4] out, as a plan's: status bits, confirmed rows, free-list entries used so far
+                               (the plan's less the pages given back), longest length */
+    uint64_t rows, requests, table_stride, free_count;
+    void *stream;
+};
+/* A request's first row is certain. After a confirmed row comes, if there is
+   one, the first of the rows whose parent it is and whose token is the one
+   chosen after it. The pages that only rows not kept had reached are given back,
+   in the requests' order, to the end of the entries used so far: a plan whose
+   `head` is &summary[2] takes them first. Give back before another plan takes
+   pages from the list; entries of the tables stay, and the moves of plamo_paged_keep
+   for the same step may come after. Where the list cannot have held the pages (fewer
+   entries used than come back) none is given back and summary[0] gets
+   PLAMO_PAGED_NO_PAGES; a page table too short for its request's rows sets PLAMO_PAGED_TABLE;
+   a step that the plan declined keeps what was held. `summary` may be `plan`
+   itself; outputs overlap nothing else. */
+int plamo_paged_accept(struct plamo_cuda *, const struct plamo_paged_accept_args *);
+
+struct plamo_paged_keep_args {
+    void *const *pools;     /* [layers] on the host: device pools of one shape and type */
+    const int32_t *path;    /* [rows] of plamo_paged_accept */
+    const int32_t *starts, *lengths; /* of the step's plan */
+    const int32_t *tables;  /* [requests][table_stride] */
+    uint32_t *status;
+    uint64_t layers, rows, requests, table_stride, pages;
+    uint32_t kv_heads, type;
+    void *stream;
+};
+/* In every pool: request r's new row path[starts[r] + k], its keys and values, becomes
+   its own row held + k, for k from 0 as long as the path rises. Rows that it does
+   not reach stay as they are. */
+int plamo_paged_keep(struct plamo_cuda *, const struct plamo_paged_keep_args *);
+
+struct plamo_paged_adapters_args {
+    const void *x;         /* [rows][columns], rows x_stride elements apart: the projection's input */
+    const void *base;      /* [rows][outputs], rows base_stride elements apart: its result */
+    void *out;             /* as base, rows out_stride elements apart; may be base itself */
+    const uint16_t *a;     /* [adapters][rank][columns] BF16 */
+    const uint16_t *b;     /* [adapters][outputs][rank] BF16 */
+    const float *scales;   /* [adapters], or NULL for 1 */
+    const int32_t *ids;    /* [requests] each request's adapter, -1 for none */
+    const int32_t *starts; /* [requests + 1] */
+    void *workspace;       /* plamo_paged_adapters_workspace() bytes, 256-byte aligned */
+    uint64_t workspace_bytes;
+    uint32_t *status;
+    uint64_t rows, columns, outputs, x_stride, base_stride, out_stride, requests, adapters;
+    uint32_t rank, x_type, type; /* `type`: of base and out */
+    void *stream;
+    uint64_t most_new;     /* rows of the request that adds most, 0: not known; it chooses the kernels */
+};
+/* Device bytes a call with these shapes needs (its pointers are not read); 0
+   when the shapes would be declined: rank, columns and outputs are multiples of
+   8 (pad with zeros), rank at most 256. */
+uint64_t plamo_paged_adapters_workspace(struct plamo_cuda *, const struct plamo_paged_adapters_args *);
+/* out = base + scale * B (A x) for the rows of requests that have an adapter;
+   the other rows, and the padding, are base's. Both products are summed in FP32, of x
+   and of A x as they are; out is rounded once. Requests with the same adapter
+   one after another share its reading. An id outside the adapters is
+   reported (PLAMO_PAGED_ADAPTER) and none. */
+int plamo_paged_adapters(struct plamo_cuda *, const struct plamo_paged_adapters_args *);
 
 #ifdef __cplusplus
 }

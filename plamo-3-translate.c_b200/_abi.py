@@ -269,8 +269,43 @@ class PagedAttentionArgs(ctypes.Structure):
                 ("stream", c_void_p), ("most_new", c_uint64)]
 
 
+class PagedTreeArgs(ctypes.Structure):
+    """struct plamo_paged_tree_args (include/plamo_paged.h)."""
+    _fields_ = [(n, c_void_p) for n in ("parents", "starts", "lengths", "positions", "masks", "status")] + \
+               [("rows", c_uint64), ("requests", c_uint64), ("words", c_uint32), ("base", c_int64), ("stream", c_void_p)]
+
+
+class PagedTreeAttentionArgs(ctypes.Structure):
+    """struct plamo_paged_tree_attention_args (include/plamo_paged.h)."""
+    _fields_ = [("step", PagedAttentionArgs), ("masks", c_void_p), ("words", c_uint32)]
+
+
+class PagedAcceptArgs(ctypes.Structure):
+    """struct plamo_paged_accept_args (include/plamo_paged.h)."""
+    _fields_ = [(n, c_void_p) for n in ("parents", "tokens", "chosen", "starts", "lengths", "tables", "free_pages", "plan",
+                                        "counts", "kept", "last", "path", "next", "summary")] + \
+               [(n, c_uint64) for n in ("rows", "requests", "table_stride", "free_count")] + [("stream", c_void_p)]
+
+
+class PagedKeepArgs(ctypes.Structure):
+    """struct plamo_paged_keep_args (include/plamo_paged.h)."""
+    _fields_ = [(n, c_void_p) for n in ("pools", "path", "starts", "lengths", "tables", "status")] + \
+               [(n, c_uint64) for n in ("layers", "rows", "requests", "table_stride", "pages")] + \
+               [("kv_heads", c_uint32), ("type", c_uint32), ("stream", c_void_p)]
+
+
+class PagedAdaptersArgs(ctypes.Structure):
+    """struct plamo_paged_adapters_args (include/plamo_paged.h)."""
+    _fields_ = [(n, c_void_p) for n in ("x", "base", "out", "a", "b", "scales", "ids", "starts", "workspace")] + \
+               [("workspace_bytes", c_uint64), ("status", c_void_p)] + \
+               [(n, c_uint64) for n in ("rows", "columns", "outputs", "x_stride", "base_stride", "out_stride", "requests",
+                                        "adapters")] + \
+               [("rank", c_uint32), ("x_type", c_uint32), ("type", c_uint32), ("stream", c_void_p), ("most_new", c_uint64)]
+
+
 PAGED_ROWS, PAGED_DIM = 64, 128  # PLAMO_PAGED_ROWS, PLAMO_PAGED_DIM
 PAGED_BF16, PAGED_FP32 = 0, 1  # PLAMO_PAGED_BF16, PLAMO_PAGED_FP32
+PAGED_TREE_ROWS = 256  # PLAMO_PAGED_TREE_ROWS
 # include/plamo_paged.h: operators of a paged batch step
 PAGED_SIGNATURES = {
     "plamo_paged_plan": (c_int, [P, POINTER(PagedPlanArgs)]),
@@ -278,6 +313,13 @@ PAGED_SIGNATURES = {
     "plamo_paged_status": (c_uint32, [P]),
     "plamo_paged_attention": (c_int, [P, POINTER(PagedAttentionArgs)]),
     "plamo_paged_attention_workspace": (c_uint64, [P, POINTER(PagedAttentionArgs)]),
+    "plamo_paged_tree": (c_int, [P, POINTER(PagedTreeArgs)]),
+    "plamo_paged_tree_attention": (c_int, [P, POINTER(PagedTreeAttentionArgs)]),
+    "plamo_paged_tree_attention_workspace": (c_uint64, [P, POINTER(PagedTreeAttentionArgs)]),
+    "plamo_paged_accept": (c_int, [P, POINTER(PagedAcceptArgs)]),
+    "plamo_paged_keep": (c_int, [P, POINTER(PagedKeepArgs)]),
+    "plamo_paged_adapters": (c_int, [P, POINTER(PagedAdaptersArgs)]),
+    "plamo_paged_adapters_workspace": (c_uint64, [P, POINTER(PagedAdaptersArgs)]),
 }
 
 _libs = {}

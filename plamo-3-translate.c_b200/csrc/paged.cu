@@ -3,11 +3,15 @@
 #include "../../include/plamo_paged.h"
 #include "context.h"
 #include "paged.cuh"
+#include "paged_adapters.cuh"
 #include "paged_attention.cuh"
 #include "paged_tiles.cuh"
+#include "paged_trees.cuh"
 
 #include <algorithm>
 #include <cmath>
+#include <new>
+#include <vector>
 
 using namespace plamo;
 
@@ -56,14 +60,24 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
     return nullptr;
 }
 
+// Prefix rows from which trees share tiles over them.
+constexpr uint64_t kTreeShareRows = 512;
+
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
     uint32_t prefix_tiles, row_slots, workers, tile_rows, tile_grid, tile_cap;
     uint64_t record, row_sum, row_ml;
     uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
+    bool share;  // trees: all rows share the prefix's tiles
 };
 
-AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attention_args *d) {
+// Draft trees: what a call has beside the step's records.
+struct TreeMasks {
+    const uint32_t *masks;
+    uint32_t words;  // 0: no trees
+};
+
+AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attention_args *d, bool trees) {
     AttentionLayout a{};
     const uint64_t group = d->query_heads / d->kv_heads, sms = static_cast<uint64_t>(context_sms(c));
     const uint64_t pairs = d->rows * group, prefix_pages = ceil_div(d->prefix_rows, kPgRows);
@@ -95,6 +109,7 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
         a.tile_grid = static_cast<uint32_t>(f32 ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
         a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
+        a.share = trees && d->prefix_rows >= kTreeShareRows;
     }
     a.prefix_tiles = prefix_pages && !a.tile_rows ? static_cast<uint32_t>(ceil_div(pairs, kRtPairs)) : 0;
     a.workers = static_cast<uint32_t>(2 * sms - 1);  // beside the schedule's CTA
@@ -118,7 +133,9 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     a.row_ml = part(static_cast<uint64_t>(a.row_slots) * kRtPairs * sizeof(float2));
     if (a.tile_rows) {
         // Two runs of a CTA may end inside a prompt's tile; every run of a prefix tile is a part.
-        const uint64_t shared = prefix_pages ? a.tile_grid + ceil_div(d->rows, a.tile_rows) * d->kv_heads : 0;
+        // Where trees share the prefix, so is every run of any tile.
+        const uint64_t kept = a.share ? a.tile_cap : ceil_div(d->rows, a.tile_rows);
+        const uint64_t shared = prefix_pages ? a.tile_grid + kept * d->kv_heads : 0;
         const uint64_t slots = 2ull * a.tile_grid + shared;
         a.tile_shape = part(a.tile_cap * sizeof(TileShape));
         a.tile_unit = part((a.tile_cap + 1ull) * 4);
@@ -129,8 +146,8 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     return a;
 }
 
-template <bool F32>
-bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const AttentionLayout &a, cudaStream_t stream) {
+template <bool F32, bool TREE>
+bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const TreeMasks &t, const AttentionLayout &a, cudaStream_t stream) {
     const auto pool_map = [&](CUtensorMap *map, uint32_t rows) {
         return tensor_map_2d(map, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, F32 ? 4 : 2,
                              d->pool, d->pages * 2 * kPgRows, static_cast<uint64_t>(d->kv_heads) * kPgDim, F32 ? 32 : 64, rows);
@@ -162,6 +179,11 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     p.max_length = static_cast<int32_t>(d->table_stride * kPgRows);
     // A window that reaches back past every row hides nothing.
     p.window = d->window > d->prefix_rows + d->table_stride * kPgRows ? 0 : static_cast<int32_t>(d->window);
+    // A plain request's first new row sees itself, the masks' rows perhaps none of the new ones.
+    p.reach = p.window - (TREE ? 0 : 1);
+    p.masks = t.masks;
+    p.words = static_cast<int32_t>(t.words);
+    p.share = a.share;
     p.scale2 = d->scale * 1.4426950408889634f;
     // The tile kernel masks before it scales: -inf must stay so.
     if (std::fabs(p.scale2) < 1e-30f) p.scale2 = std::copysign(1e-30f, p.scale2);
@@ -186,8 +208,8 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
         p.tile_sum = reinterpret_cast<float *>(ws + a.tile_sum);
         p.tile_ml = reinterpret_cast<float2 *>(ws + a.tile_ml);
     }
-    if (!launch(c, "paged_attention rows", paged_rows_kernel<F32>, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
-        (a.tile_rows && !launch(c, "paged_attention tiles", F32 ? paged_tile_f32_kernel : paged_tile_kernel, dim3(a.tile_grid),
+    if (!launch(c, "paged_attention rows", paged_rows_kernel<F32, TREE>, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
+        (a.tile_rows && !launch(c, "paged_attention tiles", F32 ? paged_tile_f32_kernel<TREE> : paged_tile_kernel<TREE>, dim3(a.tile_grid),
                                 dim3(F32 ? kTfThreads : kTlThreads), F32 ? kTfSmem : kTlSmem, stream, true, page_map, p)))
         return false;
     // Two results to a block, its warps sharing their parts, while that takes two
@@ -197,9 +219,9 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Att
     // warp); then eight to a warp (256 requests, 6 parts: 21 us against 39).
     const uint64_t sms = static_cast<uint64_t>(context_sms(c)), twos = d->rows * ceil_div(d->query_heads, 2);
     const uint64_t eights = d->rows * ceil_div(d->query_heads, 8);
-    const auto join = twos <= 2 * sms     ? paged_join_kernel<F32, 2, true>
-                      : eights <= 4 * sms ? paged_join_kernel<F32, 8, true>
-                                          : paged_join_kernel<F32, 8, false>;
+    const auto join = twos <= 2 * sms     ? paged_join_kernel<F32, 2, true, TREE>
+                      : eights <= 4 * sms ? paged_join_kernel<F32, 8, true, TREE>
+                                          : paged_join_kernel<F32, 8, false, TREE>;
     const uint64_t blocks = std::min(4 * sms, std::max<uint64_t>(a.tile_rows ? 4 * sms : 1, twos <= 2 * sms ? twos : eights));
     return launch(c, "paged_attention join", join, dim3(static_cast<uint32_t>(blocks)), dim3(kJoinThreads), 0, stream, true, p);
 }
@@ -220,6 +242,71 @@ bool run_store(plamo_cuda *c, const plamo_paged_store_args *d, cudaStream_t stre
     return launch(c, "paged_store", paged_store_kernel<In, Out, 1>, grid, dim3(256), 0, stream, false, args);
 }
 
+// Buffers of 32-bit entries that must not overlap: each output none of the inputs and no other output.
+struct Span {
+    const int32_t *at;
+    uint64_t count;
+};
+template <size_t O, size_t I>
+bool spans_meet(const Span (&outputs)[O], const Span (&inputs)[I]) {
+    for (size_t i = 0; i < O; ++i) {
+        for (size_t j = i + 1; j < O; ++j)
+            if (overlap(outputs[i].at, outputs[i].count, outputs[j].at, outputs[j].count)) return true;
+        for (size_t j = 0; j < I; ++j)
+            if (overlap(outputs[i].at, outputs[i].count, inputs[j].at, inputs[j].count)) return true;
+    }
+    return false;
+}
+
+// Shapes of an adapters call; NULL when they are fine, else what is wrong.
+const char *adapters_shapes(const plamo_paged_adapters_args *d) {
+    if (!type_ok(d->x_type) || !type_ok(d->type)) return "paged_adapters: types must be PLAMO_PAGED_BF16 or PLAMO_PAGED_FP32";
+    if (!d->rank || d->rank % 8 || d->rank > kAdMaxRank) return "paged_adapters: rank must be a multiple of 8, at most 256";
+    if (!d->columns || d->columns % 8 || !d->outputs || d->outputs % 8 || d->columns > 1u << 22 || d->outputs > 1u << 22)
+        return "paged_adapters: columns and outputs must be multiples of 8, at most 2^22";
+    if (d->rows > 1u << 24 || d->requests > kPgMaxCount || d->adapters > 1u << 24)
+        return "paged_adapters: at most 2^24 rows and adapters, 2^30 requests";
+    return nullptr;
+}
+
+struct AdaptersLayout {
+    uint32_t splits, share;
+    uint64_t bytes;
+};
+AdaptersLayout adapters_layout(const plamo_cuda *c, const plamo_paged_adapters_args *d) {
+    AdaptersLayout a{};
+    // Shares of the columns until there are four CTAs to an SM.
+    const uint64_t tiles = ceil_div(d->rows, kAdRows) * ceil_div(d->rank, 16), rounds = ceil_div(d->columns, kAdColumns);
+    const uint64_t want = std::min<uint64_t>(rounds, std::max<uint64_t>(1, 4ull * context_sms(c) / std::max<uint64_t>(1, tiles)));
+    a.share = static_cast<uint32_t>(ceil_div(rounds, want) * kAdColumns);
+    a.splits = static_cast<uint32_t>(ceil_div(d->columns, a.share));
+    a.bytes = std::max<uint64_t>(256, static_cast<uint64_t>(a.splits) * d->rows * d->rank * 4);
+    return a;
+}
+
+int attention(plamo_cuda *c, const plamo_paged_attention_args *d, const TreeMasks &t) {
+    if (const char *why = attention_shapes(d)) return context_decline(c, why);
+    const uint64_t width = static_cast<uint64_t>(d->query_heads) * kPgDim, per16 = 16 / element_bytes(d->type);
+    if (d->q_stride < width || d->out_stride < width)
+        return context_decline(c, "paged_attention: a row stride is shorter than its row");
+    if (!std::isfinite(d->scale)) return context_decline(c, "paged_attention: scale must be finite");
+    if (!d->rows) return 1;
+    if (!d->q || !d->pool || !d->out || !d->starts || (d->requests && (!d->lengths || (d->table_stride && !d->tables))) ||
+        (d->prefix_rows && !d->prefix_pages))
+        return context_decline(c, "paged_attention: a buffer is missing");
+    if (!aligned(d->q, 16) || !aligned(d->out, 16) || !aligned(d->pool, 16) || d->q_stride % per16 || d->out_stride % per16)
+        return context_decline(c, "paged_attention: pool, queries and results must start on 16-byte boundaries, row by row");
+    const AttentionLayout a = attention_layout(c, d, t.words);
+    if (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < a.bytes)
+        return context_decline(c, "paged_attention: the workspace is missing, too small or not 256-byte aligned");
+    ContextDevice device(c);
+    const cudaStream_t stream = stream_of(c, d->stream);
+    const bool f32 = d->type == PLAMO_PAGED_FP32;
+    const bool ok = t.words ? (f32 ? run_attention<true, true>(c, d, t, a, stream) : run_attention<false, true>(c, d, t, a, stream))
+                            : (f32 ? run_attention<true, false>(c, d, t, a, stream) : run_attention<false, false>(c, d, t, a, stream));
+    return ok ? 1 : -1;
+}
+
 }  // namespace
 
 namespace plamo {
@@ -227,10 +314,14 @@ cudaError_t paged_configure() {
     const auto allow = [](auto kernel, int bytes) {
         return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-    cudaError_t e = allow(paged_rows_kernel<false>, kRtSmem);
-    if (e == cudaSuccess) e = allow(paged_rows_kernel<true>, kRtSmem);
-    if (e == cudaSuccess) e = allow(paged_tile_kernel, kTlSmem);
-    if (e == cudaSuccess) e = allow(paged_tile_f32_kernel, kTfSmem);
+    cudaError_t e = allow(paged_rows_kernel<false, false>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_rows_kernel<true, false>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_rows_kernel<false, true>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_rows_kernel<true, true>, kRtSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_kernel<false>, kTlSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_kernel<true>, kTlSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<false>, kTfSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<true>, kTfSmem);
     return e;
 }
 }  // namespace plamo
@@ -317,29 +408,196 @@ uint32_t plamo_paged_status(struct plamo_cuda *c) {
 uint64_t plamo_paged_attention_workspace(struct plamo_cuda *c, const struct plamo_paged_attention_args *d) {
     if (!c || !d) return 0;
     if (const char *why = attention_shapes(d)) return static_cast<uint64_t>(context_decline(c, why));
-    return attention_layout(c, d).bytes;
+    return attention_layout(c, d, false).bytes;
 }
 
 int plamo_paged_attention(struct plamo_cuda *c, const struct plamo_paged_attention_args *d) {
+    return c && d ? attention(c, d, TreeMasks{nullptr, 0}) : 0;
+}
+
+uint64_t plamo_paged_tree_attention_workspace(struct plamo_cuda *c, const struct plamo_paged_tree_attention_args *d) {
     if (!c || !d) return 0;
-    if (const char *why = attention_shapes(d)) return context_decline(c, why);
-    const uint64_t width = static_cast<uint64_t>(d->query_heads) * kPgDim, per16 = 16 / element_bytes(d->type);
-    if (d->q_stride < width || d->out_stride < width)
-        return context_decline(c, "paged_attention: a row stride is shorter than its row");
-    if (!std::isfinite(d->scale)) return context_decline(c, "paged_attention: scale must be finite");
+    if (const char *why = attention_shapes(&d->step)) return static_cast<uint64_t>(context_decline(c, why));
+    return attention_layout(c, &d->step, true).bytes;
+}
+
+int plamo_paged_tree_attention(struct plamo_cuda *c, const struct plamo_paged_tree_attention_args *d) {
+    if (!c || !d) return 0;
+    if (!d->words || d->words > kTreeRows / 32) return context_decline(c, "paged_tree_attention: a mask has 1 to 8 words");
+    if (d->step.rows && (!d->masks || !aligned(d->masks, 4)))
+        return context_decline(c, "paged_tree_attention: the masks are missing or not 4-byte aligned");
+    return attention(c, &d->step, TreeMasks{d->masks, d->words});
+}
+
+int plamo_paged_tree(struct plamo_cuda *c, const struct plamo_paged_tree_args *d) {
+    if (!c || !d) return 0;
+    if (!d->words || d->words > kTreeRows / 32) return context_decline(c, "paged_tree: a mask has 1 to 8 words");
+    if (d->rows > kPgMaxCount || d->requests > kPgMaxCount || d->base < 0 || d->base > INT32_MAX)
+        return context_decline(c, "paged_tree: a count is out of range");
     if (!d->rows) return 1;
-    if (!d->q || !d->pool || !d->out || !d->starts || (d->requests && (!d->lengths || (d->table_stride && !d->tables))) ||
-        (d->prefix_rows && !d->prefix_pages))
-        return context_decline(c, "paged_attention: a buffer is missing");
-    if (!aligned(d->q, 16) || !aligned(d->out, 16) || !aligned(d->pool, 16) || d->q_stride % per16 || d->out_stride % per16)
-        return context_decline(c, "paged_attention: pool, queries and results must start on 16-byte boundaries, row by row");
-    const AttentionLayout a = attention_layout(c, d);
-    if (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < a.bytes)
-        return context_decline(c, "paged_attention: the workspace is missing, too small or not 256-byte aligned");
+    if (!d->parents || !d->positions || !d->masks || (d->requests && (!d->starts || !d->lengths)))
+        return context_decline(c, "paged_tree: a buffer is missing");
+    const Span inputs[] = {{d->parents, d->rows}, {d->starts, d->requests + 1}, {d->lengths, d->requests}};
+    const Span outputs[] = {{d->positions, d->rows}, {reinterpret_cast<const int32_t *>(d->masks), d->rows * d->words}};
+    if (spans_meet(outputs, inputs)) return context_decline(c, "paged_tree: buffers overlap");
+    ContextDevice device(c);
+    plamo_paged_tree_args args = *d;
+    if (!args.status) args.status = context_paged_status(c);
+    return launch(c, "paged_tree", paged_tree_kernel, dim3(static_cast<uint32_t>(std::max<uint64_t>(1, d->requests))),
+                  dim3(32 * d->words), 0, stream_of(c, d->stream), false, args)
+               ? 1
+               : -1;
+}
+
+int plamo_paged_accept(struct plamo_cuda *c, const struct plamo_paged_accept_args *d) {
+    if (!c || !d) return 0;
+    const uint64_t R = d->requests;
+    if (!d->plan || !d->summary || !d->starts || (R && (!d->lengths || !d->counts || !d->kept || !d->last || (d->table_stride && !d->tables))) ||
+        (d->rows && (!d->parents || !d->tokens || !d->chosen || !d->path || !d->next)) || (d->free_count && !d->free_pages))
+        return context_decline(c, "paged_accept: a buffer is missing");
+    if (d->rows > kPgMaxCount || R > kPgMaxCount || d->free_count > INT32_MAX || d->table_stride > static_cast<uint64_t>(kPgMaxPages))
+        return context_decline(c, "paged_accept: a count is out of range");
+    const Span inputs[] = {{d->parents, d->rows}, {d->tokens, d->rows}, {d->chosen, d->rows}, {d->starts, R + 1},
+                           {d->lengths, R}, {d->tables, R * d->table_stride}, {d->plan, 4}};
+    const Span outputs[] = {{d->counts, R}, {d->kept, R}, {d->last, R}, {d->path, d->rows}, {d->next, d->rows},
+                            {d->summary, 4}, {d->free_pages, d->free_count}};
+    if (spans_meet(outputs, inputs)) return context_decline(c, "paged_accept: buffers overlap");
     ContextDevice device(c);
     const cudaStream_t stream = stream_of(c, d->stream);
-    const bool ok = d->type == PLAMO_PAGED_FP32 ? run_attention<true>(c, d, a, stream) : run_attention<false>(c, d, a, stream);
-    return ok ? 1 : -1;
+    if (R <= kAcceptAlone)
+        return launch(c, "paged_accept", paged_accept_kernel, dim3(1), dim3(kAcceptThreads), 0, stream, false, *d) ? 1 : -1;
+    return launch(c, "paged_accept walk", paged_accept_walk_kernel, dim3(static_cast<uint32_t>(ceil_div(R, kAcceptWarps))),
+                  dim3(32 * kAcceptWarps), 0, stream, false, *d) &&
+                   launch(c, "paged_accept settle", paged_accept_settle_kernel, dim3(1), dim3(kAcceptThreads), 0, stream, true, *d)
+               ? 1
+               : -1;
+}
+
+int plamo_paged_keep(struct plamo_cuda *c, const struct plamo_paged_keep_args *d) {
+    if (!c || !d) return 0;
+    if (!type_ok(d->type)) return context_decline(c, "paged_keep: type must be PLAMO_PAGED_BF16 or PLAMO_PAGED_FP32");
+    if (!d->kv_heads || d->kv_heads > 4096) return context_decline(c, "paged_keep: kv_heads must be 1 to 4096");
+    if (!d->pages || d->pages > static_cast<uint64_t>(kPgMaxPages) || d->rows > kPgMaxCount || d->requests > kPgMaxCount ||
+        d->table_stride > static_cast<uint64_t>(kPgMaxPages) || d->layers > 65536)
+        return context_decline(c, "paged_keep: a count is out of range");
+    if (!d->rows || !d->requests || !d->layers) return 1;
+    if (!d->pools || !d->path || !d->starts || !d->lengths || (d->table_stride && !d->tables))
+        return context_decline(c, "paged_keep: a buffer is missing");
+    // A pool named twice would have its rows moved twice.
+    std::vector<const void *> sorted;
+    try {
+        sorted.assign(d->pools, d->pools + d->layers);
+    } catch (const std::bad_alloc &) {
+        return context_decline(c, "paged_keep: out of host memory");
+    }
+    std::sort(sorted.begin(), sorted.end());
+    const uint64_t row_bytes = d->kv_heads * kPgDim * element_bytes(d->type), pool_bytes = d->pages * 2 * kPgRows * row_bytes;
+    for (uint64_t i = 0; i < d->layers; ++i) {
+        if (!sorted[i] || !aligned(sorted[i], 16)) return context_decline(c, "paged_keep: a pool is missing or not 16-byte aligned");
+        if (i && static_cast<const char *>(sorted[i - 1]) + pool_bytes > sorted[i])
+            return context_decline(c, "paged_keep: pools overlap");
+    }
+    ContextDevice device(c);
+    const cudaStream_t stream = stream_of(c, d->stream);
+    for (uint64_t first = 0; first < d->layers; first += kKeepLayers) {
+        KeepParams p{};
+        p.layers = static_cast<int32_t>(std::min<uint64_t>(kKeepLayers, d->layers - first));
+        std::copy(d->pools + first, d->pools + first + p.layers, p.pools);
+        p.path = d->path;
+        p.starts = d->starts;
+        p.lengths = d->lengths;
+        p.tables = d->tables;
+        p.status = d->status ? d->status : context_paged_status(c);
+        p.rows = d->rows;
+        p.table_stride = d->table_stride;
+        p.pages = static_cast<int32_t>(d->pages);
+        p.row_bytes = static_cast<int32_t>(row_bytes);
+        // Looking the slots up takes as long as moving a layer or two: few layers to a CTA
+        // until there are CTAs for every place on the SMs.
+        const uint64_t places = 8ull * static_cast<uint64_t>(context_sms(c));
+        p.per = static_cast<int32_t>(std::min<uint64_t>(p.layers, std::max<uint64_t>(1, p.layers * d->requests / places)));
+        if (!launch(c, "paged_keep", paged_keep_kernel, dim3(static_cast<uint32_t>(d->requests), static_cast<uint32_t>(ceil_div(p.layers, p.per))),
+                    dim3(kKeepThreads), 0, stream, false, p))
+            return -1;
+    }
+    return 1;
+}
+
+uint64_t plamo_paged_adapters_workspace(struct plamo_cuda *c, const struct plamo_paged_adapters_args *d) {
+    if (!c || !d) return 0;
+    if (const char *why = adapters_shapes(d)) return static_cast<uint64_t>(context_decline(c, why));
+    return adapters_layout(c, d).bytes;
+}
+
+int plamo_paged_adapters(struct plamo_cuda *c, const struct plamo_paged_adapters_args *d) {
+    if (!c || !d) return 0;
+    if (const char *why = adapters_shapes(d)) return context_decline(c, why);
+    if (d->x_stride < d->columns || d->base_stride < d->outputs || d->out_stride < d->outputs)
+        return context_decline(c, "paged_adapters: a row stride is shorter than its row");
+    if (!d->rows) return 1;
+    if (!d->x || !d->base || !d->out || !d->starts || (d->requests && !d->ids) || (d->adapters && (!d->a || !d->b)))
+        return context_decline(c, "paged_adapters: a buffer is missing");
+    const uint64_t x_bytes = element_bytes(d->x_type), bytes = element_bytes(d->type);
+    if (!aligned(d->x, 16) || !aligned(d->base, 16) || !aligned(d->out, 16) || !aligned(d->a, 16) || !aligned(d->b, 16) ||
+        d->x_stride * x_bytes % 16 || d->base_stride * bytes % 16 || d->out_stride * bytes % 16)
+        return context_decline(c, "paged_adapters: rows and adapters must start on 16-byte boundaries");
+    // Rows of one wide matrix may lie between another's: of buffers with one stride only
+    // those are declined whose rows meet.
+    const auto meet = [&](const void *a, uint64_t a_stride, uint64_t a_row, const void *b, uint64_t b_stride, uint64_t b_row) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+        if (x >= y + (d->rows - 1) * b_stride + b_row || y >= x + (d->rows - 1) * a_stride + a_row) return false;
+        if (a_stride != b_stride) return true;
+        const uint64_t off = x >= y ? (x - y) % a_stride : (a_stride - (y - x) % a_stride) % a_stride;  // of a's rows in b's
+        return off < b_row || off + a_row > a_stride;
+    };
+    const uint64_t out_row = d->outputs * bytes, out_step = d->out_stride * bytes;
+    const bool in_place = d->out == d->base && d->out_stride == d->base_stride;
+    if ((!in_place && meet(d->out, out_step, out_row, d->base, d->base_stride * bytes, out_row)) ||
+        meet(d->out, out_step, out_row, d->x, d->x_stride * x_bytes, d->columns * x_bytes))
+        return context_decline(c, "paged_adapters: out may be base, row by row, and overlaps nothing else");
+    const AdaptersLayout a = adapters_layout(c, d);
+    if (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < a.bytes)
+        return context_decline(c, "paged_adapters: the workspace is missing, too small or not 256-byte aligned");
+    ContextDevice device(c);
+    const cudaStream_t stream = stream_of(c, d->stream);
+    AdapterParams p{};
+    p.x = d->x;
+    p.base = d->base;
+    p.out = d->out;
+    p.a = d->a;
+    p.b = d->b;
+    p.scales = d->scales;
+    p.ids = d->ids;
+    p.starts = d->starts;
+    p.status = d->status ? d->status : context_paged_status(c);
+    p.inner = static_cast<float *>(d->workspace);
+    p.x_stride = d->x_stride;
+    p.base_stride = d->base_stride;
+    p.out_stride = d->out_stride;
+    p.rows = static_cast<int32_t>(d->rows);
+    p.columns = static_cast<int32_t>(d->columns);
+    p.outputs = static_cast<int32_t>(d->outputs);
+    p.requests = static_cast<int32_t>(d->requests);
+    p.adapters = static_cast<int32_t>(d->adapters);
+    p.rank = static_cast<int32_t>(d->rank);
+    p.splits = static_cast<int32_t>(a.splits);
+    p.share = static_cast<int32_t>(a.share);
+    const uint32_t tiles = static_cast<uint32_t>(ceil_div(d->rows, kAdRows));
+    const dim3 inner(tiles, a.splits, static_cast<uint32_t>(ceil_div(d->rank, 16)));
+    if (!(d->x_type == PLAMO_PAGED_FP32
+              ? launch(c, "paged_adapters inner", paged_adapters_inner_kernel<float>, inner, dim3(kAdThreads), 0, stream, false, p)
+              : launch(c, "paged_adapters inner", paged_adapters_inner_kernel<uint16_t>, inner, dim3(kAdThreads), 0, stream, false, p)))
+        return -1;
+    // Outputs' blocks to a CTA: one while that takes four CTAs to an SM at most.
+    const uint64_t blocks = ceil_div(d->outputs, kAdOutputs);
+    const uint64_t per = std::max<uint64_t>(1, tiles * blocks / (4ull * context_sms(c)));
+    const dim3 outer(tiles, static_cast<uint32_t>(ceil_div(blocks, per)));
+    return (d->type == PLAMO_PAGED_FP32 ? launch(c, "paged_adapters outer", paged_adapters_outer_kernel<float>, outer, dim3(kAdThreads), 0,
+                                                 stream, true, p, static_cast<int32_t>(per))
+                                        : launch(c, "paged_adapters outer", paged_adapters_outer_kernel<uint16_t>, outer, dim3(kAdThreads), 0,
+                                                 stream, true, p, static_cast<int32_t>(per)))
+               ? 1
+               : -1;
 }
 
 }  // extern "C"

@@ -65,6 +65,11 @@ struct PagedAttnParams {
     uint32_t *tile_unit;           // [tile_cap + 1] key steps before each tile
     float *tile_sum;               // [slot][tile_pairs][128], [slot][tile_pairs] {m, l}
     float2 *tile_ml;
+    int32_t reach;  // rows that a request's first new row sees before the held rows' end, at most (with a window)
+    // Draft trees: what the new rows see of one another.
+    const uint32_t *masks;  // [rows][words]
+    int32_t words;
+    int32_t share;  // all rows share the prefix's tiles, the requests' own tiles have none of it
 };
 enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlFirst, kTlTaken, kRtRun, kRtLonger, kTlHeader };
 // Requests of up to so many pairs keep their own rows in the row kernel and share
@@ -110,15 +115,16 @@ struct OwnShape {
     int32_t page0, pages;
     int32_t tiles;
 };
+template <bool TREE>
 __device__ __forceinline__ OwnShape own_shape(const PagedAttnParams &p, int32_t r) {
     OwnShape s;
     s.row0 = min(max(p.starts[r], 0), p.rows);
     s.rows = min(max(p.starts[r + 1], s.row0), p.rows) - s.row0;
     s.length = min(max(p.lengths[r], 0), p.max_length);
     s.at0 = s.length - s.rows;
-    const int32_t first = p.window ? max(max(s.at0, 0) - p.window + 1, 0) : 0;
+    const int32_t first = p.window ? max(max(s.at0, 0) - p.reach, 0) : 0;
     s.page0 = first / kPgRows;
-    s.pages = s.rows ? max((s.length + kPgRows - 1) / kPgRows - s.page0, 0) : 0;
+    s.pages = s.rows && !(TREE && s.at0 < 0) ? max((s.length + kPgRows - 1) / kPgRows - s.page0, 0) : 0;
     s.tiles = (s.rows * p.group + kRtPairs - 1) / kRtPairs;
     return s;
 }
@@ -127,8 +133,9 @@ __device__ __forceinline__ OwnShape own_shape(const PagedAttnParams &p, int32_t 
 __device__ __forceinline__ bool request_is_short(const PagedAttnParams &p, const OwnShape &s) {
     return !p.tile_rows || s.rows * p.group <= kTlShortPairs;
 }
+template <bool TREE>
 __device__ __forceinline__ OwnShape short_shape(const PagedAttnParams &p, int32_t r) {
-    OwnShape s = own_shape(p, r);
+    OwnShape s = own_shape<TREE>(p, r);
     if (!request_is_short(p, s)) s.tiles = s.pages = 0;
     return s;
 }
@@ -141,7 +148,8 @@ struct __align__(16) TileShape {
     int32_t pre0, pre1;  // prefix key steps
     int32_t own0, own1;  // own key steps
     int32_t own_limit;   // own keys from here on are seen by none
-    int32_t unused[3];
+    int32_t added;       // trees: the request's new rows (at0: its held rows)
+    int32_t unused[2];
     __device__ int32_t steps() const { return pre1 - pre0 + own1 - own0; }
 };
 
@@ -203,6 +211,71 @@ __device__ __forceinline__ float2 pg_ml(float m, float l) { return make_float2(l
 // sees itself at least: where l is zero all the same, every score is -inf, and
 // the result is none (0 / 0). One that is not held sees nothing: zero.
 __device__ __forceinline__ float pg_inverse(int32_t at, float l) { return at < 0 ? 0.0f : 1.0f / l; }
+// Bits k of the 32 in [lo, hi).
+__device__ __forceinline__ uint32_t tl_bits(int32_t lo, int32_t hi) {
+    const uint32_t below = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1u;
+    return below & (lo <= 0 ? 0xffffffffu : lo >= 32 ? 0u : 0xffffffffu << lo);
+}
+
+// ---- trees -----------------------------------------------------------------------------
+// A row sees, in this order, the prefix, its request's held rows and the new
+// rows of its mask. A window leaves out the first `skip` of them: prefix rows
+// below min(skip, prefix), then held ones, then the mask's lowest bits.
+struct TreeSees {
+    int32_t pre, lo, drop;  // first prefix row, first held row, bits left out
+};
+__device__ __forceinline__ uint32_t tree_word(const PagedAttnParams &p, int32_t row, int32_t added, int32_t w) {
+    return w >= 0 && w < p.words ? p.masks[static_cast<uint64_t>(row) * p.words + w] & tl_bits(0, added - 32 * w) : 0u;
+}
+__device__ __noinline__ int32_t tree_skip(const PagedAttnParams &p, int32_t row, int32_t held, int32_t added) {
+    if (!p.window) return 0;
+    int32_t count = 0;
+#pragma unroll 1
+    for (int32_t w = 0; w < p.words; ++w) count += __popc(tree_word(p, row, added, w));
+    return max(p.prefix + held + count - p.window, 0);
+}
+__device__ __forceinline__ TreeSees tree_sees(const PagedAttnParams &p, int32_t skip, int32_t held) {
+    TreeSees s;
+    s.pre = min(skip, p.prefix);
+    s.lo = min(skip - s.pre, held);
+    s.drop = skip - s.pre - s.lo;
+    return s;
+}
+// The first new row that is left when the mask's `drop` lowest bits are left out.
+__device__ __noinline__ int32_t tree_first(const PagedAttnParams &p, int32_t row, int32_t added, int32_t drop) {
+    if (!drop) return 0;
+#pragma unroll 1
+    for (int32_t w = 0; w < p.words; ++w) {
+        uint32_t m = tree_word(p, row, added, w);
+        const int32_t count = __popc(m);
+        if (drop >= count) {
+            drop -= count;
+            continue;
+        }
+        for (; drop; --drop) m &= m - 1;
+        return 32 * w + __ffs(m) - 1;
+    }
+    return 32 * p.words;
+}
+// Which of the new rows at, at + 1, ... at + 31 a row sees, of those from `first` on. `at` may be negative.
+__device__ __noinline__ uint32_t tree_bits(const PagedAttnParams &p, int32_t row, int32_t added, int32_t first, int32_t at) {
+    const int32_t w = at >> 5;
+    return __funnelshift_r(tree_word(p, row, added, w), tree_word(p, row, added, w + 1), at & 31) & tl_bits(first - at, 32);
+}
+// Whether a row sees nothing at all; its request holds `held` rows (-1: it is not held, then it does not).
+__device__ __noinline__ bool tree_blank(const PagedAttnParams &p, int32_t row, int32_t held, int32_t added) {
+    if (held < 0) return true;
+    if (p.prefix || held) return false;
+    uint32_t any = 0;
+#pragma unroll 1
+    for (int32_t w = 0; w < p.words; ++w) any |= tree_word(p, row, added, w);
+    return !any;
+}
+// As pg_inverse, for a row of a tree.
+__device__ __forceinline__ float tree_inverse(const PagedAttnParams &p, int32_t row, int32_t held, int32_t added, float l) {
+    return l == 0.0f && tree_blank(p, row, held, added) ? 0.0f : 1.0f / l;
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -259,13 +332,20 @@ struct RowCta {
     float2 (*warp_ml)[kRtPairs];  // [warps]
 };
 
-// The keys that a pair of an item sees, [lo, hi); lo -1 where there is no such pair.
-__device__ __noinline__ int2 rt_sees(const PagedAttnParams &p, const RowItem &it, int32_t pair) {
-    if (pair >= it.rows * p.group) return make_int2(-1, 0);
+// The keys that a pair of an item sees, [x, y); x -1 where there is no such pair.
+// Trees: and of the new rows, those of batch row z's mask from bit w on (z -1: none).
+template <bool TREE>
+__device__ __noinline__ int4 rt_sees(const PagedAttnParams &p, const RowItem &it, int32_t pair) {
+    if (pair >= it.rows * p.group) return make_int4(-1, 0, -1, 0);
     const int32_t i = p.by_group.div(pair);
     if (it.request >= 0) {
+        if constexpr (TREE) {
+            const int32_t row = it.row0 + i;
+            const TreeSees s = tree_sees(p, tree_skip(p, row, it.at0, it.rows), it.at0);
+            return make_int4(s.lo, it.at0, row, tree_first(p, row, it.rows, s.drop));
+        }
         const int32_t at = it.at0 + i;
-        return make_int2(p.window ? max(max(at, 0) - p.window + 1, 0) : 0, max(at + 1, 0));
+        return make_int4(p.window ? max(max(at, 0) - p.window + 1, 0) : 0, max(at + 1, 0), -1, 0);
     }
     int32_t lo = 0;
     if (p.window && p.requests) {  // its request's length decides: the last one to start at or before row i
@@ -276,10 +356,11 @@ __device__ __noinline__ int2 rt_sees(const PagedAttnParams &p, const RowItem &it
             r = below ? r + half : r;
             n = below ? n - half : half;
         }
-        const OwnShape s = own_shape(p, r);
-        lo = min(max(p.prefix + max(s.at0 + i - s.row0, 0) - p.window + 1, 0), p.prefix);
+        const OwnShape s = own_shape<TREE>(p, r);
+        if constexpr (TREE) lo = tree_sees(p, tree_skip(p, i, max(s.at0, 0), s.rows), max(s.at0, 0)).pre;
+        else lo = min(max(p.prefix + max(s.at0 + i - s.row0, 0) - p.window + 1, 0), p.prefix);
     }
-    return make_int2(lo, p.prefix);
+    return make_int4(lo, p.prefix, -1, 0);
 }
 // Where a pair's query starts (in elements), or -1.
 __device__ __forceinline__ int64_t rt_query(const PagedAttnParams &p, const RowItem &it, int32_t pair) {
@@ -288,18 +369,23 @@ __device__ __forceinline__ int64_t rt_query(const PagedAttnParams &p, const RowI
     return static_cast<int64_t>(it.row0 + i) * static_cast<int64_t>(p.q_stride) + (it.head * p.group + pair - i * p.group) * kPgDim;
 }
 
+template <bool TREE>
 __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const RowItem &it, const RowCta &cta, int32_t begin, int32_t end,
                                              int32_t slabs, uint32_t ring, bool &dead) {
     constexpr int SLAB = rt_slab_bytes<false>(), SLABS = kRtRing / SLAB;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int32_t pair0 = it.tile * kRtPairs;
     // This thread's pairs, 2 t + c: which keys they see.
-    int32_t see_lo[2], see_hi[2];
+    int32_t see_lo[2], see_hi[2], tree_row[2], tree_from[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const int2 sees = rt_sees(p, it, pair0 + 2 * t + c);
+        const int4 sees = rt_sees<TREE>(p, it, pair0 + 2 * t + c);
         see_lo[c] = sees.x;
         see_hi[c] = sees.y;
+        if constexpr (TREE) {
+            tree_row[c] = sees.z;
+            tree_from[c] = sees.w;
+        }
     }
     // Queries as MMA operands.
     uint32_t qf[kPgDim / 16][2];
@@ -341,10 +427,21 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
         // ---- masks; a key that exists and that some pair does not see?
         const int32_t left = min(end - key0, kRtKeys);
         bool hidden = false, move = false;
+        uint32_t drafts[2] = {0, 0};  // keys of the slab that are new rows and seen
+        if constexpr (TREE) {
+            if (it.request >= 0 && key0 + kRtKeys > it.at0) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (tree_row[c] >= 0) drafts[c] = tree_bits(p, tree_row[c], it.rows, tree_from[c], key0 - it.at0);
+            }
+        }
+        const auto sees = [&](int c, int key) {
+            return (key0 + key >= see_lo[c] && key0 + key < see_hi[c]) || (TREE && ((drafts[c] >> key) & 1u));
+        };
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int c = x & 1, key = g + 8 * (x >> 1);
-            const bool seen = key0 + key >= see_lo[c] && key0 + key < see_hi[c] && key < left;
+            const bool seen = sees(c, key) && key < left;
             hidden |= !seen && key < left && see_lo[c] >= 0;
             s[x] = seen ? (s[x] + c1[x]) * p.scale2 : -INFINITY;
             move |= s[x] > mx[c] + kLazy;
@@ -419,7 +516,7 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
                     const int src = (key & 7) * 4 + t;
                     const float a = __shfl_sync(0xffffffffu, s[c], src), b = __shfl_sync(0xffffffffu, s[2 + c], src);
                     w[c] = key < 8 ? a : b;
-                    seen[c] = key0 + key >= see_lo[c] && key0 + key < see_hi[c];
+                    seen[c] = sees(c, key);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -479,12 +576,13 @@ __device__ __forceinline__ void rt_item_bf16(const PagedAttnParams &p, const Row
 // the numbers and sends the other; with key and pair of a register chosen by
 // the lane's own number (key ^ l / 8, pair ^ l % 8) it is always the same half
 // of the registers, and nothing is selected.
+template <bool TREE>
 __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowItem &it, const RowCta &cta, float *weights,
                                             int32_t begin, int32_t end, int32_t slabs, uint32_t ring, bool &dead) {
     constexpr int SLAB = rt_slab_bytes<true>(), SLABS = kRtRing / SLAB;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int32_t pair0 = it.tile * 8;
-    const int2 sees = rt_sees(p, it, pair0 + (lane & 7));
+    const int4 sees = rt_sees<TREE>(p, it, pair0 + (lane & 7));
     float4 q[8], o[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -533,10 +631,14 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
         const int32_t left = min(end - key0, kRtKeys);
         bool hidden = false, move = false;
         uint32_t seen_by[4];  // bit 8 * key + pair of four keys
+        uint32_t drafts = 0;  // keys of the slab that are new rows and seen
+        if constexpr (TREE) {
+            if (it.request >= 0 && key0 + kRtKeys > it.at0 && sees.z >= 0) drafts = tree_bits(p, sees.z, it.rows, sees.w, key0 - it.at0);
+        }
 #pragma unroll
         for (int four = 0; four < 4; ++four) {
             const int key = 4 * four + (lane >> 3);
-            const bool seen = key0 + key >= sees.x && key0 + key < sees.y && key < left;
+            const bool seen = ((key0 + key >= sees.x && key0 + key < sees.y) || (TREE && ((drafts >> key) & 1u))) && key < left;
             hidden |= !seen && sees.x >= 0;
             seen_by[four] = __ballot_sync(0xffffffffu, seen);
             s[four] = seen ? s[four] * p.scale2 : -INFINITY;
@@ -638,12 +740,14 @@ __device__ __forceinline__ void rt_item_f32(const PagedAttnParams &p, const RowI
 // TB/s); on short items their ends, about 4 us each (256 requests of 500 rows
 // and eight KV heads: 133 us, 4.0 TB/s). The FP32 kernel spills (48 bytes
 // stored, 112 loaded) at the 128 registers that two CTAs to an SM leave a thread.
+template <bool TREE>
 __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums);  // paged_tiles.cuh
 
 // Request r's work, or the prefix's (r == requests) from page pp0 on.
+template <bool TREE>
 __device__ __forceinline__ OwnShape row_work(const PagedAttnParams &p, int32_t r, int32_t pp0) {
     if (r < p.requests) {
-        OwnShape s = short_shape(p, r);
+        OwnShape s = short_shape<TREE>(p, r);
         if (!s.pages) s.tiles = 0;
         return s;
     }
@@ -656,7 +760,7 @@ __device__ __forceinline__ OwnShape row_work(const PagedAttnParams &p, int32_t r
     return s;
 }
 
-template <bool F32>
+template <bool F32, bool TREE>
 __global__ void __launch_bounds__(kRtThreads, 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
     constexpr int SLAB = rt_slab_bytes<F32>(), SLABS = kRtRing / SLAB;
@@ -675,7 +779,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_launch_dependents();
     if (blockIdx.x == 0) {  // for the kernels that follow, while the others work
-        paged_schedule(p, scan);
+        paged_schedule<TREE>(p, scan);
         return;
     }
     const int32_t worker = static_cast<int32_t>(blockIdx.x) - 1;
@@ -702,18 +806,18 @@ __global__ void __launch_bounds__(kRtThreads, 2)
         __syncthreads();
         int32_t lowest = INT32_MAX;
         for (int32_t r = r0; r < min(r1, p.requests); ++r) {
-            const OwnShape s = own_shape(p, r);
+            const OwnShape s = own_shape<TREE>(p, r);
             if (s.rows) lowest = min(lowest, max(s.at0, 0));
         }
         lowest = __reduce_min_sync(0xffffffffu, lowest);
         if (lane == 0) atomicMin(&lowest_at, lowest);
         __syncthreads();
-        if (lowest_at != INT32_MAX) pp0 = min(max(p.prefix + lowest_at - p.window + 1, 0), p.prefix) / kPgRows;
+        if (lowest_at != INT32_MAX) pp0 = min(max(p.prefix + lowest_at - p.reach, 0), p.prefix) / kPgRows;
     }
     int64_t units = 0, strips = 0, all_units, all_strips;
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
-        const OwnShape s = row_work(p, r, pp0);
+        const OwnShape s = row_work<TREE>(p, r, pp0);
         strips += s.tiles * p.kh;
         units += static_cast<int64_t>(s.tiles) * s.pages * p.kh;
     }
@@ -733,7 +837,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
         int32_t unit = static_cast<int32_t>(unit0), strip = strip0;
 #pragma unroll 1
         for (int32_t r = r0; r < r1; ++r) {
-            const OwnShape s = row_work(p, r, pp0);
+            const OwnShape s = row_work<TREE>(p, r, pp0);
             f(s, r, unit, strip);
             strip += s.tiles * p.kh;
             unit += s.tiles * s.pages * p.kh;
@@ -774,7 +878,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                 it.page0 = s.page0 + lo;
                 it.pages = hi - lo;
                 // Keys past the tile's last row are seen by none of its rows.
-                const int32_t last = s.at0 + min(s.rows - 1, p.by_group.div(it.tile * kRtPairs + kRtPairs - 1));
+                const int32_t last = TREE ? s.length - 1 : s.at0 + min(s.rows - 1, p.by_group.div(it.tile * kRtPairs + kRtPairs - 1));
                 it.limit = r < p.requests ? min(max(last + 1, 0), s.length) : p.prefix;
                 it.row0 = s.row0;
                 it.rows = s.rows;
@@ -828,8 +932,8 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                 continue;
             }
             // ---- the computing warps
-            if constexpr (F32) rt_item_f32(p, it, cta, weights[warp], begin, end, slabs, ring, dead);
-            else rt_item_bf16(p, it, cta, begin, end, slabs, ring, dead);
+            if constexpr (F32) rt_item_f32<TREE>(p, it, cta, weights[warp], begin, end, slabs, ring, dead);
+            else rt_item_bf16<TREE>(p, it, cta, begin, end, slabs, ring, dead);
             ring += slabs;
             // ---- result, or the tile's partial sums
 #pragma unroll 1
@@ -850,7 +954,7 @@ __global__ void __launch_bounds__(kRtThreads, 2)
                     const int32_t m = it.tile * kRtPairs + pair;
                     if (m >= it.rows * p.group) continue;
                     const int32_t i = p.by_group.div(m);
-                    const float inv = pg_inverse(it.at0 + i, l);
+                    const float inv = TREE ? tree_inverse(p, it.row0 + i, it.at0, it.rows, l) : pg_inverse(it.at0 + i, l);
                     v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                     const uint64_t at = (it.row0 + i) * p.out_stride + (it.head * p.group + m - i * p.group) * kPgDim + d;
                     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + at, v);
@@ -941,9 +1045,12 @@ __device__ __forceinline__ void join_parts(const PartList &a, const PartList &b,
 #pragma unroll
     for (int k = RES; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
 }
+// The new rows of a listed row's request (trees).
+__device__ __forceinline__ int32_t listed_added(const PagedAttnParams &p, const int4 &e) {
+    return e.z < 0 ? p.tile_shape[-1 - e.z].added : own_shape<true>(p, e.z).rows;
+}
 template <bool F32>
-__device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row, int32_t at, int32_t head, float4 o, float l) {
-    const float inv = pg_inverse(at, l);
+__device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row, float inv, int32_t head, float4 o) {
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     const uint64_t to = row * p.out_stride + head * kPgDim + 4 * (threadIdx.x & 31);
     if constexpr (F32) pg_store4(static_cast<float *>(p.out) + to, o);
@@ -954,7 +1061,7 @@ __device__ __forceinline__ void join_store(const PagedAttnParams &p, int32_t row
 // shared (a warp to RES pairs), and zeroes the rows that see nothing. FEW: a
 // block to RES results, its warps sharing their parts; else a warp to RES.
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
-template <bool F32, int RES, bool FEW>
+template <bool F32, int RES, bool FEW, bool TREE>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
     __shared__ float4 warp_sums[FEW ? kJoinWarps : 1][RES][32];
     __shared__ float2 warp_ml[FEW ? kJoinWarps : 1][RES];
@@ -984,21 +1091,33 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                 return PartList{p.row_sum, p.row_ml, c0 + rec.z + strip, 1, kRtPairs, m % kRtPairs,
                                 rec.y ? of_rows.cta_of(u0 + rec.y - 1) - c0 + 1 : 0};
             };
-            own = row_parts(e.z, e.w * p.group + in_group);
-            written = own.count == 1 && p.prefix == 0;  // where it was computed
+            // The parts of place `at` of a tile for this head, where all of them are kept.
+            const auto tile_parts = [&](int32_t tile, int32_t at) {
+                const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
+                const int32_t u0 = unit * p.kh + kv * steps, c0 = runs.cta_of(u0);
+                return PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, p.tile_pairs,
+                                at * p.group + in_group, steps ? runs.cta_of(u0 + steps - 1) - c0 + 1 : 0};
+            };
+            if (TREE && e.z < 0) {
+                own = tile_parts(-1 - e.z, e.w);
+            } else {
+                own = row_parts(e.z, e.w * p.group + in_group);
+                written = own.count == 1 && p.prefix == 0;  // where it was computed
+            }
             if (p.prefix_tiles) {
                 shared = row_parts(p.requests, e.x * p.group + in_group);
             } else if (pre_tiles && ctas) {
                 const int32_t tile = p.by_tile_rows.div(listed);
-                const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
-                const int32_t u0 = unit * p.kh + kv * steps, c0 = runs.cta_of(u0);
-                shared = PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, p.tile_pairs,
-                                  (listed - tile * p.tile_rows) * p.group + in_group, steps ? runs.cta_of(u0 + steps - 1) - c0 + 1 : 0};
+                shared = tile_parts(tile, listed - tile * p.tile_rows);
             }
         }
         const uint32_t skip = __ballot_sync(0xffffffffu, written || head >= p.qh);  // (the same in all warps of an item)
         if (skip == 0xffffffffu) continue;
         join_parts<RES>(shared, own, FEW ? warp : 0, FEW ? kJoinWarps : 1, o, l, top);
+        const auto inverse = [&](float sum) {
+            if constexpr (!TREE) return pg_inverse(e.y, sum);
+            return sum == 0.0f && (e.y < 0 || tree_blank(p, e.x, e.y, listed_added(p, e))) ? 0.0f : 1.0f / sum;
+        };
         if constexpr (FEW) {
 #pragma unroll
             for (int i = 0; i < RES; ++i) warp_sums[warp][i][lane] = o[i];
@@ -1018,21 +1137,22 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
                     if (f != 0.0f) v = make_float4(fmaf(f, u.x, v.x), fmaf(f, u.y, v.y), fmaf(f, u.z, v.z), fmaf(f, u.w, v.w));
                     l = fmaf(f, ml.y, l);
                 }
-                join_store<F32>(p, e.x, e.y, head0 + warp, v, l);
+                join_store<F32>(p, e.x, inverse(l), head0 + warp, v);
             }
             __syncthreads();
         } else {
 #pragma unroll
             for (int i = 0; i < RES; ++i) {
                 const float li = __shfl_sync(0xffffffffu, l, i);
-                if (!((skip >> i) & 1u)) join_store<F32>(p, e.x, e.y, head0 + i, o[i], li);
+                if (!((skip >> i) & 1u)) join_store<F32>(p, e.x, inverse(li), head0 + i, o[i]);
             }
         }
     }
     // Prompts' tiles that a CTA's end cuts: the first such end does the tile.
     const int32_t blocks = p.tile_pairs / (RES * kJoinWarps);  // to a tile
+    const bool listed_all = TREE && p.share;  // every row was in the list
 #pragma unroll 1
-    for (int32_t n = blockIdx.x; n < blocks * (ctas - 1); n += gridDim.x) {
+    for (int32_t n = blockIdx.x; !listed_all && n < blocks * (ctas - 1); n += gridDim.x) {
         const int32_t c = n / blocks + 1, pair0 = ((n - (c - 1) * blocks) * kJoinWarps + warp) * RES, cut = runs.start(c);
         const int32_t tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles), p.by_kh.div(cut));
         if (tile < pre_tiles) continue;
@@ -1050,7 +1170,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
             const float li = __shfl_sync(0xffffffffu, l, i);
             if (pair0 + i >= pairs) break;
             const int32_t row = p.by_group.div(pair0 + i);
-            join_store<F32>(p, row0 + row, p.tile_shape[tile].at0 + row, kv * p.group + pair0 + i - row * p.group, o[i], li);
+            const float inv = TREE ? tree_inverse(p, row0 + row, p.tile_shape[tile].at0, p.tile_shape[tile].added, li)
+                                   : pg_inverse(p.tile_shape[tile].at0 + row, li);
+            join_store<F32>(p, row0 + row, inv, kv * p.group + pair0 + i - row * p.group, o[i]);
         }
     }
     // Rows that no request has, and tiles without a key.
@@ -1065,7 +1187,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 #pragma unroll 1
     for (int32_t row = end_row + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
 #pragma unroll 1
-    for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); tile < tiles; tile += gridDim.x)
+    for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); !listed_all && tile < tiles; tile += gridDim.x)
         if (p.tile_unit[tile + 1] == p.tile_unit[tile])
             for (int32_t i = 0; i < p.tile_shape[tile].rows; ++i) clear(p.tile_shape[tile].row0 + i);
 }

@@ -35,12 +35,24 @@ constexpr int kTlQBytes = kTlPairs * kPgDim * 2;
 constexpr int kTlSmem = 1024 + kTlQBytes + kTlUnits * kTlUnitBytes;
 
 // Tile t of a prompt (its rows [t * tile_rows, ...)).
+template <bool TREE>
 __device__ __forceinline__ TileShape prompt_tile(const PagedAttnParams &p, int32_t request, const OwnShape &o, int32_t t) {
     TileShape s{};
     const int32_t first = t * p.tile_rows;
     s.request = request;
     s.row0 = o.row0 + first;
     s.rows = min(p.tile_rows, o.rows - first);
+    if constexpr (TREE) {  // any new row may be seen
+        s.at0 = o.at0;
+        s.added = o.rows;
+        if (o.at0 < 0) return s;
+        s.pre1 = p.share ? 0 : (p.prefix + p.tile_keys - 1) / p.tile_keys;
+        s.pre0 = p.window ? min(max(p.prefix + s.at0 - p.reach, 0) / p.tile_keys, s.pre1) : 0;
+        s.own_limit = o.length;
+        s.own1 = (s.own_limit + p.tile_keys - 1) / p.tile_keys;
+        s.own0 = p.window ? min(max(s.at0 - p.reach, 0) / p.tile_keys, s.own1) : 0;
+        return s;
+    }
     s.at0 = o.at0 + first;
     const int32_t last = s.at0 + s.rows - 1;
     if (last < 0) return s;  // rows before own row 0 see nothing
@@ -59,6 +71,9 @@ __device__ __forceinline__ TileShape prompt_tile(const PagedAttnParams &p, int32
 // and prompts (tiles of their own over prefix and own rows), and numbers the
 // key steps of all tiles. A step of a tile and KV head is the unit of work: the
 // tile kernel's CTAs take equal runs of consecutive ones.
+// Trees that share the prefix's tiles: all rows are listed, and a request that is
+// not short has tiles of its own over its own rows only.
+template <bool TREE>
 __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     __shared__ int32_t first_at;
     const int tid = threadIdx.x;
@@ -73,17 +88,18 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     int32_t lowest = INT32_MAX;
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
-        const OwnShape s = own_shape(p, r);
+        const OwnShape s = own_shape<TREE>(p, r);
         if (p.lengths[r] > p.max_length) pg_flag(p.status, PLAMO_PAGED_TABLE);
         if (p.lengths[r] < 0) pg_flag(p.status, PLAMO_PAGED_COUNT);
         if (p.starts[r] < 0 || p.starts[r + 1] > p.rows) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
         decreases |= p.starts[r + 1] < p.starts[r];
-        if (request_is_short(p, s)) {
+        if (TREE && s.rows > 32 * p.words) pg_flag(p.status, PLAMO_PAGED_TREE);
+        const bool is_short = request_is_short(p, s);
+        if (is_short || (TREE && p.share)) {
             short_rows += s.rows;
             if (s.rows) lowest = min(lowest, max(s.at0, 0));
-        } else {
-            prompt_tiles += p.by_tile_rows.div(s.rows + p.tile_rows - 1);
         }
+        if (!is_short) prompt_tiles += p.by_tile_rows.div(s.rows + p.tile_rows - 1);
     }
     lowest = __reduce_min_sync(0xffffffffu, lowest);
     if ((tid & 31) == 0) atomicMin(&first_at, lowest);
@@ -97,20 +113,30 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         pre_tiles = p.by_tile_rows.div(all_short + p.tile_rows - 1);
         pre.request = -1;
         pre.pre1 = (p.prefix + p.tile_keys - 1) / p.tile_keys;
-        if (p.window && first_at != INT32_MAX) pre.pre0 = min(max(p.prefix + first_at - p.window + 1, 0) / p.tile_keys, pre.pre1);
+        if (p.window && first_at != INT32_MAX) pre.pre0 = min(max(p.prefix + first_at - p.reach, 0) / p.tile_keys, pre.pre1);
     }
     bool fits = ordered && pre_tiles + all_tiles <= p.tile_cap;  // (no tile kernel: 0 <= 0)
     if (!fits) pre_tiles = all_tiles = 0;
     const int32_t all = pre_tiles + static_cast<int32_t>(all_tiles);
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
-        const OwnShape s = own_shape(p, r);
-        if (request_is_short(p, s)) {
+        const OwnShape s = own_shape<TREE>(p, r);
+        const bool is_short = request_is_short(p, s);
+        if (is_short || (TREE && p.share)) {
+            const int32_t first_tile = pre_tiles + static_cast<int32_t>(tile_at);
 #pragma unroll 1
-            for (int32_t i = 0; i < s.rows && short_at + i < all_short; ++i)
-                p.short_list[short_at + i] = make_int4(s.row0 + i, max(s.at0 + i, -1), r, i);
+            for (int32_t i = 0; i < s.rows && short_at + i < all_short; ++i) {
+                int4 e = make_int4(s.row0 + i, TREE ? max(s.at0, -1) : max(s.at0 + i, -1), r, i);
+                if (TREE && !is_short) {
+                    const int32_t t = p.by_tile_rows.div(i);
+                    e.z = -1 - (first_tile + t);
+                    e.w = i - t * p.tile_rows;
+                }
+                p.short_list[short_at + i] = e;
+            }
             short_at += s.rows;
-        } else if (fits) {
+        }
+        if (!is_short && fits) {
             const int32_t n = p.by_tile_rows.div(s.rows + p.tile_rows - 1);
 #pragma unroll 1
             for (int32_t t = 0; t < n; ++t, ++tile_at) {  // whose it is; the rest below, by all threads
@@ -131,7 +157,7 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
             shape.rows = min(p.tile_rows, all_short - shape.row0);
         } else if (t < all) {
             const int32_t r = p.tile_shape[t].request;
-            shape = prompt_tile(p, r, own_shape(p, r), p.tile_shape[t].row0);
+            shape = prompt_tile<TREE>(p, r, own_shape<TREE>(p, r), p.tile_shape[t].row0);
         }
         int64_t sum;
         const int64_t at = total + pg_block_scan<kRtThreads>(shape.steps(), sums, &sum);
@@ -182,21 +208,20 @@ __device__ __forceinline__ bool tl_wait(uint64_t *bar, uint32_t parity, volatile
 }
 // Whether the values of a step are looked over before use: keys past the end,
 // or keys that exist and some row of the tile does not see.
+template <bool TREE>
 __device__ __forceinline__ bool step_is_mended(const PagedAttnParams &p, const TileShape &s, int32_t step, bool *masked) {
     const bool own = step >= s.pre1 - s.pre0;
     const int32_t key0 = (own ? s.own0 + step - (s.pre1 - s.pre0) : s.pre0 + step) * p.tile_keys;
     const int32_t limit = own ? s.own_limit : p.prefix;
     bool m = s.request >= 0 && s.at0 < 0;
-    if (own) m |= s.at0 + 1 < min(key0 + p.tile_keys, limit) || (p.window && max(s.at0 + s.rows, 0) - p.window > key0);
+    if constexpr (TREE) {
+        const int32_t skipped = s.at0 + min(s.added, 32 * p.words) - p.window;  // held rows that some row does not see
+        if (own) m |= key0 + p.tile_keys > s.at0 || (p.window && skipped > key0);
+        else if (p.window) m |= s.request < 0 || p.prefix + skipped > key0;
+    } else if (own) m |= s.at0 + 1 < min(key0 + p.tile_keys, limit) || (p.window && max(s.at0 + s.rows, 0) - p.window > key0);
     else if (p.window) m |= s.request < 0 || p.prefix + max(s.at0 + s.rows, 0) - p.window > key0;
     *masked = m;
     return m || key0 + p.tile_keys > limit;
-}
-
-// Bits k of the 32 in [lo, hi).
-__device__ __forceinline__ uint32_t tl_bits(int32_t lo, int32_t hi) {
-    const uint32_t below = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1u;
-    return below & (lo <= 0 ? 0xffffffffu : lo >= 32 ? 0u : 0xffffffffu << lo);
 }
 
 // Piece c (16 bytes) of row r of a warp's 32 rows of 256 bytes, laid out as an
@@ -227,19 +252,23 @@ __device__ __noinline__ bool walk_next(const PagedAttnParams &p, TileWalk &w) {
 
 // Values that are not finite left the products of steps with masked keys: the
 // rows that see them get them here (a weight times one of them is itself).
-__device__ __noinline__ void add_odd_values(const PagedAttnParams &p, const TileShape &s, const TileWalk &w, int32_t at, int c, float (&o)[32]) {
+template <bool TREE>
+__device__ __noinline__ void add_odd_values(const PagedAttnParams &p, const TileShape &s, const TileWalk &w, int32_t row, int32_t at,
+                                            const TreeSees &sees, int c, float (&o)[32]) {
     const int32_t pre_steps = s.pre1 - s.pre0;
     for (int32_t n = 0; n < w.steps; ++n) {
         const int32_t step = w.step + n;
         bool masked;
-        step_is_mended(p, s, step, &masked);
+        step_is_mended<TREE>(p, s, step, &masked);
         if (!masked) continue;
         const bool own = step >= pre_steps;
         const int32_t key0 = (own ? s.own0 + step - pre_steps : s.pre0 + step) * kTlKeys;
-        const int32_t hi = at < 0 ? 0 : min(key0 + kTlKeys, own ? min(at + 1, s.own_limit) : p.prefix);
-        const int32_t lo = p.window ? max(key0, (own ? at : p.prefix + at) - p.window + 1) : key0;
+        const int32_t hi = at < 0 ? 0 : min(key0 + kTlKeys, own ? (TREE ? s.own_limit : min(at + 1, s.own_limit)) : p.prefix);
+        const int32_t lo = TREE ? max(key0, own ? sees.lo : sees.pre) : p.window ? max(key0, (own ? at : p.prefix + at) - p.window + 1) : key0;
+        const int32_t from = TREE && own ? tree_first(p, row, s.added, sees.drop) : 0;
 #pragma unroll 1
         for (int32_t key = lo; key < hi; ++key) {
+            if (TREE && own && key >= at && !(tree_bits(p, row, s.added, from, key - at) & 1u)) continue;
             const int32_t id = own ? p.tables[static_cast<uint64_t>(s.request) * p.table_stride + key / kPgRows] : p.prefix_pages[key / kPgRows];
             if (id < 0 || id >= p.pages) continue;
             const uint16_t *v = static_cast<const uint16_t *>(p.pool) + ((static_cast<uint64_t>(id) * 2 + 1) * kPgRows + key % kPgRows) * p.kh * kPgDim +
@@ -253,6 +282,7 @@ __device__ __noinline__ void add_odd_values(const PagedAttnParams &p, const Tile
     }
 }
 
+template <bool TREE>
 __global__ void __launch_bounds__(kTlThreads, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(128) unsigned char tl_smem[];
@@ -399,7 +429,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     const bool more = n + 1 < w.steps;
                     bool masked;
                     ok = tl_wait(&full[vs], (v / kTlUnits) & 1u, quit);
-                    if (ok && step_is_mended(p, s, w.step + n, &masked)) {
+                    if (ok && step_is_mended<TREE>(p, s, w.step + n, &masked)) {
                         ok = tl_wait(&mended[vs], (mends >> vs) & 1u, quit);
                         mends ^= 1u << vs;
                     }
@@ -443,7 +473,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     bool masked;
-                    if (kind && step_is_mended(p, s, w.step + n, &masked)) {
+                    if (kind && step_is_mended<TREE>(p, s, w.step + n, &masked)) {
                         const int32_t step = w.step + n;
                         const bool own = step >= pre_steps;
                         const int32_t key0 = (own ? s.own0 + step - pre_steps : s.pre0 + step) * kTlKeys;
@@ -496,11 +526,20 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             const int32_t pairs = s.rows * p.group, pre_steps = s.pre1 - s.pre0;
             const bool active = i == 0 || pairs > 128, there = pair < pairs;
             const int32_t local = p.by_group.div(pair);
-            int32_t row = s.row0 + local, at = s.at0 + local;
+            int32_t row = s.row0 + local, at = TREE ? s.at0 : s.at0 + local, added = s.added;  // trees: `at` is the held rows
             if (s.request < 0 && there) {
                 const int4 e = p.short_list[row];
                 row = e.x;
                 at = e.y;
+                if (TREE && p.window) added = listed_added(p, e);
+            }
+            TreeSees sees{0, 0, 0};
+            int32_t from = 0;  // bits of the mask below it are outside the window
+            if constexpr (TREE) {
+                if (there && at >= 0 && p.window) {
+                    sees = tree_sees(p, tree_skip(p, row, at, added), at);
+                    from = tree_first(p, row, added, sees.drop);
+                }
             }
             const int32_t head = w.head * p.group + pair - local * p.group;
             if (!active) continue;
@@ -527,9 +566,9 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 
             const float scale2 = fabsf(p.scale2);
             // Keys this row sees, prefix and own: [lo, hi).
-            const int32_t pre_hi = at < 0 ? 0 : p.prefix, own_hi = at < 0 ? 0 : min(at + 1, s.own_limit);
-            const int32_t pre_lo = p.window ? max(p.prefix + max(at, 0) - p.window + 1, 0) : 0;
-            const int32_t own_lo = p.window ? max(max(at, 0) - p.window + 1, 0) : 0;
+            const int32_t pre_hi = at < 0 ? 0 : p.prefix, own_hi = at < 0 ? 0 : TREE ? at : min(at + 1, s.own_limit);
+            const int32_t pre_lo = TREE ? sees.pre : p.window ? max(p.prefix + max(at, 0) - p.window + 1, 0) : 0;
+            const int32_t own_lo = TREE ? sees.lo : p.window ? max(max(at, 0) - p.window + 1, 0) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int32_t n = 0; n < w.steps; ++n) {
                 ok = tl_wait(&s_full[i], n_scores & 1u, quit);
@@ -544,6 +583,13 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 const int32_t hi = min(max((own ? own_hi : pre_hi) - key0, 0), kTlKeys);
                 const int32_t lo = min(max((own ? own_lo : pre_lo) - key0, 0), kTlKeys);
                 const bool partial = __any_sync(0xffffffffu, there && (lo > 0 || hi < kTlKeys));
+                uint32_t drafts[4] = {0, 0, 0, 0};  // new rows among the keys that this row sees
+                if constexpr (TREE) {
+                    if (own && key0 + kTlKeys > s.at0 && there) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) drafts[k] = tree_bits(p, row, s.added, from, key0 + 32 * k - at);
+                    }
+                }
                 // 64 scores at a time, twice: for the maximum, then for the weights, which replace them
                 // (two BF16 terms). Loops, not straight code: a segment is a few steps long, and
                 // code that runs a few times costs its fetching.
@@ -553,7 +599,11 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     tmem_ld32_async(scol + 64 * half + 32, reinterpret_cast<uint32_t(&)[32]>(x[32]));
                     tmem_wait_ld();
                     if (partial) {
-                        const uint32_t see0 = tl_bits(lo - 64 * half, hi - 64 * half), see1 = tl_bits(lo - 64 * half - 32, hi - 64 * half - 32);
+                        uint32_t see0 = tl_bits(lo - 64 * half, hi - 64 * half), see1 = tl_bits(lo - 64 * half - 32, hi - 64 * half - 32);
+                        if constexpr (TREE) {
+                            see0 |= half ? drafts[2] : drafts[0];
+                            see1 |= half ? drafts[3] : drafts[1];
+                        }
 #pragma unroll
                         for (int k = 0; k < 64; ++k)
                             if (!((k < 32 ? see0 : see1) >> (k & 31) & 1u)) x[k] = 0xff800000u;  // -inf
@@ -625,10 +675,11 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles;
-            const int32_t slot = w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
+            const bool parts = w.tile < pre_tiles || (TREE && p.share);  // all segments are kept, to be joined with others
+            const bool whole = w.steps == w.tile_steps && !parts;
+            const int32_t slot = parts ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
             const bool odd = *reinterpret_cast<volatile int *>(&odd_values);
-            const float inv = pg_inverse(at, l);
+            const float inv = !TREE ? pg_inverse(at, l) : whole && there ? tree_inverse(p, row, at, s.added, l) : 1.0f;
             // Through shared memory (the queries' place: the scores are done with them), so that rows
             // leave 256 bytes at a time: the whole result, or half of the partial sums.
             const int64_t to = !there ? -1 : whole ? row * static_cast<int64_t>(p.out_stride) + head * kPgDim
@@ -645,7 +696,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     float more[32];
 #pragma unroll
                     for (int k = 0; k < 32; ++k) more[k] = o[k];
-                    add_odd_values(p, s, w, at, c, more);
+                    add_odd_values<TREE>(p, s, w, row, at, sees, c, more);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = more[k];
                 }
@@ -703,7 +754,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 constexpr int kTfPairs = 64, kTfKeys = 64, kTfThreads = 128;
 constexpr int kTfTile = kTfKeys * kPgDim * 4;  // keys, values or queries
 constexpr int kTfTables = 3 * kTfTile + kTfPairs * kTfKeys * 4;  // barriers and the pairs' rows behind the tiles
-constexpr int kTfSmem = kTfTables + 16 + 2 * kTfPairs * 4;       // no static part: two CTAs just fit an SM
+constexpr int kTfSmem = kTfTables + 16 + 3 * kTfPairs * 4;       // no static part: two CTAs just fit an SM
 
 // A 16-byte piece of row r: the copy engine's swizzle; the queries' rows r and
 // r + 8, read together, lie apart too; the weights' keys are rows.
@@ -723,13 +774,15 @@ __device__ __forceinline__ float4 lds_f32x4(uint32_t addr) {
     return v;
 }
 
+template <bool TREE>
 __global__ void __launch_bounds__(kTfThreads, 2)
     paged_tile_f32_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(1024) unsigned char tf_smem[];
     unsigned char *const base = tf_smem;
     uint64_t *const full = reinterpret_cast<uint64_t *>(base + kTfTables);           // keys, values
     int32_t *const pair_row = reinterpret_cast<int32_t *>(base + kTfTables + 16);    // batch row, -1: no such pair
-    int32_t *const pair_at = pair_row + kTfPairs;                                    // own row
+    int32_t *const pair_at = pair_row + kTfPairs;                                    // own row; trees: held rows
+    int32_t *const pair_skip = pair_at + kTfPairs;                                   // trees: rows outside the window
     if (smem_u32(base) & 1023u) {  // the copies' swizzle needs it; dynamic shared memory starts so when there is no other
         pg_flag(p.status, PLAMO_PAGED_FAILED);
         return;
@@ -779,22 +832,27 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             copy(0, 0);
             copy(0, 1);
         }
-        const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles;
-        const int32_t slot = w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
+        const bool parts = w.tile < pre_tiles || (TREE && p.share);  // all segments are kept, to be joined with others
+        const bool whole = w.steps == w.tile_steps && !parts;
+        const int32_t slot = parts ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
         if (tid < kTfPairs) {
-            int32_t row = -1, at = 0;
+            int32_t row = -1, at = 0, skip = 0;
             if (tid < pairs) {
                 const int32_t local = p.by_group.div(tid);
+                int32_t added = s.added;
                 row = s.row0 + local;
-                at = s.at0 + local;
+                at = TREE ? s.at0 : s.at0 + local;
                 if (s.request < 0) {
                     const int4 e = p.short_list[row];
                     row = e.x;
                     at = e.y;
+                    if (TREE && p.window) added = listed_added(p, e);
                 }
+                if (TREE && at >= 0) skip = tree_skip(p, row, at, added);
             }
             pair_row[tid] = row;
             pair_at[tid] = at;
+            if constexpr (TREE) pair_skip[tid] = skip;
         }
         const auto head_of = [&](int32_t pair) { return w.head * p.group + pair - p.by_group.div(pair) * p.group; };
         __syncthreads();
@@ -868,15 +926,38 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             // Keys that each pair sees, of this step's: [lo, hi).
             int32_t lo[8], hi[8];
             bool move = false;
+            const bool drafted = TREE && own && key0 + kTfKeys > s.at0;  // new rows are among the keys
+            // New rows among the step's keys at, at + 1, ... at + 31 that pair i of this thread sees.
+            const auto drafts = [&](int i, int at) {
+                const int32_t row = pair_row[8 * ty + i];
+                if (row < 0) return 0u;
+                const TreeSees sees = tree_sees(p, pair_skip[8 * ty + i], s.at0);
+                return tree_bits(p, row, s.added, tree_first(p, row, s.added, sees.drop), key0 + at - s.at0);
+            };
+            uint32_t mine = 0;  // bit 4 i + j
+            if (drafted) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t a = drafts(i, 0) >> tx, b = drafts(i, 32) >> tx;
+                    mine |= ((a & 1u) | ((a >> 16 & 1u) << 1) | ((b & 1u) << 2) | ((b >> 16 & 1u) << 3)) << (4 * i);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int32_t at = pair_at[8 * ty + i], place = max(at, 0) + (own ? 0 : p.prefix);
-                lo[i] = p.window ? max(place - p.window + 1 - key0, 0) : 0;
-                hi[i] = at < 0 ? 0 : min((own ? min(at + 1, limit) : limit) - key0, kTfKeys);
+                if constexpr (TREE) {
+                    const TreeSees sees = tree_sees(p, pair_skip[8 * ty + i], max(at, 0));
+                    lo[i] = max((own ? sees.lo : sees.pre) - key0, 0);
+                    hi[i] = at < 0 ? 0 : min((own ? at : limit) - key0, kTfKeys);
+                } else {
+                    lo[i] = p.window ? max(place - p.window + 1 - key0, 0) : 0;
+                    hi[i] = at < 0 ? 0 : min((own ? min(at + 1, limit) : limit) - key0, kTfKeys);
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = tx + 16 * j;
-                    x[i][j] = key >= lo[i] && key < hi[i] ? x[i][j] * p.scale2 : -INFINITY;
+                    const bool seen = (key >= lo[i] && key < hi[i]) || (TREE && (mine >> (4 * i + j) & 1u));
+                    x[i][j] = seen ? x[i][j] * p.scale2 : -INFINITY;
                     move |= x[i][j] > m[i] + kLazy;
                 }
             }
@@ -910,7 +991,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             // some pair, the values are looked over.
             bool masked, odd = false;
             const int32_t valid = min(limit - key0, kTfKeys);  // keys that exist
-            step_is_mended(p, s, step, &masked);
+            step_is_mended<TREE>(p, s, step, &masked);
             if (masked) {
 #pragma unroll 4
                 for (int k = tid; k < valid * (kPgDim / 4); k += kTfThreads) {
@@ -928,7 +1009,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                 const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, z[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (all || (key >= lo[i] && key < hi[i])) {
+                    if (all || (key >= lo[i] && key < hi[i]) || (drafted && (drafts(i, key) & 1u))) {
 #pragma unroll
                         for (int d = 0; d < 8; ++d) o[i][d] = fmaf(y[i], z[d], o[i][d]);
                     }
@@ -960,7 +1041,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
 #pragma unroll 1
             for (int key = 8 * eights; key < valid; ++key)
                 add(key, *tf_weight(weights, key, 2 * ty), *tf_weight(weights, key, 2 * ty + 1), *tf_piece(tile_at[1], key, tx),
-                    *tf_piece(tile_at[1], key, 16 + tx), false);
+                    *tf_piece(tile_at[1], key, 16 + tx), TREE && !odd);
             __syncthreads();  // values and weights have been read
             if (tid == 0 && n + 1 < w.steps) copy(n + 1, 1);
             phase ^= 1u;
@@ -976,7 +1057,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             if (row < 0) continue;
             const uint64_t to = whole ? row * p.out_stride + head_of(pair) * kPgDim : (static_cast<uint64_t>(slot) * kTfPairs + pair) * kPgDim;
             const float2 ml = pg_ml(m[i], sum);
-            const float inv = whole ? pg_inverse(pair_at[pair], sum) : 1.0f;
+            const float inv = !whole ? 1.0f : TREE ? tree_inverse(p, row, pair_at[pair], s.added, sum) : pg_inverse(pair_at[pair], sum);
             float *dst = (whole ? static_cast<float *>(p.out) : p.tile_sum) + to + 4 * tx;
             *reinterpret_cast<float4 *>(dst) = make_float4(o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
             *reinterpret_cast<float4 *>(dst + 64) = make_float4(o[i][4] * inv, o[i][5] * inv, o[i][6] * inv, o[i][7] * inv);

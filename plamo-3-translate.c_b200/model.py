@@ -601,10 +601,26 @@ class Backend:
         return paged.store(self, qkv, pool, slots, positions, q_norm, k_norm, table, status)
 
     def paged_attention(self, q, pool, starts, lengths, tables, prefix_pages=None, prefix_rows=0, window=0, scale=None,
-                        out=None, status=None, most_new=0):
+                        out=None, status=None, most_new=0, masks=None):
         """Attention over a shared prefix and each request's own rows; see paged.attention."""
         return paged.attention(self, q, pool, starts, lengths, tables, prefix_pages, prefix_rows, window, scale, out,
-                               status, most_new)
+                               status, most_new, masks)
+
+    def paged_tree(self, parents, starts, lengths, most_new, base=0, status=None):
+        """Positions and masks of a step's draft trees; see paged.tree."""
+        return paged.tree(self, parents, starts, lengths, most_new, base, status)
+
+    def paged_accept(self, parents, tokens, chosen, starts, lengths, tables, free_pages, after):
+        """The confirmed path of each draft tree; see paged.accept."""
+        return paged.accept(self, parents, tokens, chosen, starts, lengths, tables, free_pages, after)
+
+    def paged_keep(self, pools, path, starts, lengths, tables, status=None):
+        """Confirmed rows moved together in every layer's pool; see paged.keep."""
+        return paged.keep(self, pools, path, starts, lengths, tables, status)
+
+    def paged_adapters(self, x, base, a, b, ids, starts, scales=None, out=None, status=None, most_new=0):
+        """A projection's result with each request's low-rank adapter added; see paged.adapters."""
+        return paged.adapters(self, x, base, a, b, ids, starts, scales, out, status, most_new)
 
     def paged_status(self):
         """PLAMO_PAGED_* bits of stores and attention calls without a status tensor; see paged.status."""

@@ -6,7 +6,10 @@ its rows once (`plan`), then per layer stores the projection's rows (`store`)
 and attends (`attention`). Calls are enqueued on torch's current stream and
 return without waiting; tensors they allocate come from torch's allocator.
 Wrong arguments raise ValueError, tensors of another GPU than the backend's
-among them. What only the GPU can see is reported as PLAMO_PAGED_* bits, in the
+among them. A step that verifies drafted tokens adds trees of rows: `tree` gives
+their positions and masks, `attention` takes the masks, `accept` finds the
+confirmed path and `keep` moves its rows together. `adapters` adds each request's
+own low-rank adapter to a projection. What only the GPU can see is reported as PLAMO_PAGED_* bits, in the
 plan's summary and in a `status` tensor (one int32, zeroed by the caller), or
 where a call is given none in a word of the backend's that `status()` reads.
 """
@@ -25,6 +28,22 @@ class Plan(NamedTuple):
     slots: object      # [rows] page * 64 + row in the page, -1 for padding, -2 where the page id is none
     positions: object  # [rows]
     summary: object    # [4] status bits, new rows, free-list entries used so far, longest length
+
+
+class Tree(NamedTuple):
+    """What a step of draft trees has beside its plan (int32 tensors)."""
+    positions: object  # [rows], for the store
+    masks: object      # [rows, words], for attention
+
+
+class Accepted(NamedTuple):
+    """What a step of draft trees leaves (int32 tensors)."""
+    counts: object   # [requests] confirmed rows
+    lengths: object  # [requests] own rows held from here on
+    last: object     # [requests] the newest token, chosen after the last confirmed row; -1 where there is none
+    path: object     # [rows] at starts[r] + k: which of request r's new rows is its k-th confirmed one; else -1
+    tokens: object   # [rows] at starts[r] + k: the token chosen after it; else -1
+    summary: object  # [4] status bits, confirmed rows, free-list entries used so far, longest length
 
 
 _t = None
@@ -113,7 +132,7 @@ def plan(backend, held, added, tables, free_pages, rows, base=0, after=None):
         raise ValueError("free_pages: one dimension")
     stride = _tables(torch, tables, requests, device)
     head = 0
-    if after is not None:
+    if after is not None:  # (an Accepted too)
         _ints(torch, after.summary, 4, device, "after.summary")
         head = after.summary.data_ptr() + 8
     buffer = held.new_empty(2 * requests + 2 * rows + 5)
@@ -165,7 +184,7 @@ def store(backend, qkv, pool, slots, positions, q_norm, k_norm, table, status=No
 
 
 def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, prefix_rows=0, window=0, scale=None, out=None,
-              status=None, most_new=0):
+              status=None, most_new=0, masks=None):
     """Every query over the shared prefix and its own request's rows, causal.
 
     q: [rows, query_heads, 128] of the pool's type (rows may be strided);
@@ -174,7 +193,9 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
     window: rows a query sees, itself included (0: all before it); scale: of
     the scores, 1 / sqrt(128) unless given; most_new: rows of the request that
     adds most (1 in a decode step; 0: not known), which chooses the kernels where
-    q has rows of padding or lengths idle slots. Returns `out`, allocated if None.
+    q has rows of padding or lengths idle slots; masks: of a tree ([rows, words]
+    int32): of the rows that its request adds, a query sees those of its bits, and
+    `window` counts the rows seen. Returns `out`, allocated if None.
     """
     torch = _torch()
     kind, pages, kv_heads, device = _pool(torch, pool, backend)
@@ -203,12 +224,167 @@ def attention(backend, q, pool, starts, lengths, tables, prefix_pages=None, pref
                                    tables.data_ptr(), prefix, 0, 0, _status(torch, status, device), rows, q_stride, out_stride,
                                    requests, stride, prefix_rows, pages, window, query_heads, kv_heads, kind,
                                    DIM ** -0.5 if scale is None else scale, _stream(torch, device), most_new)
-    size = backend.lib.plamo_paged_attention_workspace(backend.ctx, ctypes.byref(args))
+    if masks is None:
+        step, call, measure = args, backend.lib.plamo_paged_attention, backend.lib.plamo_paged_attention_workspace
+    else:
+        if masks.dim() != 2 or masks.shape[0] != rows or not 0 < masks.shape[1] <= _abi.PAGED_TREE_ROWS // 32:
+            raise ValueError(f"masks: [rows, 1 to {_abi.PAGED_TREE_ROWS // 32} words]")
+        _ints(torch, masks, -1, device, "masks")
+        args = _abi.PagedTreeAttentionArgs(args, masks.data_ptr(), masks.shape[1])
+        step, call, measure = args.step, backend.lib.plamo_paged_tree_attention, backend.lib.plamo_paged_tree_attention_workspace
+    size = measure(backend.ctx, ctypes.byref(args))
     if not size:
         raise ValueError(backend.info().note.decode())
     workspace = pool.new_empty(size, dtype=torch.uint8)
+    step.workspace, step.workspace_bytes = workspace.data_ptr(), size
+    _run(backend, call, args)
+    return out
+
+
+def tree(backend, parents, starts, lengths, most_new, base=0, status=None):
+    """Positions and masks of a step whose requests add trees of drafted rows.
+
+    parents: [rows] place of each row's parent among its request's new rows,
+    before its own (-1: it follows the held rows); starts, lengths: of the plan;
+    most_new: rows of the request that adds most, at most 256 (it sets the masks'
+    words, 32 rows each); base: position of own row 0 (the prefix's rows).
+    """
+    torch = _torch()
+    rows, requests, device = parents.numel(), lengths.numel(), parents.get_device()
+    if device != backend.device:
+        raise ValueError(f"parents: on the backend's GPU, {backend.device}")
+    if not 0 <= most_new <= _abi.PAGED_TREE_ROWS:
+        raise ValueError(f"most_new: at most {_abi.PAGED_TREE_ROWS} rows")
+    _ints(torch, parents, rows, device, "parents")
+    _ints(torch, starts, requests + 1, device, "starts")
+    _ints(torch, lengths, requests, device, "lengths")
+    words = max(1, (most_new + 31) // 32)
+    positions, masks = parents.new_empty(rows), parents.new_empty((rows, words))
+    args = _abi.PagedTreeArgs(parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(), masks.data_ptr(),
+                              _status(torch, status, device), rows, requests, words, base, _stream(torch, device))
+    _run(backend, backend.lib.plamo_paged_tree, args)
+    return Tree(positions, masks)
+
+
+def accept(backend, parents, tokens, chosen, starts, lengths, tables, free_pages, after):
+    """The path of drafted rows that the model's choices confirm, after a step's last layer.
+
+    parents: of `tree`; tokens, chosen: [rows] int32, each row's token and the one
+    the model chooses after it; starts, lengths: of the plan; tables, free_pages:
+    as given to it; after: that Plan, or its summary. A request's first row is
+    certain; after a confirmed row comes the first row whose parent it is and
+    whose token was chosen after it. Pages that only dropped rows had reached go
+    back to the front of what is left of free_pages (in place): plan the next
+    step with `after` this result, `held` its lengths.
+    """
+    torch = _torch()
+    rows, requests, device = parents.numel(), lengths.numel(), parents.get_device()
+    if device != backend.device:
+        raise ValueError(f"parents: on the backend's GPU, {backend.device}")
+    for t, name in ((parents, "parents"), (tokens, "tokens"), (chosen, "chosen")):
+        _ints(torch, t, rows, device, name)
+    _ints(torch, starts, requests + 1, device, "starts")
+    _ints(torch, lengths, requests, device, "lengths")
+    stride = _tables(torch, tables, requests, device)
+    _ints(torch, free_pages, -1, device, "free_pages")
+    summary = getattr(after, "summary", after)
+    _ints(torch, summary, 4, device, "after")
+    buffer = parents.new_empty(3 * requests + 2 * rows + 4)
+    counts = buffer.data_ptr()
+    path = counts + 12 * requests
+    args = _abi.PagedAcceptArgs(parents.data_ptr(), tokens.data_ptr(), chosen.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
+                                tables.data_ptr(), free_pages.data_ptr(), summary.data_ptr(), counts, counts + 4 * requests,
+                                counts + 8 * requests, path, path + 4 * rows, path + 8 * rows, rows, requests, stride,
+                                free_pages.numel(), _stream(torch, device))
+    _run(backend, backend.lib.plamo_paged_accept, args)
+    return Accepted(*buffer.unsafe_split_with_sizes((requests, requests, requests, rows, rows, 4)))
+
+
+def keep(backend, pools, path, starts, lengths, tables, status=None):
+    """The confirmed rows' keys and values, moved to follow the held ones.
+
+    pools: a layer's pool or a sequence of them, all of one shape and type, no two
+    the same; path: of `accept`; starts, lengths, tables: of the step's plan.
+    """
+    torch = _torch()
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    if not pools:
+        return
+    kind, pages, kv_heads, device = _pool(torch, pools[0], backend)
+    for pool in pools[1:]:
+        if pool.shape != pools[0].shape or pool.dtype != pools[0].dtype or pool.get_device() != device or not pool.is_contiguous():
+            raise ValueError(f"pools: contiguous, all of one shape and type on the backend's GPU, {device}")
+    rows, requests = path.numel(), lengths.numel()
+    _ints(torch, path, rows, device, "path")
+    _ints(torch, starts, requests + 1, device, "starts")
+    _ints(torch, lengths, requests, device, "lengths")
+    stride = _tables(torch, tables, requests, device)
+    at = (ctypes.c_void_p * len(pools))(*[pool.data_ptr() for pool in pools])
+    args = _abi.PagedKeepArgs(ctypes.addressof(at), path.data_ptr(), starts.data_ptr(), lengths.data_ptr(), tables.data_ptr(),
+                              _status(torch, status, device), len(pools), rows, requests, stride, pages, kv_heads, kind,
+                              _stream(torch, device))
+    _run(backend, backend.lib.plamo_paged_keep, args)
+
+
+def _matrix(torch, t, rows, device, name):
+    """(type, row stride) of a [rows, width] BF16 or FP32 tensor whose rows are contiguous."""
+    if t.dim() != 2 or t.get_device() != device or (rows >= 0 and t.shape[0] != rows):
+        raise ValueError(f"{name}: two dimensions, " + (f"{rows} rows, " if rows >= 0 else "") + f"on GPU {device}")
+    row, step = t.stride()
+    if t.numel() and step != 1 and t.shape[1] > 1:
+        raise ValueError(f"{name}: each row contiguous")
+    return _type(torch, t, name), row if t.shape[0] > 1 else t.shape[1]
+
+
+def adapters(backend, x, base, a, b, ids, starts, scales=None, out=None, status=None, most_new=0):
+    """base + scale * B (A x), each request's rows with its own adapter.
+
+    x: [rows, columns], the projection's input, base: [rows, outputs], its result,
+    BF16 or FP32 each (rows may be strided); a: [adapters, rank, columns], b:
+    [adapters, outputs, rank] BF16 (rank, columns and outputs multiples of 8, rank
+    at most 256: pad with zeros); ids: [requests] int32, -1 for none; starts:
+    [requests + 1]; scales: [adapters] FP32 (1 if None). Requests with the same
+    adapter one after another share its reading. Rows without an adapter are
+    base's. most_new: rows of the request that adds most (0: not known); it
+    chooses the kernels. Returns `out`, allocated if None; it may be `base`.
+    """
+    torch = _torch()
+    device = backend.device
+    x_kind, x_stride = _matrix(torch, x, -1, device, "x")
+    rows, columns = x.shape
+    kind, base_stride = _matrix(torch, base, rows, device, "base")
+    outputs = base.shape[1]
+    if out is None:
+        out = base.new_empty((rows, outputs))
+    out_kind, out_stride = _matrix(torch, out, rows, device, "out")
+    if out.shape != base.shape or out_kind != kind:
+        raise ValueError("out: of base's shape and type")
+    for t, name in ((a, "a"), (b, "b")):
+        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.get_device() != device or not t.is_contiguous():
+            raise ValueError(f"{name}: three dimensions, contiguous BF16 on the backend's GPU, {device}")
+    count, rank, _ = a.shape
+    if a.shape[2] != columns or tuple(b.shape) != (count, outputs, rank):
+        raise ValueError(f"a: [adapters, rank, {columns}], b: [adapters, {outputs}, rank]")
+    requests = ids.numel()
+    _ints(torch, ids, requests, device, "ids")
+    _ints(torch, starts, requests + 1, device, "starts")
+    scale_at = 0
+    if scales is not None:
+        if scales.dtype != torch.float32 or scales.numel() != count or scales.get_device() != device or not scales.is_contiguous():
+            raise ValueError(f"scales: {count} contiguous FP32 entries on the backend's GPU, {device}")
+        scale_at = scales.data_ptr()
+    if most_new < 0:
+        raise ValueError("most_new: not negative")
+    args = _abi.PagedAdaptersArgs(x.data_ptr(), base.data_ptr(), out.data_ptr(), a.data_ptr(), b.data_ptr(), scale_at,
+                                  ids.data_ptr(), starts.data_ptr(), 0, 0, _status(torch, status, device), rows, columns, outputs,
+                                  x_stride, base_stride, out_stride, requests, count, rank, x_kind, kind,
+                                  _stream(torch, device), most_new)
+    size = backend.lib.plamo_paged_adapters_workspace(backend.ctx, ctypes.byref(args))
+    if not size:
+        raise ValueError(backend.info().note.decode())
+    workspace = base.new_empty(size, dtype=torch.uint8)
     args.workspace, args.workspace_bytes = workspace.data_ptr(), size
-    _run(backend, backend.lib.plamo_paged_attention, args)
+    _run(backend, backend.lib.plamo_paged_adapters, args)
     return out
 
 
