@@ -3436,4 +3436,15 @@ bool tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t element_
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+bool tensor_map_heads(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t heads, uint64_t row_stride, uint32_t box_heads,
+                      uint32_t box_rows) {
+    if (!tensor_maps_available()) return false;
+    cuuint64_t dims[3] = {128, heads, rows};
+    cuuint64_t strides[2] = {256, row_stride * 2};
+    cuuint32_t box[3] = {64, box_heads, box_rows};
+    cuuint32_t elem[3] = {1, 1, 1};
+    return g_encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(ptr), dims, strides, box, elem,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 }  // namespace plamo

@@ -37,6 +37,10 @@ bool context_launched(plamo_cuda *c, const char *what, cudaError_t e);
 // 128-byte swizzle; false when the driver refuses it.
 bool tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t element_bytes, const void *ptr, uint64_t rows,
                    uint64_t cols, uint32_t box_cols, uint32_t box_rows);
+// BF16 rows of heads, [rows][heads][128], rows row_stride elements apart: boxes of 64 dimensions of box_heads heads of
+// box_rows rows, 128-byte swizzle.
+bool tensor_map_heads(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t heads, uint64_t row_stride, uint32_t box_heads,
+                      uint32_t box_rows);
 
 // One-time setup of the paged kernels on the context's device.
 cudaError_t paged_configure();

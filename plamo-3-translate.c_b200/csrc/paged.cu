@@ -6,6 +6,7 @@
 #include "paged_adapters.cuh"
 #include "paged_attention.cuh"
 #include "paged_tiles.cuh"
+#include "paged_tree_tiles.cuh"
 #include "paged_trees.cuh"
 
 #include <algorithm>
@@ -62,13 +63,16 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 
 // Prefix rows from which trees share tiles over them.
 constexpr uint64_t kTreeShareRows = 512;
+// What a strip's beginning and end are worth, in units of half a step of a full tile.
+constexpr int32_t kTreeStripPad = 4;
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
     uint32_t prefix_tiles, row_slots, workers, tile_rows, tile_grid, tile_cap;
     uint64_t record, row_sum, row_ml;
     uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
-    bool share;  // trees: all rows share the prefix's tiles
+    bool share;            // trees: all rows share the prefix's tiles
+    uint32_t split_pairs;  // of tiles whose halves take alternate steps
 };
 
 // Draft trees: what a call has beside the step's records.
@@ -110,6 +114,7 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
         a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
         a.share = trees && d->prefix_rows >= kTreeShareRows;
+        a.split_pairs = trees && !f32 ? kTlPairs / 2 : 0;
     }
     a.prefix_tiles = prefix_pages && !a.tile_rows ? static_cast<uint32_t>(ceil_div(pairs, kRtPairs)) : 0;
     a.workers = static_cast<uint32_t>(2 * sms - 1);  // beside the schedule's CTA
@@ -133,9 +138,9 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     a.row_ml = part(static_cast<uint64_t>(a.row_slots) * kRtPairs * sizeof(float2));
     if (a.tile_rows) {
         // Two runs of a CTA may end inside a prompt's tile; every run of a prefix tile is a part.
-        // Where trees share the prefix, so is every run of any tile.
-        const uint64_t kept = a.share ? a.tile_cap : ceil_div(d->rows, a.tile_rows);
-        const uint64_t shared = prefix_pages ? a.tile_grid + kept * d->kv_heads : 0;
+        // Trees: so is every run of any tile.
+        const uint64_t kept = trees ? a.tile_cap : ceil_div(d->rows, a.tile_rows);
+        const uint64_t shared = trees || prefix_pages ? a.tile_grid + kept * d->kv_heads : 0;
         const uint64_t slots = 2ull * a.tile_grid + shared;
         a.tile_shape = part(a.tile_cap * sizeof(TileShape));
         a.tile_unit = part((a.tile_cap + 1ull) * 4);
@@ -184,6 +189,11 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
     p.masks = t.masks;
     p.words = static_cast<int32_t>(t.words);
     p.share = a.share;
+    // Tiles of their own that have the prefix, too, leave the row kernel nothing to share it with.
+    p.short_pairs = a.share || !d->prefix_rows ? kTlShortPairs : 0;
+    p.split_pairs = static_cast<int32_t>(a.split_pairs);
+    p.step_units = F32 ? 1 : 2;
+    p.strip_pad = kTreeStripPad;
     p.scale2 = d->scale * 1.4426950408889634f;
     // The tile kernel masks before it scales: -inf must stay so.
     if (std::fabs(p.scale2) < 1e-30f) p.scale2 = std::copysign(1e-30f, p.scale2);
@@ -208,9 +218,16 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
         p.tile_sum = reinterpret_cast<float *>(ws + a.tile_sum);
         p.tile_ml = reinterpret_cast<float2 *>(ws + a.tile_ml);
     }
+    CUtensorMap q_map{};
+    if (TREE && !F32 && a.tile_rows && !tensor_map_heads(&q_map, d->q, d->rows, d->query_heads, d->q_stride, p.group, a.tile_rows))
+        return context_launched(c, "paged_attention: tensor map", cudaErrorInvalidValue);
     if (!launch(c, "paged_attention rows", paged_rows_kernel<F32, TREE>, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
-        (a.tile_rows && !launch(c, "paged_attention tiles", F32 ? paged_tile_f32_kernel<TREE> : paged_tile_kernel<TREE>, dim3(a.tile_grid),
-                                dim3(F32 ? kTfThreads : kTlThreads), F32 ? kTfSmem : kTlSmem, stream, true, page_map, p)))
+        (a.tile_rows && !(F32    ? launch(c, "paged_attention tiles", paged_tile_f32_kernel<TREE>, dim3(a.tile_grid), dim3(kTfThreads),
+                                          kTfSmem, stream, true, page_map, p)
+                          : TREE ? launch(c, "paged_attention tiles", paged_tree_tile_kernel, dim3(a.tile_grid), dim3(kTlThreads), kTlSmem,
+                                          stream, true, page_map, q_map, p)
+                                 : launch(c, "paged_attention tiles", paged_tile_kernel, dim3(a.tile_grid), dim3(kTlThreads), kTlSmem, stream,
+                                          true, page_map, p))))
         return false;
     // Two results to a block, its warps sharing their parts, while that takes two
     // blocks to an SM at most (one request over 131,072 rows, 74 parts each: 10 us
@@ -318,8 +335,8 @@ cudaError_t paged_configure() {
     if (e == cudaSuccess) e = allow(paged_rows_kernel<true, false>, kRtSmem);
     if (e == cudaSuccess) e = allow(paged_rows_kernel<false, true>, kRtSmem);
     if (e == cudaSuccess) e = allow(paged_rows_kernel<true, true>, kRtSmem);
-    if (e == cudaSuccess) e = allow(paged_tile_kernel<false>, kTlSmem);
-    if (e == cudaSuccess) e = allow(paged_tile_kernel<true>, kTlSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_kernel, kTlSmem);
+    if (e == cudaSuccess) e = allow(paged_tree_tile_kernel, kTlSmem);
     if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<false>, kTfSmem);
     if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<true>, kTfSmem);
     return e;

@@ -69,7 +69,11 @@ struct PagedAttnParams {
     // Draft trees: what the new rows see of one another.
     const uint32_t *masks;  // [rows][words]
     int32_t words;
-    int32_t share;  // all rows share the prefix's tiles, the requests' own tiles have none of it
+    int32_t share;        // all rows share the prefix's tiles, the requests' own tiles have none of it
+    int32_t short_pairs;  // of requests whose own rows are the row kernel's
+    int32_t split_pairs;  // of tiles whose two halves take alternate steps, at most
+    int32_t step_units;   // units of a step of other tiles (of theirs: 1)
+    int32_t strip_pad;    // units that a strip's beginning and end are worth
 };
 enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlFirst, kTlTaken, kRtRun, kRtLonger, kTlHeader };
 // Requests of up to so many pairs keep their own rows in the row kernel and share
@@ -130,13 +134,14 @@ __device__ __forceinline__ OwnShape own_shape(const PagedAttnParams &p, int32_t 
 }
 // Short requests' own rows go through the row kernel, eight pairs at a time;
 // the others are the tile kernel's, where there is one.
+template <bool TREE>
 __device__ __forceinline__ bool request_is_short(const PagedAttnParams &p, const OwnShape &s) {
-    return !p.tile_rows || s.rows * p.group <= kTlShortPairs;
+    return !p.tile_rows || s.rows * p.group <= (TREE ? p.short_pairs : kTlShortPairs);
 }
 template <bool TREE>
 __device__ __forceinline__ OwnShape short_shape(const PagedAttnParams &p, int32_t r) {
     OwnShape s = own_shape<TREE>(p, r);
-    if (!request_is_short(p, s)) s.tiles = s.pages = 0;
+    if (!request_is_short<TREE>(p, s)) s.tiles = s.pages = 0;
     return s;
 }
 
@@ -168,6 +173,23 @@ struct Runs {
 };
 __device__ __forceinline__ Runs tile_runs(const PagedAttnParams &p) { return Runs{p.header[kTlRun], p.header[kTlLonger]}; }
 __device__ __forceinline__ Runs row_runs(const PagedAttnParams &p) { return Runs{p.header[kRtRun], p.header[kRtLonger]}; }
+
+// A tree's strip: units that stand for its beginning and end, then those of its
+// steps. A CTA has the steps whose first unit is in its run.
+constexpr int kTreeMinUnits = 4;
+struct StripUnits {
+    int32_t pad, per_step, steps;
+    __device__ __forceinline__ int32_t unit_of(int32_t step) const { return pad + step * per_step; }
+    __device__ __forceinline__ int32_t step_at(int32_t unit) const { return max(0, (unit - pad + per_step - 1) / per_step); }
+};
+__device__ __forceinline__ bool tile_is_split(const PagedAttnParams &p, const TileShape &s) { return s.rows * p.group <= p.split_pairs; }
+__device__ __forceinline__ int32_t tree_strip_length(const PagedAttnParams &p, const TileShape &s) {
+    return s.steps() ? p.strip_pad + s.steps() * (tile_is_split(p, s) ? 1 : p.step_units) : 0;
+}
+__device__ __forceinline__ StripUnits strip_units(const PagedAttnParams &p, int32_t tile, int32_t length) {
+    const int32_t per_step = tile_is_split(p, p.tile_shape[tile]) ? 1 : p.step_units;
+    return {p.strip_pad, per_step, (length - p.strip_pad) / per_step};
+}
 
 struct RowItem {
     int32_t request;  // -1: prefix
@@ -979,18 +1001,23 @@ __global__ void __launch_bounds__(kRtThreads, 2)
 // ---- joining the parts ----------------------------------------------------------------
 // One result (a row and head): its parts lie in two arrays, the sums of part x
 // at (first + x * stride) * rows + place, joined in that order.
+// `halves` 1: two parts to a slot, half of its rows apart.
 struct PartList {
     const float *sum;
     const float2 *ml;
-    int32_t first, stride, rows, place, count;
-    __device__ __forceinline__ int64_t at(int32_t x) const { return static_cast<int64_t>(first + x * stride) * rows + place; }
+    int32_t first, stride, rows, place, count, halves;
+    template <bool HALVES>
+    __device__ __forceinline__ int64_t at(int32_t x) const {
+        if constexpr (HALVES) return static_cast<int64_t>(first + (x >> halves) * stride) * rows + place + (x & halves) * (rows / 2);
+        return static_cast<int64_t>(first + x * stride) * rows + place;
+    }
 };
 // Joins RES (2 or 8) results, lane y's lists those of result y % RES (empty
 // where there is none). Warp `sub` of `warps` takes every warps-th part of each,
 // 32 / RES at a time: a lane weighs one part of one result, then the parts' sums
 // are loaded eight at once. Every lane returns with four dimensions of the sums
 // over its warp's parts, and l and the maximum m over them of its own result.
-template <int RES>
+template <int RES, bool HALVES>
 __device__ __forceinline__ void join_parts(const PartList &a, const PartList &b, int32_t sub, int32_t warps, float4 (&o)[RES], float &l,
                                            float &m) {
     const int32_t lane = threadIdx.x & 31, all = a.count + b.count;
@@ -1006,7 +1033,7 @@ __device__ __forceinline__ void join_parts(const PartList &a, const PartList &b,
         const float *from = nullptr;
         if (x < all) {
             const bool first = x < a.count;
-            const int64_t at = first ? a.at(x) : b.at(x - a.count);
+            const int64_t at = first ? a.at<HALVES>(x) : b.at<HALVES>(x - a.count);
             v = (first ? a.ml : b.ml)[at];
             from = (first ? a.sum : b.sum) + at * kPgDim;
         }
@@ -1094,12 +1121,22 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
             // The parts of place `at` of a tile for this head, where all of them are kept.
             const auto tile_parts = [&](int32_t tile, int32_t at) {
                 const int32_t unit = p.tile_unit[tile], steps = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
-                const int32_t u0 = unit * p.kh + kv * steps, c0 = runs.cta_of(u0);
+                const int32_t u0 = unit * p.kh + kv * steps;
+                if constexpr (TREE) {
+                    if (!steps) return PartList{};
+                    const StripUnits strip = strip_units(p, tile, steps);
+                    const int32_t c0 = runs.cta_of(u0 + strip.unit_of(0)), c1 = runs.cta_of(u0 + strip.unit_of(strip.steps - 1));
+                    const int32_t halves = tile_is_split(p, p.tile_shape[tile]);
+                    return PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, p.tile_pairs,
+                                    at * p.group + in_group, (c1 - c0 + 1) << halves, halves};
+                }
+                const int32_t c0 = runs.cta_of(u0);
                 return PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, p.tile_pairs,
                                 at * p.group + in_group, steps ? runs.cta_of(u0 + steps - 1) - c0 + 1 : 0};
             };
             if (TREE && e.z < 0) {
                 own = tile_parts(-1 - e.z, e.w);
+                written = own.count == 1 && !p.share && !own.halves;  // (one of two halves' parts is not a result)
             } else {
                 own = row_parts(e.z, e.w * p.group + in_group);
                 written = own.count == 1 && p.prefix == 0;  // where it was computed
@@ -1113,7 +1150,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         }
         const uint32_t skip = __ballot_sync(0xffffffffu, written || head >= p.qh);  // (the same in all warps of an item)
         if (skip == 0xffffffffu) continue;
-        join_parts<RES>(shared, own, FEW ? warp : 0, FEW ? kJoinWarps : 1, o, l, top);
+        join_parts<RES, TREE>(shared, own, FEW ? warp : 0, FEW ? kJoinWarps : 1, o, l, top);
         const auto inverse = [&](float sum) {
             if constexpr (!TREE) return pg_inverse(e.y, sum);
             return sum == 0.0f && (e.y < 0 || tree_blank(p, e.x, e.y, listed_added(p, e))) ? 0.0f : 1.0f / sum;
@@ -1150,9 +1187,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     }
     // Prompts' tiles that a CTA's end cuts: the first such end does the tile.
     const int32_t blocks = p.tile_pairs / (RES * kJoinWarps);  // to a tile
-    const bool listed_all = TREE && p.share;  // every row was in the list
 #pragma unroll 1
-    for (int32_t n = blockIdx.x; !listed_all && n < blocks * (ctas - 1); n += gridDim.x) {
+    for (int32_t n = blockIdx.x; !TREE && n < blocks * (ctas - 1); n += gridDim.x) {  // (trees' rows were all in the list)
         const int32_t c = n / blocks + 1, pair0 = ((n - (c - 1) * blocks) * kJoinWarps + warp) * RES, cut = runs.start(c);
         const int32_t tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(tiles), p.by_kh.div(cut));
         if (tile < pre_tiles) continue;
@@ -1164,15 +1200,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
         const int32_t pair = pair0 + (lane & (RES - 1)), there = pair < pairs;
         shared = PartList{p.tile_sum, p.tile_ml, 2 * (c - 1) + (before == u0 ? 0 : 1), 0, p.tile_pairs, pair, there};
         own = PartList{p.tile_sum, p.tile_ml, 2 * c, 2, p.tile_pairs, pair, there * (runs.cta_of(u0 + steps - 1) - c + 1)};
-        join_parts<RES>(shared, own, 0, 1, o, l, top);
+        join_parts<RES, TREE>(shared, own, 0, 1, o, l, top);
 #pragma unroll
         for (int i = 0; i < RES; ++i) {
             const float li = __shfl_sync(0xffffffffu, l, i);
             if (pair0 + i >= pairs) break;
             const int32_t row = p.by_group.div(pair0 + i);
-            const float inv = TREE ? tree_inverse(p, row0 + row, p.tile_shape[tile].at0, p.tile_shape[tile].added, li)
-                                   : pg_inverse(p.tile_shape[tile].at0 + row, li);
-            join_store<F32>(p, row0 + row, inv, kv * p.group + pair0 + i - row * p.group, o[i]);
+            join_store<F32>(p, row0 + row, pg_inverse(p.tile_shape[tile].at0 + row, li), kv * p.group + pair0 + i - row * p.group, o[i]);
         }
     }
     // Rows that no request has, and tiles without a key.
@@ -1187,7 +1221,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 #pragma unroll 1
     for (int32_t row = end_row + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
 #pragma unroll 1
-    for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); !listed_all && tile < tiles; tile += gridDim.x)
+    for (int32_t tile = pre_tiles + static_cast<int32_t>(blockIdx.x); !TREE && tile < tiles; tile += gridDim.x)
         if (p.tile_unit[tile + 1] == p.tile_unit[tile])
             for (int32_t i = 0; i < p.tile_shape[tile].rows; ++i) clear(p.tile_shape[tile].row0 + i);
 }

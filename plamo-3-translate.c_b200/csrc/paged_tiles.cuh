@@ -71,8 +71,8 @@ __device__ __forceinline__ TileShape prompt_tile(const PagedAttnParams &p, int32
 // and prompts (tiles of their own over prefix and own rows), and numbers the
 // key steps of all tiles. A step of a tile and KV head is the unit of work: the
 // tile kernel's CTAs take equal runs of consecutive ones.
-// Trees that share the prefix's tiles: all rows are listed, and a request that is
-// not short has tiles of its own over its own rows only.
+// Trees: all rows are listed. Where they share the prefix's tiles, a request that
+// is not short has tiles of its own over its own rows only; else over the prefix, too.
 template <bool TREE>
 __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     __shared__ int32_t first_at;
@@ -94,8 +94,8 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         if (p.starts[r] < 0 || p.starts[r + 1] > p.rows) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
         decreases |= p.starts[r + 1] < p.starts[r];
         if (TREE && s.rows > 32 * p.words) pg_flag(p.status, PLAMO_PAGED_TREE);
-        const bool is_short = request_is_short(p, s);
-        if (is_short || (TREE && p.share)) {
+        const bool is_short = request_is_short<TREE>(p, s);
+        if (is_short || TREE) {
             short_rows += s.rows;
             if (s.rows) lowest = min(lowest, max(s.at0, 0));
         }
@@ -109,7 +109,7 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
     const int32_t all_short = ordered ? static_cast<int32_t>(all_short_rows) : 0;
     int32_t pre_tiles = 0;
     TileShape pre{};
-    if (p.tile_rows && p.prefix) {
+    if (p.tile_rows && p.prefix && (!TREE || p.share)) {
         pre_tiles = p.by_tile_rows.div(all_short + p.tile_rows - 1);
         pre.request = -1;
         pre.pre1 = (p.prefix + p.tile_keys - 1) / p.tile_keys;
@@ -121,8 +121,8 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
 #pragma unroll 1
     for (int32_t r = r0; r < r1; ++r) {
         const OwnShape s = own_shape<TREE>(p, r);
-        const bool is_short = request_is_short(p, s);
-        if (is_short || (TREE && p.share)) {
+        const bool is_short = request_is_short<TREE>(p, s);
+        if (is_short || TREE) {
             const int32_t first_tile = pre_tiles + static_cast<int32_t>(tile_at);
 #pragma unroll 1
             for (int32_t i = 0; i < s.rows && short_at + i < all_short; ++i) {
@@ -160,7 +160,7 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
             shape = prompt_tile<TREE>(p, r, own_shape<TREE>(p, r), p.tile_shape[t].row0);
         }
         int64_t sum;
-        const int64_t at = total + pg_block_scan<kRtThreads>(shape.steps(), sums, &sum);
+        const int64_t at = total + pg_block_scan<kRtThreads>(TREE ? tree_strip_length(p, shape) : shape.steps(), sums, &sum);
         if (t < all) {
             p.tile_shape[t] = shape;
             p.tile_unit[t] = static_cast<uint32_t>(at);
@@ -177,7 +177,9 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         p.header[kTlTaken] = fits ? min(max(taken, 0), p.rows) : 0;
         p.header[kTlShortRows] = fits ? all_short : 0;
         const int32_t units = fits ? static_cast<int32_t>(total * p.kh) : 0;
-        const int32_t ctas = p.tile_rows ? min(p.tile_grid, (units + kTlMinUnits - 1) / kTlMinUnits) : 0;
+        // (a tree's CTA has more units than a step costs: each but a strip's first owns a step)
+        const int32_t least = TREE ? max(units / kTreeMinUnits, units > 0) : (units + kTlMinUnits - 1) / kTlMinUnits;
+        const int32_t ctas = p.tile_rows ? min(p.tile_grid, least) : 0;
         p.header[kTlCtas] = ctas;
         p.header[kTlRun] = ctas ? units / ctas : 1;
         p.header[kTlLonger] = ctas ? units % ctas : 0;
@@ -236,6 +238,27 @@ struct TileWalk {
     int32_t tile, head, step, steps;  // current segment: first step and count
     int32_t tile_steps;
 };
+// The same for trees, whose strips' units are not their steps (strip_units);
+// moves on to the unit behind the segment.
+__device__ __noinline__ bool tree_walk_next(const PagedAttnParams &p, TileWalk &w) {
+    while (w.unit < w.end) {
+        const int32_t t0 = p.tile_unit[w.tile], length = static_cast<int32_t>(p.tile_unit[w.tile + 1]) - t0;
+        if (w.unit >= (t0 + length) * p.kh) {
+            ++w.tile;
+            continue;
+        }
+        const StripUnits strip = strip_units(p, w.tile, length);
+        const int32_t x = w.unit - t0 * p.kh;
+        w.head = x / length;
+        const int32_t from = t0 * p.kh + w.head * length, until = min(w.end, from + length);
+        w.step = strip.step_at(w.unit - from);
+        w.steps = strip.step_at(until - from) - w.step;
+        w.tile_steps = strip.steps;
+        w.unit = until;
+        if (w.steps) return true;
+    }
+    return false;
+}
 __device__ __noinline__ bool walk_next(const PagedAttnParams &p, TileWalk &w) {
     if (w.unit >= w.end) return false;
     for (;; ++w.tile) {
@@ -252,23 +275,19 @@ __device__ __noinline__ bool walk_next(const PagedAttnParams &p, TileWalk &w) {
 
 // Values that are not finite left the products of steps with masked keys: the
 // rows that see them get them here (a weight times one of them is itself).
-template <bool TREE>
-__device__ __noinline__ void add_odd_values(const PagedAttnParams &p, const TileShape &s, const TileWalk &w, int32_t row, int32_t at,
-                                            const TreeSees &sees, int c, float (&o)[32]) {
+__device__ __noinline__ void add_odd_values(const PagedAttnParams &p, const TileShape &s, const TileWalk &w, int32_t at, int c, float (&o)[32]) {
     const int32_t pre_steps = s.pre1 - s.pre0;
     for (int32_t n = 0; n < w.steps; ++n) {
         const int32_t step = w.step + n;
         bool masked;
-        step_is_mended<TREE>(p, s, step, &masked);
+        step_is_mended<false>(p, s, step, &masked);
         if (!masked) continue;
         const bool own = step >= pre_steps;
         const int32_t key0 = (own ? s.own0 + step - pre_steps : s.pre0 + step) * kTlKeys;
-        const int32_t hi = at < 0 ? 0 : min(key0 + kTlKeys, own ? (TREE ? s.own_limit : min(at + 1, s.own_limit)) : p.prefix);
-        const int32_t lo = TREE ? max(key0, own ? sees.lo : sees.pre) : p.window ? max(key0, (own ? at : p.prefix + at) - p.window + 1) : key0;
-        const int32_t from = TREE && own ? tree_first(p, row, s.added, sees.drop) : 0;
+        const int32_t hi = at < 0 ? 0 : min(key0 + kTlKeys, own ? min(at + 1, s.own_limit) : p.prefix);
+        const int32_t lo = p.window ? max(key0, (own ? at : p.prefix + at) - p.window + 1) : key0;
 #pragma unroll 1
         for (int32_t key = lo; key < hi; ++key) {
-            if (TREE && own && key >= at && !(tree_bits(p, row, s.added, from, key - at) & 1u)) continue;
             const int32_t id = own ? p.tables[static_cast<uint64_t>(s.request) * p.table_stride + key / kPgRows] : p.prefix_pages[key / kPgRows];
             if (id < 0 || id >= p.pages) continue;
             const uint16_t *v = static_cast<const uint16_t *>(p.pool) + ((static_cast<uint64_t>(id) * 2 + 1) * kPgRows + key % kPgRows) * p.kh * kPgDim +
@@ -282,7 +301,6 @@ __device__ __noinline__ void add_odd_values(const PagedAttnParams &p, const Tile
     }
 }
 
-template <bool TREE>
 __global__ void __launch_bounds__(kTlThreads, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(128) unsigned char tl_smem[];
@@ -429,7 +447,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     const bool more = n + 1 < w.steps;
                     bool masked;
                     ok = tl_wait(&full[vs], (v / kTlUnits) & 1u, quit);
-                    if (ok && step_is_mended<TREE>(p, s, w.step + n, &masked)) {
+                    if (ok && step_is_mended<false>(p, s, w.step + n, &masked)) {
                         ok = tl_wait(&mended[vs], (mends >> vs) & 1u, quit);
                         mends ^= 1u << vs;
                     }
@@ -473,7 +491,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     bool masked;
-                    if (kind && step_is_mended<TREE>(p, s, w.step + n, &masked)) {
+                    if (kind && step_is_mended<false>(p, s, w.step + n, &masked)) {
                         const int32_t step = w.step + n;
                         const bool own = step >= pre_steps;
                         const int32_t key0 = (own ? s.own0 + step - pre_steps : s.pre0 + step) * kTlKeys;
@@ -526,20 +544,11 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             const int32_t pairs = s.rows * p.group, pre_steps = s.pre1 - s.pre0;
             const bool active = i == 0 || pairs > 128, there = pair < pairs;
             const int32_t local = p.by_group.div(pair);
-            int32_t row = s.row0 + local, at = TREE ? s.at0 : s.at0 + local, added = s.added;  // trees: `at` is the held rows
+            int32_t row = s.row0 + local, at = s.at0 + local;
             if (s.request < 0 && there) {
                 const int4 e = p.short_list[row];
                 row = e.x;
                 at = e.y;
-                if (TREE && p.window) added = listed_added(p, e);
-            }
-            TreeSees sees{0, 0, 0};
-            int32_t from = 0;  // bits of the mask below it are outside the window
-            if constexpr (TREE) {
-                if (there && at >= 0 && p.window) {
-                    sees = tree_sees(p, tree_skip(p, row, at, added), at);
-                    from = tree_first(p, row, added, sees.drop);
-                }
             }
             const int32_t head = w.head * p.group + pair - local * p.group;
             if (!active) continue;
@@ -566,9 +575,9 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 
             const float scale2 = fabsf(p.scale2);
             // Keys this row sees, prefix and own: [lo, hi).
-            const int32_t pre_hi = at < 0 ? 0 : p.prefix, own_hi = at < 0 ? 0 : TREE ? at : min(at + 1, s.own_limit);
-            const int32_t pre_lo = TREE ? sees.pre : p.window ? max(p.prefix + max(at, 0) - p.window + 1, 0) : 0;
-            const int32_t own_lo = TREE ? sees.lo : p.window ? max(max(at, 0) - p.window + 1, 0) : 0;
+            const int32_t pre_hi = at < 0 ? 0 : p.prefix, own_hi = at < 0 ? 0 : min(at + 1, s.own_limit);
+            const int32_t pre_lo = p.window ? max(p.prefix + max(at, 0) - p.window + 1, 0) : 0;
+            const int32_t own_lo = p.window ? max(max(at, 0) - p.window + 1, 0) : 0;
             float m = -INFINITY, l = 0.0f;
             for (int32_t n = 0; n < w.steps; ++n) {
                 ok = tl_wait(&s_full[i], n_scores & 1u, quit);
@@ -583,13 +592,6 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 const int32_t hi = min(max((own ? own_hi : pre_hi) - key0, 0), kTlKeys);
                 const int32_t lo = min(max((own ? own_lo : pre_lo) - key0, 0), kTlKeys);
                 const bool partial = __any_sync(0xffffffffu, there && (lo > 0 || hi < kTlKeys));
-                uint32_t drafts[4] = {0, 0, 0, 0};  // new rows among the keys that this row sees
-                if constexpr (TREE) {
-                    if (own && key0 + kTlKeys > s.at0 && there) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) drafts[k] = tree_bits(p, row, s.added, from, key0 + 32 * k - at);
-                    }
-                }
                 // 64 scores at a time, twice: for the maximum, then for the weights, which replace them
                 // (two BF16 terms). Loops, not straight code: a segment is a few steps long, and
                 // code that runs a few times costs its fetching.
@@ -599,11 +601,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     tmem_ld32_async(scol + 64 * half + 32, reinterpret_cast<uint32_t(&)[32]>(x[32]));
                     tmem_wait_ld();
                     if (partial) {
-                        uint32_t see0 = tl_bits(lo - 64 * half, hi - 64 * half), see1 = tl_bits(lo - 64 * half - 32, hi - 64 * half - 32);
-                        if constexpr (TREE) {
-                            see0 |= half ? drafts[2] : drafts[0];
-                            see1 |= half ? drafts[3] : drafts[1];
-                        }
+                        const uint32_t see0 = tl_bits(lo - 64 * half, hi - 64 * half), see1 = tl_bits(lo - 64 * half - 32, hi - 64 * half - 32);
 #pragma unroll
                         for (int k = 0; k < 64; ++k)
                             if (!((k < 32 ? see0 : see1) >> (k & 31) & 1u)) x[k] = 0xff800000u;  // -inf
@@ -675,11 +673,10 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const bool parts = w.tile < pre_tiles || (TREE && p.share);  // all segments are kept, to be joined with others
-            const bool whole = w.steps == w.tile_steps && !parts;
-            const int32_t slot = parts ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
+            const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles;
+            const int32_t slot = w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
             const bool odd = *reinterpret_cast<volatile int *>(&odd_values);
-            const float inv = !TREE ? pg_inverse(at, l) : whole && there ? tree_inverse(p, row, at, s.added, l) : 1.0f;
+            const float inv = pg_inverse(at, l);
             // Through shared memory (the queries' place: the scores are done with them), so that rows
             // leave 256 bytes at a time: the whole result, or half of the partial sums.
             const int64_t to = !there ? -1 : whole ? row * static_cast<int64_t>(p.out_stride) + head * kPgDim
@@ -696,7 +693,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     float more[32];
 #pragma unroll
                     for (int k = 0; k < 32; ++k) more[k] = o[k];
-                    add_odd_values<TREE>(p, s, w, row, at, sees, c, more);
+                    add_odd_values(p, s, w, at, c, more);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = more[k];
                 }
@@ -810,7 +807,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
     bool ok = true;
     uint32_t phase = 0;
 #pragma unroll 1
-    for (bool begins = true; ok && walk_next(p, w); w.unit += w.steps, begins = false) {
+    for (bool begins = true; ok && (TREE ? tree_walk_next(p, w) : walk_next(p, w)); w.unit += TREE ? 0 : w.steps, begins = false) {
         const TileShape s = p.tile_shape[w.tile];
         const int32_t pre_steps = s.pre1 - s.pre0, pairs = s.rows * p.group;
         // Step n's page, first key and the key from which on nothing is seen.
@@ -832,9 +829,8 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             copy(0, 0);
             copy(0, 1);
         }
-        const bool parts = w.tile < pre_tiles || (TREE && p.share);  // all segments are kept, to be joined with others
-        const bool whole = w.steps == w.tile_steps && !parts;
-        const int32_t slot = parts ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
+        const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles && !(TREE && p.share);
+        const int32_t slot = TREE || w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
         if (tid < kTfPairs) {
             int32_t row = -1, at = 0, skip = 0;
             if (tid < pairs) {

@@ -1,0 +1,573 @@
+// Attention of draft trees on the tensor cores: BF16, tiles of up to 256 (row,
+// head) pairs by steps of 128 keys. FP32 trees have paged_tile_f32_kernel.
+#pragma once
+#include "paged_tiles.cuh"
+
+namespace plamo {
+
+// As the plain tile kernel, a tile is two halves of 128 pairs with four softmax
+// warps each, scores and sums in tensor memory and the weights, as two BF16 terms
+// (16 bits), in the scores' place. What differs:
+//  - A step's scores are made and weighed 64 keys at a time, in two places by turns.
+//    The products of one place run under the softmax of the other, so that a half
+//    waits for nobody while the tensor pipe keeps up; 64 scores stay in a thread's
+//    registers from the maximum to the weights.
+//  - A tile of at most 128 pairs (a request's tree of 16 rows and eight heads to a KV
+//    head is one) has both halves: they take alternate steps with the same queries,
+//    and have sums of their own that the join adds up.
+//  - Strips (a tile and KV head) are a few steps long where they are a request's own
+//    rows, so their ends count. The copying warp walks the work and tells the others
+//    what comes next through shared memory. The rows of all tiles follow one another
+//    in the batch, so that it can copy a tile's queries, too, as a box, which arrive
+//    under the last softmax of the strip before. Sums leave tensor memory for global
+//    memory 32 bytes at a time. And strips count as longer than their steps where the
+//    work is divided.
+//  - The products' warp stays converged and elects a lane for each instruction: from a
+//    branch of one lane an MMA took 55 cycles to issue, and as long again around it.
+
+constexpr int kTsSegments = 4;  // segments told ahead
+// A segment, a run of steps of one (tile, KV head).
+struct __align__(16) TreeSegment {
+    int32_t steps;  // 0: there is no more work
+    int32_t split;  // halves take alternate steps
+    int32_t tile, head, step, tile_steps;
+    int32_t row0, pairs, held, added;  // first batch row; the tile's pairs; its request's held (-1: of many requests) and new rows
+    int32_t pre0, pre_steps, own0;     // first key step and number of steps over the prefix, first over its own rows
+    int32_t unused[3];
+};
+// The units (keys or values of one step) of a segment come in rounds: a step's keys
+// and values, or, of split tiles, the keys and then the values of two steps, one for
+// each half.
+__device__ __forceinline__ int32_t ts_width(int32_t steps, bool split, int32_t d) { return split ? min(2, steps - 2 * d) : min(1, steps - d); }
+// A half's step in round d; none where it is not below the number of steps.
+__device__ __forceinline__ int32_t ts_step(bool split, int32_t d, int32_t half) { return split ? 2 * d + half : d; }
+// What the others need of a unit: its rows that exist, and whether some row does not see all of them.
+constexpr int32_t kTsMasked = 256;
+
+// Values that are not finite left the products of steps with masked keys: the
+// rows that see them get them here (a weight times one of them is itself).
+__device__ __noinline__ void tree_add_odd_values(const PagedAttnParams &p, const TreeSegment &t, int32_t row, int32_t held, int32_t added,
+                                                 const TreeSees &sees, int32_t from, int half, int c, float (&o)[32]) {
+    const TileShape s = p.tile_shape[t.tile];
+#pragma unroll 1
+    for (int32_t n = t.split ? half : 0; n < t.steps; n += t.split ? 2 : 1) {
+        const int32_t step = t.step + n;
+        bool masked;
+        step_is_mended<true>(p, s, step, &masked);
+        if (!masked) continue;
+        const bool own = step >= t.pre_steps;
+        const int32_t key0 = (own ? t.own0 + step - t.pre_steps : t.pre0 + step) * kTlKeys;
+        const int32_t hi = min(key0 + kTlKeys, own ? s.own_limit : p.prefix);
+#pragma unroll 1
+        for (int32_t key = max(key0, own ? sees.lo : sees.pre); key < hi; ++key) {
+            if (own && key >= held && !(tree_bits(p, row, added, from, key - held) & 1u)) continue;
+            const int32_t id = own ? p.tables[static_cast<uint64_t>(s.request) * p.table_stride + key / kPgRows] : p.prefix_pages[key / kPgRows];
+            if (id < 0 || id >= p.pages) continue;
+            const uint16_t *v = static_cast<const uint16_t *>(p.pool) + ((static_cast<uint64_t>(id) * 2 + 1) * kPgRows + key % kPgRows) * p.kh * kPgDim +
+                                static_cast<uint64_t>(t.head) * kPgDim + c;
+#pragma unroll 1
+            for (int k = 0; k < 32; ++k) {
+                const float x = bf16_to_f32(v[k]);
+                if (!isfinite(x)) o[k] += x;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void store_256(float *to, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+__global__ void __launch_bounds__(kTlThreads, 1)
+    paged_tree_tile_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap q_map,
+                           const __grid_constant__ PagedAttnParams p) {
+    extern __shared__ __align__(128) unsigned char tl_smem[];
+    __shared__ __align__(8) uint64_t full[kTlUnits], empty[kTlUnits], mended[kTlUnits];
+    __shared__ __align__(8) uint64_t seg_full[kTsSegments], seg_empty[kTsSegments];
+    __shared__ __align__(8) uint64_t q_full, q_empty, s_full[4], p_full[4], pv_done[4];  // [2 * half + place]
+    __shared__ TreeSegment segments[kTsSegments];
+    __shared__ int32_t unit_rows[kTlUnits];
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up, odd_values;
+    unsigned char *base = reinterpret_cast<unsigned char *>(
+        (reinterpret_cast<uintptr_t>(tl_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char *units_at = base + kTlQBytes;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < kTlUnits; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 2);  // the products, and the mending warp
+            mbar_init(&mended[s], 1);
+        }
+        for (int s = 0; s < kTsSegments; ++s) {
+            mbar_init(&seg_full[s], 1);
+            mbar_init(&seg_empty[s], 10);  // the products, the mending warp, eight of softmax
+        }
+        mbar_init(&q_full, 1);
+        mbar_init(&q_empty, 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+        }
+        gave_up = odd_values = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&map);
+        prefetch_tensormap(&q_map);
+    }
+    if (warp == kTlProducts) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    pdl_launch_dependents();
+    volatile int *quit = &gave_up;
+    bool ok = true;
+
+    if (warp == kTlCopies) {
+        // ---- copies: the work's segments, their queries and the units of each round
+        pdl_wait();
+        const int32_t ctas = p.header[kTlCtas], cta = static_cast<int32_t>(blockIdx.x);
+        const int32_t first_row = p.header[kTlFirst];
+        TileWalk w{};
+        if (cta < ctas) {
+            const Runs runs = tile_runs(p);
+            w.unit = runs.start(cta);
+            w.end = runs.start(cta + 1);
+            w.tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(p.header[kTlTiles]), p.by_kh.div(w.unit));
+        }
+        uint32_t q = 0, seg = 0;
+        for (bool more = true; more && ok; ++seg) {
+            more = tree_walk_next(p, w);
+            TileShape s{};
+            if (more) s = p.tile_shape[w.tile];
+            const bool split = more && tile_is_split(p, s);
+            const int32_t pre_steps = s.pre1 - s.pre0, row0 = s.request < 0 ? first_row + s.row0 : s.row0;
+            if (lane == 0) {
+                const uint32_t e = seg % kTsSegments;
+                ok = seg < kTsSegments || tl_wait(&seg_empty[e], (seg / kTsSegments - 1) & 1u, quit);
+                TreeSegment t{};
+                if (more)
+                    t = TreeSegment{w.steps, split, w.tile, w.head, w.step, w.tile_steps, row0, s.rows * p.group,
+                                    s.request < 0 ? -1 : s.at0, s.added, s.pre0, pre_steps, s.own0, {}};
+                if (ok) segments[e] = t;
+                if (ok) mbar_arrive(&seg_full[e]);
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!more || !ok) break;
+            const int32_t pair = split ? 2 : 1;  // steps to a round
+            const int32_t *own_table = p.tables + static_cast<uint64_t>(max(s.request, 0)) * p.table_stride;
+            const int32_t pre_pages = (p.prefix + kPgRows - 1) / kPgRows;
+            const int32_t own_pages = (s.own_limit + kPgRows - 1) / kPgRows;
+            bool queries = true;  // still to be copied, behind the first round's units
+            for (int32_t base_step = 0; base_step < w.steps && ok; base_step += 16) {
+                // Page ids of 16 steps, two to a step.
+                int32_t id = -1;
+                bool there = false;
+                {
+                    const int32_t st = w.step + base_step + (lane >> 1);
+                    if (base_step + (lane >> 1) < w.steps) {
+                        const bool own = st >= pre_steps;
+                        const int32_t pg = 2 * (own ? s.own0 + st - pre_steps : s.pre0 + st) + (lane & 1);
+                        there = pg < (own ? own_pages : pre_pages);
+                        if (there) id = own ? own_table[pg] : p.prefix_pages[pg];
+                    }
+                }
+                if (there && (id < 0 || id >= p.pages)) {
+                    pg_flag(p.status, PLAMO_PAGED_PAGE);
+                    id = p.pages;  // past the pool: reads as zeros
+                }
+                const uint32_t present = __ballot_sync(0xffffffffu, there);
+                const int32_t here = min(16, w.steps - base_step);
+#pragma unroll 1
+                for (int32_t k = 0; k < 2 * here && ok; ++k) {  // (16 is even: no round is cut)
+                    // Unit k: round k / (2 pair), its keys, then its values.
+                    const int32_t first = k / (2 * pair) * pair, width = min(pair, here - first), y = k - 2 * first;
+                    const int kind = y >= width;
+                    const int32_t n = first + y - kind * width;
+                    const int32_t id0 = __shfl_sync(0xffffffffu, id, 2 * n), id1 = __shfl_sync(0xffffffffu, id, 2 * n + 1);
+                    const bool two = (present >> (2 * n + 1)) & 1;
+                    if (lane == 0) {
+                        const uint32_t st = q % kTlUnits;
+                        if (q >= kTlUnits && !tl_wait(&empty[st], (q / kTlUnits - 1) & 1u, quit)) {
+                            ok = false;
+                        } else {
+                            unsigned char *dst = units_at + st * kTlUnitBytes;
+                            const int32_t step = w.step + base_step + n;
+                            const bool own = step >= pre_steps;
+                            const int32_t key0 = (own ? s.own0 + step - pre_steps : s.pre0 + step) * kTlKeys;
+                            bool masked = false;
+                            if (kind) step_is_mended<true>(p, s, step, &masked);
+                            unit_rows[st] = min((own ? s.own_limit : p.prefix) - key0, kTlKeys) | (masked ? kTsMasked : 0);
+                            mbar_expect_tx(&full[st], two ? kTlUnitBytes : kTlUnitBytes / 2);
+                            const int x = w.head * kPgDim, y0 = (id0 * 2 + kind) * kPgRows, y1 = (id1 * 2 + kind) * kPgRows;
+                            tma_load_2d(dst, &map, x, y0, &full[st]);
+                            tma_load_2d(dst + kTlUnitBytes / 2, &map, x + 64, y0, &full[st]);
+                            if (two) {
+                                tma_load_2d(dst + kPgRows * 128, &map, x, y1, &full[st]);
+                                tma_load_2d(dst + kTlUnitBytes / 2 + kPgRows * 128, &map, x + 64, y1, &full[st]);
+                            }
+                            ++q;
+                            if (queries && k + 1 == 2 * width) {
+                                if (seg && !tl_wait(&q_empty, (seg - 1) & 1u, quit)) {
+                                    ok = false;
+                                } else {
+                                    mbar_expect_tx(&q_full, 2u * p.tile_rows * p.group * 128);
+                                    tma_load_3d(base, &q_map, 0, w.head * p.group, row0, &q_full);
+                                    tma_load_3d(base + kTlQBytes / 2, &q_map, 64, w.head * p.group, row0, &q_full);
+                                }
+                                queries = false;
+                            }
+                        }
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                }
+            }
+        }
+        if (lane == 0) {  // every copy issued has landed before the CTA can exit
+            for (uint32_t n = q > kTlUnits ? q - kTlUnits : 0; n < q; ++n)
+                if (!mbar_wait(&full[n % kTlUnits], (n / kTlUnits) & 1u)) break;
+            // (the queries' last copy, too: where all went well the products have waited for it)
+            if (!ok && q && seg) mbar_wait(&q_full, (seg - 1) & 1u);
+        }
+    } else if (warp == kTlProducts) {
+        // ---- products
+        constexpr uint32_t idesc_s = tc_idesc(128, kTlKeys / 2), idesc_o = tc_idesc(128, kPgDim) | kTcIdescMnB;
+        constexpr uint32_t kBlock = kTlPairs * 128 / 16;  // between the queries' blocks of 64 dimensions
+        // Bit 2 i + h: half i, place h. `weights`: phases waited for; `sums`: the last value product's phase;
+        // `unread`: its weights may not have been read yet.
+        uint32_t q = 0, weights = 0, sums = 0xf, unread = 0, mends = 0;
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(base)), k_desc = smem_desc_sw128(smem_u32(units_at));
+        const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(units_at), kTlKeys * 128);
+        const bool leader = elect_one();
+        const auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, tl_wait(bar, parity, quit)) != 0; };
+        const auto arrived = [&](uint32_t unit) { return wait(&full[unit % kTlUnits], (unit / kTlUnits) & 1u); };
+        for (uint32_t seg = 0; ok; ++seg) {
+            ok = wait(&seg_full[seg % kTsSegments], (seg / kTsSegments) & 1u);
+            if (!ok) break;
+            const int32_t steps = __shfl_sync(0xffffffffu, segments[seg % kTsSegments].steps, 0);
+            const bool split = __shfl_sync(0xffffffffu, segments[seg % kTsSegments].split, 0);
+            __syncwarp();
+            if (leader) mbar_arrive(&seg_empty[seg % kTsSegments]);
+            if (!steps) break;
+            int32_t left = steps * (split ? 2 : 4);  // scores still to be made
+            // (addresses in descriptors count 16 bytes)
+            const auto scores = [&](uint32_t bit, uint32_t unit) {
+                const uint32_t i = bit >> 1, h = bit & 1;
+                if ((unread >> bit) & 1u) {  // they replace the weights
+                    if (!wait(&pv_done[bit], (sums >> bit) & 1u)) return false;
+                    unread &= ~(1u << bit);
+                    tc_fence_after();
+                }
+                --left;
+                const uint64_t a = q_desc + (split ? 0 : i * (128 * 128 / 16)), b = k_desc + (unit % kTlUnits) * (kTlUnitBytes / 16) + h * (64 * 128 / 16);
+                const uint32_t d = tmem + 64 * bit;
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < kPgDim / 16; ++k)
+                        tc_mma(d, a + (k / 4) * kBlock + (k % 4) * 2, b + ((k / 4) * (kTlKeys * 128) + (k % 4) * 32) / 16, idesc_s, k ? 1u : 0u);
+                    tc_commit(&s_full[bit]);
+                    if (h && (i || split)) tc_commit(&empty[unit % kTlUnits]);
+                    if (!left) tc_commit(&q_empty);
+                }
+                __syncwarp();
+                return true;
+            };
+            // The first round's scores.
+            ok = wait(&q_full, seg & 1u);
+            tc_fence_after();
+#pragma unroll 1
+            for (uint32_t i = 0; i < 2 && ok; ++i) {
+                if (ts_step(split, 0, i) >= steps) continue;
+                const uint32_t unit = q + (split ? i : 0);
+                if (i == 0 || split) ok = arrived(unit);
+                for (uint32_t h = 0; h < 2 && ok; ++h) ok = scores(2 * i + h, unit);
+            }
+            // Each value product is followed by the next round's scores for the place of the product
+            // before it, which is done by then or nearly so.
+            uint32_t next = 4, next_unit = 0;  // that place's bit, 4: none
+            const int32_t rounds = split ? (steps + 1) / 2 : steps;
+#pragma unroll 1
+            for (int32_t d = 0; d < rounds && ok; ++d) {
+                const int32_t width = ts_width(steps, split, d);
+                const uint32_t q_next = q + 2 * width;
+#pragma unroll 1
+                for (uint32_t job = 0; job < 4 && ok; ++job) {
+                    const uint32_t i = job & 1, h = job >> 1, bit = 2 * i + h;
+                    if (ts_step(split, d, i) >= steps) continue;
+                    const uint32_t v = q + width + (split ? i : 0), vs = v % kTlUnits;
+                    if (h == 0 && (i == 0 || split)) {
+                        ok = arrived(v);
+                        if (ok && __shfl_sync(0xffffffffu, unit_rows[vs], 0) != kTlKeys) {
+                            ok = wait(&mended[vs], (mends >> vs) & 1u);
+                            mends ^= 1u << vs;
+                        }
+                    }
+                    if (ok) ok = wait(&p_full[bit], (weights >> bit) & 1u);
+                    weights ^= 1u << bit;
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t b = v_desc + vs * (kTlUnitBytes / 16) + h * 4 * 128;
+                    const uint32_t o = tmem + 256 + 128 * i, a = tmem + 64 * bit, more = d || h;
+                    if (leader) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {  // both terms of 16 keys' weights
+                            tc_mma_ts(o, a + 8 * k, b + k * 128, idesc_o, k ? 1u : more);
+                            tc_mma_ts(o, a + 8 * k + 32, b + k * 128, idesc_o, 1u);
+                        }
+                        tc_commit(&pv_done[bit]);
+                        if (h && (i || split)) tc_commit(&empty[vs]);
+                    }
+                    __syncwarp();
+                    sums ^= 1u << bit;
+                    unread |= 1u << bit;
+                    if (next < 4) {
+                        if (!(next & 1) && (next == 0 || split)) ok = arrived(next_unit);
+                        if (ok) ok = scores(next, next_unit);
+                        next = 4;
+                    }
+                    if (ts_step(split, d + 1, i) < steps) {
+                        next = bit;
+                        next_unit = q_next + (split ? i : 0);
+                    }
+                }
+                q = q_next;
+            }
+        }
+    } else if (warp == kTlMending) {
+        // ---- mending: values that no weight may touch become zero before the products read them
+        uint32_t q = 0;
+        for (uint32_t seg = 0; ok; ++seg) {
+            ok = __all_sync(0xffffffffu, tl_wait(&seg_full[seg % kTsSegments], (seg / kTsSegments) & 1u, quit));
+            if (!ok) break;
+            const int32_t units = 2 * segments[seg % kTsSegments].steps;
+            const bool split = segments[seg % kTsSegments].split;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[seg % kTsSegments]);
+            if (!units) break;
+            for (int32_t n = 0; n < units && ok; ++n, ++q) {
+                const uint32_t st = q % kTlUnits;
+                ok = __all_sync(0xffffffffu, tl_wait(&full[st], (q / kTlUnits) & 1u, quit));
+                if (!ok) break;
+                const int32_t word = unit_rows[st], rows = word & (kTsMasked - 1);
+                const bool values = split ? (n & 3) >= min(2, (units - (n & ~3)) / 2) : n & 1, masked = word & kTsMasked;
+                if (values && word != kTlKeys) {
+                    unsigned char *unit = units_at + st * kTlUnitBytes;
+                    bool odd = false;
+                    for (int c = lane; c < kTlUnitBytes / 16; c += 32) {  // 16-byte pieces, row by row
+                        const int row = (c >> 3) & (kTlKeys - 1);
+                        uint4 *at = reinterpret_cast<uint4 *>(unit + 16 * c);
+                        if (row >= rows) {
+                            *at = make_uint4(0, 0, 0, 0);
+                        } else if (masked) {
+                            uint4 v = *at;
+                            bool bad = false;
+                            uint32_t *half = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                if ((half[x] & 0x7f80u) == 0x7f80u) {
+                                    half[x] &= 0xffff0000u;
+                                    bad = true;
+                                }
+                                if ((half[x] & 0x7f800000u) == 0x7f800000u) {
+                                    half[x] &= 0x0000ffffu;
+                                    bad = true;
+                                }
+                            }
+                            if (bad) *at = v;
+                            odd |= bad;
+                        }
+                    }
+                    if (odd) odd_values = 1;
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&mended[st]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[st]);
+            }
+        }
+    } else {
+        // ---- softmax: a thread per pair
+        pdl_wait();
+        const int i = warp >> 2;  // half
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t scol = tmem + lanes + 128 * i, ocol = tmem + lanes + 256 + 128 * i;
+        const float scale2 = fabsf(p.scale2);
+        const uint32_t flip = p.scale2 < 0.0f ? 0x80000000u : 0u;
+        const int32_t cta = static_cast<int32_t>(blockIdx.x);
+        uint32_t n_scores = 0, n_sums = 0x3;  // bit h: phase of the scores to wait for; of the last value product
+        for (uint32_t seg = 0; ok; ++seg) {
+            ok = __all_sync(0xffffffffu, tl_wait(&seg_full[seg % kTsSegments], (seg / kTsSegments) & 1u, quit));
+            if (!ok) break;
+            const TreeSegment t = segments[seg % kTsSegments];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[seg % kTsSegments]);
+            if (!t.steps) break;
+            const int pair = (t.split ? 0 : 128 * i) + (warp & 3) * 32 + lane;
+            const bool there = pair < t.pairs;
+            const int32_t row = t.row0 + p.by_group.div(pair);
+            int32_t held = t.held, added = t.added, from = 0;  // `from`: bits of the mask below it are outside the window
+            TreeSees sees{0, 0, 0};
+            if (p.window && there) {
+                if (held < 0) {  // rows of many requests
+                    const int4 e = p.short_list[row - p.header[kTlFirst]];
+                    held = max(e.y, 0);
+                    added = listed_added(p, e);
+                }
+                sees = tree_sees(p, tree_skip(p, row, held, added), held);
+                from = tree_first(p, row, added, sees.drop);
+            }
+            float m = -INFINITY, l = 0.0f;
+            bool any = false;  // value products of this segment
+            for (int32_t d = 0; ok && ts_step(t.split, d, i) < t.steps; ++d) {
+                const int32_t step = t.step + ts_step(t.split, d, i);
+                const bool own = step >= t.pre_steps;
+                const int32_t step0 = (own ? t.own0 + step - t.pre_steps : t.pre0 + step) * kTlKeys;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    // Keys this row sees, of the prefix or the held rows: [lo, hi).
+                    const int32_t key0 = step0 + 64 * h;
+                    const int32_t hi = min(max((own ? held : p.prefix) - key0, 0), 64);
+                    const int32_t lo = min(max((own ? sees.lo : sees.pre) - key0, 0), 64);
+                    const bool partial = __any_sync(0xffffffffu, there && (lo > 0 || hi < 64));
+                    uint32_t see0 = 0xffffffffu, see1 = 0xffffffffu;
+                    if (partial) {
+                        see0 = tl_bits(lo, hi);
+                        see1 = tl_bits(lo - 32, hi - 32);
+                        if (own && key0 + 64 > held && there) {  // new rows among the keys
+                            see0 |= tree_bits(p, row, added, from, key0 - held);
+                            see1 |= tree_bits(p, row, added, from, key0 + 32 - held);
+                        }
+                    }
+                    ok = __all_sync(0xffffffffu, tl_wait(&s_full[2 * i + h], (n_scores >> h) & 1u, quit));
+                    if (!ok) break;
+                    n_scores ^= 1u << h;
+                    tc_fence_after();
+                    uint32_t x[64];
+                    tmem_ld32_async(scol + 64 * h, reinterpret_cast<uint32_t(&)[32]>(x[0]));
+                    tmem_ld32_async(scol + 64 * h + 32, reinterpret_cast<uint32_t(&)[32]>(x[32]));
+                    tmem_wait_ld();
+                    if (flip) {
+#pragma unroll
+                        for (int k = 0; k < 64; ++k) x[k] ^= flip;
+                    }
+                    if (partial) {
+#pragma unroll
+                        for (int k = 0; k < 64; ++k)
+                            if (!((k < 32 ? see0 : see1) >> (k & 31) & 1u)) x[k] = 0xff800000u;  // -inf
+                    }
+                    float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 64; k += 8)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) y[z] = fmaxf(fmaxf(y[z], __uint_as_float(x[k + 2 * z])), __uint_as_float(x[k + 2 * z + 1]));
+                    const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * scale2;
+                    // The reference point moves only when passed by 2^8: the weights stay below 2^8, FP32
+                    // sums lose nothing by it, and the sums in tensor memory are rarely touched.
+                    const bool move = top > m + kLazy;
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float factor = move ? pg_exp2(m - top) : 1.0f;
+                        if (move) m = top;
+                        l *= factor;
+                        if (any) {  // behind this half's last product, the other place's; its next needs these weights
+                            ok = __all_sync(0xffffffffu, tl_wait(&pv_done[2 * i + (h ^ 1)], (n_sums >> (h ^ 1)) & 1u, quit));
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < kPgDim; c += 32) {
+                                uint32_t o[32];
+                                tmem_ld32_async(ocol + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                                tmem_st32(ocol + c, o);
+                            }
+                        }
+                    }
+                    const float shift = m == -INFINITY ? 0.0f : -m;
+                    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        uint32_t first[16], rest[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float a = pg_exp2(fmaf(__uint_as_float(x[32 * part + 2 * k]), scale2, shift));
+                            const float b = pg_exp2(fmaf(__uint_as_float(x[32 * part + 2 * k + 1]), scale2, shift));
+                            l0 += a;
+                            l1 += b;
+                            pg_split(a, b, first[k], rest[k]);
+                        }
+                        tmem_st16(scol + 64 * h + 16 * part, first);
+                        tmem_st16(scol + 64 * h + 32 + 16 * part, rest);
+                    }
+                    l += l0 + l1;
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+                    n_sums ^= 1u << h;
+                    any = true;
+                }
+            }
+            if (!ok) break;
+            // ---- the segment's sums
+            const bool whole = t.steps == t.tile_steps && t.held >= 0 && !p.share && !t.split;
+            const int64_t place = static_cast<int64_t>(2 * p.tile_grid + cta + t.tile * p.kh + t.head) * kTlPairs + pair + (t.split ? 128 * i : 0);
+            if (any) {
+                ok = __all_sync(0xffffffffu, tl_wait(&pv_done[2 * i + 1], (n_sums >> 1) & 1u, quit));
+                if (!ok) break;
+                tc_fence_after();
+                const bool odd = *reinterpret_cast<volatile int *>(&odd_values);
+                const float inv = whole && there ? tree_inverse(p, row, held, added, l) : 1.0f;
+                const int32_t head = t.head * p.group + pair - p.by_group.div(pair) * p.group;
+#pragma unroll 1
+                for (int c = 0; c < kPgDim; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_async(ocol + c, o);
+                    tmem_wait_ld();
+                    if (!there) continue;
+                    if (odd) {
+                        float with[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) with[k] = __uint_as_float(o[k]);
+                        tree_add_odd_values(p, t, row, held, added, sees, from, i, c, with);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(with[k]);
+                    }
+                    if (whole) {
+                        uint16_t *to = static_cast<uint16_t *>(p.out) + row * p.out_stride + head * kPgDim + c;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            uint32_t b[4];
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) b[z] = pg_pack(__uint_as_float(o[k + 2 * z]) * inv, __uint_as_float(o[k + 2 * z + 1]) * inv);
+                            *reinterpret_cast<uint4 *>(to + k) = make_uint4(b[0], b[1], b[2], b[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) store_256(p.tile_sum + place * kPgDim + c + k, o + k);
+                    }
+                }
+                tc_fence_before();
+            }
+            if (there && !whole) p.tile_ml[place] = pg_ml(m, l);
+        }
+    }
+    if (!ok && lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kTlProducts) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+}  // namespace plamo
