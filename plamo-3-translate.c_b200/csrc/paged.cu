@@ -224,7 +224,7 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
     if (!launch(c, "paged_attention rows", paged_rows_kernel<F32, TREE>, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
         (a.tile_rows && !(F32    ? launch(c, "paged_attention tiles", paged_tile_f32_kernel<TREE>, dim3(a.tile_grid), dim3(kTfThreads),
                                           kTfSmem, stream, true, page_map, p)
-                          : TREE ? launch(c, "paged_attention tiles", paged_tree_tile_kernel, dim3(a.tile_grid), dim3(kTlThreads), kTlSmem,
+                          : TREE ? launch(c, "paged_attention tiles", paged_tree_tile_kernel, dim3(a.tile_grid), dim3(kTsThreads), kTlSmem,
                                           stream, true, page_map, q_map, p)
                                  : launch(c, "paged_attention tiles", paged_tile_kernel, dim3(a.tile_grid), dim3(kTlThreads), kTlSmem, stream,
                                           true, page_map, p))))

@@ -22,10 +22,13 @@ namespace plamo {
 //    under the last softmax of the strip before. Sums leave tensor memory for global
 //    memory 32 bytes at a time. And strips count as longer than their steps where the
 //    work is divided.
-//  - The products' warp stays converged and elects a lane for each instruction: from a
-//    branch of one lane an MMA took 55 cycles to issue, and as long again around it.
+//  - A warp to a half issues its products, converged, with a lane elected for each
+//    instruction: from a branch of one lane an MMA took 55 cycles to issue, and one
+//    warp for both halves left the tensor pipe waiting for half of the time.
 
 constexpr int kTsSegments = 4;  // segments told ahead
+constexpr int kTsCopies = 8, kTsMending = 10, kTsProducts = 9;  // warps; half 1's products are warp 11's, 0-7 softmax
+constexpr int kTsThreads = 384;
 // A segment, a run of steps of one (tile, KV head).
 struct __align__(16) TreeSegment {
     int32_t steps;  // 0: there is no more work
@@ -74,13 +77,17 @@ __device__ __noinline__ void tree_add_odd_values(const PagedAttnParams &p, const
     }
 }
 
+__device__ __forceinline__ void mbar_arrive_count(uint64_t *bar, uint32_t count) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __noinline__ bool ts_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up) { return tl_wait(bar, parity, gave_up); }
 __device__ __forceinline__ void store_256(float *to, const uint32_t *v) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
                  "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 
-__global__ void __launch_bounds__(kTlThreads, 1)
+__global__ void __launch_bounds__(kTsThreads, 1)
     paged_tree_tile_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap q_map,
                            const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(128) unsigned char tl_smem[];
@@ -98,15 +105,15 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     if (tid == 0) {
         for (int s = 0; s < kTlUnits; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 2);  // the products, and the mending warp
+            mbar_init(&empty[s], 3);  // both halves' products, and the mending warp (for a half without the unit, too)
             mbar_init(&mended[s], 1);
         }
         for (int s = 0; s < kTsSegments; ++s) {
             mbar_init(&seg_full[s], 1);
-            mbar_init(&seg_empty[s], 10);  // the products, the mending warp, eight of softmax
+            mbar_init(&seg_empty[s], 11);  // two of products, one of mending, eight of softmax
         }
         mbar_init(&q_full, 1);
-        mbar_init(&q_empty, 1);
+        mbar_init(&q_empty, 2);
         for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
@@ -117,7 +124,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
         prefetch_tensormap(&map);
         prefetch_tensormap(&q_map);
     }
-    if (warp == kTlProducts) {
+    if (warp == kTsProducts) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
                      "r"(512)
                      : "memory");
@@ -131,7 +138,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     volatile int *quit = &gave_up;
     bool ok = true;
 
-    if (warp == kTlCopies) {
+    if (warp == kTsCopies) {
         // ---- copies: the work's segments, their queries and the units of each round
         pdl_wait();
         const int32_t ctas = p.header[kTlCtas], cta = static_cast<int32_t>(blockIdx.x);
@@ -237,17 +244,23 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             // (the queries' last copy, too: where all went well the products have waited for it)
             if (!ok && q && seg) mbar_wait(&q_full, (seg - 1) & 1u);
         }
-    } else if (warp == kTlProducts) {
-        // ---- products
+    } else if (warp == kTsProducts || warp == kTsProducts + 2) {
+        // ---- products of one half
         constexpr uint32_t idesc_s = tc_idesc(128, kTlKeys / 2), idesc_o = tc_idesc(128, kPgDim) | kTcIdescMnB;
         constexpr uint32_t kBlock = kTlPairs * 128 / 16;  // between the queries' blocks of 64 dimensions
-        // Bit 2 i + h: half i, place h. `weights`: phases waited for; `sums`: the last value product's phase;
-        // `unread`: its weights may not have been read yet.
-        uint32_t q = 0, weights = 0, sums = 0xf, unread = 0, mends = 0;
+        const uint32_t i = warp != kTsProducts;
+        uint64_t *const s_bar = s_full + 2 * i, *const p_bar = p_full + 2 * i, *const pv_bar = pv_done + 2 * i;
+        // Bit h, a place: phases of weights waited for; the last value product's phase; whether its
+        // weights may not have been read yet.
+        uint32_t q = 0, weights = 0, sums = 3, unread = 0;
+        // (addresses in descriptors count 16 bytes)
         const uint64_t q_desc = smem_desc_sw128(smem_u32(base)), k_desc = smem_desc_sw128(smem_u32(units_at));
         const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(units_at), kTlKeys * 128);
+        const uint32_t s_at = tmem + 128 * i, o_at = tmem + 256 + 128 * i;
         const bool leader = elect_one();
-        const auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, tl_wait(bar, parity, quit)) != 0; };
+        const auto wait = [&](uint64_t *bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, ts_wait(bar, parity, quit));
+        };
         const auto arrived = [&](uint32_t unit) { return wait(&full[unit % kTlUnits], (unit / kTlUnits) & 1u); };
         for (uint32_t seg = 0; ok; ++seg) {
             ok = wait(&seg_full[seg % kTsSegments], (seg / kTsSegments) & 1u);
@@ -257,91 +270,79 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             __syncwarp();
             if (leader) mbar_arrive(&seg_empty[seg % kTsSegments]);
             if (!steps) break;
-            int32_t left = steps * (split ? 2 : 4);  // scores still to be made
-            // (addresses in descriptors count 16 bytes)
-            const auto scores = [&](uint32_t bit, uint32_t unit) {
-                const uint32_t i = bit >> 1, h = bit & 1;
-                if ((unread >> bit) & 1u) {  // they replace the weights
-                    if (!wait(&pv_done[bit], (sums >> bit) & 1u)) return false;
-                    unread &= ~(1u << bit);
-                    tc_fence_after();
-                }
-                --left;
-                const uint64_t a = q_desc + (split ? 0 : i * (128 * 128 / 16)), b = k_desc + (unit % kTlUnits) * (kTlUnitBytes / 16) + h * (64 * 128 / 16);
-                const uint32_t d = tmem + 64 * bit;
+            const int32_t rounds = split ? (steps + 1 - static_cast<int32_t>(i)) / 2 : steps;  // with a step of this half
+            const uint64_t a = q_desc + (split ? 0 : i * (128 * 128 / 16));
+            const auto scores = [&](uint32_t h, uint32_t unit, bool last) {
+                const uint64_t b = k_desc + (unit % kTlUnits) * (kTlUnitBytes / 16) + h * (64 * 128 / 16);
                 if (leader) {
 #pragma unroll
                     for (int k = 0; k < kPgDim / 16; ++k)
-                        tc_mma(d, a + (k / 4) * kBlock + (k % 4) * 2, b + ((k / 4) * (kTlKeys * 128) + (k % 4) * 32) / 16, idesc_s, k ? 1u : 0u);
-                    tc_commit(&s_full[bit]);
-                    if (h && (i || split)) tc_commit(&empty[unit % kTlUnits]);
-                    if (!left) tc_commit(&q_empty);
+                        tc_mma(s_at + 64 * h, a + (k / 4) * kBlock + (k % 4) * 2, b + ((k / 4) * (kTlKeys * 128) + (k % 4) * 32) / 16, idesc_s, k ? 1u : 0u);
+                    tc_commit(&s_bar[h]);
+                    if (h) tc_commit(&empty[unit % kTlUnits]);
+                    if (h && last) tc_commit(&q_empty);
                 }
                 __syncwarp();
-                return true;
             };
-            // The first round's scores.
+            // Scores replace weights: those have been read when the place's last value product is done.
+            const auto place_free = [&](uint32_t h) {
+                if (!((unread >> h) & 1u)) return true;
+                unread &= ~(1u << h);
+                return wait(&pv_bar[h], (sums >> h) & 1u);
+            };
             ok = wait(&q_full, seg & 1u);
-            tc_fence_after();
-#pragma unroll 1
-            for (uint32_t i = 0; i < 2 && ok; ++i) {
-                if (ts_step(split, 0, i) >= steps) continue;
-                const uint32_t unit = q + (split ? i : 0);
-                if (i == 0 || split) ok = arrived(unit);
-                for (uint32_t h = 0; h < 2 && ok; ++h) ok = scores(2 * i + h, unit);
+            if (!ok) break;
+            uint32_t unit = q + (split ? i : 0);  // of the next keys
+            if (rounds) {
+                ok = arrived(unit) && place_free(0);
+                tc_fence_after();
+                if (ok) scores(0, unit, rounds == 1);
+                ok = ok && place_free(1);
+                tc_fence_after();
+                if (ok) scores(1, unit, rounds == 1);
+            } else if (leader) {
+                mbar_arrive(&q_empty);
             }
-            // Each value product is followed by the next round's scores for the place of the product
-            // before it, which is done by then or nearly so.
-            uint32_t next = 4, next_unit = 0;  // that place's bit, 4: none
-            const int32_t rounds = split ? (steps + 1) / 2 : steps;
 #pragma unroll 1
             for (int32_t d = 0; d < rounds && ok; ++d) {
                 const int32_t width = ts_width(steps, split, d);
-                const uint32_t q_next = q + 2 * width;
-#pragma unroll 1
-                for (uint32_t job = 0; job < 4 && ok; ++job) {
-                    const uint32_t i = job & 1, h = job >> 1, bit = 2 * i + h;
-                    if (ts_step(split, d, i) >= steps) continue;
-                    const uint32_t v = q + width + (split ? i : 0), vs = v % kTlUnits;
-                    if (h == 0 && (i == 0 || split)) {
-                        ok = arrived(v);
-                        if (ok && __shfl_sync(0xffffffffu, unit_rows[vs], 0) != kTlKeys) {
-                            ok = wait(&mended[vs], (mends >> vs) & 1u);
-                            mends ^= 1u << vs;
-                        }
-                    }
-                    if (ok) ok = wait(&p_full[bit], (weights >> bit) & 1u);
-                    weights ^= 1u << bit;
+                const uint32_t v = q + width + (split ? i : 0), vs = v % kTlUnits;
+                q += 2 * width;
+                unit = q + (split ? i : 0);
+                const bool more = d + 1 < rounds;
+                ok = arrived(v);
+                if (ok && __shfl_sync(0xffffffffu, unit_rows[vs], 0) != kTlKeys) ok = wait(&mended[vs], (v / kTlUnits) & 1u);
+                const uint64_t b = v_desc + vs * (kTlUnitBytes / 16);
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    if (ok) ok = wait(&p_bar[h], (weights >> h) & 1u);
+                    weights ^= 1u << h;
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t b = v_desc + vs * (kTlUnitBytes / 16) + h * 4 * 128;
-                    const uint32_t o = tmem + 256 + 128 * i, a = tmem + 64 * bit, more = d || h;
                     if (leader) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {  // both terms of 16 keys' weights
-                            tc_mma_ts(o, a + 8 * k, b + k * 128, idesc_o, k ? 1u : more);
-                            tc_mma_ts(o, a + 8 * k + 32, b + k * 128, idesc_o, 1u);
+                            tc_mma_ts(o_at, s_at + 64 * h + 8 * k, b + (4 * h + k) * 128, idesc_o, h || k ? 1u : d > 0);
+                            tc_mma_ts(o_at, s_at + 64 * h + 8 * k + 32, b + (4 * h + k) * 128, idesc_o, 1u);
                         }
-                        tc_commit(&pv_done[bit]);
-                        if (h && (i || split)) tc_commit(&empty[vs]);
+                        tc_commit(&pv_bar[h]);
+                        if (h) tc_commit(&empty[vs]);
                     }
                     __syncwarp();
-                    sums ^= 1u << bit;
-                    unread |= 1u << bit;
-                    if (next < 4) {
-                        if (!(next & 1) && (next == 0 || split)) ok = arrived(next_unit);
-                        if (ok) ok = scores(next, next_unit);
-                        next = 4;
-                    }
-                    if (ts_step(split, d + 1, i) < steps) {
-                        next = bit;
-                        next_unit = q_next + (split ? i : 0);
+                    sums ^= 1u << h;
+                    unread |= 1u << h;
+                    if (more) {
+                        if (!h) ok = arrived(unit);
+                        ok = ok && place_free(h);
+                        tc_fence_after();
+                        if (ok) scores(h, unit, d + 2 == rounds);
                     }
                 }
-                q = q_next;
             }
+            // (a split segment's last round may be the other half's alone)
+            if (split && i && (steps & 1)) q += 2;
         }
-    } else if (warp == kTlMending) {
+    } else if (warp == kTsMending) {
         // ---- mending: values that no weight may touch become zero before the products read them
         uint32_t q = 0;
         for (uint32_t seg = 0; ok; ++seg) {
@@ -387,11 +388,10 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     }
                     if (odd) odd_values = 1;
                     fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&mended[st]);
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[st]);
+                if (lane == 0) mbar_arrive(&mended[st]);  // (of every unit: its phases are the ring's)
+                if (lane == 0) mbar_arrive_count(&empty[st], split ? 2 : 1);
             }
         }
     } else {
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     if (!ok && lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
     tc_fence_before();
     __syncthreads();
-    if (warp == kTlProducts) {
+    if (warp == kTsProducts) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
