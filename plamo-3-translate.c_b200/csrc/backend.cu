@@ -3426,10 +3426,10 @@ bool context_launched(plamo_cuda *c, const char *what, cudaError_t e) {
     return note(c, what, e);
 }
 bool tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t element_bytes, const void *ptr, uint64_t rows,
-                   uint64_t cols, uint32_t box_cols, uint32_t box_rows) {
+                   uint64_t cols, uint32_t box_cols, uint32_t box_rows, uint64_t row_stride) {
     if (!tensor_maps_available()) return false;
     cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {cols * element_bytes};
+    cuuint64_t strides[1] = {(row_stride ? row_stride : cols) * element_bytes};
     cuuint32_t box[2] = {box_cols, box_rows};
     cuuint32_t elem[2] = {1, 1};
     return g_encode_tiled(map, type, 2, const_cast<void *>(ptr), dims, strides, box, elem,

@@ -34,9 +34,10 @@ bool context_note(plamo_cuda *c, const char *what, cudaError_t e);
 bool context_launched(plamo_cuda *c, const char *what, cudaError_t e);
 
 // Row-major 2-D tensor map [rows][cols] with a {box_cols x box_rows} box and
-// 128-byte swizzle; false when the driver refuses it.
+// 128-byte swizzle, rows row_stride elements apart (0: cols); false when the driver refuses it.
 bool tensor_map_2d(CUtensorMap *map, CUtensorMapDataType type, uint32_t element_bytes, const void *ptr, uint64_t rows,
-                   uint64_t cols, uint32_t box_cols, uint32_t box_rows);
+                   uint64_t cols, uint32_t box_cols, uint32_t box_rows, uint64_t row_stride = 0);
+
 // BF16 rows of heads, [rows][heads][128], rows row_stride elements apart: boxes of 64 dimensions of box_heads heads of
 // box_rows rows, 128-byte swizzle.
 bool tensor_map_heads(CUtensorMap *map, const void *ptr, uint64_t rows, uint64_t heads, uint64_t row_stride, uint32_t box_heads,

@@ -62,9 +62,10 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 }
 
 // Prefix rows from which trees share tiles over them.
-constexpr uint64_t kTreeShareRows = 512;
+constexpr uint64_t kTreeShareRows = 1024;
+constexpr uint32_t kTreeShortPairs = 8;
 // What a strip's beginning and end are worth, in units of half a step of a full tile.
-constexpr int32_t kTreeStripPad = 4;
+constexpr int32_t kTreeStripPad = 12;
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
@@ -73,6 +74,7 @@ struct AttentionLayout {
     uint64_t header, short_list, tile_shape, tile_unit, tile_sum, tile_ml, bytes;
     bool share;            // trees: all rows share the prefix's tiles
     uint32_t split_pairs;  // of tiles whose halves take alternate steps
+    uint32_t short_pairs;  // of requests whose own rows are the row kernel's
 };
 
 // Draft trees: what a call has beside the step's records.
@@ -106,14 +108,21 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     const uint64_t tile_pairs = f32 ? kTfPairs : kTlPairs;
     const uint64_t strips = ceil_div(pairs, kRtPairs) * d->kv_heads;
     const uint64_t prefix_steps = ceil_div(pairs, kTlPairs) * d->kv_heads * ceil_div(d->prefix_rows, kTlKeys);
-    const bool prompts = (d->most_new ? std::min(d->most_new, d->rows) * group : d->rows > d->requests ? pairs : 0) > kTlShortPairs;
+    const uint64_t most = d->most_new ? std::min(d->most_new, d->rows) : d->rows > d->requests ? d->rows : 0;  // rows of a request
+    a.short_pairs = trees && !f32 ? kTreeShortPairs : kTlShortPairs;
+    const bool prompts = most * group > a.short_pairs;
     if (group <= tile_pairs && ((prompts && strips * (prefix_pages + d->table_stride) > kTlPromptUnits) ||
                                 (!f32 && strips * prefix_pages > kTlPrefixUnits + 4 * prefix_steps))) {
         a.tile_rows = static_cast<uint32_t>(tile_pairs / group);
         a.tile_grid = static_cast<uint32_t>(f32 ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
         a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
-        a.share = trees && d->prefix_rows >= kTreeShareRows;
+        // Tiles over the prefix that all trees share are full; their own have room for whole rows of
+        // one tree only, but need no joining with others.
+        const uint64_t room = d->requests * ceil_div(std::max<uint64_t>(most, 1), a.tile_rows) * tile_pairs;
+        a.share = trees && d->prefix_rows >= kTreeShareRows && 5 * pairs < 4 * room;
+        // (tiles of their own that have the prefix, too, leave the row kernel nothing to share it with)
+        if (trees && !a.share && d->prefix_rows) a.short_pairs = 0;
         a.split_pairs = trees && !f32 ? kTlPairs / 2 : 0;
     }
     a.prefix_tiles = prefix_pages && !a.tile_rows ? static_cast<uint32_t>(ceil_div(pairs, kRtPairs)) : 0;
@@ -189,11 +198,11 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
     p.masks = t.masks;
     p.words = static_cast<int32_t>(t.words);
     p.share = a.share;
-    // Tiles of their own that have the prefix, too, leave the row kernel nothing to share it with.
-    p.short_pairs = a.share || !d->prefix_rows ? kTlShortPairs : 0;
+    p.short_pairs = static_cast<int32_t>(a.short_pairs);
     p.split_pairs = static_cast<int32_t>(a.split_pairs);
     p.step_units = F32 ? 1 : 2;
-    p.strip_pad = kTreeStripPad;
+    p.strip_pad = F32 ? 0 : kTreeStripPad;
+    p.least_units = F32 ? 1 : 4;
     p.scale2 = d->scale * 1.4426950408889634f;
     // The tile kernel masks before it scales: -inf must stay so.
     if (std::fabs(p.scale2) < 1e-30f) p.scale2 = std::copysign(1e-30f, p.scale2);
@@ -288,17 +297,105 @@ const char *adapters_shapes(const plamo_paged_adapters_args *d) {
 
 struct AdaptersLayout {
     uint32_t splits, share;
+    bool tall;  // 16 rows to a warp
     uint64_t bytes;
 };
+// Rows to a request from which a warp takes 16 rows instead of a CTA eight.
+constexpr uint64_t kAdTallRows = 16;
+
+// Parts that each tile's `rounds` stages are cut into: those that end first, where a CTA's beginning
+// and end take as long as so many stages and two CTAs are on an SM at a time.
+constexpr uint64_t kAdTallEnds = 12;
+uint64_t parts_for(uint64_t tiles, uint64_t rounds, uint64_t sms) {
+    const auto time = [&](uint64_t parts) { return ceil_div(tiles * parts, 2 * sms) * (ceil_div(rounds, parts) + kAdTallEnds); };
+    uint64_t best = 1;
+    for (uint64_t parts = 2; parts <= std::min<uint64_t>(rounds, 4 * sms); ++parts)
+        if (time(parts) < time(best)) best = parts;
+    return best;
+}
+
+// CTAs that the rows' tiles take: of all there can be, each request's last one and the padding's partial, or about.
+uint64_t tall_ctas(const plamo_paged_adapters_args *d, bool about) {
+    return ceil_div(about ? d->rows / kAdTall + d->requests / 2 : d->rows / kAdTall + std::min(d->requests, d->rows) + 2, kAdTileWarps);
+}
+
 AdaptersLayout adapters_layout(const plamo_cuda *c, const plamo_paged_adapters_args *d) {
     AdaptersLayout a{};
-    // Shares of the columns until there are four CTAs to an SM.
-    const uint64_t tiles = ceil_div(d->rows, kAdRows) * ceil_div(d->rank, 16), rounds = ceil_div(d->columns, kAdColumns);
-    const uint64_t want = std::min<uint64_t>(rounds, std::max<uint64_t>(1, 4ull * context_sms(c) / std::max<uint64_t>(1, tiles)));
-    a.share = static_cast<uint32_t>(ceil_div(rounds, want) * kAdColumns);
+    const uint64_t sms = context_sms(c), longest = 1ull << 34;  // row strides that a tensor map holds
+    a.tall = d->rows >= kAdTallRows * std::max<uint64_t>(1, d->requests) && d->rank <= kAdTallRank && d->x_stride < longest &&
+             d->base_stride < longest && d->out_stride < longest;
+    if (a.tall) {
+        const uint64_t round = 256 / element_bytes(d->x_type), rounds = ceil_div(d->columns, round);
+        a.share = static_cast<uint32_t>(ceil_div(rounds, parts_for(tall_ctas(d, true), rounds, sms)) * round);
+    } else {
+        // Shares of the columns until there are four CTAs to an SM.
+        const uint64_t tiles = ceil_div(d->rows, kAdRows) * ceil_div(d->rank, 16), rounds = ceil_div(d->columns, kAdColumns);
+        const uint64_t want = std::min<uint64_t>(rounds, std::max<uint64_t>(1, 4 * sms / std::max<uint64_t>(1, tiles)));
+        a.share = static_cast<uint32_t>(ceil_div(rounds, want) * kAdColumns);
+    }
     a.splits = static_cast<uint32_t>(ceil_div(d->columns, a.share));
     a.bytes = std::max<uint64_t>(256, static_cast<uint64_t>(a.splits) * d->rows * d->rank * 4);
     return a;
+}
+
+using AdapterTallInner = void (*)(CUtensorMap, AdapterParams);
+using AdapterTallOuter = void (*)(CUtensorMap, CUtensorMap, AdapterParams, int32_t);
+template <typename X>
+AdapterTallInner adapters_tall_inner(uint64_t rank) {
+    return rank <= 16   ? paged_adapters_tall_inner_kernel<X, 2>
+           : rank <= 32 ? paged_adapters_tall_inner_kernel<X, 4>
+           : rank <= 64 ? paged_adapters_tall_inner_kernel<X, 8>
+                        : paged_adapters_tall_inner_kernel<X, 16>;
+}
+template <typename T>
+AdapterTallOuter adapters_tall_outer(uint64_t rank) {
+    return rank <= 32   ? paged_adapters_tall_outer_kernel<T, 1>
+           : rank <= 64 ? paged_adapters_tall_outer_kernel<T, 2>
+                        : paged_adapters_tall_outer_kernel<T, 4>;
+}
+
+bool run_tall_adapters(plamo_cuda *c, const plamo_paged_adapters_args *d, const AdapterParams &p, cudaStream_t stream) {
+    const auto rows_map = [&](CUtensorMap *map, uint32_t type, const void *at, uint64_t width, uint64_t stride) {
+        const bool f32 = type == PLAMO_PAGED_FP32;
+        return tensor_map_2d(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, f32 ? 4 : 2, at, d->rows, width,
+                             f32 ? 32 : 64, kAdTall, stride);
+    };
+    CUtensorMap x_map, base_map, out_map;
+    if (!rows_map(&x_map, d->x_type, d->x, d->columns, d->x_stride) ||
+        !rows_map(&base_map, d->type, d->base, d->outputs, d->base_stride) ||
+        !rows_map(&out_map, d->type, d->out, d->outputs, d->out_stride))
+        return context_launched(c, "paged_adapters: tensor map", cudaErrorInvalidValue);
+    const uint64_t tiles = tall_ctas(d, false), sms = context_sms(c);
+    const AdapterTallInner inner = d->x_type == PLAMO_PAGED_FP32 ? adapters_tall_inner<float>(d->rank) : adapters_tall_inner<uint16_t>(d->rank);
+    const AdapterTallOuter outer = d->type == PLAMO_PAGED_FP32 ? adapters_tall_outer<float>(d->rank) : adapters_tall_outer<uint16_t>(d->rank);
+    const uint64_t blocks = ceil_div(d->outputs, 256 / element_bytes(d->type)), per = ceil_div(blocks, parts_for(tall_ctas(d, true), blocks, sms));
+    return launch(c, "paged_adapters inner", inner, dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(p.splits)), dim3(kAdTileThreads),
+                  kAdTileSmem, stream, false, x_map, p) &&
+           launch(c, "paged_adapters outer", outer, dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(ceil_div(blocks, per))),
+                  dim3(kAdTileThreads), kAdTileSmem, stream, true, base_map, out_map, p, static_cast<int32_t>(per));
+}
+
+bool run_adapters(plamo_cuda *c, const plamo_paged_adapters_args *d, const AdapterParams &p, cudaStream_t stream) {
+    const uint64_t tiles = ceil_div(d->rows, kAdRows), sms = context_sms(c);
+    const auto inner = d->x_type == PLAMO_PAGED_FP32 ? paged_adapters_inner_kernel<float> : paged_adapters_inner_kernel<uint16_t>;
+    const auto outer = d->type == PLAMO_PAGED_FP32 ? paged_adapters_outer_kernel<float> : paged_adapters_outer_kernel<uint16_t>;
+    // Outputs' blocks to a CTA: one while that takes four CTAs to an SM at most.
+    const uint64_t blocks = ceil_div(d->outputs, kAdOutputs), per = std::max<uint64_t>(1, tiles * blocks / (4 * sms));
+    return launch(c, "paged_adapters inner", inner,
+                  dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(p.splits), static_cast<uint32_t>(ceil_div(d->rank, 16))), dim3(kAdThreads), 0,
+                  stream, false, p) &&
+           launch(c, "paged_adapters outer", outer, dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(ceil_div(blocks, per))),
+                  dim3(kAdThreads), 0, stream, true, p, static_cast<int32_t>(per));
+}
+
+template <typename T>
+cudaError_t configure_adapters() {
+    cudaError_t e = cudaSuccess;
+    for (const uint64_t rank : {16, 32, 64, 128}) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(adapters_tall_inner<T>(rank), cudaFuncAttributeMaxDynamicSharedMemorySize, kAdTileSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(adapters_tall_outer<T>(rank), cudaFuncAttributeMaxDynamicSharedMemorySize, kAdTileSmem);
+    }
+    return e;
 }
 
 int attention(plamo_cuda *c, const plamo_paged_attention_args *d, const TreeMasks &t) {
@@ -339,6 +436,8 @@ cudaError_t paged_configure() {
     if (e == cudaSuccess) e = allow(paged_tree_tile_kernel, kTlSmem);
     if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<false>, kTfSmem);
     if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<true>, kTfSmem);
+    if (e == cudaSuccess) e = configure_adapters<float>();
+    if (e == cudaSuccess) e = configure_adapters<uint16_t>();
     return e;
 }
 }  // namespace plamo
@@ -599,22 +698,7 @@ int plamo_paged_adapters(struct plamo_cuda *c, const struct plamo_paged_adapters
     p.rank = static_cast<int32_t>(d->rank);
     p.splits = static_cast<int32_t>(a.splits);
     p.share = static_cast<int32_t>(a.share);
-    const uint32_t tiles = static_cast<uint32_t>(ceil_div(d->rows, kAdRows));
-    const dim3 inner(tiles, a.splits, static_cast<uint32_t>(ceil_div(d->rank, 16)));
-    if (!(d->x_type == PLAMO_PAGED_FP32
-              ? launch(c, "paged_adapters inner", paged_adapters_inner_kernel<float>, inner, dim3(kAdThreads), 0, stream, false, p)
-              : launch(c, "paged_adapters inner", paged_adapters_inner_kernel<uint16_t>, inner, dim3(kAdThreads), 0, stream, false, p)))
-        return -1;
-    // Outputs' blocks to a CTA: one while that takes four CTAs to an SM at most.
-    const uint64_t blocks = ceil_div(d->outputs, kAdOutputs);
-    const uint64_t per = std::max<uint64_t>(1, tiles * blocks / (4ull * context_sms(c)));
-    const dim3 outer(tiles, static_cast<uint32_t>(ceil_div(blocks, per)));
-    return (d->type == PLAMO_PAGED_FP32 ? launch(c, "paged_adapters outer", paged_adapters_outer_kernel<float>, outer, dim3(kAdThreads), 0,
-                                                 stream, true, p, static_cast<int32_t>(per))
-                                        : launch(c, "paged_adapters outer", paged_adapters_outer_kernel<uint16_t>, outer, dim3(kAdThreads), 0,
-                                                 stream, true, p, static_cast<int32_t>(per)))
-               ? 1
-               : -1;
+    return (a.tall ? run_tall_adapters(c, d, p, stream) : run_adapters(c, d, p, stream)) ? 1 : -1;
 }
 
 }  // extern "C"

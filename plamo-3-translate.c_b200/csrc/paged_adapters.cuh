@@ -24,20 +24,24 @@ constexpr int kAdRows = 8;       // to a tile: the N of one mma.sync
 constexpr int kAdWarps = 8, kAdThreads = 32 * kAdWarps;
 constexpr int kAdColumns = 64 * kAdWarps;  // a round of a CTA's warps
 
-// FP32 as BF16 terms whose sum is the value: the upper 16 bits, and twice the upper bits of what is
-// left. A value that is not finite is its first term alone (infinity less itself would be no number).
-__device__ __forceinline__ uint32_t ad_top(float v) {  // (a number's upper half may not turn a NaN into an infinity)
-    return v != v ? 0x7fff0000u : __float_as_uint(v) & 0xffff0000u;
-}
-__device__ __forceinline__ float ad_rest(float v, uint32_t top) { return isfinite(v) ? v - __uint_as_float(top) : 0.0f; }
+// Two FP32 numbers as BF16 terms whose sum is the number: the upper 16 bits, those of
+// what is left, and (of three) of what is left then, which is all. One that is not
+// finite is its first term alone, without a branch: infinity less itself is no number,
+// and the sum with zero keeps a NaN's upper half from being an infinity's.
 template <int TERMS>
 __device__ __forceinline__ void ad_split(float v0, float v1, uint32_t (&t)[TERMS]) {
+    v0 += 0.0f;
+    v1 += 0.0f;
 #pragma unroll
     for (int i = 0; i < TERMS; ++i) {
-        const uint32_t a = ad_top(v0), b = ad_top(v1);
+        const uint32_t a = __float_as_uint(v0), b = __float_as_uint(v1);
         t[i] = __byte_perm(a, b, 0x7632);
-        v0 = ad_rest(v0, a);
-        v1 = ad_rest(v1, b);
+        v0 -= __uint_as_float(a & 0xffff0000u);
+        v1 -= __uint_as_float(b & 0xffff0000u);
+        if (i == 0) {
+            v0 = v0 == v0 ? v0 : 0.0f;
+            v1 = v1 == v1 ? v1 : 0.0f;
+        }
     }
 }
 
@@ -235,6 +239,383 @@ __global__ void __launch_bounds__(kAdThreads) paged_adapters_outer_kernel(const 
             else *to = *from;
         }
     }
+}
+
+// ---- many rows to an adapter -----------------------------------------------------------------
+// A warp takes 16 rows of one request, now the M of its MMAs, and the adapter's rows are
+// their N. x (and base and out) come and go by the copy engine, 256 bytes of each row
+// at a time through a ring; two CTAs of 98 KB to an SM keep 190 KB on their way.
+// (Loads into registers, whose number bounds what is on its way, took 73 us for the
+// inner sums of 7,952 rows and rank 32, and 102 for the outputs.) The order along the
+// contraction is free, so lane t of four takes columns 8 t to 8 t + 7 of 32, whole
+// 16-byte pieces of a row. The adapter's pieces come from the L1 cache, which the
+// CTA's warps mostly share, a block or two ahead. HBM bounds both kernels up to ranks of
+// about 64: a row's bytes cover the products, which mma.sync makes fast enough
+// (tcgen05 would want the terms of x in shared memory, six bytes written and read for
+// each four that arrive).
+constexpr int kAdTall = 16, kAdBlock = 32;  // rows to a warp, columns or outputs at a time
+constexpr int kAdTallRank = 128;            // terms of h in registers: 3/4 of a register for each rank
+constexpr int kAdTileWarps = 4, kAdTileThreads = 32 * (kAdTileWarps + 1);
+// A stage: for each warp two boxes of 128 bytes of its rows.
+constexpr int kAdStages = 6, kAdBox = kAdTall * 128, kAdStage = 2 * kAdTileWarps * kAdBox;
+constexpr int kAdTileSmem = 1024 + kAdStages * kAdStage;
+template <typename X>
+__host__ __device__ constexpr int ad_box_columns() { return 128 / sizeof(X); }
+
+// Eight neighbouring columns of a row, and their terms by pairs.
+template <typename X>
+struct AdPiece;
+template <>
+struct AdPiece<float> {
+    float4 v[2];
+    // Block `block` of a row of the warp's boxes: eight columns of lane t.
+    __device__ __forceinline__ void load(const unsigned char *stage, int row, int block, int t) {
+        const unsigned char *at = stage + block * kAdBox + row * 128;
+        v[0] = *reinterpret_cast<const float4 *>(at + ((2 * t ^ (row & 7)) << 4));
+        v[1] = *reinterpret_cast<const float4 *>(at + (((2 * t + 1) ^ (row & 7)) << 4));
+    }
+    template <int TERMS>
+    __device__ __forceinline__ void split(uint32_t (&t)[4][TERMS]) const {
+        ad_split<TERMS>(v[0].x, v[0].y, t[0]);
+        ad_split<TERMS>(v[0].z, v[0].w, t[1]);
+        ad_split<TERMS>(v[1].x, v[1].y, t[2]);
+        ad_split<TERMS>(v[1].z, v[1].w, t[3]);
+    }
+    __device__ __forceinline__ void add(const float (&s)[8]) {
+        v[0] = make_float4(v[0].x + s[0], v[0].y + s[1], v[0].z + s[2], v[0].w + s[3]);
+        v[1] = make_float4(v[1].x + s[4], v[1].y + s[5], v[1].z + s[6], v[1].w + s[7]);
+    }
+    __device__ __forceinline__ void store(unsigned char *stage, int row, int block, int t) const {
+        unsigned char *at = stage + block * kAdBox + row * 128;
+        *reinterpret_cast<float4 *>(at + ((2 * t ^ (row & 7)) << 4)) = v[0];
+        *reinterpret_cast<float4 *>(at + (((2 * t + 1) ^ (row & 7)) << 4)) = v[1];
+    }
+};
+template <>
+struct AdPiece<uint16_t> {
+    uint4 v;
+    __device__ __forceinline__ void load(const unsigned char *stage, int row, int block, int t) {
+        v = *reinterpret_cast<const uint4 *>(stage + (block >> 1) * kAdBox + row * 128 + (((4 * (block & 1) + t) ^ (row & 7)) << 4));
+    }
+    template <int TERMS>
+    __device__ __forceinline__ void split(uint32_t (&t)[4][TERMS]) const {  // one term is the number
+        t[0][0] = v.x, t[1][0] = v.y, t[2][0] = v.z, t[3][0] = v.w;
+    }
+    __device__ __forceinline__ void add(const float (&s)[8]) {
+        v = make_uint4(pg_pack(bf16_lo(v.x) + s[0], bf16_hi(v.x) + s[1]), pg_pack(bf16_lo(v.y) + s[2], bf16_hi(v.y) + s[3]),
+                       pg_pack(bf16_lo(v.z) + s[4], bf16_hi(v.z) + s[5]), pg_pack(bf16_lo(v.w) + s[6], bf16_hi(v.w) + s[7]));
+    }
+    __device__ __forceinline__ void store(unsigned char *stage, int row, int block, int t) const {
+        *reinterpret_cast<uint4 *>(stage + (block >> 1) * kAdBox + row * 128 + (((4 * (block & 1) + t) ^ (row & 7)) << 4)) = v;
+    }
+};
+
+// Rows of one request, or of none, that a warp takes.
+struct AdTile {
+    int32_t row0, rows, id;  // rows 0: no work
+};
+// The CTA's four: every request's rows by sixteens, in order, and the rows before the
+// first request's and behind the last one's. Rows without an adapter are left out
+// unless `copied`. Each CTA finds its own, a few loads to a thread and a scan.
+__device__ __forceinline__ void ad_tiles(const AdapterParams &p, bool copied, AdTile *tiles) {
+    __shared__ int64_t sums[kAdTileThreads / 32];
+    const int tid = threadIdx.x;
+    if (tid < kAdTileWarps) tiles[tid].rows = 0;
+    const int32_t all = p.requests + 2, per = (all + kAdTileThreads - 1) / kAdTileThreads;
+    const int32_t e0 = min(all, tid * per), e1 = min(all, e0 + per);
+    const auto entry = [&](int32_t e) {  // entry 0: before the requests; the last: behind them
+        const int32_t from = e ? min(max(p.starts[e - 1], 0), p.rows) : 0;
+        const int32_t to = e <= p.requests ? min(max(p.starts[e], from), p.rows) : p.rows;
+        AdTile t{from, to - from, e && e <= p.requests ? p.ids[e - 1] : -1};
+        if (t.id < -1 || t.id >= p.adapters) {
+            if (t.rows) pg_flag(p.status, PLAMO_PAGED_ADAPTER);
+            t.id = -1;
+        }
+        if (t.id < 0 && !copied) t.rows = 0;
+        return t;
+    };
+    int64_t count = 0, total;
+#pragma unroll 1
+    for (int32_t e = e0; e < e1; ++e) count += (entry(e).rows + kAdTall - 1) / kAdTall;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kAdTileWarps;
+    int64_t at = pg_block_scan<kAdTileThreads>(count, sums, &total);
+#pragma unroll 1
+    for (int32_t e = e0; e < e1 && at < first + kAdTileWarps; ++e) {
+        const AdTile t = entry(e);
+        const int32_t n = (t.rows + kAdTall - 1) / kAdTall;
+        for (int64_t k = max(first, at); k < min(first + kAdTileWarps, at + n); ++k) {
+            const int32_t skip = static_cast<int32_t>(k - at) * kAdTall;
+            tiles[k - first] = AdTile{t.row0 + skip, min(kAdTall, t.rows - skip), t.id};
+        }
+        at += n;
+    }
+    __syncthreads();
+}
+
+// A wait that ends when the phase completes, or after about two seconds (the clock is slow to read).
+__device__ __forceinline__ bool ad_wait(uint64_t *bar, uint32_t parity) {
+    uint64_t start = 0;
+    for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n) {
+        if (n % 64) continue;
+        const uint64_t now = global_ns();
+        if (!start) start = now;
+        if (now - start > 2000000000ull) return false;
+    }
+    return true;
+}
+struct AdRing {
+    uint64_t *full, *empty;
+    unsigned char *stages;
+};
+__device__ __forceinline__ AdRing ad_ring(unsigned char *smem, uint64_t *full, uint64_t *empty, const CUtensorMap *map) {
+    AdRing r{full, empty, reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~static_cast<uintptr_t>(1023))};
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kAdStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], kAdTileWarps);
+        }
+        fence_barrier_init();
+        prefetch_tensormap(map);
+    }
+    return r;  // (the tiles' barrier is behind it)
+}
+// The copying warp's lane: `count` stages of the tiles' rows, columns from `column` on.
+template <typename X>
+__device__ __forceinline__ void ad_copy(const AdapterParams &p, const AdRing &r, const CUtensorMap *map, const AdTile *tiles, int32_t column, int32_t count) {
+    constexpr int BOX = ad_box_columns<X>();
+    int32_t n = 0, used = 0;
+    for (int w = 0; w < kAdTileWarps; ++w) used += tiles[w].rows > 0;
+    for (; n < count; ++n) {
+        const int st = n % kAdStages;
+        if (n >= kAdStages && !ad_wait(&r.empty[st], (n / kAdStages - 1) & 1u)) {
+            pg_flag(p.status, PLAMO_PAGED_FAILED);
+            break;
+        }
+        mbar_expect_tx(&r.full[st], used * 2 * kAdBox);
+        for (int w = 0; w < kAdTileWarps; ++w) {
+            if (!tiles[w].rows) continue;
+            unsigned char *to = r.stages + st * kAdStage + 2 * w * kAdBox;
+            tma_load_2d(to, map, column + 2 * BOX * n, tiles[w].row0, &r.full[st]);
+            tma_load_2d(to + kAdBox, map, column + 2 * BOX * n + BOX, tiles[w].row0, &r.full[st]);
+        }
+    }
+    // Every copy issued has landed before the CTA can exit.
+    for (int32_t k = max(0, n - kAdStages); k < n; ++k)
+        if (!ad_wait(&r.full[k % kAdStages], (k / kAdStages) & 1u)) break;
+}
+
+// x: the tiles' rows by a share of the columns; ranks to a CTA: 8 NT.
+template <typename X, int NT>
+__global__ void __launch_bounds__(kAdTileThreads, 2)
+    paged_adapters_tall_inner_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ AdapterParams p) {
+    constexpr int TERMS = sizeof(X) == 4 ? 3 : 1, COLUMNS = 2 * ad_box_columns<X>(), BLOCKS = COLUMNS / kAdBlock;  // to a stage
+    constexpr int WIDE = NT <= 8 ? NT : 8;  // tiles of the adapter loaded at a time
+    constexpr int AHEAD = NT <= 4 ? 2 : 1;  // so many ahead
+    extern __shared__ __align__(128) unsigned char ad_smem[];
+    __shared__ __align__(8) uint64_t full[kAdStages], empty[kAdStages];
+    __shared__ AdTile tiles[kAdTileWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    pdl_launch_dependents();
+    const AdRing ring = ad_ring(ad_smem, full, empty, &map);
+    ad_tiles(p, false, tiles);
+    if (!tiles[0].rows) return;
+    const int32_t begin = blockIdx.y * p.share, end = min(begin + p.share, p.columns);
+    const int32_t stages = (end - begin + COLUMNS - 1) / COLUMNS;
+    if (warp == kAdTileWarps) {
+        if (lane == 0) ad_copy<X>(p, ring, &map, tiles, begin, stages);
+        return;
+    }
+    const AdTile tile = tiles[warp];
+    const bool there = tile.rows > 0;
+    const uint16_t *const a = p.a + (static_cast<uint64_t>(max(tile.id, 0)) * p.rank + g) * p.columns + 8 * t;
+    uint4 w[AHEAD][WIDE];
+    const auto fetch = [&](int32_t c, int j0, uint4 (&w)[WIDE]) {  // columns c + 8 t of adapter rows 8 (j0 + j) + g
+        const bool in = there && c + 8 * t < end;
+#pragma unroll
+        for (int j = 0; j < WIDE; ++j)
+            w[j] = in && 8 * (j0 + j) + g < p.rank ? *reinterpret_cast<const uint4 *>(a + static_cast<uint64_t>(8 * (j0 + j)) * p.columns + c)
+                                                   : make_uint4(0, 0, 0, 0);
+    };
+    float s[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[j][k] = 0.0f;
+#pragma unroll
+    for (int y = 0; y < AHEAD; ++y) fetch(begin + y * kAdBlock, 0, w[y]);
+#pragma unroll 1
+    for (int32_t n = 0; n < stages; ++n) {
+        const int st = n % kAdStages;
+        if (!__all_sync(0xffffffffu, ad_wait(&ring.full[st], (n / kAdStages) & 1u))) {
+            if (lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
+            break;
+        }
+        AdPiece<X> v[BLOCKS][2];
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[b][i].load(ring.stages + st * kAdStage + 2 * warp * kAdBox, g + 8 * i, b, t);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ring.empty[st]);
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            const int32_t c = begin + (n * BLOCKS + b) * kAdBlock;
+            uint32_t f0[4][TERMS], f1[4][TERMS];  // pairs of columns of rows g and g + 8
+            v[b][0].split(f0);
+            v[b][1].split(f1);
+#pragma unroll
+            for (int j0 = 0; j0 < NT; j0 += WIDE) {
+                uint4 u[WIDE];
+#pragma unroll
+                for (int j = 0; j < WIDE; ++j) u[j] = w[b % AHEAD][j];
+                fetch(j0 + WIDE < NT ? c : c + AHEAD * kAdBlock, j0 + WIDE < NT ? j0 + WIDE : 0, w[b % AHEAD]);  // the next ones
+#pragma unroll
+                for (int j = 0; j < WIDE; ++j)
+#pragma unroll
+                    for (int term = TERMS - 1; term >= 0; --term) {
+                        const uint32_t m0[4] = {f0[0][term], f1[0][term], f0[1][term], f1[1][term]};
+                        const uint32_t m1[4] = {f0[2][term], f1[2][term], f0[3][term], f1[3][term]};
+                        mma_bf16(s[j0 + j], m0, u[j].x, u[j].y);
+                        mma_bf16(s[j0 + j], m1, u[j].z, u[j].w);
+                    }
+            }
+        }
+    }
+    float *to = p.inner + (static_cast<uint64_t>(blockIdx.y) * p.rows + tile.row0 + g) * p.rank + 2 * t;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        if (8 * j >= p.rank) break;
+        if (g < tile.rows) *reinterpret_cast<float2 *>(to + 8 * j) = make_float2(s[j][0], s[j][1]);
+        if (g + 8 < tile.rows) *reinterpret_cast<float2 *>(to + 8ull * p.rank + 8 * j) = make_float2(s[j][2], s[j][3]);
+    }
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int x, int y, const void *src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(src))
+                 : "memory");
+}
+
+// The tiles' rows by `per` stages of outputs, added to base in the ring and sent off. Tile j
+// of four has outputs 8 t + 2 j and 8 t + 2 j + 1 of lane t, so that a lane's sums are
+// eight neighbouring outputs of two rows.
+template <typename T, int RANKS>  // blocks of 32 ranks
+__global__ void __launch_bounds__(kAdTileThreads, 2)
+    paged_adapters_tall_outer_kernel(const __grid_constant__ CUtensorMap base_map, const __grid_constant__ CUtensorMap out_map,
+                                     const __grid_constant__ AdapterParams p, int32_t per) {
+    constexpr int BOX = ad_box_columns<T>(), COLUMNS = 2 * BOX, BLOCKS = COLUMNS / kAdBlock, PIECE = 16 / static_cast<int>(sizeof(T));
+    extern __shared__ __align__(128) unsigned char ad_smem[];
+    __shared__ __align__(8) uint64_t full[kAdStages], empty[kAdStages];
+    __shared__ AdTile tiles[kAdTileWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const AdRing ring = ad_ring(ad_smem, full, empty, &base_map);
+    ad_tiles(p, p.out != p.base, tiles);
+    if (!tiles[0].rows) return;
+    const int32_t all = (p.outputs + COLUMNS - 1) / COLUMNS, first_stage = blockIdx.y * per, stages = min(per, all - first_stage);
+    if (warp == kAdTileWarps) {
+        // (base was there before the launch that this one waits for)
+        if (lane == 0) ad_copy<T>(p, ring, &base_map, tiles, first_stage * COLUMNS, stages);
+        return;
+    }
+    const AdTile tile = tiles[warp];
+    const bool there = tile.rows > 0 && tile.id >= 0;
+    uint4 w[4][RANKS];
+    const auto fetch = [&](int32_t n0) {  // ranks 8 t of B's rows for tile j, column g
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int32_t row = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+            const uint16_t *from = p.b + (static_cast<uint64_t>(max(tile.id, 0)) * p.outputs + row) * p.rank + 8 * t;
+#pragma unroll
+            for (int b = 0; b < RANKS; ++b)
+                w[j][b] = there && row < p.outputs && kAdBlock * b + 8 * t < p.rank ? *reinterpret_cast<const uint4 *>(from + kAdBlock * b)
+                                                                                    : make_uint4(0, 0, 0, 0);
+        }
+    };
+    fetch(first_stage * COLUMNS);
+    pdl_wait();
+    uint32_t h[RANKS][4][2][3];  // terms of scale * h: [block][pair of ranks][row g or g + 8]
+#pragma unroll
+    for (int b = 0; b < RANKS; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+            if (there && g + 8 * i < tile.rows && kAdBlock * b + 8 * t < p.rank) {
+                const float *from = p.inner + static_cast<uint64_t>(tile.row0 + g + 8 * i) * p.rank + kAdBlock * b + 8 * t;
+#pragma unroll 4
+                for (int32_t y = 0; y < p.splits; ++y) {
+                    const float4 c = ld4(from + static_cast<uint64_t>(y) * p.rows * p.rank), d = ld4(from + static_cast<uint64_t>(y) * p.rows * p.rank + 4);
+                    u = make_float4(u.x + c.x, u.y + c.y, u.z + c.z, u.w + c.w);
+                    v = make_float4(v.x + d.x, v.y + d.y, v.z + d.z, v.w + d.w);
+                }
+                const float scale = p.scales ? p.scales[tile.id] : 1.0f;
+                u = make_float4(u.x * scale, u.y * scale, u.z * scale, u.w * scale);
+                v = make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+            }
+            ad_split<3>(u.x, u.y, h[b][0][i]);
+            ad_split<3>(u.z, u.w, h[b][1][i]);
+            ad_split<3>(v.x, v.y, h[b][2][i]);
+            ad_split<3>(v.z, v.w, h[b][3][i]);
+        }
+#pragma unroll 1
+    for (int32_t n = 0; n < stages; ++n) {
+        const int st = n % kAdStages;
+        unsigned char *const boxes = ring.stages + st * kAdStage + 2 * warp * kAdBox;
+        if (!__all_sync(0xffffffffu, ad_wait(&ring.full[st], (n / kAdStages) & 1u))) {
+            if (lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
+            break;
+        }
+        const int32_t column = (first_stage + n) * COLUMNS;
+#pragma unroll 1
+        for (int b = 0; there && b < BLOCKS; ++b) {
+            float s[2][8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < RANKS; ++k)
+#pragma unroll
+                    for (int term = 2; term >= 0; --term) {
+                        const uint32_t m0[4] = {h[k][0][0][term], h[k][0][1][term], h[k][1][0][term], h[k][1][1][term]};
+                        const uint32_t m1[4] = {h[k][2][0][term], h[k][2][1][term], h[k][3][0][term], h[k][3][1][term]};
+                        mma_bf16(d, m0, w[j][k].x, w[j][k].y);
+                        mma_bf16(d, m1, w[j][k].z, w[j][k].w);
+                    }
+                s[0][2 * j] = d[0], s[0][2 * j + 1] = d[1];
+                s[1][2 * j] = d[2], s[1][2 * j + 1] = d[3];
+            }
+            fetch(column + (b + 1) * kAdBlock);  // the next block's
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                AdPiece<T> v;
+                v.load(boxes, g + 8 * i, b, t);
+                v.add(s[i]);
+                v.store(boxes, g + 8 * i, b, t);
+            }
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (tile.rows == kAdTall && lane == 0) {
+            tma_store_2d(&out_map, column, tile.row0, boxes);
+            if (column + BOX < p.outputs) tma_store_2d(&out_map, column + BOX, tile.row0, boxes + kAdBox);
+        } else if (tile.rows < kAdTall) {
+            // The box's other rows are another warp's: row by row, 16 bytes a lane.
+#pragma unroll 1
+            for (int x = lane; x < tile.rows * 16; x += 32) {
+                const int row = x >> 4, box = (x >> 3) & 1, chunk = x & 7;
+                const int32_t n0 = column + box * BOX + chunk * PIECE;
+                if (n0 < p.outputs)
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + (tile.row0 + row) * p.out_stride + n0) =
+                        *reinterpret_cast<const uint4 *>(boxes + box * kAdBox + row * 128 + ((chunk ^ (row & 7)) << 4));
+            }
+            __syncwarp();
+        }
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            // The stage before has left shared memory.
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            if (n) mbar_arrive(&ring.empty[(n - 1) % kAdStages]);
+        }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 }  // namespace plamo

@@ -74,6 +74,7 @@ struct PagedAttnParams {
     int32_t split_pairs;  // of tiles whose two halves take alternate steps, at most
     int32_t step_units;   // units of a step of other tiles (of theirs: 1)
     int32_t strip_pad;    // units that a strip's beginning and end are worth
+    int32_t least_units;  // to a CTA, 2 * step_units at least: each but a strip's first then owns a step
 };
 enum { kTlShortRows, kTlTiles, kTlPreTiles, kTlCtas, kTlRun, kTlLonger, kTlFirst, kTlTaken, kRtRun, kRtLonger, kTlHeader };
 // Requests of up to so many pairs keep their own rows in the row kernel and share
@@ -176,7 +177,6 @@ __device__ __forceinline__ Runs row_runs(const PagedAttnParams &p) { return Runs
 
 // A tree's strip: units that stand for its beginning and end, then those of its
 // steps. A CTA has the steps whose first unit is in its run.
-constexpr int kTreeMinUnits = 4;
 struct StripUnits {
     int32_t pad, per_step, steps;
     __device__ __forceinline__ int32_t unit_of(int32_t step) const { return pad + step * per_step; }

@@ -177,8 +177,7 @@ __device__ void paged_schedule(const PagedAttnParams &p, int64_t *sums) {
         p.header[kTlTaken] = fits ? min(max(taken, 0), p.rows) : 0;
         p.header[kTlShortRows] = fits ? all_short : 0;
         const int32_t units = fits ? static_cast<int32_t>(total * p.kh) : 0;
-        // (a tree's CTA has more units than a step costs: each but a strip's first owns a step)
-        const int32_t least = TREE ? max(units / kTreeMinUnits, units > 0) : (units + kTlMinUnits - 1) / kTlMinUnits;
+        const int32_t least = TREE ? max(units / p.least_units, units > 0) : (units + kTlMinUnits - 1) / kTlMinUnits;
         const int32_t ctas = p.tile_rows ? min(p.tile_grid, least) : 0;
         p.header[kTlCtas] = ctas;
         p.header[kTlRun] = ctas ? units / ctas : 1;

@@ -19,9 +19,8 @@ namespace plamo {
 //    rows, so their ends count. The copying warp walks the work and tells the others
 //    what comes next through shared memory. The rows of all tiles follow one another
 //    in the batch, so that it can copy a tile's queries, too, as a box, which arrive
-//    under the last softmax of the strip before. Sums leave tensor memory for global
-//    memory 32 bytes at a time. And strips count as longer than their steps where the
-//    work is divided.
+//    under the last softmax of the strip before. Sums go from tensor memory straight to
+//    global memory. And strips count as longer than their steps where the work is divided.
 //  - A warp to a half issues its products, converged, with a lane elected for each
 //    instruction: from a branch of one lane an MMA took 55 cycles to issue, and one
 //    warp for both halves left the tensor pipe waiting for half of the time.
@@ -81,6 +80,45 @@ __device__ __forceinline__ void mbar_arrive_count(uint64_t *bar, uint32_t count)
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
 __device__ __noinline__ bool ts_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up) { return tl_wait(bar, parity, gave_up); }
+// Two FP32 numbers to a register pair, and instructions that take both.
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float low_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+// The 4 x 4 transpose, over the lanes of each four, of blocks of eight numbers: lane j's block y becomes
+// lane y's block j.
+__device__ __forceinline__ void transpose_blocks(uint32_t (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int bit = 2; bit >= 1; bit >>= 1) {
+        const bool high = lane & bit;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            if (y & bit) continue;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {  // block y | bit of the low lane against block y of the high one
+                const uint32_t lo = v[8 * y + k], hi = v[8 * (y | bit) + k];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? lo : hi, bit);
+                v[8 * y + k] = high ? got : lo;
+                v[8 * (y | bit) + k] = high ? hi : got;
+            }
+        }
+    }
+}
 __device__ __forceinline__ void store_256(float *to, const uint32_t *v) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
                  "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -493,22 +531,27 @@ __global__ void __launch_bounds__(kTsThreads, 1)
                         }
                     }
                     const float shift = m == -INFINITY ? 0.0f : -m;
-                    float l0 = 0.0f, l1 = 0.0f;
+                    const uint64_t scale_pair = pair_of(scale2, scale2), shift_pair = pair_of(shift, shift);
+                    uint64_t sums = pair_of(0.0f, 0.0f);
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {
                         uint32_t first[16], rest[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            const float a = pg_exp2(fmaf(__uint_as_float(x[32 * part + 2 * k]), scale2, shift));
-                            const float b = pg_exp2(fmaf(__uint_as_float(x[32 * part + 2 * k + 1]), scale2, shift));
-                            l0 += a;
-                            l1 += b;
-                            pg_split(a, b, first[k], rest[k]);
+                            const uint64_t y2 = fma_pair(pair_of(x[32 * part + 2 * k], x[32 * part + 2 * k + 1]), scale_pair, shift_pair);
+                            const uint32_t a = __float_as_uint(pg_exp2(low_of(y2))), b = __float_as_uint(pg_exp2(high_of(y2)));
+                            const uint64_t e = pair_of(a, b);
+                            sums = add_pair(sums, e);
+                            // As pg_split; the weights are not negative.
+                            const uint64_t less = pair_of((a & 0xffff0000u) | 0x80000000u, (b & 0xffff0000u) | 0x80000000u);
+                            const uint64_t left = fma_pair(e, pair_of(1.0f + 0x1p-22f, 1.0f + 0x1p-22f), less);
+                            first[k] = __byte_perm(a, b, 0x7632);
+                            rest[k] = pg_pack(low_of(left), high_of(left));
                         }
                         tmem_st16(scol + 64 * h + 16 * part, first);
                         tmem_st16(scol + 64 * h + 32 + 16 * part, rest);
                     }
-                    l += l0 + l1;
+                    l += low_of(sums) + high_of(sums);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -533,8 +576,7 @@ __global__ void __launch_bounds__(kTsThreads, 1)
                     uint32_t o[32];
                     tmem_ld32_async(ocol + c, o);
                     tmem_wait_ld();
-                    if (!there) continue;
-                    if (odd) {
+                    if (odd && there) {
                         float with[32];
 #pragma unroll
                         for (int k = 0; k < 32; ++k) with[k] = __uint_as_float(o[k]);
@@ -543,6 +585,7 @@ __global__ void __launch_bounds__(kTsThreads, 1)
                         for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(with[k]);
                     }
                     if (whole) {
+                        if (!there) continue;
                         uint16_t *to = static_cast<uint16_t *>(p.out) + row * p.out_stride + head * kPgDim + c;
 #pragma unroll
                         for (int k = 0; k < 32; k += 8) {
@@ -552,8 +595,12 @@ __global__ void __launch_bounds__(kTsThreads, 1)
                             *reinterpret_cast<uint4 *>(to + k) = make_uint4(b[0], b[1], b[2], b[3]);
                         }
                     } else {
+                        // Four lanes write 128 bytes of one row at a time: a line is written once.
+                        transpose_blocks(o);
+                        float *to = p.tile_sum + (place - (lane & 3)) * kPgDim + c + 8 * (lane & 3);
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) store_256(p.tile_sum + place * kPgDim + c + k, o + k);
+                        for (int y = 0; y < 4; ++y)
+                            if (pair - (lane & 3) + y < t.pairs) store_256(to + y * kPgDim, o + 8 * y);
                     }
                 }
                 tc_fence_before();
