@@ -247,7 +247,8 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
     const uint64_t eights = d->rows * ceil_div(d->query_heads, 8);
     const auto join = twos <= 2 * sms     ? paged_join_kernel<F32, 2, true, TREE>
                       : eights <= 4 * sms ? paged_join_kernel<F32, 8, true, TREE>
-                                          : paged_join_kernel<F32, 8, false, TREE>;
+                      : TREE              ? paged_tree_join_kernel<F32>
+                                          : paged_join_kernel<F32, 8, false, false>;
     const uint64_t blocks = std::min(4 * sms, std::max<uint64_t>(a.tile_rows ? 4 * sms : 1, twos <= 2 * sms ? twos : eights));
     return launch(c, "paged_attention join", join, dim3(static_cast<uint32_t>(blocks)), dim3(kJoinThreads), 0, stream, true, p);
 }
@@ -300,17 +301,27 @@ struct AdaptersLayout {
     bool tall;  // 16 rows to a warp
     uint64_t bytes;
 };
-// Rows to a request from which a warp takes 16 rows instead of a CTA eight.
-constexpr uint64_t kAdTallRows = 16;
+// Where a warp takes 16 rows of one request instead of a CTA eight of any: requests of that many
+// rows, and enough of them. FP32, rank 16: 16 requests of 24 rows 19 us so and 20 the other
+// way, 64 of 16 27 and 39; BF16, rank 64: 32 of 16 28 and 33, 8 of 16 25 and 19; rank 128 holds
+// more in registers than it hides: 32 of 16 60 and 51, 16 of 500 426 and 874.
+constexpr uint64_t kAdTallRows = 12, kAdTallAll = 384, kAdTallAllWide = 1024;
 
-// Parts that each tile's `rounds` stages are cut into: those that end first, where a CTA's beginning
-// and end take as long as so many stages and two CTAs are on an SM at a time.
-constexpr uint64_t kAdTallEnds = 12;
+// Parts that the `rounds` stages of each of `tiles` CTAs' work are cut into: those that end
+// first, of the most that one, two, three or four rounds of CTAs hold, two to an SM. A
+// CTA's beginning and end take about as long as six stages, and many parts' inner sums
+// as long to add up.
+constexpr uint64_t kAdTallEnds = 6, kAdMostParts = 16;
 uint64_t parts_for(uint64_t tiles, uint64_t rounds, uint64_t sms) {
-    const auto time = [&](uint64_t parts) { return ceil_div(tiles * parts, 2 * sms) * (ceil_div(rounds, parts) + kAdTallEnds); };
-    uint64_t best = 1;
-    for (uint64_t parts = 2; parts <= std::min<uint64_t>(rounds, 4 * sms); ++parts)
-        if (time(parts) < time(best)) best = parts;
+    uint64_t best = 1, least = ~0ull;
+    for (uint64_t turn = 1; turn <= 4; ++turn) {
+        const uint64_t parts = std::clamp<uint64_t>(turn * 2 * sms / std::max<uint64_t>(1, tiles), 1, std::min(rounds, kAdMostParts));
+        const uint64_t time = ceil_div(tiles * parts, 2 * sms) * (ceil_div(rounds, parts) + kAdTallEnds);
+        if (time < least) {
+            least = time;
+            best = parts;
+        }
+    }
     return best;
 }
 
@@ -322,7 +333,7 @@ uint64_t tall_ctas(const plamo_paged_adapters_args *d, bool about) {
 AdaptersLayout adapters_layout(const plamo_cuda *c, const plamo_paged_adapters_args *d) {
     AdaptersLayout a{};
     const uint64_t sms = context_sms(c), longest = 1ull << 34;  // row strides that a tensor map holds
-    a.tall = d->rows >= kAdTallRows * std::max<uint64_t>(1, d->requests) && d->rank <= kAdTallRank && d->x_stride < longest &&
+    a.tall = d->rows >= kAdTallRows * d->requests && d->rows >= (d->rank <= 64 ? kAdTallAll : kAdTallAllWide) && d->rank <= kAdTallRank && d->x_stride < longest &&
              d->base_stride < longest && d->out_stride < longest;
     if (a.tall) {
         const uint64_t round = 256 / element_bytes(d->x_type), rounds = ceil_div(d->columns, round);

@@ -518,19 +518,21 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
     }
     const AdTile tile = tiles[warp];
     const bool there = tile.rows > 0 && tile.id >= 0;
-    uint4 w[4][RANKS];
-    const auto fetch = [&](int32_t n0) {  // ranks 8 t of B's rows for tile j, column g
+    // So many blocks' pieces of the adapter are on their way; none where h takes the registers.
+    constexpr int AHEAD = RANKS == 1 ? 2 : RANKS == 2 ? 1 : 0, STEP = AHEAD ? AHEAD : 1;
+    uint4 ahead[STEP][4][RANKS];
+    const auto fetch = [&](int32_t n0, int j, uint4 (&w)[RANKS]) {  // ranks 8 t of B's rows for tile j, column g
+        const int32_t row = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+        const uint16_t *from = p.b + (static_cast<uint64_t>(max(tile.id, 0)) * p.outputs + row) * p.rank + 8 * t;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int32_t row = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
-            const uint16_t *from = p.b + (static_cast<uint64_t>(max(tile.id, 0)) * p.outputs + row) * p.rank + 8 * t;
-#pragma unroll
-            for (int b = 0; b < RANKS; ++b)
-                w[j][b] = there && row < p.outputs && kAdBlock * b + 8 * t < p.rank ? *reinterpret_cast<const uint4 *>(from + kAdBlock * b)
-                                                                                    : make_uint4(0, 0, 0, 0);
-        }
+        for (int b = 0; b < RANKS; ++b)
+            w[b] = there && row < p.outputs && kAdBlock * b + 8 * t < p.rank ? *reinterpret_cast<const uint4 *>(from + kAdBlock * b)
+                                                                             : make_uint4(0, 0, 0, 0);
     };
-    fetch(first_stage * COLUMNS);
+#pragma unroll
+    for (int y = 0; y < AHEAD; ++y)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fetch(first_stage * COLUMNS + y * kAdBlock, j, ahead[y][j]);
     pdl_wait();
     uint32_t h[RANKS][4][2][3];  // terms of scale * h: [block][pair of ranks][row g or g + 8]
 #pragma unroll
@@ -565,10 +567,23 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
         }
         const int32_t column = (first_stage + n) * COLUMNS;
 #pragma unroll 1
-        for (int b = 0; there && b < BLOCKS; ++b) {
+        for (int b0 = 0; there && b0 < BLOCKS; b0 += STEP)
+#pragma unroll
+        for (int y = 0; y < STEP; ++y) {
+            const int b = b0 + y;
             float s[2][8];
+            uint4 w[4][RANKS];
+            if constexpr (AHEAD > 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int k = 0; k < RANKS; ++k) w[j][k] = ahead[y][j][k];
+                    fetch(column + (b + AHEAD) * kAdBlock, j, ahead[y][j]);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if constexpr (AHEAD == 0) fetch(column + b * kAdBlock, j, w[j]);
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < RANKS; ++k)
@@ -582,7 +597,6 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
                 s[0][2 * j] = d[0], s[0][2 * j + 1] = d[1];
                 s[1][2 * j] = d[2], s[1][2 * j + 1] = d[3];
             }
-            fetch(column + (b + 1) * kAdBlock);  // the next block's
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 AdPiece<T> v;

@@ -1226,4 +1226,110 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
             for (int32_t i = 0; i < p.tile_shape[tile].rows; ++i) clear(p.tile_shape[tile].row0 + i);
 }
 
+// The join of draft trees' rows when there are many, a warp to eight results of a row:
+// lane y's list is that of result y % 8. A part's sums are loaded beside its {m, l},
+// not behind them, and the next row's entry beside this one's parts: what is in the list,
+// the tiles' units and the parts depend on one another, and each load takes as long as
+// adding up a part. (The plain join takes 33 us for the 61 trees of up to 32 rows behind 4,097,
+// 97 for 64 of up to 64 behind 8,192.)
+template <bool F32>
+__global__ void __launch_bounds__(kJoinThreads, 3) paged_tree_join_kernel(const __grid_constant__ PagedAttnParams p) {
+    const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    const int32_t pre_tiles = p.tile_rows ? p.header[kTlPreTiles] : 0, ctas = p.tile_rows ? p.header[kTlCtas] : 0;
+    const int32_t first_row = p.header[kTlFirst], end_row = p.header[kTlTaken];
+    const Runs runs = tile_runs(p), of_rows = row_runs(p);
+    const int32_t groups = (p.qh + 7) / 8, items = p.header[kTlShortRows] * groups, step = gridDim.x * kJoinWarps;
+    int32_t n = blockIdx.x * kJoinWarps + warp;
+    int4 coming = n < items ? p.short_list[n / groups] : int4{};
+#pragma unroll 1
+    for (; n < items; n += step) {
+        const int32_t listed = n / groups, head0 = 8 * (n - listed * groups), head = min(head0 + (lane & 7), p.qh - 1);
+        const int4 e = coming;
+        if (n + step < items) coming = p.short_list[(n + step) / groups];
+        const int32_t kv = p.by_group.div(head), in_group = head - kv * p.group;
+        // The parts of row tile m / kRtPairs of request r (or of the prefix), and of place `at` of a tile, for this head.
+        const auto row_parts = [&](int32_t r, int32_t m) {
+            const int4 rec = p.row_record[r];
+            const int32_t strip = m / kRtPairs * p.kh + kv, u0 = rec.x + strip * rec.y;
+            const int32_t c0 = rec.y ? of_rows.cta_of(u0) : 0;
+            return PartList{p.row_sum, p.row_ml, c0 + rec.z + strip, 1, kRtPairs, m % kRtPairs, rec.y ? of_rows.cta_of(u0 + rec.y - 1) - c0 + 1 : 0, 0};
+        };
+        const auto tile_parts = [&](int32_t tile, int32_t at) {
+            const int32_t unit = p.tile_unit[tile], length = static_cast<int32_t>(p.tile_unit[tile + 1]) - unit;
+            if (!length) return PartList{};
+            const StripUnits strip = strip_units(p, tile, length);
+            const int32_t u0 = unit * p.kh + kv * length;
+            const int32_t c0 = runs.cta_of(u0 + strip.unit_of(0)), c1 = runs.cta_of(u0 + strip.unit_of(strip.steps - 1));
+            const int32_t halves = tile_is_split(p, p.tile_shape[tile]);
+            return PartList{p.tile_sum, p.tile_ml, 2 * p.tile_grid + c0 + tile * p.kh + kv, 1, p.tile_pairs, at * p.group + in_group, (c1 - c0 + 1) << halves, halves};
+        };
+        PartList shared{}, own{};
+        if (e.y >= 0) {
+            if (p.prefix_tiles) {
+                shared = row_parts(p.requests, e.x * p.group + in_group);
+            } else if (pre_tiles && ctas) {
+                const int32_t tile = p.by_tile_rows.div(listed);
+                shared = tile_parts(tile, listed - tile * p.tile_rows);
+            }
+            own = e.z < 0 ? tile_parts(-1 - e.z, e.w) : row_parts(e.z, e.w * p.group + in_group);
+        }
+        // (written where it was computed: the only part, no half of a tile)
+        const bool written = own.count == 1 && !own.halves && (e.z < 0 ? !p.share : p.prefix == 0);
+        const uint32_t skip = __ballot_sync(0xffffffffu, written || head0 + (lane & 7) >= p.qh) & 0xffu;
+        if (skip == 0xffu) continue;
+        const int32_t all = written ? 0 : shared.count + own.count, most = __reduce_max_sync(0xffffffffu, all);
+        float m = -INFINITY, l = 0.0f;
+        float4 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int32_t x = 0; x < most; ++x) {
+            float2 v = make_float2(-INFINITY, 0.0f);
+            const float *from = nullptr;
+            if (x < all) {
+                const bool first = x < shared.count;
+                const int64_t at = first ? shared.at<true>(x) : own.at<true>(x - shared.count);
+                from = (first ? shared.sum : own.sum) + at * kPgDim;
+                v = (first ? shared.ml : own.ml)[at];
+            }
+            float4 u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), i));
+                u[i] = src ? ld4(src + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            const float top = fmaxf(m, v.x);
+            const float w = v.x == -INFINITY ? 0.0f : pg_exp2(v.x - top), corr = m == -INFINITY ? 0.0f : pg_exp2(m - top);
+            m = top;
+            l = fmaf(w, v.y, l * corr);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = __shfl_sync(0xffffffffu, w, i), c = __shfl_sync(0xffffffffu, corr, i);
+                if (f != 0.0f)  // (a part that saw nothing has written no sums)
+                    o[i] = make_float4(fmaf(f, u[i].x, o[i].x * c), fmaf(f, u[i].y, o[i].y * c), fmaf(f, u[i].z, o[i].z * c), fmaf(f, u[i].w, o[i].w * c));
+                else if (c != 1.0f)
+                    o[i] = make_float4(o[i].x * c, o[i].y * c, o[i].z * c, o[i].w * c);
+            }
+        }
+        const float inv = l == 0.0f && (e.y < 0 || tree_blank(p, e.x, e.y, listed_added(p, e))) ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = __shfl_sync(0xffffffffu, inv, i);
+            if (!((skip >> i) & 1u)) join_store<F32>(p, e.x, f, head0 + i, o[i]);
+        }
+    }
+    // Rows that no request has.
+    const auto clear = [&](int32_t row) {
+        for (int32_t x = threadIdx.x; x < p.qh * kPgDim / 4; x += blockDim.x) {
+            if constexpr (F32) pg_store4(static_cast<float *>(p.out) + row * p.out_stride + 4 * x, make_float4(0.f, 0.f, 0.f, 0.f));
+            else pg_store4(static_cast<uint16_t *>(p.out) + row * p.out_stride + 4 * x, make_float4(0.f, 0.f, 0.f, 0.f));
+        }
+    };
+#pragma unroll 1
+    for (int32_t row = blockIdx.x; row < first_row; row += gridDim.x) clear(row);
+#pragma unroll 1
+    for (int32_t row = end_row + blockIdx.x; row < p.rows; row += gridDim.x) clear(row);
+}
+
 }  // namespace plamo
