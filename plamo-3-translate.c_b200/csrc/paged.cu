@@ -390,8 +390,8 @@ bool run_adapters(plamo_cuda *c, const plamo_paged_adapters_args *d, const Adapt
     const uint64_t tiles = ceil_div(d->rows, kAdRows), sms = context_sms(c);
     const auto inner = d->x_type == PLAMO_PAGED_FP32 ? paged_adapters_inner_kernel<float> : paged_adapters_inner_kernel<uint16_t>;
     const auto outer = d->type == PLAMO_PAGED_FP32 ? paged_adapters_outer_kernel<float> : paged_adapters_outer_kernel<uint16_t>;
-    // Outputs' blocks to a CTA: one while that takes four CTAs to an SM at most.
-    const uint64_t blocks = ceil_div(d->outputs, kAdOutputs), per = std::max<uint64_t>(1, tiles * blocks / (4 * sms));
+    // Outputs' blocks to a CTA: one while all CTAs, five to an SM, begin at once.
+    const uint64_t blocks = ceil_div(d->outputs, kAdOutputs), per = std::max<uint64_t>(1, ceil_div(tiles * blocks, 5 * sms));
     return launch(c, "paged_adapters inner", inner,
                   dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(p.splits), static_cast<uint32_t>(ceil_div(d->rank, 16))), dim3(kAdThreads), 0,
                   stream, false, p) &&

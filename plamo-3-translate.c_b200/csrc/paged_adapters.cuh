@@ -53,11 +53,31 @@ __device__ __forceinline__ int32_t ad_row_adapter(const AdapterParams &p, int32_
     if ((threadIdx.x & 31) == 0) pg_flag(p.status, PLAMO_PAGED_ADAPTER);
     return -1;
 }
-// Fills adapter[] (kAdRows entries, shared) for the tile's rows, a warp to a row.
-__device__ __forceinline__ void ad_tile(const AdapterParams &p, int32_t row0, int32_t *adapter) {
+// The runs of the CTA's eight rows: neighbours with one adapter. A warp to a row.
+struct AdRuns {
+    int32_t adapter[kAdRows];
+    int32_t count, first[kAdRows], end[kAdRows], id[kAdRows];
+};
+__device__ __forceinline__ void ad_runs(const AdapterParams &p, int32_t row0, AdRuns &runs) {
     const int32_t warp = threadIdx.x >> 5;
     const int32_t id = ad_row_adapter(p, row0 + warp);
-    if ((threadIdx.x & 31) == 0) adapter[warp] = id;
+    if ((threadIdx.x & 31) == 0) runs.adapter[warp] = id;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int32_t n = 0;
+        for (int32_t row = 0; row < kAdRows; ++row) {
+            const int32_t of = runs.adapter[row];
+            if (of < 0) continue;
+            if (row && runs.adapter[row - 1] == of) {
+                runs.end[n - 1] = row + 1;
+            } else {
+                runs.first[n] = row;
+                runs.end[n] = row + 1;
+                runs.id[n++] = of;
+            }
+        }
+        runs.count = n;
+    }
     __syncthreads();
 }
 
@@ -67,22 +87,37 @@ __device__ __forceinline__ void ad_tile(const AdapterParams &p, int32_t row0, in
 // so that a single row of a decode step costs no more than reading A. The
 // products' order along the columns is free: lane t of four takes columns 16 t to
 // 16 t + 15 of 64, so that both operands come in whole 16-byte pieces from
-// global memory, A's once per run of rows with the same adapter.
+// global memory, A's once per run of rows with the same adapter, the next
+// run's while this one's are multiplied.
 template <typename X>
 __global__ void __launch_bounds__(kAdThreads) paged_adapters_inner_kernel(const __grid_constant__ AdapterParams p) {
     constexpr int TERMS = sizeof(X) == 4 ? 3 : 1;
-    __shared__ int32_t adapter[kAdRows];
+    __shared__ AdRuns runs;
     __shared__ float sums[kAdWarps][16][kAdRows + 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int32_t row0 = blockIdx.x * kAdRows, rank0 = blockIdx.z * 16;
     pdl_launch_dependents();
-    ad_tile(p, row0, adapter);
+    ad_runs(p, row0, runs);
     const int32_t begin = blockIdx.y * p.share, end = min(begin + p.share, p.columns);
-    const bool there = row0 + g < p.rows && adapter[g] >= 0;
+    const bool there = row0 + g < p.rows && runs.adapter[g] >= 0;
     const X *x = static_cast<const X *>(p.x) + static_cast<uint64_t>(there ? row0 + g : 0) * p.x_stride;
+    uint4 ahead[2][2];
+    const auto fetch = [&](int32_t c, int32_t run) {  // 16 columns of A's rows g and g + 8
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int32_t r = rank0 + g + 8 * i;
+                ahead[i][j] = r < p.rank && c + 8 * j < end
+                                  ? *reinterpret_cast<const uint4 *>(p.a + (static_cast<uint64_t>(runs.id[run]) * p.rank + r) * p.columns + c + 8 * j)
+                                  : make_uint4(0, 0, 0, 0);
+            }
+    };
     float total[4] = {0.f, 0.f, 0.f, 0.f};
+    const int32_t first = begin + 64 * warp, count = runs.count;
+    if (count) fetch(first + 16 * t, 0);
 #pragma unroll 1
-    for (int32_t c0 = begin + 64 * warp; c0 < end; c0 += kAdColumns) {
+    for (int32_t c0 = first; count && c0 < end; c0 += kAdColumns) {
         const int32_t c = c0 + 16 * t;
         // x of this lane's row: pairs (2 j, 2 j + 1) of its 16 columns
         uint32_t xf[8][TERMS];
@@ -104,36 +139,27 @@ __global__ void __launch_bounds__(kAdThreads) paged_adapters_inner_kernel(const 
             }
         }
 #pragma unroll 1
-        for (int first = 0; first < kAdRows;) {  // runs of rows with one adapter
-            const int32_t id = adapter[first];
-            int last = first + 1;
-            while (last < kAdRows && adapter[last] == id) ++last;
-            if (id >= 0) {
-                uint4 w[2][2];
+        for (int32_t run = 0; run < count; ++run) {
+            uint4 w[2][2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int32_t r = rank0 + g + 8 * i;
-                        w[i][j] = r < p.rank && c + 8 * j < end
-                                      ? *reinterpret_cast<const uint4 *>(p.a + (static_cast<uint64_t>(id) * p.rank + r) * p.columns + c + 8 * j)
-                                      : make_uint4(0, 0, 0, 0);
-                    }
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 2; ++j) w[i][j] = ahead[i][j];
+            // (one place to load from, not a branch each: behind those the loads would be waited for)
+            fetch(run + 1 < count ? c : c + kAdColumns, run + 1 < count ? run + 1 : 0);
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint4 lo = w[0][j >> 1], hi = w[1][j >> 1];
-                    const uint32_t m[4] = {j & 1 ? lo.z : lo.x, j & 1 ? hi.z : hi.x, j & 1 ? lo.w : lo.y, j & 1 ? hi.w : hi.y};
+            for (int j = 0; j < 4; ++j) {
+                const uint4 lo = w[0][j >> 1], hi = w[1][j >> 1];
+                const uint32_t m[4] = {j & 1 ? lo.z : lo.x, j & 1 ? hi.z : hi.x, j & 1 ? lo.w : lo.y, j & 1 ? hi.w : hi.y};
 #pragma unroll
-                    for (int term = TERMS - 1; term >= 0; --term) mma_bf16(s, m, xf[2 * j][term], xf[2 * j + 1][term]);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {  // the other rows' sums are not theirs, whatever this adapter holds
-                    const int row = 2 * t + (k & 1);
-                    if (row >= first && row < last) total[k] += s[k];
-                }
+                for (int term = TERMS - 1; term >= 0; --term) mma_bf16(s, m, xf[2 * j][term], xf[2 * j + 1][term]);
             }
-            first = last;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // the other rows' sums are not theirs, whatever this adapter holds
+                const int row = 2 * t + (k & 1);
+                if (row >= runs.first[run] && row < runs.end[run]) total[k] += s[k];
+            }
         }
     }
 #pragma unroll
@@ -167,17 +193,32 @@ __device__ __forceinline__ void ad_store(T *p, float v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kAdThreads) paged_adapters_outer_kernel(const __grid_constant__ AdapterParams p, int32_t per) {
-    __shared__ int32_t adapter[kAdRows];
-    __shared__ uint32_t h[3][kAdRows][kAdMaxRank / 2 + 4];  // terms of scale * h, two ranks to a word
+__global__ void __launch_bounds__(kAdThreads, 5) paged_adapters_outer_kernel(const __grid_constant__ AdapterParams p, int32_t per) {
+    __shared__ AdRuns runs;
+    __shared__ __align__(16) uint32_t h[3][kAdRows][kAdMaxRank / 2 + 4];  // terms of scale * h, two ranks to a word
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int32_t row0 = blockIdx.x * kAdRows, pairs = p.rank / 2, steps = (p.rank + 15) / 16;
-    ad_tile(p, row0, adapter);
+    const int32_t row0 = blockIdx.x * kAdRows, pairs = p.rank / 2, blocks = (p.rank + 31) / 32;
+    ad_runs(p, row0, runs);
+    // Units of up to two blocks of 32 ranks of one run and 16 outputs; the next one's part of B is
+    // on its way while this one's is multiplied, the first one's before the sums are there.
+    const int32_t count = runs.count, chunks = (blocks + 1) / 2;
+    const auto output = [&](int32_t y) { return (static_cast<int32_t>(blockIdx.y) * per + y) * kAdOutputs + 16 * warp; };
+    uint4 ahead[2][2];
+    const auto fetch = [&](int32_t n0, int32_t run, int32_t chunk) {  // lane t has 8 t to 8 t + 7 of 32 ranks
+        const uint16_t *w = p.b + (static_cast<uint64_t>(runs.id[run]) * p.outputs + n0 + g) * p.rank + 64 * chunk + 8 * t;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const bool in = 64 * chunk + 32 * k + 8 * t < p.rank;
+            ahead[k][0] = in && n0 + g < p.outputs ? *reinterpret_cast<const uint4 *>(w + 32 * k) : make_uint4(0, 0, 0, 0);
+            ahead[k][1] = in && n0 + g + 8 < p.outputs ? *reinterpret_cast<const uint4 *>(w + 8ull * p.rank + 32 * k) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (count) fetch(output(0), 0, 0);
     pdl_wait();
-    for (int32_t x = tid; x < kAdRows * 8 * steps; x += kAdThreads) {
-        const int32_t row = x / (8 * steps), pair = x - row * 8 * steps;
+    for (int32_t x = tid; x < kAdRows * 16 * blocks; x += kAdThreads) {
+        const int32_t row = x / (16 * blocks), pair = x - row * 16 * blocks, id = runs.adapter[row];
         float2 s = make_float2(0.f, 0.f);
-        if (adapter[row] >= 0 && pair < pairs) {
+        if (id >= 0 && pair < pairs) {
             const float *from = p.inner + static_cast<uint64_t>(row0 + row) * p.rank + 2 * pair;
 #pragma unroll 4
             for (int32_t y = 0; y < p.splits; ++y) {
@@ -185,7 +226,7 @@ __global__ void __launch_bounds__(kAdThreads) paged_adapters_outer_kernel(const 
                 s.x += v.x;
                 s.y += v.y;
             }
-            const float scale = p.scales ? p.scales[adapter[row]] : 1.0f;
+            const float scale = p.scales ? p.scales[id] : 1.0f;
             s.x *= scale;
             s.y *= scale;
         }
@@ -197,37 +238,37 @@ __global__ void __launch_bounds__(kAdThreads) paged_adapters_outer_kernel(const 
     __syncthreads();
 #pragma unroll 1
     for (int32_t y = 0; y < per; ++y) {
-        const int32_t n0 = (blockIdx.y * per + y) * kAdOutputs + 16 * warp;
+        const int32_t n0 = output(y);
         if (n0 >= p.outputs) break;
         float total[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-        for (int first = 0; first < kAdRows;) {
-            const int32_t id = adapter[first];
-            int last = first + 1;
-            while (last < kAdRows && adapter[last] == id) ++last;
-            if (id >= 0) {
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
-                const uint16_t *w = p.b + (static_cast<uint64_t>(id) * p.outputs + n0 + g) * p.rank + 4 * t;
-                const bool lo = n0 + g < p.outputs, hi = n0 + g + 8 < p.outputs;
-#pragma unroll 4
-                for (int32_t k = 0; k < steps; ++k) {  // 16 ranks: lane t has 4 t to 4 t + 3 of them
-                    const bool in = 16 * k + 4 * t < p.rank;
-                    const uint2 a = lo && in ? *reinterpret_cast<const uint2 *>(w + 16 * k) : make_uint2(0, 0);
-                    const uint2 b = hi && in ? *reinterpret_cast<const uint2 *>(w + 8ull * p.rank + 16 * k) : make_uint2(0, 0);
-                    const uint32_t m[4] = {a.x, b.x, a.y, b.y};
+        for (int32_t run = 0; run < count; ++run) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int32_t chunk = 0; chunk < chunks; ++chunk) {
+                uint4 w[2][2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) w[k][0] = ahead[k][0], w[k][1] = ahead[k][1];
+                // (one place to load from, not a branch each: behind those the loads would be waited for)
+                const bool same_run = chunk + 1 < chunks, same_block = same_run || run + 1 < count;
+                fetch(same_block ? n0 : y + 1 < per ? output(y + 1) : p.outputs, same_run ? run : same_block ? run + 1 : 0, same_run ? chunk + 1 : 0);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (k && 2 * chunk + 1 >= blocks) break;
+                    const uint32_t m0[4] = {w[k][0].x, w[k][1].x, w[k][0].y, w[k][1].y}, m1[4] = {w[k][0].z, w[k][1].z, w[k][0].w, w[k][1].w};
 #pragma unroll
                     for (int term = 2; term >= 0; --term) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(&h[term][g][8 * k + 2 * t]);
-                        mma_bf16(s, m, v.x, v.y);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(&h[term][g][32 * chunk + 16 * k + 4 * t]);
+                        mma_bf16(s, m0, v.x, v.y);
+                        mma_bf16(s, m1, v.z, v.w);
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = 2 * t + (k & 1);
-                    if (row >= first && row < last) total[k] = s[k];
-                }
             }
-            first = last;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = 2 * t + (k & 1);
+                if (row >= runs.first[run] && row < runs.end[run]) total[k] = s[k];
+            }
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -235,7 +276,7 @@ __global__ void __launch_bounds__(kAdThreads) paged_adapters_outer_kernel(const 
             if (row >= p.rows || n >= p.outputs) continue;
             const T *from = static_cast<const T *>(p.base) + row * p.base_stride + n;
             T *to = static_cast<T *>(p.out) + row * p.out_stride + n;
-            if (adapter[2 * t + (k & 1)] >= 0) ad_store(to, ad_load(from) + total[k]);
+            if (runs.adapter[2 * t + (k & 1)] >= 0) ad_store(to, ad_load(from) + total[k]);
             else *to = *from;
         }
     }

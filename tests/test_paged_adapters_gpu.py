@@ -51,6 +51,7 @@ LAYOUTS = {
     "none": ([1, 3, 0, 20, 1], [-1, 0, 1, -1, 2]),
     "trees": ([17, 1, 33, 0, 8, 24], [3, 3, 0, 1, 0, 2]),
     "prompts": ([129, 300, 1, 64, 511], [0, 0, 1, 2, 1]),
+    "gaps": ([0, 17, 33, 0, 400, 15, 16], [0, -1, 1, 2, 2, -1, 0]),
 }
 
 
@@ -66,7 +67,7 @@ def test_adapters_match_their_formula(be, name, columns, outputs, rank, x_type, 
 
 @pytest.mark.parametrize("rank", [8, 16, 24, 32, 48, 72, 96, 128, 136, 200, 256])
 @pytest.mark.parametrize("kind", [FP32, BF16])
-@pytest.mark.parametrize("new", [[1, 2, 5], [70, 200, 3]])
+@pytest.mark.parametrize("new", [[1, 2, 5], [70, 200, 3], [333, 690, 12]])
 def test_adapters_of_every_rank(be, rank, kind, new):
     c = Case(new, [0, 1, 0], 776, 520, rank, kind, kind, seed=rank)
     check(c.run(be), *c.expected(), f"rank {rank}")
@@ -74,14 +75,14 @@ def test_adapters_of_every_rank(be, rank, kind, new):
 
 @pytest.mark.parametrize("columns,outputs", [(4096, 5120), (16384, 4096), (4096, 32768), (5120, 10240)])
 @pytest.mark.parametrize("kind", [FP32, BF16])
-@pytest.mark.parametrize("new", [[1] * 9, [150, 90]])
+@pytest.mark.parametrize("new", [[1] * 9, [250, 190]])
 def test_adapters_of_the_models_projections(be, columns, outputs, kind, new):
     c = Case(new, [i % 3 for i in range(len(new))], columns, outputs, 16, kind, kind, seed=1)
     check(c.run(be), *c.expected(), "projection")
 
 
 @pytest.mark.parametrize("kind", [FP32, BF16])
-@pytest.mark.parametrize("new", [[1, 4, 3], [140, 4, 3]])
+@pytest.mark.parametrize("new", [[1, 4, 3], [540, 4, 3]])
 def test_adapters_strides_and_places(be, kind, new):
     """Strided rows, a result of its own, the result in place; padding keeps base's."""
     c = Case(new, [0, -1, 1], 264, 392, 16, kind, kind, spare=5, seed=2)
@@ -102,7 +103,7 @@ def test_adapters_strides_and_places(be, kind, new):
     assert torch.equal(in_place, plain) and (base[:, :8] == 3).all()
 
 
-@pytest.mark.parametrize("new", [[1, 1, 1, 1], [3, 70, 200, 1]])
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [3, 170, 400, 1]])
 def test_adapters_of_others_never_matter(be, new):
     """Adapters and rows that hold no numbers reach their own requests only."""
     c = Case(new, [0, 1, 2, 0], 256, 136, 24, seed=3)
@@ -116,7 +117,7 @@ def test_adapters_of_others_never_matter(be, new):
     assert not torch.isfinite(got[c.starts[1]:c.starts[3]]).any()
 
 
-@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("new", [1, 500])
 @pytest.mark.parametrize("kind", [FP32, BF16])
 def test_adapters_of_infinite_rows(be, kind, new):
     """One infinite entry times weights of one sign is infinite, not undefined."""
@@ -129,7 +130,7 @@ def test_adapters_of_infinite_rows(be, kind, new):
 
 
 def test_adapters_without_scales_requests_or_adapters(be):
-    c = Case([2, 90], [1, 0], 64, 72, 16, seed=5)
+    c = Case([2, 490], [1, 0], 64, 72, 16, seed=5)
     ones, c.scales = c.scales, None
     check(c.run(be), *c.expected(), "no scales")
     c.scales = ones
@@ -141,7 +142,7 @@ def test_adapters_without_scales_requests_or_adapters(be):
     assert be.paged_status() == 0
 
 
-@pytest.mark.parametrize("new", [[2, 3, 1], [2, 300, 1]])
+@pytest.mark.parametrize("new", [[2, 3, 1], [2, 500, 1]])
 @pytest.mark.parametrize("bad", [2, -2, 2 ** 31 - 1, -2 ** 31])
 def test_adapters_report_ids_that_are_none(be, bad, new):
     c = Case(new, [0, -1, 1], 64, 72, 16, adapters=2, seed=6)
@@ -152,17 +153,18 @@ def test_adapters_report_ids_that_are_none(be, bad, new):
     assert status.item() == 256
 
 
+@pytest.mark.parametrize("rows", [20, 200])
 @pytest.mark.parametrize("starts", [[0, 50, 20, 70], [-9, 10, 20, 10 ** 9], [5, 10, 20, 30], [2 ** 31 - 1, -2 ** 31, 7, 9]])
-def test_adapters_of_starts_outside_the_batch_stay_in_bounds(be, starts):
-    c = Case([20, 30, 20], [0, 1, 0], 64, 72, 16, seed=7)
-    out = torch.full((72, 72), 7.0, device="cuda")
+def test_adapters_of_starts_outside_the_batch_stay_in_bounds(be, starts, rows):
+    c = Case([rows, 30, rows], [0, 1, 0], 64, 72, 16, seed=7)
+    out = torch.full((2 * rows + 32, 72), 7.0, device="cuda")
     c.starts = starts
     c.run(be, out=out[1:-1])
     torch.cuda.synchronize()
     assert (out[0] == 7).all() and (out[-1] == 7).all()
 
 
-@pytest.mark.parametrize("new", [[1, 1, 6], [129, 3, 200]])
+@pytest.mark.parametrize("new", [[1, 1, 6], [229, 3, 200]])
 def test_adapters_are_the_same_every_time_captured_and_on_another_stream(be, new):
     c = Case(new, [0, 1, 0], 1024, 264, 32, seed=8)
     first = c.run(be)
