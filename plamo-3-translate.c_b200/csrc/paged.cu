@@ -6,6 +6,7 @@
 #include "paged_adapters.cuh"
 #include "paged_attention.cuh"
 #include "paged_tiles.cuh"
+#include "paged_tree_f32.cuh"
 #include "paged_tree_tiles.cuh"
 #include "paged_trees.cuh"
 
@@ -65,7 +66,7 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 constexpr uint64_t kTreeShareRows = 1024;
 constexpr uint32_t kTreeShortPairs = 8;
 // What a strip's beginning and end are worth, in units of half a step of a full tile.
-constexpr int32_t kTreeStripPad = 12;
+constexpr int32_t kTreeStripPad = 12, kTreeStripPadF32 = 2;
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
@@ -105,7 +106,7 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     // 512 rows 76 us in it; behind 1,000, 2,000 with tiles 103, 136: the same slope,
     // 12 us more).
     const bool f32 = d->type == PLAMO_PAGED_FP32;
-    const uint64_t tile_pairs = f32 ? kTfPairs : kTlPairs;
+    const uint64_t tile_pairs = !f32 ? kTlPairs : trees ? kTqPairs : kTfPairs;
     const uint64_t strips = ceil_div(pairs, kRtPairs) * d->kv_heads;
     const uint64_t prefix_steps = ceil_div(pairs, kTlPairs) * d->kv_heads * ceil_div(d->prefix_rows, kTlKeys);
     const uint64_t most = d->most_new ? std::min(d->most_new, d->rows) : d->rows > d->requests ? d->rows : 0;  // rows of a request
@@ -114,7 +115,7 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     if (group <= tile_pairs && ((prompts && strips * (prefix_pages + d->table_stride) > kTlPromptUnits) ||
                                 (!f32 && strips * prefix_pages > kTlPrefixUnits + 4 * prefix_steps))) {
         a.tile_rows = static_cast<uint32_t>(tile_pairs / group);
-        a.tile_grid = static_cast<uint32_t>(f32 ? 2 * sms : sms);
+        a.tile_grid = static_cast<uint32_t>(f32 && !trees ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
         a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
         // Tiles over the prefix that all trees share are full; their own have room for whole rows of
@@ -201,7 +202,7 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
     p.short_pairs = static_cast<int32_t>(a.short_pairs);
     p.split_pairs = static_cast<int32_t>(a.split_pairs);
     p.step_units = F32 ? 1 : 2;
-    p.strip_pad = F32 ? 0 : kTreeStripPad;
+    p.strip_pad = F32 ? kTreeStripPadF32 : kTreeStripPad;
     p.least_units = F32 ? 1 : 4;
     p.scale2 = d->scale * 1.4426950408889634f;
     // The tile kernel masks before it scales: -inf must stay so.
@@ -218,7 +219,7 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
         p.pool = d->pool;
         p.tile_rows = static_cast<int32_t>(a.tile_rows);
         p.by_tile_rows = FastDiv::of(a.tile_rows);
-        p.tile_pairs = F32 ? kTfPairs : kTlPairs;
+        p.tile_pairs = !F32 ? kTlPairs : TREE ? kTqPairs : kTfPairs;
         p.tile_keys = F32 ? kTfKeys : kTlKeys;
         p.tile_grid = static_cast<int32_t>(a.tile_grid);
         p.tile_cap = static_cast<int32_t>(a.tile_cap);
@@ -231,12 +232,14 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
     if (TREE && !F32 && a.tile_rows && !tensor_map_heads(&q_map, d->q, d->rows, d->query_heads, d->q_stride, p.group, a.tile_rows))
         return context_launched(c, "paged_attention: tensor map", cudaErrorInvalidValue);
     if (!launch(c, "paged_attention rows", paged_rows_kernel<F32, TREE>, dim3(a.workers + 1), dim3(kRtThreads), kRtSmem, stream, false, map, p) ||
-        (a.tile_rows && !(F32    ? launch(c, "paged_attention tiles", paged_tile_f32_kernel<TREE>, dim3(a.tile_grid), dim3(kTfThreads),
-                                          kTfSmem, stream, true, page_map, p)
-                          : TREE ? launch(c, "paged_attention tiles", paged_tree_tile_kernel, dim3(a.tile_grid), dim3(kTsThreads), kTlSmem,
-                                          stream, true, page_map, q_map, p)
-                                 : launch(c, "paged_attention tiles", paged_tile_kernel, dim3(a.tile_grid), dim3(kTlThreads), kTlSmem, stream,
-                                          true, page_map, p))))
+        (a.tile_rows && !(F32 && TREE ? launch(c, "paged_attention tiles", paged_tree_f32_kernel, dim3(a.tile_grid), dim3(kTqThreads), kTqSmem, stream,
+                                               true, p)
+                          : F32       ? launch(c, "paged_attention tiles", paged_tile_f32_kernel, dim3(a.tile_grid), dim3(kTfThreads), kTfSmem, stream,
+                                               true, page_map, p)
+                          : TREE      ? launch(c, "paged_attention tiles", paged_tree_tile_kernel, dim3(a.tile_grid), dim3(kTsThreads), kTlSmem, stream,
+                                               true, page_map, q_map, p)
+                                      : launch(c, "paged_attention tiles", paged_tile_kernel, dim3(a.tile_grid), dim3(kTlThreads), kTlSmem, stream,
+                                               true, page_map, p))))
         return false;
     // Two results to a block, its warps sharing their parts, while that takes two
     // blocks to an SM at most (one request over 131,072 rows, 74 parts each: 10 us
@@ -445,8 +448,8 @@ cudaError_t paged_configure() {
     if (e == cudaSuccess) e = allow(paged_rows_kernel<true, true>, kRtSmem);
     if (e == cudaSuccess) e = allow(paged_tile_kernel, kTlSmem);
     if (e == cudaSuccess) e = allow(paged_tree_tile_kernel, kTlSmem);
-    if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<false>, kTfSmem);
-    if (e == cudaSuccess) e = allow(paged_tile_f32_kernel<true>, kTfSmem);
+    if (e == cudaSuccess) e = allow(paged_tile_f32_kernel, kTfSmem);
+    if (e == cudaSuccess) e = allow(paged_tree_f32_kernel, kTqSmem);
     if (e == cudaSuccess) e = configure_adapters<float>();
     if (e == cudaSuccess) e = configure_adapters<uint16_t>();
     return e;

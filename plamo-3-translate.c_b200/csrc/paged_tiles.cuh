@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 constexpr int kTfPairs = 64, kTfKeys = 64, kTfThreads = 128;
 constexpr int kTfTile = kTfKeys * kPgDim * 4;  // keys, values or queries
 constexpr int kTfTables = 3 * kTfTile + kTfPairs * kTfKeys * 4;  // barriers and the pairs' rows behind the tiles
-constexpr int kTfSmem = kTfTables + 16 + 3 * kTfPairs * 4;       // no static part: two CTAs just fit an SM
+constexpr int kTfSmem = kTfTables + 16 + 2 * kTfPairs * 4;       // no static part: two CTAs just fit an SM
 
 // A 16-byte piece of row r: the copy engine's swizzle; the queries' rows r and
 // r + 8, read together, lie apart too; the weights' keys are rows.
@@ -770,15 +770,13 @@ __device__ __forceinline__ float4 lds_f32x4(uint32_t addr) {
     return v;
 }
 
-template <bool TREE>
 __global__ void __launch_bounds__(kTfThreads, 2)
     paged_tile_f32_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ PagedAttnParams p) {
     extern __shared__ __align__(1024) unsigned char tf_smem[];
     unsigned char *const base = tf_smem;
     uint64_t *const full = reinterpret_cast<uint64_t *>(base + kTfTables);           // keys, values
     int32_t *const pair_row = reinterpret_cast<int32_t *>(base + kTfTables + 16);    // batch row, -1: no such pair
-    int32_t *const pair_at = pair_row + kTfPairs;                                    // own row; trees: held rows
-    int32_t *const pair_skip = pair_at + kTfPairs;                                   // trees: rows outside the window
+    int32_t *const pair_at = pair_row + kTfPairs;                                    // own row
     if (smem_u32(base) & 1023u) {  // the copies' swizzle needs it; dynamic shared memory starts so when there is no other
         pg_flag(p.status, PLAMO_PAGED_FAILED);
         return;
@@ -806,7 +804,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
     bool ok = true;
     uint32_t phase = 0;
 #pragma unroll 1
-    for (bool begins = true; ok && (TREE ? tree_walk_next(p, w) : walk_next(p, w)); w.unit += TREE ? 0 : w.steps, begins = false) {
+    for (bool begins = true; ok && walk_next(p, w); w.unit += w.steps, begins = false) {
         const TileShape s = p.tile_shape[w.tile];
         const int32_t pre_steps = s.pre1 - s.pre0, pairs = s.rows * p.group;
         // Step n's page, first key and the key from which on nothing is seen.
@@ -828,26 +826,22 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             copy(0, 0);
             copy(0, 1);
         }
-        const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles && !(TREE && p.share);
-        const int32_t slot = TREE || w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
+        const bool whole = w.steps == w.tile_steps && w.tile >= pre_tiles;
+        const int32_t slot = w.tile < pre_tiles ? 2 * p.tile_grid + cta + w.tile * p.kh + w.head : 2 * cta + (begins ? 0 : 1);
         if (tid < kTfPairs) {
-            int32_t row = -1, at = 0, skip = 0;
+            int32_t row = -1, at = 0;
             if (tid < pairs) {
                 const int32_t local = p.by_group.div(tid);
-                int32_t added = s.added;
                 row = s.row0 + local;
-                at = TREE ? s.at0 : s.at0 + local;
+                at = s.at0 + local;
                 if (s.request < 0) {
                     const int4 e = p.short_list[row];
                     row = e.x;
                     at = e.y;
-                    if (TREE && p.window) added = listed_added(p, e);
                 }
-                if (TREE && at >= 0) skip = tree_skip(p, row, at, added);
             }
             pair_row[tid] = row;
             pair_at[tid] = at;
-            if constexpr (TREE) pair_skip[tid] = skip;
         }
         const auto head_of = [&](int32_t pair) { return w.head * p.group + pair - p.by_group.div(pair) * p.group; };
         __syncthreads();
@@ -921,38 +915,15 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             // Keys that each pair sees, of this step's: [lo, hi).
             int32_t lo[8], hi[8];
             bool move = false;
-            const bool drafted = TREE && own && key0 + kTfKeys > s.at0;  // new rows are among the keys
-            // New rows among the step's keys at, at + 1, ... at + 31 that pair i of this thread sees.
-            const auto drafts = [&](int i, int at) {
-                const int32_t row = pair_row[8 * ty + i];
-                if (row < 0) return 0u;
-                const TreeSees sees = tree_sees(p, pair_skip[8 * ty + i], s.at0);
-                return tree_bits(p, row, s.added, tree_first(p, row, s.added, sees.drop), key0 + at - s.at0);
-            };
-            uint32_t mine = 0;  // bit 4 i + j
-            if (drafted) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t a = drafts(i, 0) >> tx, b = drafts(i, 32) >> tx;
-                    mine |= ((a & 1u) | ((a >> 16 & 1u) << 1) | ((b & 1u) << 2) | ((b >> 16 & 1u) << 3)) << (4 * i);
-                }
-            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int32_t at = pair_at[8 * ty + i], place = max(at, 0) + (own ? 0 : p.prefix);
-                if constexpr (TREE) {
-                    const TreeSees sees = tree_sees(p, pair_skip[8 * ty + i], max(at, 0));
-                    lo[i] = max((own ? sees.lo : sees.pre) - key0, 0);
-                    hi[i] = at < 0 ? 0 : min((own ? at : limit) - key0, kTfKeys);
-                } else {
-                    lo[i] = p.window ? max(place - p.window + 1 - key0, 0) : 0;
-                    hi[i] = at < 0 ? 0 : min((own ? min(at + 1, limit) : limit) - key0, kTfKeys);
-                }
+                lo[i] = p.window ? max(place - p.window + 1 - key0, 0) : 0;
+                hi[i] = at < 0 ? 0 : min((own ? min(at + 1, limit) : limit) - key0, kTfKeys);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = tx + 16 * j;
-                    const bool seen = (key >= lo[i] && key < hi[i]) || (TREE && (mine >> (4 * i + j) & 1u));
-                    x[i][j] = seen ? x[i][j] * p.scale2 : -INFINITY;
+                    x[i][j] = key >= lo[i] && key < hi[i] ? x[i][j] * p.scale2 : -INFINITY;
                     move |= x[i][j] > m[i] + kLazy;
                 }
             }
@@ -986,7 +957,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             // some pair, the values are looked over.
             bool masked, odd = false;
             const int32_t valid = min(limit - key0, kTfKeys);  // keys that exist
-            step_is_mended<TREE>(p, s, step, &masked);
+            step_is_mended<false>(p, s, step, &masked);
             if (masked) {
 #pragma unroll 4
                 for (int k = tid; k < valid * (kPgDim / 4); k += kTfThreads) {
@@ -1004,7 +975,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
                 const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, z[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (all || (key >= lo[i] && key < hi[i]) || (drafted && (drafts(i, key) & 1u))) {
+                    if (all || (key >= lo[i] && key < hi[i])) {
 #pragma unroll
                         for (int d = 0; d < 8; ++d) o[i][d] = fmaf(y[i], z[d], o[i][d]);
                     }
@@ -1036,7 +1007,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
 #pragma unroll 1
             for (int key = 8 * eights; key < valid; ++key)
                 add(key, *tf_weight(weights, key, 2 * ty), *tf_weight(weights, key, 2 * ty + 1), *tf_piece(tile_at[1], key, tx),
-                    *tf_piece(tile_at[1], key, 16 + tx), TREE && !odd);
+                    *tf_piece(tile_at[1], key, 16 + tx), false);
             __syncthreads();  // values and weights have been read
             if (tid == 0 && n + 1 < w.steps) copy(n + 1, 1);
             phase ^= 1u;
@@ -1052,7 +1023,7 @@ __global__ void __launch_bounds__(kTfThreads, 2)
             if (row < 0) continue;
             const uint64_t to = whole ? row * p.out_stride + head_of(pair) * kPgDim : (static_cast<uint64_t>(slot) * kTfPairs + pair) * kPgDim;
             const float2 ml = pg_ml(m[i], sum);
-            const float inv = !whole ? 1.0f : TREE ? tree_inverse(p, row, pair_at[pair], s.added, sum) : pg_inverse(pair_at[pair], sum);
+            const float inv = whole ? pg_inverse(pair_at[pair], sum) : 1.0f;
             float *dst = (whole ? static_cast<float *>(p.out) : p.tile_sum) + to + 4 * tx;
             *reinterpret_cast<float4 *>(dst) = make_float4(o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv);
             *reinterpret_cast<float4 *>(dst + 64) = make_float4(o[i][4] * inv, o[i][5] * inv, o[i][6] * inv, o[i][7] * inv);

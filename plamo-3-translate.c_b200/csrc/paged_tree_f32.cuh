@@ -1,0 +1,504 @@
+// Attention of draft trees on the tensor cores: FP32, tiles of up to 128 (row, head)
+// pairs by steps of 64 keys, a page.
+#pragma once
+#include "paged_tree_tiles.cuh"
+
+namespace plamo {
+
+// Queries, keys, weights and values each enter as three BF16 terms x1 + x2 + x3 (24
+// bits), and of the nine products of two those six are made whose size is above 2^-24
+// of the whole: (3,1) (1,3) (2,2) (2,1) (1,2) (1,1), the small ones first. Tensor cores
+// cut what they add up, by 1e-5 of the sum over some thousand keys; so a step's value
+// products start from zero and are added to FP32 registers, and nothing is cut by more
+// than a few products of 2^-24. 128 pairs by 64 keys are 3,072 cycles of the tensor pipe;
+// as many multiply-adds of the CUDA cores are 16,384.
+//  - Sixteen warps do all but the products. Warp w has the rows of tensor-memory lanes
+//    32 (w % 4) up; its quarter w / 4 has 16 of a step's keys and 32 of the dimensions. In
+//    each step a thread makes its keys' weights, adds its dimensions' sums of the step
+//    before to its registers, and turns its share of the next keys and values, which its
+//    loads brought a step earlier, into terms in shared memory.
+//  - Tensor memory (512 columns): the queries' terms 3 x 64, a step's sums 128, and two
+//    places by turns of 96 for a step's scores (64), then its weights' terms (3 x 32).
+//  - Shared memory: two steps' terms of keys and of values, 4 x 48 KB.
+// Values that are not finite leave the products, and rows that see them get them at the
+// end of a segment; a key that has such a number gets its scores one by one.
+constexpr int kTqPairs = 128, kTqKeys = 64, kTqWarps = 16, kTqThreads = 32 * (kTqWarps + 2);
+constexpr int kTqWalk = 16, kTqProducts = 17;  // warps
+constexpr int kTqTerm = kTqKeys * kPgDim * 2, kTqBlock = kTqKeys * 128;  // bytes: a term of keys or values, its block of 64 dimensions
+constexpr int kTqSmem = 1024 + 4 * 3 * kTqTerm;
+constexpr uint32_t kTqQueries = 0, kTqSums = 192, kTqPlaces = 320, kTqPlace = 96;  // columns
+
+// A pair of numbers as terms; of finite ones all.
+__device__ __forceinline__ void tq_split(float a, float b, uint32_t (&t)[3]) {
+    t[0] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+    b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    t[1] = pg_pack(a, b);
+    t[2] = pg_pack(a - bf16_lo(t[1]), b - bf16_hi(t[1]));
+}
+__device__ __forceinline__ bool tq_finite(const float4 &v) { return isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w); }
+__device__ __forceinline__ float tq_or_zero(float x) { return isfinite(x) ? x : 0.0f; }
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// A barrier of the sixteen warps that says whether any thread asks.
+__device__ __forceinline__ bool tq_any(bool ask) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(static_cast<uint32_t>(ask)), "n"(32 * kTqWarps)
+        : "memory");
+    return any != 0;
+}
+
+// Values that are not finite, for a row that sees them (a weight times one of them is itself): dimensions c to c + 31.
+__device__ __noinline__ void tq_add_odd_values(const PagedAttnParams &p, const TreeSegment &t, int32_t row, int32_t held, int32_t added,
+                                               const TreeSees &sees, int32_t from, int c, float (&o)[32]) {
+    const TileShape s = p.tile_shape[t.tile];
+#pragma unroll 1
+    for (int32_t n = 0; n < t.steps; ++n) {
+        const int32_t step = t.step + n;
+        const bool own = step >= t.pre_steps;
+        const int32_t key0 = (own ? t.own0 + step - t.pre_steps : t.pre0 + step) * kTqKeys, hi = min(key0 + kTqKeys, own ? s.own_limit : p.prefix);
+        const int32_t id = own ? p.tables[static_cast<uint64_t>(s.request) * p.table_stride + key0 / kPgRows] : p.prefix_pages[key0 / kPgRows];
+        if (id < 0 || id >= p.pages) continue;
+#pragma unroll 1
+        for (int32_t key = max(key0, own ? sees.lo : sees.pre); key < hi; ++key) {
+            if (own && key >= held && !(tree_bits(p, row, added, from, key - held) & 1u)) continue;
+            const float *v = static_cast<const float *>(p.pool) +
+                             (((static_cast<uint64_t>(id) * 2 + 1) * kPgRows + key % kPgRows) * p.kh + t.head) * static_cast<uint64_t>(kPgDim) + c;
+#pragma unroll 1
+            for (int k = 0; k < 32; ++k)
+                if (!isfinite(v[k])) o[k] += v[k];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __grid_constant__ PagedAttnParams p) {
+    extern __shared__ __align__(128) unsigned char tq_smem[];
+    __shared__ __align__(8) uint64_t seg_full[kTsSegments], seg_empty[kTsSegments];
+    __shared__ __align__(8) uint64_t q_ready, k_ready[2], k_free[2], v_ready[2], v_free[2], s_full[2], p_ready[2], o_full, o_free;
+    __shared__ TreeSegment segments[kTsSegments];
+    __shared__ float tops[4][kTqPairs];
+    __shared__ uint32_t odd_keys[4][2];  // of step s, at s % 4: keys with a number that is not finite
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up, odd_values;
+    unsigned char *base = reinterpret_cast<unsigned char *>(
+        (reinterpret_cast<uintptr_t>(tq_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char *const keys_at = base, *const values_at = base + 2 * 3 * kTqTerm;  // two steps' each
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < kTsSegments; ++s) {
+            mbar_init(&seg_full[s], 1);
+            mbar_init(&seg_empty[s], kTqWarps + 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_ready[i], kTqWarps);
+            mbar_init(&v_ready[i], kTqWarps);
+            mbar_init(&p_ready[i], kTqWarps);
+            mbar_init(&k_free[i], 1);
+            mbar_init(&v_free[i], 1);
+            mbar_init(&s_full[i], 1);
+        }
+        mbar_init(&q_ready, kTqWarps);
+        mbar_init(&o_full, 1);
+        mbar_init(&o_free, kTqWarps);
+        gave_up = odd_values = 0;
+        fence_barrier_init();
+    }
+    if (tid < 8) odd_keys[tid >> 1][tid & 1] = 0;
+    if (warp == kTqProducts) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    pdl_launch_dependents();
+    volatile int *quit = &gave_up;
+    bool ok = true;
+    const auto wait = [&](uint64_t *bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, ts_wait(bar, parity, quit));
+    };
+
+    if (warp == kTqWalk) {
+        // ---- the work's segments
+        pdl_wait();
+        const int32_t ctas = p.header[kTlCtas], cta = static_cast<int32_t>(blockIdx.x);
+        const int32_t first_row = p.header[kTlFirst];
+        TileWalk w{};
+        if (cta < ctas) {
+            const Runs runs = tile_runs(p);
+            w.unit = runs.start(cta);
+            w.end = runs.start(cta + 1);
+            w.tile = pg_owner(reinterpret_cast<const int32_t *>(p.tile_unit), static_cast<uint32_t>(p.header[kTlTiles]), p.by_kh.div(w.unit));
+        }
+        uint32_t seg = 0;
+        for (bool more = true; more && ok; ++seg) {
+            more = tree_walk_next(p, w);
+            TileShape s{};
+            if (more) s = p.tile_shape[w.tile];
+            const uint32_t e = seg % kTsSegments;
+            ok = seg < kTsSegments || wait(&seg_empty[e], (seg / kTsSegments - 1) & 1u);
+            if (ok && lane == 0) {
+                TreeSegment t{};
+                if (more)
+                    t = TreeSegment{w.steps, 0, w.tile, w.head, w.step, w.tile_steps, s.request < 0 ? first_row + s.row0 : s.row0, s.rows * p.group,
+                                    s.request < 0 ? -1 : s.at0, s.added, s.pre0, s.pre1 - s.pre0, s.own0, {s.request, s.own_limit, 0}};
+                segments[e] = t;
+                mbar_arrive(&seg_full[e]);
+            }
+            __syncwarp();
+        }
+    } else if (warp == kTqProducts) {
+        // ---- products
+        constexpr uint32_t idesc_s = tc_idesc(128, kTqKeys), idesc_o = tc_idesc(128, kPgDim) | kTcIdescMnB;
+        constexpr int kOf[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};  // terms of the first and second operand
+        const bool leader = elect_one();
+        const uint64_t k_desc = smem_desc_sw128(smem_u32(keys_at)), v_desc = smem_desc_mn_sw128(smem_u32(values_at), kTqBlock);
+        uint32_t c = 0;  // steps before the segment's
+        for (uint32_t seg = 0; ok; ++seg) {
+            ok = wait(&seg_full[seg % kTsSegments], (seg / kTsSegments) & 1u);
+            if (!ok) break;
+            const int32_t steps = __shfl_sync(0xffffffffu, segments[seg % kTsSegments].steps, 0);
+            __syncwarp();
+            if (leader) mbar_arrive(&seg_empty[seg % kTsSegments]);
+            if (!steps) break;
+            // Of step s: its place is free when the value products of step s - 2 are done. (Of a segment's
+            // first step they are, and those of s - 1: the queries were put there behind them.)
+            const auto scores = [&](uint32_t s, bool first) {
+                const uint32_t i = s & 1;
+                if (!wait(&k_ready[i], (s >> 1) & 1u) || (!first && s >= 2 && !wait(&o_full, (s - 2) & 1u))) return false;
+                tc_fence_after();
+                if (leader) {
+                    const uint32_t d = tmem + kTqPlaces + i * kTqPlace;
+                    const uint64_t b = k_desc + i * (3 * kTqTerm / 16);
+#pragma unroll
+                    for (int y = 0; y < 6; ++y)
+#pragma unroll
+                        for (int k = 0; k < kPgDim / 16; ++k)
+                            tc_mma_ts(d, tmem + kTqQueries + 64 * kOf[y][0] + 8 * k, b + (kOf[y][1] * kTqTerm + (k / 4) * kTqBlock + (k % 4) * 32) / 16,
+                                      idesc_s, y || k ? 1u : 0u);
+                    tc_commit(&s_full[i]);
+                    tc_commit(&k_free[i]);
+                }
+                __syncwarp();
+                return true;
+            };
+            ok = wait(&q_ready, seg & 1u) && scores(c, true);
+#pragma unroll 1
+            for (int32_t n = 0; n < steps && ok; ++n) {
+                const uint32_t s = c + n, i = s & 1;
+                if (n + 1 < steps) ok = scores(s + 1, false);
+                ok = ok && wait(&p_ready[i], (s >> 1) & 1u) && wait(&v_ready[i], (s >> 1) & 1u) && (!s || wait(&o_free, (s - 1) & 1u));
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
+                    const uint32_t a = tmem + kTqPlaces + i * kTqPlace;
+                    const uint64_t b = v_desc + i * (3 * kTqTerm / 16);
+#pragma unroll
+                    for (int y = 0; y < 6; ++y)
+#pragma unroll
+                        for (int k = 0; k < kTqKeys / 16; ++k)
+                            tc_mma_ts(tmem + kTqSums, a + 32 * kOf[y][0] + 8 * k, b + (kOf[y][1] * kTqTerm + k * 16 * 128) / 16, idesc_o, y || k ? 1u : 0u);
+                    tc_commit(&o_full);
+                    tc_commit(&v_free[i]);
+                }
+                __syncwarp();
+            }
+            c += steps;
+        }
+    } else {
+        // ---- all else: sixteen warps
+        pdl_wait();
+        const int quarter = warp >> 2, pair = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const int32_t cta = static_cast<int32_t>(blockIdx.x), pre_tiles = p.header[kTlPreTiles];
+        uint32_t c = 0;  // steps before the segment's
+        // (The sixteen warps meet at barriers, so none leaves alone: a wait that runs out is asked for.)
+        for (uint32_t seg = 0;; ++seg) {
+            ok = wait(&seg_full[seg % kTsSegments], (seg / kTsSegments) & 1u);
+            if (tq_any(!ok)) {
+                ok = false;
+                break;
+            }
+            const TreeSegment t = segments[seg % kTsSegments];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[seg % kTsSegments]);
+            if (!t.steps) break;
+            const int32_t request = t.unused[0], own_limit = t.unused[1];
+            // This warp's rows of a step's keys and values, four each, 16 bytes a lane: loaded ...
+            float4 k_raw[4], v_raw[4];
+            const auto load = [&](int32_t n) {
+                const int32_t step = t.step + n;
+                const bool own = step >= t.pre_steps, there = n < t.steps;
+                const int32_t page = own ? t.own0 + step - t.pre_steps : t.pre0 + step, limit = own ? own_limit : p.prefix;
+                int32_t id = -1;
+                if (there) id = own ? p.tables[static_cast<uint64_t>(max(request, 0)) * p.table_stride + page] : p.prefix_pages[page];
+                const bool good = id >= 0 && id < p.pages;
+                if (there && !good && tid == 0) pg_flag(p.status, PLAMO_PAGED_PAGE);
+                const float *from = static_cast<const float *>(p.pool) +
+                                    ((static_cast<uint64_t>(good ? id : 0) * 2 * kPgRows + 4 * warp) * p.kh + t.head) * static_cast<uint64_t>(kPgDim) + 4 * lane;
+                const uint64_t row = static_cast<uint64_t>(p.kh) * kPgDim;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const bool in = good && page * kTqKeys + 4 * warp + y < limit;
+                    k_raw[y] = in ? ld4(from + y * row) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v_raw[y] = in ? ld4(from + (kPgRows + y) * row) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            };
+            // ... and put into shared memory as terms.
+            const auto put = [&](float4 (&raw)[4], unsigned char *to, uint32_t s, bool keys) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int row = 4 * warp + y;
+                    float4 v = raw[y];
+                    const uint32_t odd = __ballot_sync(0xffffffffu, !tq_finite(v));
+                    if (odd) {
+                        v = make_float4(tq_or_zero(v.x), tq_or_zero(v.y), tq_or_zero(v.z), tq_or_zero(v.w));
+                        if (lane == 0) {
+                            if (keys) atomicOr(&odd_keys[s & 3][row >> 5], 1u << (row & 31));
+                            else odd_values = 1;
+                        }
+                    }
+                    uint32_t a[3], b[3];
+                    tq_split(v.x, v.y, a);
+                    tq_split(v.z, v.w, b);
+                    unsigned char *at = to + (s & 1) * 3 * kTqTerm + (lane >> 4) * kTqBlock + row * 128 + ((((lane & 15) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) *reinterpret_cast<uint2 *>(at + x * kTqTerm) = make_uint2(a[x], b[x]);
+                }
+                fence_async_shared();
+                __syncwarp();
+            };
+            const auto put_keys = [&](uint32_t s) {
+                if (s >= 2 && !wait(&k_free[s & 1], ((s >> 1) - 1) & 1u)) return false;
+                put(k_raw, keys_at, s, true);
+                if (lane == 0) mbar_arrive(&k_ready[s & 1]);
+                return true;
+            };
+            const auto put_values = [&](uint32_t s) {
+                if (s >= 2 && !wait(&v_free[s & 1], ((s >> 1) - 1) & 1u)) return false;
+                put(v_raw, values_at, s, false);
+                if (lane == 0) mbar_arrive(&v_ready[s & 1]);
+                return true;
+            };
+            load(0);
+            const bool there = pair < t.pairs;
+            const int32_t local = p.by_group.div(pair), row = t.row0 + local, head = t.head * p.group + pair - local * p.group;
+            const float *const query = static_cast<const float *>(p.q) + static_cast<int64_t>(there ? row : t.row0) * static_cast<int64_t>(p.q_stride) + (there ? head : 0) * kPgDim;
+            // 32 dimensions of this row's query into tensor memory; the last segment's products are done with it.
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t term[3][8];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float4 v = there ? ld4(query + 32 * quarter + 16 * half + 4 * y) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    uint32_t a[3], b[3];
+                    tq_split(v.x, v.y, a);
+                    tq_split(v.z, v.w, b);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) term[x][2 * y] = a[x], term[x][2 * y + 1] = b[x];
+                }
+#pragma unroll
+                for (int x = 0; x < 3; ++x) tmem_st8(lanes + kTqQueries + 64 * x + 16 * quarter + 8 * half, term[x]);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready);
+            ok = put_keys(c) && put_values(c);
+            load(1);
+            int32_t held = t.held, added = t.added, from = 0;  // `from`: bits of the mask below it are outside the window
+            TreeSees sees{0, 0, 0};
+            if (p.window && there) {
+                if (held < 0) {  // rows of many requests
+                    const int4 e = p.short_list[row - p.header[kTlFirst]];
+                    held = max(e.y, 0);
+                    added = listed_added(p, e);
+                }
+                sees = tree_sees(p, tree_skip(p, row, held, added), held);
+                from = tree_first(p, row, added, sees.drop);
+            }
+            float o[32], m = -INFINITY, l = 0.0f, later = 1.0f;  // `later`: what the step's sums on their way are multiplied with
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0.0f;
+            const auto fold = [&](uint32_t s) {  // adds step s's sums
+                if (!wait(&o_full, s & 1u)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t x[16];
+                    tmem_ld16_async(lanes + kTqSums + 32 * quarter + 16 * half, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[16 * half + k] = fmaf(__uint_as_float(x[k]), later, o[16 * half + k]);
+                }
+                later = 1.0f;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&o_free);
+                return true;
+            };
+#pragma unroll 1
+            for (int32_t n = 0; n < t.steps; ++n) {
+                const uint32_t s = c + n;
+                const int32_t step = t.step + n;
+                const bool own = step >= t.pre_steps;
+                if (n + 1 < t.steps) ok = ok && put_keys(s + 1);
+                // ---- this thread's 16 keys of the step: which of them the row sees
+                const int32_t key0 = (own ? t.own0 + step - t.pre_steps : t.pre0 + step) * kTqKeys + 16 * quarter;
+                const int32_t hi = min(max((own ? held : p.prefix) - key0, 0), 16);
+                const int32_t lo = min(max((own ? sees.lo : sees.pre) - key0, 0), 16);
+                uint32_t see = 0;
+                if (there) {
+                    see = tl_bits(lo, hi);
+                    if (own && key0 + 16 > held) see |= tree_bits(p, row, added, from, key0 - held);
+                }
+                ok = ok && wait(&s_full[s & 1], (s >> 1) & 1u);
+                const uint32_t at = lanes + kTqPlaces + (s & 1) * kTqPlace;
+                float x[16], top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[k] = -INFINITY;
+                if (ok) {
+                    tc_fence_after();
+                    uint32_t raw[16];
+                    tmem_ld16_async(at + 16 * quarter, raw);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) x[k] = (see >> k) & 1u ? __uint_as_float(raw[k]) * p.scale2 : -INFINITY;
+                    uint32_t odd = (odd_keys[s & 3][quarter >> 1] >> (16 * (quarter & 1))) & see & 0xffffu;
+                    if (odd) {
+                        // Keys with a number that is not finite: their scores one by one.
+                        const int32_t page = key0 / kTqKeys;
+                        const int32_t id = own ? p.tables[static_cast<uint64_t>(max(request, 0)) * p.table_stride + page] : p.prefix_pages[page];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            if (!((odd >> k) & 1u)) continue;
+                            const float *key = static_cast<const float *>(p.pool) +
+                                               ((static_cast<uint64_t>(id) * 2 * kPgRows + 16 * quarter + k) * p.kh + t.head) * static_cast<uint64_t>(kPgDim);
+                            float dot = 0.0f;
+#pragma unroll 1
+                            for (int d = 0; d < kPgDim; ++d) dot = fmaf(query[d], key[d], dot);
+                            x[k] = dot * p.scale2;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) top = fmaxf(top, x[k]);
+                    tc_fence_before();
+                }
+                // The reference point of a row moves when some key passes it by 2^8, for all four quarters
+                // alike. The barrier also says that all have read the scores, which the weights replace.
+                if (tq_any(top > m + kLazy)) {
+                    tops[quarter][pair] = top;
+                    tq_any(false);
+                    const float all = fmaxf(fmaxf(tops[0][pair], tops[1][pair]), fmaxf(tops[2][pair], tops[3][pair]));
+                    if (all > m + kLazy) {
+                        const float factor = pg_exp2(m - all);
+                        m = all;
+                        l *= factor;
+                        if (n) later = factor;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] *= factor;
+                    }
+                    tq_any(false);  // before the next step's
+                }
+                if (tq_any(!ok)) {  // (all leave together)
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                {
+                    const float shift = m == -INFINITY ? 0.0f : m;
+                    uint32_t term[3][8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float a = pg_exp2(x[2 * k] - shift), b = pg_exp2(x[2 * k + 1] - shift);
+                        l += a + b;
+                        uint32_t w[3];
+                        tq_split(a, b, w);
+#pragma unroll
+                        for (int y = 0; y < 3; ++y) term[y][k] = w[y];
+                    }
+#pragma unroll
+                    for (int y = 0; y < 3; ++y) tmem_st8(at + 32 * y + 8 * quarter, term[y]);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_ready[s & 1]);
+                }
+                if (tid < 2) odd_keys[(s + 3) & 3][tid] = 0;  // (step s - 1's: of no more use, and not yet of step s + 3's)
+                if (n) ok = ok && fold(s - 1);
+                if (n + 1 < t.steps) {
+                    ok = ok && put_values(s + 1);
+                    load(n + 2);
+                }
+            }
+            ok = ok && fold(c + t.steps - 1);
+            c += t.steps;
+            // ---- the segment's sums
+            tops[quarter][pair] = l;
+            if (tq_any(!ok)) {
+                ok = false;
+                break;
+            }
+            l = (tops[0][pair] + tops[1][pair]) + (tops[2][pair] + tops[3][pair]);
+            if (*reinterpret_cast<volatile int *>(&odd_values) && there) {
+                float with[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) with[k] = o[k];
+                tq_add_odd_values(p, t, row, held, added, sees, from, 32 * quarter, with);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = with[k];
+            }
+            const bool whole = t.steps == t.tile_steps && t.tile >= pre_tiles && !p.share;
+            const int64_t place = static_cast<int64_t>(2 * p.tile_grid + cta + t.tile * p.kh + t.head) * kTqPairs + pair;
+            if (whole) {
+                if (there) {
+                    const float inv = tree_inverse(p, row, held, added, l);
+                    float *to = static_cast<float *>(p.out) + row * p.out_stride + head * kPgDim + 32 * quarter;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(to + k) = make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv);
+                }
+            } else {
+                // Four lanes write 128 bytes of one row at a time: a line is written once.
+                uint32_t v[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(o[k]);
+                transpose_blocks(v);
+                float *to = p.tile_sum + (place - (lane & 3)) * kPgDim + 32 * quarter + 8 * (lane & 3);
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    if (pair - (lane & 3) + y < t.pairs) store_256(to + y * kPgDim, v + 8 * y);
+                if (there && quarter == 0) p.tile_ml[place] = pg_ml(m, l);
+            }
+            tq_any(false);  // before the next segment's tops
+        }
+    }
+    if (!ok && lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kTqProducts) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+}  // namespace plamo
