@@ -28,15 +28,16 @@ constexpr int kTqTerm = kTqKeys * kPgDim * 2, kTqBlock = kTqKeys * 128;  // byte
 constexpr int kTqSmem = 1024 + 4 * 3 * kTqTerm;
 constexpr uint32_t kTqQueries = 0, kTqSums = 192, kTqPlaces = 320, kTqPlace = 96;  // columns
 
-// A pair of numbers as terms; of finite ones all.
-__device__ __forceinline__ void tq_split(float a, float b, uint32_t (&t)[3]) {
-    t[0] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-    a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-    b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-    t[1] = pg_pack(a, b);
-    t[2] = pg_pack(a - bf16_lo(t[1]), b - bf16_hi(t[1]));
+// A pair of finite numbers as terms: the upper halves, what is left rounded, and what is left then rounded.
+__device__ __forceinline__ void tq_split(uint32_t a, uint32_t b, uint32_t (&t)[3]) {
+    const uint64_t less = pair_of(-1.0f, -1.0f);
+    t[0] = __byte_perm(a, b, 0x7632);
+    uint64_t left = fma_pair(pair_of(a & 0xffff0000u, b & 0xffff0000u), less, pair_of(a, b));
+    t[1] = pg_pack(low_of(left), high_of(left));
+    left = fma_pair(pair_of(t[1] << 16, t[1] & 0xffff0000u), less, left);
+    t[2] = pg_pack(low_of(left), high_of(left));
 }
-__device__ __forceinline__ bool tq_finite(const float4 &v) { return isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w); }
+__device__ __forceinline__ void tq_split(float a, float b, uint32_t (&t)[3]) { tq_split(__float_as_uint(a), __float_as_uint(b), t); }
 __device__ __forceinline__ float tq_or_zero(float x) { return isfinite(x) ? x : 0.0f; }
 
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -231,6 +232,8 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
         const int quarter = warp >> 2, pair = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const int32_t cta = static_cast<int32_t>(blockIdx.x), pre_tiles = p.header[kTlPreTiles];
+        const float scale2 = fabsf(p.scale2);
+        const uint32_t flip = p.scale2 < 0.0f ? 0x80000000u : 0u;
         uint32_t c = 0;  // steps before the segment's
         // (The sixteen warps meet at barriers, so none leaves alone: a wait that runs out is asked for.)
         for (uint32_t seg = 0;; ++seg) {
@@ -244,44 +247,55 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
             if (lane == 0) mbar_arrive(&seg_empty[seg % kTsSegments]);
             if (!t.steps) break;
             const int32_t request = t.unused[0], own_limit = t.unused[1];
-            // This warp's rows of a step's keys and values, four each, 16 bytes a lane: loaded ...
+            // This warp's rows of a step's keys and values, four each, 16 bytes a lane: loaded a step ahead, the
+            // page's id two ...
             float4 k_raw[4], v_raw[4];
-            const auto load = [&](int32_t n) {
+            const auto page_id = [&](int32_t n) {
                 const int32_t step = t.step + n;
-                const bool own = step >= t.pre_steps, there = n < t.steps;
-                const int32_t page = own ? t.own0 + step - t.pre_steps : t.pre0 + step, limit = own ? own_limit : p.prefix;
-                int32_t id = -1;
-                if (there) id = own ? p.tables[static_cast<uint64_t>(max(request, 0)) * p.table_stride + page] : p.prefix_pages[page];
-                const bool good = id >= 0 && id < p.pages;
-                if (there && !good && tid == 0) pg_flag(p.status, PLAMO_PAGED_PAGE);
-                const float *from = static_cast<const float *>(p.pool) +
-                                    ((static_cast<uint64_t>(good ? id : 0) * 2 * kPgRows + 4 * warp) * p.kh + t.head) * static_cast<uint64_t>(kPgDim) + 4 * lane;
+                const bool own = step >= t.pre_steps;
+                const int32_t *table = own ? p.tables + static_cast<uint64_t>(max(request, 0)) * p.table_stride + t.own0 - t.pre_steps : p.prefix_pages + t.pre0;
+                return n < t.steps ? table[step] : 0;
+            };
+            const auto load = [&](float4 (&raw)[4], int32_t n, int32_t id, int kind) {
+                const int32_t step = t.step + n;
+                const bool own = step >= t.pre_steps, good = id >= 0 && id < p.pages;
+                const int32_t left = (own ? own_limit - (t.own0 + step - t.pre_steps) * kTqKeys : p.prefix - (t.pre0 + step) * kTqKeys) - 4 * warp;
+                if (!good && tid == 0) pg_flag(p.status, PLAMO_PAGED_PAGE);
                 const uint64_t row = static_cast<uint64_t>(p.kh) * kPgDim;
+                const float *from = static_cast<const float *>(p.pool) + ((static_cast<uint64_t>(good ? id : 0) * 2 + kind) * kPgRows + 4 * warp) * row +
+                                    t.head * kPgDim + 4 * lane;
+                const int32_t rows = good && n < t.steps ? left : 0;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const bool in = good && page * kTqKeys + 4 * warp + y < limit;
-                    k_raw[y] = in ? ld4(from + y * row) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    v_raw[y] = in ? ld4(from + (kPgRows + y) * row) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
+                for (int y = 0; y < 4; ++y) raw[y] = y < rows ? ld4(from + y * row) : make_float4(0.f, 0.f, 0.f, 0.f);
             };
             // ... and put into shared memory as terms.
-            const auto put = [&](float4 (&raw)[4], unsigned char *to, uint32_t s, bool keys) {
+            unsigned char *const put_at = base + (lane >> 4) * kTqBlock + 4 * warp * 128 + (lane & 1) * 8;
+            const auto put = [&](float4 (&raw)[4], uint32_t to, uint32_t s, bool keys) {
+                uint64_t z = pair_of(0.0f, 0.0f);  // no number where one of them is none
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                    const int row = 4 * warp + y;
-                    float4 v = raw[y];
-                    const uint32_t odd = __ballot_sync(0xffffffffu, !tq_finite(v));
-                    if (odd) {
-                        v = make_float4(tq_or_zero(v.x), tq_or_zero(v.y), tq_or_zero(v.z), tq_or_zero(v.w));
-                        if (lane == 0) {
-                            if (keys) atomicOr(&odd_keys[s & 3][row >> 5], 1u << (row & 31));
+                    z = fma_pair(pair_of(raw[y].x, raw[y].y), pair_of(0.0f, 0.0f), z);
+                    z = fma_pair(pair_of(raw[y].z, raw[y].w), pair_of(0.0f, 0.0f), z);
+                }
+                if (__any_sync(0xffffffffu, low_of(z) + high_of(z) != 0.0f)) {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const float4 v = raw[y];
+                        raw[y] = make_float4(tq_or_zero(v.x), tq_or_zero(v.y), tq_or_zero(v.z), tq_or_zero(v.w));
+                        const bool odd = __any_sync(0xffffffffu, !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w)));
+                        if (odd && lane == 0) {
+                            if (keys) atomicOr(&odd_keys[s & 3][warp >> 3], 1u << (4 * (warp & 7) + y));
                             else odd_values = 1;
                         }
                     }
+                }
+                unsigned char *const at0 = put_at + to + (s & 1) * 3 * kTqTerm;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
                     uint32_t a[3], b[3];
-                    tq_split(v.x, v.y, a);
-                    tq_split(v.z, v.w, b);
-                    unsigned char *at = to + (s & 1) * 3 * kTqTerm + (lane >> 4) * kTqBlock + row * 128 + ((((lane & 15) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
+                    tq_split(raw[y].x, raw[y].y, a);
+                    tq_split(raw[y].z, raw[y].w, b);
+                    unsigned char *const at = at0 + y * 128 + ((((lane & 15) >> 1) ^ ((4 * warp + y) & 7)) << 4);
 #pragma unroll
                     for (int x = 0; x < 3; ++x) *reinterpret_cast<uint2 *>(at + x * kTqTerm) = make_uint2(a[x], b[x]);
                 }
@@ -290,17 +304,19 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
             };
             const auto put_keys = [&](uint32_t s) {
                 if (s >= 2 && !wait(&k_free[s & 1], ((s >> 1) - 1) & 1u)) return false;
-                put(k_raw, keys_at, s, true);
+                put(k_raw, 0, s, true);
                 if (lane == 0) mbar_arrive(&k_ready[s & 1]);
                 return true;
             };
             const auto put_values = [&](uint32_t s) {
                 if (s >= 2 && !wait(&v_free[s & 1], ((s >> 1) - 1) & 1u)) return false;
-                put(v_raw, values_at, s, false);
+                put(v_raw, 2 * 3 * kTqTerm, s, false);
                 if (lane == 0) mbar_arrive(&v_ready[s & 1]);
                 return true;
             };
-            load(0);
+            int32_t id = page_id(0), id_next = page_id(1);
+            load(k_raw, 0, id, 0);
+            load(v_raw, 0, id, 1);
             const bool there = pair < t.pairs;
             const int32_t local = p.by_group.div(pair), row = t.row0 + local, head = t.head * p.group + pair - local * p.group;
             const float *const query = static_cast<const float *>(p.q) + static_cast<int64_t>(there ? row : t.row0) * static_cast<int64_t>(p.q_stride) + (there ? head : 0) * kPgDim;
@@ -324,8 +340,11 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_ready);
-            ok = put_keys(c) && put_values(c);
-            load(1);
+            ok = put_keys(c);
+            load(k_raw, 1, id_next, 0);
+            ok = ok && put_values(c);
+            load(v_raw, 1, id_next, 1);
+            id = page_id(2);
             int32_t held = t.held, added = t.added, from = 0;  // `from`: bits of the mask below it are outside the window
             TreeSees sees{0, 0, 0};
             if (p.window && there) {
@@ -363,6 +382,8 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
                 const int32_t step = t.step + n;
                 const bool own = step >= t.pre_steps;
                 if (n + 1 < t.steps) ok = ok && put_keys(s + 1);
+                load(k_raw, n + 2, id, 0);
+                id_next = page_id(n + 3);
                 // ---- this thread's 16 keys of the step: which of them the row sees
                 const int32_t key0 = (own ? t.own0 + step - t.pre_steps : t.pre0 + step) * kTqKeys + 16 * quarter;
                 const int32_t hi = min(max((own ? held : p.prefix) - key0, 0), 16);
@@ -374,41 +395,55 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
                 }
                 ok = ok && wait(&s_full[s & 1], (s >> 1) & 1u);
                 const uint32_t at = lanes + kTqPlaces + (s & 1) * kTqPlace;
-                float x[16], top = -INFINITY;
+                uint32_t x[16];
+                float top = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) x[k] = -INFINITY;
+                for (int k = 0; k < 16; ++k) x[k] = 0xff800000u;  // -inf
                 if (ok) {
                     tc_fence_after();
-                    uint32_t raw[16];
-                    tmem_ld16_async(at + 16 * quarter, raw);
+                    tmem_ld16_async(at + 16 * quarter, x);
                     tmem_wait_ld();
+                    if (flip) {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) x[k] = (see >> k) & 1u ? __uint_as_float(raw[k]) * p.scale2 : -INFINITY;
-                    uint32_t odd = (odd_keys[s & 3][quarter >> 1] >> (16 * (quarter & 1))) & see & 0xffffu;
-                    if (odd) {
-                        // Keys with a number that is not finite: their scores one by one.
-                        const int32_t page = key0 / kTqKeys;
-                        const int32_t id = own ? p.tables[static_cast<uint64_t>(max(request, 0)) * p.table_stride + page] : p.prefix_pages[page];
+                        for (int k = 0; k < 16; ++k) x[k] ^= flip;
+                    }
+                    const uint32_t odd = (odd_keys[s & 3][quarter >> 1] >> (16 * (quarter & 1))) & see;
+                    if (__any_sync(0xffffffffu, see != 0xffffu || odd)) {
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            if (!((odd >> k) & 1u)) continue;
-                            const float *key = static_cast<const float *>(p.pool) +
-                                               ((static_cast<uint64_t>(id) * 2 * kPgRows + 16 * quarter + k) * p.kh + t.head) * static_cast<uint64_t>(kPgDim);
-                            float dot = 0.0f;
+                        for (int k = 0; k < 16; ++k)
+                            if (!((see >> k) & 1u)) x[k] = 0xff800000u;
+                        if (odd) {
+                            // Keys with a number that is not finite: their scores one by one.
+                            const int32_t page = key0 / kTqKeys;
+                            const int32_t id = own ? p.tables[static_cast<uint64_t>(max(request, 0)) * p.table_stride + page] : p.prefix_pages[page];
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                if (!((odd >> k) & 1u)) continue;
+                                const float *key = static_cast<const float *>(p.pool) +
+                                                   ((static_cast<uint64_t>(id) * 2 * kPgRows + 16 * quarter + k) * p.kh + t.head) * static_cast<uint64_t>(kPgDim);
+                                float dot = 0.0f;
 #pragma unroll 1
-                            for (int d = 0; d < kPgDim; ++d) dot = fmaf(query[d], key[d], dot);
-                            x[k] = dot * p.scale2;
+                                for (int d = 0; d < kPgDim; ++d) dot = fmaf(query[d], key[d], dot);
+                                x[k] = __float_as_uint(dot) ^ flip;
+                            }
                         }
                     }
+                    float y[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) top = fmaxf(top, x[k]);
+                    for (int k = 0; k < 16; k += 4)
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) y[z] = fmaxf(fmaxf(y[z], __uint_as_float(x[k + 2 * z])), __uint_as_float(x[k + 2 * z + 1]));
+                    top = fmaxf(y[0], y[1]) * scale2;
                     tc_fence_before();
                 }
                 // The reference point of a row moves when some key passes it by 2^8, for all four quarters
                 // alike. The barrier also says that all have read the scores, which the weights replace.
-                if (tq_any(top > m + kLazy)) {
+                if (tq_any(top > m + kLazy || !ok)) {
                     tops[quarter][pair] = top;
-                    tq_any(false);
+                    if (tq_any(!ok)) {  // (all leave together)
+                        ok = false;
+                        break;
+                    }
                     const float all = fmaxf(fmaxf(tops[0][pair], tops[1][pair]), fmaxf(tops[2][pair], tops[3][pair]));
                     if (all > m + kLazy) {
                         const float factor = pg_exp2(m - all);
@@ -420,23 +455,22 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
                     }
                     tq_any(false);  // before the next step's
                 }
-                if (tq_any(!ok)) {  // (all leave together)
-                    ok = false;
-                    break;
-                }
                 tc_fence_after();
                 {
-                    const float shift = m == -INFINITY ? 0.0f : m;
+                    const float shift = m == -INFINITY ? 0.0f : -m;
+                    uint64_t sums = pair_of(0.0f, 0.0f);
                     uint32_t term[3][8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const float a = pg_exp2(x[2 * k] - shift), b = pg_exp2(x[2 * k + 1] - shift);
-                        l += a + b;
+                        const uint64_t y = fma_pair(pair_of(x[2 * k], x[2 * k + 1]), pair_of(scale2, scale2), pair_of(shift, shift));
+                        const uint32_t a = __float_as_uint(pg_exp2(low_of(y))), b = __float_as_uint(pg_exp2(high_of(y)));
+                        sums = add_pair(sums, pair_of(a, b));
                         uint32_t w[3];
                         tq_split(a, b, w);
 #pragma unroll
-                        for (int y = 0; y < 3; ++y) term[y][k] = w[y];
+                        for (int z = 0; z < 3; ++z) term[z][k] = w[z];
                     }
+                    l += low_of(sums) + high_of(sums);
 #pragma unroll
                     for (int y = 0; y < 3; ++y) tmem_st8(at + 32 * y + 8 * quarter, term[y]);
                     tmem_wait_st();
@@ -446,10 +480,9 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
                 }
                 if (tid < 2) odd_keys[(s + 3) & 3][tid] = 0;  // (step s - 1's: of no more use, and not yet of step s + 3's)
                 if (n) ok = ok && fold(s - 1);
-                if (n + 1 < t.steps) {
-                    ok = ok && put_values(s + 1);
-                    load(n + 2);
-                }
+                if (n + 1 < t.steps) ok = ok && put_values(s + 1);
+                load(v_raw, n + 2, id, 1);
+                id = id_next;
             }
             ok = ok && fold(c + t.steps - 1);
             c += t.steps;
