@@ -134,8 +134,8 @@ struct plamo_paged_store_args {
    a*cos - b*sin, the upper b*cos + a*sin. */
 int plamo_paged_store(struct plamo_cuda *, const struct plamo_paged_store_args *);
 
-/* The PLAMO_PAGED_* bits that store and attention calls without a word of their
-   own have set since it was last asked; they are then clear. Waits for the
+/* The PLAMO_PAGED_* bits that calls without a word of their own (all but plans and
+   acceptances, whose summary has them) have set since it was last asked; they are then clear. Waits for the
    context's own stream: a call on another one counts once that has run it
    (synchronise it first). PLAMO_PAGED_FAILED also where the word cannot be
    read. Not while a stream is being captured. */
@@ -246,8 +246,8 @@ struct plamo_paged_accept_args {
    for the same step may come after. Where the list cannot have held the pages (fewer
    entries used than come back) none is given back and summary[0] gets
    PLAMO_PAGED_NO_PAGES; a page table too short for its request's rows sets PLAMO_PAGED_TABLE;
-   a step that the plan declined keeps what was held. `summary` may be `plan`
-   itself; outputs overlap nothing else. */
+   a step that the plan declined keeps what was held. Outputs overlap neither
+   one another nor an input. */
 int plamo_paged_accept(struct plamo_cuda *, const struct plamo_paged_accept_args *);
 
 struct plamo_paged_keep_args {

@@ -62,11 +62,31 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
     return nullptr;
 }
 
-// Prefix rows from which trees share tiles over them.
-constexpr uint64_t kTreeShareRows = 1024;
-constexpr uint32_t kTreeShortPairs = 8;
-// What a strip's beginning and end are worth, in units of half a step of a full tile.
+// Draft trees, eight heads to each of four KV heads, requests that hold 430 to 1,455 rows
+// of their own (430 to 455 where it says "held 450").
+//
+// Trees share tiles over a prefix of so many rows or more (BF16, FP32). Such tiles are
+// full; a tree's own leave room, but need no joining with others. So sharing is for
+// trees that fill less than 4/5 of tiles of their own. BF16: 61 of 20 rows behind 2,000,
+// held 450, shared 125 us and not 133, 32 of 8 rows 63 and 61, behind 600 50 and 46; 16 of 32 rows,
+// full tiles, behind 2,000 70 and 64. FP32: 32 of 8 rows behind 2,000, held 450, 166 and 221,
+// 12 of 8 rows behind 600 60 and 62, of 10 rows 61 and 64.
+constexpr uint64_t kTreeShareRows = 1024, kTreeShareRowsF32 = 512;
+// Pairs up to which a request's own rows are the row kernel's, which has tiles of eight.
+// BF16: 32 requests of 4 rows behind 2,000 89 us in it and 52 in tiles, of 2 rows 58 and
+// 46. FP32: 32 of 4 rows behind 2,000 330 and 165, 12 behind 1,000 90 and 84, 32 with no
+// prefix, held 450, 70 and 74; but 12 of 2 rows behind 1,000 54 and 83, 32 behind 2,000 171 and 144.
+constexpr uint32_t kTreeShortPairs = 8, kTreeShortPairsF32 = 16;
+// As kTlPromptUnits, for FP32 trees, whose tile kernel takes less than the plain one: one
+// request of 16 rows behind 12, held 450, 23 us in the row kernel and 31 in tiles, two 36 and 33, three 43 and 33.
+constexpr uint64_t kTreePromptUnitsF32 = 1000;
+// What a strip's beginning and end are worth, in units of half a step of a full tile (BF16)
+// or a step (FP32), where the work is divided. BF16, 4 / 8 / 12 / 16: 64 trees of 64 rows behind 8,192
+// 1,075 / 957 / 870 / 913 us, 61 of 20 to 32 behind 2,000 218 / 205 / 208 / -. FP32, 0 / 2 / 4 / 6: 8 trees of 16
+// behind 12, held 450, 51 / 45 / 45 / 49, 24 behind 12 128 / 113 / 119 / 131, 60 of 24 behind 1,000 651 / 655 / 658 / 674.
 constexpr int32_t kTreeStripPad = 12, kTreeStripPadF32 = 2;
+// A CTA has no fewer units than this: 8 trees of 16 in FP32, 1 / 2 / 4: 45 / 45 / 50 us.
+constexpr int32_t kTreeLeast = 4, kTreeLeastF32 = 1;
 
 // How an attention call is laid out: the workspace's parts and the grid.
 struct AttentionLayout {
@@ -110,18 +130,16 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     const uint64_t strips = ceil_div(pairs, kRtPairs) * d->kv_heads;
     const uint64_t prefix_steps = ceil_div(pairs, kTlPairs) * d->kv_heads * ceil_div(d->prefix_rows, kTlKeys);
     const uint64_t most = d->most_new ? std::min(d->most_new, d->rows) : d->rows > d->requests ? d->rows : 0;  // rows of a request
-    a.short_pairs = trees && !f32 ? kTreeShortPairs : kTlShortPairs;
+    a.short_pairs = !trees ? kTlShortPairs : f32 ? kTreeShortPairsF32 : kTreeShortPairs;
     const bool prompts = most * group > a.short_pairs;
-    if (group <= tile_pairs && ((prompts && strips * (prefix_pages + d->table_stride) > kTlPromptUnits) ||
+    if (group <= tile_pairs && ((prompts && strips * (prefix_pages + d->table_stride) > (trees && f32 ? kTreePromptUnitsF32 : kTlPromptUnits)) ||
                                 (!f32 && strips * prefix_pages > kTlPrefixUnits + 4 * prefix_steps))) {
         a.tile_rows = static_cast<uint32_t>(tile_pairs / group);
         a.tile_grid = static_cast<uint32_t>(f32 && !trees ? 2 * sms : sms);
         // Prefix tiles of the short requests' rows, and each prompt's own with a last partial one.
         a.tile_cap = static_cast<uint32_t>(2 * ceil_div(d->rows, a.tile_rows) + std::min(d->requests, d->rows));
-        // Tiles over the prefix that all trees share are full; their own have room for whole rows of
-        // one tree only, but need no joining with others.
         const uint64_t room = d->requests * ceil_div(std::max<uint64_t>(most, 1), a.tile_rows) * tile_pairs;
-        a.share = trees && d->prefix_rows >= kTreeShareRows && 5 * pairs < 4 * room;
+        a.share = trees && d->prefix_rows >= (f32 ? kTreeShareRowsF32 : kTreeShareRows) && 5 * pairs < 4 * room;
         // (tiles of their own that have the prefix, too, leave the row kernel nothing to share it with)
         if (trees && !a.share && d->prefix_rows) a.short_pairs = 0;
         a.split_pairs = trees && !f32 ? kTlPairs / 2 : 0;
@@ -203,7 +221,7 @@ bool run_attention(plamo_cuda *c, const plamo_paged_attention_args *d, const Tre
     p.split_pairs = static_cast<int32_t>(a.split_pairs);
     p.step_units = F32 ? 1 : 2;
     p.strip_pad = F32 ? kTreeStripPadF32 : kTreeStripPad;
-    p.least_units = F32 ? 1 : 4;
+    p.least_units = F32 ? kTreeLeastF32 : kTreeLeast;
     p.scale2 = d->scale * 1.4426950408889634f;
     // The tile kernel masks before it scales: -inf must stay so.
     if (std::fabs(p.scale2) < 1e-30f) p.scale2 = std::copysign(1e-30f, p.scale2);

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
                 TreeSegment t{};
                 if (more)
                     t = TreeSegment{w.steps, 0, w.tile, w.head, w.step, w.tile_steps, s.request < 0 ? first_row + s.row0 : s.row0, s.rows * p.group,
-                                    s.request < 0 ? -1 : s.at0, s.added, s.pre0, s.pre1 - s.pre0, s.own0, {s.request, s.own_limit, 0}};
+                                    s.request < 0 ? -1 : s.at0, s.added, s.pre0, s.pre1 - s.pre0, s.own0, s.request, s.own_limit, 0};
                 segments[e] = t;
                 mbar_arrive(&seg_full[e]);
             }
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
             __syncwarp();
             if (lane == 0) mbar_arrive(&seg_empty[seg % kTsSegments]);
             if (!t.steps) break;
-            const int32_t request = t.unused[0], own_limit = t.unused[1];
+            const int32_t request = t.request, own_limit = t.own_limit;
             // This warp's rows of a step's keys and values, four each, 16 bytes a lane: loaded a step ahead, the
             // page's id two ...
             float4 k_raw[4], v_raw[4];

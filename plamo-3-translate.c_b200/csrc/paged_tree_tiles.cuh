@@ -1,5 +1,5 @@
 // Attention of draft trees on the tensor cores: BF16, tiles of up to 256 (row,
-// head) pairs by steps of 128 keys. FP32 trees have paged_tile_f32_kernel.
+// head) pairs by steps of 128 keys. FP32 trees have paged_tree_f32_kernel.
 #pragma once
 #include "paged_tiles.cuh"
 
@@ -35,7 +35,8 @@ struct __align__(16) TreeSegment {
     int32_t tile, head, step, tile_steps;
     int32_t row0, pairs, held, added;  // first batch row; the tile's pairs; its request's held (-1: of many requests) and new rows
     int32_t pre0, pre_steps, own0;     // first key step and number of steps over the prefix, first over its own rows
-    int32_t unused[3];
+    int32_t request, own_limit;        // its request (-1: of many) and the end of its own rows
+    int32_t unused;
 };
 // The units (keys or values of one step) of a segment come in rounds: a step's keys
 // and values, or, of split tiles, the keys and then the values of two steps, one for
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kTsThreads, 1)
                 TreeSegment t{};
                 if (more)
                     t = TreeSegment{w.steps, split, w.tile, w.head, w.step, w.tile_steps, row0, s.rows * p.group,
-                                    s.request < 0 ? -1 : s.at0, s.added, s.pre0, pre_steps, s.own0, {}};
+                                    s.request < 0 ? -1 : s.at0, s.added, s.pre0, pre_steps, s.own0, s.request, s.own_limit, 0};
                 if (ok) segments[e] = t;
                 if (ok) mbar_arrive(&seg_full[e]);
             }

@@ -623,7 +623,7 @@ class Backend:
         return paged.adapters(self, x, base, a, b, ids, starts, scales, out, status, most_new)
 
     def paged_status(self):
-        """PLAMO_PAGED_* bits of stores and attention calls without a status tensor; see paged.status."""
+        """PLAMO_PAGED_* bits of calls without a status tensor; see paged.status."""
         return paged.status(self)
 
     def __enter__(self):

@@ -389,8 +389,8 @@ def adapters(backend, x, base, a, b, ids, starts, scales=None, out=None, status=
 
 
 def status(backend):
-    """PLAMO_PAGED_* bits set by stores and attention calls without a `status`
-    tensor since last asked (they are then clear). Waits for torch's current
+    """PLAMO_PAGED_* bits set by calls without a `status` tensor (all but plans and
+    acceptances, whose summary has them) since last asked (they are then clear). Waits for torch's current
     stream; calls on others count once those have run them."""
     _torch().cuda.current_stream(backend.device).synchronize()
     return backend.lib.plamo_paged_status(backend.ctx)

@@ -1,10 +1,13 @@
 """Draft trees in a paged batch (include/plamo_paged.h) against 64-bit statements:
 masks and positions, attention, the confirmed path, the moved rows, refusals
 and status bits, streams, graphs and a whole step."""
+import importlib.util
+import os
+
 import pytest
 import torch
 
-from conftest import load_package
+from conftest import ROOT, load_package
 from paged_reference import DIM, ROWS, Scene, check, pages_for
 from paged_tree_reference import TreeScene, accept_by_hand, random_tree, signed, tree_by_hand
 
@@ -586,3 +589,15 @@ def test_refusals(be):
             be.paged_attention(q, pool, s, n, tables, masks=masks.cuda())
     s2 = Scene([(3, 1)], 0, 8, 2, BF16)
     check(be.paged_attention(s2.q, s2.pool, s2.starts, s2.lengths, s2.tables), *s2.expected())
+
+
+@pytest.mark.parametrize("args", [[], ["--bf16"], ["--requests", "70", "--steps", "6", "--prefix", "1100"]])
+def test_example_decodes_with_drafts_as_row_by_row(args):
+    """FP32 pools: rows in trees and alone differ by 1e-6 or so, the two likeliest tokens' scores by more. In BF16 a
+    rounding may choose another token, and what follows is another text."""
+    spec = importlib.util.spec_from_file_location("paged_trees", os.path.join(ROOT, "examples", "paged_trees.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    drafted, plain = module.main(args)
+    for d, p in zip(drafted, plain, strict=True):
+        assert len(d) <= len(p) and (d == p[:len(d)] or "--bf16" in args)
