@@ -323,10 +323,12 @@ struct AdaptersLayout {
     uint64_t bytes;
 };
 // Where a warp takes 16 rows of one request instead of a CTA eight of any: requests of that many
-// rows, and enough of them. FP32, rank 16: 16 requests of 24 rows 19 us so and 20 the other
-// way, 64 of 16 27 and 39; BF16, rank 64: 32 of 16 28 and 33, 8 of 16 25 and 19; rank 128 holds
-// more in registers than it hides: 32 of 16 60 and 51, 16 of 500 426 and 874.
-constexpr uint64_t kAdTallRows = 12, kAdTallAll = 384, kAdTallAllWide = 1024;
+// rows, and enough of them; of ranks above 64, of which less is on its way at a time, more
+// (8B QKV, so / the other way). FP32, rank 32: 128 requests of 4 rows 43 us / 30, of 6
+// 42 / 39, of 8 31 / 47; rank 64: 16 of 16 27 / 23, 128 of 6 59 / 56, of 8 45 / 66; BF16, rank 64: 8 of 16 25 / 19,
+// 32 of 16 29 / 31, 100 of 4 37 / 27, of 8 31 / 39. FP32, rank 128: 256 of 8 242 / 200, 64 of 16
+// 104 / 101, 16 of 40 71 / 64, 32 of 40 102 / 112, 16 of 500 469 / 714.
+constexpr uint64_t kAdTallRows = 8, kAdTallAll = 384, kAdTallRowsWide = 12, kAdTallAllWide = 1024;
 
 // Parts that the `rounds` stages of each of `tiles` CTAs' work are cut into: those that end
 // first, of the most that one, two, three or four rounds of CTAs hold, two to an SM. A
@@ -354,7 +356,8 @@ uint64_t tall_ctas(const plamo_paged_adapters_args *d, bool about) {
 AdaptersLayout adapters_layout(const plamo_cuda *c, const plamo_paged_adapters_args *d) {
     AdaptersLayout a{};
     const uint64_t sms = context_sms(c), longest = 1ull << 34;  // row strides that a tensor map holds
-    a.tall = d->rows >= kAdTallRows * d->requests && d->rows >= (d->rank <= 64 ? kAdTallAll : kAdTallAllWide) && d->rank <= kAdTallRank && d->x_stride < longest &&
+    const bool wide = d->rank > kAdTallRanks;
+    a.tall = d->rows >= (wide ? kAdTallRowsWide : kAdTallRows) * d->requests && d->rows >= (wide ? kAdTallAllWide : kAdTallAll) && d->rank <= kAdTallRank && d->x_stride < longest &&
              d->base_stride < longest && d->out_stride < longest;
     if (a.tall) {
         const uint64_t round = 256 / element_bytes(d->x_type), rounds = ceil_div(d->columns, round);
@@ -376,8 +379,7 @@ template <typename X>
 AdapterTallInner adapters_tall_inner(uint64_t rank) {
     return rank <= 16   ? paged_adapters_tall_inner_kernel<X, 2>
            : rank <= 32 ? paged_adapters_tall_inner_kernel<X, 4>
-           : rank <= 64 ? paged_adapters_tall_inner_kernel<X, 8>
-                        : paged_adapters_tall_inner_kernel<X, 16>;
+                        : paged_adapters_tall_inner_kernel<X, 8>;
 }
 template <typename T>
 AdapterTallOuter adapters_tall_outer(uint64_t rank) {
@@ -401,7 +403,7 @@ bool run_tall_adapters(plamo_cuda *c, const plamo_paged_adapters_args *d, const 
     const AdapterTallInner inner = d->x_type == PLAMO_PAGED_FP32 ? adapters_tall_inner<float>(d->rank) : adapters_tall_inner<uint16_t>(d->rank);
     const AdapterTallOuter outer = d->type == PLAMO_PAGED_FP32 ? adapters_tall_outer<float>(d->rank) : adapters_tall_outer<uint16_t>(d->rank);
     const uint64_t blocks = ceil_div(d->outputs, 256 / element_bytes(d->type)), per = ceil_div(blocks, parts_for(tall_ctas(d, true), blocks, sms));
-    return launch(c, "paged_adapters inner", inner, dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(p.splits)), dim3(kAdTileThreads),
+    return launch(c, "paged_adapters inner", inner, dim3(static_cast<uint32_t>(tiles * ceil_div(d->rank, kAdTallRanks)), static_cast<uint32_t>(p.splits)), dim3(kAdTileThreads),
                   kAdTileSmem, stream, false, x_map, p) &&
            launch(c, "paged_adapters outer", outer, dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(ceil_div(blocks, per))),
                   dim3(kAdTileThreads), kAdTileSmem, stream, true, base_map, out_map, p, static_cast<int32_t>(per));
@@ -423,7 +425,7 @@ bool run_adapters(plamo_cuda *c, const plamo_paged_adapters_args *d, const Adapt
 template <typename T>
 cudaError_t configure_adapters() {
     cudaError_t e = cudaSuccess;
-    for (const uint64_t rank : {16, 32, 64, 128}) {
+    for (const uint64_t rank : {16, 32, 64, kAdTallRank}) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(adapters_tall_inner<T>(rank), cudaFuncAttributeMaxDynamicSharedMemorySize, kAdTileSmem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(adapters_tall_outer<T>(rank), cudaFuncAttributeMaxDynamicSharedMemorySize, kAdTileSmem);
     }

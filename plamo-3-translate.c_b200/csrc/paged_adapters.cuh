@@ -243,9 +243,9 @@ __global__ void __launch_bounds__(kAdThreads, 5) paged_adapters_outer_kernel(con
         float total[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int32_t run = 0; run < count; ++run) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
             for (int32_t chunk = 0; chunk < chunks; ++chunk) {
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
                 uint4 w[2][2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) w[k][0] = ahead[k][0], w[k][1] = ahead[k][1];
@@ -263,11 +263,11 @@ __global__ void __launch_bounds__(kAdThreads, 5) paged_adapters_outer_kernel(con
                         mma_bf16(s, m1, v.z, v.w);
                     }
                 }
-            }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int row = 2 * t + (k & 1);
-                if (row >= runs.first[run] && row < runs.end[run]) total[k] = s[k];
+                for (int k = 0; k < 4; ++k) {
+                    const int row = 2 * t + (k & 1);
+                    if (row >= runs.first[run] && row < runs.end[run]) total[k] += s[k];
+                }
             }
         }
 #pragma unroll
@@ -286,8 +286,9 @@ __global__ void __launch_bounds__(kAdThreads, 5) paged_adapters_outer_kernel(con
 // A warp takes 16 rows of one request, now the M of its MMAs, and the adapter's rows are
 // their N. x (and base and out) come and go by the copy engine, 256 bytes of each row
 // at a time through a ring; two CTAs of 98 KB to an SM keep 190 KB on their way.
-// (Loads into registers, whose number bounds what is on its way, took 73 us for the
-// inner sums of 7,952 rows and rank 32, and 102 for the outputs.) The order along the
+// (16 prompts of 129 to 1,023 rows, rank 32, 4,096 columns and outputs, FP32: inner 48 us,
+// outputs 56, at 3.1 and 5.4 TB/s; with loads into registers, whose number bounds what is on
+// its way, 73 and 102.) The order along the
 // contraction is free, so lane t of four takes columns 8 t to 8 t + 7 of 32, whole
 // 16-byte pieces of a row. The adapter's pieces come from the L1 cache, which the
 // CTA's warps mostly share, a block or two ahead. HBM bounds both kernels up to ranks of
@@ -358,7 +359,7 @@ struct AdTile {
 // The CTA's four: every request's rows by sixteens, in order, and the rows before the
 // first request's and behind the last one's. Rows without an adapter are left out
 // unless `copied`. Each CTA finds its own, a few loads to a thread and a scan.
-__device__ __forceinline__ void ad_tiles(const AdapterParams &p, bool copied, AdTile *tiles) {
+__device__ __forceinline__ void ad_tiles(const AdapterParams &p, uint32_t cta, bool copied, AdTile *tiles) {
     __shared__ int64_t sums[kAdTileThreads / 32];
     const int tid = threadIdx.x;
     if (tid < kAdTileWarps) tiles[tid].rows = 0;
@@ -378,7 +379,7 @@ __device__ __forceinline__ void ad_tiles(const AdapterParams &p, bool copied, Ad
     int64_t count = 0, total;
 #pragma unroll 1
     for (int32_t e = e0; e < e1; ++e) count += (entry(e).rows + kAdTall - 1) / kAdTall;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kAdTileWarps;
+    const int64_t first = static_cast<int64_t>(cta) * kAdTileWarps;
     int64_t at = pg_block_scan<kAdTileThreads>(count, sums, &total);
 #pragma unroll 1
     for (int32_t e = e0; e < e1 && at < first + kAdTileWarps; ++e) {
@@ -445,20 +446,26 @@ __device__ __forceinline__ void ad_copy(const AdapterParams &p, const AdRing &r,
         if (!ad_wait(&r.full[k % kAdStages], (k / kAdStages) & 1u)) break;
 }
 
-// x: the tiles' rows by a share of the columns; ranks to a CTA: 8 NT.
+// x: the tiles' rows by a share of the columns; ranks to a CTA: 8 NT, of 64 at most (more
+// would leave no registers for what is on its way), so that x comes once for each 64, the second
+// time from L2. The chain of MMAs that a stage's columns make for two tiles of eight ranks at a
+// time starts from zero and is folded in FP32: tensor cores cut what they add up, by
+// 6e-6 over 4,096 columns in one chain, which is 1.5e-7 so.
+constexpr int kAdTallRanks = 64;
 template <typename X, int NT>
 __global__ void __launch_bounds__(kAdTileThreads, 2)
     paged_adapters_tall_inner_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ AdapterParams p) {
     constexpr int TERMS = sizeof(X) == 4 ? 3 : 1, COLUMNS = 2 * ad_box_columns<X>(), BLOCKS = COLUMNS / kAdBlock;  // to a stage
-    constexpr int WIDE = NT <= 8 ? NT : 8;  // tiles of the adapter loaded at a time
-    constexpr int AHEAD = NT <= 4 ? 2 : 1;  // so many ahead
+    constexpr int PAIRS = NT / 2, AHEAD = TERMS == 1 || PAIRS < 2 ? 1 : PAIRS;  // pairs of tiles of the adapter; so many on their way
     extern __shared__ __align__(128) unsigned char ad_smem[];
     __shared__ __align__(8) uint64_t full[kAdStages], empty[kAdStages];
     __shared__ AdTile tiles[kAdTileWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
+    const int32_t groups = (p.rank + kAdTallRanks - 1) / kAdTallRanks;
+    const int32_t rank0 = static_cast<int32_t>(blockIdx.x % groups) * kAdTallRanks, ranks = p.rank - rank0;
     const AdRing ring = ad_ring(ad_smem, full, empty, &map);
-    ad_tiles(p, false, tiles);
+    ad_tiles(p, blockIdx.x / groups, false, tiles);
     if (!tiles[0].rows) return;
     const int32_t begin = blockIdx.y * p.share, end = min(begin + p.share, p.columns);
     const int32_t stages = (end - begin + COLUMNS - 1) / COLUMNS;
@@ -468,14 +475,16 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
     }
     const AdTile tile = tiles[warp];
     const bool there = tile.rows > 0;
-    const uint16_t *const a = p.a + (static_cast<uint64_t>(max(tile.id, 0)) * p.rank + g) * p.columns + 8 * t;
-    uint4 w[AHEAD][WIDE];
-    const auto fetch = [&](int32_t c, int j0, uint4 (&w)[WIDE]) {  // columns c + 8 t of adapter rows 8 (j0 + j) + g
-        const bool in = there && c + 8 * t < end;
+    const uint16_t *const a = p.a + (static_cast<uint64_t>(max(tile.id, 0)) * p.rank + rank0 + g) * p.columns + 8 * t;
+    uint4 w[AHEAD][2][BLOCKS];
+    const auto fetch = [&](int32_t c, int q, uint4 (&w)[2][BLOCKS]) {  // columns c + 8 t of a stage's blocks, adapter rows 16 q + 8 i + g
 #pragma unroll
-        for (int j = 0; j < WIDE; ++j)
-            w[j] = in && 8 * (j0 + j) + g < p.rank ? *reinterpret_cast<const uint4 *>(a + static_cast<uint64_t>(8 * (j0 + j)) * p.columns + c)
-                                                   : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+                w[i][b] = there && c + b * kAdBlock + 8 * t < end && 16 * q + 8 * i + g < ranks
+                              ? *reinterpret_cast<const uint4 *>(a + static_cast<uint64_t>(16 * q + 8 * i) * p.columns + c + b * kAdBlock)
+                              : make_uint4(0, 0, 0, 0);
     };
     float s[NT][4];
 #pragma unroll
@@ -483,7 +492,7 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
 #pragma unroll
         for (int k = 0; k < 4; ++k) s[j][k] = 0.0f;
 #pragma unroll
-    for (int y = 0; y < AHEAD; ++y) fetch(begin + y * kAdBlock, 0, w[y]);
+    for (int y = 0; y < AHEAD; ++y) fetch(begin, y, w[y]);
 #pragma unroll 1
     for (int32_t n = 0; n < stages; ++n) {
         const int st = n % kAdStages;
@@ -491,41 +500,50 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
             if (lane == 0) pg_flag(p.status, PLAMO_PAGED_FAILED);
             break;
         }
-        AdPiece<X> v[BLOCKS][2];
+        uint32_t f[BLOCKS][2][4][TERMS];  // pairs of columns of rows g and g + 8
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) v[b][i].load(ring.stages + st * kAdStage + 2 * warp * kAdBox, g + 8 * i, b, t);
+            for (int i = 0; i < 2; ++i) {
+                AdPiece<X> v;
+                v.load(ring.stages + st * kAdStage + 2 * warp * kAdBox, g + 8 * i, b, t);
+                v.split(f[b][i]);
+            }
         __syncwarp();
         if (lane == 0) mbar_arrive(&ring.empty[st]);
+        const int32_t c = begin + n * COLUMNS;
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-            const int32_t c = begin + (n * BLOCKS + b) * kAdBlock;
-            uint32_t f0[4][TERMS], f1[4][TERMS];  // pairs of columns of rows g and g + 8
-            v[b][0].split(f0);
-            v[b][1].split(f1);
+        for (int q = 0; q < PAIRS; ++q) {
+            uint4 u[2][BLOCKS];
 #pragma unroll
-            for (int j0 = 0; j0 < NT; j0 += WIDE) {
-                uint4 u[WIDE];
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < WIDE; ++j) u[j] = w[b % AHEAD][j];
-                fetch(j0 + WIDE < NT ? c : c + AHEAD * kAdBlock, j0 + WIDE < NT ? j0 + WIDE : 0, w[b % AHEAD]);  // the next ones
+                for (int b = 0; b < BLOCKS; ++b) u[i][b] = w[q % AHEAD][i][b];
+            const auto next = [&] { fetch(q + AHEAD < PAIRS ? c : c + COLUMNS, (q + AHEAD) % PAIRS, w[q % AHEAD]); };
+            if constexpr (AHEAD < 4) next();
+            float d[2][4] = {};
 #pragma unroll
-                for (int j = 0; j < WIDE; ++j)
+            for (int term = TERMS - 1; term >= 0; --term)
 #pragma unroll
-                    for (int term = TERMS - 1; term >= 0; --term) {
-                        const uint32_t m0[4] = {f0[0][term], f1[0][term], f0[1][term], f1[1][term]};
-                        const uint32_t m1[4] = {f0[2][term], f1[2][term], f0[3][term], f1[3][term]};
-                        mma_bf16(s[j0 + j], m0, u[j].x, u[j].y);
-                        mma_bf16(s[j0 + j], m1, u[j].z, u[j].w);
-                    }
-            }
+                for (int b = 0; b < BLOCKS; ++b) {
+                    const uint32_t m0[4] = {f[b][0][0][term], f[b][1][0][term], f[b][0][1][term], f[b][1][1][term]};
+                    const uint32_t m1[4] = {f[b][0][2][term], f[b][1][2][term], f[b][0][3][term], f[b][1][3][term]};
+                    mma_bf16(d[0], m0, u[0][b].x, u[0][b].y);
+                    mma_bf16(d[1], m0, u[1][b].x, u[1][b].y);
+                    mma_bf16(d[0], m1, u[0][b].z, u[0][b].w);
+                    mma_bf16(d[1], m1, u[1][b].z, u[1][b].w);
+                }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[2 * q + i][k] += d[i][k];
+            if constexpr (AHEAD == 4) next();
         }
     }
-    float *to = p.inner + (static_cast<uint64_t>(blockIdx.y) * p.rows + tile.row0 + g) * p.rank + 2 * t;
+    float *to = p.inner + (static_cast<uint64_t>(blockIdx.y) * p.rows + tile.row0 + g) * p.rank + rank0 + 2 * t;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        if (8 * j >= p.rank) break;
+        if (8 * j >= ranks) break;
         if (g < tile.rows) *reinterpret_cast<float2 *>(to + 8 * j) = make_float2(s[j][0], s[j][1]);
         if (g + 8 < tile.rows) *reinterpret_cast<float2 *>(to + 8ull * p.rank + 8 * j) = make_float2(s[j][2], s[j][3]);
     }
@@ -549,7 +567,7 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
     __shared__ AdTile tiles[kAdTileWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const AdRing ring = ad_ring(ad_smem, full, empty, &base_map);
-    ad_tiles(p, p.out != p.base, tiles);
+    ad_tiles(p, blockIdx.x, p.out != p.base, tiles);
     if (!tiles[0].rows) return;
     const int32_t all = (p.outputs + COLUMNS - 1) / COLUMNS, first_stage = blockIdx.y * per, stages = min(per, all - first_stage);
     if (warp == kAdTileWarps) {
@@ -559,9 +577,12 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
     }
     const AdTile tile = tiles[warp];
     const bool there = tile.rows > 0 && tile.id >= 0;
-    // So many blocks' pieces of the adapter are on their way; none where h takes the registers.
-    constexpr int AHEAD = RANKS == 1 ? 2 : RANKS == 2 ? 1 : 0, STEP = AHEAD ? AHEAD : 1;
-    uint4 ahead[STEP][4][RANKS];
+    // The adapter's pieces on their way: of the next eight tiles (of four to a block of 32 outputs), four or two,
+    // where h takes the registers. (Rank 32 and 16 requests of 500 rows, a block's four
+    // loaded at once / one by one: FP32 122 / 142 us, BF16 105 / 87; rank 128 one and two tiles ahead 544 / 476, 536 / 398.)
+    constexpr int AHEAD = 8 / RANKS, STEP = RANKS == 1 ? 2 : 1;
+    constexpr bool BLOCK = sizeof(T) == 4 && RANKS <= 2;
+    uint4 ahead[AHEAD][RANKS];
     const auto fetch = [&](int32_t n0, int j, uint4 (&w)[RANKS]) {  // ranks 8 t of B's rows for tile j, column g
         const int32_t row = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
         const uint16_t *from = p.b + (static_cast<uint64_t>(max(tile.id, 0)) * p.outputs + row) * p.rank + 8 * t;
@@ -571,9 +592,7 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
                                                                              : make_uint4(0, 0, 0, 0);
     };
 #pragma unroll
-    for (int y = 0; y < AHEAD; ++y)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) fetch(first_stage * COLUMNS + y * kAdBlock, j, ahead[y][j]);
+    for (int y = 0; y < AHEAD; ++y) fetch(first_stage * COLUMNS + (y >> 2) * kAdBlock, y & 3, ahead[y]);
     pdl_wait();
     uint32_t h[RANKS][4][2][3];  // terms of scale * h: [block][pair of ranks][row g or g + 8]
 #pragma unroll
@@ -614,20 +633,22 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
             const int b = b0 + y;
             float s[2][8];
             uint4 w[4][RANKS];
-            if constexpr (AHEAD > 0) {
+            const auto take = [&](int j) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int k = 0; k < RANKS; ++k) w[j][k] = ahead[(4 * y + j) % AHEAD][k];
+                fetch(column + (b + (j + AHEAD) / 4) * kAdBlock, (j + AHEAD) & 3, ahead[(4 * y + j) % AHEAD]);
+            };
+            if constexpr (BLOCK) {
 #pragma unroll
-                    for (int k = 0; k < RANKS; ++k) w[j][k] = ahead[y][j][k];
-                    fetch(column + (b + AHEAD) * kAdBlock, j, ahead[y][j]);
-                }
+                for (int j = 0; j < 4; ++j) take(j);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (AHEAD == 0) fetch(column + b * kAdBlock, j, w[j]);
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (!BLOCK) take(j);
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < RANKS; ++k)
+                for (int k = 0; k < RANKS; ++k) {
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int term = 2; term >= 0; --term) {
                         const uint32_t m0[4] = {h[k][0][0][term], h[k][0][1][term], h[k][1][0][term], h[k][1][1][term]};
@@ -635,8 +656,11 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
                         mma_bf16(d, m0, w[j][k].x, w[j][k].y);
                         mma_bf16(d, m1, w[j][k].z, w[j][k].w);
                     }
-                s[0][2 * j] = d[0], s[0][2 * j + 1] = d[1];
-                s[1][2 * j] = d[2], s[1][2 * j + 1] = d[3];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sum[x] += d[x];
+                }
+                s[0][2 * j] = sum[0], s[0][2 * j + 1] = sum[1];
+                s[1][2 * j] = sum[2], s[1][2 * j + 1] = sum[3];
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {

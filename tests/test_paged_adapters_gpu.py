@@ -212,3 +212,21 @@ def test_refusals(be):
     call("out may be base", base=wide[:2, :72], out=wide[1:, :72])
     call("out may be base", x=wide[:2, 72:136], out=wide[:2, :80][:, 8:])
     be.paged_adapters(**{**good, "base": wide[:2, :72], "out": wide[:2, 72:]})  # beside one another
+
+
+@pytest.mark.parametrize("rows,rank", [(20_000, 8), (700, 64), (2_000, 128), (60, 256)])
+def test_long_sums_of_one_sign_lose_nothing(be, rows, rank):
+    """All terms positive, so that what is cut off sums adds up. Chains of 12 MMAs at most, cut by up to 2^-23 of the
+    sum each, then FP32 additions: 4,096 columns by no fewer than 64, or ranks by 32, and up to 64 partial sums,
+    a rounding of 2^-24 each. (One chain over the columns would be off by some 4e-5.)"""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    columns, outputs = 4096, 16
+    x = torch.rand(rows, columns, generator=g, device="cuda")
+    a = torch.rand(1, rank, columns, generator=g, device="cuda").to(torch.bfloat16)
+    b = torch.rand(1, outputs, rank, generator=g, device="cuda").to(torch.bfloat16)
+    starts, ids = torch.tensor([0, rows], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = be.paged_adapters(x, torch.zeros(rows, outputs, device="cuda"), a, b, ids, starts)
+    want = x.double() @ a[0].double().T @ b[0].double().T
+    bound = 12 * 2 ** -23 + (64 + 64) * 2 ** -24 + 12 * 2 ** -23 + 8 * 2 ** -24
+    assert ((got.double() - want).abs() / want).max().item() <= bound
+    assert be.paged_status() == 0
