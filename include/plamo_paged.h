@@ -290,7 +290,9 @@ uint64_t plamo_paged_adapters_workspace(struct plamo_cuda *, const struct plamo_
    the other rows, and the padding, are base's. Both products are summed in FP32, of x
    and of A x as they are; out is rounded once. Requests with the same adapter
    one after another share its reading. An id outside the adapters is
-   reported (PLAMO_PAGED_ADAPTER) and none. */
+   reported (PLAMO_PAGED_ADAPTER) and none; starts that decrease or leave the rows
+   are reported (PLAMO_PAGED_BATCH_ROWS), and rows that no request has by then
+   may stay as they are. */
 int plamo_paged_adapters(struct plamo_cuda *, const struct plamo_paged_adapters_args *);
 
 #ifdef __cplusplus

@@ -45,6 +45,10 @@ __device__ __forceinline__ void ad_split(float v0, float v1, uint32_t (&t)[TERMS
     }
 }
 
+// Requests must follow one another among the rows; else there are rows that nobody takes.
+__device__ __forceinline__ bool ad_starts_wrong(const AdapterParams &p, int32_t r) {
+    return p.starts[r] < 0 || p.starts[r + 1] < p.starts[r] || p.starts[r + 1] > p.rows;
+}
 // The adapter of batch row `row`, -1 where it has none; whole warp.
 __device__ __forceinline__ int32_t ad_row_adapter(const AdapterParams &p, int32_t row) {
     if (!p.requests || row >= p.rows || row < p.starts[0] || row >= p.starts[p.requests]) return -1;
@@ -173,6 +177,9 @@ __global__ void __launch_bounds__(kAdThreads) paged_adapters_inner_kernel(const 
         if (rank0 + r < p.rank && row0 + row < p.rows)
             p.inner[(static_cast<uint64_t>(blockIdx.y) * p.rows + row0 + row) * p.rank + rank0 + r] = s;
     }
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0)
+        for (int32_t e = tid; e < p.requests; e += kAdThreads)
+            if (ad_starts_wrong(p, e)) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
 }
 
 // ---- outputs, few rows ----------------------------------------------------------------------
@@ -378,7 +385,10 @@ __device__ __forceinline__ void ad_tiles(const AdapterParams &p, uint32_t cta, b
     };
     int64_t count = 0, total;
 #pragma unroll 1
-    for (int32_t e = e0; e < e1; ++e) count += (entry(e).rows + kAdTall - 1) / kAdTall;
+    for (int32_t e = e0; e < e1; ++e) {
+        count += (entry(e).rows + kAdTall - 1) / kAdTall;
+        if (e && e <= p.requests && ad_starts_wrong(p, e - 1)) pg_flag(p.status, PLAMO_PAGED_BATCH_ROWS);
+    }
     const int64_t first = static_cast<int64_t>(cta) * kAdTileWarps;
     int64_t at = pg_block_scan<kAdTileThreads>(count, sums, &total);
 #pragma unroll 1

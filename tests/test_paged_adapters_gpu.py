@@ -221,6 +221,7 @@ def test_long_sums_of_one_sign_lose_nothing(be, rows, rank):
     a rounding of 2^-24 each. (One chain over the columns would be off by some 4e-5.)"""
     g = torch.Generator(device="cuda").manual_seed(3)
     columns, outputs = 4096, 16
+    be.paged_status()
     x = torch.rand(rows, columns, generator=g, device="cuda")
     a = torch.rand(1, rank, columns, generator=g, device="cuda").to(torch.bfloat16)
     b = torch.rand(1, outputs, rank, generator=g, device="cuda").to(torch.bfloat16)
@@ -230,3 +231,45 @@ def test_long_sums_of_one_sign_lose_nothing(be, rows, rank):
     bound = 12 * 2 ** -23 + (64 + 64) * 2 ** -24 + 12 * 2 ** -23 + 8 * 2 ** -24
     assert ((got.double() - want).abs() / want).max().item() <= bound
     assert be.paged_status() == 0
+
+
+@pytest.mark.parametrize("each", [1, 40])
+def test_starts_that_decrease_are_reported(be, each):
+    """By the kernels of few rows and of many; rows before the fault are those of their request."""
+    requests, rank = 12, 16
+    rows = requests * each
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(rows, 64, generator=g, device="cuda")
+    a, b = (torch.randn(1, *shape, generator=g, device="cuda").to(torch.bfloat16) for shape in ((rank, 64), (24, rank)))
+    ids = torch.zeros(requests, dtype=torch.int32, device="cuda")
+    base = torch.zeros(rows, 24, device="cuda")
+    good = [each * r for r in range(requests + 1)]
+    be.paged_status()
+    for wrong in (good[:3] + [good[3] - 2 * each] + good[4:], good[:-1] + [rows + 1]):
+        be.paged_adapters(x, base, a, b, ids, torch.tensor(wrong, dtype=torch.int32, device="cuda"))
+        assert be.paged_status() == 4
+    be.paged_adapters(x, base, a, b, ids, torch.tensor(good, dtype=torch.int32, device="cuda"))
+    assert be.paged_status() == 0
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_calls_on_two_streams_at_once(be, new):
+    """Each has a workspace of its own."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    requests, columns, outputs, rank = 24, 1024, 512, 32
+    starts = torch.arange(requests + 1, dtype=torch.int32, device="cuda") * new
+    ids = torch.arange(requests, dtype=torch.int32, device="cuda") % 3
+    sides = []
+    for _ in range(2):
+        x, base = (torch.randn(requests * new, n, generator=g, device="cuda") for n in (columns, outputs))
+        a, b = (torch.randn(3, *shape, generator=g, device="cuda").to(torch.bfloat16) for shape in ((rank, columns), (outputs, rank)))
+        sides.append((x, base, a, b, ids, starts))
+    want = [be.paged_adapters(*side) for side in sides]
+    streams, got = [torch.cuda.Stream() for _ in sides], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(be.paged_adapters(*sides[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])

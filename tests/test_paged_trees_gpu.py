@@ -360,6 +360,48 @@ def test_attention_is_the_same_every_time_captured_and_on_another_stream(be, dty
     assert torch.equal(captured, first)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_attention_on_two_streams_at_once(be, dtype):
+    """Each call has a workspace of its own."""
+    scenes = [wide(TreeScene([(i * 97 % 400, t) for i, t in enumerate(some_trees(sizes, 21))], prefix, 16, 2, dtype, seed=4))
+              for sizes, prefix in (([16, 40, 1, 33, 8], 700), ([12, 30, 64], 12))]
+    want = [attend(be, s) for s in scenes]
+    streams, got = [torch.cuda.Stream() for _ in scenes], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(attend(be, scenes[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+@pytest.mark.parametrize("tables", ["short", "long"])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_pages_past_four_gigabytes(be, dtype, tables):
+    """A pool whose used pages lie more than 2^32 bytes behind its start gives what a small one does."""
+    s = TreeScene([(i * 131 % 300, t) for i, t in enumerate(some_trees([16, 40, 3], 2))], 200, 16, 8, dtype, seed=6)
+    if tables == "long":
+        wide(s)
+    be.paged_status()
+    small, used = attend(be, s), s.pool.shape[0]
+    page_bytes = s.pool[0].numel() * s.pool.element_size()
+    first = 2 ** 32 // page_bytes + 5
+    large = torch.empty(first + used, *s.pool.shape[1:], dtype=dtype, device="cuda")
+    large[first:] = s.pool
+    s.pool = large
+    s.tables = torch.where(s.tables >= 0, s.tables + first, s.tables)
+    s.prefix_pages = s.prefix_pages + first
+    assert torch.equal(attend(be, s), small)
+    path = torch.full((s.q.shape[0],), -1, dtype=torch.int32, device="cuda")
+    path[:3] = ints([0, 5, 9])
+    before = large[first:].clone()
+    be.paged_keep([large], path, s.starts, s.lengths, s.tables)
+    be.paged_keep([before], path, s.starts, s.lengths, torch.where(s.tables >= 0, s.tables - first, s.tables))
+    assert torch.equal(large[first:].view(torch.uint8), before.view(torch.uint8))  # (rows of no request hold NaN)
+    assert be.paged_status() == 0
+
+
 # ---- acceptance and the moved rows --------------------------------------------------
 
 def accept_scene(sizes, seed, vocabulary=3, held=None, tables=None):
