@@ -306,8 +306,9 @@ constexpr int kAdTall = 16, kAdBlock = 32;  // rows to a warp, columns or output
 constexpr int kAdTallRank = 128;            // terms of h in registers: 3/4 of a register for each rank
 constexpr int kAdTileWarps = 4, kAdTileThreads = 32 * (kAdTileWarps + 1);
 // A stage: for each warp two boxes of 128 bytes of its rows.
-constexpr int kAdStages = 6, kAdBox = kAdTall * 128, kAdStage = 2 * kAdTileWarps * kAdBox;
-constexpr int kAdTileSmem = 1024 + kAdStages * kAdStage;
+constexpr int kAdStages = 4, kAdBox = kAdTall * 128, kAdStage = 2 * kAdTileWarps * kAdBox;
+constexpr int kAdPieces = 8192;  // and so many bytes of the adapter's pieces
+constexpr int kAdTileSmem = 1024 + kAdStages * kAdStage + kAdTileWarps * kAdPieces;
 template <typename X>
 __host__ __device__ constexpr int ad_box_columns() { return 128 / sizeof(X); }
 
@@ -419,6 +420,28 @@ struct AdRing {
     uint64_t *full, *empty;
     unsigned char *stages;
 };
+// A warp's ring of the adapter's pieces, PIECES of 16 bytes of each lane to an item. A
+// lane copies and reads its own, so no lane waits for another, and no register for a
+// copy; an item's place is filled again when its products, which needed it, have been issued.
+template <int PIECES>
+struct AdAhead {
+    static constexpr int DEPTH = kAdPieces / (PIECES * 512);
+    uint32_t base;
+    __device__ __forceinline__ explicit AdAhead(const AdRing &r)
+        : base(smem_u32(r.stages + kAdStages * kAdStage + (threadIdx.x >> 5) * kAdPieces) + (threadIdx.x & 31) * 16) {}
+    __device__ __forceinline__ void copy(int32_t item, int piece, const uint16_t *from, bool there) const {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(base + (item % DEPTH * PIECES + piece) * 512), "l"(from), "r"(there ? 16 : 0)
+                     : "memory");
+    }
+    __device__ __forceinline__ void sent() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    // The oldest of DEPTH items has arrived.
+    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory"); }
+    __device__ __forceinline__ uint4 piece(int32_t item, int piece) const {
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(base + (item % DEPTH * PIECES + piece) * 512) : "memory");
+        return v;
+    }
+};
 __device__ __forceinline__ AdRing ad_ring(unsigned char *smem, uint64_t *full, uint64_t *empty, const CUtensorMap *map) {
     AdRing r{full, empty, reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~static_cast<uintptr_t>(1023))};
     if (threadIdx.x == 0) {
@@ -466,7 +489,7 @@ template <typename X, int NT>
 __global__ void __launch_bounds__(kAdTileThreads, 2)
     paged_adapters_tall_inner_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ AdapterParams p) {
     constexpr int TERMS = sizeof(X) == 4 ? 3 : 1, COLUMNS = 2 * ad_box_columns<X>(), BLOCKS = COLUMNS / kAdBlock;  // to a stage
-    constexpr int PAIRS = NT / 2, AHEAD = TERMS == 1 || PAIRS < 2 ? 1 : PAIRS;  // pairs of tiles of the adapter; so many on their way
+    constexpr int PAIRS = NT / 2;  // of tiles of eight ranks; an item to a stage each
     extern __shared__ __align__(128) unsigned char ad_smem[];
     __shared__ __align__(8) uint64_t full[kAdStages], empty[kAdStages];
     __shared__ AdTile tiles[kAdTileWarps];
@@ -486,15 +509,17 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
     const AdTile tile = tiles[warp];
     const bool there = tile.rows > 0;
     const uint16_t *const a = p.a + (static_cast<uint64_t>(max(tile.id, 0)) * p.rank + rank0 + g) * p.columns + 8 * t;
-    uint4 w[AHEAD][2][BLOCKS];
-    const auto fetch = [&](int32_t c, int q, uint4 (&w)[2][BLOCKS]) {  // columns c + 8 t of a stage's blocks, adapter rows 16 q + 8 i + g
+    const AdAhead<2 * BLOCKS> ahead(ring);
+    const auto fetch = [&](int32_t item) {  // columns 8 t of a stage's blocks, adapter rows 16 q + 8 i + g
+        const int32_t c = begin + item / PAIRS * COLUMNS, q = item % PAIRS;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
-                w[i][b] = there && c + b * kAdBlock + 8 * t < end && 16 * q + 8 * i + g < ranks
-                              ? *reinterpret_cast<const uint4 *>(a + static_cast<uint64_t>(16 * q + 8 * i) * p.columns + c + b * kAdBlock)
-                              : make_uint4(0, 0, 0, 0);
+            for (int b = 0; b < BLOCKS; ++b) {
+                const bool in = there && c + b * kAdBlock + 8 * t < end && 16 * q + 8 * i + g < ranks;
+                ahead.copy(item, i * BLOCKS + b, in ? a + static_cast<uint64_t>(16 * q + 8 * i) * p.columns + c + b * kAdBlock : p.a, in);
+            }
+        ahead.sent();
     };
     float s[NT][4];
 #pragma unroll
@@ -502,7 +527,7 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
 #pragma unroll
         for (int k = 0; k < 4; ++k) s[j][k] = 0.0f;
 #pragma unroll
-    for (int y = 0; y < AHEAD; ++y) fetch(begin, y, w[y]);
+    for (int y = 0; y < ahead.DEPTH; ++y) fetch(y);
 #pragma unroll 1
     for (int32_t n = 0; n < stages; ++n) {
         const int st = n % kAdStages;
@@ -521,16 +546,15 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
             }
         __syncwarp();
         if (lane == 0) mbar_arrive(&ring.empty[st]);
-        const int32_t c = begin + n * COLUMNS;
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q) {
+            const int32_t item = n * PAIRS + q;
+            ahead.wait();
             uint4 u[2][BLOCKS];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b) u[i][b] = w[q % AHEAD][i][b];
-            const auto next = [&] { fetch(q + AHEAD < PAIRS ? c : c + COLUMNS, (q + AHEAD) % PAIRS, w[q % AHEAD]); };
-            if constexpr (AHEAD < 4) next();
+                for (int b = 0; b < BLOCKS; ++b) u[i][b] = ahead.piece(item, i * BLOCKS + b);
             float d[2][4] = {};
 #pragma unroll
             for (int term = TERMS - 1; term >= 0; --term)
@@ -547,9 +571,10 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s[2 * q + i][k] += d[i][k];
-            if constexpr (AHEAD == 4) next();
+            fetch(item + ahead.DEPTH);
         }
     }
+    cp_async_wait_all();
     float *to = p.inner + (static_cast<uint64_t>(blockIdx.y) * p.rows + tile.row0 + g) * p.rank + rank0 + 2 * t;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -587,22 +612,23 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
     }
     const AdTile tile = tiles[warp];
     const bool there = tile.rows > 0 && tile.id >= 0;
-    // The adapter's pieces on their way: of the next eight tiles (of four to a block of 32 outputs), four or two,
-    // where h takes the registers. (Rank 32 and 16 requests of 500 rows, a block's four
-    // loaded at once / one by one: FP32 122 / 142 us, BF16 105 / 87; rank 128 one and two tiles ahead 544 / 476, 536 / 398.)
-    constexpr int AHEAD = 8 / RANKS, STEP = RANKS == 1 ? 2 : 1;
-    constexpr bool BLOCK = sizeof(T) == 4 && RANKS <= 2;
-    uint4 ahead[AHEAD][RANKS];
-    const auto fetch = [&](int32_t n0, int j, uint4 (&w)[RANKS]) {  // ranks 8 t of B's rows for tile j, column g
-        const int32_t row = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+    // An item: the ranks of eight outputs, column g, of four items to a block of 32 outputs.
+    const AdAhead<RANKS> ahead(ring);
+    const int32_t column0 = first_stage * COLUMNS, end = min(column0 + stages * COLUMNS, p.outputs);
+    const auto fetch = [&](int32_t item) {
+        const int32_t row = column0 + (item >> 2) * kAdBlock + 8 * (g >> 1) + 2 * (item & 3) + (g & 1);
         const uint16_t *from = p.b + (static_cast<uint64_t>(max(tile.id, 0)) * p.outputs + row) * p.rank + 8 * t;
 #pragma unroll
-        for (int b = 0; b < RANKS; ++b)
-            w[b] = there && row < p.outputs && kAdBlock * b + 8 * t < p.rank ? *reinterpret_cast<const uint4 *>(from + kAdBlock * b)
-                                                                             : make_uint4(0, 0, 0, 0);
+        for (int b = 0; b < RANKS; ++b) {
+            const bool in = row < end && kAdBlock * b + 8 * t < p.rank;
+            ahead.copy(item, b, in ? from + kAdBlock * b : p.b, in);
+        }
+        ahead.sent();
     };
+    if (there) {
 #pragma unroll
-    for (int y = 0; y < AHEAD; ++y) fetch(first_stage * COLUMNS + (y >> 2) * kAdBlock, y & 3, ahead[y]);
+        for (int y = 0; y < ahead.DEPTH; ++y) fetch(y);
+    }
     pdl_wait();
     uint32_t h[RANKS][4][2][3];  // terms of scale * h: [block][pair of ranks][row g or g + 8]
 #pragma unroll
@@ -637,24 +663,15 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
         }
         const int32_t column = (first_stage + n) * COLUMNS;
 #pragma unroll 1
-        for (int b0 = 0; there && b0 < BLOCKS; b0 += STEP)
-#pragma unroll
-        for (int y = 0; y < STEP; ++y) {
-            const int b = b0 + y;
+        for (int b = 0; there && b < BLOCKS; ++b) {
             float s[2][8];
-            uint4 w[4][RANKS];
-            const auto take = [&](int j) {
-#pragma unroll
-                for (int k = 0; k < RANKS; ++k) w[j][k] = ahead[(4 * y + j) % AHEAD][k];
-                fetch(column + (b + (j + AHEAD) / 4) * kAdBlock, (j + AHEAD) & 3, ahead[(4 * y + j) % AHEAD]);
-            };
-            if constexpr (BLOCK) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) take(j);
-            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (!BLOCK) take(j);
+                const int32_t item = 4 * (n * BLOCKS + b) + j;
+                ahead.wait();
+                uint4 w[RANKS];
+#pragma unroll
+                for (int k = 0; k < RANKS; ++k) w[k] = ahead.piece(item, k);
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < RANKS; ++k) {
@@ -663,12 +680,13 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
                     for (int term = 2; term >= 0; --term) {
                         const uint32_t m0[4] = {h[k][0][0][term], h[k][0][1][term], h[k][1][0][term], h[k][1][1][term]};
                         const uint32_t m1[4] = {h[k][2][0][term], h[k][2][1][term], h[k][3][0][term], h[k][3][1][term]};
-                        mma_bf16(d, m0, w[j][k].x, w[j][k].y);
-                        mma_bf16(d, m1, w[j][k].z, w[j][k].w);
+                        mma_bf16(d, m0, w[k].x, w[k].y);
+                        mma_bf16(d, m1, w[k].z, w[k].w);
                     }
 #pragma unroll
                     for (int x = 0; x < 4; ++x) sum[x] += d[x];
                 }
+                fetch(item + ahead.DEPTH);
                 s[0][2 * j] = sum[0], s[0][2 * j + 1] = sum[1];
                 s[1][2 * j] = sum[2], s[1][2 * j + 1] = sum[3];
             }
@@ -704,6 +722,7 @@ __global__ void __launch_bounds__(kAdTileThreads, 2)
             if (n) mbar_arrive(&ring.empty[(n - 1) % kAdStages]);
         }
     }
+    cp_async_wait_all();
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
