@@ -202,7 +202,7 @@ __device__ __forceinline__ void ad_store(T *p, float v) {
 template <typename T>
 __global__ void __launch_bounds__(kAdThreads, 5) paged_adapters_outer_kernel(const __grid_constant__ AdapterParams p, int32_t per) {
     __shared__ AdRuns runs;
-    __shared__ __align__(16) uint32_t h[3][kAdRows][kAdMaxRank / 2 + 4];  // terms of scale * h, two ranks to a word
+    __shared__ __align__(16) uint32_t h[3][kAdRows][kAdMaxRank / 2 + 16];  // terms of scale * h, two ranks to a word; rows half the banks apart
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int32_t row0 = blockIdx.x * kAdRows, pairs = p.rank / 2, blocks = (p.rank + 31) / 32;
     ad_runs(p, row0, runs);
