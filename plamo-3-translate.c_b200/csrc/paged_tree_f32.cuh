@@ -12,18 +12,18 @@ namespace plamo {
 // products start from zero and are added to FP32 registers, and nothing is cut by more
 // than a few products of 2^-24. 128 pairs by 64 keys are 3,072 cycles of the tensor pipe;
 // as many multiply-adds of the CUDA cores are 16,384.
-//  - Sixteen warps do all but the products. Warp w has the rows of tensor-memory lanes
+//  - Sixteen warps have the softmax and the sums. Warp w has the rows of tensor-memory lanes
 //    32 (w % 4) up; its quarter w / 4 has 16 of a step's keys and 32 of the dimensions. In
-//    each step a thread makes its keys' weights, adds its dimensions' sums of the step
-//    before to its registers, and turns its share of the next keys and values, which its
-//    loads brought a step earlier, into terms in shared memory.
+//    each step a thread makes its keys' weights and adds its dimensions' sums of the step
+//    before to its registers. Eight more turn keys and values into terms in shared memory,
+//    as far ahead as there is room. (The sixteen doing that, too, in turn: 9,000 cycles a step.)
 //  - Tensor memory (512 columns): the queries' terms 3 x 64, a step's sums 128, and two
 //    places by turns of 96 for a step's scores (64), then its weights' terms (3 x 32).
 //  - Shared memory: two steps' terms of keys and of values, 4 x 48 KB.
 // Values that are not finite leave the products, and rows that see them get them at the
 // end of a segment; a key that has such a number gets its scores one by one.
-constexpr int kTqPairs = 128, kTqKeys = 64, kTqWarps = 16, kTqThreads = 32 * (kTqWarps + 2);
-constexpr int kTqWalk = 16, kTqProducts = 17;  // warps
+constexpr int kTqPairs = 128, kTqKeys = 64, kTqWarps = 16, kTqTurning = 8, kTqThreads = 32 * (kTqWarps + kTqTurning + 2);
+constexpr int kTqWalk = 24, kTqProducts = 25;  // warps; 0-15 softmax, 16-23 turn keys and values into terms
 constexpr int kTqTerm = kTqKeys * kPgDim * 2, kTqBlock = kTqKeys * 128;  // bytes: a term of keys or values, its block of 64 dimensions
 constexpr int kTqSmem = 1024 + 4 * 3 * kTqTerm;
 constexpr uint32_t kTqQueries = 0, kTqSums = 192, kTqPlaces = 320, kTqPlace = 96;  // columns
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
     __shared__ __align__(8) uint64_t q_ready, k_ready[2], k_free[2], v_ready[2], v_free[2], s_full[2], p_ready[2], o_full, o_free;
     __shared__ TreeSegment segments[kTsSegments];
     __shared__ float tops[4][kTqPairs];
-    __shared__ uint32_t odd_keys[4][2];  // of step s, at s % 4: keys with a number that is not finite
+    __shared__ __align__(8) unsigned char odd_keys[4][kTqKeys / 8];  // of step s, at s % 4: keys with a number that is not finite
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up, odd_values;
     unsigned char *base = reinterpret_cast<unsigned char *>(
@@ -105,11 +105,11 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
     if (tid == 0) {
         for (int s = 0; s < kTsSegments; ++s) {
             mbar_init(&seg_full[s], 1);
-            mbar_init(&seg_empty[s], kTqWarps + 1);
+            mbar_init(&seg_empty[s], kTqWarps + kTqTurning + 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_ready[i], kTqWarps);
-            mbar_init(&v_ready[i], kTqWarps);
+            mbar_init(&k_ready[i], kTqTurning);
+            mbar_init(&v_ready[i], kTqTurning);
             mbar_init(&p_ready[i], kTqWarps);
             mbar_init(&k_free[i], 1);
             mbar_init(&v_free[i], 1);
@@ -121,7 +121,6 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
         gave_up = odd_values = 0;
         fence_barrier_init();
     }
-    if (tid < 8) odd_keys[tid >> 1][tid & 1] = 0;
     if (warp == kTqProducts) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
                      "r"(512)
@@ -226,8 +225,119 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
             }
             c += steps;
         }
-    } else {
-        // ---- all else: sixteen warps
+    } else if (warp >= kTqWarps && warp < kTqWalk) {
+        // ---- keys and values into terms: eight rows of a step to a warp, 16 bytes of each to a lane; four
+        // are turned while four are on their way
+        pdl_wait();
+        const int turning = warp - kTqWarps;
+        unsigned char *const put_at = base + (lane >> 4) * kTqBlock + 8 * turning * 128 + (lane & 1) * 8;
+        const uint64_t row_size = static_cast<uint64_t>(p.kh) * kPgDim;
+        uint32_t c = 0;  // steps before the segment's
+        for (uint32_t seg = 0; ok; ++seg) {
+            ok = wait(&seg_full[seg % kTsSegments], (seg / kTsSegments) & 1u);
+            if (!ok) break;
+            const TreeSegment t = segments[seg % kTsSegments];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[seg % kTsSegments]);
+            if (!t.steps) break;
+            const auto page_id = [&](int32_t n) {
+                const int32_t step = t.step + n;
+                const bool own = step >= t.pre_steps;
+                const int32_t *table = own ? p.tables + static_cast<uint64_t>(max(t.request, 0)) * p.table_stride + t.own0 - t.pre_steps : p.prefix_pages + t.pre0;
+                return n < t.steps ? table[step] : -1;
+            };
+            // The first of this warp's rows of page `id`; and how many of them step n has.
+            const auto rows_at = [&](int32_t id) {
+                const bool good = id >= 0 && id < p.pages;
+                return static_cast<const float *>(p.pool) + (static_cast<uint64_t>(good ? id : 0) * 2 * kPgRows + 8 * turning) * row_size + t.head * kPgDim;
+            };
+            const auto rows_of = [&](int32_t n, int32_t id) {
+                const int32_t step = t.step + n;
+                const bool own = step >= t.pre_steps;
+                const int32_t left = own ? t.own_limit - (t.own0 + step - t.pre_steps) * kTqKeys : p.prefix - (t.pre0 + step) * kTqKeys;
+                return id >= 0 && id < p.pages ? left - 8 * turning : 0;
+            };
+            float4 raw[2][4];
+            const auto load = [&](int i, const float *from, int32_t rows) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) raw[i][y] = 4 * i + y < rows ? ld4(from + (4 * i + y) * row_size + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            // A line of 128 bytes to a lane: they are in L2 when their turn comes.
+            const auto ahead = [&](const float *from, int32_t rows) {
+                if ((lane >> 2) < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + (lane >> 2) * row_size + 32 * (lane & 3)));
+            };
+            const auto put = [&](int i, uint32_t to, uint32_t s) {  // says which rows had a number that is not finite
+                uint64_t z = pair_of(0.0f, 0.0f);  // no number where one of them is none
+                uint32_t odd = 0;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    z = fma_pair(pair_of(raw[i][y].x, raw[i][y].y), pair_of(0.0f, 0.0f), z);
+                    z = fma_pair(pair_of(raw[i][y].z, raw[i][y].w), pair_of(0.0f, 0.0f), z);
+                }
+                if (__any_sync(0xffffffffu, low_of(z) + high_of(z) != 0.0f)) {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const float4 v = raw[i][y];
+                        raw[i][y] = make_float4(tq_or_zero(v.x), tq_or_zero(v.y), tq_or_zero(v.z), tq_or_zero(v.w));
+                        if (__any_sync(0xffffffffu, !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w)))) odd |= 1u << y;
+                    }
+                }
+                unsigned char *const at0 = put_at + to + (s & 1) * 3 * kTqTerm + 4 * i * 128;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    uint32_t a[3], b[3];
+                    tq_split(raw[i][y].x, raw[i][y].y, a);
+                    tq_split(raw[i][y].z, raw[i][y].w, b);
+                    unsigned char *const at = at0 + y * 128 + ((((lane & 15) >> 1) ^ (4 * i + y)) << 4);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) *reinterpret_cast<uint2 *>(at + x * kTqTerm) = make_uint2(a[x], b[x]);
+                }
+                return odd;
+            };
+            const auto ready = [&](uint64_t *bar) {
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+            };
+            int32_t id = page_id(0), id_next = page_id(1);
+            const float *keys = rows_at(id);
+            load(0, keys, rows_of(0, id));
+            load(1, keys, rows_of(0, id));
+            ahead(keys + kPgRows * row_size, rows_of(0, id));
+#pragma unroll 1
+            for (int32_t n = 0; n < t.steps && ok; ++n) {
+                const uint32_t s = c + n;
+                const int32_t rows = rows_of(n, id), rows_next = n + 1 < t.steps ? rows_of(n + 1, id_next) : 0, id_after = page_id(n + 2);
+                const float *const values = keys + kPgRows * row_size, *const keys_next = rows_at(id_next);
+                if ((id < 0 || id >= p.pages) && turning == 0 && lane == 0) pg_flag(p.status, PLAMO_PAGED_PAGE);
+                ahead(keys_next, rows_next);
+                ahead(keys_next + kPgRows * row_size, rows_next);
+                ok = s < 2 || wait(&k_free[s & 1], ((s >> 1) - 1) & 1u);
+                if (!ok) break;
+                uint32_t odd = 0;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    odd |= put(i, 0, s) << 4 * i;
+                    load(i, values, rows);
+                }
+                if (lane == 0) odd_keys[s & 3][turning] = static_cast<unsigned char>(odd);
+                ready(&k_ready[s & 1]);
+                ok = s < 2 || wait(&v_free[s & 1], ((s >> 1) - 1) & 1u);
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (put(i, 2 * 3 * kTqTerm, s) && lane == 0) odd_values = 1;
+                    load(i, keys_next, rows_next);
+                }
+                ready(&v_ready[s & 1]);
+                id = id_next;
+                id_next = id_after;
+                keys = keys_next;
+            }
+            c += t.steps;
+        }
+    } else if (warp < kTqWarps) {
+        // ---- softmax, sums
         pdl_wait();
         const int quarter = warp >> 2, pair = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -246,77 +356,7 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
             __syncwarp();
             if (lane == 0) mbar_arrive(&seg_empty[seg % kTsSegments]);
             if (!t.steps) break;
-            const int32_t request = t.request, own_limit = t.own_limit;
-            // This warp's rows of a step's keys and values, four each, 16 bytes a lane: loaded a step ahead, the
-            // page's id two ...
-            float4 k_raw[4], v_raw[4];
-            const auto page_id = [&](int32_t n) {
-                const int32_t step = t.step + n;
-                const bool own = step >= t.pre_steps;
-                const int32_t *table = own ? p.tables + static_cast<uint64_t>(max(request, 0)) * p.table_stride + t.own0 - t.pre_steps : p.prefix_pages + t.pre0;
-                return n < t.steps ? table[step] : 0;
-            };
-            const auto load = [&](float4 (&raw)[4], int32_t n, int32_t id, int kind) {
-                const int32_t step = t.step + n;
-                const bool own = step >= t.pre_steps, good = id >= 0 && id < p.pages;
-                const int32_t left = (own ? own_limit - (t.own0 + step - t.pre_steps) * kTqKeys : p.prefix - (t.pre0 + step) * kTqKeys) - 4 * warp;
-                if (!good && tid == 0) pg_flag(p.status, PLAMO_PAGED_PAGE);
-                const uint64_t row = static_cast<uint64_t>(p.kh) * kPgDim;
-                const float *from = static_cast<const float *>(p.pool) + ((static_cast<uint64_t>(good ? id : 0) * 2 + kind) * kPgRows + 4 * warp) * row +
-                                    t.head * kPgDim + 4 * lane;
-                const int32_t rows = good && n < t.steps ? left : 0;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) raw[y] = y < rows ? ld4(from + y * row) : make_float4(0.f, 0.f, 0.f, 0.f);
-            };
-            // ... and put into shared memory as terms.
-            unsigned char *const put_at = base + (lane >> 4) * kTqBlock + 4 * warp * 128 + (lane & 1) * 8;
-            const auto put = [&](float4 (&raw)[4], uint32_t to, uint32_t s, bool keys) {
-                uint64_t z = pair_of(0.0f, 0.0f);  // no number where one of them is none
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    z = fma_pair(pair_of(raw[y].x, raw[y].y), pair_of(0.0f, 0.0f), z);
-                    z = fma_pair(pair_of(raw[y].z, raw[y].w), pair_of(0.0f, 0.0f), z);
-                }
-                if (__any_sync(0xffffffffu, low_of(z) + high_of(z) != 0.0f)) {
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float4 v = raw[y];
-                        raw[y] = make_float4(tq_or_zero(v.x), tq_or_zero(v.y), tq_or_zero(v.z), tq_or_zero(v.w));
-                        const bool odd = __any_sync(0xffffffffu, !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w)));
-                        if (odd && lane == 0) {
-                            if (keys) atomicOr(&odd_keys[s & 3][warp >> 3], 1u << (4 * (warp & 7) + y));
-                            else odd_values = 1;
-                        }
-                    }
-                }
-                unsigned char *const at0 = put_at + to + (s & 1) * 3 * kTqTerm;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    uint32_t a[3], b[3];
-                    tq_split(raw[y].x, raw[y].y, a);
-                    tq_split(raw[y].z, raw[y].w, b);
-                    unsigned char *const at = at0 + y * 128 + ((((lane & 15) >> 1) ^ ((4 * warp + y) & 7)) << 4);
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) *reinterpret_cast<uint2 *>(at + x * kTqTerm) = make_uint2(a[x], b[x]);
-                }
-                fence_async_shared();
-                __syncwarp();
-            };
-            const auto put_keys = [&](uint32_t s) {
-                if (s >= 2 && !wait(&k_free[s & 1], ((s >> 1) - 1) & 1u)) return false;
-                put(k_raw, 0, s, true);
-                if (lane == 0) mbar_arrive(&k_ready[s & 1]);
-                return true;
-            };
-            const auto put_values = [&](uint32_t s) {
-                if (s >= 2 && !wait(&v_free[s & 1], ((s >> 1) - 1) & 1u)) return false;
-                put(v_raw, 2 * 3 * kTqTerm, s, false);
-                if (lane == 0) mbar_arrive(&v_ready[s & 1]);
-                return true;
-            };
-            int32_t id = page_id(0), id_next = page_id(1);
-            load(k_raw, 0, id, 0);
-            load(v_raw, 0, id, 1);
+            const int32_t request = t.request;
             const bool there = pair < t.pairs;
             const int32_t local = p.by_group.div(pair), row = t.row0 + local, head = t.head * p.group + pair - local * p.group;
             const float *const query = static_cast<const float *>(p.q) + static_cast<int64_t>(there ? row : t.row0) * static_cast<int64_t>(p.q_stride) + (there ? head : 0) * kPgDim;
@@ -340,11 +380,6 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_ready);
-            ok = put_keys(c);
-            load(k_raw, 1, id_next, 0);
-            ok = ok && put_values(c);
-            load(v_raw, 1, id_next, 1);
-            id = page_id(2);
             int32_t held = t.held, added = t.added, from = 0;  // `from`: bits of the mask below it are outside the window
             TreeSees sees{0, 0, 0};
             if (p.window && there) {
@@ -381,9 +416,6 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
                 const uint32_t s = c + n;
                 const int32_t step = t.step + n;
                 const bool own = step >= t.pre_steps;
-                if (n + 1 < t.steps) ok = ok && put_keys(s + 1);
-                load(k_raw, n + 2, id, 0);
-                id_next = page_id(n + 3);
                 // ---- this thread's 16 keys of the step: which of them the row sees
                 const int32_t key0 = (own ? t.own0 + step - t.pre_steps : t.pre0 + step) * kTqKeys + 16 * quarter;
                 const int32_t hi = min(max((own ? held : p.prefix) - key0, 0), 16);
@@ -407,7 +439,7 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
 #pragma unroll
                         for (int k = 0; k < 16; ++k) x[k] ^= flip;
                     }
-                    const uint32_t odd = (odd_keys[s & 3][quarter >> 1] >> (16 * (quarter & 1))) & see;
+                    const uint32_t odd = *reinterpret_cast<const uint16_t *>(&odd_keys[s & 3][2 * quarter]) & see;
                     if (__any_sync(0xffffffffu, see != 0xffffu || odd)) {
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
@@ -478,11 +510,7 @@ __global__ void __launch_bounds__(kTqThreads, 1) paged_tree_f32_kernel(const __g
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&p_ready[s & 1]);
                 }
-                if (tid < 2) odd_keys[(s + 3) & 3][tid] = 0;  // (step s - 1's: of no more use, and not yet of step s + 3's)
                 if (n) ok = ok && fold(s - 1);
-                if (n + 1 < t.steps) ok = ok && put_values(s + 1);
-                load(v_raw, n + 2, id, 1);
-                id = id_next;
             }
             ok = ok && fold(c + t.steps - 1);
             c += t.steps;
