@@ -69,23 +69,23 @@ const char *attention_shapes(const plamo_paged_attention_args *d) {
 // full; a tree's own leave room, but need no joining with others. So sharing is for
 // trees that fill less than 4/5 of tiles of their own. BF16: 61 of 20 rows behind 2,000,
 // held 450, shared 125 us and not 133, 32 of 8 rows 63 and 61, behind 600 50 and 46; 16 of 32 rows,
-// full tiles, behind 2,000 70 and 64. FP32: 32 of 8 rows behind 2,000, held 450, 166 and 221,
-// 12 of 8 rows behind 600 60 and 62, of 10 rows 61 and 64.
+// full tiles, behind 2,000 70 and 64. FP32: 32 of 8 rows behind 2,000, held 450, 113 and 145,
+// 12 of 10 rows behind 600 50 and 52, of 8 rows behind 300 49 and 43.
 constexpr uint64_t kTreeShareRows = 1024, kTreeShareRowsF32 = 512;
 // Pairs up to which a request's own rows are the row kernel's, which has tiles of eight.
 // BF16: 32 requests of 4 rows behind 2,000 89 us in it and 52 in tiles, of 2 rows 58 and
-// 46. FP32: 32 of 4 rows behind 2,000 330 and 165, 12 behind 1,000 90 and 84, 32 with no
-// prefix, held 450, 70 and 74; but 12 of 2 rows behind 1,000 54 and 83, 32 behind 2,000 171 and 144.
-constexpr uint32_t kTreeShortPairs = 8, kTreeShortPairsF32 = 16;
+// 46. FP32: 32 of 4 rows behind 2,000 329 and 111, 12 behind 1,000 90 and 51, 32 with no
+// prefix, held 450, 70 and 56; 32 of 2 rows behind 2,000 171 and 95, 12 behind 1,000 54 and 51.
+constexpr uint32_t kTreeShortPairs = 8;
 // As kTlPromptUnits, for FP32 trees, whose tile kernel takes less than the plain one: one
-// request of 16 rows behind 12, held 450, 23 us in the row kernel and 31 in tiles, two 36 and 33, three 43 and 33.
+// request of 16 rows behind 12, held 450, 23 us in the row kernel and 29 in tiles, two 36 and 31, three 43 and 31.
 constexpr uint64_t kTreePromptUnitsF32 = 1000;
 // What a strip's beginning and end are worth, in units of half a step of a full tile (BF16)
 // or a step (FP32), where the work is divided. BF16, 4 / 8 / 12 / 16: 64 trees of 64 rows behind 8,192
 // 1,075 / 957 / 870 / 913 us, 61 of 20 to 32 behind 2,000 218 / 205 / 208 / -. FP32, 0 / 2 / 4 / 6: 8 trees of 16
-// behind 12, held 450, 51 / 45 / 45 / 49, 24 behind 12 128 / 113 / 119 / 131, 60 of 24 behind 1,000 651 / 655 / 658 / 674.
+// behind 12, held 450, 46 / 40 / 41 / 42, 24 behind 12 94 / 81 / 83 / 88, 60 of 24 behind 1,000 448 / 422 / 428 / 440.
 constexpr int32_t kTreeStripPad = 12, kTreeStripPadF32 = 2;
-// A CTA has no fewer units than this: 8 trees of 16 in FP32, 1 / 2 / 4: 45 / 45 / 50 us.
+// A CTA has no fewer units than this (8 trees of 16 in FP32, 1 / 2 / 4: 40 / 40 / 44 us).
 constexpr int32_t kTreeLeast = 4, kTreeLeastF32 = 1;
 
 // How an attention call is laid out: the workspace's parts and the grid.
@@ -130,7 +130,7 @@ AttentionLayout attention_layout(const plamo_cuda *c, const plamo_paged_attentio
     const uint64_t strips = ceil_div(pairs, kRtPairs) * d->kv_heads;
     const uint64_t prefix_steps = ceil_div(pairs, kTlPairs) * d->kv_heads * ceil_div(d->prefix_rows, kTlKeys);
     const uint64_t most = d->most_new ? std::min(d->most_new, d->rows) : d->rows > d->requests ? d->rows : 0;  // rows of a request
-    a.short_pairs = !trees ? kTlShortPairs : f32 ? kTreeShortPairsF32 : kTreeShortPairs;
+    a.short_pairs = trees ? kTreeShortPairs : kTlShortPairs;
     const bool prompts = most * group > a.short_pairs;
     if (group <= tile_pairs && ((prompts && strips * (prefix_pages + d->table_stride) > (trees && f32 ? kTreePromptUnitsF32 : kTlPromptUnits)) ||
                                 (!f32 && strips * prefix_pages > kTlPrefixUnits + 4 * prefix_steps))) {

@@ -292,16 +292,15 @@ __global__ void __launch_bounds__(kAdThreads, 5) paged_adapters_outer_kernel(con
 // ---- many rows to an adapter -----------------------------------------------------------------
 // A warp takes 16 rows of one request, now the M of its MMAs, and the adapter's rows are
 // their N. x (and base and out) come and go by the copy engine, 256 bytes of each row
-// at a time through a ring; two CTAs of 98 KB to an SM keep 190 KB on their way.
-// (16 prompts of 129 to 1,023 rows, rank 32, 4,096 columns and outputs, FP32: inner 48 us,
-// outputs 56, at 3.1 and 5.4 TB/s; with loads into registers, whose number bounds what is on
-// its way, 73 and 102.) The order along the
-// contraction is free, so lane t of four takes columns 8 t to 8 t + 7 of 32, whole
-// 16-byte pieces of a row. The adapter's pieces come from the L1 cache, which the
-// CTA's warps mostly share, a block or two ahead. HBM bounds both kernels up to ranks of
-// about 64: a row's bytes cover the products, which mma.sync makes fast enough
-// (tcgen05 would want the terms of x in shared memory, six bytes written and read for
-// each four that arrive).
+// at a time through a ring; two CTAs of 98 KB to an SM keep 128 KB on their way. The order
+// along the contraction is free, so lane t of four takes columns 8 t to 8 t + 7 of 32,
+// whole 16-byte pieces of a row. The adapter's pieces come from the L1 cache, which the CTA's
+// warps mostly share, by asynchronous copies, 8 KB a warp ahead (in registers, which allow
+// two tiles of rank 128, 16 requests of 500 rows took 469 us; so 283).
+// 16 prompts of 129 to 1,023 rows, rank 32, 4,096 columns and outputs, FP32: inner 44 us,
+// outputs 56 to 60, 3.4 and 5.2 TB/s of what they have to move (rows by loads into registers: 73 and 102). HBM
+// bounds the outputs up to ranks of about 64, latency the rest (tcgen05 would want the terms of x
+// in shared memory, six bytes written and read for each four that arrive).
 constexpr int kAdTall = 16, kAdBlock = 32;  // rows to a warp, columns or outputs at a time
 constexpr int kAdTallRank = 128;            // terms of h in registers: 3/4 of a register for each rank
 constexpr int kAdTileWarps = 4, kAdTileThreads = 32 * (kAdTileWarps + 1);

@@ -16,7 +16,8 @@ namespace plamo {
 //    32 (w % 4) up; its quarter w / 4 has 16 of a step's keys and 32 of the dimensions. In
 //    each step a thread makes its keys' weights and adds its dimensions' sums of the step
 //    before to its registers. Eight more turn keys and values into terms in shared memory,
-//    as far ahead as there is room. (The sixteen doing that, too, in turn: 9,000 cycles a step.)
+//    as far ahead as there is room: 5,700 cycles a step, the 12 trees of 24 rows in a window 97 us
+//    (9,000 and 148 where the sixteen did that, too; four warps for it 178).
 //  - Tensor memory (512 columns): the queries' terms 3 x 64, a step's sums 128, and two
 //    places by turns of 96 for a step's scores (64), then its weights' terms (3 x 32).
 //  - Shared memory: two steps' terms of keys and of values, 4 x 48 KB.
