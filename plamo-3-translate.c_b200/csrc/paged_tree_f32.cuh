@@ -10,7 +10,7 @@ namespace plamo {
 // of the whole: (3,1) (1,3) (2,2) (2,1) (1,2) (1,1), the small ones first. Tensor cores
 // cut what they add up, by 1e-5 of the sum over some thousand keys; so a step's value
 // products start from zero and are added to FP32 registers, and nothing is cut by more
-// than a few products of 2^-24. 128 pairs by 64 keys are 3,072 cycles of the tensor pipe;
+// than a few products of 2^-24. 128 pairs by 64 keys are some 3,100 cycles of the tensor pipe;
 // as many multiply-adds of the CUDA cores are 16,384.
 //  - Sixteen warps have the softmax and the sums. Warp w has the rows of tensor-memory lanes
 //    32 (w % 4) up; its quarter w / 4 has 16 of a step's keys and 32 of the dimensions. In

@@ -1,6 +1,6 @@
 // Draft trees of a paged batch step (include/plamo_paged.h): positions and
 // masks before the layers, the confirmed path and its rows after them. The
-// trees' attention is in paged_attention.cuh and paged_tiles.cuh.
+// trees' attention is in paged_attention.cuh, paged_tree_tiles.cuh and paged_tree_f32.cuh.
 #pragma once
 #include "paged.cuh"
 
