@@ -326,12 +326,11 @@ struct AdaptersLayout {
     uint64_t bytes;
 };
 // Where a warp takes 16 rows of one request instead of a CTA eight of any: requests of that many
-// rows, and enough of them; of ranks above 64, of which less is on its way at a time, more
-// (8B QKV, so / the other way). FP32, rank 32: 128 requests of 4 rows 43 us / 30, of 6
-// 42 / 39, of 8 31 / 47; rank 64: 16 of 16 27 / 23, 128 of 6 59 / 56, of 8 45 / 66; BF16, rank 64: 8 of 16 25 / 19,
-// 32 of 16 29 / 31, 100 of 4 37 / 27, of 8 31 / 39. FP32, rank 128: 256 of 8 242 / 200, 64 of 16
-// 104 / 101, 16 of 40 71 / 64, 32 of 40 102 / 112, 16 of 500 469 / 714.
-constexpr uint64_t kAdTallRows = 8, kAdTallAll = 384, kAdTallRowsWide = 12, kAdTallAllWide = 1024;
+// rows, and enough of them (8B QKV, so / the other way). FP32, rank 32: 128 requests of 4 rows 47 us / 30, of 6
+// 45 / 39, of 8 34 / 47; rank 64: 16 of 16 27 / 23, 24 of 16 31 / 29, 128 of 8 45 / 65; rank 128: 16 of 16 49 / 32,
+// 32 of 16 50 / 52, 8 of 40 49 / 39, 16 of 40 56 / 61, 128 of 8 83 / 95, 16 of 500 283 / 667. BF16, rank 64: 16 of 16
+// 25 / 21, 32 of 16 29 / 28, 100 of 4 37 / 25, of 6 33 / 38, of 8 33 / 37.
+constexpr uint64_t kAdTallRows = 8, kAdTallAll = 512;
 
 // Parts that the `rounds` stages of each of `tiles` CTAs' work are cut into: those that end
 // first, of the most that one, two, three or four rounds of CTAs hold, two to an SM. A
@@ -359,8 +358,7 @@ uint64_t tall_ctas(const plamo_paged_adapters_args *d, bool about) {
 AdaptersLayout adapters_layout(const plamo_cuda *c, const plamo_paged_adapters_args *d) {
     AdaptersLayout a{};
     const uint64_t sms = context_sms(c), longest = 1ull << 34;  // row strides that a tensor map holds
-    const bool wide = d->rank > kAdTallRanks;
-    a.tall = d->rows >= (wide ? kAdTallRowsWide : kAdTallRows) * d->requests && d->rows >= (wide ? kAdTallAllWide : kAdTallAll) && d->rank <= kAdTallRank && d->x_stride < longest &&
+    a.tall = d->rows >= kAdTallRows * d->requests && d->rows >= kAdTallAll && d->rank <= kAdTallRank && d->x_stride < longest &&
              d->base_stride < longest && d->out_stride < longest;
     if (a.tall) {
         const uint64_t round = 256 / element_bytes(d->x_type), rounds = ceil_div(d->columns, round);

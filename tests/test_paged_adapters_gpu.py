@@ -52,6 +52,7 @@ LAYOUTS = {
     "trees": ([17, 1, 33, 0, 8, 24], [3, 3, 0, 1, 0, 2]),
     "prompts": ([129, 300, 1, 64, 511], [0, 0, 1, 2, 1]),
     "gaps": ([0, 17, 33, 0, 400, 15, 16], [0, -1, 1, 2, 2, -1, 0]),
+    "more_gaps": ([0, 17, 33, 0, 500, 15, 16], [0, -1, 1, 2, 2, -1, 0]),
 }
 
 
@@ -117,7 +118,7 @@ def test_adapters_of_others_never_matter(be, new):
     assert not torch.isfinite(got[c.starts[1]:c.starts[3]]).any()
 
 
-@pytest.mark.parametrize("new", [1, 500])
+@pytest.mark.parametrize("new", [1, 500, 600])
 @pytest.mark.parametrize("kind", [FP32, BF16])
 def test_adapters_of_infinite_rows(be, kind, new):
     """One infinite entry times weights of one sign is infinite, not undefined."""
@@ -130,7 +131,7 @@ def test_adapters_of_infinite_rows(be, kind, new):
 
 
 def test_adapters_without_scales_requests_or_adapters(be):
-    c = Case([2, 490], [1, 0], 64, 72, 16, seed=5)
+    c = Case([2, 590], [1, 0], 64, 72, 16, seed=5)
     ones, c.scales = c.scales, None
     check(c.run(be), *c.expected(), "no scales")
     c.scales = ones
@@ -153,7 +154,7 @@ def test_adapters_report_ids_that_are_none(be, bad, new):
     assert status.item() == 256
 
 
-@pytest.mark.parametrize("rows", [20, 200])
+@pytest.mark.parametrize("rows", [20, 200, 300])
 @pytest.mark.parametrize("starts", [[0, 50, 20, 70], [-9, 10, 20, 10 ** 9], [5, 10, 20, 30], [2 ** 31 - 1, -2 ** 31, 7, 9]])
 def test_adapters_of_starts_outside_the_batch_stay_in_bounds(be, starts, rows):
     c = Case([rows, 30, rows], [0, 1, 0], 64, 72, 16, seed=7)
@@ -164,7 +165,7 @@ def test_adapters_of_starts_outside_the_batch_stay_in_bounds(be, starts, rows):
     assert (out[0] == 7).all() and (out[-1] == 7).all()
 
 
-@pytest.mark.parametrize("new", [[1, 1, 6], [229, 3, 200]])
+@pytest.mark.parametrize("new", [[1, 1, 6], [229, 3, 200], [229, 3, 330]])
 def test_adapters_are_the_same_every_time_captured_and_on_another_stream(be, new):
     c = Case(new, [0, 1, 0], 1024, 264, 32, seed=8)
     first = c.run(be)
@@ -233,7 +234,7 @@ def test_long_sums_of_one_sign_lose_nothing(be, rows, rank):
     assert be.paged_status() == 0
 
 
-@pytest.mark.parametrize("each", [1, 40])
+@pytest.mark.parametrize("each", [1, 40, 50])
 def test_starts_that_decrease_are_reported(be, each):
     """By the kernels of few rows and of many; rows before the fault are those of their request."""
     requests, rank = 12, 16
